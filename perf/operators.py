@@ -24,7 +24,7 @@ own = False
 DEV = "cuda"
 F8 = torch.float8_e4m3fn
 TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
-LEAST, MOST = -100, 120          # exponents of a scale
+LEAST, MOST = -40, 40           # exponents of a scale
 
 
 def _dsk():

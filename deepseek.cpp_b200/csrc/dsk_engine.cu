@@ -31,6 +31,7 @@
 
 #include <algorithm>
 #include <array>
+#include "dsk_host.h"
 #include "dsk_kernels.cuh"
 #include "dsk_mega.cuh"
 #include "dsk_decode.cuh"
@@ -48,10 +49,14 @@ using namespace dsk;
 // errors
 // ---------------------------------------------------------------------------------------------------
 static thread_local char g_err[1024] = "";
+int dsk::fail_text(int code, const char* fmt, va_list ap) {
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  return code;
+}
 static int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  fail_text(code, fmt, ap);
   va_end(ap);
   return code;
 }

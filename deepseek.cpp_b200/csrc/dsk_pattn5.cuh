@@ -39,15 +39,6 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
 __device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kP5Tile >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void tc_mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {   // A in TMEM
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
-}
-__device__ __forceinline__ void tc_store8(uint32_t addr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-               ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
-
 // VB: 64-column blocks of values in a CTA (blockIdx.z picks the columns); kst, vst: in shared memory, pieces of 64 entries of a tile's keys and tiles of values
 template <int PARTS, int VB>
 __global__ void __launch_bounds__(kP5Threads, 1) pattn5(const __grid_constant__ PattnP P, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, int kst,

@@ -1,0 +1,286 @@
+// dsk_serve.cu — C-ABI (include/dsk.h) of the operators on device memory: the 8-bit key / value cache (write, read, attention) and the verification of
+// drafted tokens.  They belong to no model: the caller gives memory, workspace, device and stream; nothing is allocated, waited for or kept, so that calls can be
+// captured into graphs and run on several streams and devices at a time.
+
+#include "../../include/dsk.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <mutex>
+
+#include "dsk_host.h"
+#include "dsk_kv8.cuh"
+#include "dsk_kv8_attn.cuh"
+#include "dsk_verify.cuh"
+
+using namespace dsk;
+
+static int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  fail_text(code, fmt, ap);
+  va_end(ap);
+  return code;
+}
+#define CK(call)                                                                                   \
+  do {                                                                                             \
+    cudaError_t e_ = (call);                                                                       \
+    if (e_ != cudaSuccess) { cudaGetLastError(); return fail(-2, "%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); } \
+  } while (0)
+
+namespace {
+constexpr int kMaxDevices = 64;
+
+// The caller's current device comes back at the end of a call.
+struct OnDevice {
+  int before = -1, device;
+  cudaError_t error;
+  explicit OnDevice(int d) : device(d) {
+    error = cudaGetDevice(&before);
+    if (error == cudaSuccess && before != d) error = cudaSetDevice(d);
+  }
+  ~OnDevice() { if (before >= 0 && before != device) cudaSetDevice(before); }
+};
+int multiprocessors(int device) {
+  static std::mutex lock;
+  static int known[kMaxDevices];
+  std::lock_guard<std::mutex> hold(lock);
+  if (!known[device] && cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); known[device] = 0; }
+  return known[device];
+}
+// Shared memory beyond 48 KB, granted once for a kernel and device.
+template <auto KERNEL> cudaError_t allow(int device, int bytes) {
+  static std::mutex lock;
+  static int granted[kMaxDevices];
+  std::lock_guard<std::mutex> hold(lock);
+  if (granted[device] >= bytes) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) granted[device] = bytes;
+  return e;
+}
+// A launch behind another one of the same call: its CTAs may come up under the kernel ahead and wait there (grid_wait).
+template <typename... KA, typename... A>
+cudaError_t launch_behind(void (*kernel)(KA...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster, A... a) {
+  cudaLaunchConfig_t c{};
+  cudaLaunchAttribute at[2];
+  c.gridDim = grid; c.blockDim = block; c.dynamicSmemBytes = smem; c.stream = stream; c.attrs = at; c.numAttrs = 1;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    c.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&c, kernel, static_cast<KA>(a)...);
+}
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int size_of(int dtype) { return dtype == DSK_DT_F32 ? 4 : 2; }
+
+int check_device(int device) {
+  int n = 0;
+  const cudaError_t e = cudaGetDeviceCount(&n);
+  if (e != cudaSuccess || n == 0) { cudaGetLastError(); return fail(-1, "no CUDA device available (%s) — libdsk has no CPU fallback", cudaGetErrorString(e)); }
+  if (device < 0 || device >= n || device >= kMaxDevices) return fail(-1, "device %d out of range (have %d)", device, n);
+  return 0;
+}
+int check_cache(const dsk_kv8* c, const dsk_kv8_rows* s) {
+  if (!c || !s) return fail(-1, "null cache or rows");
+  if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128) return fail(-4, "blocks of %d tokens: 16, 32, 64 or 128 are supported", c->block);
+  if (c->n_blocks <= 0 || c->kv_heads <= 0 || c->kv_heads > 32767) return fail(-4, "%d blocks of %d key heads: both must be positive, heads at most 32767", c->n_blocks, c->kv_heads);
+  for (int d : {c->dim_k, c->dim_v})
+    if (d <= 0 || d % 16 || d > 256) return fail(-4, "heads of %d entries: a multiple of 16 up to 256 is needed", d);
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(-1, "cache: null memory");
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) || !aligned(c->status, 4)) return fail(-1, "cache: codes need 16-byte alignment, scales and status 4");
+  if (s->batch < 0 || s->rows < 0 || s->batch > 65535 || s->table_blocks < 0 || s->table_blocks > (1 << 30) / c->block)
+    return fail(-4, "batch %d (at most 65535), %d rows, tables of %d blocks (2^30 tokens at most)", s->batch, s->rows, s->table_blocks);
+  if (s->batch && s->rows && (!s->table || !s->first || s->table_blocks == 0)) return fail(-1, "rows: null or empty table, or null first");
+  return check_device(c->device);
+}
+int check_view(const char* what, const dsk_view* v, int dtype) {
+  if (!v || !v->data) return fail(-1, "%s: null", what);
+  if (v->dtype != dtype) return fail(-4, "%s: element type %d where %d is needed", what, v->dtype, dtype);
+  if (!aligned(v->data, size_of(dtype))) return fail(-1, "%s: memory is not aligned to its element", what);
+  return 0;
+}
+bool wide(const dsk_view* v) {
+  const int n = 16 / size_of(v->dtype);
+  return aligned(v->data, 16) && v->batch % n == 0 && v->row % n == 0 && v->head % n == 0;
+}
+kv8::Cache cache_of(const dsk_kv8* c) {
+  return kv8::Cache{{static_cast<unsigned char*>(c->k), static_cast<unsigned char*>(c->v)}, {c->k_scale, c->v_scale}, c->status, c->n_blocks, c->block, c->kv_heads, {c->dim_k, c->dim_v}};
+}
+kv8::Rows rows_of(const dsk_kv8_rows* s) { return kv8::Rows{s->table, s->table_pitch, s->first, s->count, s->table_blocks, s->batch, s->rows}; }
+kv8::Pitch pitch_of(const dsk_view* v) { return kv8::Pitch{v->batch, v->row, v->head}; }
+// blocks that the rows of one sequence may touch
+unsigned touched(const dsk_kv8* c, const dsk_kv8_rows* s) {
+  return (unsigned)std::min<long long>(s->table_blocks, ((long long)s->rows + c->block - 2) / c->block + 1);
+}
+
+template <typename T> int write_as(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, cudaStream_t stream) {
+  const dim3 grid(touched(c, s), 2 * c->kv_heads, s->batch);
+  const T *pk = static_cast<const T*>(k->data), *pv = static_cast<const T*>(v->data);
+  const int w = wide(k) && wide(v), eights = std::min(s->rows, c->block) * std::max(c->dim_k, c->dim_v) / 8;
+  // a CTA's values stay in registers: a warp of four eights a lane for a few rows (no barrier), otherwise as few threads as hold them
+  if (eights <= 128) kv8::write_rows<T, 32, 4><<<grid, 32, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
+  else if (eights <= 1024) kv8::write_rows<T, 128, 8><<<grid, 128, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
+  else if (eights <= 2048) kv8::write_rows<T, 256, 8><<<grid, 256, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
+  else kv8::write_rows<T, 256, 16><<<grid, 256, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
+  CK(cudaGetLastError());
+  return 0;
+}
+template <typename T> int read_as(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, cudaStream_t stream) {
+  const dim3 grid(touched(c, s), 2 * c->kv_heads, s->batch);
+  kv8::read_rows<T><<<grid, kv8::kReadThreads, 0, stream>>>(cache_of(c), rows_of(s), static_cast<T*>(k->data), static_cast<T*>(v->data), pitch_of(k), pitch_of(v), wide(k) && wide(v));
+  CK(cudaGetLastError());
+  return 0;
+}
+
+// How an attention call is laid out
+struct Layout { int shape, tiles, row_tiles, ctas; size_t ends, bytes; };
+constexpr int kShapes[4][2] = {{64, 64}, {128, 128}, {192, 128}, {256, 256}};
+int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, Layout* L) {
+  if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
+  if (s->batch > kv8::kMaxBatch) return fail(-4, "attention over %d sequences: at most %d a call", s->batch, kv8::kMaxBatch);
+  const long long rows = (long long)(heads / c->kv_heads) * s->rows;
+  if (rows > (1 << 24)) return fail(-4, "%lld query rows of a key head: at most 2^24", rows);
+  for (L->shape = 0; c->dim_k > kShapes[L->shape][0] || c->dim_v > kShapes[L->shape][1];) L->shape++;
+  L->tiles = rows > 16 && L->shape < 3 ? 2 : 1;
+  L->row_tiles = (int)((rows + 16 * L->tiles - 1) / (16 * L->tiles));
+  const int sms = multiprocessors(c->device);
+  if (!sms) return fail(-2, "device %d: no attributes", c->device);
+  const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * (((long long)s->table_blocks * c->block + kv8::kUnit - 1) / kv8::kUnit + 1);
+  L->ctas = (int)std::min<long long>(2 * sms, std::max<long long>(1, units));
+  L->ends = ((size_t)(s->batch + 1) * sizeof(long long) + 15) / 16 * 16;
+  L->bytes = L->ends + (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 8 * 128 + 32) * sizeof(float);
+  return 0;
+}
+template <int DK, int DV, int MT> int attend_as(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
+  const int smem = kv8::attn_smem<DK, DV, MT>() + 8 + 8 * P.S.batch;
+  CK((allow<kv8::attend_tokens<DK, DV, MT>>(device, kv8::attn_smem<DK, DV, MT>() + 8 + 8 * kv8::kMaxBatch)));
+  kv8::attend_tokens<DK, DV, MT><<<L.ctas, kv8::kThreads, smem, stream>>>(P);
+  CK(cudaGetLastError());
+  CK(launch_behind(kv8::join<DV, MT>, dim3(P.C.heads * P.row_tiles, P.S.batch), dim3(MT * DV / 16 * 32), 0, stream, 1, P, L.ctas));
+  return 0;
+}
+}  // namespace
+
+extern "C" int dsk_kv8_write(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, void* stream) {
+  if (check_cache(c, s)) return -1;
+  const int dt = k ? k->dtype : -1;
+  if (dt != DSK_DT_F32 && dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_write: keys and values are F32, F16 or BF16");
+  if (!s->batch || !s->rows) return 0;
+  if (check_view("keys", k, dt) || check_view("values", v, dt)) return -1;
+  OnDevice on(c->device);
+  CK(on.error);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dt == DSK_DT_F32 ? write_as<float>(c, s, k, v, st) : dt == DSK_DT_F16 ? write_as<__half>(c, s, k, v, st) : write_as<__nv_bfloat16>(c, s, k, v, st);
+}
+
+extern "C" int dsk_kv8_read(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, void* stream) {
+  if (check_cache(c, s)) return -1;
+  const int dt = k ? k->dtype : -1;
+  if (dt != DSK_DT_F32 && dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_read: keys and values are F32, F16 or BF16");
+  if (!s->batch || !s->rows) return 0;
+  if (check_view("keys", k, dt) || check_view("values", v, dt)) return -1;
+  OnDevice on(c->device);
+  CK(on.error);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dt == DSK_DT_F32 ? read_as<float>(c, s, k, v, st) : dt == DSK_DT_F16 ? read_as<__half>(c, s, k, v, st) : read_as<__nv_bfloat16>(c, s, k, v, st);
+}
+
+extern "C" int dsk_kv8_attn_workspace(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, size_t* bytes) {
+  if (!bytes) return fail(-1, "bad arguments");
+  if (check_cache(c, s)) return -1;
+  Layout L{};
+  if (layout_of(c, s, heads, &L)) return -1;
+  *bytes = L.bytes;
+  return 0;
+}
+
+extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* q, const dsk_view* out, int heads, float scale, int window, int keep_first, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  if (check_cache(c, s)) return -1;
+  const int dt = q ? q->dtype : -1;
+  if (dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_attn: queries are F16 or BF16");
+  if (!(std::fabs(scale) < INFINITY)) return fail(-4, "dsk_kv8_attn: the scale is not a number");
+  if (window < 0 || keep_first < 0) return fail(-4, "dsk_kv8_attn: window %d and keep_first %d must not be negative", window, keep_first);
+  if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
+  if (!s->batch || !s->rows) return 0;
+  if (check_view("queries", q, dt) || check_view("output", out, dt)) return -1;
+  Layout L{};
+  if (layout_of(c, s, heads, &L)) return -1;
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < L.bytes) return fail(-1, "dsk_kv8_attn: a workspace of %zu bytes is needed, 16-byte aligned (%zu given)", L.bytes, workspace_bytes);
+  OnDevice on(c->device);
+  CK(on.error);
+  kv8::Attn P;
+  P.C = cache_of(c); P.S = rows_of(s);
+  P.q = q->data; P.out = out->data; P.pq = pitch_of(q); P.po = pitch_of(out);
+  P.heads = heads; P.group = heads / c->kv_heads; P.row_tiles = L.row_tiles; P.bf16 = dt == DSK_DT_BF16; P.wide_q = wide(q); P.wide_o = wide(out);
+  P.window = window; P.keep = keep_first;
+  P.scale = scale * 1.44269504088896340736f;
+  P.ends = static_cast<long long*>(workspace);
+  P.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.ends);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (L.shape * 2 + L.tiles - 1) {
+    case 0: return attend_as<64, 64, 1>(P, L, c->device, st);
+    case 1: return attend_as<64, 64, 2>(P, L, c->device, st);
+    case 2: return attend_as<128, 128, 1>(P, L, c->device, st);
+    case 3: return attend_as<128, 128, 2>(P, L, c->device, st);
+    case 4: return attend_as<192, 128, 1>(P, L, c->device, st);
+    case 5: return attend_as<192, 128, 2>(P, L, c->device, st);
+    default: return attend_as<256, 256, 1>(P, L, c->device, st);
+  }
+}
+
+static int check_verify(const dsk_verify_args* a) {
+  if (!a) return fail(-1, "null arguments");
+  if (a->batch < 0 || a->batch > 65535 || a->drafts < 0 || a->drafts > verify::kMaxDrafts || a->vocab <= 0 || a->vocab > (1 << 28))
+    return fail(-4, "batch %d (at most 65535), %d drafts (at most %d), vocabulary %d (at most 2^28)", a->batch, a->drafts, verify::kMaxDrafts, a->vocab);
+  return 0;
+}
+static int pieces_of(const dsk_verify_args* a) { return (a->vocab + verify::kPiece - 1) / verify::kPiece; }
+
+extern "C" int dsk_verify_workspace(const dsk_verify_args* a, size_t* bytes) {
+  if (!bytes) return fail(-1, "bad arguments");
+  if (check_verify(a)) return -1;
+  *bytes = (size_t)a->batch * (a->drafts + 1) * pieces_of(a) * sizeof(float2);
+  return 0;
+}
+
+template <typename T> static int verify_as(const verify::Params& P, cudaStream_t stream) {
+  verify::row_stats<T><<<dim3((P.pieces + verify::kWarps - 1) / verify::kWarps, P.n + 1, P.batch), verify::kThreads, 0, stream>>>(P);
+  CK(cudaGetLastError());
+  CK(launch_behind(verify::pick<T>, dim3(P.batch * P.cluster), dim3(verify::kThreads), 0, stream, P.cluster, P));
+  return 0;
+}
+
+extern "C" int dsk_verify(const dsk_verify_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (check_verify(a)) return -1;
+  if (a->logits_dtype != DSK_DT_F32 && a->logits_dtype != DSK_DT_F16 && a->logits_dtype != DSK_DT_BF16) return fail(-4, "dsk_verify: logits are F32, F16 or BF16");
+  if (!(a->temperature >= 0.f && a->temperature < INFINITY)) return fail(-4, "temperature must be >= 0");
+  if (!a->batch) return 0;
+  if (!a->logits || !a->coins || !a->accepted || !a->tokens || (a->drafts && !a->draft_tokens)) return fail(-1, "dsk_verify: null memory");
+  size_t need = 0;
+  if (dsk_verify_workspace(a, &need)) return -1;
+  if (!workspace || !aligned(workspace, 8) || workspace_bytes < need) return fail(-1, "dsk_verify: a workspace of %zu bytes is needed, 8-byte aligned (%zu given)", need, workspace_bytes);
+  if (!aligned(a->logits, size_of(a->logits_dtype)) || !aligned(a->draft_probs, 4)) return fail(-1, "dsk_verify: memory is not aligned to its element");
+  if (check_device(a->device)) return -1;
+  OnDevice on(a->device);
+  CK(on.error);
+  verify::Params P;
+  const int size = size_of(a->logits_dtype);
+  P.logits = a->logits; P.l_batch = a->logits_batch; P.l_row = a->logits_row;
+  P.probs = a->draft_probs; P.p_batch = a->probs_batch; P.p_row = a->probs_row;
+  P.drafts = a->draft_tokens; P.count = a->count; P.coins = a->coins; P.part = static_cast<float2*>(workspace); P.accepted = a->accepted; P.tokens = a->tokens;
+  P.batch = a->batch; P.n = a->drafts; P.vocab = a->vocab; P.pieces = pieces_of(a);
+  P.wide_l = aligned(a->logits, 4 * size) && a->logits_batch % 4 == 0 && a->logits_row % 4 == 0;
+  P.wide_p = aligned(a->draft_probs, 16) && a->probs_batch % 4 == 0 && a->probs_row % 4 == 0;
+  P.slope = a->temperature == 0.f ? 0.0 : 1.44269504088896340736 / (double)a->temperature;
+  P.cluster = 8;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->logits_dtype == DSK_DT_F32 ? verify_as<float>(P, st) : a->logits_dtype == DSK_DT_F16 ? verify_as<__half>(P, st) : verify_as<__nv_bfloat16>(P, st);
+}

@@ -125,6 +125,28 @@ class HybridConfig(C.Structure):
                                        "norm_bias", "token_shift", "norm_one_plus", "loop_embed")] + [("logit_softcap", C.c_float), ("loop_in", C.c_int)]
 
 
+class Kv8(C.Structure):
+    """dsk_kv8 (include/dsk.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "status")] + [(n, C.c_int) for n in ("device", "n_blocks", "block", "kv_heads", "dim_k", "dim_v")]
+
+
+class Kv8Rows(C.Structure):
+    """dsk_kv8_rows (include/dsk.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("table", "first", "count")] + [("table_pitch", C.c_int64)] + [(n, C.c_int) for n in ("table_blocks", "batch", "rows")]
+
+
+class View(C.Structure):
+    """dsk_view (include/dsk.h)."""
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("batch", C.c_int64), ("row", C.c_int64), ("head", C.c_int64)]
+
+
+class VerifyArgs(C.Structure):
+    """dsk_verify_args (include/dsk.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "draft_probs", "draft_tokens", "count", "coins", "accepted", "tokens")] + \
+               [(n, C.c_int64) for n in ("logits_batch", "logits_row", "probs_batch", "probs_row")] + \
+               [(n, C.c_int) for n in ("device", "batch", "drafts", "vocab", "logits_dtype")] + [("temperature", C.c_float)]
+
+
 # mixer "type" strings of a layer-list config.json -> mixer kernel family.  Two names may map to one mechanism.
 MIXER_TYPES = {"mamba2": MIX_SSD, "mamba2_2": MIX_SSD, "latent_attention": MIX_LATENT_SWA, "attention": MIX_GQA}
 
@@ -468,7 +490,7 @@ ARCHITECTURES = {"Desarax": hybrid_from_config, "Rutulix": rutulix_from_config, 
                  "Zetivik": zetivik_from_config, "Netusun": netusun_from_config}
 
 _lib = None
-ABI_VERSION = 9   # DSK_ABI_VERSION (include/dsk.h)
+ABI_VERSION = 10  # DSK_ABI_VERSION (include/dsk.h)
 
 
 def build(force: bool = False) -> str:
@@ -542,6 +564,11 @@ def lib():
         L.dsk_moe_gate.argtypes = [f32p, f32p, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, C.c_int, C.c_int,
                                    i32p, f32p]
         L.dsk_bench_gemv.argtypes = [C.c_int] * 6 + [f32p, C.POINTER(C.c_double)]
+        L.dsk_kv8_write.argtypes = L.dsk_kv8_read.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.POINTER(View), C.POINTER(View), C.c_void_p]
+        L.dsk_kv8_attn_workspace.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.c_int, C.POINTER(C.c_size_t)]
+        L.dsk_kv8_attn.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.POINTER(View), C.POINTER(View), C.c_int, C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.dsk_verify_workspace.argtypes = [C.POINTER(VerifyArgs), C.POINTER(C.c_size_t)]
+        L.dsk_verify.argtypes = [C.POINTER(VerifyArgs), C.c_void_p, C.c_size_t, C.c_void_p]
         L.dsk_attn.argtypes = [f32p, u16p, u16p, C.c_int, C.c_int, C.c_int, C.c_int, f32p]
         _lib = L
     return _lib
@@ -865,6 +892,162 @@ class Model:
         if self.h:
             self.L.dsk_model_destroy(self.h)
             self.h = None
+
+
+# ---- operators on device memory: torch tensors of one GPU, work on torch's current stream of that GPU ------------------------------
+
+def _device_of(t) -> int:
+    if not getattr(t, "is_cuda", False):
+        raise DskError("tensors on a CUDA device are needed: libdsk has no CPU fallback")
+    return t.device.index
+
+
+def _stream_of(torch, device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _dense(what, t, dtype, shape, device):
+    """A contiguous tensor of that type and shape on the device (its address)."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or _device_of(t) != device:
+        raise DskError(f"{what}: a contiguous {dtype} tensor {tuple(shape)} on cuda:{device} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+class Cache8:
+    """A key / value cache in 8 bits (dsk_kv8, include/dsk.h): blocks of `block` tokens, E4M3 codes [n_blocks, kv_heads, block, dim] and a scale, a power of
+    two, for every block and head [n_blocks, kv_heads].  A sequence is a row of a table of block numbers (int32 [batch, blocks]); which blocks are free is the
+    caller's to know.  `first`, `lens`, `count` are int32 [batch] tensors on the GPU, so that a captured graph serves other lengths.  No call waits for
+    the GPU: what only the GPU sees (a block number outside the cache, tokens outside the table) shows in `check`.  Memory of a call comes
+    from torch's allocator on the current stream; calls may run on several streams at a time as long as none writes what another one uses."""
+
+    def __init__(self, n_blocks: int, kv_heads: int, dim_k: int, dim_v: Optional[int] = None, block: int = 64, device=None):
+        import torch
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device) if not isinstance(device, int) else torch.device("cuda", device)
+        dim_v = dim_k if dim_v is None else dim_v
+        f8 = torch.float8_e4m3fn
+        self._bind(torch.zeros((n_blocks, kv_heads, block, dim_k), dtype=torch.uint8, device=dev).view(f8), torch.zeros((n_blocks, kv_heads, block, dim_v), dtype=torch.uint8, device=dev).view(f8),
+                   torch.ones((n_blocks, kv_heads), device=dev), torch.ones((n_blocks, kv_heads), device=dev))
+
+    @classmethod
+    def of(cls, k, v, k_scale, v_scale) -> "Cache8":
+        """A cache over the caller's tensors (laid out as above; scales as `write` makes them)."""
+        c = cls.__new__(cls)
+        c._bind(k, v, k_scale, v_scale)
+        return c
+
+    def _bind(self, k, v, k_scale, v_scale):
+        import torch
+        self._torch = torch
+        self.device = _device_of(k)
+        if k.dim() != 4 or v.dim() != 4:
+            raise DskError("codes are [n_blocks, kv_heads, block, dim]")
+        _dense("keys", k, torch.float8_e4m3fn, k.shape, self.device)
+        _dense("values", v, torch.float8_e4m3fn, k.shape[:3] + v.shape[3:], self.device)
+        _dense("key scales", k_scale, torch.float32, k.shape[:2], self.device)
+        _dense("value scales", v_scale, torch.float32, k.shape[:2], self.device)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_blocks, self.kv_heads, self.block, self.dim_k = k.shape
+        self.dim_v = v.shape[3]
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self._c = Kv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.status.data_ptr(), self.device, *k.shape[:1], self.block, self.kv_heads, self.dim_k, self.dim_v)
+        self._L = lib()
+
+    def _rows(self, table, first, count, rows):
+        torch = self._torch
+        if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) not in (1, 0) and table.shape[1] > 1 or _device_of(table) != self.device:
+            raise DskError(f"table: int32 [batch, blocks] on cuda:{self.device} with rows of neighbours is needed, got {table.dtype} {tuple(table.shape)} on {table.device}")
+        if table.stride(1) == 0 and table.shape[1] > 1:
+            raise DskError("table: its rows must not be broadcast")
+        batch = table.shape[0]
+        return Kv8Rows(table.data_ptr(), _dense("first tokens / lengths", first, torch.int32, (batch,), self.device),
+                       _dense("count", count, torch.int32, (batch,), self.device) if count is not None else None, table.stride(0), table.shape[1], batch, rows)
+
+    def _view(self, what, t, shape, written=False):
+        if t.shape != shape or t.dtype not in self._types or _device_of(t) != self.device or t.stride(3) != 1:
+            raise DskError(f"{what}: float32, float16 or bfloat16 {tuple(shape)} on cuda:{self.device} with neighbouring entries is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        s = t.stride()
+        if written and any(s[i] < t.shape[3] and t.shape[i] > 1 for i in range(3)):
+            raise DskError(f"{what}: rows of the result must not overlap")
+        return View(t.data_ptr(), self._types[t.dtype], s[0], s[1], s[2])
+
+    def write(self, k, v, table, first, count=None):
+        """Tokens first[b] .. of every sequence from rows k, v [batch, rows, kv_heads, dim] (dsk_kv8_write)."""
+        if k.dim() != 4 or v.dim() != 4:
+            raise DskError("keys and values are [batch, rows, kv_heads, dim]")
+        batch, rows = k.shape[:2]
+        if batch != table.shape[0] or k.dtype != v.dtype:
+            raise DskError(f"keys of {batch} sequences and {k.dtype}, values of {v.dtype}, a table of {table.shape[0]} sequences")
+        s = self._rows(table, first, count, rows)
+        a, b = self._view("keys", k, (batch, rows, self.kv_heads, self.dim_k)), self._view("values", v, (batch, rows, self.kv_heads, self.dim_v))
+        _ck(self._L.dsk_kv8_write(self._c, s, a, b, _stream_of(self._torch, self.device)))
+
+    def read(self, table, first, rows: int, count=None, dtype=None, out=None):
+        """The values of tokens first[b] .. first[b] + rows - 1 (dsk_kv8_read): (keys, values) [batch, rows, kv_heads, dim], `out` or new ones (zeros in rows from count[b] on)."""
+        torch = self._torch
+        batch = table.shape[0]
+        shapes = (batch, rows, self.kv_heads, self.dim_k), (batch, rows, self.kv_heads, self.dim_v)
+        if out is None:
+            out = tuple(torch.zeros(x, dtype=dtype or torch.bfloat16, device=table.device) for x in shapes)
+        elif dtype is not None and any(x.dtype != dtype for x in out) or out[0].dtype != out[1].dtype:
+            raise DskError(f"results of {out[0].dtype} and {out[1].dtype} where {dtype or 'one type'} is asked for")
+        s = self._rows(table, first, count, rows)
+        a, b = self._view("keys", out[0], shapes[0], True), self._view("values", out[1], shapes[1], True)
+        _ck(self._L.dsk_kv8_read(self._c, s, a, b, _stream_of(torch, self.device)))
+        return out
+
+    def attend(self, q, table, lens, count=None, scale: Optional[float] = None, window: int = 0, keep_first: int = 0, out=None):
+        """Attention of queries q [batch, rows, heads, dim_k] (float16 or bfloat16), the last count[b] of a sequence's lens[b] tokens, over the cache (dsk_kv8_attn); scale: dim_k ** -0.5
+        unless given.  Returns [batch, rows, heads, dim_v] in the queries' type, `out` or a new tensor (zeros in rows from count[b] on)."""
+        torch = self._torch
+        if q.dim() != 4 or q.shape[0] != table.shape[0]:
+            raise DskError(f"queries are [batch, rows, heads, dim_k], got {tuple(q.shape)} for a table of {table.shape[0]} sequences")
+        batch, rows, heads = q.shape[:3]
+        shape = (batch, rows, heads, self.dim_v)
+        if out is None:
+            out = (torch.empty if count is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
+        elif out.dtype != q.dtype:
+            raise DskError(f"results of {out.dtype} for queries of {q.dtype}")
+        s = self._rows(table, lens, count, rows)
+        a, b = self._view("queries", q, (batch, rows, heads, self.dim_k)), self._view("output", out, shape, True)
+        need = C.c_size_t(0)
+        _ck(self._L.dsk_kv8_attn_workspace(self._c, s, heads, need))
+        work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        _ck(self._L.dsk_kv8_attn(self._c, s, a, b, heads, self.dim_k ** -0.5 if scale is None else scale, window, keep_first, work.data_ptr(), need.value, _stream_of(torch, self.device)))
+        return out
+
+    def check(self):
+        """Waits for the GPU and raises if a call met a block number outside the cache, tokens outside a table or a wait that gave up; the status is cleared."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            raise DskError("8-bit cache: " + ", ".join(t for b, t in ((1, "a block number outside the cache"), (2, "tokens outside the table"), (4, "a wait inside a kernel gave up")) if bits & b))
+
+
+def verify_drafts(logits, drafts, coins, probs=None, count=None, temperature: float = 1.0):
+    """Verification of drafted tokens (dsk_verify, include/dsk.h): logits [batch, drafts + 1, vocab] of the model at the last token and behind every draft, drafts int32 [batch, drafts],
+    coins float32 [batch, drafts + 1] in [0, 1) (the last one draws), probs float32 [batch, drafts, vocab] of the draft model (none: the drafts are certain), count int32 [batch] drafts that
+    exist.  Returns (accepted int32 [batch], tokens int32 [batch, drafts + 1]: the accepted drafts, the drawn token, -1 behind it)."""
+    import torch
+    device = _device_of(logits)
+    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if logits.dim() != 3 or logits.dtype not in types or logits.stride(2) != 1 and logits.shape[2] > 1:
+        raise DskError(f"logits: float32, float16 or bfloat16 [batch, drafts + 1, vocab] with neighbouring entries is needed, got {logits.dtype} {tuple(logits.shape)}")
+    batch, n, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    if n < 0:
+        raise DskError("logits of no row")
+    if probs is not None and (probs.shape != (batch, n, vocab) or probs.dtype != torch.float32 or _device_of(probs) != device or probs.stride(2) != 1 and vocab > 1):
+        raise DskError(f"probs: float32 {(batch, n, vocab)} on cuda:{device} with neighbouring entries is needed, got {probs.dtype} {tuple(probs.shape)} on {probs.device}")
+    accepted, tokens = torch.empty(batch, dtype=torch.int32, device=logits.device), torch.empty((batch, n + 1), dtype=torch.int32, device=logits.device)
+    a = VerifyArgs(logits.data_ptr(), probs.data_ptr() if probs is not None and n else None, _dense("drafts", drafts, torch.int32, (batch, n), device),
+                   _dense("count", count, torch.int32, (batch,), device) if count is not None else None, _dense("coins", coins, torch.float32, (batch, n + 1), device),
+                   accepted.data_ptr(), tokens.data_ptr(), logits.stride(0), logits.stride(1), *((probs.stride(0), probs.stride(1)) if probs is not None else (0, 0)),
+                   device, batch, n, vocab, types[logits.dtype], temperature)
+    need = C.c_size_t(0)
+    _ck(lib().dsk_verify_workspace(a, need))
+    work = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
+    _ck(lib().dsk_verify(a, work.data_ptr(), need.value, _stream_of(torch, device)))
+    return accepted, tokens
 
 
 # ---- kernel-level hooks (mirror the reference's test-exposed statics) ------------------------------

@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define DSK_ABI_VERSION 9
+#define DSK_ABI_VERSION 10
 
 /* Quant: src/codec.h:79-85 (same numbering) */
 enum { DSK_F32 = 0, DSK_F16 = 1, DSK_F8E5M2 = 2, DSK_Q2_K = 3, DSK_Q3_K = 4,
@@ -338,6 +338,65 @@ int dsk_sample_prob(dsk_model* m, dsk_state* s, int index, float* prob);
  * sequence of dsk_forward / dsk_block_forward / dsk_decode_greedy calls. */
 int dsk_comm_unique_id(void* out128);
 int dsk_comm_init(dsk_model* m, const void* nccl_unique_id128);
+
+/* ---- operators on device memory -----------------------------------------------------------------------------------
+ * A key / value cache held in 8 bits, attention over it, and the verification of drafted tokens, for programs that serve several sequences or decode
+ * speculatively.  (The reference has neither.)  They belong to no model and need no dsk_init: pointers are device memory of `device`, work goes to `stream` (a cudaStream_t, null: the
+ * default stream), nothing is allocated, waited for or kept between calls, the caller's current device stays what it is, and calls can be captured into graphs.  Calls that may
+ * run at the same time need workspaces of their own.  What the device alone can see (a block outside the cache, tokens outside the table) sets bits of `status`: such rows are not
+ * written, not read and not seen by attention.
+ *
+ * The cache is made of blocks of `block` tokens (16, 32, 64 or 128): codes [n_blocks][kv_heads][block][dim] in E4M3, one scale [n_blocks][kv_heads] for every block and head, value =
+ * code x scale; dim_k and dim_v are multiples of 16 up to 256.  Token t of sequence b lies in block table[b][t / block] at row t % block.  Scales are powers of two from 2^-40 to 2^40:
+ * dsk_kv8_write takes the smallest s with |x| <= 448 s over the finite values that it writes to a block and head, never less than the old one while the block holds
+ * tokens ahead of the first written one, and where that grows it rounds their codes again; a block whose first token is written starts anew.  Values beyond the range (infinities
+ * too) become +-448 s, NaN stays NaN.  A block that is written to belongs to one sequence; blocks that are only read may be shared. */
+enum { DSK_KV8_PAGE = 1,   /* status: a block number outside the cache */
+       DSK_KV8_RANGE = 2,  /* status: tokens ahead of the first or behind the last block of a table */
+       DSK_KV8_WAIT = 4 }; /* status: a wait inside a kernel gave up (results are not valid) */
+typedef struct dsk_kv8 {
+  void *k, *v;                     /* codes, 16-byte aligned */
+  float *k_scale, *v_scale;
+  int32_t* status;                 /* nullable; bits are added, never cleared */
+  int device, n_blocks, block, kv_heads, dim_k, dim_v;
+} dsk_kv8;
+typedef struct dsk_kv8_rows {      /* a padded batch: `rows` rows of every sequence, of which the first count[b] exist (the others are neither read nor written) */
+  const int32_t *table, *first, *count;   /* [batch][table_blocks] rows table_pitch apart; [batch], see each call; [batch], nullable: all rows */
+  int64_t table_pitch;
+  int table_blocks, batch, rows;
+} dsk_kv8_rows;
+typedef struct dsk_view {          /* [batch][row][head][entry], entries side by side, pitches in elements */
+  void* data;
+  int dtype;                       /* DSK_DT_F32, DSK_DT_F16, DSK_DT_BF16 */
+  int64_t batch, row, head;
+} dsk_view;
+/* Rows become tokens first[b] .. of their sequences (heads: kv_heads). */
+int dsk_kv8_write(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* k, const dsk_view* v, void* stream);
+/* The values of tokens first[b] .. in rows, rounded to the view's type. */
+int dsk_kv8_read(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* k, const dsk_view* v, void* stream);
+/* Softmax attention.  first[b]: the sequence's tokens in the cache, the last count[b] of which are the queries' (written ahead of the call): query i is at t = first[b] - count[b] + i and
+ * sees the tokens j <= t, with window > 0 those with t - j < window or j < keep_first.  Query head h reads key head h / (heads / kv_heads); out = softmax(scale q k) v in the queries' type
+ * (F16 or BF16), zeros for a query that sees nothing.  At most 1024 sequences a call. */
+int dsk_kv8_attn_workspace(const dsk_kv8* cache, const dsk_kv8_rows* rows, int heads, size_t* bytes);
+int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* q, const dsk_view* out, int heads, float scale, int window, int keep_first,
+                 void* workspace, size_t workspace_bytes, void* stream);
+/* Speculative sampling, beside dsk_sample: sequence b has count[b] drafted tokens x_i and the model's logits of count[b] + 1 rows.  p_i = softmax(logits_i / temperature); draft i is accepted
+ * while coins[i] q_i(x_i) < p_i(x_i) (no draft_probs: q_i(x_i) = 1, the drafts are certain).  The first draft that is not is replaced by a draw from max(p_i - q_i, 0); behind
+ * accepted ones the next token is drawn from p.  A draw is the lowest index whose running sum is over coins[drafts] x (whole sum), in 64 bits.  temperature 0: a draft is accepted
+ * if it is the lowest index of the largest logit, which replaces it otherwise.  Coins lie in [0, 1).  accepted[b]: drafts accepted; tokens[b]: those, the drawn token, -1 in the places behind.
+ * A drafted token outside the vocabulary is refused; where a row's logits hold a NaN, or are no distribution (+inf at a temperature, nothing but -inf), its draft is refused and the drawn token is -1. */
+typedef struct dsk_verify_args {
+  const void* logits;              /* [batch][drafts + 1][vocab], pitches in elements */
+  const float* draft_probs;        /* [batch][drafts][vocab], nullable */
+  const int32_t *draft_tokens, *count;   /* [batch][drafts]; [batch], nullable: all */
+  const float* coins;              /* [batch][drafts + 1] */
+  int32_t *accepted, *tokens;      /* [batch]; [batch][drafts + 1] */
+  int64_t logits_batch, logits_row, probs_batch, probs_row;
+  int device, batch, drafts, vocab, logits_dtype;   /* drafts: at most 127; logits F32, F16 or BF16 */
+  float temperature;
+} dsk_verify_args;
+int dsk_verify_workspace(const dsk_verify_args* args, size_t* bytes);
+int dsk_verify(const dsk_verify_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- kernel-level test hooks (mirror the statics reached by the reference's tests) ----------------
  * Every hook builds a one-stage program and runs it through the SAME persistent decode kernel that produces the

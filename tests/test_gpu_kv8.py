@@ -1,0 +1,429 @@
+"""The 8-bit key / value cache and attention over it against their float64 restatement (oracle/serve_oracle.py).
+
+Tolerances of attention, from the arithmetic of the kernels: queries and codes are exact in fp16; a score's sum of d products in fp32 is off by at most (d + 4) 2^-23 sum |q k| scale, which
+changes a weight by that factor, numerator and denominator alike; a weight is rounded to fp16, 2^-11 of it, or by 2^-25 of the reference where it is below 2^-14 of
+that (the reference is at most the largest weight times its value scale); the exponential is good to 2^-21; sums over L keys in fp32 to L 2^-24; the result is rounded to its type once."""
+import numpy as np
+import pytest
+import torch
+
+import dsk
+import serve_oracle as so
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F8 = torch.float8_e4m3fn
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+class Case:
+    """A cache in which the blocks of all sequences lie scattered; what no token holds is NaN."""
+
+    def __init__(self, lens, H, dk, dv, block, seed=0, spread=0.7, dead=127, share=False):
+        self.rng = np.random.default_rng(seed)
+        self.lens, self.H, self.dk, self.dv, self.block = list(lens), H, dk, dv, block
+        self.B, per = len(lens), max(1, max(-(-max(n, 1) // block) for n in lens))
+        self.blocks = self.B * per + 2
+        self.table = self.rng.permutation(self.blocks)[:self.B * per].reshape(self.B, per).astype(np.int32)
+        if share:
+            self.table[1:] = self.table[0]
+        self.k, self.v = (np.full((self.blocks, H, block, d), dead, dtype=np.uint8) for d in (dk, dv))
+        self.ks, self.vs = np.ones((self.blocks, H)), np.ones((self.blocks, H))
+        for codes, scales, d in ((self.k, self.ks, dk), (self.v, self.vs, dv)):
+            x = self.rng.normal(size=(self.B, max(1, max(lens)), H, d)) * np.exp(spread * self.rng.normal(size=(self.B, max(1, max(lens)), H, 1)))
+            so.write(codes, scales, self.table, [0] * self.B, lens, x)
+
+    def device(self):
+        t = lambda a: torch.from_numpy(a.copy()).to(DEV)
+        self.cache = dsk.Cache8.of(t(self.k).view(F8), t(self.v).view(F8), t(self.ks.astype(np.float32)), t(self.vs.astype(np.float32)))
+        self.t = t(self.table)
+        return self.cache
+
+    def bytes(self):
+        return self.cache.k.view(torch.uint8).cpu().numpy(), self.cache.v.view(torch.uint8).cpu().numpy(), self.cache.k_scale.cpu().numpy(), self.cache.v_scale.cpu().numpy()
+
+
+def ints(x):
+    return torch.tensor(list(x), dtype=torch.int32, device=DEV)
+
+
+def expect(c, q, count, heads, scale, window=0, keep=0, lens=None):
+    """(what attention gives, how far it may be off before its last rounding)"""
+    lens = c.lens if lens is None else lens
+    want, mass, size, top = so.attend(c.k, c.ks, c.v, c.vs, c.table, lens, count, q, heads, scale, window, keep)
+    L = max(max(lens), 1)
+    tol = mass * (2.0 ** -11 + 2 * (c.dk + 4) * 2.0 ** -23 * size + 2.0 ** -20 + L * 2.0 ** -24) + L * 2.0 ** -25 * 448 * top
+    return want, tol
+
+
+def check(got, want, tol, count, dtype, left=None):
+    got = got.double().cpu().numpy()
+    half = torch.finfo(DT[dtype]).eps / 2
+    for b, n in enumerate(count):
+        w, g = want[b, :n], got[b, :n]
+        assert np.array_equal(np.isnan(w), np.isnan(g)), (b, np.argwhere(np.isnan(w) != np.isnan(g))[:4])
+        off, may = np.abs(g - w), tol[b, :n] + half * (np.abs(w) + tol[b, :n]) + 2.0 ** -25
+        assert (np.isnan(w) | (off <= may)).all(), (b, float(np.nanmax(off / may)))
+        if left is not None:
+            assert (got[b, n:] == left).all()
+
+
+# ---- write --------------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("H,dk,dv,block", [(1, 16, 16, 16), (2, 80, 64, 32), (3, 128, 128, 64), (2, 192, 128, 128), (1, 256, 256, 128), (5, 48, 240, 16)])
+def test_write(dtype, H, dk, dv, block):
+    """Calls of one token, of a few, across borders and of whole blocks, in turn, on ragged sequences: codes and scales are those of the definition, bit for bit."""
+    c = Case([0, 0, 0], H, dk, dv, block, dead=0)
+    per = 5
+    c.blocks = 3 * per + 2
+    c.table = c.rng.permutation(c.blocks)[:3 * per].reshape(3, per).astype(np.int32)
+    c.k, c.v = (c.rng.integers(0, 127, size=(c.blocks, H, block, d)).astype(np.uint8) for d in (dk, dv))
+    c.ks, c.vs = (2.0 ** c.rng.integers(-3, 20, size=(c.blocks, H)) for _ in range(2))
+    cache = c.device()
+    at = [0, 3, block - 1]
+    for n, count in ((1, [1, 1, 1]), (2, [2, 1, 0]), (block, [block, 3, block - 1]), (1, [1, 0, 1]), (2 * block + 3, [block, 2 * block + 3, block // 2]), (5, [5, 5, 5])):
+        size = np.exp(2.5 * c.rng.normal(size=(3, n, H, 1)))
+        x, y = (torch.from_numpy(c.rng.normal(size=(3, n, H, d)) * size).to(DT[dtype]) for d in (dk, dv))
+        cache.write(x.to(DEV), y.to(DEV), c.t, ints(at), ints(count))
+        so.write(c.k, c.ks, c.table, at, count, x.double().numpy())
+        so.write(c.v, c.vs, c.table, at, count, y.double().numpy())
+        at = [a + m for a, m in zip(at, count)]
+        k, v, ks, vs = c.bytes()
+        assert np.array_equal(ks, c.ks) and np.array_equal(vs, c.vs)
+        assert np.array_equal(k, c.k) and np.array_equal(v, c.v)
+    cache.check()
+
+
+def test_write_strided_and_unaligned():
+    c = Case([0, 0], 2, 64, 64, 16, dead=0)
+    c.table = np.array([[0, 1, 2], [3, 4, 5]], dtype=np.int32)
+    c.blocks = 6
+    c.k, c.v = (np.zeros((6, 2, 16, 64), dtype=np.uint8) for _ in range(2))
+    c.ks, c.vs = np.ones((6, 2)), np.ones((6, 2))
+    cache = c.device()
+    whole = torch.randn(2, 2, 40, 2 * 64 + 3, device=DEV).to(torch.bfloat16)          # [batch, head, row, key | value | pad]: odd pitches, an odd offset for the values
+    k, v = whole[..., :64].transpose(1, 2), whole[..., 65:129].transpose(1, 2)
+    wide_table = torch.full((2, 7), -1, dtype=torch.int32, device=DEV)
+    wide_table[:, :3] = c.t
+    cache.write(k, v, wide_table[:, :3], ints([1, 0]), ints([40, 33]))
+    so.write(c.k, c.ks, c.table, [1, 0], [40, 33], k.double().cpu().numpy())
+    so.write(c.v, c.vs, c.table, [1, 0], [40, 33], v.double().cpu().numpy())
+    gk, gv, ks, vs = c.bytes()
+    assert np.array_equal(gk, c.k) and np.array_equal(gv, c.v) and np.array_equal(ks, c.ks) and np.array_equal(vs, c.vs)
+
+
+def test_write_what_is_not_finite_and_the_ends_of_the_range():
+    c = Case([0], 4, 16, 16, 16, dead=0)
+    cache = c.device()
+    x = torch.zeros(1, 6, 4, 16)
+    x[0, 0, 0, :4] = torch.tensor([float("inf"), -float("inf"), float("nan"), 2.0])   # head 0: 2 is the largest number
+    x[0, 1, 0, 0] = -0.0
+    x[0, :, 1] = float("nan")                                                        # head 1: nothing but NaN, then a number
+    x[0, 2, 1, 3] = 1e-30
+    x[0, 3, 2, 5] = 3e38                                                             # head 2: beyond the range of the scales
+    x[0, 1, 3, :] = torch.linspace(-448, 448, 16) * 2.0 ** -30                         # head 3: below its neighbours' range
+    x[0, 2, 3, 1] = 1.0
+    for lo, hi in ((0, 2), (2, 6)):
+        cache.write(x[:, lo:hi].to(DEV), x[:, lo:hi].to(DEV), c.t, ints([lo]))
+        so.write(c.k, c.ks, c.table, [lo], [hi - lo], x[:, lo:hi].double().numpy())
+    k, v, ks, vs = c.bytes()
+    assert np.array_equal(ks, c.ks) and np.array_equal(vs, c.ks)
+    assert np.array_equal(so.TABLE[k], so.TABLE[c.k], equal_nan=True) and np.array_equal(k, v)
+    cache.check()
+
+
+def test_write_and_read_outside_are_noted_and_skipped():
+    c = Case([32, 32, 32], 2, 16, 16, 16)
+    cache = c.device()
+    before = c.bytes()
+    bad = c.t.clone()
+    bad[0, 1], bad[1, 1], bad[2, 1] = -1, c.blocks, 2 ** 31 - 1
+    x = torch.randn(3, 16, 2, 16, device=DEV)
+    cache.write(x, x, bad, ints([16, 16, 16]))
+    with pytest.raises(dsk.DskError, match="block number"):
+        cache.check()
+    cache.check()
+    cache.write(x, x, c.t, ints([-1, 32, 2 ** 31 - 1]))
+    with pytest.raises(dsk.DskError, match="outside the table"):
+        cache.check()
+    for a, b in zip(before, c.bytes()):
+        assert np.array_equal(a, b, equal_nan=a.dtype.kind == "f")
+    out = tuple(torch.full((3, 16, 2, 16), 7.0, device=DEV) for _ in range(2))
+    cache.read(bad, ints([16, 16, 16]), 16, out=out)
+    assert all((o == 7).all() for o in out)
+    with pytest.raises(dsk.DskError, match="block number"):
+        cache.check()
+
+
+# ---- read ---------------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("H,dk,dv,block", [(1, 16, 16, 16), (3, 128, 96, 64), (2, 192, 128, 32), (1, 256, 256, 128)])
+def test_read(dtype, H, dk, dv, block):
+    c = Case([3 * block + 5, 1, block], H, dk, dv, block)
+    cache = c.device()
+    first, count, n = [block - 3, 0, block - 1], [2 * block + 8, 1, 1], 2 * block + 8
+    out = tuple(torch.full((3, n, H, d), 7.0, device=DEV, dtype=DT[dtype]) for d in (dk, dv))
+    cache.read(c.t, ints(first), n, ints(count), out=out)
+    for o, codes, scales in zip(out, (c.k, c.v), (c.ks, c.vs)):
+        for b in range(3):
+            for h in range(H):
+                x, _ = so.gather(codes, scales, c.table[b], first[b] + count[b], h)
+                assert torch.equal(o[b, :count[b], h].cpu(), torch.from_numpy(x[first[b]:]).to(DT[dtype]))
+            assert (o[b, count[b]:] == 7).all()
+    k, v = cache.read(c.t, ints(first), n, ints(count), dtype=DT[dtype])
+    assert torch.equal(k[0], out[0][0]) and (k[1, 1:] == 0).all() and torch.equal(v[0], out[1][0])
+    odd = tuple(torch.zeros((3, n, H, d + 3), device=DEV, dtype=DT[dtype])[..., 1:d + 1] for d in (dk, dv))
+    cache.read(c.t, ints(first), n, ints(count), out=odd)
+    assert torch.equal(odd[0][0], out[0][0]) and torch.equal(odd[1][0], out[1][0])
+    cache.check()
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------------------------
+
+SHAPES = [
+    # lens, count, rows, heads, kv_heads, dk, dv, block, dtype, window, keep
+    ([1], [1], 1, 1, 1, 16, 16, 16, "bf16", 0, 0),
+    ([17, 1, 0, 333], [1, 1, 1, 1], 1, 4, 2, 64, 64, 16, "f16", 0, 0),
+    ([1000], [1], 1, 16, 4, 128, 128, 64, "bf16", 0, 0),
+    ([700, 90, 2100], [1, 1, 1], 1, 16, 1, 128, 128, 128, "f16", 0, 0),
+    ([700, 90, 2100], [5, 2, 0], 5, 8, 2, 128, 128, 64, "bf16", 0, 0),
+    ([513, 64, 65], [3, 3, 3], 3, 24, 2, 192, 128, 32, "bf16", 0, 0),
+    ([513, 64, 65], [1, 1, 1], 1, 2, 2, 192, 128, 64, "f16", 0, 0),
+    ([300, 20], [2, 7], 7, 2, 1, 256, 256, 64, "bf16", 0, 0),
+    ([300, 20], [2, 1], 2, 6, 2, 80, 48, 32, "f16", 0, 0),
+    ([150, 31], [9, 4], 9, 6, 2, 96, 256, 16, "bf16", 0, 0),
+    ([900, 40, 130], [1, 1, 1], 1, 8, 4, 64, 64, 64, "bf16", 100, 0),
+    ([900, 40, 130], [5, 3, 2], 5, 8, 4, 128, 128, 32, "f16", 33, 4),
+    ([900, 140, 13], [2, 2, 2], 2, 4, 4, 112, 128, 128, "f16", 16, 17),
+    ([450, 450], [1, 4], 4, 4, 1, 64, 128, 16, "bf16", 1, 0),
+    ([100, 3], [100, 3], 100, 4, 2, 64, 64, 16, "bf16", 0, 0),
+    ([260, 70], [200, 70], 200, 3, 1, 128, 128, 64, "f16", 50, 3),
+    ([257], [257], 257, 2, 2, 192, 128, 64, "bf16", 0, 0),
+    ([300, 129, 70], [130, 129, 1], 130, 8, 1, 128, 128, 32, "bf16", 0, 0),
+    ([400], [300], 300, 2, 1, 80, 96, 64, "f16", 0, 0),
+    ([333], [140], 140, 40, 2, 64, 48, 128, "f16", 77, 20),
+]
+
+
+@pytest.mark.parametrize("lens,count,rows,heads,kv_heads,dk,dv,block,dtype,window,keep", SHAPES)
+def test_attend(lens, count, rows, heads, kv_heads, dk, dv, block, dtype, window, keep):
+    c = Case(lens, kv_heads, dk, dv, block, seed=len(lens) + dk)
+    cache = c.device()
+    q = (torch.randn(len(lens), rows, heads, dk, generator=torch.Generator().manual_seed(3)) * 1.5).to(DT[dtype])
+    scale = dk ** -0.5
+    out = torch.full((len(lens), rows, heads, dv), 7.0, device=DEV, dtype=DT[dtype])
+    cache.attend(q.to(DEV), c.t, ints(lens), count=ints(count), window=window, keep_first=keep, out=out)
+    want, tol = expect(c, q.double().numpy(), count, heads, scale, window, keep)
+    check(out, want, tol, count, dtype, left=7.0)
+    cache.check()
+    if all(n == rows for n in count):
+        again = cache.attend(q.to(DEV), c.t, ints(lens), window=window, keep_first=keep)
+        assert torch.equal(again, out)                        # the same sums in the same order
+
+
+def test_attend_long_and_ragged():
+    """Pieces of one head in many CTAs, and many heads in one: all joined in a fixed order."""
+    lens = [9000, 1, 37, 4100, 64, 0, 2500]
+    c = Case(lens, 2, 64, 64, 64, seed=9)
+    cache = c.device()
+    q = torch.randn(7, 1, 4, 64, device=DEV, dtype=torch.bfloat16)
+    out = cache.attend(q, c.t, ints(lens))
+    want, tol = expect(c, q.double().cpu().numpy(), [1] * 7, 4, 0.125)
+    check(out, want, tol, [1] * 7, "bf16")
+    assert (out[5] == 0).all()
+
+
+def test_attend_strided_rows_and_an_unaligned_result():
+    c = Case([100, 30], 2, 64, 64, 16)
+    cache = c.device()
+    qkv = torch.randn(2, 3, 8 * 64 + 5, device=DEV, dtype=torch.float16)
+    q = qkv[..., 1:1 + 4 * 64].unflatten(-1, (4, 64))
+    room = torch.zeros(2, 4, 3, 67, device=DEV, dtype=torch.float16)
+    out = room[..., 1:65].transpose(1, 2)
+    cache.attend(q, c.t, ints([100, 30]), out=out, scale=0.2)
+    want, tol = expect(c, q.double().cpu().numpy(), [3, 3], 4, 0.2)
+    check(out, want, tol, [3, 3], "f16")
+    assert (room[..., 0] == 0).all() and (room[..., 65:] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [4, 90])
+def test_attend_nan_and_large_values_where_a_row_does_not_look(rows):
+    """A NaN key or value reaches the rows that see its token, entry by entry, and no other row; +-448 everywhere else is no harm."""
+    n = 200
+    c = Case([n, n], 2, 64, 64, 64, dead=126)
+    for b, t, h, d in ((0, n - 1, 0, 5), (0, n - 2, 1, 60), (1, n - rows // 2, 0, 0), (1, n - rows // 2, 0, 63)):
+        c.v[c.table[b][t // 64], h, t % 64, d] = 127 if d % 2 else 255
+    c.k[c.table[1][(n - 2) // 64], 1, (n - 2) % 64, 3] = 255
+    cache = c.device()
+    q = torch.randn(2, rows, 4, 64, device=DEV, dtype=torch.bfloat16)
+    out = cache.attend(q, c.t, ints([n, n]))
+    want, tol = expect(c, q.double().cpu().numpy(), [rows] * 2, 4, 0.125)
+    assert np.isnan(want).any() and not np.isnan(want[:, 0]).any()
+    check(out, want, np.nan_to_num(tol, nan=0.0), [rows] * 2, "bf16")
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_attend_windows_over_nan(rows):
+    """Tokens that have left the window are not looked at, whatever they hold."""
+    n = 500
+    c = Case([n], 1, 128, 128, 32)
+    for t in range(8, n - 60 - rows):
+        c.v[c.table[0][t // 32], 0, t % 32] = 127
+        c.k[c.table[0][t // 32], 0, t % 32, 7] = 127
+    cache = c.device()
+    q = torch.randn(1, rows, 2, 128, device=DEV, dtype=torch.float16)
+    out = cache.attend(q, c.t, ints([n]), window=60, keep_first=8)
+    want, tol = expect(c, q.double().cpu().numpy(), [rows], 2, 128 ** -0.5, 60, 8)
+    assert not np.isnan(want).any()
+    check(out, want, tol, [rows], "f16")
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attend_scales_of_very_unequal_size(rows):
+    """Value blocks of 2^-40 beside those of 2^20, queries of 1e-4 beside 1e4, scores of some hundreds."""
+    c = Case([300], 1, 64, 64, 16, seed=4)
+    for j in range(0, 19, 3):
+        c.vs[c.table[0][j], 0] = 2.0 ** -40
+    for j in range(1, 19, 3):
+        c.vs[c.table[0][j], 0] = 2.0 ** 20
+    cache = c.device()
+    q = torch.randn(1, rows, 8, 64, device=DEV) * torch.tensor([1e-4, 1e-2, 1.0, 30.0] * 2, device=DEV)[:, None]
+    q = q.to(torch.bfloat16)
+    out = cache.attend(q, c.t, ints([300]))
+    want, tol = expect(c, q.double().cpu().numpy(), [rows], 8, 0.125)
+    check(out, want, tol, [rows], "bf16")
+
+
+@pytest.mark.parametrize("rows", [2, 100])
+def test_attend_queries_that_are_not_finite(rows):
+    c = Case([120], 1, 64, 64, 16)
+    cache = c.device()
+    q = torch.randn(1, rows, 2, 64, device=DEV, dtype=torch.bfloat16)
+    q[0, 0, 0, 3], q[0, 1, 1, 5] = float("nan"), float("nan")
+    out = cache.attend(q, c.t, ints([120]))
+    bad = torch.zeros(1, rows, 2, dtype=torch.bool)
+    bad[0, 0, 0] = bad[0, 1, 1] = True
+    assert torch.equal(out.isnan().all(-1).cpu(), bad) and torch.equal(out.isnan().any(-1).cpu(), bad)
+
+
+@pytest.mark.parametrize("rows", [1, 80])
+def test_attend_blocks_outside_and_short_tables(rows):
+    """A block outside the cache is not seen; more tokens than the table has are noted."""
+    c = Case([200, 200], 1, 64, 64, 32)
+    c.table[0, 2] = -5
+    c.table[1, 6] = c.blocks
+    cache = c.device()
+    q = torch.randn(2, rows, 2, 64, device=DEV, dtype=torch.bfloat16)
+    out = cache.attend(q, c.t, ints([200, 200]))
+    want, tol = expect(c, q.double().cpu().numpy(), [rows] * 2, 2, 0.125)
+    check(out, want, tol, [rows] * 2, "bf16")
+    with pytest.raises(dsk.DskError, match="block number"):
+        cache.check()
+    c.table[0, 2], c.table[1, 6] = c.table[0, 1], c.table[1, 0]
+    c.device()
+    lens = [10 ** 6, -3]
+    out = c.cache.attend(q, c.t, ints(lens))
+    want, tol = expect(c, q.double().cpu().numpy(), [rows] * 2, 2, 0.125, lens=lens)
+    check(out[:1], want[:1], tol[:1] * 2, [rows], "bf16")
+    assert (out[1] == 0).all()
+    with pytest.raises(dsk.DskError, match="outside the table"):
+        c.cache.check()
+
+
+def test_attend_sequences_that_share_blocks():
+    c = Case([256, 256, 256], 2, 128, 128, 64, share=True)
+    cache = c.device()
+    q = torch.randn(3, 1, 4, 128, device=DEV, dtype=torch.bfloat16)
+    lens = [256, 100, 7]
+    out = cache.attend(q, c.t, ints(lens))
+    want, tol = expect(c, q.double().cpu().numpy(), [1] * 3, 4, 128 ** -0.5, lens=lens)
+    check(out, want, tol, [1] * 3, "bf16")
+
+
+def test_attend_empty_calls():
+    c = Case([20], 1, 64, 64, 16)
+    cache = c.device()
+    assert cache.attend(torch.zeros(1, 0, 2, 64, device=DEV, dtype=torch.bfloat16), c.t, ints([20])).shape == (1, 0, 2, 64)
+    assert cache.attend(torch.zeros(0, 1, 2, 64, device=DEV, dtype=torch.bfloat16), c.t[:0], ints([])).shape == (0, 1, 2, 64)
+    z = torch.zeros(1, 0, 1, 64, device=DEV)
+    cache.write(z, z, c.t, ints([3]))
+    out = cache.attend(torch.ones(1, 2, 2, 64, device=DEV, dtype=torch.bfloat16), c.t, ints([20]), count=ints([0]))
+    assert (out == 0).all()
+    cache.check()
+
+
+def test_attend_many_sequences():
+    B = 700
+    lens = [(37 * b) % 90 for b in range(B)]
+    c = Case(lens, 1, 16, 16, 16)
+    cache = c.device()
+    q = torch.randn(B, 1, 1, 16, device=DEV, dtype=torch.float16)
+    out = cache.attend(q, c.t, ints(lens))
+    want, tol = expect(c, q.double().cpu().numpy(), [1] * B, 1, 0.25)
+    check(out, want, tol, [1] * B, "f16")
+
+
+@pytest.mark.parametrize("rows", [1, 96])
+def test_attend_captured_replayed_and_on_two_streams(rows):
+    """A captured call serves other lengths; two captured calls and an eager one on streams of their own, on the same cache, do not meet."""
+    c = Case([600, 600], 2, 128, 128, 64)
+    cache = c.device()
+    lens = ints([600, 600])
+    q = torch.randn(2, rows, 8, 128, device=DEV, dtype=torch.bfloat16)
+    outs = [torch.zeros(2, rows, 8, 128, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+    cache.attend(q, c.t, lens, out=outs[0])
+    graphs = []
+    for o in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            cache.attend(q, c.t, lens, out=o)
+        graphs.append(g)
+    for n in ([600, 600], [rows + 5, 431], [rows, 598]):
+        lens.copy_(ints(n))
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        for _ in range(5):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+            with torch.cuda.stream(streams[2]):
+                third = cache.attend(q, c.t, lens)
+        torch.cuda.synchronize()
+        want, tol = expect(c, q.double().cpu().numpy(), [rows] * 2, 8, 128 ** -0.5, lens=n)
+        check(outs[0], want, tol, [rows] * 2, "bf16")
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], third)
+
+
+def test_refusals():
+    c = Case([20], 2, 64, 64, 16)
+    cache = c.device()
+    q = torch.zeros(1, 1, 4, 64, device=DEV, dtype=torch.bfloat16)
+    bad = [
+        (dict(q=q.float()), "F16 or BF16"), (dict(q=q[:, :, :3]), "multiple"), (dict(q=q[..., :32]), "queries"), (dict(q=q[..., ::2]), "queries"), (dict(q=q.cpu()), "CUDA"),
+        (dict(table=c.t.long()), "table"), (dict(table=c.t.cpu()), "CUDA"), (dict(lens=ints([20, 20])), "lengths"), (dict(lens=ints([20]).long()), "lengths"), (dict(count=ints([1, 1])), "count"),
+        (dict(window=-1), "negative"), (dict(keep_first=-1), "negative"), (dict(scale=float("nan")), "number"), (dict(out=q.half()), "results"), (dict(out=q[..., :32]), "output"),
+        (dict(out=q[:, :, :1].expand(1, 1, 4, 64)), "overlap"), (dict(q=q[:, :, :0]), "multiple"),
+    ]
+    for kw, text in bad:
+        a = dict(q=q, table=c.t, lens=ints([20]))
+        a.update(kw)
+        with pytest.raises(dsk.DskError, match=text):
+            cache.attend(**a)
+    x = torch.zeros(1, 1, 2, 64, device=DEV)
+    for a, text in (((x.long(), x), "values of"), ((x.double(), x.double()), "float32"), ((x, x.half()), "values of"), ((x[:, :, :1], x), "keys"), ((x, x[..., :48]), "values"), ((x[0], x), "batch, rows")):
+        with pytest.raises(dsk.DskError, match=text):
+            cache.write(*a, c.t, ints([0]))
+    with pytest.raises(dsk.DskError, match="one type"):
+        cache.read(c.t, ints([0]), 1, out=(x, x.half()))
+    with pytest.raises(dsk.DskError, match="contiguous"):
+        dsk.Cache8.of(cache.k[:, :, ::2], cache.v, cache.k_scale, cache.v_scale)
+    with pytest.raises(dsk.DskError, match="multiple of 16"):
+        odd = dsk.Cache8(2, 1, 24)
+        odd.write(torch.zeros(1, 1, 1, 24, device=DEV), torch.zeros(1, 1, 1, 24, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV), ints([0]))
+    v = dsk.View(x.data_ptr(), 3, 128, 128, 64)
+    s = cache._rows(c.t, ints([0]), None, 1)
+    assert dsk.lib().dsk_kv8_write(cache._c, s, v, v, None) != 0 and b"F32, F16 or BF16" in dsk.lib().dsk_last_error()
+    a, b = cache._view("q", q, q.shape), cache._view("o", q, q.shape)
+    assert dsk.lib().dsk_kv8_attn(cache._c, s, a, b, 4, 1.0, 0, 0, None, 0, None) != 0 and b"workspace" in dsk.lib().dsk_last_error()

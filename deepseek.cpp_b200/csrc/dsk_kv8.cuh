@@ -74,6 +74,9 @@ __device__ __forceinline__ uint32_t two_halves(uint32_t codes) {                
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(codes));
   return r;
 }
+__device__ __forceinline__ void four_halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 __device__ __forceinline__ float2 two_values(uint32_t codes) {
   const uint32_t h = two_halves(codes);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));

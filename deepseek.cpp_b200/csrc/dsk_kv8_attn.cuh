@@ -1,14 +1,15 @@
 // dsk_kv8_attn.cuh — softmax attention of decoded tokens and drafts over the 8-bit cache (dsk_kv8.cuh).
 //
-// The rows of a key head are its query heads' queries, `group` heads x `rows` tokens; a tile of 16 (two tiles: 32) meets the keys in steps of 16 on mma.sync, fp16 operands
-// and fp32 sums.  An E4M3 code is exact in fp16, so keys and values go from their codes to operands by a conversion alone; a query row is divided by a power of two that
-// puts its largest entry near 2^10 (what that leaves below fp16's range is 2^-24 of the row).  The scales are applied around the products: the key block's to the scores, and the value block's
-// inside the softmax, w_j = 2^(t_j - m) with t_j = score_j + log2(value scale), so that a weight with its scale is one fp16 number of at most 2^kSlack and the sum takes w_j / (value scale).
-// Rounding: the weights to fp16, 2^-11 of each; queries in fp16 or bf16 are exact.
-// Work: the steps of all sequences, key heads and row tiles lie in one line that the CTAs share out evenly (four steps, 64 keys, to a unit), whatever the lengths; a CTA that has a
-// whole (sequence, head, row tile) stores it, pieces are joined by `join`.  Every warp has every fourth step, with stages of its own that cp.async fills: no barrier but where
+// The queries of a key head are its query heads' queries, `group` heads x `rows` tokens, in tiles of 8.  Products run on mma.sync with keys and values as the left operand:
+// scores (16 keys x 8 queries) = K Q^T, results (16 entries x 8 queries) = V^T W; a left operand is converted once whatever the number of query tiles (1, 2 or 4), and no row of a product is
+// empty with the few queries of decoding.  An E4M3 code is exact in fp16, so keys and values go from their codes to operands by a conversion alone; a query is divided by a power
+// of two that puts its largest entry near 2^10 (what that leaves below fp16's range is 2^-24 of it).  The scales are applied around the products: the key block's to the
+// scores, the value block's inside the softmax, w_j = 2^(t_j - m) with t_j = score_j + log2(value scale), so that a weight with its scale is one fp16 number of at most 2^kSlack
+// and the sum takes w_j / (value scale).  Rounding: the weights to fp16, 2^-11 of each; queries in fp16 or bf16 are exact.
+// Work: the steps (16 or 32 keys) of all sequences, key heads and query tiles lie in one line that the CTAs share out evenly, four steps to a unit, whatever the lengths; a CTA that has
+// a whole (sequence, head, tile) stores it, pieces are joined by `join`.  Every warp has every fourth step, with stages of its own that cp.async fills: no barrier but where
 // a piece ends, and the copies run on across pieces.
-// Bound: bytes of the cache.  Fragments come from shared memory as whole 16-byte pieces, entries and keys permuted alike on both sides of a product: a quarter warp's lanes (two
+// Fragments come from shared memory as whole 16-byte pieces, entries and keys permuted alike on both sides of a product: a quarter warp's lanes (two
 // keys x four pieces) are keys j and j + 4, whose rows lie 16 banks apart.
 #pragma once
 
@@ -17,7 +18,8 @@
 namespace dsk {
 namespace kv8 {
 
-constexpr int kStep = 16, kWarps = 4, kUnit = kStep * kWarps, kThreads = 32 * kWarps, kMaxBatch = 1024;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxBatch = 1024;
+__host__ __device__ constexpr int step_of(int qt) { return qt < 4 ? 32 : 16; }   // keys of a warp's step
 constexpr float kSlack = 8.f;                                // the reference of a row's weights follows its maximum once that is 2^8 ahead
 
 struct Attn {
@@ -26,38 +28,50 @@ struct Attn {
   const void* q;
   void* out;
   Pitch pq, po;
-  int heads, group, row_tiles, bf16, wide_q, wide_o, window, keep;
+  int heads, group, row_tiles, bf16, wide_q, wide_o, window, keep, shift;   // shift: log2 of the block
   float scale;                                               // times log2(e)
   long long* ends;                                           // workspace: [batch + 1] first units of the sequences (a head's row tile), and pieces
   float* part;
 };
 
 // What a sequence has: visible steps are the first `kept` ones and those from `low` on
-struct Seq { int len, count, kept, low, steps, units; };
-__device__ __forceinline__ Seq sequence(const Attn& P, int b) {
+struct Seq { int len, count, kept, low, steps, units, first, last; };   // first, last: positions of the queries
+template <int STEP> __device__ __forceinline__ Seq sequence(const Attn& P, int b) {
   Seq q;
-  const long long room = (long long)P.S.table_blocks * P.C.block;
+  const long long room = (long long)P.S.table_blocks << P.shift;
   const int len = P.S.first[b];
   q.count = P.S.count ? min(max(P.S.count[b], 0), P.S.rows) : P.S.rows;
   q.len = (int)min((long long)max(len, 0), room);
   const long long first = (long long)len - q.count + 1 - P.window;
-  q.low = P.window > 0 && first > 0 ? (int)min(first, (long long)q.len) / kStep : 0;
-  q.kept = P.window > 0 ? min((min(P.keep, q.len) + kStep - 1) / kStep, q.low) : 0;
-  q.steps = q.kept + (q.len + kStep - 1) / kStep - q.low;
+  q.low = P.window > 0 && first > 0 ? (int)min(first, (long long)q.len) / STEP : 0;
+  q.kept = P.window > 0 ? min((min(P.keep, q.len) + STEP - 1) / STEP, q.low) : 0;
+  q.steps = q.kept + (q.len + STEP - 1) / STEP - q.low;
   q.units = q.count ? max(1, (q.steps + kWarps - 1) / kWarps) : 0;
+  q.last = len - 1;
+  q.first = len - q.count;
   return q;
 }
 
-template <int DK, int DV, int MT> __host__ __device__ constexpr int stages() {   // as many as two CTAs of an SM have room for
-  return DK == 64 ? 6 : DK == 128 ? (MT == 1 ? 4 : 3) : DK == 192 ? (MT == 1 ? 3 : 2) : 2;
+template <int DK, int DV, int QT> __host__ __device__ constexpr int stages() {   // as many as two CTAs of an SM have room for
+  return DK == 64 ? (QT < 4 ? 3 : 6) : DK == 128 ? (QT < 4 ? 2 : 3) : 2;
 }
-template <int DK, int DV> __host__ __device__ constexpr int stage_bytes() { return kStep * (DK + 16 + DV + 32) + 16; }
-template <int DK, int DV, int MT> __host__ __device__ constexpr int attn_smem() {
-  return kWarps * stages<DK, DV, MT>() * stage_bytes<DK, DV>() + MT * 16 * (2 * DK + 16) + 2 * MT * DV / 8 * 4 * 128 + (2 * kWarps + 1) * MT * 16 * 4;
+template <int DK, int DV> __host__ __device__ constexpr int stage_bytes(int step) { return step * (DK + 16 + DV + 32) + 16; }
+template <int DK, int DV, int QT> __host__ __device__ constexpr int attn_smem() {
+  return kWarps * stages<DK, DV, QT>() * stage_bytes<DK, DV>(step_of(QT)) + QT * 8 * (2 * DK + 16) + 2 * QT * DV / 4 * 128 + (2 * kWarps + 1) * QT * 8 * 4;
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+template <int to, int from> __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(to), "n"(from) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+// pieces J .. N - 1 of a lane, 512 bytes apart where they come from; they go to place[j] of the u-th 16 rows
+template <int N, int J, int HALF> __device__ __forceinline__ void copy_rows(uint32_t to, const uint32_t (&place)[N], const unsigned char* from, int u) {
+  if constexpr (J < N) {
+    if (u == 0) copy16<0, J * 512>(to + place[J], from); else copy16<HALF, J * 512>(to + place[J], from);
+    copy_rows<N, J + 1, HALF>(to, place, from, u);
+  }
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -70,6 +84,11 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t x) {     // an 8 x 8 matrix of 16-bit entries (row lane / 4, two entries a lane), transposed
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {        // 2 ulp, results below 2^-126 are zero
   float r;
@@ -86,9 +105,10 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {   // 0xff where a by
 }
 
 // A place in the line of units
-struct Place {
+template <int STEP> struct Place {
   Seq q;
-  int b, hr, unit;
+  int b, head, tile, unit;
+  const int* table;                                          // the sequence's row
   __device__ __forceinline__ void find(const Attn& P, const long long* ends, long long x, int per) {   // per: heads x row tiles
     int lo = 0, hi = P.S.batch - 1;
     while (lo < hi) {
@@ -96,19 +116,25 @@ struct Place {
       if (ends[mid] * per <= x) lo = mid; else hi = mid - 1;
     }
     b = lo;
-    q = sequence(P, b);
+    table = P.S.table + b * P.S.table_pitch;
+    q = sequence<STEP>(P, b);
     const long long in = x - ends[b] * per;
-    hr = (int)(in / q.units);
+    const int hr = (int)(in / q.units);
     unit = (int)(in - (long long)hr * q.units);
+    head = hr / P.row_tiles;
+    tile = hr - head * P.row_tiles;
   }
-  __device__ __forceinline__ void next(const Attn& P, int per) {
+  __device__ __forceinline__ void next(const Attn& P) {
     if (++unit < q.units) return;
     unit = 0;
-    if (++hr < per) return;
-    hr = 0;
+    if (++tile < P.row_tiles) return;
+    tile = 0;
+    if (++head < P.C.heads) return;
+    head = 0;
     do {
       if (++b >= P.S.batch) return;
-      q = sequence(P, b);
+      table += P.S.table_pitch;
+      q = sequence<STEP>(P, b);
     } while (q.units == 0);
   }
 };
@@ -135,28 +161,30 @@ struct Out {
   }
 };
 
-// DK, DV: entries of keys and values, rounded up; MT: tiles of 16 rows
-template <int DK, int DV, int MT>
+// DK, DV: entries of keys and values, rounded up; QT: tiles of 8 queries
+template <int DK, int DV, int QT>
 __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
-  constexpr int NST = stages<DK, DV, MT>(), KS = DK + 16, VS = DV + 32, SB = stage_bytes<DK, DV>(), QS = 2 * DK + 16, NT = DV / 8, VCH = DV >= 128 ? 16 : 8, HF = DV / (8 * VCH);
-  constexpr bool QREG = MT == 1 && DK <= 128;
+  constexpr int NST = stages<DK, DV, QT>(), KS = DK + 16, VS = DV + 32, STEP = step_of(QT), HV = STEP / 16, SB = stage_bytes<DK, DV>(STEP), QS = 2 * DK + 16, VCH = DV >= 128 ? 16 : 8,
+                HF = DV / (8 * VCH), NO = DV / 16;           // NO: tiles of 16 entries; a lane's entries are VCH neighbours, two to a tile
+  constexpr bool QREG = QT * DK <= 256;
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ long long warp_sums[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, B = P.S.batch;
   unsigned char* q_raw = raw + kWarps * NST * SB;
-  float* turn = reinterpret_cast<float*>(q_raw + MT * 16 * QS);          // [2][accumulators][lane]
-  float* row_m = turn + 2 * MT * NT * 4 * 32;                            // [warp][row]
-  float* row_l = row_m + kWarps * MT * 16;
-  float* row_q = row_l + kWarps * MT * 16;                               // factor of a row's scores
-  long long* ends = reinterpret_cast<long long*>(raw + ((attn_smem<DK, DV, MT>() + 7) & ~7));
+  float* turn = reinterpret_cast<float*>(q_raw + QT * 8 * QS);           // [2][accumulators][lane]
+  float* row_m = turn + 2 * QT * NO * 4 * 32;                            // [warp][query]
+  float* row_l = row_m + kWarps * QT * 8;
+  float* row_q = row_l + kWarps * QT * 8;                                // factor of a query's scores
+  long long* ends = reinterpret_cast<long long*>(raw + ((attn_smem<DK, DV, QT>() + 7) & ~7));
   const uint32_t stage0 = smem_u32(raw) + warp * NST * SB, q0 = smem_u32(q_raw);
   grid_release();
   // line of units: running sums over the sequences
-  for (int i = threadIdx.x; i < NST * SB * kWarps / 16; i += kThreads) reinterpret_cast<uint4*>(raw)[i] = make_uint4(0, 0, 0, 0);   // (entries behind the last one stay zero)
+  if (P.C.dim[0] < DK || P.C.dim[1] < DV)
+    for (int i = threadIdx.x; i < NST * SB * kWarps / 16; i += kThreads) reinterpret_cast<uint4*>(raw)[i] = make_uint4(0, 0, 0, 0);   // (entries behind the last one stay zero)
   long long run = 0;
   for (int b0 = 0; b0 < B; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    const long long own = b < B ? sequence(P, b).units : 0;
+    const long long own = b < B ? sequence<STEP>(P, b).units : 0;
     long long v = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += t; }
@@ -182,97 +210,117 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
   if ((long long)blockIdx.x >= N) return;
   const long long x0 = blockIdx.x * total / N, x1 = (blockIdx.x + 1) * total / N;
   __syncthreads();
-  const int dk = P.C.dim[0], dv = P.C.dim[1], dk16 = dk / 16, dv16 = dv / 16;
-  const size_t block_k = (size_t)P.C.block * dk, block_v = (size_t)P.C.block * dv;
+  const int dk = P.C.dim[0], dv = P.C.dim[1], dk16 = dk / 16, dv16 = dv / 16, mine = (int)(x1 - x0);
+  const bool exact = dk == DK && dv == DV;
+  const uint32_t head_k = P.C.block * dk, head_v = P.C.block * dv, block_k = P.C.heads * head_k, block_v = P.C.heads * head_v;   // bytes of a head and of a block (at most 2^30)
+  const float* my_scale = P.C.scale[lane & 1];
 
-  // copies: a step of this warp to a unit, from a block whose number was looked up a unit ahead
-  Place at;                                                  // of the next copies
+  // copies: a step of this warp to a unit, from a block whose number was looked up a unit ahead; 16-byte pieces lane, lane + 32, .. of a step's rows, which lie side by side
+  uint32_t to_k[DK / 32], to_v[DV / 32];
+#pragma unroll
+  for (int j = 0; j < DK / 32; j++) { const int i = lane + 32 * j, row = i / dk16; to_k[j] = row * KS + (i - row * dk16) * 16; }
+#pragma unroll
+  for (int j = 0; j < DV / 32; j++) { const int i = lane + 32 * j, row = i / dv16; to_v[j] = STEP * KS + row * VS + (i - row * dv16) * 16; }
+  Place<STEP> at;                                            // of the next copies
   at.find(P, ends, x0, per);
-  long long x = x0;
-  int page = -1, key = 0;
+  int ahead = mine, page[HV], key = -1;                      // units that are not under way yet; the next step's blocks (of 16 keys each) and first key (-1: this warp has none)
   auto look = [&]() {
-    page = -1;
     const int s = at.unit * kWarps + warp;
-    if (x < x1 && s < at.q.steps) {
-      key = (s < at.q.kept ? s : at.q.low + s - at.q.kept) * kStep;
-      page = __ldg(P.S.table + at.b * P.S.table_pitch + key / P.C.block);
+    key = -1;
+    if (ahead > 0 && s < at.q.steps) {
+      key = (s < at.q.kept ? s : at.q.low + s - at.q.kept) * STEP;
+      page[0] = __ldg(at.table + (key >> P.shift));
+      if (HV == 2) page[HV - 1] = P.shift > 4 ? page[0] : key + 16 < at.q.len ? __ldg(at.table + (key >> 4) + 1) : 0;
     }
   };
   auto fetch = [&](int stage) {
-    const int s = at.unit * kWarps + warp;
-    if (x < x1 && s < at.q.steps) {
-      const bool ok = (unsigned)page < (unsigned)P.C.n_blocks;
-      if (!ok && lane == 0) note(P.C, ST_PAGE);
-      const size_t slot = ok ? (size_t)page * P.C.heads + at.hr / P.row_tiles : 0;
-      const int there = ok ? at.q.len - key : 0, row0 = key % P.C.block;     // (what is behind the last key comes as zeros)
-      const unsigned char* k = P.C.code[0] + slot * block_k + row0 * dk;
-      const unsigned char* v = P.C.code[1] + slot * block_v + row0 * dv;
+    if (key >= 0) {
       const uint32_t to = stage0 + stage * SB;
-      for (int i = lane; i < dk; i += 32) { const int row = i / dk16; copy16(to + row * KS + (i - row * dk16) * 16, row < there ? k + i * 16 : k, row < there ? 16 : 0); }
-      for (int i = lane; i < dv; i += 32) { const int row = i / dv16; copy16(to + kStep * KS + row * VS + (i - row * dv16) * 16, row < there ? v + i * 16 : v, row < there ? 16 : 0); }
-      if (lane < 2) copy4(to + kStep * (KS + VS) + lane * 4, P.C.scale[lane] + slot, ok ? 4 : 0);
+#pragma unroll
+      for (int u = 0; u < HV; u++) {
+        const bool ok = (unsigned)page[u] < (unsigned)P.C.n_blocks;
+        const uint32_t at_page = ok ? page[u] : 0, row0 = (key + 16 * u) & (P.C.block - 1);
+        const unsigned char* k = P.C.code[0] + ((uint64_t)at_page * block_k + (at.head * head_k + row0 * dk + lane * 16));
+        const unsigned char* v = P.C.code[1] + ((uint64_t)at_page * block_v + (at.head * head_v + row0 * dv + lane * 16));
+        const float* scale = my_scale + ((uint64_t)at_page * (uint32_t)P.C.heads + at.head);
+        if (ok && exact && key + 16 * u + 16 <= at.q.len) {
+          copy_rows<DK / 32, 0, 16 * KS>(to, to_k, k, u);
+          copy_rows<DV / 32, 0, 16 * VS>(to, to_v, v, u);
+          if (lane < 2) copy4(to + STEP * (KS + VS) + u * 8 + lane * 4, scale, 4);
+        } else {                                             // what is behind the last key, or in a block outside the cache, comes as zeros
+          if (!ok && lane == 0) note(P.C, ST_PAGE);
+          const int there = ok ? at.q.len - key - 16 * u : 0;
+          for (int i = lane; i < dk; i += 32) { const int row = i / dk16; copy16_or_zero(to + (u * 16 + row) * KS + (i - row * dk16) * 16, row < there ? k + (i - lane) * 16 : P.C.code[0], row < there); }
+          for (int i = lane; i < dv; i += 32) { const int row = i / dv16; copy16_or_zero(to + STEP * KS + (u * 16 + row) * VS + (i - row * dv16) * 16, row < there ? v + (i - lane) * 16 : P.C.code[1], row < there); }
+          if (lane < 2) copy4(to + STEP * (KS + VS) + u * 8 + lane * 4, ok ? scale : P.C.scale[0], ok ? 4 : 0);
+        }
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (x < x1) { at.next(P, per); x++; }
+    if (--ahead > 0) at.next(P);
     look();
   };
   look();
 #pragma unroll 1
   for (int i = 0; i < NST - 1; i++) fetch(i);
 
-  float o[MT][NT][4], m[MT][2], l[MT][2];
-  uint32_t qf[QREG ? DK / 16 : 1][4];
-  Place pl;
+  float o[QT][NO][4], m[QT][2], l[QT][2], fq[QT][2];         // a lane's queries: 2 c and 2 c + 1 of a tile; fq: factor of their scores
+  uint32_t qf[QREG ? QT : 1][QREG ? DK / 16 : 1][2];
+  Place<STEP> pl;
   pl.find(P, ends, x0, per);
   int begun = pl.unit, stage = 0;                            // the piece's first unit
   bool fresh = true;
 #pragma unroll 1
-  for (long long y = x0; y < x1; y++) {
-    const Seq q = pl.q;
-    const int head = pl.hr / P.row_tiles, row0 = (pl.hr - head * P.row_tiles) * MT * 16;
+  for (int y = 0; y < mine; y++) {
+    const Seq& q = pl.q;
+    const int head = pl.head, row0 = pl.tile * QT * 8;
     if (fresh) {                                             // query rows as fp16, each by its own power of two
       __syncthreads();
-      for (int row = warp; row < MT * 16; row += kWarps) {
-        const int i = (row0 + row) / P.group;
-        const uint16_t* src = static_cast<const uint16_t*>(P.q) + pl.b * P.pq.batch + i * P.pq.row + (long long)(head * P.group + row0 + row - i * P.group) * P.pq.head;
+      uint32_t qv[QT * 2][DK / 64];
+#pragma unroll
+      for (int u = 0; u < QT * 2; u++) {
+        const int row = row0 + u * kWarps + warp, i = row / P.group;
+        const uint16_t* src = static_cast<const uint16_t*>(P.q) + pl.b * P.pq.batch + i * P.pq.row + (long long)(head * P.group + row - i * P.group) * P.pq.head + lane * 2;
+#pragma unroll
+        for (int k = 0; k < DK / 64; k++) {
+          qv[u][k] = 0;
+          if (i < q.count && k * 64 + lane * 2 < dk) qv[u][k] = P.wide_q ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 64)) : src[k * 64] | (uint32_t)src[k * 64 + 1] << 16;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < QT * 2; u++) {
+        const int row = u * kWarps + warp;
         float v[DK / 32], top = 0.f;
 #pragma unroll
-        for (int k = 0; k < DK / 64; k++)
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const int d = k * 64 + lane * 2 + u;
-            float f = 0.f;
-            if (i < q.count && d < dk) f = P.bf16 ? __bfloat162float(__ushort_as_bfloat16(src[d])) : __half2float(__ushort_as_half(src[d]));
-            v[2 * k + u] = f;
-            const float a = fabsf(f);
-            top = fmaxf(top, a < INFINITY ? a : 0.f);
-          }
+        for (int k = 0; k < DK / 64; k++) {
+          const float2 f = P.bf16 ? make_float2(__uint_as_float(qv[u][k] << 16), __uint_as_float(qv[u][k] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&qv[u][k]));
+          v[2 * k] = f.x; v[2 * k + 1] = f.y;
+          const float x = fabsf(f.x), y = fabsf(f.y);
+          top = fmaxf(top, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
+        }
         top = warp_max(top);
         const int e = top > 0.f ? max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127 - 10)) : 0;
-        const float by = pow2(-e);
+        const float by = P.scale < 0.f ? -pow2(-e) : pow2(-e);               // (factors of scores are positive)
 #pragma unroll
         for (int k = 0; k < DK / 64; k++) *reinterpret_cast<uint32_t*>(q_raw + row * QS + (k * 64 + lane * 2) * 2) = halves(v[2 * k] * by, v[2 * k + 1] * by);
-        if (lane == 0) row_q[row] = pow2(e) * P.scale;
+        if (lane == 0) row_q[row] = pow2(e) * fabsf(P.scale);
       }
       __syncthreads();
       if constexpr (QREG) {
 #pragma unroll
-        for (int g = 0; g < DK / 64; g++)
+        for (int t = 0; t < QT; t++)
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const uint4 a = lds128(q0 + r * QS + (g * 64 + 16 * c + 8 * h) * 2), b = lds128(q0 + (r + 8) * QS + (g * 64 + 16 * c + 8 * h) * 2);
-            uint32_t* f = qf[g * 4 + 2 * h];
-            f[0] = a.x; f[1] = b.x; f[2] = a.y; f[3] = b.y;
-            f = qf[g * 4 + 2 * h + 1];
-            f[0] = a.z; f[1] = b.z; f[2] = a.w; f[3] = b.w;
+          for (int i = 0; i < DK / 32; i++) {
+            const uint4 a = lds128(q0 + (t * 8 + r) * QS + (i / 2 * 64 + 16 * c + 8 * (i & 1)) * 2);
+            qf[t][2 * i][0] = a.x; qf[t][2 * i][1] = a.y; qf[t][2 * i + 1][0] = a.z; qf[t][2 * i + 1][1] = a.w;
           }
       }
 #pragma unroll
-      for (int t = 0; t < MT; t++) {
-        m[t][0] = m[t][1] = -1e30f;
-        l[t][0] = l[t][1] = 0.f;
+      for (int t = 0; t < QT; t++) {
 #pragma unroll
-        for (int k = 0; k < NT; k++)
+        for (int e = 0; e < 2; e++) { m[t][e] = -1e30f; l[t][e] = 0.f; fq[t][e] = row_q[t * 8 + 2 * c + e]; }
+#pragma unroll
+        for (int k = 0; k < NO; k++)
 #pragma unroll
           for (int u = 0; u < 4; u++) o[t][k][u] = 0.f;
       }
@@ -284,158 +332,180 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     const int step = pl.unit * kWarps + warp;
     if (step < q.steps) {
       const uint32_t from = stage0 + stage * SB;
-      const int key0 = (step < q.kept ? step : q.low + step - q.kept) * kStep;
-      const float ks = __uint_as_float(lds32(from + kStep * (KS + VS))), vs = __uint_as_float(lds32(from + kStep * (KS + VS) + 4));
-      const float lift = (float)((int)(__float_as_uint(vs) >> 23) - 127), back = vs > 0.f ? 1.f / vs : 0.f;
-      float s[MT][2][4];
+      const int key0 = (step < q.kept ? step : q.low + step - q.kept) * STEP;
+      float ks[HV], lift[HV], back[HV];                      // scales: of keys; of values as exponent and reciprocal
+      bool gone = false;
 #pragma unroll
-      for (int t = 0; t < MT; t++)
+      for (int u = 0; u < HV; u++) {
+        ks[u] = __uint_as_float(lds32(from + STEP * (KS + VS) + u * 8));
+        const float vs = __uint_as_float(lds32(from + STEP * (KS + VS) + u * 8 + 4));
+        lift[u] = (float)((int)(__float_as_uint(vs) >> 23) - 127);
+        back[u] = pow2(-(int)lift[u]);
+        if (vs == 0.f) { back[u] = 0.f; gone = true; }
+      }
+      float s[QT][HV][4];                                    // keys r, r + 8 (permuted) x queries 2 c, 2 c + 1
 #pragma unroll
-        for (int u = 0; u < 4; u++) s[t][0][u] = s[t][1][u] = 0.f;
-      const uint32_t krow = from + ((r >> 1) + 4 * (r & 1)) * KS + c * 16;
+      for (int t = 0; t < QT; t++)
+#pragma unroll
+        for (int u = 0; u < HV; u++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[t][u][i] = 0.f;
+      const int turn_r = (r >> 1) + 4 * (r & 1);
+      const uint32_t krow = from + turn_r * KS + c * 16;
 #pragma unroll
       for (int g = 0; g < DK / 64; g++) {
-        const uint4 k0 = lds128(krow + g * 64), k1 = lds128(krow + 8 * KS + g * 64);
-        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+        uint32_t kw[HV][2][4];
+#pragma unroll
+        for (int u = 0; u < HV; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) { const uint4 x = lds128(krow + (u * 16 + e * 8) * KS + g * 64); kw[u][e][0] = x.x; kw[u][e][1] = x.y; kw[u][e][2] = x.z; kw[u][e][3] = x.w; }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          uint32_t a[MT][2][4];
-          if constexpr (QREG) {
+          uint32_t a[HV][2][4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) { a[0][0][u] = qf[g * 4 + 2 * h][u]; a[0][1][u] = qf[g * 4 + 2 * h + 1][u]; }
-          } else {
+          for (int u = 0; u < HV; u++)
 #pragma unroll
-            for (int t = 0; t < MT; t++) {
-              const uint4 x = lds128(q0 + (t * 16 + r) * QS + (g * 64 + 16 * c + 8 * h) * 2), y = lds128(q0 + (t * 16 + r + 8) * QS + (g * 64 + 16 * c + 8 * h) * 2);
-              a[t][0][0] = x.x; a[t][0][1] = y.x; a[t][0][2] = x.y; a[t][0][3] = y.y;
-              a[t][1][0] = x.z; a[t][1][1] = y.z; a[t][1][2] = x.w; a[t][1][3] = y.w;
+            for (int x = 0; x < 2; x++) { four_halves(kw[u][0][2 * h + x], a[u][x][0], a[u][x][2]); four_halves(kw[u][1][2 * h + x], a[u][x][1], a[u][x][3]); }
+#pragma unroll
+          for (int t = 0; t < QT; t++) {
+            uint32_t b[2][2];
+            if constexpr (QREG) {
+#pragma unroll
+              for (int x = 0; x < 2; x++) { b[x][0] = qf[t][g * 4 + 2 * h + x][0]; b[x][1] = qf[t][g * 4 + 2 * h + x][1]; }
+            } else {
+              const uint4 y = lds128(q0 + (t * 8 + r) * QS + (g * 64 + 16 * c + 8 * h) * 2);
+              b[0][0] = y.x; b[0][1] = y.y; b[1][0] = y.z; b[1][1] = y.w;
             }
-          }
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const uint32_t b0 = two_halves(w0[2 * h + e]), b1 = two_halves(w0[2 * h + e] >> 16), b2 = two_halves(w1[2 * h + e]), b3 = two_halves(w1[2 * h + e] >> 16);
+            for (int x = 0; x < 2; x++)
 #pragma unroll
-            for (int t = 0; t < MT; t++) { mma16(s[t][0], a[t][e], b0, b1); mma16(s[t][1], a[t][e], b2, b3); }
+              for (int u = 0; u < HV; u++) mma16(s[t][u], a[u][x], b[x][0], b[x][1]);
           }
         }
       }
-      // a step that every row sees needs no mask
-      const int last = P.S.first[pl.b] - 1, first = last + 1 - q.count;    // positions of the last and first query
-      const bool masked = key0 + kStep - 1 > first || (P.window > 0 && last - key0 >= P.window && key0 + kStep > P.keep) || vs == 0.f;
-      uint32_t pf[MT][4], seen[MT] = {};                     // weights as fp16; keys that this lane's rows see: a bit to a score
+      // a step that every query sees needs no mask
+      const bool masked = key0 + STEP - 1 > q.first || (P.window > 0 && q.last - key0 >= P.window && key0 + STEP > P.keep) || gone;
+      uint32_t seen[QT] = {};                                // keys that this lane's queries see: a bit to a score
+      if (masked) {
 #pragma unroll
-      for (int t = 0; t < MT; t++) {
+        for (int t = 0; t < QT; t++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const float f = row_q[t * 16 + r + 8 * h] * ks;
+          for (int e = 0; e < 2; e++) {
+            const int pos = q.first + (row0 + t * 8 + 2 * c + e) / P.group;
 #pragma unroll
-          for (int g = 0; g < 2; g++)
+            for (int u = 0; u < HV; u++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) s[t][g][2 * h + e] = fmaf(s[t][g][2 * h + e], f, lift);
-          if (masked) {
-            const int pos = first + (row0 + t * 16 + r + 8 * h) / P.group;
-#pragma unroll
-            for (int g = 0; g < 2; g++)
-#pragma unroll
-              for (int e = 0; e < 2; e++) {
-                const int j = key0 + 8 * g + c + 4 * e;
-                const bool ok = vs != 0.f && j < q.len && j <= pos && (P.window <= 0 || pos - j < P.window || j < P.keep);
-                if (ok) seen[t] |= 1u << (g * 4 + 2 * h + e); else s[t][g][2 * h + e] = -INFINITY;
+              for (int h = 0; h < 2; h++) {
+                const int j = key0 + 16 * u + 8 * h + turn_r;
+                const bool ok = back[u] != 0.f && j < q.len && j <= pos && (P.window <= 0 || pos - j < P.window || j < P.keep);
+                if (ok) seen[t] |= 1u << (u * 4 + 2 * h + e); else s[t][u][2 * h + e] = -INFINITY;
               }
           }
-        }
-        float mx[2];
+      }
+      uint32_t w[QT][HV][2];                                 // weights as right operands: [query r][keys 2 c, 2 c + 1]
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          mx[h] = fmaxf(fmaxf(s[t][0][2 * h], s[t][0][2 * h + 1]), fmaxf(s[t][1][2 * h], s[t][1][2 * h + 1]));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      for (int t = 0; t < QT; t++) {
+        float f[2][HV], mx[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          mx[e] = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < HV; u++) {
+            f[e][u] = fmaxf(fq[t][e] * ks[u], 1.17549435e-38f);      // (positive: -inf stays what it is)
+            mx[e] = fmaxf(mx[e], fmaf(fmaxf(s[t][u][e], s[t][u][2 + e]), f[e][u], lift[u]));
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
         }
         if (__any_sync(0xffffffffu, mx[0] > m[t][0] + kSlack || mx[1] > m[t][1] + kSlack)) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const float to = fmaxf(m[t][h], mx[h]), f = exp2_fast(m[t][h] - to);
-            m[t][h] = to;
-            l[t][h] *= f;
+          for (int e = 0; e < 2; e++) {
+            const float to = fmaxf(m[t][e], mx[e]), by = exp2_fast(m[t][e] - to);
+            m[t][e] = to;
+            l[t][e] *= by;
 #pragma unroll
-            for (int k = 0; k < NT; k++) { o[t][k][2 * h] *= f; o[t][k][2 * h + 1] *= f; }
+            for (int k = 0; k < NO; k++) { o[t][k][e] *= by; o[t][k][2 + e] *= by; }
           }
         }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float sum = 0.f;
+        for (int u = 0; u < HV; u++) {
+          float p[4];
 #pragma unroll
-          for (int g = 0; g < 2; g++) {
-            const float p0 = exp2_fast(s[t][g][2 * h] - m[t][h]), p1 = exp2_fast(s[t][g][2 * h + 1] - m[t][h]);
-            sum += p0 + p1;
-            pf[t][2 * g + h] = halves(p0, p1);
+          for (int e = 0; e < 2; e++) {
+            const float off = lift[u] - m[t][e];
+            p[e] = exp2_fast(fmaf(s[t][u][e], f[e][u], off));
+            p[2 + e] = exp2_fast(fmaf(s[t][u][2 + e], f[e][u], off));
+            l[t][e] = fmaf(p[e] + p[2 + e], back[u], l[t][e]);
           }
-          l[t][h] = fmaf(sum, back, l[t][h]);
+          w[t][u][0] = turned(halves(p[0], p[1]));
+          w[t][u][1] = turned(halves(p[2], p[3]));
         }
       }
-      const uint32_t vrow = from + kStep * KS + c * VS + r * VCH;
-      auto values = [&](int hf, int key, uint32_t (&w)[VCH / 4]) {
-        if constexpr (VCH == 16) { const uint4 x = lds128(vrow + key * VS + hf * 128); w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; }
-        else { const uint2 x = lds64(vrow + key * VS); w[0] = x.x; w[1] = x.y; }
+      const uint32_t vrow = from + STEP * KS + c * VS + r * VCH;
+      auto values = [&](int hf, int key, uint32_t (&x)[VCH / 4]) {
+        if constexpr (VCH == 16) { const uint4 y = lds128(vrow + key * VS + hf * 128); x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; }
+        else { const uint2 y = lds64(vrow + key * VS); x[0] = y.x; x[1] = y.y; }
       };
       bool nan = false;
-      if (masked) {                                          // a NaN among values that some row does not see must not reach that row, whose weight for it is zero
-#pragma unroll
+      if (masked) {                                          // a NaN among values that some query does not see must not reach that query, whose weight for it is zero
+#pragma unroll 1
         for (int hf = 0; hf < HF; hf++)
+#pragma unroll 1
+          for (int k = 0; k < STEP / 4; k++) {
+            uint32_t x[VCH / 4];
+            values(hf, k * 4, x);
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            uint32_t w[VCH / 4];
-            values(hf, (k & 1) * 4 + (k >> 1) * 8, w);
-#pragma unroll
-            for (int u = 0; u < VCH / 4; u++) nan |= nan_bytes(w[u]) != 0;
+            for (int u = 0; u < VCH / 4; u++) nan |= nan_bytes(x[u]) != 0;
           }
         nan = __any_sync(0xffffffffu, nan);
       }
 #pragma unroll
-      for (int hf = 0; hf < HF; hf++) {
-        uint32_t w[4][VCH / 4];
-        values(hf, 0, w[0]); values(hf, 4, w[1]); values(hf, 8, w[2]); values(hf, 12, w[3]);
-        if (nan) {                                           // counts of the NaN that a row sees, entry by entry, then numbers alone
-#pragma unroll 1
-          for (int u = 0; u < VCH; u++) {
-            uint32_t b[2];
+      for (int y = 0; y < HV * HF; y++) {
+        const int hf = y % HF, sub = y / HF;                 // (constants once unrolled)
+        uint32_t x[4][VCH / 4];
+        values(hf, sub * 16, x[0]); values(hf, sub * 16 + 4, x[1]); values(hf, sub * 16 + 8, x[2]); values(hf, sub * 16 + 12, x[3]);
+        if (nan) {                                           // counts of the NaN that a query sees, two entries at a time, then numbers alone
+          uint32_t see[QT][2];
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-              uint32_t n0 = 0, n1 = 0;
+          for (int t = 0; t < QT; t++)
 #pragma unroll
-              for (int k = 0; k < VCH / 4; k++) if (k == u >> 2) { n0 = nan_bytes(w[2 * g][k]); n1 = nan_bytes(w[2 * g + 1][k]); }
-              b[g] = ((n0 >> (8 * (u & 3))) & 1 ? 0x3c00u : 0u) | ((n1 >> (8 * (u & 3))) & 1 ? 0x3c000000u : 0u);
-            }
+            for (int h = 0; h < 2; h++) see[t][h] = turned(((seen[t] >> (sub * 4 + 2 * h)) & 1 ? 0x3c00u : 0u) | ((seen[t] >> (sub * 4 + 2 * h + 1)) & 1 ? 0x3c000000u : 0u));
 #pragma unroll
-            for (int t = 0; t < MT; t++) {
-              uint32_t a[4];
+          for (int k = 0; k < VCH / 2; k++) {
+            uint32_t a[4];
 #pragma unroll
-              for (int g = 0; g < 2; g++)
+            for (int e = 0; e < 2; e++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) a[2 * g + h] = ((seen[t] >> (g * 4 + 2 * h)) & 1 ? 0x3c00u : 0u) | ((seen[t] >> (g * 4 + 2 * h + 1)) & 1 ? 0x3c000000u : 0u);
+              for (int h = 0; h < 2; h++) {
+                const int byte = 8 * ((2 * k + e) & 3);
+                a[2 * h + e] = ((nan_bytes(x[2 * h][(2 * k + e) / 4]) >> byte) & 1 ? 0x3c00u : 0u) | ((nan_bytes(x[2 * h + 1][(2 * k + e) / 4]) >> byte) & 1 ? 0x3c000000u : 0u);
+              }
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
               float d[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16(d, a, b[0], b[1]);
+              mma16(d, a, see[t][0], see[t][1]);
 #pragma unroll
-              for (int k = 0; k < VCH; k++)
-                if (k == u)
-#pragma unroll
-                  for (int e = 0; e < 4; e++) if (d[e] > 0.f) o[t][hf * VCH + k][e] = NAN;
+              for (int i = 0; i < 4; i++) if (d[i] > 0.f) o[t][hf * VCH / 2 + k][i] = NAN;
             }
           }
 #pragma unroll
           for (int k = 0; k < 4; k++)
 #pragma unroll
-            for (int u = 0; u < VCH / 4; u++) w[k][u] &= ~nan_bytes(w[k][u]);
+            for (int u = 0; u < VCH / 4; u++) x[k][u] &= ~nan_bytes(x[k][u]);
         }
 #pragma unroll
-        for (int u = 0; u < VCH / 4; u++) {
-          const uint32_t lo0 = __byte_perm(w[0][u], w[1][u], 0x5140), hi0 = __byte_perm(w[0][u], w[1][u], 0x7362);
-          const uint32_t lo1 = __byte_perm(w[2][u], w[3][u], 0x5140), hi1 = __byte_perm(w[2][u], w[3][u], 0x7362);
-          const uint32_t b[4][2] = {{two_halves(lo0), two_halves(lo1)}, {two_halves(lo0 >> 16), two_halves(lo1 >> 16)}, {two_halves(hi0), two_halves(hi1)}, {two_halves(hi0 >> 16), two_halves(hi1 >> 16)}};
+        for (int u = 0; u < VCH / 4; u++) {                  // four entries: two tiles, whose rows r and r + 8 are neighbouring entries
+          const uint32_t lo0 = __byte_perm(x[0][u], x[1][u], 0x5140), hi0 = __byte_perm(x[0][u], x[1][u], 0x7362);
+          const uint32_t lo1 = __byte_perm(x[2][u], x[3][u], 0x5140), hi1 = __byte_perm(x[2][u], x[3][u], 0x7362);
+          uint32_t a[2][4];
+          four_halves(lo0, a[0][0], a[0][1]);
+          four_halves(lo1, a[0][2], a[0][3]);
+          four_halves(hi0, a[1][0], a[1][1]);
+          four_halves(hi1, a[1][2], a[1][3]);
 #pragma unroll
-          for (int e = 0; e < 4; e++)
+          for (int k = 0; k < 2; k++)
 #pragma unroll
-            for (int t = 0; t < MT; t++) mma16(o[t][hf * VCH + u * 4 + e], pf[t], b[e][0], b[e][1]);
+            for (int t = 0; t < QT; t++) mma16(o[t][hf * VCH / 2 + u * 2 + k], a[k], w[t][sub][0], w[t][sub][1]);
         }
       }
     }
@@ -443,102 +513,99 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     if (++stage == NST) stage = 0;
     // where the piece ends: the warps' sums in one
     const bool whole_end = pl.unit + 1 == q.units;
-    if (whole_end || y + 1 == x1) {
+    if (whole_end || y + 1 == mine) {
 #pragma unroll
-      for (int t = 0; t < MT; t++)
+      for (int t = 0; t < QT; t++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 1);
-          l[t][h] += __shfl_xor_sync(0xffffffffu, l[t][h], 2);
-          if (c == 0) { row_m[warp * MT * 16 + t * 16 + r + 8 * h] = m[t][h]; row_l[warp * MT * 16 + t * 16 + r + 8 * h] = l[t][h]; }
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], x);
+          if (r == 0) { row_m[warp * QT * 8 + t * 8 + 2 * c + e] = m[t][e]; row_l[warp * QT * 8 + t * 8 + 2 * c + e] = l[t][e]; }
         }
       __syncthreads();
-      float top[MT][2], sum[MT][2];
+      float top[QT][2], sum[QT][2];
 #pragma unroll
-      for (int t = 0; t < MT; t++)
+      for (int t = 0; t < QT; t++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int row = t * 16 + r + 8 * h;
-          top[t][h] = row_m[row];
+        for (int e = 0; e < 2; e++) {
+          const int row = t * 8 + 2 * c + e;
+          top[t][e] = row_m[row];
 #pragma unroll
-          for (int w = 1; w < kWarps; w++) top[t][h] = fmaxf(top[t][h], row_m[w * MT * 16 + row]);
-          sum[t][h] = 0.f;
+          for (int w = 1; w < kWarps; w++) top[t][e] = fmaxf(top[t][e], row_m[w * QT * 8 + row]);
+          sum[t][e] = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; w++) sum[t][h] += row_l[w * MT * 16 + row] * exp2_fast(row_m[w * MT * 16 + row] - top[t][h]);
-          const float f = exp2_fast(m[t][h] - top[t][h]);
+          for (int w = 0; w < kWarps; w++) sum[t][e] += row_l[w * QT * 8 + row] * exp2_fast(row_m[w * QT * 8 + row] - top[t][e]);
+          const float f = exp2_fast(m[t][e] - top[t][e]);
 #pragma unroll
-          for (int k = 0; k < NT; k++) { o[t][k][2 * h] *= f; o[t][k][2 * h + 1] *= f; }
+          for (int k = 0; k < NO; k++) { o[t][k][e] *= f; o[t][k][2 + e] *= f; }
         }
-      float* mine = turn + (warp & 1) * MT * NT * 128 + lane;
+      float* mine_at = turn + (warp & 1) * QT * NO * 128 + lane;
       auto put = [&]() {
 #pragma unroll
-        for (int t = 0; t < MT; t++)
+        for (int t = 0; t < QT; t++)
 #pragma unroll
-          for (int k = 0; k < NT; k++)
+          for (int k = 0; k < NO; k++)
 #pragma unroll
-            for (int u = 0; u < 4; u++) mine[((t * NT + k) * 4 + u) * 32] = o[t][k][u];
+            for (int u = 0; u < 4; u++) mine_at[((t * NO + k) * 4 + u) * 32] = o[t][k][u];
       };
-      auto add = [&](const float* from) {
+      auto add = [&](const float* other) {
 #pragma unroll
-        for (int t = 0; t < MT; t++)
+        for (int t = 0; t < QT; t++)
 #pragma unroll
-          for (int k = 0; k < NT; k++)
+          for (int k = 0; k < NO; k++)
 #pragma unroll
-            for (int u = 0; u < 4; u++) o[t][k][u] += from[((t * NT + k) * 4 + u) * 32];
+            for (int u = 0; u < 4; u++) o[t][k][u] += other[((t * NO + k) * 4 + u) * 32];
       };
       if (warp >= 2) put();
       __syncthreads();
-      if (warp < 2) add(mine);
+      if (warp < 2) add(mine_at);
       if (warp == 1) put();
       __syncthreads();
       if (warp == 0) {
-        add(turn + MT * NT * 128 + lane);
+        add(turn + QT * NO * 128 + lane);
         if (begun == 0 && whole_end) {
 #pragma unroll
-          for (int t = 0; t < MT; t++)
+          for (int t = 0; t < QT; t++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const int row = row0 + t * 16 + r + 8 * h;
-              const float inv = sum[t][h] == 0.f ? 0.f : 1.f / sum[t][h];        // (a row that sees nothing: zeros)
+            for (int e = 0; e < 2; e++) {
+              const float inv = sum[t][e] == 0.f ? 0.f : 1.f / sum[t][e];        // (a query that sees nothing: zeros)
 #pragma unroll
-              for (int hf = 0; hf < HF; hf++)
+              for (int hf = 0; hf < HF; hf++) {
+                float x[16];
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                  float x[16];
-#pragma unroll
-                  for (int k = 0; k < VCH; k++) x[k] = o[t][hf * VCH + k][2 * h + e];
-                  Out::store(P, q, pl.b, head, row, hf * 128 + (2 * c + e) * VCH, VCH, x, inv);
-                }
+                for (int k = 0; k < VCH; k++) x[k] = o[t][hf * VCH / 2 + k / 2][2 * (k & 1) + e];
+                Out::store(P, q, pl.b, head, row0 + t * 8 + 2 * c + e, hf * 128 + r * VCH, VCH, x, inv);
+              }
             }
-        } else {                                             // a piece: [accumulator][lane], then maxima and sums of the rows
-          float* to = P.part + (size_t)(2 * blockIdx.x + (y + 1 - x0 == pl.unit - begun + 1 ? 0 : 1)) * (MT * (NT * 128 + 32));
+        } else {                                             // a piece: [accumulator][lane], then maxima and sums of the queries
+          float* to = P.part + (size_t)(2 * blockIdx.x + (y == pl.unit - begun ? 0 : 1)) * (QT * (NO * 128 + 16));
 #pragma unroll
-          for (int t = 0; t < MT; t++) {
+          for (int t = 0; t < QT; t++) {
 #pragma unroll
-            for (int k = 0; k < NT; k++)
+            for (int k = 0; k < NO; k++)
 #pragma unroll
-              for (int u = 0; u < 4; u++) to[((t * NT + k) * 4 + u) * 32 + lane] = o[t][k][u];
-            if (c == 0)
+              for (int u = 0; u < 4; u++) to[((t * NO + k) * 4 + u) * 32 + lane] = o[t][k][u];
+            if (r == 0)
 #pragma unroll
-              for (int h = 0; h < 2; h++) {
-                to[MT * NT * 128 + t * 16 + r + 8 * h] = top[t][h];
-                to[MT * NT * 128 + MT * 16 + t * 16 + r + 8 * h] = sum[t][h];
+              for (int e = 0; e < 2; e++) {
+                to[QT * NO * 128 + t * 8 + 2 * c + e] = top[t][e];
+                to[QT * NO * 128 + QT * 8 + t * 8 + 2 * c + e] = sum[t][e];
               }
           }
         }
       }
       fresh = true;
     }
-    pl.next(P, per);
+    pl.next(P);
     if (fresh) begun = pl.unit;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Joins the pieces of a (sequence, head, row tile) that several CTAs of attend_tokens had: a warp has eight entries of every lane's row
-template <int DV, int MT>
-__global__ void __launch_bounds__(MT * DV / 16 * 32) join(const Attn P, int ctas) {
-  constexpr int NT = DV / 8, VCH = DV >= 128 ? 16 : 8;
+// Joins the pieces of a (sequence, head, query tiles) that several CTAs of attend_tokens had: a warp has eight entries of one of every lane's two queries
+template <int DV, int QT>
+__global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
+  constexpr int NO = DV / 16, VCH = DV >= 128 ? 16 : 8;
   grid_wait();
   const int b = blockIdx.y, hr = blockIdx.x, per = gridDim.x;
   const long long total = P.ends[P.S.batch] * per, units = P.ends[b + 1] - P.ends[b];
@@ -548,10 +615,10 @@ __global__ void __launch_bounds__(MT * DV / 16 * 32) join(const Attn P, int ctas
   if (i0 == i1) return;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   int w = threadIdx.x >> 5;
-  const int e = w & 1, h = (w >> 1) & 1;
-  w >>= 2;
-  const int k0 = (w % (NT / 8)) * 8, t = w / (NT / 8), row = t * 16 + r + 8 * h;
-  float x[8], m = -1e30f, l = 0.f;
+  const int e = w & 1;
+  w >>= 1;
+  const int k0 = (w % (DV / 64)) * 8, t = w / (DV / 64), row = t * 8 + 2 * c + e;   // k0: of a lane's DV / 8 entries
+  float x[16], m = -1e30f, l = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; k++) x[k] = 0.f;
   for (int i = i0; i <= i1; i += 4) {
@@ -559,11 +626,11 @@ __global__ void __launch_bounds__(MT * DV / 16 * 32) join(const Attn P, int ctas
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       if (i + u > i1) { pm[u] = -INFINITY; continue; }
-      const float* from = P.part + (size_t)(2 * (i + u) + ((i + u) * total / N >= u0 ? 0 : 1)) * (MT * (NT * 128 + 32));
-      pm[u] = from[MT * NT * 128 + row];
-      pl[u] = from[MT * NT * 128 + MT * 16 + row];
+      const float* from = P.part + (size_t)(2 * (i + u) + ((i + u) * total / N >= u0 ? 0 : 1)) * (QT * (NO * 128 + 16));
+      pm[u] = from[QT * NO * 128 + row];
+      pl[u] = from[QT * NO * 128 + QT * 8 + row];
 #pragma unroll
-      for (int k = 0; k < 8; k++) px[u][k] = from[((t * NT + k0 + k) * 4 + 2 * h + e) * 32 + lane];
+      for (int k = 0; k < 8; k++) px[u][k] = from[((t * NO + (k0 + k) / 2) * 4 + 2 * (k & 1) + e) * 32 + lane];
     }
     const float to = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), f = exp2_fast(m - to);
     m = to;
@@ -579,12 +646,8 @@ __global__ void __launch_bounds__(MT * DV / 16 * 32) join(const Attn P, int ctas
       for (int k = 0; k < 8; k++) x[k] = fmaf(px[u][k], g, x[k]);
     }
   }
-  const int head = hr / P.row_tiles, row0 = (hr - head * P.row_tiles) * MT * 16;
-  const int hf = k0 / VCH;
-  float y[16];
-#pragma unroll
-  for (int k = 0; k < 8; k++) y[k] = x[k];
-  Out::store(P, sequence(P, b), b, head, row0 + row, hf * 128 + (2 * c + e) * VCH + k0 % VCH, 8, y, l == 0.f ? 0.f : 1.f / l);
+  const int head = hr / P.row_tiles, row0 = (hr - head * P.row_tiles) * QT * 8;
+  Out::store(P, sequence<step_of(QT)>(P, b), b, head, row0 + row, k0 / VCH * 128 + r * VCH + k0 % VCH, 8, x, l == 0.f ? 0.f : 1.f / l);
 }
 
 }  // namespace kv8

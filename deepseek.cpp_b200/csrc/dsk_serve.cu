@@ -148,23 +148,29 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, Layout* L) {
   const long long rows = (long long)(heads / c->kv_heads) * s->rows;
   if (rows > (1 << 24)) return fail(-4, "%lld query rows of a key head: at most 2^24", rows);
   for (L->shape = 0; c->dim_k > kShapes[L->shape][0] || c->dim_v > kShapes[L->shape][1];) L->shape++;
-  L->tiles = rows > 16 && L->shape < 3 ? 2 : 1;
-  L->row_tiles = (int)((rows + 16 * L->tiles - 1) / (16 * L->tiles));
+  L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
+  L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
   const int sms = multiprocessors(c->device);
   if (!sms) return fail(-2, "device %d: no attributes", c->device);
-  const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * (((long long)s->table_blocks * c->block + kv8::kUnit - 1) / kv8::kUnit + 1);
+  const int unit = kv8::kWarps * kv8::step_of(L->tiles);
+  const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * (((long long)s->table_blocks * c->block + unit - 1) / unit + 1);
   L->ctas = (int)std::min<long long>(2 * sms, std::max<long long>(1, units));
   L->ends = ((size_t)(s->batch + 1) * sizeof(long long) + 15) / 16 * 16;
-  L->bytes = L->ends + (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 8 * 128 + 32) * sizeof(float);
+  L->bytes = L->ends + (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 16 * 128 + 16) * sizeof(float);
   return 0;
 }
-template <int DK, int DV, int MT> int attend_as(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
-  const int smem = kv8::attn_smem<DK, DV, MT>() + 8 + 8 * P.S.batch;
-  CK((allow<kv8::attend_tokens<DK, DV, MT>>(device, kv8::attn_smem<DK, DV, MT>() + 8 + 8 * kv8::kMaxBatch)));
-  kv8::attend_tokens<DK, DV, MT><<<L.ctas, kv8::kThreads, smem, stream>>>(P);
+template <int DK, int DV, int QT> int attend_as(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
+  const int smem = kv8::attn_smem<DK, DV, QT>() + 8 + 8 * P.S.batch;
+  CK((allow<kv8::attend_tokens<DK, DV, QT>>(device, kv8::attn_smem<DK, DV, QT>() + 8 + 8 * kv8::kMaxBatch)));
+  kv8::attend_tokens<DK, DV, QT><<<L.ctas, kv8::kThreads, smem, stream>>>(P);
   CK(cudaGetLastError());
-  CK(launch_behind(kv8::join<DV, MT>, dim3(P.C.heads * P.row_tiles, P.S.batch), dim3(MT * DV / 16 * 32), 0, stream, 1, P, L.ctas));
+  CK(launch_behind(kv8::join<DV, QT>, dim3(P.C.heads * P.row_tiles, P.S.batch), dim3(QT * DV), 0, stream, 1, P, L.ctas));
   return 0;
+}
+template <int DK, int DV> int attend_tiles(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
+  if (L.tiles == 1) return attend_as<DK, DV, 1>(P, L, device, stream);
+  if constexpr (DV < 256) if (L.tiles == 4) return attend_as<DK, DV, 4>(P, L, device, stream);
+  return attend_as<DK, DV, 2>(P, L, device, stream);
 }
 }  // namespace
 
@@ -220,19 +226,16 @@ extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
   P.C = cache_of(c); P.S = rows_of(s);
   P.q = q->data; P.out = out->data; P.pq = pitch_of(q); P.po = pitch_of(out);
   P.heads = heads; P.group = heads / c->kv_heads; P.row_tiles = L.row_tiles; P.bf16 = dt == DSK_DT_BF16; P.wide_q = wide(q); P.wide_o = wide(out);
-  P.window = window; P.keep = keep_first;
+  P.window = window; P.keep = keep_first; P.shift = c->block == 16 ? 4 : c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
   P.scale = scale * 1.44269504088896340736f;
   P.ends = static_cast<long long*>(workspace);
   P.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.ends);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (L.shape * 2 + L.tiles - 1) {
-    case 0: return attend_as<64, 64, 1>(P, L, c->device, st);
-    case 1: return attend_as<64, 64, 2>(P, L, c->device, st);
-    case 2: return attend_as<128, 128, 1>(P, L, c->device, st);
-    case 3: return attend_as<128, 128, 2>(P, L, c->device, st);
-    case 4: return attend_as<192, 128, 1>(P, L, c->device, st);
-    case 5: return attend_as<192, 128, 2>(P, L, c->device, st);
-    default: return attend_as<256, 256, 1>(P, L, c->device, st);
+  switch (L.shape) {
+    case 0: return attend_tiles<64, 64>(P, L, c->device, st);
+    case 1: return attend_tiles<128, 128>(P, L, c->device, st);
+    case 2: return attend_tiles<192, 128>(P, L, c->device, st);
+    default: return attend_tiles<256, 256>(P, L, c->device, st);
   }
 }
 

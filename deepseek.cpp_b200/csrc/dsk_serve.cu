@@ -14,6 +14,7 @@
 #include "dsk_host.h"
 #include "dsk_kv8.cuh"
 #include "dsk_kv8_attn.cuh"
+#include "dsk_kv8_tc5.cuh"
 #include "dsk_verify.cuh"
 
 using namespace dsk;
@@ -140,20 +141,31 @@ template <typename T> int read_as(const dsk_kv8* c, const dsk_kv8_rows* s, const
 }
 
 // How an attention call is laid out
-struct Layout { int shape, tiles, row_tiles, ctas; size_t ends, bytes; };
+struct Layout { int shape, tiles, row_tiles, ctas, shares; size_t ends, bytes; };   // shares > 0: attend_rows
+constexpr int kPortionRows = 32;                             // query rows of a key head from which on attend_rows has them
 constexpr int kShapes[4][2] = {{64, 64}, {128, 128}, {192, 128}, {256, 256}};
 int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, Layout* L) {
   if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
   if (s->batch > kv8::kMaxBatch) return fail(-4, "attention over %d sequences: at most %d a call", s->batch, kv8::kMaxBatch);
   const long long rows = (long long)(heads / c->kv_heads) * s->rows;
-  if (rows > (1 << 24)) return fail(-4, "%lld query rows of a key head: at most 2^24", rows);
+  if (rows > (1 << 23)) return fail(-4, "%lld query rows of a key head: at most 2^23", rows);
   for (L->shape = 0; c->dim_k > kShapes[L->shape][0] || c->dim_v > kShapes[L->shape][1];) L->shape++;
-  L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
-  L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
   const int sms = multiprocessors(c->device);
   if (!sms) return fail(-2, "device %d: no attributes", c->device);
+  const long long keys = (long long)s->table_blocks * c->block;
+  L->shares = 0;
+  if (rows > kPortionRows && L->shape < 3) {
+    L->row_tiles = (int)((rows + kv8::kRows - 1) / kv8::kRows);
+    const long long tiles = (long long)s->batch * c->kv_heads * L->row_tiles;
+    L->shares = (int)std::max<long long>(1, std::min<long long>(sms / tiles, (keys + kv8::kTile - 1) / kv8::kTile));   // where the row tiles leave SMs idle, their keys are shared out
+    L->ends = 0;
+    L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * kv8::kRows * (kShapes[L->shape][1] + 2) * sizeof(float) : 16;
+    return 0;
+  }
+  L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
+  L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
   const int unit = kv8::kWarps * kv8::step_of(L->tiles);
-  const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * (((long long)s->table_blocks * c->block + unit - 1) / unit + 1);
+  const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * ((keys + unit - 1) / unit + 1);
   L->ctas = (int)std::min<long long>(2 * sms, std::max<long long>(1, units));
   L->ends = ((size_t)(s->batch + 1) * sizeof(long long) + 15) / 16 * 16;
   L->bytes = L->ends + (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 16 * 128 + 16) * sizeof(float);
@@ -167,7 +179,16 @@ template <int DK, int DV, int QT> int attend_as(const kv8::Attn& P, const Layout
   CK(launch_behind(kv8::join<DV, QT>, dim3(P.C.heads * P.row_tiles, P.S.batch), dim3(QT * DV), 0, stream, 1, P, L.ctas));
   return 0;
 }
+template <int DK, int DV> int attend_portion(const kv8::Attn& A, const Layout& L, int device, cudaStream_t stream) {
+  const kv8::Portion P{A, L.shares};
+  CK((allow<kv8::attend_rows<DK, DV>>(device, kv8::rows_smem<DK, DV>())));
+  kv8::attend_rows<DK, DV><<<dim3(A.C.heads * L.shares, L.row_tiles, A.S.batch), kv8::kRowThreads, kv8::rows_smem<DK, DV>(), stream>>>(P);
+  CK(cudaGetLastError());
+  if (L.shares > 1) CK(launch_behind(kv8::join_rows<DV>, dim3(A.C.heads * (DV / 16), L.row_tiles, A.S.batch), dim3(kv8::kRows), 0, stream, 1, P));
+  return 0;
+}
 template <int DK, int DV> int attend_tiles(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
+  if constexpr (DV < 256) if (L.shares) return attend_portion<DK, DV>(P, L, device, stream);
   if (L.tiles == 1) return attend_as<DK, DV, 1>(P, L, device, stream);
   if constexpr (DV < 256) if (L.tiles == 4) return attend_as<DK, DV, 4>(P, L, device, stream);
   return attend_as<DK, DV, 2>(P, L, device, stream);

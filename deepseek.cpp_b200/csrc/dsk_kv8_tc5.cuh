@@ -1,8 +1,9 @@
 // dsk_kv8_tc5.cuh — softmax attention of portions (many query rows to a key head) over the 8-bit cache on the 5th-generation tensor cores, keys up to 192 entries, values up to 128.
 //
 // A CTA has 256 query rows of a key head (its query heads' rows one behind the other, so that all of them share the keys), two tiles of 128, and walks the keys that they see in tiles
-// of 128.  Roles: four warps bring codes from the cache, turn them into fp16 (exact) and store them as swizzled operands, so that the cache crosses HBM and L2 as bytes; one thread
-// issues the products, scores into TMEM, weights from TMEM; two groups of four warps have the softmax, a thread to a row, each for its own tile, so that one tile's products run under the
+// of 128.  Roles: seven warps bring codes from the cache, four the keys' and three the values', turn them into fp16 (exact) and store them as swizzled operands, so that the cache
+// crosses HBM and L2 as bytes; one thread
+// issues the products, scores into TMEM, weights from TMEM; two groups of four warps have the softmax, a thread to a row, each group for its own tile, so that one tile's products run under the
 // other one's softmax.  Scales and weights as in dsk_kv8_attn.cuh: key scales on the scores, value scales inside the exponent, fp16 weights of at most 2^kSlack.
 // The results stay in TMEM; they are scaled again only where a row's maximum has moved by more than 2^kSlack, by the thread that has the row.  Weights lie where the scores were:
 // a tile's next scores wait for the product that reads its weights.
@@ -28,15 +29,22 @@ template <int DK, int DV> __host__ __device__ constexpr int rows_smem() {
   return 1024 + kRows * DK * 2 + k_stages<DK, DV>() * kTile * DK * 2 + v_stages<DK, DV>() * kTile * DV * 2 + kSlots * 3 * 8 * 4 + 256;
 }
 
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Cache& C) {   // bounded; every lane of a warp gets the same answer
-  if (hy::tc_poll(bar, parity)) return true;
+// Bounded.  A poll sleeps until the phase is through, up to the time that it is given: polls that return at once take the issue slots of the warps that work (13300 instead of 8000
+// instructions to a tile of keys).
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* status) {
   const long long from = clock64();
   do {
-    if (hy::tc_poll(bar, parity)) return true;
+    if (poll(bar, parity)) return true;
   } while (clock64() - from < hy::kTcWaitCycles);
-  note(C, ST_WAIT);
+  if (status) atomicOr(status, ST_WAIT);
   return false;
 }
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Cache& C) { return poll(bar, parity) || wait_long(bar, parity, C.status); }
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const Cache& C) { return __all_sync(0xffffffffu, wait_bar(bar, parity, C)); }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -62,6 +70,37 @@ __device__ __forceinline__ void tmem_read16(uint32_t addr, uint32_t (&r)[16]) { 
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
 }
+// two fp32 operations at a time
+__device__ __forceinline__ uint64_t both(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void fma2(uint32_t x0, uint32_t x1, uint64_t f, uint64_t a, float& y0, float& y1) {
+  asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%2, %3};\n\tfma.rn.f32x2 x, x, %4, %5;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(y0), "=f"(y1) : "r"(x0), "r"(x1), "l"(f), "l"(a));
+}
+__device__ __forceinline__ void add2(uint64_t& s, float y0, float y1) {
+  asm("{\n\t.reg .b64 y;\n\tmov.b64 y, {%1, %2};\n\tadd.rn.f32x2 %0, %0, y;\n\t}" : "+l"(s) : "f"(y0), "f"(y1));
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return r;
+}
+// Products and commits of one lane of a warp whose lanes all run the same code: descriptors then stay in uniform registers, where a branch to that lane would have them copied there
+// for every product
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead) {   // A in TMEM
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t lead) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
+}
+__device__ __forceinline__ uint32_t lower_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -96,6 +135,120 @@ __device__ __forceinline__ bool sees_all(const Attn& A, const Walk& w, int i0, i
   return key0 + kTile - 1 <= w.first + i0 && (A.window <= 0 || w.first + i1 - key0 < A.window || key0 + kTile <= A.keep);
 }
 
+// Codes to operands, keys or values of all tiles, by WARPS warps: a thread has the c-th 16 entries of every 64 of rows r0, r0 + 8 WARPS, ..  (G of them).  A warp's loads are 64 bytes
+// of eight rows, its stores meet no bank twice (neighbouring rows are swizzled to even and odd pieces), and places in shared memory differ by constants.  A tile's codes are
+// loaded a tile ahead, with its scales, and the numbers of its blocks two tiles ahead.
+template <int D, int G, int WARPS>
+__device__ __forceinline__ void bring(const Attn& A, const Walk& w, int b, int h, int which, int warp, int lane, uint32_t ring, uint32_t stage_bytes, int stages, uint32_t full, uint32_t empty,
+                                      uint32_t scaled, float* scales, int* nan_seen) {
+  constexpr int NB = D / 64;
+  const int n = w.end - w.begin, dim = A.C.dim[which], r0 = warp * 8 + (lane >> 2), c0 = lane & 3;
+  const uint32_t head = A.C.block * dim, block = A.C.heads * head, place = r0 * 128 + (((c0 * 2) ^ (r0 & 7)) << 4);
+  const unsigned char* code = A.C.code[which];
+  const int* table = A.S.table + b * A.S.table_pitch;
+  const bool scaling = which == 0 && warp == 0;
+  auto look = [&](int i) {                                   // lane g < 8: block of keys 16 g .. of a tile (-1: behind the last key, or outside the cache)
+    int p = -1;
+    if (i < n && lane < 8) {
+      const int key = key_of(w, w.begin + i) + 16 * lane;
+      if (key < w.len) p = __ldg(table + (key >> A.shift));
+    }
+    return p;
+  };
+  auto checked = [&](int p, int i) {
+    const bool bad = i < n && lane < 8 && (unsigned)p >= (unsigned)A.C.n_blocks;
+    if (bad && scaling && key_of(w, w.begin + i) + 16 * lane < w.len) note(A.C, ST_PAGE);
+    return bad ? -1 : p;
+  };
+  float k_scale = 0.f, v_scale = 0.f;
+  auto look_scales = [&](int p) {
+    if (scaling && p >= 0) {
+      const uint64_t slot = (uint64_t)(uint32_t)p * (uint32_t)A.C.heads + h;
+      k_scale = __ldg(A.C.scale[0] + slot);
+      v_scale = __ldg(A.C.scale[1] + slot);
+    }
+  };
+  uint4 x[G * NB];
+  const bool exact = dim == D;
+  auto load = [&](int i, int page) {
+    const int key0 = key_of(w, w.begin + i);
+    if (exact && key0 + kTile <= w.len && __all_sync(0xffffffffu, lane >= 8 || page >= 0)) {   // a whole tile
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int at = min(g * WARPS * 8 + r0, kTile - 1);   // (G x 8 x WARPS rows may be more than a tile has)
+        const uint32_t p = __shfl_sync(0xffffffffu, page, at >> 4);
+        const unsigned char* from = code + ((uint64_t)p * block + (h * head + ((key0 + at) & (A.C.block - 1)) * D + c0 * 16));
+#pragma unroll
+        for (int k = 0; k < NB; k++) x[g * NB + k] = __ldg(reinterpret_cast<const uint4*>(from + k * 64));
+      }
+      return;
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int at = g * WARPS * 8 + r0, row = key0 + at, p = __shfl_sync(0xffffffffu, page, at >> 4);
+      const bool there = at < kTile && p >= 0 && row < w.len;
+      const unsigned char* from = code + ((uint64_t)(uint32_t)max(p, 0) * block + (h * head + (row & (A.C.block - 1)) * dim + c0 * 16));
+#pragma unroll
+      for (int k = 0; k < NB; k++) {
+        x[g * NB + k] = make_uint4(0, 0, 0, 0);
+        if (there && k * 64 + c0 * 16 < dim) x[g * NB + k] = __ldg(reinterpret_cast<const uint4*>(from + k * 64));
+      }
+    }
+  };
+  int stage = 0, page = checked(look(0), 0);
+  uint32_t turn = 1;
+  if (n > 0) load(0, page);
+  look_scales(page);
+  int next = look(1);
+  for (int i = 0; i < n; i++) {
+    if (!wait_warp(empty + 8 * stage, turn, A.C)) break;
+    if (scaling) {
+      if (lane < 8) {
+        float* to = scales + (i % kSlots) * 24 + lane;
+        const int e = (int)(__float_as_uint(v_scale) >> 23) - 127;
+        to[0] = page >= 0 ? k_scale : 0.f;
+        to[8] = page >= 0 ? (float)e : 0.f;
+        to[16] = page >= 0 ? pow2(-e) : 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) hy::tc_arrive(scaled + 8 * (i % kSlots));
+    }
+    if (which == 1 && !sees_all(A, w, w.i0, w.i1, key_of(w, w.begin + i))) {   // NaN become zeros
+      uint32_t found = 0;
+#pragma unroll
+      for (int j = 0; j < G * NB; j++) {
+        uint32_t* c = reinterpret_cast<uint32_t*>(&x[j]);
+#pragma unroll
+        for (int u = 0; u < 4; u++) { const uint32_t z = nan_bytes(c[u]); found |= z; c[u] &= ~z; }
+      }
+      if (found) *nan_seen = 1;
+    }
+    const uint32_t to = ring + stage * stage_bytes + place, to_other = ring + stage * stage_bytes + (place ^ 16);
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int k = 0; k < NB; k++) {
+        const uint4 c = x[g * NB + k];
+        uint32_t f[8];
+        four_halves(c.x, f[0], f[1]);
+        four_halves(c.y, f[2], f[3]);
+        four_halves(c.z, f[4], f[5]);
+        four_halves(c.w, f[6], f[7]);
+        const uint32_t at = k * (kTile * 128) + g * WARPS * 8 * 128;
+        if (kTile % (WARPS * 8) == 0 || g * WARPS * 8 + r0 < kTile) { sts128(to + at, f[0], f[1], f[2], f[3]); sts128(to_other + at, f[4], f[5], f[6], f[7]); }
+      }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) hy::tc_arrive(full + 8 * stage);
+    if (++stage == stages) { stage = 0; turn ^= 1; }
+    page = checked(next, i + 1);
+    if (i + 1 < n) load(i + 1, page);
+    look_scales(page);
+    next = look(i + 2);
+  }
+  __syncwarp();
+}
+
 template <int DK, int DV>
 __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_constant__ Portion P) {
   constexpr int KST = k_stages<DK, DV>(), VST = v_stages<DK, DV>(), KB = kTile * DK * 2, VB = kTile * DV * 2;
@@ -108,7 +261,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   const uint32_t qs = base, ks = qs + kRows * DK * 2, vs = ks + KST * KB, cs = vs + VST * VB, bars = cs + kSlots * 3 * 8 * 4;
   float* scales = reinterpret_cast<float*>(gbase + (cs - base));          // [slot][key scale | exponent of the value scale | its reciprocal, zero: not there][16 keys]
   const uint32_t kfull = bars, kempty = bars + 24, vfull = bars + 48, vempty = bars + 72, sfull = bars + 96, pfull = bars + 112, pvdone = bars + 128, cfull = bars + 144, cdone = bars + 176, flushed = bars + 184;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int h = blockIdx.x / P.shares, share = blockIdx.x - h * P.shares, b = blockIdx.z, row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kRows;   // late rows, which see most, first
   const Walk w = walk_of(P, b, row0, share);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
@@ -118,10 +271,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   if (w.i0 >= w.count) return;                               // (the whole CTA: none of its rows exists)
   const int n = w.end - w.begin;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 3; i++) { mbar_init(kfull + 8 * i, 4); mbar_init(kempty + 8 * i, 1); mbar_init(vfull + 8 * i, 4); mbar_init(vempty + 8 * i, 1); }
+    for (int i = 0; i < 3; i++) { mbar_init(kfull + 8 * i, 4); mbar_init(kempty + 8 * i, 1); mbar_init(vfull + 8 * i, 3); mbar_init(vempty + 8 * i, 1); }
     for (int i = 0; i < 2; i++) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); }
     for (int i = 0; i < kSlots; i++) mbar_init(cfull + 8 * i, 1);
-    mbar_init(cdone, 4);
+    mbar_init(cdone, 3);
     mbar_init(flushed, 1);
     nan_seen = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -131,8 +284,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   const int dk = A.C.dim[0], dv = A.C.dim[1];
-  if (dk < DK || dv < DV)                                    // entries behind the last one stay zero
-    for (int i = threadIdx.x; i < (KST * KB + VST * VB) / 16; i += kRowThreads) sts128(ks + i * 16, 0, 0, 0, 0);
   // query rows as fp16, two threads to a row, each by its own power of two (dsk_kv8_attn.cuh)
   float row_scale = 0.f;                                     // of the row that this thread has in the softmax
   {
@@ -171,14 +322,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       const int tile = row >> 7, rr = row & 127;             // [tile][64 entries][row], 16-byte pieces swizzled
       sts128(qs + tile * (kTile * DK * 2) + (d >> 6) * (kTile * 128) + rr * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4), x[0], x[1], x[2], x[3]);
     }
-    // thread t of the softmax has row t: its factor comes from threads 2 t, 2 t + 1 (through the scales' memory, which nobody uses yet)
+    // rows' factors on their way to the softmax's threads, through memory that nobody uses yet
     __syncthreads();
     float* f = reinterpret_cast<float*>(gbase + (vs - base));               // (the first values come behind the barrier below)
     if (half == 0) f[row] = pow2(e) * fabsf(A.scale);
     __syncthreads();
-    if (threadIdx.x < kRows) row_scale = f[threadIdx.x];
+    if (warp < 8) row_scale = f[threadIdx.x];
     __syncthreads();
-    if (dv < DV && half == 0) f[row] = 0.f;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -187,7 +337,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [2][128], results [2][128]
 
   if (warp >= 12) {
-    if (warp == 12 && hy::tc_elect()) {
+    if (warp == 12) {
+      const uint32_t lead = hy::tc_elect();
       const uint32_t idesc = (1u << 4) | ((uint32_t)(kTile / 16) << 24);       // fp32 sums, fp16 x fp16, 128 rows
       const uint32_t sdesc = idesc | ((uint32_t)(kTile / 8) << 17), pdesc = idesc | (1u << 16) | ((uint32_t)(DV / 8) << 17);
       auto score = [&](int t, int stage) {
@@ -195,146 +346,59 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
 #pragma unroll
         for (int g = 0; g < DK / 64; g++)
 #pragma unroll
-          for (int u = 0; u < 4; u++) hy::tc_mma(tmem + t * 128, a + g * (kTile * 128 >> 4) + 2 * u, k + g * (kTile * 128 >> 4) + 2 * u, sdesc, g > 0 || u > 0);
-        hy::tc_commit(sfull + 8 * t);
+          for (int u = 0; u < 4; u++) mma_ss(tmem + t * 128, a + g * (kTile * 128 >> 4) + 2 * u, k + g * (kTile * 128 >> 4) + 2 * u, sdesc, g > 0 || u > 0, lead);
+        commit(sfull + 8 * t, lead);
       };
-      bool alive = n > 0 && wait_bar(kfull, 0, A.C);
+      bool alive = n > 0 && wait_warp(kfull, 0, A.C);
       if (alive) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         score(0, 0);
         score(1, 0);
-        hy::tc_commit(kempty);
+        commit(kempty, lead);
       }
       int kst = 0, vst = 0;
       uint32_t kturn = 0, vturn = 0;                         // the stage that was read last, parity of its tile
       for (int i = 0; i < n && alive; i++) {
-        alive = wait_bar(vfull + 8 * vst, vturn, A.C);
+        alive = wait_warp(vfull + 8 * vst, vturn, A.C);
         if (!alive) break;
         const uint64_t v = value_desc(vs + vst * VB);
         const bool more = i + 1 < n;
         if (more && ++kst == KST) { kst = 0; kturn ^= 1; }
-        for (int t = 0; t < 2 && alive; t++) {
-          alive = wait_bar(pfull + 8 * t, i & 1, A.C);
-          if (!alive) break;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          if (!alive) continue;
+          alive = wait_warp(pfull + 8 * t, i & 1, A.C);
+          if (!alive) continue;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-          for (int u = 0; u < kTile / 16; u++) hy::tc_mma_ta(o_at + t * 128, tmem + t * 128 + (u >> 2) * 64 + (u & 3) * 8, v + u * 128, pdesc, i > 0 || u > 0);
-          hy::tc_commit(pvdone + 8 * t);
-          if (t == 1) hy::tc_commit(vempty + 8 * vst);
+          for (int u = 0; u < kTile / 16; u++) mma_ts(o_at + t * 128, tmem + t * 128 + (u >> 2) * 64 + (u & 3) * 8, v + u * 128, pdesc, i > 0 || u > 0, lead);
+          commit(pvdone + 8 * t, lead);
+          if (t == 1) commit(vempty + 8 * vst, lead);
           if (!more) continue;
-          if (t == 0) { alive = wait_bar(kfull + 8 * kst, kturn, A.C); if (!alive) break; }
-          alive = wait_bar(pvdone + 8 * t, i & 1, A.C);      // the weights are read: their columns may have the next scores
-          if (!alive) break;
+          if (t == 0) { alive = wait_warp(kfull + 8 * kst, kturn, A.C); if (!alive) continue; }
+          alive = wait_warp(pvdone + 8 * t, i & 1, A.C);     // the weights are read: their columns may have the next scores
+          if (!alive) continue;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           score(t, kst);
-          if (t == 1) hy::tc_commit(kempty + 8 * kst);
+          if (t == 1) commit(kempty + 8 * kst, lead);
         }
         if (++vst == VST) { vst = 0; vturn ^= 1; }
       }
-      hy::tc_commit(flushed);                                // no product is under way when TMEM is given back
-      wait_bar(flushed, 0, A.C);
+      commit(flushed, lead);                                 // no product is under way when TMEM is given back
+      wait_warp(flushed, 0, A.C);
     }
     __syncwarp();
+    if (warp > 12) {
+      bring<DV, (kTile + 23) / 24, 3>(A, w, b, h, 1, warp - 13, lane, vs, VB, VST, vfull, vempty, 0, nullptr, &nan_seen);
+      if (lane == 0) hy::tc_arrive(cdone);
+    }
   } else if (warp >= 8) {
-    // codes to operands: 16-byte pieces tid, tid + 128, .. of a tile's rows, keys and values in turn, the next piece's load under way
-    const int tid = threadIdx.x - 256;
-    const uint32_t head_k = A.C.block * dk, head_v = A.C.block * dv, block_k = A.C.heads * head_k, block_v = A.C.heads * head_v;
-    int page = 0, next_page = -1;                            // lane g < 8: block of keys 16 g .. of the tile
-    auto look = [&](int i) {                                 // (-1: behind the last key)
-      int p = -1;
-      if (i < n && lane < 8) {
-        const int key = key_of(w, w.begin + i) + 16 * lane;
-        if (key < w.len) { p = __ldg(A.S.table + b * A.S.table_pitch + (key >> A.shift)); if ((unsigned)p >= (unsigned)A.C.n_blocks) { if (tid < 32) note(A.C, ST_PAGE); p = -1; } }
-      }
-      return p;
-    };
-    uint4 kx[DK / 16], vx[DV / 16];
-    auto load = [&](auto& x, int per, const unsigned char* code, uint32_t head, uint32_t block, int dim, int key0) {
-      int row = tid / per, col = tid - row * per;
-      const int dr = 128 / per, dc = 128 - dr * per;
-#pragma unroll
-      for (int j = 0; j < (int)(sizeof(x) / sizeof(uint4)); j++) {
-        if (j >= per) break;
-        const int p = __shfl_sync(0xffffffffu, page, row >> 4);
-        x[j] = make_uint4(0, 0, 0, 0);
-        if (p >= 0 && key0 + row < w.len) x[j] = __ldg(reinterpret_cast<const uint4*>(code + ((uint64_t)(uint32_t)p * block + (h * head + ((key0 + row) & (A.C.block - 1)) * dim + col * 16))));
-        row += dr; col += dc;
-        if (col >= per) { col -= per; row++; }
-      }
-    };
-    auto store = [&](const auto& x, int per, uint32_t to, bool clean) {
-      int row = tid / per, col = tid - row * per;
-      const int dr = 128 / per, dc = 128 - dr * per;
-      uint32_t found = 0;
-#pragma unroll
-      for (int j = 0; j < (int)(sizeof(x) / sizeof(uint4)); j++) {
-        if (j >= per) break;
-        uint32_t c[4] = {x[j].x, x[j].y, x[j].z, x[j].w}, f[8];
-        if (clean)
-#pragma unroll
-          for (int u = 0; u < 4; u++) { const uint32_t z = nan_bytes(c[u]); found |= z; c[u] &= ~z; }
-#pragma unroll
-        for (int u = 0; u < 4; u++) four_halves(c[u], f[2 * u], f[2 * u + 1]);
-        const uint32_t at = to + (col >> 2) * (kTile * 128) + row * 128, p0 = ((col & 3) * 2) ^ (row & 7);
-        // two 16-byte pieces; lanes of odd 64-entry blocks begin with the second one: eight lanes never meet a bank twice
-        if ((col >> 2) & 1) { sts128(at + ((p0 ^ 1) << 4), f[4], f[5], f[6], f[7]); sts128(at + (p0 << 4), f[0], f[1], f[2], f[3]); }
-        else { sts128(at + (p0 << 4), f[0], f[1], f[2], f[3]); sts128(at + ((p0 ^ 1) << 4), f[4], f[5], f[6], f[7]); }
-        row += dr; col += dc;
-        if (col >= per) { col -= per; row++; }
-      }
-      return found;
-    };
-    const int pk = dk / 16, pv = dv / 16;
-    int kst = 0, vst = 0;
-    uint32_t kturn = 1, vturn = 1;
-    bool alive = true;
-    next_page = look(0);
-    page = next_page;
-    if (n > 0) load(kx, pk, A.C.code[0], head_k, block_k, dk, key_of(w, w.begin));
-    for (int i = 0; i < n && alive; i++) {
-      const int key0 = key_of(w, w.begin + i);
-      next_page = look(i + 1);
-      float k_scale = 0.f, v_scale = 0.f;
-      if (warp == 8 && lane < 8 && page >= 0) {
-        const uint64_t slot = (uint64_t)(uint32_t)page * (uint32_t)A.C.heads + h;
-        k_scale = __ldg(A.C.scale[0] + slot);
-        v_scale = __ldg(A.C.scale[1] + slot);
-      }
-      load(vx, pv, A.C.code[1], head_v, block_v, dv, key0);
-      alive = wait_warp(kempty + 8 * kst, kturn, A.C);
-      if (!alive) break;
-      if (warp == 8) {
-        if (lane < 8) {
-          float* to = scales + (i % kSlots) * 24 + lane;
-          const int e = (int)(__float_as_uint(v_scale) >> 23) - 127;
-          to[0] = k_scale;
-          to[8] = page >= 0 ? (float)e : 0.f;
-          to[16] = page >= 0 ? pow2(-e) : 0.f;
-        }
-        __syncwarp();
-        if (lane == 0) hy::tc_arrive(cfull + 8 * (i % kSlots));
-      }
-      store(kx, pk, ks + kst * KB, false);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) hy::tc_arrive(kfull + 8 * kst);
-      if (++kst == KST) { kst = 0; kturn ^= 1; }
-      page = next_page;
-      if (i + 1 < n) load(kx, pk, A.C.code[0], head_k, block_k, dk, key_of(w, w.begin + i + 1));
-      alive = wait_warp(vempty + 8 * vst, vturn, A.C);
-      if (!alive) break;
-      if (store(vx, pv, vs + vst * VB, !sees_all(A, w, w.i0, w.i1, key0))) nan_seen = 1;
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) hy::tc_arrive(vfull + 8 * vst);
-      if (++vst == VST) { vst = 0; vturn ^= 1; }
-    }
-    __syncwarp();
-    if (lane == 0) hy::tc_arrive(cdone);
-  } else {
+    bring<DK, kTile / 32, 4>(A, w, b, h, 0, warp - 8, lane, ks, KB, KST, kfull, kempty, cfull, scales, &nan_seen);
+    } else {
     const int t = warp >> 2, quad = warp & 3, row = row0 + threadIdx.x, i_row = row / A.group, pos = w.first + i_row;
     const int r_first = (row0 + t * 128) / A.group, r_last = min((row0 + t * 128 + 127) / A.group, w.i1);   // tokens of the tile's rows
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_at = tmem + t * 128 + lanes, res = o_at + t * 128 + lanes;
+    auto factor = [&](float key_scale) { return fmaxf(row_scale * key_scale, 1.17549435e-38f); };   // (positive: -inf stays what it is)
     float m = -1e30f, l = 0.f;
     bool ok = true;
     for (int i = 0; i < n; i++) {
@@ -342,73 +406,77 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       ok = wait_warp(cfull + 8 * slot, (i / kSlots) & 1, A.C) && wait_warp(sfull + 8 * t, i & 1, A.C);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const float* sc = scales + slot * 24;
-      bool gone = false;
-#pragma unroll
-      for (int g = 0; g < 8; g++) gone |= sc[16 + g] == 0.f;
-      const bool masked = gone || !sees_all(A, w, r_first, r_last, key0);
-      // half a row of scores in registers at a time: both halves for the maximum, the second one stays, the first one is read again
-      float s[64], top = -INFINITY;
-      auto half = [&](int c) {
+      const float4* sc = reinterpret_cast<const float4*>(scales + slot * 24);   // key scales of 16 keys each [8], exponents of their value scales [8], reciprocals of those [8] (zero: not there)
+      const float4 there[2] = {sc[4], sc[5]};
+      const bool masked = there[0].x == 0.f || there[0].y == 0.f || there[0].z == 0.f || there[0].w == 0.f || there[1].x == 0.f || there[1].y == 0.f || there[1].z == 0.f || there[1].w == 0.f ||
+                          !sees_all(A, w, r_first, r_last, key0);
+      // half a row of scores in registers at a time: the first half for the maximum, the second one for the maximum and its weights, the first one again for its weights
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int pass = 0; pass < 3; pass++) {
+        const int half = pass == 1, c = half * 64;
+        const float4 k4 = sc[half], l4 = sc[2 + half];
+        const float fs[4] = {factor(k4.x), factor(k4.y), factor(k4.z), factor(k4.w)}, lift[4] = {l4.x, l4.y, l4.z, l4.w};
         uint32_t x[64];
         tmem_read64(s_at + c, x);
+        if (masked) {                                        // keys that the row sees, a bit each: not behind its own, in the window or among the first, in the cache
+          const float4 back = sc[4 + half];
 #pragma unroll
-        for (int k = 0; k < 64; k++) s[k] = __uint_as_float(x[k]);
-        if (masked) {
+          for (int u = 0; u < 64; u += 32) {
+            const int j = key0 + c + u, window = A.window > 0 ? pos - A.window + 1 - j : 0;
+            uint32_t see = lower_bits(pos + 1 - j) & (~lower_bits(window) | lower_bits(A.keep - j));
+            if ((u ? back.z : back.x) == 0.f) see &= 0xffff0000u;
+            if ((u ? back.w : back.y) == 0.f) see &= 0xffffu;
 #pragma unroll
-          for (int k = 0; k < 64; k++) {
-            const int j = key0 + c + k;
-            if (sc[16 + (c + k) / 16] == 0.f || j > pos || (A.window > 0 && pos - j >= A.window && j >= A.keep)) s[k] = -INFINITY;
+            for (int k = 0; k < 32; k++) if (!(see >> k & 1)) x[u + k] = 0xff800000u;
           }
         }
-      };
-      auto highest = [&](int c) {
+        if (pass < 2) {
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-          float x = s[16 * g];
+          for (int g = 0; g < 4; g++) {
+            float y[5];
 #pragma unroll
-          for (int k = 1; k < 16; k++) x = fmaxf(x, s[16 * g + k]);
-          top = fmaxf(top, fmaf(x, fmaxf(row_scale * sc[c / 16 + g], 1.17549435e-38f), sc[8 + c / 16 + g]));
-        }
-      };
-      half(0);
-      highest(0);
-      half(64);
-      highest(64);
-      if (__any_sync(0xffffffffu, top > m + kSlack)) {
-        const float to = fmaxf(m, top), by = exp2_fast(m - to);
-        m = to;
-        l *= by;
-        if (i > 0) {                                         // (the tile's last product was through ahead of these scores)
+            for (int k = 0; k < 5; k++) y[k] = max3(x[16 * g + 3 * k], x[16 * g + 3 * k + 1], x[16 * g + 3 * k + 2]);
+            const float z = max3(__float_as_uint(max3(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]))), __float_as_uint(fmaxf(y[3], y[4])), x[16 * g + 15]);
+            top = fmaxf(top, fmaf(z, fs[g], lift[g]));
+          }
+          if (pass == 0) continue;
+          if (__any_sync(0xffffffffu, top > m + kSlack)) {
+            const float to = fmaxf(m, top), by = exp2_fast(m - to);
+            m = to;
+            l *= by;
+            if (i > 0) {                                     // (the tile's last product was through ahead of these scores)
 #pragma unroll 1
-          for (int c = 0; c < DV; c += 16) {
-            uint32_t x[16];
-            tmem_read16(res + c, x);
+              for (int d = 0; d < DV; d += 16) {
+                uint32_t y[16];
+                tmem_read16(res + d, y);
 #pragma unroll
-            for (int k = 0; k < 16; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * by);
-            tmem_store16(res + c, x);
+                for (int k = 0; k < 16; k++) y[k] = __float_as_uint(__uint_as_float(y[k]) * by);
+                tmem_store16(res + d, y);
+              }
+            }
           }
         }
-      }
-      auto weigh = [&](int c) {                              // weights of a half lie in the first 32 of its columns
-        uint32_t x[32];
+        const float4 b4 = sc[4 + half];
+        const float back[4] = {b4.x, b4.y, b4.z, b4.w};
+        uint32_t p[32];                                      // weights of a half lie in the first 32 of its columns
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-          const float f = fmaxf(row_scale * sc[c / 16 + g], 1.17549435e-38f), off = sc[8 + c / 16 + g] - m;
-          float sum = 0.f;
+          const uint64_t f = both(fs[g], fs[g]), off = both(lift[g] - m, lift[g] - m);
+          uint64_t sum = 0;
 #pragma unroll
           for (int k = 0; k < 8; k++) {
-            const float p0 = exp2_fast(fmaf(s[16 * g + 2 * k], f, off)), p1 = exp2_fast(fmaf(s[16 * g + 2 * k + 1], f, off));
-            sum += p0 + p1;
-            x[8 * g + k] = halves(p0, p1);
+            float y0, y1;
+            fma2(x[16 * g + 2 * k], x[16 * g + 2 * k + 1], f, off, y0, y1);
+            y0 = exp2_fast(y0);
+            y1 = exp2_fast(y1);
+            add2(sum, y0, y1);
+            p[8 * g + k] = halves(y0, y1);
           }
-          l = fmaf(sum, sc[16 + c / 16 + g], l);
+          l = fmaf(__uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)), back[g], l);
         }
-        tmem_store32(s_at + c, x);
-      };
-      weigh(64);
-      half(0);
-      weigh(0);
+        tmem_store32(s_at + c, p);
+      }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -436,23 +504,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
         }
       }
       const float inv = P.shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      float* part = A.part + ((((size_t)b * A.C.heads + h) * gridDim.y + (gridDim.y - 1 - blockIdx.y)) * P.shares + share) * kRows * (DV + 2);
+      float* part = A.part + ((((size_t)b * A.C.heads + h) * gridDim.y + (gridDim.y - 1 - blockIdx.y)) * P.shares + share) * kRows * (DV + 2) + threadIdx.x;
 #pragma unroll
-      for (int c = 0; c < DV; c += 32) {
-        uint32_t x[32];
-        if (n > 0) tmem_read32(res + c, x);
-        float f[32];
+      for (int c = 0; c < DV; c += 16) {
+        uint32_t x[16];
+        if (n > 0) tmem_read16(res + c, x);
+        float f[16];
 #pragma unroll
-        for (int k = 0; k < 32; k++) f[k] = n == 0 ? 0.f : (lost[c / 32] >> k) & 1 ? NAN : __uint_as_float(x[k]);
+        for (int k = 0; k < 16; k++) f[k] = n == 0 ? 0.f : (lost[c / 32] >> ((c & 31) + k)) & 1 ? NAN : __uint_as_float(x[k]);
         if (P.shares > 1) {                                  // [entry][row]: neighbouring threads side by side
 #pragma unroll
-          for (int k = 0; k < 32; k++) part[(c + k) * kRows + threadIdx.x] = f[k];
-        } else {
-          Out::store(A, Seq{w.len, w.count, 0, 0, 0, 0, 0, 0}, b, h, row, c, 16, f, inv);
-          Out::store(A, Seq{w.len, w.count, 0, 0, 0, 0, 0, 0}, b, h, row, c + 16, 16, f + 16, inv);
-        }
+          for (int k = 0; k < 16; k++) part[(c + k) * kRows] = f[k];
+        } else Out::store(A, Seq{w.len, w.count, 0, 0, 0, 0, 0, 0}, b, h, row, c, 16, f, inv);
       }
-      if (P.shares > 1) { part[DV * kRows + threadIdx.x] = m; part[(DV + 1) * kRows + threadIdx.x] = l; }
+      if (P.shares > 1) { part[DV * kRows] = m; part[(DV + 1) * kRows] = l; }
     }
   }
   __syncthreads();

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <mutex>
@@ -82,9 +83,13 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 int size_of(int dtype) { return dtype == DSK_DT_F32 ? 4 : 2; }
 
 int check_device(int device) {
-  int n = 0;
-  const cudaError_t e = cudaGetDeviceCount(&n);
-  if (e != cudaSuccess || n == 0) { cudaGetLastError(); return fail(-1, "no CUDA device available (%s) — libdsk has no CPU fallback", cudaGetErrorString(e)); }
+  static std::atomic<int> known{0};                          // (devices do not come and go within a process)
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    const cudaError_t e = cudaGetDeviceCount(&n);
+    if (e != cudaSuccess || n == 0) { cudaGetLastError(); return fail(-1, "no CUDA device available (%s) — libdsk has no CPU fallback", cudaGetErrorString(e)); }
+    known.store(n, std::memory_order_relaxed);
+  }
   if (device < 0 || device >= n || device >= kMaxDevices) return fail(-1, "device %d out of range (have %d)", device, n);
   return 0;
 }
@@ -262,8 +267,8 @@ extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
 
 static int check_verify(const dsk_verify_args* a) {
   if (!a) return fail(-1, "null arguments");
-  if (a->batch < 0 || a->batch > 65535 || a->drafts < 0 || a->drafts > verify::kMaxDrafts || a->vocab <= 0 || a->vocab > (1 << 28))
-    return fail(-4, "batch %d (at most 65535), %d drafts (at most %d), vocabulary %d (at most 2^28)", a->batch, a->drafts, verify::kMaxDrafts, a->vocab);
+  if (a->batch < 0 || a->batch > 65535 || a->drafts < 0 || a->drafts > verify::kMaxDrafts || a->vocab <= 0 || a->vocab > (1 << 20))
+    return fail(-4, "batch %d (at most 65535), %d drafts (at most %d), vocabulary %d (at most 2^20)", a->batch, a->drafts, verify::kMaxDrafts, a->vocab);
   return 0;
 }
 static int pieces_of(const dsk_verify_args* a) { return (a->vocab + verify::kPiece - 1) / verify::kPiece; }
@@ -276,9 +281,10 @@ extern "C" int dsk_verify_workspace(const dsk_verify_args* a, size_t* bytes) {
 }
 
 template <typename T> static int verify_as(const verify::Params& P, cudaStream_t stream) {
-  verify::row_stats<T><<<dim3((P.pieces + verify::kWarps - 1) / verify::kWarps, P.n + 1, P.batch), verify::kThreads, 0, stream>>>(P);
+  verify::row_stats<T><<<dim3((P.pieces + verify::kStatWarps - 1) / verify::kStatWarps, P.n + 1, P.batch), verify::kStatThreads, 0, stream>>>(P);
   CK(cudaGetLastError());
-  CK(launch_behind(verify::pick<T>, dim3(P.batch * P.cluster), dim3(verify::kThreads), 0, stream, P.cluster, P));
+  if (P.vocab <= 1 << 17) CK(launch_behind(verify::pick<T, 45>, dim3(P.batch * P.cluster), dim3(verify::kThreads), 0, stream, P.cluster, P));   // (sums of a row stay below 2^62)
+  else CK(launch_behind(verify::pick<T, 42>, dim3(P.batch * P.cluster), dim3(verify::kThreads), 0, stream, P.cluster, P));
   return 0;
 }
 

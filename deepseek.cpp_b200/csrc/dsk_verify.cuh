@@ -3,9 +3,11 @@
 // p_i = softmax(logits_i / temperature).  Draft x_i is accepted while coin_i q_i(x_i) < p_i(x_i); the first one that is not is replaced by a draw from max(p_i - q_i, 0), and
 // behind accepted ones the next token is drawn from p.  Both draws take the lowest index whose running sum is over (last coin) x (whole sum).
 // Two kernels: row_stats reads every row of logits once (maximum and sum of a piece of 1024 per warp, in fp32); pick has a cluster of CTAs for each sequence, which decides
-// on the drafts and draws from one row.  A draw's result hangs on sums of up to the whole vocabulary next to a border, so pick takes exponentials, sums and differences
-// of that row in 64 bits: in 32 one draw in some thousands of a flat row would take a neighbour.  Where coin x q is within 1e-4 of p, the row's sum is taken again in 64 bits as well.
-// Bound: row_stats by the bytes of the logits; pick by the latency of three walks over a row that L2 holds, with a cluster's barrier behind two of them.
+// on the drafts and draws from one row.  A draw's result hangs on sums of up to the whole vocabulary next to a border: in fp32 one draw in some thousands of a flat row would take a
+// neighbour.  pick takes that row's exponentials in two fp32 parts, good to 2^-33 of each, as whole numbers of 2^-45 (2^-42 where the vocabulary has more than 2^17 entries), whose sums
+// are exact in any order; p and q meet as such numbers too.  Where coin x q is
+// within 1e-4 of p, the row's sum is taken that way as well.
+// Bound: row_stats by the bytes of the logits; pick by the latency of its steps, two walks over a row that L2 holds and a cluster's barrier behind each among them.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -15,7 +17,7 @@
 namespace dsk {
 namespace verify {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kPiece = 1024, kMaxDrafts = 127, kMaxCluster = 16;
+constexpr int kStatThreads = 256, kStatWarps = kStatThreads / 32, kThreads = 512, kWarps = kThreads / 32, kPiece = 1024, kMaxDrafts = 127, kMaxCluster = 8;
 
 struct Params {
   const void* logits;
@@ -47,9 +49,9 @@ template <typename T> __device__ __forceinline__ void four(const T* row, int i, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) row_stats(const Params P) {
+__global__ void __launch_bounds__(kStatThreads) row_stats(const Params P) {
   grid_release();
-  const int warp = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = blockIdx.y, b = blockIdx.z;
+  const int warp = blockIdx.x * kStatWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = blockIdx.y, b = blockIdx.z;
   if (warp >= P.pieces || r > drafts_of(P, b)) return;
   const T* row = static_cast<const T*>(P.logits) + b * P.l_batch + r * P.l_row;
   float x[kPiece / 128][4], m = -INFINITY;
@@ -86,76 +88,104 @@ __global__ void __launch_bounds__(kThreads) row_stats(const Params P) {
   if (lane == 0) *out = make_float2(top, s);
 }
 
-// 2^y for y <= 0 in 64 bits: 2^(k / 64) from a table, the rest of at most 1/128 by the series of e^z (z^6 / 720 < 4e-17); Tang, "Table-driven implementation of the exponential
-// function in IEEE floating-point arithmetic" (1989)
-__device__ __forceinline__ double power(double y, const double* table) {
-  const double magic = 6755399441055744.0, t = fma(y, 64.0, magic);   // 1.5 x 2^52: the integer next to 64 y stands in the low bits
-  const int k = __double2loint(t);
-  const double z = fma(t - magic, -1.0 / 64.0, y) * 0.693147180559945309417;
-  double p = fma(z, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(z, p, 1.0 / 6.0);
-  p = fma(z, p, 0.5);
-  p = fma(z, p, 1.0);
-  p = fma(z, p, 1.0);
-  const double r = table[k & 63] * p;
-  return y > -1000.0 ? __hiloint2double(__double2hiint(r) + ((k >> 6) << 20), __double2loint(r)) : (y <= -1000.0 ? 0.0 : y);
+// 2^y for y <= 0 in fp64, for the few values that drafts are judged by: 2^(k / 64) from a table, the rest by the series of e^z (Tang, "Table-driven implementation of the
+// exponential function in IEEE floating-point arithmetic", 1989)
+__device__ __forceinline__ double power(double y) { return y > -1000.0 ? exp2(y) : y <= -1000.0 ? 0.0 : y; }
+
+// 2^y of many values as whole numbers of 2^-BITS.  y = 64 (l - m) / temperature log2(e) in two parts, its integer part k looks up 2^(k mod 64 / 64), the rest f gives e^(f ln2 / 64) - 1
+// in two parts, of at most 0.0055; relative error 2^-36 (checked on 200000 values).  What the shift to the value's size cuts off counts as half a step: sums are not biased.
+struct Slope { float hi, lo; };                              // 64 log2(e) / temperature
+template <int BITS> __device__ __forceinline__ uint64_t whole_power(float l, float m, Slope s, const uint4* table) {
+  constexpr float C = 0.010830424726009369f, C_LO = -2.976022e-11f;   // ln 2 / 64 in two parts
+  const float d = l - m, b = d - l, d_lo = (l - (d - b)) - (m + b);   // l - m exactly
+  float y = d * s.hi;
+  const bool none = !(y > -3200.f);                          // below 2^-50 (-inf among them)
+  const float e = fmaf(d_lo, s.hi, fmaf(d, s.lo, fmaf(d, s.hi, -y)));
+  const float t = y + 12582912.f, f0 = y - (t - 12582912.f), f = f0 + e, f_lo = (f0 - f) + e;
+  const float z = f * C, z_lo = fmaf(f_lo, C, fmaf(f, C_LO, fmaf(f, C, -z)));
+  const float r = fmaf(z * z, fmaf(z, fmaf(z, 1.f / 24.f, 1.f / 6.f), 0.5f), z_lo);
+  const int q = __float2int_rn(z * 274877906944.f) + __float2int_rn(r * 274877906944.f);   // 2^38
+  const int n = __float_as_int(t) - 0x4b400000;
+  const uint4 p = table[n & 63];                             // 2^BITS to 2^(BITS + 1), and its first 31 bits
+  const uint64_t v = (((uint64_t)p.y << 32) | p.x) + (uint64_t)(((int64_t)(int)p.z * q) >> (68 - BITS));
+  return none ? 0 : (v >> (-(n >> 6) & 63)) | 1;
 }
-__device__ __forceinline__ double sum64(double v) {
+__device__ __forceinline__ uint64_t sum64(uint64_t v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ uint64_t running(uint64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const uint64_t t = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += t; }
+  return v;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) pick(const Params P) {
+template <typename T, int BITS>
+__global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
   namespace cg = cooperative_groups;
-  __shared__ double table[64], ends[kMaxCluster * kWarps], sums[2][kWarps], row_sum[kMaxDrafts + 1];
+  __shared__ uint4 table[64];
+  __shared__ uint64_t ends[kMaxCluster * kWarps], sums[2][kWarps];
+  __shared__ double row_sum[kMaxDrafts + 1];
   __shared__ float row_max[kMaxDrafts + 1];
   __shared__ int flag[kMaxDrafts + 1], top_at[kMaxDrafts + 1];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), b = blockIdx.x / P.cluster, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid < 64) table[tid] = exp2(tid / 64.0);
-  grid_wait();
-  __syncthreads();
   const int n = drafts_of(P, b), V = P.vocab;
   const bool greedy = P.slope == 0.0;
   const T* logits = static_cast<const T*>(P.logits) + b * P.l_batch;
   const int* drafts = P.drafts + (size_t)b * P.n;
   const float* coins = P.coins + (size_t)b * (P.n + 1);
+  const double slope64 = 64.0 * P.slope;
+  const Slope slope{(float)slope64, (float)(slope64 - (float)slope64)};
+  if (tid < 64) {
+    const uint64_t p = (uint64_t)__double2ll_rn(exp2(tid / 64.0 + BITS));
+    table[tid] = make_uint4((uint32_t)p, (uint32_t)(p >> 32), (uint32_t)(p >> (BITS - 30)), 0);
+  }
+  // what drafts are judged by does not wait for the kernel ahead, which only reads it
+  struct Row { int x; float l, q, coin; };
+  auto look = [&](int r) {
+    Row w{r < n ? drafts[r] : -1, 0.f, 1.f, coins[min(r, P.n)]};
+    if ((unsigned)w.x >= (unsigned)V) w.x = -1;
+    else { w.l = value(logits[r * P.l_row + w.x]); if (P.probs) w.q = P.probs[b * P.p_batch + r * P.p_row + w.x]; }
+    return w;
+  };
+  Row w = look(warp <= n ? warp : n);
+  const float last_coin = coins[P.n];
+  grid_wait();
   // rows: maximum and sum of the pieces; 0: refused, 1: accepted, 2: next to the border, 4: not a distribution (a NaN, +inf or nothing but -inf)
   for (int r = warp; r <= n; r += kWarps) {
+    if (r != warp) w = look(r);
     const float2* part = P.part + ((size_t)b * (P.n + 1) + r) * P.pieces;
     float m = -INFINITY;
     bool nan = false;
     for (int i = lane; i < P.pieces; i += 32) { const float t = part[i].x; m = fmaxf(m, t); nan |= t != t; }
     m = warp_max(m);
     nan = __any_sync(0xffffffffu, nan);
-    int x = r < n ? drafts[r] : -1;
-    if ((unsigned)x >= (unsigned)V) x = -1;
     if (greedy) {
       unsigned at = 0x7fffffffu;
       for (int i = lane; i < P.pieces; i += 32) if (part[i].x == m) at = min(at, (unsigned)__float_as_int(part[i].y));
       at = __reduce_min_sync(0xffffffffu, at);
-      if (lane == 0) { flag[r] = nan || m == -INFINITY ? 4 : x == (int)at ? 1 : 0; top_at[r] = (int)at; }
+      if (lane == 0) { flag[r] = nan || m == -INFINITY ? 4 : w.x == (int)at ? 1 : 0; top_at[r] = (int)at; }
       continue;
     }
-    double s = 0.0;
-    for (int i = lane; i < P.pieces; i += 32) { const float2 t = part[i]; s += t.x == -INFINITY ? (double)t.y : (double)t.y * power(((double)t.x - m) * P.slope, table); }
-    s = sum64(s);
+    float s = 0.f;                                           // (to 1e-5; what hangs on more is taken again)
+    for (int i = lane; i < P.pieces; i += 32) { const float2 t = part[i]; s += t.x == -INFINITY ? t.y : t.y * exp2f((t.x - m) * (float)P.slope); }
+    s = warp_sum(s);
     if (lane == 0) {
       int f = 0;
       if (!(m > -INFINITY && m < INFINITY) || !(s < INFINITY)) f = 4;
-      else if (x >= 0) {
-        const double p = power(((double)value(logits[r * P.l_row + x]) - m) * P.slope, table) / s, q = P.probs ? (double)P.probs[b * P.p_batch + r * P.p_row + x] : 1.0, want = (double)coins[r] * q;
+      else if (w.x >= 0) {
+        const double p = power(((double)w.l - m) * P.slope) / s, want = (double)w.coin * w.q;
         f = fabs(want - p) <= 1e-4 * p && p > 0.0 ? 2 : want < p ? 1 : 0;
       }
       flag[r] = f; row_max[r] = m; row_sum[r] = s;
     }
   }
   __syncthreads();
-  auto walk = [&](int r, int from, int to, double m) {       // sum of a row's exponentials over indices from .. to - 1 (from a multiple of four), by a warp
+  auto walk = [&](int r, int from, int to, float m) {        // sum of a row's exponentials over indices from .. to - 1 (from a multiple of four), by a warp
     const T* row = logits + r * P.l_row;
-    double s = 0.0;
+    uint64_t s = 0;
     for (int i = from + lane * 4; i < to; i += 512) {
       float x[4][4];
 #pragma unroll
@@ -163,10 +193,11 @@ __global__ void __launch_bounds__(kThreads) pick(const Params P) {
 #pragma unroll
       for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int w = 0; w < 4; w++) s += power(((double)x[u][w] - m) * P.slope, table);
+        for (int k = 0; k < 4; k++) s += whole_power<BITS>(x[u][k], m, slope, table);
     }
     return sum64(s);
   };
+  const double unit = exp2(-(double)BITS);
   const int all = P.cluster * kWarps, share = ((V + all - 1) / all + 127) / 128 * 128, mine = rank * kWarps + warp;   // a warp's indices of the row that is drawn from
   const int from = min(V, mine * share), to = min(V, from + share);
   int r = 0;                                                 // (the same in every CTA of the cluster)
@@ -174,19 +205,17 @@ __global__ void __launch_bounds__(kThreads) pick(const Params P) {
     int f = flag[r];
     if (f == 2) {
       const int each = ((V + kWarps - 1) / kWarps + 3) / 4 * 4;
-      const double s = walk(r, min(V, warp * each), min(V, (warp + 1) * each), row_max[r]);
+      const uint64_t s = walk(r, min(V, warp * each), min(V, (warp + 1) * each), row_max[r]);
       if (lane == 0) sums[0][warp] = s;
       __syncthreads();
-      double whole = 0.0;
-      for (int w = 0; w < kWarps; w++) whole += sums[0][w];
+      uint64_t whole = 0;
+      for (int k = 0; k < kWarps; k++) whole += sums[0][k];
       __syncthreads();
-      const int x = drafts[r];
-      const double p = power(((double)value(logits[r * P.l_row + x]) - row_max[r]) * P.slope, table) / whole, q = P.probs ? (double)P.probs[b * P.p_batch + r * P.p_row + x] : 1.0;
-      f = (double)coins[r] * q < p;
+      const Row y = look(r);
+      f = (double)y.coin * y.q < power(((double)y.l - row_max[r]) * P.slope) / ((double)whole * unit);
     }
     if (f != 1) break;
   }
-  int token = -1;
   int* out = P.tokens + (size_t)b * (P.n + 1);
   if (rank == 0) {
     for (int i = tid; i <= P.n; i += kThreads) if (i != r) out[i] = i < r ? drafts[i] : -1;
@@ -196,43 +225,49 @@ __global__ void __launch_bounds__(kThreads) pick(const Params P) {
     if (rank == 0 && tid == 0) out[r] = flag[r] == 4 ? -1 : top_at[r];
     return;                                                  // (the whole cluster)
   }
-  const double m = row_max[r];
-  {
-    const double s = walk(r, from, to, m);
-    if (lane == 0) sums[0][warp] = s;
-  }
-  cluster.sync();
+  const float m = row_max[r];
+  const bool drafted = r < n;
+  const float* q = drafted && P.probs ? P.probs + b * P.p_batch + r * P.p_row : nullptr;
   auto gather = [&](int which) {                             // sums of all warps of the cluster, in order
     if (tid < all) ends[tid] = *cluster.map_shared_rank(&sums[which][tid % kWarps], tid / kWarps);
     __syncthreads();
   };
-  gather(0);
-  double whole = 0.0;
-  for (int i = lane; i < all; i += 32) whole += ends[i];
-  whole = sum64(whole);
-  const double inv = 1.0 / whole;
-  const bool drafted = r < n;
+  uint64_t whole = 0;
+  if (q) {                                                   // (a row that is drawn from by itself needs no sum ahead of its draw)
+    const uint64_t s = walk(r, from, to, m);
+    if (lane == 0) sums[0][warp] = s;
+    cluster.sync();
+    gather(0);
+    for (int i = lane; i < all; i += 32) whole += ends[i];
+    whole = sum64(whole);
+  }
+  const int high = 63 - __clzll(whole | 1);                  // q x whole = (24 bits) x (the first 32 of whole), shifted
+  const uint32_t first = (uint32_t)(high >= 31 ? whole >> (high - 31) : whole << (31 - high));
+  const int past = 150 + 7 - (high - 31);                    // minus the exponent of q: how far to the right
   const T* row = logits + r * P.l_row;
-  const float* q = drafted && P.probs ? P.probs + b * P.p_batch + r * P.p_row : nullptr;
   const int certain = drafted && !P.probs ? drafts[r] : -1;
-  auto left = [&](int i, double (&d)[4]) {                   // what four indices have in the draw
+  auto left = [&](int i, int end, uint64_t (&d)[4]) {        // what four indices have in the draw: (p - q) x (sum of the row), none below zero
     float x[4], y[4] = {0.f, 0.f, 0.f, 0.f};
-    four(row, i, i < to ? V : 0, P.wide_l, x);
-    if (q && i < to) four(q, i, V, P.wide_p, y);
+    four(row, i, i < end ? V : 0, P.wide_l, x);
+    if (q && i < end) four(q, i, V, P.wide_p, y);
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const double p = power(((double)x[u] - m) * P.slope, table) * inv;
-      d[u] = i + u >= to ? 0.0 : q ? fmax(p - (double)y[u], 0.0) : i + u == certain ? 0.0 : p;
+      const uint64_t p = whole_power<BITS>(x[u], m, slope, table);
+      if (!q) { d[u] = i + u >= end || i + u == certain ? 0 : p; continue; }
+      const uint32_t bits = __float_as_uint(y[u]);           // (nothing is left where q is negative or not a number; numbers below 2^-126 count as none)
+      const int ex = (int)(bits >> 23), by = past - ex;
+      const uint64_t t = ((uint64_t)((bits & 0x7fffffu) | 0x800000u) * first) << 7;
+      const uint64_t other = by < 0 ? p : ex == 0 || by > 63 ? 0 : t >> by;
+      d[u] = i + u >= end || other >= p ? 0 : p - other;
     }
   };
   {
-    double s = 0.0;
-    for (int i = from + lane * 4; i < to; i += 256) {
-      double d[2][4];
-      left(i, d[0]);
-      left(i + 128, d[1]);
-#pragma unroll
-      for (int u = 0; u < 4; u++) s += d[0][u] + d[1][u];
+    uint64_t s = 0;
+#pragma unroll 2
+    for (int i = from + lane * 4; i < to; i += 128) {
+      uint64_t d[4];
+      left(i, to, d);
+      s += (d[0] + d[1]) + (d[2] + d[3]);
     }
     s = sum64(s);
     if (lane == 0) sums[1][warp] = s;
@@ -240,51 +275,46 @@ __global__ void __launch_bounds__(kThreads) pick(const Params P) {
   cluster.sync();
   gather(1);
   if (warp == 0) {                                           // running sums of the warps, in order
-    double run = 0.0;
+    uint64_t run = 0;
     for (int i0 = 0; i0 < all; i0 += 32) {
-      double v = i0 + lane < all ? ends[i0 + lane] : 0.0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const double t = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += t; }
+      const uint64_t v = running(i0 + lane < all ? ends[i0 + lane] : 0, lane);
       if (i0 + lane < all) ends[i0 + lane] = run + v;
       run += __shfl_sync(0xffffffffu, v, 31);
     }
   }
   __syncthreads();
-  const double total = ends[all - 1], want = (double)coins[P.n] * total;
-  int owner = -1;                                            // the first warp whose running sum is over it; behind all of them (a coin of one, rounding) the last that has anything
+  const uint64_t total = ends[all - 1], want = min((uint64_t)((double)last_coin * (double)total), total ? total - 1 : 0);   // (behind all: the last index that has anything)
+  int owner = -1;                                            // the warp whose indices hold the border
   for (int i0 = 0; i0 < all && owner < 0; i0 += 32) {
     const uint32_t over = __ballot_sync(0xffffffffu, i0 + lane < all && ends[i0 + lane] > want);
     if (over) owner = i0 + __ffs(over) - 1;
   }
-  for (int i = all - 1; i >= 0 && owner < 0; i--) if (ends[i] > (i ? ends[i - 1] : 0.0)) owner = i;
-  if (owner < 0 && mine == 0 && lane == 0) out[r] = -1;      // nothing is left
-  if (mine == owner) {
-    double run = owner ? ends[owner - 1] : 0.0;
-    int last = -1;
-    for (int i0 = from; i0 < to && token < 0; i0 += 128) {
-      double d[4];
-      left(i0 + lane * 4, d);
-      double v = d[0] + d[1] + d[2] + d[3];
-      const double own = v;
+  if (owner < 0) {                                           // nothing is left
+    if (mine == 0 && lane == 0) out[r] = -1;
+  } else if (owner / kWarps == rank) {                       // its CTA takes 128 indices a warp at a time
+    const int begin = min(V, owner * share), end = min(V, begin + share);
+    uint64_t run = owner ? ends[owner - 1] : 0;
+    for (int i0 = begin; i0 < end; i0 += kWarps * 128) {
+      uint64_t d[4];
+      const int i = i0 + warp * 128 + lane * 4;
+      left(i, end, d);
+      const uint64_t own = d[0] + d[1] + d[2] + d[3], v = running(own, lane);
+      if (lane == 31) sums[0][warp] = v;
+      __syncthreads();
+      uint64_t before = run, next = run;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const double t = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += t; }
-      const uint32_t over = __ballot_sync(0xffffffffu, run + v > want && own > 0.0), some = __ballot_sync(0xffffffffu, own > 0.0);
-      const int hit = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
-      int at = -1, latest = -1;
-      double c = run + v - own;
+      for (int k = 0; k < kWarps; k++) { if (k < warp) before += sums[0][k]; next += sums[0][k]; }
+      uint64_t c = before + v - own;
+      if (c <= want && c + own > want) {                     // (one lane)
+        int at = 0;
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        c += d[u];
-        if (d[u] > 0.0) { latest = i0 + lane * 4 + u; if (at < 0 && c > want) at = latest; }
+        for (int u = 0; u < 3; u++) { c += d[u]; if (c <= want) at = u + 1; }
+        out[r] = i + at;
       }
-      if (at < 0) at = latest;
-      const int found = __shfl_sync(0xffffffffu, at, max(hit, 0));
-      if (over) token = found;
-      else if (some) last = __shfl_sync(0xffffffffu, latest, hit);
-      run += __shfl_sync(0xffffffffu, v, 31);
+      if (next > want) break;
+      run = next;
+      __syncthreads();
     }
-    if (token < 0) token = last;
-    if (lane == 0) out[r] = token;
   }
   cluster.sync();                                            // nobody's shared memory is read any more
 }

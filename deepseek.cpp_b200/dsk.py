@@ -10,6 +10,7 @@ from __future__ import annotations
 import collections
 import ctypes as C
 import os
+import struct
 import subprocess
 import threading
 import weakref
@@ -896,19 +897,38 @@ class Model:
 
 # ---- operators on device memory: torch tensors of one GPU, work on torch's current stream of that GPU ------------------------------
 
-def _device_of(t) -> int:
-    if not getattr(t, "is_cuda", False):
-        raise DskError("tensors on a CUDA device are needed: libdsk has no CPU fallback")
-    return t.device.index
+# Arguments travel as packed structures (the classes above, laid out by struct): a call takes a few microseconds on the host, of which ctypes structures would be half.
+_ROWS, _VIEW, _VERIFY = struct.Struct("@PPPqiii4x"), struct.Struct("@Pi4xqqq"), struct.Struct("@PPPPPPPqqqqiiiiif")
+_raw = {}
+
+
+def _fast(name):
+    """The library's function `name` for packed structures and addresses."""
+    f = _raw.get(name)
+    if f is None:
+        f = lib()[name]
+        P = C.c_void_p
+        f.argtypes = {"dsk_kv8_write": [P, C.c_char_p, C.c_char_p, C.c_char_p, P], "dsk_kv8_read": [P, C.c_char_p, C.c_char_p, C.c_char_p, P],
+                      "dsk_kv8_attn_workspace": [P, C.c_char_p, C.c_int, C.POINTER(C.c_size_t)],
+                      "dsk_kv8_attn": [P, C.c_char_p, C.c_char_p, C.c_char_p, C.c_int, C.c_float, C.c_int, C.c_int, P, C.c_size_t, P],
+                      "dsk_verify_workspace": [C.c_char_p, C.POINTER(C.c_size_t)], "dsk_verify": [C.c_char_p, P, C.c_size_t, P]}[name]
+        _raw[name] = f
+    return f
+
+
+def _no_device(t):
+    raise DskError(f"tensors on a CUDA device are needed, got {t.device}: libdsk has no CPU fallback")
 
 
 def _stream_of(torch, device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _dense(what, t, dtype, shape, device):
-    """A contiguous tensor of that type and shape on the device (its address)."""
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or _device_of(t) != device:
+    """The address of a contiguous tensor of that type and shape on the device."""
+    if t.get_device() != device or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        if t.get_device() < 0:
+            _no_device(t)
         raise DskError(f"{what}: a contiguous {dtype} tensor {tuple(shape)} on cuda:{device} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -922,7 +942,7 @@ class Cache8:
 
     def __init__(self, n_blocks: int, kv_heads: int, dim_k: int, dim_v: Optional[int] = None, block: int = 64, device=None):
         import torch
-        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device) if not isinstance(device, int) else torch.device("cuda", device)
+        dev = torch.device("cuda", torch.cuda.current_device() if device is None else device) if device is None or isinstance(device, int) else torch.device(device)
         dim_v = dim_k if dim_v is None else dim_v
         f8 = torch.float8_e4m3fn
         self._bind(torch.zeros((n_blocks, kv_heads, block, dim_k), dtype=torch.uint8, device=dev).view(f8), torch.zeros((n_blocks, kv_heads, block, dim_v), dtype=torch.uint8, device=dev).view(f8),
@@ -937,8 +957,9 @@ class Cache8:
 
     def _bind(self, k, v, k_scale, v_scale):
         import torch
-        self._torch = torch
-        self.device = _device_of(k)
+        self._torch, self.device = torch, k.get_device()
+        if self.device < 0:
+            _no_device(k)
         if k.dim() != 4 or v.dim() != 4:
             raise DskError("codes are [n_blocks, kv_heads, block, dim]")
         _dense("keys", k, torch.float8_e4m3fn, k.shape, self.device)
@@ -949,38 +970,39 @@ class Cache8:
         self.n_blocks, self.kv_heads, self.block, self.dim_k = k.shape
         self.dim_v = v.shape[3]
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
-        self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-        self._c = Kv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.status.data_ptr(), self.device, *k.shape[:1], self.block, self.kv_heads, self.dim_k, self.dim_v)
-        self._L = lib()
+        self._i32, self._types = torch.int32, {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self._c = Kv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.status.data_ptr(), self.device, self.n_blocks, self.block, self.kv_heads, self.dim_k, self.dim_v)
+        self._at = C.addressof(self._c)
+        self._needs = {}            # bytes of attention's workspace by shape of the call
 
     def _rows(self, table, first, count, rows):
-        torch = self._torch
-        if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) not in (1, 0) and table.shape[1] > 1 or _device_of(table) != self.device:
+        if table.dim() != 2 or table.dtype is not self._i32 or table.get_device() != self.device or table.stride(1) != 1 and table.shape[1] > 1:
+            if table.get_device() < 0:
+                _no_device(table)
             raise DskError(f"table: int32 [batch, blocks] on cuda:{self.device} with rows of neighbours is needed, got {table.dtype} {tuple(table.shape)} on {table.device}")
-        if table.stride(1) == 0 and table.shape[1] > 1:
-            raise DskError("table: its rows must not be broadcast")
-        batch = table.shape[0]
-        return Kv8Rows(table.data_ptr(), _dense("first tokens / lengths", first, torch.int32, (batch,), self.device),
-                       _dense("count", count, torch.int32, (batch,), self.device) if count is not None else None, table.stride(0), table.shape[1], batch, rows)
+        batch, blocks = table.shape
+        return _ROWS.pack(table.data_ptr(), _dense("first tokens / lengths", first, self._i32, (batch,), self.device),
+                          0 if count is None else _dense("count", count, self._i32, (batch,), self.device), table.stride(0), blocks, batch, rows)
 
     def _view(self, what, t, shape, written=False):
-        if t.shape != shape or t.dtype not in self._types or _device_of(t) != self.device or t.stride(3) != 1:
-            raise DskError(f"{what}: float32, float16 or bfloat16 {tuple(shape)} on cuda:{self.device} with neighbouring entries is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
         s = t.stride()
-        if written and any(s[i] < t.shape[3] and t.shape[i] > 1 for i in range(3)):
+        if t.shape != shape or t.dtype not in self._types or t.get_device() != self.device or s[3] != 1:
+            if t.get_device() < 0:
+                _no_device(t)
+            raise DskError(f"{what}: float32, float16 or bfloat16 {tuple(shape)} on cuda:{self.device} with neighbouring entries is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if written and not t.is_contiguous() and any(s[i] < t.shape[3] and t.shape[i] > 1 for i in range(3)):
             raise DskError(f"{what}: rows of the result must not overlap")
-        return View(t.data_ptr(), self._types[t.dtype], s[0], s[1], s[2])
+        return _VIEW.pack(t.data_ptr(), self._types[t.dtype], s[0], s[1], s[2])
 
     def write(self, k, v, table, first, count=None):
         """Tokens first[b] .. of every sequence from rows k, v [batch, rows, kv_heads, dim] (dsk_kv8_write)."""
         if k.dim() != 4 or v.dim() != 4:
             raise DskError("keys and values are [batch, rows, kv_heads, dim]")
         batch, rows = k.shape[:2]
-        if batch != table.shape[0] or k.dtype != v.dtype:
+        if batch != table.shape[0] or k.dtype is not v.dtype:
             raise DskError(f"keys of {batch} sequences and {k.dtype}, values of {v.dtype}, a table of {table.shape[0]} sequences")
-        s = self._rows(table, first, count, rows)
-        a, b = self._view("keys", k, (batch, rows, self.kv_heads, self.dim_k)), self._view("values", v, (batch, rows, self.kv_heads, self.dim_v))
-        _ck(self._L.dsk_kv8_write(self._c, s, a, b, _stream_of(self._torch, self.device)))
+        _ck(_fast("dsk_kv8_write")(self._at, self._rows(table, first, count, rows), self._view("keys", k, (batch, rows, self.kv_heads, self.dim_k)),
+                                   self._view("values", v, (batch, rows, self.kv_heads, self.dim_v)), _stream_of(self._torch, self.device)))
 
     def read(self, table, first, rows: int, count=None, dtype=None, out=None):
         """The values of tokens first[b] .. first[b] + rows - 1 (dsk_kv8_read): (keys, values) [batch, rows, kv_heads, dim], `out` or new ones (zeros in rows from count[b] on)."""
@@ -989,11 +1011,10 @@ class Cache8:
         shapes = (batch, rows, self.kv_heads, self.dim_k), (batch, rows, self.kv_heads, self.dim_v)
         if out is None:
             out = tuple(torch.zeros(x, dtype=dtype or torch.bfloat16, device=table.device) for x in shapes)
-        elif dtype is not None and any(x.dtype != dtype for x in out) or out[0].dtype != out[1].dtype:
+        elif dtype is not None and any(x.dtype is not dtype for x in out) or out[0].dtype is not out[1].dtype:
             raise DskError(f"results of {out[0].dtype} and {out[1].dtype} where {dtype or 'one type'} is asked for")
-        s = self._rows(table, first, count, rows)
-        a, b = self._view("keys", out[0], shapes[0], True), self._view("values", out[1], shapes[1], True)
-        _ck(self._L.dsk_kv8_read(self._c, s, a, b, _stream_of(torch, self.device)))
+        _ck(_fast("dsk_kv8_read")(self._at, self._rows(table, first, count, rows), self._view("keys", out[0], shapes[0], True), self._view("values", out[1], shapes[1], True),
+                                  _stream_of(torch, self.device)))
         return out
 
     def attend(self, q, table, lens, count=None, scale: Optional[float] = None, window: int = 0, keep_first: int = 0, out=None):
@@ -1006,14 +1027,20 @@ class Cache8:
         shape = (batch, rows, heads, self.dim_v)
         if out is None:
             out = (torch.empty if count is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
-        elif out.dtype != q.dtype:
+        elif out.dtype is not q.dtype:
             raise DskError(f"results of {out.dtype} for queries of {q.dtype}")
         s = self._rows(table, lens, count, rows)
         a, b = self._view("queries", q, (batch, rows, heads, self.dim_k)), self._view("output", out, shape, True)
-        need = C.c_size_t(0)
-        _ck(self._L.dsk_kv8_attn_workspace(self._c, s, heads, need))
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        _ck(self._L.dsk_kv8_attn(self._c, s, a, b, heads, self.dim_k ** -0.5 if scale is None else scale, window, keep_first, work.data_ptr(), need.value, _stream_of(torch, self.device)))
+        key = (batch, rows, heads, table.shape[1])
+        need = self._needs.get(key)
+        if need is None:
+            got = C.c_size_t(0)
+            _ck(_fast("dsk_kv8_attn_workspace")(self._at, s, heads, C.byref(got)))
+            if len(self._needs) > 4096:
+                self._needs.clear()
+            need = self._needs[key] = got.value
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _ck(_fast("dsk_kv8_attn")(self._at, s, a, b, heads, self.dim_k ** -0.5 if scale is None else scale, window, keep_first, work.data_ptr(), need, _stream_of(torch, self.device)))
         return out
 
     def check(self):
@@ -1029,24 +1056,28 @@ def verify_drafts(logits, drafts, coins, probs=None, count=None, temperature: fl
     coins float32 [batch, drafts + 1] in [0, 1) (the last one draws), probs float32 [batch, drafts, vocab] of the draft model (none: the drafts are certain), count int32 [batch] drafts that
     exist.  Returns (accepted int32 [batch], tokens int32 [batch, drafts + 1]: the accepted drafts, the drawn token, -1 behind it)."""
     import torch
-    device = _device_of(logits)
-    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    if logits.dim() != 3 or logits.dtype not in types or logits.stride(2) != 1 and logits.shape[2] > 1:
+    device = logits.get_device()
+    if device < 0:
+        _no_device(logits)
+    i32, f32 = torch.int32, torch.float32
+    kind = {f32: 0, torch.float16: 1, torch.bfloat16: 2}.get(logits.dtype)
+    if logits.dim() != 3 or kind is None or logits.stride(2) != 1 and logits.shape[2] > 1:
         raise DskError(f"logits: float32, float16 or bfloat16 [batch, drafts + 1, vocab] with neighbouring entries is needed, got {logits.dtype} {tuple(logits.shape)}")
-    batch, n, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    batch, n, vocab = logits.shape
+    n -= 1
     if n < 0:
         raise DskError("logits of no row")
-    if probs is not None and (probs.shape != (batch, n, vocab) or probs.dtype != torch.float32 or _device_of(probs) != device or probs.stride(2) != 1 and vocab > 1):
+    if probs is not None and (probs.shape != (batch, n, vocab) or probs.dtype is not f32 or probs.get_device() != device or probs.stride(2) != 1 and vocab > 1):
         raise DskError(f"probs: float32 {(batch, n, vocab)} on cuda:{device} with neighbouring entries is needed, got {probs.dtype} {tuple(probs.shape)} on {probs.device}")
-    accepted, tokens = torch.empty(batch, dtype=torch.int32, device=logits.device), torch.empty((batch, n + 1), dtype=torch.int32, device=logits.device)
-    a = VerifyArgs(logits.data_ptr(), probs.data_ptr() if probs is not None and n else None, _dense("drafts", drafts, torch.int32, (batch, n), device),
-                   _dense("count", count, torch.int32, (batch,), device) if count is not None else None, _dense("coins", coins, torch.float32, (batch, n + 1), device),
-                   accepted.data_ptr(), tokens.data_ptr(), logits.stride(0), logits.stride(1), *((probs.stride(0), probs.stride(1)) if probs is not None else (0, 0)),
-                   device, batch, n, vocab, types[logits.dtype], temperature)
+    accepted, tokens = torch.empty(batch, dtype=i32, device=logits.device), torch.empty((batch, n + 1), dtype=i32, device=logits.device)
+    with_probs = probs is not None and n > 0
+    a = _VERIFY.pack(logits.data_ptr(), probs.data_ptr() if with_probs else 0, _dense("drafts", drafts, i32, (batch, n), device),
+                     0 if count is None else _dense("count", count, i32, (batch,), device), _dense("coins", coins, f32, (batch, n + 1), device), accepted.data_ptr(), tokens.data_ptr(),
+                     logits.stride(0), logits.stride(1), probs.stride(0) if with_probs else 0, probs.stride(1) if with_probs else 0, device, batch, n, vocab, kind, temperature)
     need = C.c_size_t(0)
-    _ck(lib().dsk_verify_workspace(a, need))
+    _ck(_fast("dsk_verify_workspace")(a, C.byref(need)))
     work = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
-    _ck(lib().dsk_verify(a, work.data_ptr(), need.value, _stream_of(torch, device)))
+    _ck(_fast("dsk_verify")(a, work.data_ptr(), need.value, _stream_of(torch, device)))
     return accepted, tokens
 
 

@@ -423,7 +423,7 @@ def test_refusals():
         odd = dsk.Cache8(2, 1, 24)
         odd.write(torch.zeros(1, 1, 1, 24, device=DEV), torch.zeros(1, 1, 1, 24, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV), ints([0]))
     v = dsk.View(x.data_ptr(), 3, 128, 128, 64)
-    s = cache._rows(c.t, ints([0]), None, 1)
+    s = dsk.Kv8Rows.from_buffer_copy(cache._rows(c.t, ints([0]), None, 1))
     assert dsk.lib().dsk_kv8_write(cache._c, s, v, v, None) != 0 and b"F32, F16 or BF16" in dsk.lib().dsk_last_error()
-    a, b = cache._view("q", q, q.shape), cache._view("o", q, q.shape)
+    a = b = dsk.View.from_buffer_copy(cache._view("q", q, q.shape))
     assert dsk.lib().dsk_kv8_attn(cache._c, s, a, b, 4, 1.0, 0, 0, None, 0, None) != 0 and b"workspace" in dsk.lib().dsk_last_error()

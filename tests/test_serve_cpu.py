@@ -107,6 +107,9 @@ def test_structures_have_the_compilers_layout(tmp_path):
     for _, p in names:
         want += [C.sizeof(p)] + [getattr(p, n).offset for n, _ in p._fields_]
     assert got == want
+    assert [dsk._ROWS.size, dsk._VIEW.size, dsk._VERIFY.size] == [C.sizeof(p) for p in (dsk.Kv8Rows, dsk.View, dsk.VerifyArgs)]      # (and as the calls pack them)
+    assert bytes(dsk.VerifyArgs(*range(1, 17), 0.5)) == dsk._VERIFY.pack(*range(1, 17), 0.5)
+    assert bytes(dsk.Kv8Rows(*range(1, 8)))[:44] == dsk._ROWS.pack(*range(1, 8))[:44] and bytes(dsk.View(1, 2, 3, 4, 5)) == dsk._VIEW.pack(1, 2, 3, 4, 5)
 
 
 # ---- the oracle ---------------------------------------------------------------------------------------------------------------------------------

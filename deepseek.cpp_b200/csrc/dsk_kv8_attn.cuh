@@ -28,7 +28,7 @@ struct Attn {
   const void* q;
   void* out;
   Pitch pq, po;
-  int heads, group, row_tiles, bf16, wide_q, wide_o, window, keep, shift;   // shift: log2 of the block
+  int heads, group, row_tiles, bf16, wide_q, wide_o, window, keep;
   float scale;                                               // times log2(e)
   long long* ends;                                           // workspace: [batch + 1] first units of the sequences (a head's row tile), and pieces
   float* part;
@@ -38,7 +38,7 @@ struct Attn {
 struct Seq { int len, count, kept, low, steps, units, first, last; };   // first, last: positions of the queries
 template <int STEP> __device__ __forceinline__ Seq sequence(const Attn& P, int b) {
   Seq q;
-  const long long room = (long long)P.S.table_blocks << P.shift;
+  const long long room = (long long)P.S.table_blocks << P.C.shift;
   const int len = P.S.first[b];
   q.count = P.S.count ? min(max(P.S.count[b], 0), P.S.rows) : P.S.rows;
   q.len = (int)min((long long)max(len, 0), room);
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     key = -1;
     if (ahead > 0 && s < at.q.steps) {
       key = (s < at.q.kept ? s : at.q.low + s - at.q.kept) * STEP;
-      page[0] = __ldg(at.table + (key >> P.shift));
-      if (HV == 2) page[HV - 1] = P.shift > 4 ? page[0] : key + 16 < at.q.len ? __ldg(at.table + (key >> 4) + 1) : 0;
+      page[0] = __ldg(at.table + (key >> P.C.shift));
+      if (HV == 2) page[HV - 1] = P.C.shift > 4 ? page[0] : key + 16 < at.q.len ? __ldg(at.table + (key >> 4) + 1) : 0;
     }
   };
   auto fetch = [&](int stage) {

@@ -114,7 +114,7 @@ struct Walk { int len, count, first, kept, low, begin, end, i0, i1; };   // firs
 __device__ __forceinline__ Walk walk_of(const Portion& P, int b, int row0, int share) {
   const Attn& A = P.A;
   Walk w;
-  const long long room = (long long)A.S.table_blocks << A.shift;
+  const long long room = (long long)A.S.table_blocks << A.C.shift;
   const int len = A.S.first[b];
   w.count = A.S.count ? min(max(A.S.count[b], 0), A.S.rows) : A.S.rows;
   w.first = len - w.count;
@@ -151,7 +151,7 @@ __device__ __forceinline__ void bring(const Attn& A, const Walk& w, int b, int h
     int p = -1;
     if (i < n && lane < 8) {
       const int key = key_of(w, w.begin + i) + 16 * lane;
-      if (key < w.len) p = __ldg(table + (key >> A.shift));
+      if (key < w.len) p = __ldg(table + (key >> A.C.shift));
     }
     return p;
   };
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   const Walk w = walk_of(P, b, row0, share);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     const long long len = A.S.first[b];
-    if (len < 0 || len > (long long)A.S.table_blocks << A.shift) note(A.C, ST_RANGE);
+    if (len < 0 || len > (long long)A.S.table_blocks << A.C.shift) note(A.C, ST_RANGE);
   }
   if (w.i0 >= w.count) return;                               // (the whole CTA: none of its rows exists)
   const int n = w.end - w.begin;
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
           if (sees_all(A, w, w.i0, w.i1, key0)) continue;
           for (int j = key0; j < min(key0 + kTile, min(w.len, pos + 1)); j++) {
             if (A.window > 0 && pos - j >= A.window && j >= A.keep) continue;
-            const int page = A.S.table[b * A.S.table_pitch + (j >> A.shift)];
+            const int page = A.S.table[b * A.S.table_pitch + (j >> A.C.shift)];
             if ((unsigned)page >= (unsigned)A.C.n_blocks) continue;
             const uint32_t* code = reinterpret_cast<const uint32_t*>(A.C.code[1] + (((size_t)page * A.C.heads + h) * A.C.block + (j & (A.C.block - 1))) * dv);
             for (int d = 0; d < dv / 4; d++) {

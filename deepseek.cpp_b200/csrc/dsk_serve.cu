@@ -117,7 +117,7 @@ bool wide(const dsk_view* v) {
   return aligned(v->data, 16) && v->batch % n == 0 && v->row % n == 0 && v->head % n == 0;
 }
 kv8::Cache cache_of(const dsk_kv8* c) {
-  return kv8::Cache{{static_cast<unsigned char*>(c->k), static_cast<unsigned char*>(c->v)}, {c->k_scale, c->v_scale}, c->status, c->n_blocks, c->block, c->kv_heads, {c->dim_k, c->dim_v}};
+  return kv8::Cache{{static_cast<unsigned char*>(c->k), static_cast<unsigned char*>(c->v)}, {c->k_scale, c->v_scale}, c->status, c->n_blocks, c->block, c->kv_heads, {c->dim_k, c->dim_v}, c->block == 16 ? 4 : c->block == 32 ? 5 : c->block == 64 ? 6 : 7};
 }
 kv8::Rows rows_of(const dsk_kv8_rows* s) { return kv8::Rows{s->table, s->table_pitch, s->first, s->count, s->table_blocks, s->batch, s->rows}; }
 kv8::Pitch pitch_of(const dsk_view* v) { return kv8::Pitch{v->batch, v->row, v->head}; }
@@ -126,17 +126,24 @@ unsigned touched(const dsk_kv8* c, const dsk_kv8_rows* s) {
   return (unsigned)std::min<long long>(s->table_blocks, ((long long)s->rows + c->block - 2) / c->block + 1);
 }
 
-template <typename T> int write_as(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, cudaStream_t stream) {
+template <typename T, bool WIDE> int write_as(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, cudaStream_t stream) {
   const dim3 grid(touched(c, s), 2 * c->kv_heads, s->batch);
   const T *pk = static_cast<const T*>(k->data), *pv = static_cast<const T*>(v->data);
-  const int w = wide(k) && wide(v), eights = std::min(s->rows, c->block) * std::max(c->dim_k, c->dim_v) / 8;
-  // a CTA's values stay in registers: a warp of four eights a lane for a few rows (no barrier), otherwise as few threads as hold them
-  if (eights <= 128) kv8::write_rows<T, 32, 4><<<grid, 32, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
-  else if (eights <= 1024) kv8::write_rows<T, 128, 8><<<grid, 128, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
-  else if (eights <= 2048) kv8::write_rows<T, 256, 8><<<grid, 256, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
-  else kv8::write_rows<T, 256, 16><<<grid, 256, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v), w);
+  const int eights = std::min(s->rows, c->block) * std::max(c->dim_k, c->dim_v) / 8;
+  // a CTA's values stay in registers: a warp of four eights a lane for a few rows (no barrier), otherwise few threads with many (what a thread does once, addresses for the most part,
+  // is 200 instructions; twice the threads with half the eights: 98 us for four prompts of 8191 tokens)
+#define WRITE(TH, R) kv8::write_rows<T, TH, R, WIDE><<<grid, TH, 0, stream>>>(cache_of(c), rows_of(s), pk, pv, pitch_of(k), pitch_of(v))
+  if (eights <= 128) WRITE(32, 4);
+  else if (eights <= 512) WRITE(64, 8);
+  else if (eights <= 1024) WRITE(64, 16);
+  else if (eights <= 2048) WRITE(128, 16);
+  else WRITE(256, 16);
+#undef WRITE
   CK(cudaGetLastError());
   return 0;
+}
+template <typename T> int write_as(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, cudaStream_t stream) {
+  return wide(k) && wide(v) ? write_as<T, true>(c, s, k, v, stream) : write_as<T, false>(c, s, k, v, stream);
 }
 template <typename T> int read_as(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, cudaStream_t stream) {
   const dim3 grid(touched(c, s), 2 * c->kv_heads, s->batch);
@@ -252,7 +259,7 @@ extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
   P.C = cache_of(c); P.S = rows_of(s);
   P.q = q->data; P.out = out->data; P.pq = pitch_of(q); P.po = pitch_of(out);
   P.heads = heads; P.group = heads / c->kv_heads; P.row_tiles = L.row_tiles; P.bf16 = dt == DSK_DT_BF16; P.wide_q = wide(q); P.wide_o = wide(out);
-  P.window = window; P.keep = keep_first; P.shift = c->block == 16 ? 4 : c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
+  P.window = window; P.keep = keep_first;
   P.scale = scale * 1.44269504088896340736f;
   P.ends = static_cast<long long*>(workspace);
   P.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.ends);

@@ -20,6 +20,7 @@ namespace kv8 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxBatch = 1024;
 __host__ __device__ constexpr int step_of(int qt) { return qt < 4 ? 32 : 16; }   // keys of a warp's step
+__device__ __forceinline__ long long quotient(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }   // (of numbers >= 0)
 constexpr float kSlack = 8.f;                                // the reference of a row's weights follows its maximum once that is 2^8 ahead
 
 struct Attn {
@@ -30,8 +31,7 @@ struct Attn {
   Pitch pq, po;
   int heads, group, row_tiles, bf16, wide_q, wide_o, window, keep;
   float scale;                                               // times log2(e)
-  long long* ends;                                           // workspace: [batch + 1] first units of the sequences (a head's row tile), and pieces
-  float* part;
+  float* part;                                               // workspace: pieces
 };
 
 // What a sequence has: visible steps are the first `kept` ones and those from `low` on
@@ -104,6 +104,12 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {   // 0xff where a by
   return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
 }
 
+// CTAs that share the line out: where each (sequence, head, tile) has several, as many to each, so that those of equal length have whole pieces
+__device__ __forceinline__ long long ctas_of(int grid, long long total, long long each) {
+  const long long n = 2 * each <= grid ? grid / (int)each * each : grid;
+  return min(n, total);
+}
+
 // A place in the line of units
 template <int STEP> struct Place {
   Seq q;
@@ -119,7 +125,7 @@ template <int STEP> struct Place {
     table = P.S.table + b * P.S.table_pitch;
     q = sequence<STEP>(P, b);
     const long long in = x - ends[b] * per;
-    const int hr = (int)(in / q.units);
+    const int hr = (int)quotient(in, q.units);
     unit = (int)(in - (long long)hr * q.units);
     head = hr / P.row_tiles;
     tile = hr - head * P.row_tiles;
@@ -198,17 +204,15 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     __syncthreads();
   }
   const int per = P.C.heads * P.row_tiles;
-  const long long total = run * per, N = min((long long)gridDim.x, total);
+  const long long total = run * per, N = ctas_of(gridDim.x, total, (long long)B * per);
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b < B; b += kThreads) {
-      P.ends[b] = ends[b];
       const long long len = P.S.first[b];
       if (len < 0 || len > (long long)P.S.table_blocks * P.C.block) note(P.C, ST_RANGE);
     }
-    if (threadIdx.x == 0) P.ends[B] = run;
   }
   if ((long long)blockIdx.x >= N) return;
-  const long long x0 = blockIdx.x * total / N, x1 = (blockIdx.x + 1) * total / N;
+  const long long x0 = quotient(blockIdx.x * total, N), x1 = quotient((blockIdx.x + 1) * total, N);
   __syncthreads();
   const int dk = P.C.dim[0], dv = P.C.dim[1], dk16 = dk / 16, dv16 = dv / 16, mine = (int)(x1 - x0);
   const bool exact = dk == DK && dv == DV;
@@ -261,13 +265,26 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     look();
   };
   look();
+  Place<STEP> pl = at;                                       // of the step that is computed
+  uint32_t qv[QT * 2][DK / 64];                              // a piece's query rows on their way, two entries a lane
+  auto load_queries = [&]() {
+#pragma unroll
+    for (int u = 0; u < QT * 2; u++) {
+      const int row = pl.tile * QT * 8 + u * kWarps + warp, i = row / P.group;
+      const uint16_t* src = static_cast<const uint16_t*>(P.q) + pl.b * P.pq.batch + i * P.pq.row + (long long)(pl.head * P.group + row - i * P.group) * P.pq.head + lane * 2;
+#pragma unroll
+      for (int k = 0; k < DK / 64; k++) {
+        qv[u][k] = 0;
+        if (i < pl.q.count && k * 64 + lane * 2 < dk) qv[u][k] = P.wide_q ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 64)) : src[k * 64] | (uint32_t)src[k * 64 + 1] << 16;
+      }
+    }
+  };
+  load_queries();
 #pragma unroll 1
   for (int i = 0; i < NST - 1; i++) fetch(i);
 
   float o[QT][NO][4], m[QT][2], l[QT][2], fq[QT][2];         // a lane's queries: 2 c and 2 c + 1 of a tile; fq: factor of their scores
   uint32_t qf[QREG ? QT : 1][QREG ? DK / 16 : 1][2];
-  Place<STEP> pl;
-  pl.find(P, ends, x0, per);
   int begun = pl.unit, stage = 0;                            // the piece's first unit
   bool fresh = true;
 #pragma unroll 1
@@ -276,17 +293,7 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     const int head = pl.head, row0 = pl.tile * QT * 8;
     if (fresh) {                                             // query rows as fp16, each by its own power of two
       __syncthreads();
-      uint32_t qv[QT * 2][DK / 64];
-#pragma unroll
-      for (int u = 0; u < QT * 2; u++) {
-        const int row = row0 + u * kWarps + warp, i = row / P.group;
-        const uint16_t* src = static_cast<const uint16_t*>(P.q) + pl.b * P.pq.batch + i * P.pq.row + (long long)(head * P.group + row - i * P.group) * P.pq.head + lane * 2;
-#pragma unroll
-        for (int k = 0; k < DK / 64; k++) {
-          qv[u][k] = 0;
-          if (i < q.count && k * 64 + lane * 2 < dk) qv[u][k] = P.wide_q ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 64)) : src[k * 64] | (uint32_t)src[k * 64 + 1] << 16;
-        }
-      }
+      if (y > 0) load_queries();
 #pragma unroll
       for (int u = 0; u < QT * 2; u++) {
         const int row = u * kWarps + warp;
@@ -606,13 +613,24 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
 template <int DV, int QT>
 __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
   constexpr int NO = DV / 16, VCH = DV >= 128 ? 16 : 8;
-  grid_wait();
+  // who had what is known without the kernel ahead
+  __shared__ long long sums[2][QT * DV / 32];
   const int b = blockIdx.y, hr = blockIdx.x, per = gridDim.x;
-  const long long total = P.ends[P.S.batch] * per, units = P.ends[b + 1] - P.ends[b];
-  if (units == 0) return;
-  const long long N = min((long long)ctas, total), u0 = P.ends[b] * per + hr * units;
-  const int i0 = (int)(((u0 + 1) * N + total - 1) / total) - 1, i1 = (int)(((u0 + units) * N + total - 1) / total) - 1;   // the CTAs of its first and last unit
+  long long before = 0, all = 0;
+  for (int i = threadIdx.x; i < P.S.batch; i += QT * DV) { const int u = sequence<step_of(QT)>(P, i).units; all += u; if (i < b) before += u; }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) { before += __shfl_xor_sync(0xffffffffu, before, o); all += __shfl_xor_sync(0xffffffffu, all, o); }
+  if ((threadIdx.x & 31) == 0) { sums[0][threadIdx.x >> 5] = before; sums[1][threadIdx.x >> 5] = all; }
+  __syncthreads();
+  before = all = 0;
+#pragma unroll
+  for (int i = 0; i < QT * DV / 32; i++) { before += sums[0][i]; all += sums[1][i]; }
+  const Seq q = sequence<step_of(QT)>(P, b);
+  const long long units = q.units, total = all * per, N = ctas_of(ctas, total, (long long)P.S.batch * per), u0 = before * per + hr * units;
+  const int i0 = units ? (int)quotient((u0 + 1) * N + total - 1, total) - 1 : 0, i1 = units ? (int)quotient((u0 + units) * N + total - 1, total) - 1 : 0;   // the CTAs of its first and last unit
   if (i0 == i1) return;
+  const int own = quotient(i0 * total, N) >= u0 ? 0 : 1;     // the first one's piece: its first or its last (the others' pieces are their first)
+  grid_wait();
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   int w = threadIdx.x >> 5;
   const int e = w & 1;
@@ -626,7 +644,7 @@ __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       if (i + u > i1) { pm[u] = -INFINITY; continue; }
-      const float* from = P.part + (size_t)(2 * (i + u) + ((i + u) * total / N >= u0 ? 0 : 1)) * (QT * (NO * 128 + 16));
+      const float* from = P.part + (size_t)(2 * (i + u) + (i + u == i0 ? own : 0)) * (QT * (NO * 128 + 16));
       pm[u] = from[QT * NO * 128 + row];
       pl[u] = from[QT * NO * 128 + QT * 8 + row];
 #pragma unroll
@@ -647,7 +665,7 @@ __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
     }
   }
   const int head = hr / P.row_tiles, row0 = (hr - head * P.row_tiles) * QT * 8;
-  Out::store(P, sequence<step_of(QT)>(P, b), b, head, row0 + row, k0 / VCH * 128 + r * VCH + k0 % VCH, 8, x, l == 0.f ? 0.f : 1.f / l);
+  Out::store(P, q, b, head, row0 + row, k0 / VCH * 128 + r * VCH + k0 % VCH, 8, x, l == 0.f ? 0.f : 1.f / l);
 }
 
 }  // namespace kv8

@@ -153,7 +153,7 @@ template <typename T> int read_as(const dsk_kv8* c, const dsk_kv8_rows* s, const
 }
 
 // How an attention call is laid out
-struct Layout { int shape, tiles, row_tiles, ctas, shares; size_t ends, bytes; };   // shares > 0: attend_rows
+struct Layout { int shape, tiles, row_tiles, ctas, shares; size_t bytes; };   // shares > 0: attend_rows
 constexpr int kPortionRows = 32;                             // query rows of a key head from which on attend_rows has them
 constexpr int kShapes[4][2] = {{64, 64}, {128, 128}, {192, 128}, {256, 256}};
 int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, Layout* L) {
@@ -170,17 +170,15 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, Layout* L) {
     L->row_tiles = (int)((rows + kv8::kRows - 1) / kv8::kRows);
     const long long tiles = (long long)s->batch * c->kv_heads * L->row_tiles;
     L->shares = (int)std::max<long long>(1, std::min<long long>(sms / tiles, (keys + kv8::kTile - 1) / kv8::kTile));   // where the row tiles leave SMs idle, their keys are shared out
-    L->ends = 0;
     L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * kv8::kRows * (kShapes[L->shape][1] + 2) * sizeof(float) : 16;
     return 0;
   }
-  L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
+  L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : rows <= 24 ? 3 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
   L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
   const int unit = kv8::kWarps * kv8::step_of(L->tiles);
   const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * ((keys + unit - 1) / unit + 1);
   L->ctas = (int)std::min<long long>(2 * sms, std::max<long long>(1, units));
-  L->ends = ((size_t)(s->batch + 1) * sizeof(long long) + 15) / 16 * 16;
-  L->bytes = L->ends + (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 16 * 128 + 16) * sizeof(float);
+  L->bytes = (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 16 * 128 + 16) * sizeof(float);
   return 0;
 }
 template <int DK, int DV, int QT> int attend_as(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
@@ -202,7 +200,10 @@ template <int DK, int DV> int attend_portion(const kv8::Attn& A, const Layout& L
 template <int DK, int DV> int attend_tiles(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
   if constexpr (DV < 256) if (L.shares) return attend_portion<DK, DV>(P, L, device, stream);
   if (L.tiles == 1) return attend_as<DK, DV, 1>(P, L, device, stream);
-  if constexpr (DV < 256) if (L.tiles == 4) return attend_as<DK, DV, 4>(P, L, device, stream);
+  if constexpr (DV < 256) {
+    if (L.tiles == 3) return attend_as<DK, DV, 3>(P, L, device, stream);
+    if (L.tiles == 4) return attend_as<DK, DV, 4>(P, L, device, stream);
+  }
   return attend_as<DK, DV, 2>(P, L, device, stream);
 }
 }  // namespace
@@ -261,8 +262,7 @@ extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
   P.heads = heads; P.group = heads / c->kv_heads; P.row_tiles = L.row_tiles; P.bf16 = dt == DSK_DT_BF16; P.wide_q = wide(q); P.wide_o = wide(out);
   P.window = window; P.keep = keep_first;
   P.scale = scale * 1.44269504088896340736f;
-  P.ends = static_cast<long long*>(workspace);
-  P.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.ends);
+  P.part = static_cast<float*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (L.shape) {
     case 0: return attend_tiles<64, 64>(P, L, c->device, st);

@@ -221,10 +221,18 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
 
   // copies: a step of this warp to a unit, from a block whose number was looked up a unit ahead; 16-byte pieces lane, lane + 32, .. of a step's rows, which lie side by side
   uint32_t to_k[DK / 32], to_v[DV / 32];
+  {
+    int row = lane / dk16, col = lane - row * dk16;
+    const int dr = 32 / dk16, dc = 32 - dr * dk16;
 #pragma unroll
-  for (int j = 0; j < DK / 32; j++) { const int i = lane + 32 * j, row = i / dk16; to_k[j] = row * KS + (i - row * dk16) * 16; }
+    for (int j = 0; j < DK / 32; j++) { to_k[j] = row * KS + col * 16; row += dr; col += dc; if (col >= dk16) { col -= dk16; row++; } }
+  }
+  {
+    int row = lane / dv16, col = lane - row * dv16;
+    const int dr = 32 / dv16, dc = 32 - dr * dv16;
 #pragma unroll
-  for (int j = 0; j < DV / 32; j++) { const int i = lane + 32 * j, row = i / dv16; to_v[j] = STEP * KS + row * VS + (i - row * dv16) * 16; }
+    for (int j = 0; j < DV / 32; j++) { to_v[j] = STEP * KS + row * VS + col * 16; row += dr; col += dc; if (col >= dv16) { col -= dv16; row++; } }
+  }
   Place<STEP> at;                                            // of the next copies
   at.find(P, ends, x0, per);
   int ahead = mine, page[HV], key = -1;                      // units that are not under way yet; the next step's blocks (of 16 keys each) and first key (-1: this warp has none)

@@ -4,8 +4,8 @@
 // of 128.  Roles: seven warps bring codes from the cache, four the keys' and three the values', turn them into fp16 (exact) and store them as swizzled operands, so that the cache
 // crosses HBM and L2 as bytes; one thread
 // issues the products, scores into TMEM, weights from TMEM; two groups of four warps have the softmax, a thread to a row, each group for its own tile, so that one tile's products run under the
-// other one's softmax.  Scales and weights as in dsk_kv8_attn.cuh: key scales on the scores, value scales inside the exponent, fp16 weights of at most 2^kSlack.
-// The results stay in TMEM; they are scaled again only where a row's maximum has moved by more than 2^kSlack, by the thread that has the row.  Weights lie where the scores were:
+// other one's softmax.  Scales and weights as in dsk_kv8_attn.cuh: key scales on the scores, value scales inside the exponent, fp16 weights of at most 2^kLag.
+// The results stay in TMEM; they are scaled again only where a row's maximum is 2^kLag ahead of the reference of its weights, by the thread that has the row.  Weights lie where the scores were:
 // a tile's next scores wait for the product that reads its weights.
 // NaN among values: a tile that some row does not see whole goes to the products with zeros in their place, and rows that do see one get it back at the end.
 #pragma once
@@ -17,6 +17,7 @@ namespace dsk {
 namespace kv8 {
 
 constexpr int kTile = 128, kRows = 256, kRowThreads = 512, kSlots = 4;       // keys of a tile; rows and threads of a CTA; tiles whose scales are held
+constexpr float kLag = 14.f;                                 // a row's weights are at most 2^kLag
 
 struct Portion {
   Attn A;                                                    // row_tiles: of kRows rows
@@ -403,24 +404,25 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
     bool ok = true;
     for (int i = 0; i < n; i++) {
       const int slot = i % kSlots, key0 = key_of(w, w.begin + i);
-      ok = wait_warp(cfull + 8 * slot, (i / kSlots) & 1, A.C) && wait_warp(sfull + 8 * t, i & 1, A.C);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      ok = wait_warp(cfull + 8 * slot, (i / kSlots) & 1, A.C);
       const float4* sc = reinterpret_cast<const float4*>(scales + slot * 24);   // key scales of 16 keys each [8], exponents of their value scales [8], reciprocals of those [8] (zero: not there)
       const float4 there[2] = {sc[4], sc[5]};
       const bool masked = there[0].x == 0.f || there[0].y == 0.f || there[0].z == 0.f || there[0].w == 0.f || there[1].x == 0.f || there[1].y == 0.f || there[1].z == 0.f || there[1].w == 0.f ||
                           !sees_all(A, w, r_first, r_last, key0);
-      // half a row of scores in registers at a time: the first half for the maximum, the second one for the maximum and its weights, the first one again for its weights
-      float top = -INFINITY;
+      ok = ok && wait_warp(sfull + 8 * t, i & 1, A.C);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      // Half a row of scores in registers at a time, each read once: the reference may lag behind the maximum by kLag, within fp16's range, so that the first half's weights do not wait for
+      // the second half's maximum; where that moves the reference after all, weights that are stored already are scaled again, exactly, since references are whole numbers.
 #pragma unroll 1
-      for (int pass = 0; pass < 3; pass++) {
-        const int half = pass == 1, c = half * 64;
+      for (int half = 1; half >= 0; half--) {
+        const int c = half * 64;
         const float4 k4 = sc[half], l4 = sc[2 + half];
         const float fs[4] = {factor(k4.x), factor(k4.y), factor(k4.z), factor(k4.w)}, lift[4] = {l4.x, l4.y, l4.z, l4.w};
         uint32_t x[64];
         tmem_read64(s_at + c, x);
         if (masked) {                                        // keys that the row sees, a bit each: not behind its own, in the window or among the first, in the cache
-          const float4 back = sc[4 + half];
+          const float4 back = half ? there[1] : there[0];
 #pragma unroll
           for (int u = 0; u < 64; u += 32) {
             const int j = key0 + c + u, window = A.window > 0 ? pos - A.window + 1 - j : 0;
@@ -431,33 +433,42 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
             for (int k = 0; k < 32; k++) if (!(see >> k & 1)) x[u + k] = 0xff800000u;
           }
         }
-        if (pass < 2) {
+        float top = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < 4; g++) {
-            float y[5];
+        for (int g = 0; g < 4; g++) {
+          float y[5];
 #pragma unroll
-            for (int k = 0; k < 5; k++) y[k] = max3(x[16 * g + 3 * k], x[16 * g + 3 * k + 1], x[16 * g + 3 * k + 2]);
-            const float z = max3(__float_as_uint(max3(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]))), __float_as_uint(fmaxf(y[3], y[4])), x[16 * g + 15]);
-            top = fmaxf(top, fmaf(z, fs[g], lift[g]));
-          }
-          if (pass == 0) continue;
-          if (__any_sync(0xffffffffu, top > m + kSlack)) {
-            const float to = fmaxf(m, top), by = exp2_fast(m - to);
-            m = to;
-            l *= by;
-            if (i > 0) {                                     // (the tile's last product was through ahead of these scores)
+          for (int k = 0; k < 5; k++) y[k] = max3(x[16 * g + 3 * k], x[16 * g + 3 * k + 1], x[16 * g + 3 * k + 2]);
+          const float z = max3(__float_as_uint(max3(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]))), __float_as_uint(fmaxf(y[3], y[4])), x[16 * g + 15]);
+          top = fmaxf(top, fmaf(z, fs[g], lift[g]));
+        }
+        if (__any_sync(0xffffffffu, top > m + kLag)) {
+          const float to = fmaxf(m, ceilf(top)), by = exp2_fast(m - to);
+          m = to;
+          l *= by;
+          if (i > 0) {                                       // (the tile's last product was through ahead of these scores)
 #pragma unroll 1
-              for (int d = 0; d < DV; d += 16) {
-                uint32_t y[16];
-                tmem_read16(res + d, y);
+            for (int d = 0; d < DV; d += 16) {
+              uint32_t y[16];
+              tmem_read16(res + d, y);
 #pragma unroll
-                for (int k = 0; k < 16; k++) y[k] = __float_as_uint(__uint_as_float(y[k]) * by);
-                tmem_store16(res + d, y);
-              }
+              for (int k = 0; k < 16; k++) y[k] = __float_as_uint(__uint_as_float(y[k]) * by);
+              tmem_store16(res + d, y);
+            }
+          }
+          if (half == 0) {
+            const __half2 by2 = __float2half2_rn(by);
+#pragma unroll 1
+            for (int d = 0; d < 32; d += 16) {
+              uint32_t y[16];
+              tmem_read16(s_at + 64 + d, y);
+#pragma unroll
+              for (int k = 0; k < 16; k++) { const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&y[k]), by2); y[k] = *reinterpret_cast<const uint32_t*>(&v); }
+              tmem_store16(s_at + 64 + d, y);
             }
           }
         }
-        const float4 b4 = sc[4 + half];
+        const float4 b4 = half ? there[1] : there[0];
         const float back[4] = {b4.x, b4.y, b4.z, b4.w};
         uint32_t p[32];                                      // weights of a half lie in the first 32 of its columns
 #pragma unroll

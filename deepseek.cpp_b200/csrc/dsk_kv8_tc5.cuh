@@ -30,22 +30,16 @@ template <int DK, int DV> __host__ __device__ constexpr int rows_smem() {
   return 1024 + kRows * DK * 2 + k_stages<DK, DV>() * kTile * DK * 2 + v_stages<DK, DV>() * kTile * DV * 2 + kSlots * 3 * 8 * 4 + 256;
 }
 
-// Bounded.  A poll sleeps until the phase is through, up to the time that it is given: polls that return at once take the issue slots of the warps that work (13300 instead of 8000
-// instructions to a tile of keys).
-__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000000u) : "memory");
-  return ok != 0;
-}
+// Bounded.  (Polls that are given a time to sleep wake some 100 cycles late.)
 __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* status) {
   const long long from = clock64();
   do {
-    if (poll(bar, parity)) return true;
+    if (hy::tc_poll(bar, parity)) return true;
   } while (clock64() - from < hy::kTcWaitCycles);
   if (status) atomicOr(status, ST_WAIT);
   return false;
 }
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Cache& C) { return poll(bar, parity) || wait_long(bar, parity, C.status); }
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Cache& C) { return hy::tc_poll(bar, parity) || wait_long(bar, parity, C.status); }
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const Cache& C) { return __all_sync(0xffffffffu, wait_bar(bar, parity, C)); }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -261,7 +255,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   unsigned char* gbase = raw + (base - smem_u32(raw));
   const uint32_t qs = base, ks = qs + kRows * DK * 2, vs = ks + KST * KB, cs = vs + VST * VB, bars = cs + kSlots * 3 * 8 * 4;
   float* scales = reinterpret_cast<float*>(gbase + (cs - base));          // [slot][key scale | exponent of the value scale | its reciprocal, zero: not there][16 keys]
-  const uint32_t kfull = bars, kempty = bars + 24, vfull = bars + 48, vempty = bars + 72, sfull = bars + 96, pfull = bars + 112, pvdone = bars + 128, cfull = bars + 144, cdone = bars + 176, flushed = bars + 184;
+  const uint32_t kfull = bars, kempty = bars + 24, vfull = bars + 48, vempty = bars + 72, sfull = bars + 96, pfull = bars + 112, pvdone = bars + 128, cfull = bars + 144, cdone = bars + 176, flushed = bars + 184, qfull = bars + 192;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int h = blockIdx.x / P.shares, share = blockIdx.x - h * P.shares, b = blockIdx.z, row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kRows;   // late rows, which see most, first
   const Walk w = walk_of(P, b, row0, share);
@@ -276,6 +270,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
     for (int i = 0; i < 2; i++) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); }
     for (int i = 0; i < kSlots; i++) mbar_init(cfull + 8 * i, 1);
     mbar_init(cdone, 3);
+    mbar_init(qfull, 8);
     mbar_init(flushed, 1);
     nan_seen = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -285,53 +280,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   const int dk = A.C.dim[0], dv = A.C.dim[1];
-  // query rows as fp16, two threads to a row, each by its own power of two (dsk_kv8_attn.cuh)
-  float row_scale = 0.f;                                     // of the row that this thread has in the softmax
-  {
-    const int row = threadIdx.x >> 1, half = threadIdx.x & 1, i = (row0 + row) / A.group;
-    const uint16_t* src = static_cast<const uint16_t*>(A.q) + b * A.pq.batch + (long long)i * A.pq.row + (long long)(h * A.group + row0 + row - i * A.group) * A.pq.head;
-    const bool there = i < w.count;
-    float top = 0.f;
-    auto eight = [&](int d, uint32_t (&x)[4]) {
-      x[0] = x[1] = x[2] = x[3] = 0;
-      if (there && d < dk) {
-        if (A.wide_q) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + d)); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-        else
-#pragma unroll
-          for (int u = 0; u < 4; u++) x[u] = src[d + 2 * u] | (uint32_t)src[d + 2 * u + 1] << 16;
-      }
-    };
-    auto pair = [&](uint32_t x) { return A.bf16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&x)); };
-    for (int d = half * 8; d < DK; d += 16) {
-      uint32_t x[4];
-      eight(d, x);
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const float2 f = pair(x[u]);
-        const float a = fabsf(f.x), c = fabsf(f.y);
-        top = fmaxf(top, fmaxf(a < INFINITY ? a : 0.f, c < INFINITY ? c : 0.f));
-      }
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    const int e = top > 0.f ? max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127 - 10)) : 0;
-    const float by = A.scale < 0.f ? -pow2(-e) : pow2(-e);
-    for (int d = half * 8; d < DK; d += 16) {
-      uint32_t x[4];
-      eight(d, x);
-#pragma unroll
-      for (int u = 0; u < 4; u++) { const float2 f = pair(x[u]); x[u] = halves(f.x * by, f.y * by); }
-      const int tile = row >> 7, rr = row & 127;             // [tile][64 entries][row], 16-byte pieces swizzled
-      sts128(qs + tile * (kTile * DK * 2) + (d >> 6) * (kTile * 128) + rr * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4), x[0], x[1], x[2], x[3]);
-    }
-    // rows' factors on their way to the softmax's threads, through memory that nobody uses yet
-    __syncthreads();
-    float* f = reinterpret_cast<float*>(gbase + (vs - base));               // (the first values come behind the barrier below)
-    if (half == 0) f[row] = pow2(e) * fabsf(A.scale);
-    __syncthreads();
-    if (warp < 8) row_scale = f[threadIdx.x];
-    __syncthreads();
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -350,7 +298,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
           for (int u = 0; u < 4; u++) mma_ss(tmem + t * 128, a + g * (kTile * 128 >> 4) + 2 * u, k + g * (kTile * 128 >> 4) + 2 * u, sdesc, g > 0 || u > 0, lead);
         commit(sfull + 8 * t, lead);
       };
-      bool alive = n > 0 && wait_warp(kfull, 0, A.C);
+      bool alive = n > 0 && wait_warp(qfull, 0, A.C) && wait_warp(kfull, 0, A.C);
       if (alive) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         score(0, 0);
@@ -399,6 +347,51 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
     const int t = warp >> 2, quad = warp & 3, row = row0 + threadIdx.x, i_row = row / A.group, pos = w.first + i_row;
     const int r_first = (row0 + t * 128) / A.group, r_last = min((row0 + t * 128 + 127) / A.group, w.i1);   // tokens of the tile's rows
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_at = tmem + t * 128 + lanes, res = o_at + t * 128 + lanes;
+    // the thread's query row as fp16, by a power of two of its own (dsk_kv8_attn.cuh), while the first keys are brought: [tile][64 entries][row], 16-byte pieces swizzled
+    float row_scale;
+    {
+      const uint16_t* src = static_cast<const uint16_t*>(A.q) + b * A.pq.batch + (long long)i_row * A.pq.row + (long long)(h * A.group + row - i_row * A.group) * A.pq.head;
+      const bool there = i_row < w.count;
+      uint4 x[DK / 8];
+#pragma unroll
+      for (int d = 0; d < DK / 8; d++) {
+        x[d] = make_uint4(0, 0, 0, 0);
+        if (there && d * 8 < dk) {
+          if (A.wide_q) x[d] = __ldg(reinterpret_cast<const uint4*>(src) + d);
+          else x[d] = make_uint4(src[8 * d] | (uint32_t)src[8 * d + 1] << 16, src[8 * d + 2] | (uint32_t)src[8 * d + 3] << 16, src[8 * d + 4] | (uint32_t)src[8 * d + 5] << 16,
+                                 src[8 * d + 6] | (uint32_t)src[8 * d + 7] << 16);
+        }
+      }
+      uint32_t top = 0;                                      // the largest number's bits, whose order is that of the magnitudes
+      const uint32_t inf = A.bf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+      for (int d = 0; d < DK / 8; d++) {
+        const uint32_t y[4] = {x[d].x, x[d].y, x[d].z, x[d].w};
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const uint32_t lo = y[u] & 0x7fffu, hi = (y[u] >> 16) & 0x7fffu;
+          top = max(top, max(lo < inf ? lo : 0u, hi < inf ? hi : 0u));
+        }
+      }
+      const float most = A.bf16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
+      const int e = most > 0.f ? max(-100, min(100, (int)(__float_as_uint(most) >> 23) - 127 - 10)) : 0;
+      const float by = A.scale < 0.f ? -pow2(-e) : pow2(-e);                 // (factors of scores are positive)
+      row_scale = pow2(e) * fabsf(A.scale);
+      const uint32_t to = qs + t * (kTile * DK * 2) + (threadIdx.x & 127) * 128;
+#pragma unroll
+      for (int d = 0; d < DK / 8; d++) {
+        uint32_t y[4] = {x[d].x, x[d].y, x[d].z, x[d].w};
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const float2 f = A.bf16 ? make_float2(__uint_as_float(y[u] << 16), __uint_as_float(y[u] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&y[u]));
+          y[u] = halves(f.x * by, f.y * by);
+        }
+        sts128(to + (d >> 3) * (kTile * 128) + (((d & 7) ^ (threadIdx.x & 7)) << 4), y[0], y[1], y[2], y[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) hy::tc_arrive(qfull);
+    }
     auto factor = [&](float key_scale) { return fmaxf(row_scale * key_scale, 1.17549435e-38f); };   // (positive: -inf stays what it is)
     float m = -1e30f, l = 0.f;
     bool ok = true;
@@ -409,6 +402,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       const float4 there[2] = {sc[4], sc[5]};
       const bool masked = there[0].x == 0.f || there[0].y == 0.f || there[0].z == 0.f || there[0].w == 0.f || there[1].x == 0.f || there[1].y == 0.f || there[1].z == 0.f || there[1].w == 0.f ||
                           !sees_all(A, w, r_first, r_last, key0);
+      float fs[4], lift[4];
+      auto scales_of = [&](int half) {
+        const float4 k4 = sc[half], l4 = sc[2 + half];
+        fs[0] = factor(k4.x); fs[1] = factor(k4.y); fs[2] = factor(k4.z); fs[3] = factor(k4.w);
+        lift[0] = l4.x; lift[1] = l4.y; lift[2] = l4.z; lift[3] = l4.w;
+      };
+      scales_of(1);
       ok = ok && wait_warp(sfull + 8 * t, i & 1, A.C);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -417,8 +417,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
 #pragma unroll 1
       for (int half = 1; half >= 0; half--) {
         const int c = half * 64;
-        const float4 k4 = sc[half], l4 = sc[2 + half];
-        const float fs[4] = {factor(k4.x), factor(k4.y), factor(k4.z), factor(k4.w)}, lift[4] = {l4.x, l4.y, l4.z, l4.w};
         uint32_t x[64];
         tmem_read64(s_at + c, x);
         if (masked) {                                        // keys that the row sees, a bit each: not behind its own, in the window or among the first, in the cache
@@ -487,6 +485,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
           l = fmaf(__uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)), back[g], l);
         }
         tmem_store32(s_at + c, p);
+        if (half) scales_of(0);
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -1051,6 +1051,9 @@ class Cache8:
             raise DskError("8-bit cache: " + ", ".join(t for b, t in ((1, "a block number outside the cache"), (2, "tokens outside the table"), (4, "a wait inside a kernel gave up")) if bits & b))
 
 
+_verify_needs = {}                   # bytes of the workspace by shape of the call
+
+
 def verify_drafts(logits, drafts, coins, probs=None, count=None, temperature: float = 1.0):
     """Verification of drafted tokens (dsk_verify, include/dsk.h): logits [batch, drafts + 1, vocab] of the model at the last token and behind every draft, drafts int32 [batch, drafts],
     coins float32 [batch, drafts + 1] in [0, 1) (the last one draws), probs float32 [batch, drafts, vocab] of the draft model (none: the drafts are certain), count int32 [batch] drafts that
@@ -1074,10 +1077,15 @@ def verify_drafts(logits, drafts, coins, probs=None, count=None, temperature: fl
     a = _VERIFY.pack(logits.data_ptr(), probs.data_ptr() if with_probs else 0, _dense("drafts", drafts, i32, (batch, n), device),
                      0 if count is None else _dense("count", count, i32, (batch,), device), _dense("coins", coins, f32, (batch, n + 1), device), accepted.data_ptr(), tokens.data_ptr(),
                      logits.stride(0), logits.stride(1), probs.stride(0) if with_probs else 0, probs.stride(1) if with_probs else 0, device, batch, n, vocab, kind, temperature)
-    need = C.c_size_t(0)
-    _ck(_fast("dsk_verify_workspace")(a, C.byref(need)))
-    work = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
-    _ck(_fast("dsk_verify")(a, work.data_ptr(), need.value, _stream_of(torch, device)))
+    need = _verify_needs.get((batch, n, vocab))
+    if need is None:
+        got = C.c_size_t(0)
+        _ck(_fast("dsk_verify_workspace")(a, C.byref(got)))
+        if len(_verify_needs) > 4096:
+            _verify_needs.clear()
+        need = _verify_needs[batch, n, vocab] = got.value
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    _ck(_fast("dsk_verify")(a, work.data_ptr(), need, _stream_of(torch, device)))
     return accepted, tokens
 
 

@@ -427,3 +427,128 @@ def test_refusals():
     assert dsk.lib().dsk_kv8_write(cache._c, s, v, v, None) != 0 and b"F32, F16 or BF16" in dsk.lib().dsk_last_error()
     a = b = dsk.View.from_buffer_copy(cache._view("q", q, q.shape))
     assert dsk.lib().dsk_kv8_attn(cache._c, s, a, b, 4, 1.0, 0, 0, None, 0, None) != 0 and b"workspace" in dsk.lib().dsk_last_error()
+
+
+@pytest.mark.parametrize("rows", [3, 90])
+@pytest.mark.parametrize("order", [1, -1])
+def test_attend_maxima_that_jump(rows, order):
+    """Scores that grow (or fall) by some tens from one stretch of 16 keys to the next, up to some hundreds: references move inside tiles and between them, by much and by little."""
+    n = 400
+    c = Case([n], 1, 64, 64, 16, seed=11, spread=0.1)
+    grow = np.concatenate([np.linspace(0, 9, 20), np.array([0, 60, -40, 90, 91])])[::order]
+    q0 = c.rng.normal(size=64)
+    x = np.zeros((1, n, 1, 64))
+    for t in range(n):
+        x[0, t, 0] = q0 * grow[t // 16] / (q0 @ q0) * 8 + 0.01 * c.rng.normal(size=64)       # (score of q0 at 1/8: grow)
+    so.write(c.k, c.ks, c.table, [0], [n], x)
+    cache = c.device()
+    q = torch.from_numpy(q0[None, None, None, :] * np.array([1.0, 0.5, -1.0, 4.0])[None, None, :, None] * np.ones((1, rows, 1, 1))).to(torch.bfloat16)
+    out = cache.attend(q.to(DEV), c.t, ints([n]))
+    want, tol = expect(c, q.double().numpy(), [rows], 4, 0.125)
+    check(out, want, tol, [rows], "bf16")
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_offsets_beyond_32_bits(rows):
+    """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""
+    blocks, H, dk, dv, block = 40000, 8, 192, 16, 128
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("12 GB of device memory are needed")
+    k = torch.empty((blocks, H, block, dk), dtype=torch.uint8, device=DEV)
+    v = torch.empty((blocks, H, block, dv), dtype=torch.uint8, device=DEV)
+    assert k.numel() > 1 << 32
+    cache = dsk.Cache8.of(k.view(F8), v.view(F8), torch.ones((blocks, H), device=DEV), torch.ones((blocks, H), device=DEV))
+    table = torch.tensor([[blocks - 1, 3, blocks - 2]], dtype=torch.int32, device=DEV)
+    n = 2 * block + 40
+    g = torch.Generator().manual_seed(0)
+    x, y = torch.randn(1, n, H, dk, generator=g), torch.randn(1, n, H, dv, generator=g)
+    cache.write(x.to(DEV), y.to(DEV), table, ints([0]))
+    c = Case([n], H, dk, dv, block)
+    c.table = np.array([[0, 1, 2]], dtype=np.int32)
+    so.write(c.k, c.ks, c.table, [0], [n], x.double().numpy())
+    so.write(c.v, c.vs, c.table, [0], [n], y.double().numpy())
+    for i, page in enumerate([blocks - 1, 3, blocks - 2]):
+        m = min(block, n - i * block)
+        assert np.array_equal(k[page, :, :m].cpu().numpy(), c.k[i, :, :m]) and np.array_equal(v[page, :, :m].cpu().numpy(), c.v[i, :, :m])
+    rk, rv = cache.read(table, ints([0]), n, dtype=torch.float32)
+    for h in range(H):
+        assert torch.equal(rk[0, :, h].cpu().double(), torch.from_numpy(so.gather(c.k, c.ks, c.table[0], n, h)[0]))
+    q = torch.randn(1, rows, H, dk, generator=g).to(torch.bfloat16)
+    out = cache.attend(q.to(DEV), table, ints([n]))
+    want, tol = expect(c, q.double().numpy(), [rows], H, dk ** -0.5)
+    check(out, want, tol, [rows], "bf16")
+    cache.check()
+
+
+def test_write_captured_and_replayed():
+    """One captured call appends token after token: its places come from the GPU."""
+    c = Case([0, 0], 2, 64, 64, 16, dead=0)
+    c.table = np.array([[0, 1, 2], [3, 4, 5]], dtype=np.int32)
+    c.blocks = 6
+    c.k, c.v = (np.zeros((6, 2, 16, 64), dtype=np.uint8) for _ in range(2))
+    c.ks, c.vs = np.ones((6, 2)), np.ones((6, 2))
+    cache = c.device()
+    first, x, y = ints([0, 5]), torch.zeros(2, 1, 2, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(2, 1, 2, 64, device=DEV, dtype=torch.bfloat16)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.write(x, y, c.t, first)
+        first += 1
+    at = [0, 5]
+    for step in range(40):
+        a, b = (torch.from_numpy(c.rng.normal(size=(2, 1, 2, 64)) * np.exp(c.rng.normal())).to(torch.bfloat16) for _ in range(2))
+        x.copy_(a)
+        y.copy_(b)
+        g.replay()
+        so.write(c.k, c.ks, c.table, at, [1, 1], a.double().numpy())
+        so.write(c.v, c.vs, c.table, at, [1, 1], b.double().numpy())
+        at = [t + 1 for t in at]
+    k, v, ks, vs = c.bytes()
+    assert np.array_equal(k, c.k) and np.array_equal(v, c.v) and np.array_equal(ks, c.ks) and np.array_equal(vs, c.vs)
+
+
+def test_steps_of_speculative_decoding():
+    """Prompt, then steps of a token and its drafts: keys and values join the cache, all queries attend, a head makes logits, the drafts are verified, and the next step's tokens lie over the
+    refused ones.  Every call's result is that of the definition on what the calls before left."""
+    B, H, G, d, V, n = 3, 2, 2, 64, 300, 4
+    g = torch.Generator().manual_seed(5)
+    emb, wq, wk, wv, wo = (torch.randn(*s, generator=g, dtype=torch.float64) * f for s, f in (((V, d), 1.0), ((d, H * G * d), 0.15), ((d, H * d), 0.15), ((d, H * d), 0.15), ((H * G * d, V), 0.2)))
+    c = Case([0] * B, H, d, d, 32, dead=0)
+    c.table = np.arange(B * 4, dtype=np.int32).reshape(B, 4)
+    c.blocks = B * 4
+    c.k, c.v = (np.zeros((c.blocks, H, 32, d), dtype=np.uint8) for _ in range(2))
+    c.ks, c.vs = np.ones((c.blocks, H)), np.ones((c.blocks, H))
+    cache = c.device()
+    lens = [40, 7, 33]
+    rng = np.random.default_rng(6)
+    tokens = torch.from_numpy(rng.integers(0, V, size=(B, 40)))
+    count, drawn = list(lens), None
+    first = [0] * B
+    for step in range(5):
+        x = emb[tokens]
+        q, k, v = ((x @ w).to(torch.bfloat16).view(B, tokens.shape[1], -1, d) for w in (wq, wk, wv))
+        cache.write(k.to(DEV), v.to(DEV), c.t, ints(first), ints(count))
+        so.write(c.k, c.ks, c.table, first, count, k.double().numpy())
+        so.write(c.v, c.vs, c.table, first, count, v.double().numpy())
+        total = [a + m for a, m in zip(first, count)]
+        out = cache.attend(q.to(DEV), c.t, ints(total), ints(count))
+        want, tol = expect(c, q.double().numpy(), count, H * G, d ** -0.5, lens=total)
+        check(out, want, tol, count, "bf16", left=0.0)
+        kk, vv, ks, vs = c.bytes()
+        assert np.array_equal(kk, c.k) and np.array_equal(vv, c.v) and np.array_equal(ks, c.ks) and np.array_equal(vs, c.vs)
+        logits = (out.double().cpu().flatten(2) @ wo).float()
+        if step:
+            probs = torch.softmax(logits[:, :n] + 0.5 * torch.from_numpy(rng.normal(size=(B, n, V))).float(), -1)
+            coins = torch.from_numpy(rng.random((B, n + 1)).astype(np.float32)).clamp(max=1 - 2.0 ** -24)
+            drafts = tokens[:, 1:].to(torch.int32).contiguous()
+            a, t = dsk.verify_drafts(logits.to(DEV), drafts.to(DEV), coins.to(DEV), probs=probs.to(DEV), count=ints([m - 1 for m in count]))
+            wa, wt = so.verify(logits.double().numpy(), drafts.numpy(), coins.numpy(), probs.numpy(), [m - 1 for m in count], 1.0)
+            assert np.array_equal(a.cpu().numpy(), wa) and np.array_equal(t.cpu().numpy(), wt)
+            first = [f + 1 + int(m) for f, m in zip(first, wa)]           # (the refused drafts' places are written again)
+            drawn = [int(wt[b, wa[b]]) for b in range(B)]
+        else:
+            first = list(lens)
+            drawn = [int(logits[b, lens[b] - 1].argmax()) for b in range(B)]
+        tokens = torch.from_numpy(rng.integers(0, V, size=(B, n + 1)))
+        tokens[:, 0] = torch.tensor(drawn)
+        count = [n + 1, n, 1 + step % n]
+    cache.check()

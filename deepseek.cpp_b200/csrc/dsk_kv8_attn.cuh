@@ -13,6 +13,8 @@
 // keys x four pieces) are keys j and j + 4, whose rows lie 16 banks apart.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "dsk_kv8.cuh"
 
 namespace dsk {
@@ -29,7 +31,7 @@ struct Attn {
   const void* q;
   void* out;
   Pitch pq, po;
-  int heads, group, row_tiles, bf16, wide_q, wide_o, window, keep;
+  int heads, group, row_tiles, bf16, wide_q, wide_o, window, keep, cluster;   // cluster: CTAs that share a (sequence, head, tile), 0: the line
   float scale;                                               // times log2(e)
   float* part;                                               // workspace: pieces
 };
@@ -167,8 +169,47 @@ struct Out {
   }
 };
 
-// DK, DV: entries of keys and values, rounded up; QT: tiles of 8 queries
-template <int DK, int DV, int QT>
+// Joins n pieces of a (sequence, head, query tiles), piece(i): [accumulator][lane], maxima, sums.  A warp has eight entries of one of every lane's two queries: warp `task` of QT DV / 32.
+template <int DV, int QT, typename F>
+__device__ __forceinline__ void join_pieces(const Attn& P, const Seq& q, int b, int head, int row0, int task, int lane, int n, F piece) {
+  constexpr int NO = DV / 16, VCH = DV >= 128 ? 16 : 8;
+  const int r = lane >> 2, c = lane & 3, e = task & 1;
+  task >>= 1;
+  const int k0 = (task % (DV / 64)) * 8, t = task / (DV / 64), row = t * 8 + 2 * c + e;   // k0: of a lane's DV / 8 entries
+  float x[16], m = -1e30f, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; k++) x[k] = 0.f;
+  for (int i = 0; i < n; i += 4) {
+    float pm[4], pl[4], px[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      if (i + u >= n) { pm[u] = -INFINITY; continue; }
+      const float* from = piece(i + u);
+      pm[u] = from[QT * NO * 128 + row];
+      pl[u] = from[QT * NO * 128 + QT * 8 + row];
+#pragma unroll
+      for (int k = 0; k < 8; k++) px[u][k] = from[((t * NO + (k0 + k) / 2) * 4 + 2 * (k & 1) + e) * 32 + lane];
+    }
+    const float to = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), f = exp2_fast(m - to);
+    m = to;
+    l *= f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      if (i + u >= n) break;
+      const float g = exp2_fast(pm[u] - m);
+      l = fmaf(pl[u], g, l);
+#pragma unroll
+      for (int k = 0; k < 8; k++) x[k] = fmaf(px[u][k], g, x[k]);
+    }
+  }
+  Out::store(P, q, b, head, row0 + row, k0 / VCH * 128 + r * VCH + k0 % VCH, 8, x, l == 0.f ? 0.f : 1.f / l);
+}
+
+// DK, DV: entries of keys and values, rounded up; QT: tiles of 8 queries.  SHARED: P.cluster CTAs have one (sequence, head, tile) and join their pieces in one another's shared memory
+// (one token behind 1000, 16 heads over 4: 10.2 us by the line with its second launch).
+template <int DK, int DV, int QT, bool SHARED>
 __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
   constexpr int NST = stages<DK, DV, QT>(), KS = DK + 16, VS = DV + 32, STEP = step_of(QT), HV = STEP / 16, SB = stage_bytes<DK, DV>(STEP), QS = 2 * DK + 16, VCH = DV >= 128 ? 16 : 8,
                 HF = DV / (8 * VCH), NO = DV / 16;           // NO: tiles of 16 entries; a lane's entries are VCH neighbours, two to a tile
@@ -183,38 +224,60 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
   float* row_q = row_l + kWarps * QT * 8;                                // factor of a query's scores
   long long* ends = reinterpret_cast<long long*>(raw + ((attn_smem<DK, DV, QT>() + 7) & ~7));
   const uint32_t stage0 = smem_u32(raw) + warp * NST * SB, q0 = smem_u32(q_raw);
-  grid_release();
-  // line of units: running sums over the sequences
+  const int per = P.C.heads * P.row_tiles;
+  int mine, rank = 0;                                        // units of this CTA
+  Place<STEP> at;                                            // of the next copies
   if (P.C.dim[0] < DK || P.C.dim[1] < DV)
     for (int i = threadIdx.x; i < NST * SB * kWarps / 16; i += kThreads) reinterpret_cast<uint4*>(raw)[i] = make_uint4(0, 0, 0, 0);   // (entries behind the last one stay zero)
-  long long run = 0;
-  for (int b0 = 0; b0 < B; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    const long long own = b < B ? sequence<STEP>(P, b).units : 0;
-    long long v = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += t; }
-    if (lane == 31) warp_sums[warp] = v;
-    __syncthreads();
-    long long before = run, all = run;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) { if (w < warp) before += warp_sums[w]; all += warp_sums[w]; }
-    if (b < B) ends[b] = before + v - own;
-    run = all;
-    __syncthreads();
-  }
-  const int per = P.C.heads * P.row_tiles;
-  const long long total = run * per, N = ctas_of(gridDim.x, total, (long long)B * per);
-  if (blockIdx.x == 0) {
-    for (int b = threadIdx.x; b < B; b += kThreads) {
-      const long long len = P.S.first[b];
-      if (len < 0 || len > (long long)P.S.table_blocks * P.C.block) note(P.C, ST_RANGE);
+  if constexpr (SHARED) {
+    const int u = blockIdx.x / P.cluster, hr = u % per;
+    rank = blockIdx.x - u * P.cluster;
+    at.b = u / per;
+    at.q = sequence<STEP>(P, at.b);
+    if (rank == 0 && hr == 0 && threadIdx.x == 0) {
+      const long long len = P.S.first[at.b];
+      if (len < 0 || len > (long long)P.S.table_blocks << P.C.shift) note(P.C, ST_RANGE);
     }
+    if (at.q.count == 0) return;                             // (the whole cluster)
+    at.head = hr / P.row_tiles;
+    at.tile = hr - at.head * P.row_tiles;
+    at.table = P.S.table + at.b * P.S.table_pitch;
+    at.unit = (int)((long long)at.q.units * rank / P.cluster);
+    mine = (int)((long long)at.q.units * (rank + 1) / P.cluster) - at.unit;
+    __syncthreads();
+  } else {
+    grid_release();
+    // line of units: running sums over the sequences
+    long long run = 0;
+    for (int b0 = 0; b0 < B; b0 += kThreads) {
+      const int b = b0 + threadIdx.x;
+      const long long own = b < B ? sequence<STEP>(P, b).units : 0;
+      long long v = own;
+  #pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += t; }
+      if (lane == 31) warp_sums[warp] = v;
+      __syncthreads();
+      long long before = run, all = run;
+  #pragma unroll
+      for (int w = 0; w < kWarps; w++) { if (w < warp) before += warp_sums[w]; all += warp_sums[w]; }
+      if (b < B) ends[b] = before + v - own;
+      run = all;
+      __syncthreads();
+    }
+    const long long total = run * per, N = ctas_of(gridDim.x, total, (long long)B * per);
+    if (blockIdx.x == 0) {
+      for (int b = threadIdx.x; b < B; b += kThreads) {
+        const long long len = P.S.first[b];
+        if (len < 0 || len > (long long)P.S.table_blocks << P.C.shift) note(P.C, ST_RANGE);
+      }
+    }
+    if ((long long)blockIdx.x >= N) return;
+    const long long x0 = quotient(blockIdx.x * total, N), x1 = quotient((blockIdx.x + 1) * total, N);
+    mine = (int)(x1 - x0);
+    __syncthreads();
+    at.find(P, ends, x0, per);
   }
-  if ((long long)blockIdx.x >= N) return;
-  const long long x0 = quotient(blockIdx.x * total, N), x1 = quotient((blockIdx.x + 1) * total, N);
-  __syncthreads();
-  const int dk = P.C.dim[0], dv = P.C.dim[1], dk16 = dk / 16, dv16 = dv / 16, mine = (int)(x1 - x0);
+  const int dk = P.C.dim[0], dv = P.C.dim[1], dk16 = dk / 16, dv16 = dv / 16;
   const bool exact = dk == DK && dv == DV;
   const uint32_t head_k = P.C.block * dk, head_v = P.C.block * dv, block_k = P.C.heads * head_k, block_v = P.C.heads * head_v;   // bytes of a head and of a block (at most 2^30)
   const float* my_scale = P.C.scale[lane & 1];
@@ -233,8 +296,6 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
 #pragma unroll
     for (int j = 0; j < DV / 32; j++) { to_v[j] = STEP * KS + row * VS + col * 16; row += dr; col += dc; if (col >= dv16) { col -= dv16; row++; } }
   }
-  Place<STEP> at;                                            // of the next copies
-  at.find(P, ends, x0, per);
   int ahead = mine, page[HV], key = -1;                      // units that are not under way yet; the next step's blocks (of 16 keys each) and first key (-1: this warp has none)
   auto look = [&]() {
     const int s = at.unit * kWarps + warp;
@@ -578,7 +639,8 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
       __syncthreads();
       if (warp == 0) {
         add(turn + QT * NO * 128 + lane);
-        if (begun == 0 && whole_end) {
+        __syncwarp();
+        if (!SHARED && begun == 0 && whole_end) {
 #pragma unroll
           for (int t = 0; t < QT; t++)
 #pragma unroll
@@ -593,7 +655,7 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
               }
             }
         } else {                                             // a piece: [accumulator][lane], then maxima and sums of the queries
-          float* to = P.part + (size_t)(2 * blockIdx.x + (y == pl.unit - begun ? 0 : 1)) * (QT * (NO * 128 + 16));
+          float* to = SHARED ? turn : P.part + (size_t)(2 * blockIdx.x + (y == pl.unit - begun ? 0 : 1)) * (QT * (NO * 128 + 16));
 #pragma unroll
           for (int t = 0; t < QT; t++) {
 #pragma unroll
@@ -615,12 +677,24 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     if (fresh) begun = pl.unit;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (SHARED) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    if (mine == 0) {                                         // (more CTAs than units)
+      for (int i = threadIdx.x; i < QT * NO * 128; i += kThreads) turn[i] = 0.f;
+      for (int i = threadIdx.x; i < QT * 8; i += kThreads) { turn[QT * NO * 128 + i] = -1e30f; turn[QT * NO * 128 + QT * 8 + i] = 0.f; }
+    }
+    cluster.sync();
+    for (int task = rank * kWarps + warp; task < QT * DV / 32; task += P.cluster * kWarps)
+      join_pieces<DV, QT>(P, at.q, at.b, at.head, at.tile * QT * 8, task, lane, P.cluster, [&](int i) { return (const float*)cluster.map_shared_rank(turn, i); });
+    cluster.sync();                                          // nobody's shared memory is read any more
+  }
 }
 
-// Joins the pieces of a (sequence, head, query tiles) that several CTAs of attend_tokens had: a warp has eight entries of one of every lane's two queries
+// Joins the pieces that several CTAs of the line had
 template <int DV, int QT>
 __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
-  constexpr int NO = DV / 16, VCH = DV >= 128 ? 16 : 8;
+  constexpr int NO = DV / 16;
   // who had what is known without the kernel ahead
   __shared__ long long sums[2][QT * DV / 32];
   const int b = blockIdx.y, hr = blockIdx.x, per = gridDim.x;
@@ -639,41 +713,9 @@ __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
   if (i0 == i1) return;
   const int own = quotient(i0 * total, N) >= u0 ? 0 : 1;     // the first one's piece: its first or its last (the others' pieces are their first)
   grid_wait();
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  int w = threadIdx.x >> 5;
-  const int e = w & 1;
-  w >>= 1;
-  const int k0 = (w % (DV / 64)) * 8, t = w / (DV / 64), row = t * 8 + 2 * c + e;   // k0: of a lane's DV / 8 entries
-  float x[16], m = -1e30f, l = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; k++) x[k] = 0.f;
-  for (int i = i0; i <= i1; i += 4) {
-    float pm[4], pl[4], px[4][8];
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      if (i + u > i1) { pm[u] = -INFINITY; continue; }
-      const float* from = P.part + (size_t)(2 * (i + u) + (i + u == i0 ? own : 0)) * (QT * (NO * 128 + 16));
-      pm[u] = from[QT * NO * 128 + row];
-      pl[u] = from[QT * NO * 128 + QT * 8 + row];
-#pragma unroll
-      for (int k = 0; k < 8; k++) px[u][k] = from[((t * NO + (k0 + k) / 2) * 4 + 2 * (k & 1) + e) * 32 + lane];
-    }
-    const float to = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), f = exp2_fast(m - to);
-    m = to;
-    l *= f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) x[k] *= f;
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      if (i + u > i1) break;
-      const float g = exp2_fast(pm[u] - m);
-      l = fmaf(pl[u], g, l);
-#pragma unroll
-      for (int k = 0; k < 8; k++) x[k] = fmaf(px[u][k], g, x[k]);
-    }
-  }
-  const int head = hr / P.row_tiles, row0 = (hr - head * P.row_tiles) * QT * 8;
-  Out::store(P, q, b, head, row0 + row, k0 / VCH * 128 + r * VCH + k0 % VCH, 8, x, l == 0.f ? 0.f : 1.f / l);
+  const int head = hr / P.row_tiles;
+  join_pieces<DV, QT>(P, q, b, head, (hr - head * P.row_tiles) * QT * 8, threadIdx.x >> 5, threadIdx.x & 31, i1 - i0 + 1,
+                      [&](int i) { return (const float*)P.part + (size_t)(2 * (i0 + i) + (i == 0 ? own : 0)) * (QT * (NO * 128 + 16)); });
 }
 
 }  // namespace kv8

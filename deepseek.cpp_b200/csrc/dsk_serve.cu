@@ -65,16 +65,17 @@ template <auto KERNEL> cudaError_t allow(int device, int bytes) {
 }
 // A launch behind another one of the same call: its CTAs may come up under the kernel ahead and wait there (grid_wait).
 template <typename... KA, typename... A>
-cudaError_t launch_behind(void (*kernel)(KA...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster, A... a) {
+cudaError_t launch_behind(void (*kernel)(KA...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster, A... a) {   // cluster < 0: clusters of -cluster, not behind anything
   cudaLaunchConfig_t c{};
   cudaLaunchAttribute at[2];
-  c.gridDim = grid; c.blockDim = block; c.dynamicSmemBytes = smem; c.stream = stream; c.attrs = at; c.numAttrs = 1;
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  if (cluster > 1) {
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
-    c.numAttrs = 2;
+  c.gridDim = grid; c.blockDim = block; c.dynamicSmemBytes = smem; c.stream = stream; c.attrs = at; c.numAttrs = 0;
+  if (cluster > 0) {
+    at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[c.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1 || cluster < -1) {
+    at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[c.numAttrs].val.clusterDim.x = std::abs(cluster); at[c.numAttrs].val.clusterDim.y = 1; at[c.numAttrs++].val.clusterDim.z = 1;
   }
   return cudaLaunchKernelEx(&c, kernel, static_cast<KA>(a)...);
 }
@@ -153,10 +154,11 @@ template <typename T> int read_as(const dsk_kv8* c, const dsk_kv8_rows* s, const
 }
 
 // How an attention call is laid out
-struct Layout { int shape, tiles, row_tiles, ctas, shares; size_t bytes; };   // shares > 0: attend_rows
+struct Layout { int shape, tiles, row_tiles, ctas, shares, cluster; size_t bytes; };   // shares > 0: attend_rows
 constexpr int kPortionRows = 32;                             // query rows of a key head from which on attend_rows has them
 constexpr int kShapes[4][2] = {{64, 64}, {128, 128}, {192, 128}, {256, 256}};
-int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, Layout* L) {
+int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, int keep_first, Layout* L) {
+  if (window < 0 || keep_first < 0) return fail(-4, "window %d and keep_first %d must not be negative", window, keep_first);
   if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
   if (s->batch > kv8::kMaxBatch) return fail(-4, "attention over %d sequences: at most %d a call", s->batch, kv8::kMaxBatch);
   const long long rows = (long long)(heads / c->kv_heads) * s->rows;
@@ -165,26 +167,37 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, Layout* L) {
   const int sms = multiprocessors(c->device);
   if (!sms) return fail(-2, "device %d: no attributes", c->device);
   const long long keys = (long long)s->table_blocks * c->block;
-  L->shares = 0;
+  L->shares = L->cluster = 0;
   if (rows > kPortionRows && L->shape < 3) {
     L->row_tiles = (int)((rows + kv8::kRows - 1) / kv8::kRows);
     const long long tiles = (long long)s->batch * c->kv_heads * L->row_tiles;
     L->shares = (int)std::max<long long>(1, std::min<long long>(sms / tiles, (keys + kv8::kTile - 1) / kv8::kTile));   // where the row tiles leave SMs idle, their keys are shared out
-    L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * kv8::kRows * (kShapes[L->shape][1] + 2) * sizeof(float) : 16;
+    L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * kv8::kRows * (kShapes[L->shape][1] + 2) * sizeof(float) : 0;
     return 0;
   }
   L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : rows <= 24 ? 3 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
   L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
   const int unit = kv8::kWarps * kv8::step_of(L->tiles);
   const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * ((keys + unit - 1) / unit + 1);
+  // A cluster to each (sequence, head, tile) where they are few and the tables short enough that eight CTAs have at most eight units each, or where clusters fill the SMs: one launch, no
+  // workspace.  Otherwise the line: any number of CTAs to a head, whatever the lengths.
+  const long long each = (long long)s->batch * c->kv_heads * L->row_tiles, most = window ? std::min(keys, (long long)window + s->rows + keep_first) : keys, longest = (most + unit - 1) / unit + (window ? 2 : 0);
+  for (int k = 8; k >= 2 && !L->cluster; k /= 2)
+    if (each * k <= 2 * sms && longest <= 8 * k) L->cluster = k;
+  if (L->cluster) { L->ctas = (int)each * L->cluster; L->bytes = 0; return 0; }
   L->ctas = (int)std::min<long long>(2 * sms, std::max<long long>(1, units));
   L->bytes = (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 16 * 128 + 16) * sizeof(float);
   return 0;
 }
 template <int DK, int DV, int QT> int attend_as(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
+  if (L.cluster) {
+    CK((allow<kv8::attend_tokens<DK, DV, QT, true>>(device, kv8::attn_smem<DK, DV, QT>())));
+    CK(launch_behind(kv8::attend_tokens<DK, DV, QT, true>, dim3(L.ctas), dim3(kv8::kThreads), kv8::attn_smem<DK, DV, QT>(), stream, -L.cluster, P));
+    return 0;
+  }
   const int smem = kv8::attn_smem<DK, DV, QT>() + 8 + 8 * P.S.batch;
-  CK((allow<kv8::attend_tokens<DK, DV, QT>>(device, kv8::attn_smem<DK, DV, QT>() + 8 + 8 * kv8::kMaxBatch)));
-  kv8::attend_tokens<DK, DV, QT><<<L.ctas, kv8::kThreads, smem, stream>>>(P);
+  CK((allow<kv8::attend_tokens<DK, DV, QT, false>>(device, kv8::attn_smem<DK, DV, QT>() + 8 + 8 * kv8::kMaxBatch)));
+  kv8::attend_tokens<DK, DV, QT, false><<<L.ctas, kv8::kThreads, smem, stream>>>(P);
   CK(cudaGetLastError());
   CK(launch_behind(kv8::join<DV, QT>, dim3(P.C.heads * P.row_tiles, P.S.batch), dim3(QT * DV), 0, stream, 1, P, L.ctas));
   return 0;
@@ -232,11 +245,11 @@ extern "C" int dsk_kv8_read(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
   return dt == DSK_DT_F32 ? read_as<float>(c, s, k, v, st) : dt == DSK_DT_F16 ? read_as<__half>(c, s, k, v, st) : read_as<__nv_bfloat16>(c, s, k, v, st);
 }
 
-extern "C" int dsk_kv8_attn_workspace(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, size_t* bytes) {
+extern "C" int dsk_kv8_attn_workspace(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, int keep_first, size_t* bytes) {
   if (!bytes) return fail(-1, "bad arguments");
   if (check_cache(c, s)) return -1;
   Layout L{};
-  if (layout_of(c, s, heads, &L)) return -1;
+  if (layout_of(c, s, heads, window, keep_first, &L)) return -1;
   *bytes = L.bytes;
   return 0;
 }
@@ -247,13 +260,13 @@ extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
   const int dt = q ? q->dtype : -1;
   if (dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_attn: queries are F16 or BF16");
   if (!(std::fabs(scale) < INFINITY)) return fail(-4, "dsk_kv8_attn: the scale is not a number");
-  if (window < 0 || keep_first < 0) return fail(-4, "dsk_kv8_attn: window %d and keep_first %d must not be negative", window, keep_first);
+  if (window < 0 || keep_first < 0) return fail(-4, "window %d and keep_first %d must not be negative", window, keep_first);
   if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
   if (!s->batch || !s->rows) return 0;
   if (check_view("queries", q, dt) || check_view("output", out, dt)) return -1;
   Layout L{};
-  if (layout_of(c, s, heads, &L)) return -1;
-  if (!workspace || !aligned(workspace, 16) || workspace_bytes < L.bytes) return fail(-1, "dsk_kv8_attn: a workspace of %zu bytes is needed, 16-byte aligned (%zu given)", L.bytes, workspace_bytes);
+  if (layout_of(c, s, heads, window, keep_first, &L)) return -1;
+  if (L.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < L.bytes)) return fail(-1, "dsk_kv8_attn: a workspace of %zu bytes is needed, 16-byte aligned (%zu given)", L.bytes, workspace_bytes);
   OnDevice on(c->device);
   CK(on.error);
   kv8::Attn P;
@@ -263,6 +276,7 @@ extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
   P.window = window; P.keep = keep_first;
   P.scale = scale * 1.44269504088896340736f;
   P.part = static_cast<float*>(workspace);
+  P.cluster = L.cluster;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (L.shape) {
     case 0: return attend_tiles<64, 64>(P, L, c->device, st);

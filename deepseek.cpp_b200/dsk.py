@@ -566,7 +566,7 @@ def lib():
                                    i32p, f32p]
         L.dsk_bench_gemv.argtypes = [C.c_int] * 6 + [f32p, C.POINTER(C.c_double)]
         L.dsk_kv8_write.argtypes = L.dsk_kv8_read.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.POINTER(View), C.POINTER(View), C.c_void_p]
-        L.dsk_kv8_attn_workspace.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.c_int, C.POINTER(C.c_size_t)]
+        L.dsk_kv8_attn_workspace.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]
         L.dsk_kv8_attn.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.POINTER(View), C.POINTER(View), C.c_int, C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
         L.dsk_verify_workspace.argtypes = [C.POINTER(VerifyArgs), C.POINTER(C.c_size_t)]
         L.dsk_verify.argtypes = [C.POINTER(VerifyArgs), C.c_void_p, C.c_size_t, C.c_void_p]
@@ -909,7 +909,7 @@ def _fast(name):
         f = lib()[name]
         P = C.c_void_p
         f.argtypes = {"dsk_kv8_write": [P, C.c_char_p, C.c_char_p, C.c_char_p, P], "dsk_kv8_read": [P, C.c_char_p, C.c_char_p, C.c_char_p, P],
-                      "dsk_kv8_attn_workspace": [P, C.c_char_p, C.c_int, C.POINTER(C.c_size_t)],
+                      "dsk_kv8_attn_workspace": [P, C.c_char_p, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)],
                       "dsk_kv8_attn": [P, C.c_char_p, C.c_char_p, C.c_char_p, C.c_int, C.c_float, C.c_int, C.c_int, P, C.c_size_t, P],
                       "dsk_verify_workspace": [C.c_char_p, C.POINTER(C.c_size_t)], "dsk_verify": [C.c_char_p, P, C.c_size_t, P]}[name]
         _raw[name] = f
@@ -1031,16 +1031,16 @@ class Cache8:
             raise DskError(f"results of {out.dtype} for queries of {q.dtype}")
         s = self._rows(table, lens, count, rows)
         a, b = self._view("queries", q, (batch, rows, heads, self.dim_k)), self._view("output", out, shape, True)
-        key = (batch, rows, heads, table.shape[1])
+        key = (batch, rows, heads, table.shape[1], window, keep_first)
         need = self._needs.get(key)
         if need is None:
             got = C.c_size_t(0)
-            _ck(_fast("dsk_kv8_attn_workspace")(self._at, s, heads, C.byref(got)))
+            _ck(_fast("dsk_kv8_attn_workspace")(self._at, s, heads, window, keep_first, C.byref(got)))
             if len(self._needs) > 4096:
                 self._needs.clear()
             need = self._needs[key] = got.value
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _ck(_fast("dsk_kv8_attn")(self._at, s, a, b, heads, self.dim_k ** -0.5 if scale is None else scale, window, keep_first, work.data_ptr(), need, _stream_of(torch, self.device)))
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _ck(_fast("dsk_kv8_attn")(self._at, s, a, b, heads, self.dim_k ** -0.5 if scale is None else scale, window, keep_first, work.data_ptr() if need else 0, need, _stream_of(torch, self.device)))
         return out
 
     def check(self):

@@ -377,7 +377,7 @@ int dsk_kv8_read(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view*
 /* Softmax attention.  first[b]: the sequence's tokens in the cache, the last count[b] of which are the queries' (written ahead of the call): query i is at t = first[b] - count[b] + i and
  * sees the tokens j <= t, with window > 0 those with t - j < window or j < keep_first.  Query head h reads key head h / (heads / kv_heads); out = softmax(scale q k) v in the queries' type
  * (F16 or BF16), zeros for a query that sees nothing.  At most 1024 sequences a call. */
-int dsk_kv8_attn_workspace(const dsk_kv8* cache, const dsk_kv8_rows* rows, int heads, size_t* bytes);
+int dsk_kv8_attn_workspace(const dsk_kv8* cache, const dsk_kv8_rows* rows, int heads, int window, int keep_first, size_t* bytes);   /* 0: none */
 int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* q, const dsk_view* out, int heads, float scale, int window, int keep_first,
                  void* workspace, size_t workspace_bytes, void* stream);
 /* Speculative sampling, beside dsk_sample: sequence b has count[b] drafted tokens x_i and the model's logits of count[b] + 1 rows.  p_i = softmax(logits_i / temperature); draft i is accepted

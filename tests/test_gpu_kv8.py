@@ -221,6 +221,31 @@ def test_attend(lens, count, rows, heads, kv_heads, dk, dv, block, dtype, window
     if all(n == rows for n in count):
         again = cache.attend(q.to(DEV), c.t, ints(lens), window=window, keep_first=keep)
         assert torch.equal(again, out)                        # the same sums in the same order
+    # the same behind a table with room for many more tokens (work is laid out for what the table could hold), whose other entries nobody may look at
+    wide = torch.full((len(lens), 3000), -7, dtype=torch.int32, device=DEV)
+    wide[:, :c.t.shape[1]] = c.t
+    out = torch.full((len(lens), rows, heads, dv), 7.0, device=DEV, dtype=DT[dtype])
+    cache.attend(q.to(DEV), wide, ints(lens), count=ints(count), window=window, keep_first=keep, out=out)
+    check(out, want, tol, count, dtype, left=7.0)
+    cache.check()
+
+
+@pytest.mark.parametrize("heads,rows", [(4, 1), (8, 1), (12, 3), (8, 8), (16, 2), (8, 11)])
+@pytest.mark.parametrize("window,keep", [(0, 0), (40, 5)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_more_heads_than_processors(heads, rows, window, keep, d):
+    """Many sequences of very unequal lengths: several heads to a CTA, pieces of one head in two, with and without a window."""
+    B = 84
+    lens = [(53 * b) % 170 + (1 if b % 7 else 0) for b in range(B)]
+    count = [min(rows, 1 + b % rows if b % 3 else rows) for b in range(B)]
+    c = Case(lens, 4, d, d, 32)
+    cache = c.device()
+    q = torch.randn(B, rows, heads, d, device=DEV, dtype=torch.bfloat16)
+    out = torch.full((B, rows, heads, d), 7.0, device=DEV, dtype=torch.bfloat16)
+    cache.attend(q, c.t, ints(lens), count=ints(count), window=window, keep_first=keep, out=out)
+    want, tol = expect(c, q.double().cpu().numpy(), count, heads, d ** -0.5, window, keep)
+    check(out, want, tol, count, "bf16", left=7.0)
+    cache.check()
 
 
 def test_attend_long_and_ragged():
@@ -426,6 +451,7 @@ def test_refusals():
     s = dsk.Kv8Rows.from_buffer_copy(cache._rows(c.t, ints([0]), None, 1))
     assert dsk.lib().dsk_kv8_write(cache._c, s, v, v, None) != 0 and b"F32, F16 or BF16" in dsk.lib().dsk_last_error()
     a = b = dsk.View.from_buffer_copy(cache._view("q", q, q.shape))
+    s.table_blocks = 1 << 20                                   # (a call that needs a workspace; refused ahead of its launch)
     assert dsk.lib().dsk_kv8_attn(cache._c, s, a, b, 4, 1.0, 0, 0, None, 0, None) != 0 and b"workspace" in dsk.lib().dsk_last_error()
 
 

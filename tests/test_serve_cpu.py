@@ -47,7 +47,7 @@ def test_cache_refusals(kw, text):
     need = C.c_size_t()
     _says(L.dsk_kv8_write(c, s, x, x, None), text)
     _says(L.dsk_kv8_read(c, s, x, x, None), text)
-    _says(L.dsk_kv8_attn_workspace(c, s, 4, need), text)
+    _says(L.dsk_kv8_attn_workspace(c, s, 4, 0, 0, need), text)
     _says(L.dsk_kv8_attn(c, s, x, x, 4, 1.0, 0, 0, None, 0, None), text)
 
 
@@ -68,7 +68,7 @@ def test_null_structures():
     L = dsk.lib()
     _says(L.dsk_kv8_write(None, s, x, x, None), "null")
     _says(L.dsk_kv8_write(c, None, x, x, None), "null")
-    _says(L.dsk_kv8_attn_workspace(c, s, 4, None), "bad arguments")
+    _says(L.dsk_kv8_attn_workspace(c, s, 4, 0, 0, None), "bad arguments")
     _says(L.dsk_verify(None, None, 0, None), "null")
     _says(L.dsk_verify_workspace(None, C.byref(C.c_size_t())), "null")
 

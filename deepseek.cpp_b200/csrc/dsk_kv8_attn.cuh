@@ -101,7 +101,7 @@ __device__ __forceinline__ uint32_t halves(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// E4M3 pairs: NaN as zero, and where the NaN are as ones
+__device__ __forceinline__ uint32_t lower_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {   // 0xff where a byte is NaN
   return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
 }
@@ -179,10 +179,11 @@ __device__ __forceinline__ void join_pieces(const Attn& P, const Seq& q, int b, 
   float x[16], m = -1e30f, l = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; k++) x[k] = 0.f;
-  for (int i = 0; i < n; i += 4) {
-    float pm[4], pl[4], px[4][8];
+  constexpr int AT = 8;                                      // pieces under way
+  for (int i = 0; i < n; i += AT) {
+    float pm[AT], pl[AT], px[AT][8], to = m;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < AT; u++) {
       if (i + u >= n) { pm[u] = -INFINITY; continue; }
       const float* from = piece(i + u);
       pm[u] = from[QT * NO * 128 + row];
@@ -190,13 +191,15 @@ __device__ __forceinline__ void join_pieces(const Attn& P, const Seq& q, int b, 
 #pragma unroll
       for (int k = 0; k < 8; k++) px[u][k] = from[((t * NO + (k0 + k) / 2) * 4 + 2 * (k & 1) + e) * 32 + lane];
     }
-    const float to = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), f = exp2_fast(m - to);
+#pragma unroll
+    for (int u = 0; u < AT; u++) to = fmaxf(to, pm[u]);
+    const float f = exp2_fast(m - to);
     m = to;
     l *= f;
 #pragma unroll
     for (int k = 0; k < 8; k++) x[k] *= f;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < AT; u++) {
       if (i + u >= n) break;
       const float g = exp2_fast(pm[u] - m);
       l = fmaf(pl[u], g, l);
@@ -461,21 +464,26 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
       }
       // a step that every query sees needs no mask
       const bool masked = key0 + STEP - 1 > q.first || (P.window > 0 && q.last - key0 >= P.window && key0 + STEP > P.keep) || gone;
-      uint32_t seen[QT] = {};                                // keys that this lane's queries see: a bit to a score
+      // keys that a query sees, a bit each: not behind its own, in the window or among the first, in the cache
+      auto sees = [&](int t, int e) {
+        const int pos = q.first + (row0 + t * 8 + 2 * c + e) / P.group;
+        uint32_t see = lower_bits(pos + 1 - key0);
+        if (P.window > 0) see &= ~lower_bits(pos - P.window + 1 - key0) | lower_bits(P.keep - key0);
+        see &= lower_bits(q.len - key0);
+        if (back[0] == 0.f) see &= ~0xffffu;
+        if (HV == 2 && back[HV - 1] == 0.f) see &= 0xffffu;
+        return see >> turn_r;                                // (bit 16 u + 8 h: key of score [u][h])
+      };
       if (masked) {
 #pragma unroll
         for (int t = 0; t < QT; t++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const int pos = q.first + (row0 + t * 8 + 2 * c + e) / P.group;
+            const uint32_t see = sees(t, e);
 #pragma unroll
             for (int u = 0; u < HV; u++)
 #pragma unroll
-              for (int h = 0; h < 2; h++) {
-                const int j = key0 + 16 * u + 8 * h + turn_r;
-                const bool ok = back[u] != 0.f && j < q.len && j <= pos && (P.window <= 0 || pos - j < P.window || j < P.keep);
-                if (ok) seen[t] |= 1u << (u * 4 + 2 * h + e); else s[t][u][2 * h + e] = -INFINITY;
-              }
+              for (int h = 0; h < 2; h++) if (!(see >> (16 * u + 8 * h) & 1)) s[t][u][2 * h + e] = -INFINITY;
           }
       }
       uint32_t w[QT][HV][2];                                 // weights as right operands: [query r][keys 2 c, 2 c + 1]
@@ -523,10 +531,11 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
         else { const uint2 y = lds64(vrow + key * VS); x[0] = y.x; x[1] = y.y; }
       };
       bool nan = false;
-      if (masked) {                                          // a NaN among values that some query does not see must not reach that query, whose weight for it is zero
+      // a NaN among values that some query does not see must not reach that query, whose weight for it is zero (behind the last key there are zeros)
+      if (masked && (min(key0 + STEP, q.len) - 1 > q.first || (P.window > 0 && q.last - key0 >= P.window))) {
 #pragma unroll 1
         for (int hf = 0; hf < HF; hf++)
-#pragma unroll 1
+#pragma unroll 4
           for (int k = 0; k < STEP / 4; k++) {
             uint32_t x[VCH / 4];
             values(hf, k * 4, x);
@@ -543,9 +552,11 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
         if (nan) {                                           // counts of the NaN that a query sees, two entries at a time, then numbers alone
           uint32_t see[QT][2];
 #pragma unroll
-          for (int t = 0; t < QT; t++)
+          for (int t = 0; t < QT; t++) {
+            const uint32_t see0 = sees(t, 0), see1 = sees(t, 1);
 #pragma unroll
-            for (int h = 0; h < 2; h++) see[t][h] = turned(((seen[t] >> (sub * 4 + 2 * h)) & 1 ? 0x3c00u : 0u) | ((seen[t] >> (sub * 4 + 2 * h + 1)) & 1 ? 0x3c000000u : 0u));
+            for (int h = 0; h < 2; h++) see[t][h] = turned(((see0 >> (16 * sub + 8 * h)) & 1 ? 0x3c00u : 0u) | ((see1 >> (16 * sub + 8 * h)) & 1 ? 0x3c000000u : 0u));
+          }
 #pragma unroll
           for (int k = 0; k < VCH / 2; k++) {
             uint32_t a[4];

@@ -23,6 +23,8 @@ namespace kv8 {
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxBatch = 1024;
 __host__ __device__ constexpr int step_of(int qt) { return qt < 4 ? 32 : 16; }   // keys of a warp's step
 __device__ __forceinline__ long long quotient(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }   // (of numbers >= 0)
+constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
+constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
 constexpr float kSlack = 8.f;                                // the reference of a row's weights follows its maximum once that is 2^8 ahead
 
 struct Attn {
@@ -41,7 +43,7 @@ struct Seq { int len, count, kept, low, steps, units, first, last; };   // first
 template <int STEP> __device__ __forceinline__ Seq sequence(const Attn& P, int b) {
   Seq q;
   const long long room = (long long)P.S.table_blocks << P.C.shift;
-  const int len = P.S.first[b];
+  const int len = max(P.S.first[b], -1);                     // (positions of the queries do not wrap)
   q.count = P.S.count ? min(max(P.S.count[b], 0), P.S.rows) : P.S.rows;
   q.len = (int)min((long long)max(len, 0), room);
   const long long first = (long long)len - q.count + 1 - P.window;
@@ -176,7 +178,7 @@ __device__ __forceinline__ void join_pieces(const Attn& P, const Seq& q, int b, 
   const int r = lane >> 2, c = lane & 3, e = task & 1;
   task >>= 1;
   const int k0 = (task % (DV / 64)) * 8, t = task / (DV / 64), row = t * 8 + 2 * c + e;   // k0: of a lane's DV / 8 entries
-  float x[16], m = -1e30f, l = 0.f;
+  float x[16], m = kLowest, l = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; k++) x[k] = 0.f;
   constexpr int AT = 8;                                      // pieces under way
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
           top = fmaxf(top, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
         }
         top = warp_max(top);
-        const int e = top > 0.f ? max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127 - 10)) : 0;
+        const int e = top > 0.f ? max(-100, min(120, (int)(__float_as_uint(top) >> 23) - 127 - 10)) : 0;
         const float by = P.scale < 0.f ? -pow2(-e) : pow2(-e);               // (factors of scores are positive)
 #pragma unroll
         for (int k = 0; k < DK / 64; k++) *reinterpret_cast<uint32_t*>(q_raw + row * QS + (k * 64 + lane * 2) * 2) = halves(v[2 * k] * by, v[2 * k + 1] * by);
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
 #pragma unroll
       for (int t = 0; t < QT; t++) {
 #pragma unroll
-        for (int e = 0; e < 2; e++) { m[t][e] = -1e30f; l[t][e] = 0.f; fq[t][e] = row_q[t * 8 + 2 * c + e]; }
+        for (int e = 0; e < 2; e++) { m[t][e] = kLowest; l[t][e] = 0.f; fq[t][e] = row_q[t * 8 + 2 * c + e]; }
 #pragma unroll
         for (int k = 0; k < NO; k++)
 #pragma unroll
@@ -501,9 +503,16 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
         }
-        if (__any_sync(0xffffffffu, mx[0] > m[t][0] + kSlack || mx[1] > m[t][1] + kSlack)) {
+        if (__any_sync(0xffffffffu, mx[0] > m[t][0] + kSlack || mx[1] > m[t][1] + kSlack || fmaxf(fabsf(mx[0]), fabsf(mx[1])) > kFar)) {
 #pragma unroll
           for (int e = 0; e < 2; e++) {
+#pragma unroll
+            for (int u = 0; u < HV; u++)
+              if (fabsf(mx[e]) > kFar) {
+                s[t][u][e] = fmaf(s[t][u][e], f[e][u], lift[u]) - lift[u];
+                s[t][u][2 + e] = fmaf(s[t][u][2 + e], f[e][u], lift[u]) - lift[u];
+                f[e][u] = 1.f;
+              }
             const float to = fmaxf(m[t][e], mx[e]), by = exp2_fast(m[t][e] - to);
             m[t][e] = to;
             l[t][e] *= by;
@@ -693,7 +702,7 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     cg::cluster_group cluster = cg::this_cluster();
     if (mine == 0) {                                         // (more CTAs than units)
       for (int i = threadIdx.x; i < QT * NO * 128; i += kThreads) turn[i] = 0.f;
-      for (int i = threadIdx.x; i < QT * 8; i += kThreads) { turn[QT * NO * 128 + i] = -1e30f; turn[QT * NO * 128 + QT * 8 + i] = 0.f; }
+      for (int i = threadIdx.x; i < QT * 8; i += kThreads) { turn[QT * NO * 128 + i] = kLowest; turn[QT * NO * 128 + QT * 8 + i] = 0.f; }
     }
     cluster.sync();
     for (int task = rank * kWarps + warp; task < QT * DV / 32; task += P.cluster * kWarps)

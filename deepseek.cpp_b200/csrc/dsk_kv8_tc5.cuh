@@ -109,7 +109,7 @@ __device__ __forceinline__ Walk walk_of(const Portion& P, int b, int row0, int s
   const Attn& A = P.A;
   Walk w;
   const long long room = (long long)A.S.table_blocks << A.C.shift;
-  const int len = A.S.first[b];
+  const int len = max(A.S.first[b], -1);                     // (positions do not wrap)
   w.count = A.S.count ? min(max(A.S.count[b], 0), A.S.rows) : A.S.rows;
   w.first = len - w.count;
   w.i0 = row0 / A.group;
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
         }
       }
       const float most = A.bf16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
-      const int e = most > 0.f ? max(-100, min(100, (int)(__float_as_uint(most) >> 23) - 127 - 10)) : 0;
+      const int e = most > 0.f ? max(-100, min(120, (int)(__float_as_uint(most) >> 23) - 127 - 10)) : 0;
       const float by = A.scale < 0.f ? -pow2(-e) : pow2(-e);                 // (factors of scores are positive)
       row_scale = pow2(e) * fabsf(A.scale);
       const uint32_t to = qs + t * (kTile * DK * 2) + (threadIdx.x & 127) * 128;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       if (lane == 0) hy::tc_arrive(qfull);
     }
     auto factor = [&](float key_scale) { return fmaxf(row_scale * key_scale, 1.17549435e-38f); };   // (positive: -inf stays what it is)
-    float m = -1e30f, l = 0.f;
+    float m = kLowest, l = 0.f;
     bool ok = true;
     for (int i = 0; i < n; i++) {
       const int slot = i % kSlots, key0 = key_of(w, w.begin + i);
@@ -439,7 +439,16 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
           const float z = max3(__float_as_uint(max3(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]))), __float_as_uint(fmaxf(y[3], y[4])), x[16 * g + 15]);
           top = fmaxf(top, fmaf(z, fs[g], lift[g]));
         }
-        if (__any_sync(0xffffffffu, top > m + kLag)) {
+        const bool far = fabsf(top) > kFar && top > -INFINITY;
+        if (__any_sync(0xffffffffu, far || top > m + kLag)) {
+          if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+#pragma unroll
+              for (int k = 0; k < 16; k++) x[16 * g + k] = __float_as_uint(fmaf(__uint_as_float(x[16 * g + k]), fs[g], lift[g]) - lift[g]);
+              fs[g] = 1.f;
+            }
+          }
           const float to = fmaxf(m, ceilf(top)), by = exp2_fast(m - to);
           m = to;
           l *= by;
@@ -545,7 +554,7 @@ __global__ void __launch_bounds__(kRows) join_rows(const __grid_constant__ Porti
   const Walk w = walk_of(P, b, tile * kRows, 0);
   if (w.i0 >= w.count || row / A.group >= w.count) return;
   const float* part = A.part + (((size_t)b * A.C.heads + h) * gridDim.y + tile) * P.shares * kRows * (DV + 2);
-  float m = -1e30f, l = 0.f, x[16];
+  float m = kLowest, l = 0.f, x[16];
 #pragma unroll
   for (int k = 0; k < 16; k++) x[k] = 0.f;
   for (int s = 0; s < P.shares; s++) {

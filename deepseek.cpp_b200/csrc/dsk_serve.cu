@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <mutex>
@@ -105,6 +106,7 @@ int check_cache(const dsk_kv8* c, const dsk_kv8_rows* s) {
   if (s->batch < 0 || s->rows < 0 || s->batch > 65535 || s->table_blocks < 0 || s->table_blocks > (1 << 30) / c->block)
     return fail(-4, "batch %d (at most 65535), %d rows, tables of %d blocks (2^30 tokens at most)", s->batch, s->rows, s->table_blocks);
   if (s->batch && s->rows && (!s->table || !s->first || s->table_blocks == 0)) return fail(-1, "rows: null or empty table, or null first");
+  if (!aligned(s->table, 4) || !aligned(s->first, 4) || !aligned(s->count, 4)) return fail(-1, "rows: table, first and count need 4-byte alignment");
   return check_device(c->device);
 }
 int check_view(const char* what, const dsk_view* v, int dtype) {
@@ -157,8 +159,10 @@ template <typename T> int read_as(const dsk_kv8* c, const dsk_kv8_rows* s, const
 struct Layout { int shape, tiles, row_tiles, ctas, shares, cluster; size_t bytes; };   // shares > 0: attend_rows
 constexpr int kPortionRows = 32;                             // query rows of a key head from which on attend_rows has them
 constexpr int kShapes[4][2] = {{64, 64}, {128, 128}, {192, 128}, {256, 256}};
+int window_of(int window) { return window >= 1 << 30 ? 0 : window; }   // (no table has more tokens)
 int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, int keep_first, Layout* L) {
   if (window < 0 || keep_first < 0) return fail(-4, "window %d and keep_first %d must not be negative", window, keep_first);
+  window = window_of(window);
   if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
   if (s->batch > kv8::kMaxBatch) return fail(-4, "attention over %d sequences: at most %d a call", s->batch, kv8::kMaxBatch);
   const long long rows = (long long)(heads / c->kv_heads) * s->rows;
@@ -177,6 +181,7 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
   }
   L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : rows <= 24 ? 3 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
   L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
+  if ((long long)c->kv_heads * L->row_tiles > INT_MAX) return fail(-4, "%d key heads of %lld query rows", c->kv_heads, rows);
   const int unit = kv8::kWarps * kv8::step_of(L->tiles);
   const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * ((keys + unit - 1) / unit + 1);
   // A cluster to each (sequence, head, tile) where they are few and the tables short enough that eight CTAs have at most eight units each, or where clusters fill the SMs: one launch, no
@@ -273,7 +278,7 @@ extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
   P.C = cache_of(c); P.S = rows_of(s);
   P.q = q->data; P.out = out->data; P.pq = pitch_of(q); P.po = pitch_of(out);
   P.heads = heads; P.group = heads / c->kv_heads; P.row_tiles = L.row_tiles; P.bf16 = dt == DSK_DT_BF16; P.wide_q = wide(q); P.wide_o = wide(out);
-  P.window = window; P.keep = keep_first;
+  P.window = window_of(window); P.keep = keep_first;
   P.scale = scale * 1.44269504088896340736f;
   P.part = static_cast<float*>(workspace);
   P.cluster = L.cluster;
@@ -313,12 +318,13 @@ extern "C" int dsk_verify(const dsk_verify_args* a, void* workspace, size_t work
   if (check_verify(a)) return -1;
   if (a->logits_dtype != DSK_DT_F32 && a->logits_dtype != DSK_DT_F16 && a->logits_dtype != DSK_DT_BF16) return fail(-4, "dsk_verify: logits are F32, F16 or BF16");
   if (!(a->temperature >= 0.f && a->temperature < INFINITY)) return fail(-4, "temperature must be >= 0");
+  if (a->temperature > 0.f && a->temperature < 0x1p-120f) return fail(-4, "a temperature of %g: 0 or at least 2^-120 is needed", (double)a->temperature);   // (64 log2(e) / temperature is an fp32 number)
   if (!a->batch) return 0;
   if (!a->logits || !a->coins || !a->accepted || !a->tokens || (a->drafts && !a->draft_tokens)) return fail(-1, "dsk_verify: null memory");
   size_t need = 0;
   if (dsk_verify_workspace(a, &need)) return -1;
   if (!workspace || !aligned(workspace, 8) || workspace_bytes < need) return fail(-1, "dsk_verify: a workspace of %zu bytes is needed, 8-byte aligned (%zu given)", need, workspace_bytes);
-  if (!aligned(a->logits, size_of(a->logits_dtype)) || !aligned(a->draft_probs, 4)) return fail(-1, "dsk_verify: memory is not aligned to its element");
+  if (!aligned(a->logits, size_of(a->logits_dtype)) || !aligned(a->draft_probs, 4) || !aligned(a->draft_tokens, 4) || !aligned(a->count, 4) || !aligned(a->coins, 4) || !aligned(a->accepted, 4) || !aligned(a->tokens, 4)) return fail(-1, "dsk_verify: memory is not aligned to its element");
   if (check_device(a->device)) return -1;
   OnDevice on(a->device);
   CK(on.error);

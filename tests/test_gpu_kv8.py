@@ -357,6 +357,41 @@ def test_attend_blocks_outside_and_short_tables(rows):
         c.cache.check()
 
 
+@pytest.mark.parametrize("rows", [1, 80, 300])
+def test_attend_lengths_and_windows_at_the_ends_of_their_type(rows):
+    c = Case([160, 150, 150], 1, 64, 64, 32)
+    q = torch.randn(3, rows, 2, 64, device=DEV, dtype=torch.bfloat16)
+    for first, seen in (([-2 ** 31, -2 ** 31 + 5, 150], 2), ([2 ** 31 - 1, 150, 150], 0)):
+        c.device()
+        out = c.cache.attend(q, c.t, ints(first), window=2 ** 31 - 1, keep_first=2 ** 31 - 1)
+        assert (out[:seen] == 0).all()
+        want, tol = expect(c, q.double().cpu().numpy(), [rows] * 3, 2, 0.125, lens=[min(max(n, -1), 1000) for n in first])   # (behind the table's end a row sees all of it)
+        check(out, want, tol, [rows] * 3, "bf16")
+        assert torch.equal(out, c.cache.attend(q, c.t, ints(first)))
+        with pytest.raises(dsk.DskError, match="outside the table"):
+            c.cache.check()
+
+
+@pytest.mark.parametrize("rows", [1, 80])
+@pytest.mark.parametrize("sign,size", [(1, 118), (-1, 118), (1, 28), (-1, 28), (1, 40)])
+def test_attend_largest_queries(rows, sign, size):
+    """Scores of +-2^30 to +-2^120, all of one sign: far apart, so that a row's result is the value of its largest one."""
+    n = 90
+    c = Case([n], 1, 64, 64, 32)
+    c.k &= 0x7f
+    cache = c.device()
+    q = torch.full((1, rows, 2, 64), sign * 2.0 ** size, device=DEV, dtype=torch.bfloat16)
+    out = cache.attend(q, c.t, ints([n]), scale=0.125).float().cpu().numpy()
+    at = lambda codes, scales, t: so.decode_table()[codes[c.table[0][t // 32], 0, t % 32]] * scales[c.table[0][t // 32], 0]
+    score = np.array([sign * at(c.k, c.ks, t).sum() for t in range(n)])
+    for i in range(rows):
+        seen = score[:n - rows + i + 1]
+        best = np.sort(seen)[-2:]
+        assert len(best) < 2 or best[1] - best[0] > 2.0 ** -20 * abs(score).max()
+        want = torch.tensor(at(c.v, c.vs, int(seen.argmax()))).bfloat16().float().numpy()
+        assert (out[0, i] == want).all(), i
+
+
 def test_attend_sequences_that_share_blocks():
     c = Case([256, 256, 256], 2, 128, 128, 64, share=True)
     cache = c.device()

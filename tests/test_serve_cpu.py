@@ -52,7 +52,8 @@ def test_cache_refusals(kw, text):
 
 
 @pytest.mark.parametrize("kw,text", [(dict(batch=-1), "batch"), (dict(batch=65536), "batch"), (dict(rows=-1), "rows"), (dict(table_blocks=-1), "blocks"), (dict(table_blocks=1 << 27), "2^30"),
-                                     (dict(table=None), "null"), (dict(first=None), "null"), (dict(table_blocks=0), "empty")])
+                                     (dict(table=None), "null"), (dict(first=None), "null"), (dict(table_blocks=0), "empty"),
+                                     (dict(table=2 + 16 * 4096), "alignment"), (dict(first=1 + 16 * 4096), "alignment"), (dict(count=2 + 16 * 4096), "alignment")])
 def test_row_refusals(kw, text):
     c, mem = _cache()
     s, x = _rows(mem, **kw), _view(mem)
@@ -74,7 +75,7 @@ def test_null_structures():
 
 
 @pytest.mark.parametrize("kw,text", [(dict(batch=-1), "batch"), (dict(drafts=-1), "drafts"), (dict(drafts=128), "drafts"), (dict(vocab=0), "vocabulary"), (dict(logits_dtype=3), "F32, F16 or BF16"),
-                                     (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"),
+                                     (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"), (dict(temperature=1e-38), "2^-120"), (dict(temperature=1e-45), "2^-120"),
                                      (dict(logits=None), "null"), (dict(coins=None), "null"), (dict(draft_tokens=None), "null"), (dict(), "workspace")])
 def test_verify_refusals(kw, text):
     mem = np.zeros(4096, dtype=np.uint8)

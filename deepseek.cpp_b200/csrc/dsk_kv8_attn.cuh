@@ -21,7 +21,7 @@ namespace dsk {
 namespace kv8 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxBatch = 1024;
-__host__ __device__ constexpr int step_of(int qt) { return qt < 4 ? 32 : 16; }   // keys of a warp's step
+__host__ __device__ constexpr int step_of(int dv, int qt) { return qt < 4 && dv < 256 ? 32 : 16; }   // keys of a warp's step (as two CTAs of an SM have registers and stages for)
 __device__ __forceinline__ long long quotient(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }   // (of numbers >= 0)
 constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
 constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
@@ -61,7 +61,7 @@ template <int DK, int DV, int QT> __host__ __device__ constexpr int stages() {  
 }
 template <int DK, int DV> __host__ __device__ constexpr int stage_bytes(int step) { return step * (DK + 16 + DV + 32) + 16; }
 template <int DK, int DV, int QT> __host__ __device__ constexpr int attn_smem() {
-  return kWarps * stages<DK, DV, QT>() * stage_bytes<DK, DV>(step_of(QT)) + QT * 8 * (2 * DK + 16) + 2 * QT * DV / 4 * 128 + (2 * kWarps + 1) * QT * 8 * 4;
+  return kWarps * stages<DK, DV, QT>() * stage_bytes<DK, DV>(step_of(DV, QT)) + QT * 8 * (2 * DK + 16) + 2 * QT * DV / 4 * 128 + (2 * kWarps + 1) * QT * 8 * 4;
 }
 
 template <int to, int from> __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -216,7 +216,7 @@ __device__ __forceinline__ void join_pieces(const Attn& P, const Seq& q, int b, 
 // (one token behind 1000, 16 heads over 4: 10.2 us by the line with its second launch).
 template <int DK, int DV, int QT, bool SHARED>
 __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
-  constexpr int NST = stages<DK, DV, QT>(), KS = DK + 16, VS = DV + 32, STEP = step_of(QT), HV = STEP / 16, SB = stage_bytes<DK, DV>(STEP), QS = 2 * DK + 16, VCH = DV >= 128 ? 16 : 8,
+  constexpr int NST = stages<DK, DV, QT>(), KS = DK + 16, VS = DV + 32, STEP = step_of(DV, QT), HV = STEP / 16, SB = stage_bytes<DK, DV>(STEP), QS = 2 * DK + 16, VCH = DV >= 128 ? 16 : 8,
                 HF = DV / (8 * VCH), NO = DV / 16;           // NO: tiles of 16 entries; a lane's entries are VCH neighbours, two to a tile
   constexpr bool QREG = QT * DK <= 256;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
   __shared__ long long sums[2][QT * DV / 32];
   const int b = blockIdx.y, hr = blockIdx.x, per = gridDim.x;
   long long before = 0, all = 0;
-  for (int i = threadIdx.x; i < P.S.batch; i += QT * DV) { const int u = sequence<step_of(QT)>(P, i).units; all += u; if (i < b) before += u; }
+  for (int i = threadIdx.x; i < P.S.batch; i += QT * DV) { const int u = sequence<step_of(DV, QT)>(P, i).units; all += u; if (i < b) before += u; }
 #pragma unroll
   for (int o = 16; o; o >>= 1) { before += __shfl_xor_sync(0xffffffffu, before, o); all += __shfl_xor_sync(0xffffffffu, all, o); }
   if ((threadIdx.x & 31) == 0) { sums[0][threadIdx.x >> 5] = before; sums[1][threadIdx.x >> 5] = all; }
@@ -727,7 +727,7 @@ __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
   before = all = 0;
 #pragma unroll
   for (int i = 0; i < QT * DV / 32; i++) { before += sums[0][i]; all += sums[1][i]; }
-  const Seq q = sequence<step_of(QT)>(P, b);
+  const Seq q = sequence<step_of(DV, QT)>(P, b);
   const long long units = q.units, total = all * per, N = ctas_of(ctas, total, (long long)P.S.batch * per), u0 = before * per + hr * units;
   const int i0 = units ? (int)quotient((u0 + 1) * N + total - 1, total) - 1 : 0, i1 = units ? (int)quotient((u0 + units) * N + total - 1, total) - 1 : 0;   // the CTAs of its first and last unit
   if (i0 == i1) return;

@@ -16,18 +16,19 @@
 namespace dsk {
 namespace kv8 {
 
-constexpr int kTile = 128, kRows = 256, kRowThreads = 512, kSlots = 4;       // keys of a tile; rows and threads of a CTA; tiles whose scales are held
+constexpr int kTile = 128, kRowThreads = 512, kSlots = 4;    // keys of a tile; threads of a CTA; tiles whose scales are held
 constexpr float kLag = 14.f;                                 // a row's weights are at most 2^kLag
 
 struct Portion {
-  Attn A;                                                    // row_tiles: of kRows rows
+  Attn A;                                                    // row_tiles: of a CTA's rows
   int shares;                                                // of a row tile's keys (CTAs), joined by join_rows where there are several
 };
 
-template <int DK, int DV> __host__ __device__ constexpr int k_stages() { return DK == 64 ? 3 : 2; }
-template <int DK, int DV> __host__ __device__ constexpr int v_stages() { return DK == 192 ? 1 : DK == 64 ? 3 : 2; }
-template <int DK, int DV> __host__ __device__ constexpr int rows_smem() {
-  return 1024 + kRows * DK * 2 + k_stages<DK, DV>() * kTile * DK * 2 + v_stages<DK, DV>() * kTile * DV * 2 + kSlots * 3 * 8 * 4 + 256;
+// TILES: tiles of 128 query rows of a CTA (256 entries: its shared memory and TMEM are full with one)
+template <int DK, int DV, int TILES> __host__ __device__ constexpr int k_stages() { return DK == 64 ? 3 : DK == 256 ? 1 : 2; }
+template <int DK, int DV, int TILES> __host__ __device__ constexpr int v_stages() { return DK == 256 || (DK == 192 && TILES == 2) ? 1 : DK == 64 ? 3 : 2; }
+template <int DK, int DV, int TILES> __host__ __device__ constexpr int rows_smem() {
+  return 1024 + 128 * TILES * DK * 2 + k_stages<DK, DV, TILES>() * kTile * DK * 2 + v_stages<DK, DV, TILES>() * kTile * DV * 2 + kSlots * 3 * 8 * 4 + 256;
 }
 
 // Bounded.  (Polls that are given a time to sleep wake some 100 cycles late.)
@@ -105,7 +106,7 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr) {
 
 // The keys of a CTA's rows, tile by tile: the first `kept` tiles, then those from `low` on; a share's are begin .. end - 1
 struct Walk { int len, count, first, kept, low, begin, end, i0, i1; };   // first: position of the sequence's first query; i0, i1: tokens of the CTA's first and last row
-__device__ __forceinline__ Walk walk_of(const Portion& P, int b, int row0, int share) {
+__device__ __forceinline__ Walk walk_of(const Portion& P, int b, int row0, int rows, int share) {
   const Attn& A = P.A;
   Walk w;
   const long long room = (long long)A.S.table_blocks << A.C.shift;
@@ -113,7 +114,7 @@ __device__ __forceinline__ Walk walk_of(const Portion& P, int b, int row0, int s
   w.count = A.S.count ? min(max(A.S.count[b], 0), A.S.rows) : A.S.rows;
   w.first = len - w.count;
   w.i0 = row0 / A.group;
-  w.i1 = min((row0 + kRows - 1) / A.group, w.count - 1);
+  w.i1 = min((row0 + rows - 1) / A.group, w.count - 1);
   w.len = (int)min((long long)max(w.first + w.i1 + 1, 0), room);                 // (what the CTA's last row sees)
   const long long lo = (long long)w.first + w.i0 + 1 - A.window;
   w.low = A.window > 0 && lo > 0 ? (int)min(lo, (long long)w.len) / kTile : 0;
@@ -243,21 +244,21 @@ __device__ __forceinline__ void bring(const Attn& A, const Walk& w, int b, int h
   __syncwarp();
 }
 
-template <int DK, int DV>
+template <int DK, int DV, int TILES>
 __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_constant__ Portion P) {
-  constexpr int KST = k_stages<DK, DV>(), VST = v_stages<DK, DV>(), KB = kTile * DK * 2, VB = kTile * DV * 2;
+  constexpr int KST = k_stages<DK, DV, TILES>(), VST = v_stages<DK, DV, TILES>(), KB = kTile * DK * 2, VB = kTile * DV * 2, ROWS = 128 * TILES, VW = TILES == 2 ? 3 : 4;   // VW: warps that bring values
   extern __shared__ unsigned char raw[];
   __shared__ uint32_t tmem_slot;
   __shared__ int nan_seen;
   const Attn& A = P.A;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   unsigned char* gbase = raw + (base - smem_u32(raw));
-  const uint32_t qs = base, ks = qs + kRows * DK * 2, vs = ks + KST * KB, cs = vs + VST * VB, bars = cs + kSlots * 3 * 8 * 4;
+  const uint32_t qs = base, ks = qs + ROWS * DK * 2, vs = ks + KST * KB, cs = vs + VST * VB, bars = cs + kSlots * 3 * 8 * 4;
   float* scales = reinterpret_cast<float*>(gbase + (cs - base));          // [slot][key scale | exponent of the value scale | its reciprocal, zero: not there][16 keys]
   const uint32_t kfull = bars, kempty = bars + 24, vfull = bars + 48, vempty = bars + 72, sfull = bars + 96, pfull = bars + 112, pvdone = bars + 128, cfull = bars + 144, cdone = bars + 176, flushed = bars + 184, qfull = bars + 192;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int h = blockIdx.x / P.shares, share = blockIdx.x - h * P.shares, b = blockIdx.z, row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kRows;   // late rows, which see most, first
-  const Walk w = walk_of(P, b, row0, share);
+  const int h = blockIdx.x / P.shares, share = blockIdx.x - h * P.shares, b = blockIdx.z, row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS;   // late rows, which see most, first
+  const Walk w = walk_of(P, b, row0, ROWS, share);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     const long long len = A.S.first[b];
     if (len < 0 || len > (long long)A.S.table_blocks << A.C.shift) note(A.C, ST_RANGE);
@@ -265,11 +266,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   if (w.i0 >= w.count) return;                               // (the whole CTA: none of its rows exists)
   const int n = w.end - w.begin;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 3; i++) { mbar_init(kfull + 8 * i, 4); mbar_init(kempty + 8 * i, 1); mbar_init(vfull + 8 * i, 3); mbar_init(vempty + 8 * i, 1); }
+    for (int i = 0; i < 3; i++) { mbar_init(kfull + 8 * i, 4); mbar_init(kempty + 8 * i, 1); mbar_init(vfull + 8 * i, VW); mbar_init(vempty + 8 * i, 1); }
     for (int i = 0; i < 2; i++) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); }
     for (int i = 0; i < kSlots; i++) mbar_init(cfull + 8 * i, 1);
-    mbar_init(cdone, 3);
-    mbar_init(qfull, 8);
+    mbar_init(cdone, VW);
+    mbar_init(qfull, 4 * TILES);
     mbar_init(flushed, 1);
     nan_seen = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -282,15 +283,15 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [2][128], results [2][128]
+  const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [2][128], results [tile][DV]
 
   if (warp >= 12) {
     if (warp == 12) {
       const uint32_t lead = hy::tc_elect();
       const uint32_t idesc = (1u << 4) | ((uint32_t)(kTile / 16) << 24);       // fp32 sums, fp16 x fp16, 128 rows
       const uint32_t sdesc = idesc | ((uint32_t)(kTile / 8) << 17), pdesc = idesc | (1u << 16) | ((uint32_t)(DV / 8) << 17);
-      auto score = [&](int t, int stage) {
-        const uint64_t a = hy::tc_desc(qs + t * (kTile * DK * 2)), k = hy::tc_desc(ks + stage * KB);
+      auto score = [&](int t, int stage) {                   // one tile of rows: into alternate columns
+        const uint64_t a = hy::tc_desc(qs + (TILES == 2 ? t * (kTile * DK * 2) : 0)), k = hy::tc_desc(ks + stage * KB);
 #pragma unroll
         for (int g = 0; g < DK / 64; g++)
 #pragma unroll
@@ -301,34 +302,51 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       if (alive) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         score(0, 0);
-        score(1, 0);
+        if (TILES == 2) score(1, 0);
         commit(kempty, lead);
       }
       int kst = 0, vst = 0;
       uint32_t kturn = 0, vturn = 0;                         // the stage that was read last, parity of its tile
       for (int i = 0; i < n && alive; i++) {
-        alive = wait_warp(vfull + 8 * vst, vturn, A.C);
-        if (!alive) break;
         const uint64_t v = value_desc(vs + vst * VB);
         const bool more = i + 1 < n;
         if (more && ++kst == KST) { kst = 0; kturn ^= 1; }
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          if (!alive) continue;
-          alive = wait_warp(pfull + 8 * t, i & 1, A.C);
-          if (!alive) continue;
+        if constexpr (TILES == 1) {                          // the next scores' products run under this tile's softmax, where the weights of the tile ahead were read
+          if (more) {
+            alive = wait_warp(kfull + 8 * kst, kturn, A.C) && (i == 0 || wait_warp(pvdone, (i - 1) & 1, A.C));
+            if (!alive) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            score((i + 1) & 1, kst);
+            commit(kempty + 8 * kst, lead);
+          }
+          alive = wait_warp(vfull + 8 * vst, vturn, A.C) && wait_warp(pfull + 8 * (i & 1), (i >> 1) & 1, A.C);
+          if (!alive) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-          for (int u = 0; u < kTile / 16; u++) mma_ts(o_at + t * 128, tmem + t * 128 + (u >> 2) * 64 + (u & 3) * 8, v + u * 128, pdesc, i > 0 || u > 0, lead);
-          commit(pvdone + 8 * t, lead);
-          if (t == 1) commit(vempty + 8 * vst, lead);
-          if (!more) continue;
-          if (t == 0) { alive = wait_warp(kfull + 8 * kst, kturn, A.C); if (!alive) continue; }
-          alive = wait_warp(pvdone + 8 * t, i & 1, A.C);     // the weights are read: their columns may have the next scores
-          if (!alive) continue;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          score(t, kst);
-          if (t == 1) commit(kempty + 8 * kst, lead);
+          for (int u = 0; u < kTile / 16; u++) mma_ts(o_at, tmem + (i & 1) * 128 + (u >> 2) * 64 + (u & 3) * 8, v + u * 128, pdesc, i > 0 || u > 0, lead);
+          commit(pvdone, lead);
+          commit(vempty + 8 * vst, lead);
+        } else {
+          alive = wait_warp(vfull + 8 * vst, vturn, A.C);
+          if (!alive) break;
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            if (!alive) continue;
+            alive = wait_warp(pfull + 8 * t, i & 1, A.C);
+            if (!alive) continue;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int u = 0; u < kTile / 16; u++) mma_ts(o_at + t * 128, tmem + t * 128 + (u >> 2) * 64 + (u & 3) * 8, v + u * 128, pdesc, i > 0 || u > 0, lead);
+            commit(pvdone + 8 * t, lead);
+            if (t == 1) commit(vempty + 8 * vst, lead);
+            if (!more) continue;
+            if (t == 0) { alive = wait_warp(kfull + 8 * kst, kturn, A.C); if (!alive) continue; }
+            alive = wait_warp(pvdone + 8 * t, i & 1, A.C);   // the weights are read: their columns may have the next scores
+            if (!alive) continue;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            score(t, kst);
+            if (t == 1) commit(kempty + 8 * kst, lead);
+          }
         }
         if (++vst == VST) { vst = 0; vturn ^= 1; }
       }
@@ -336,16 +354,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       wait_warp(flushed, 0, A.C);
     }
     __syncwarp();
-    if (warp > 12) {
-      bring<DV, (kTile + 23) / 24, 3>(A, w, b, h, 1, warp - 13, lane, vs, VB, VST, vfull, vempty, 0, nullptr, &nan_seen);
+    if (TILES == 2 && warp > 12) {
+      bring<DV, (kTile + 8 * VW - 1) / (8 * VW), VW>(A, w, b, h, 1, warp - 13, lane, vs, VB, VST, vfull, vempty, 0, nullptr, &nan_seen);
       if (lane == 0) hy::tc_arrive(cdone);
     }
   } else if (warp >= 8) {
     bring<DK, kTile / 32, 4>(A, w, b, h, 0, warp - 8, lane, ks, KB, KST, kfull, kempty, cfull, scales, &nan_seen);
-    } else {
+  } else if (TILES == 1 && warp >= 4) {
+    bring<DV, kTile / (8 * VW), VW>(A, w, b, h, 1, warp - 4, lane, vs, VB, VST, vfull, vempty, 0, nullptr, &nan_seen);
+    if (lane == 0) hy::tc_arrive(cdone);
+  } else {
     const int t = warp >> 2, quad = warp & 3, row = row0 + threadIdx.x, i_row = row / A.group, pos = w.first + i_row;
     const int r_first = (row0 + t * 128) / A.group, r_last = min((row0 + t * 128 + 127) / A.group, w.i1);   // tokens of the tile's rows
-    const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_at = tmem + t * 128 + lanes, res = o_at + t * 128 + lanes;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16, s_0 = tmem + t * 128 + lanes, res = o_at + t * 128 + lanes;
     // the thread's query row as fp16, by a power of two of its own (dsk_kv8_attn.cuh), while the first keys are brought: [tile][64 entries][row], 16-byte pieces swizzled
     float row_scale;
     {
@@ -394,6 +415,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
     auto factor = [&](float key_scale) { return fmaxf(row_scale * key_scale, 1.17549435e-38f); };   // (positive: -inf stays what it is)
     float m = kLowest, l = 0.f;
     bool ok = true;
+    const bool idle = (row0 + warp * 32) / A.group >= w.count;              // none of the warp's rows exists
     for (int i = 0; i < n; i++) {
       const int slot = i % kSlots, key0 = key_of(w, w.begin + i);
       ok = wait_warp(cfull + 8 * slot, (i / kSlots) & 1, A.C);
@@ -408,8 +430,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
         lift[0] = l4.x; lift[1] = l4.y; lift[2] = l4.z; lift[3] = l4.w;
       };
       scales_of(1);
-      ok = ok && wait_warp(sfull + 8 * t, i & 1, A.C);
+      const uint32_t s_at = TILES == 2 ? s_0 : s_0 + (i & 1) * 128;
+      ok = ok && (TILES == 2 ? wait_warp(sfull + 8 * t, i & 1, A.C) : wait_warp(sfull + 8 * (i & 1), (i >> 1) & 1, A.C));
       if (!ok) break;
+      if (idle) {                                            // (its rows' results are whatever comes of the scores as weights, and go nowhere)
+        __syncwarp();
+        if (lane == 0) hy::tc_arrive(TILES == 2 ? pfull + 8 * t : pfull + 8 * (i & 1));
+        continue;
+      }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // Half a row of scores in registers at a time, each read once: the reference may lag behind the maximum by kLag, within fp16's range, so that the first half's weights do not wait for
       // the second half's maximum; where that moves the reference after all, weights that are stored already are scaled again, exactly, since references are whole numbers.
@@ -452,7 +480,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
           const float to = fmaxf(m, ceilf(top)), by = exp2_fast(m - to);
           m = to;
           l *= by;
-          if (i > 0) {                                       // (the tile's last product was through ahead of these scores)
+          if (i > 0) {                                       // (two tiles of rows: the tile's last product was through ahead of these scores)
+            if (TILES == 1) {
+              ok = wait_warp(pvdone, (i - 1) & 1, A.C);
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
 #pragma unroll 1
             for (int d = 0; d < DV; d += 16) {
               uint32_t y[16];
@@ -498,7 +530,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) hy::tc_arrive(pfull + 8 * t);
+      if (lane == 0) hy::tc_arrive(TILES == 2 ? pfull + 8 * t : pfull + 8 * (i & 1));
     }
     ok = ok && wait_warp(cdone, 0, A.C) && (n == 0 || wait_warp(pvdone + 8 * t, (n - 1) & 1, A.C));
     if (ok) {
@@ -522,7 +554,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
         }
       }
       const float inv = P.shares > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      float* part = A.part + ((((size_t)b * A.C.heads + h) * gridDim.y + (gridDim.y - 1 - blockIdx.y)) * P.shares + share) * kRows * (DV + 2) + threadIdx.x;
+      float* part = A.part + ((((size_t)b * A.C.heads + h) * gridDim.y + (gridDim.y - 1 - blockIdx.y)) * P.shares + share) * ROWS * (DV + 2) + threadIdx.x;
 #pragma unroll
       for (int c = 0; c < DV; c += 16) {
         uint32_t x[16];
@@ -532,10 +564,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
         for (int k = 0; k < 16; k++) f[k] = n == 0 ? 0.f : (lost[c / 32] >> ((c & 31) + k)) & 1 ? NAN : __uint_as_float(x[k]);
         if (P.shares > 1) {                                  // [entry][row]: neighbouring threads side by side
 #pragma unroll
-          for (int k = 0; k < 16; k++) part[(c + k) * kRows] = f[k];
+          for (int k = 0; k < 16; k++) if (i_row < w.count) part[(c + k) * ROWS] = f[k];
         } else Out::store(A, Seq{w.len, w.count, 0, 0, 0, 0, 0, 0}, b, h, row, c, 16, f, inv);
       }
-      if (P.shares > 1) { part[DV * kRows] = m; part[(DV + 1) * kRows] = l; }
+      if (P.shares > 1 && i_row < w.count) { part[DV * ROWS] = m; part[(DV + 1) * ROWS] = l; }
     }
   }
   __syncthreads();
@@ -545,25 +577,46 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
   }
 }
 
-// Joins the shares of a row tile's keys: a thread has 16 entries of a row
-template <int DV>
-__global__ void __launch_bounds__(kRows) join_rows(const __grid_constant__ Portion P) {
-  grid_wait();
+// Joins the shares of a row tile's keys, eight at a time: a thread has 16 entries of a row
+template <int DV, int TILES>
+__global__ void __launch_bounds__(128 * TILES) join_rows(const __grid_constant__ Portion P) {
+  constexpr int ROWS = 128 * TILES, AT = 8;
   const Attn& A = P.A;
-  const int h = blockIdx.x / (DV / 16), d0 = blockIdx.x % (DV / 16) * 16, tile = blockIdx.y, b = blockIdx.z, row = tile * kRows + threadIdx.x;
-  const Walk w = walk_of(P, b, tile * kRows, 0);
+  const int h = blockIdx.x / (DV / 16), d0 = blockIdx.x % (DV / 16) * 16, tile = blockIdx.y, b = blockIdx.z, row = tile * ROWS + threadIdx.x;
+  const Walk w = walk_of(P, b, tile * ROWS, ROWS, 0);
   if (w.i0 >= w.count || row / A.group >= w.count) return;
-  const float* part = A.part + (((size_t)b * A.C.heads + h) * gridDim.y + tile) * P.shares * kRows * (DV + 2);
+  const float* part = A.part + (((size_t)b * A.C.heads + h) * gridDim.y + tile) * P.shares * ROWS * (DV + 2) + threadIdx.x;
+  grid_wait();
   float m = kLowest, l = 0.f, x[16];
 #pragma unroll
   for (int k = 0; k < 16; k++) x[k] = 0.f;
-  for (int s = 0; s < P.shares; s++) {
-    const float* from = part + (size_t)s * kRows * (DV + 2) + threadIdx.x;
-    const float pm = from[DV * kRows], pl = from[(DV + 1) * kRows], to = fmaxf(m, pm), f = exp2_fast(m - to), g = exp2_fast(pm - to);
-    m = to;
-    l = l * f + pl * g;
+  for (int s = 0; s < P.shares; s += AT) {
+    float pm[AT], pl[AT], px[AT][16], to = m;
 #pragma unroll
-    for (int k = 0; k < 16; k++) x[k] = x[k] * f + from[(d0 + k) * kRows] * g;
+    for (int u = 0; u < AT; u++) {
+      pm[u] = -INFINITY;
+      if (s + u >= P.shares) continue;
+      const float* from = part + (size_t)(s + u) * ROWS * (DV + 2);
+      pm[u] = from[DV * ROWS];
+      pl[u] = from[(DV + 1) * ROWS];
+#pragma unroll
+      for (int k = 0; k < 16; k++) px[u][k] = from[(d0 + k) * ROWS];
+    }
+#pragma unroll
+    for (int u = 0; u < AT; u++) to = fmaxf(to, pm[u]);
+    const float f = exp2_fast(m - to);
+    m = to;
+    l *= f;
+#pragma unroll
+    for (int k = 0; k < 16; k++) x[k] *= f;
+#pragma unroll
+    for (int u = 0; u < AT; u++) {
+      if (s + u >= P.shares) break;
+      const float g = exp2_fast(pm[u] - m);
+      l = fmaf(pl[u], g, l);
+#pragma unroll
+      for (int k = 0; k < 16; k++) x[k] = fmaf(px[u][k], g, x[k]);
+    }
   }
   Out::store(A, Seq{w.len, w.count, 0, 0, 0, 0, 0, 0}, b, h, row, d0, 16, x, l == 0.f ? 0.f : 1.f / l);
 }

@@ -166,29 +166,31 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
   if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
   if (s->batch > kv8::kMaxBatch) return fail(-4, "attention over %d sequences: at most %d a call", s->batch, kv8::kMaxBatch);
   const long long rows = (long long)(heads / c->kv_heads) * s->rows;
-  if (rows > (1 << 23)) return fail(-4, "%lld query rows of a key head: at most 2^23", rows);
+  if (rows > (1 << 22)) return fail(-4, "%lld query rows of a key head: at most 2^22", rows);
   for (L->shape = 0; c->dim_k > kShapes[L->shape][0] || c->dim_v > kShapes[L->shape][1];) L->shape++;
   const int sms = multiprocessors(c->device);
   if (!sms) return fail(-2, "device %d: no attributes", c->device);
   const long long keys = (long long)s->table_blocks * c->block;
   L->shares = L->cluster = 0;
-  if (rows > kPortionRows && L->shape < 3) {
-    L->row_tiles = (int)((rows + kv8::kRows - 1) / kv8::kRows);
+  if (rows > kPortionRows) {
+    L->tiles = rows > 128 && L->shape < 3 ? 2 : 1;
+    const int each = 128 * L->tiles;
+    L->row_tiles = (int)((rows + each - 1) / each);
     const long long tiles = (long long)s->batch * c->kv_heads * L->row_tiles;
     L->shares = (int)std::max<long long>(1, std::min<long long>(sms / tiles, (keys + kv8::kTile - 1) / kv8::kTile));   // where the row tiles leave SMs idle, their keys are shared out
-    L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * kv8::kRows * (kShapes[L->shape][1] + 2) * sizeof(float) : 0;
+    L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * each * (kShapes[L->shape][1] + 2) * sizeof(float) : 0;
     return 0;
   }
   L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : rows <= 24 ? 3 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
   L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
   if ((long long)c->kv_heads * L->row_tiles > INT_MAX) return fail(-4, "%d key heads of %lld query rows", c->kv_heads, rows);
-  const int unit = kv8::kWarps * kv8::step_of(L->tiles);
+  const int unit = kv8::kWarps * kv8::step_of(kShapes[L->shape][1], L->tiles);
   const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * ((keys + unit - 1) / unit + 1);
   // A cluster to each (sequence, head, tile) where they are few and the tables short enough that eight CTAs have at most eight units each, or where clusters fill the SMs: one launch, no
   // workspace.  Otherwise the line: any number of CTAs to a head, whatever the lengths.
   const long long each = (long long)s->batch * c->kv_heads * L->row_tiles, most = window ? std::min(keys, (long long)window + s->rows + keep_first) : keys, longest = (most + unit - 1) / unit + (window ? 2 : 0);
   for (int k = 8; k >= 2 && !L->cluster; k /= 2)
-    if (each * k <= 2 * sms && longest <= 8 * k) L->cluster = k;
+    if (each * k <= 7 * sms / 4 && longest <= 4 * k) L->cluster = k;
   if (L->cluster) { L->ctas = (int)each * L->cluster; L->bytes = 0; return 0; }
   L->ctas = (int)std::min<long long>(2 * sms, std::max<long long>(1, units));
   L->bytes = (size_t)2 * L->ctas * L->tiles * (kShapes[L->shape][1] / 16 * 128 + 16) * sizeof(float);
@@ -207,16 +209,19 @@ template <int DK, int DV, int QT> int attend_as(const kv8::Attn& P, const Layout
   CK(launch_behind(kv8::join<DV, QT>, dim3(P.C.heads * P.row_tiles, P.S.batch), dim3(QT * DV), 0, stream, 1, P, L.ctas));
   return 0;
 }
-template <int DK, int DV> int attend_portion(const kv8::Attn& A, const Layout& L, int device, cudaStream_t stream) {
+template <int DK, int DV, int TILES> int attend_portion(const kv8::Attn& A, const Layout& L, int device, cudaStream_t stream) {
   const kv8::Portion P{A, L.shares};
-  CK((allow<kv8::attend_rows<DK, DV>>(device, kv8::rows_smem<DK, DV>())));
-  kv8::attend_rows<DK, DV><<<dim3(A.C.heads * L.shares, L.row_tiles, A.S.batch), kv8::kRowThreads, kv8::rows_smem<DK, DV>(), stream>>>(P);
+  CK((allow<kv8::attend_rows<DK, DV, TILES>>(device, kv8::rows_smem<DK, DV, TILES>())));
+  kv8::attend_rows<DK, DV, TILES><<<dim3(A.C.heads * L.shares, L.row_tiles, A.S.batch), kv8::kRowThreads, kv8::rows_smem<DK, DV, TILES>(), stream>>>(P);
   CK(cudaGetLastError());
-  if (L.shares > 1) CK(launch_behind(kv8::join_rows<DV>, dim3(A.C.heads * (DV / 16), L.row_tiles, A.S.batch), dim3(kv8::kRows), 0, stream, 1, P));
+  if (L.shares > 1) CK(launch_behind(kv8::join_rows<DV, TILES>, dim3(A.C.heads * (DV / 16), L.row_tiles, A.S.batch), dim3(128 * TILES), 0, stream, 1, P));
   return 0;
 }
 template <int DK, int DV> int attend_tiles(const kv8::Attn& P, const Layout& L, int device, cudaStream_t stream) {
-  if constexpr (DV < 256) if (L.shares) return attend_portion<DK, DV>(P, L, device, stream);
+  if (L.shares) {
+    if constexpr (DV < 256) if (L.tiles == 2) return attend_portion<DK, DV, 2>(P, L, device, stream);
+    return attend_portion<DK, DV, 1>(P, L, device, stream);
+  }
   if (L.tiles == 1) return attend_as<DK, DV, 1>(P, L, device, stream);
   if constexpr (DV < 256) {
     if (L.tiles == 3) return attend_as<DK, DV, 3>(P, L, device, stream);

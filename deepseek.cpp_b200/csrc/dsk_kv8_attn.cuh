@@ -1,14 +1,18 @@
 // dsk_kv8_attn.cuh — softmax attention of decoded tokens and drafts over the 8-bit cache (dsk_kv8.cuh).
 //
 // The queries of a key head are its query heads' queries, `group` heads x `rows` tokens, in tiles of 8.  Products run on mma.sync with keys and values as the left operand:
-// scores (16 keys x 8 queries) = K Q^T, results (16 entries x 8 queries) = V^T W; a left operand is converted once whatever the number of query tiles (1, 2 or 4), and no row of a product is
+// scores (16 keys x 8 queries) = K Q^T, results (16 entries x 8 queries) = V^T W; a left operand is converted once whatever the number of query tiles (1 to 3), and no row of a product is
 // empty with the few queries of decoding.  An E4M3 code is exact in fp16, so keys and values go from their codes to operands by a conversion alone; a query is divided by a power
 // of two that puts its largest entry near 2^10 (what that leaves below fp16's range is 2^-24 of it).  The scales are applied around the products: the key block's to the
 // scores, the value block's inside the softmax, w_j = 2^(t_j - m) with t_j = score_j + log2(value scale), so that a weight with its scale is one fp16 number of at most 2^kSlack
 // and the sum takes w_j / (value scale).  Rounding: the weights to fp16, 2^-11 of each; queries in fp16 or bf16 are exact.
-// Work: the steps (16 or 32 keys) of all sequences, key heads and query tiles lie in one line that the CTAs share out evenly, four steps to a unit, whatever the lengths; a CTA that has
+// Work: the steps (32 keys, 16 where heads have 256 entries) of all sequences, key heads and query tiles lie in one line that the CTAs share out evenly, four steps to a unit, whatever the lengths; a CTA that has
 // a whole (sequence, head, tile) stores it, pieces are joined by `join`.  Every warp has every fourth step, with stages of its own that cp.async fills: no barrier but where
 // a piece ends, and the copies run on across pieces.
+// A call of few pieces has clusters instead of the line (SHARED).
+// Bound: with many queries' worth of bytes the instructions of a step (some 560 for 32 keys and a tile of 8 queries: conversions, fragments, products, softmax; steps of 16 keys spend more of
+// them on what a step does once), in small calls the chain of a step and the joins.  64 sequences of up to 16000 tokens, 16 heads of 128 over 4: 107 us (533 MB: 5.0 TB/s; a measured copy 6.5);
+// a token and four drafts of 16 sequences, window 1024: 18 us; one token behind 1000: 8.4 us.  With queries as the left operand, half of whose rows were empty: 295 us for the first.
 // Fragments come from shared memory as whole 16-byte pieces, entries and keys permuted alike on both sides of a product: a quarter warp's lanes (two
 // keys x four pieces) are keys j and j + 4, whose rows lie 16 banks apart.
 #pragma once
@@ -21,7 +25,7 @@ namespace dsk {
 namespace kv8 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxBatch = 1024;
-__host__ __device__ constexpr int step_of(int dv, int qt) { return qt < 4 && dv < 256 ? 32 : 16; }   // keys of a warp's step (as two CTAs of an SM have registers and stages for)
+__host__ __device__ constexpr int step_of(int dv) { return dv < 256 ? 32 : 16; }   // keys of a warp's step (as two CTAs of an SM have registers and stages for)
 __device__ __forceinline__ long long quotient(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }   // (of numbers >= 0)
 constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
 constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
@@ -57,11 +61,11 @@ template <int STEP> __device__ __forceinline__ Seq sequence(const Attn& P, int b
 }
 
 template <int DK, int DV, int QT> __host__ __device__ constexpr int stages() {   // as many as two CTAs of an SM have room for
-  return DK == 64 ? (QT < 4 ? 3 : 6) : DK == 128 ? (QT < 4 ? 2 : 3) : 2;
+  return DK == 64 ? 3 : 2;
 }
 template <int DK, int DV> __host__ __device__ constexpr int stage_bytes(int step) { return step * (DK + 16 + DV + 32) + 16; }
 template <int DK, int DV, int QT> __host__ __device__ constexpr int attn_smem() {
-  return kWarps * stages<DK, DV, QT>() * stage_bytes<DK, DV>(step_of(DV, QT)) + QT * 8 * (2 * DK + 16) + 2 * QT * DV / 4 * 128 + (2 * kWarps + 1) * QT * 8 * 4;
+  return kWarps * stages<DK, DV, QT>() * stage_bytes<DK, DV>(step_of(DV)) + QT * 8 * (2 * DK + 16) + 2 * QT * DV / 4 * 128 + (2 * kWarps + 1) * QT * 8 * 4;
 }
 
 template <int to, int from> __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -213,10 +217,10 @@ __device__ __forceinline__ void join_pieces(const Attn& P, const Seq& q, int b, 
 }
 
 // DK, DV: entries of keys and values, rounded up; QT: tiles of 8 queries.  SHARED: P.cluster CTAs have one (sequence, head, tile) and join their pieces in one another's shared memory
-// (one token behind 1000, 16 heads over 4: 10.2 us by the line with its second launch).
+// (one token behind 1000, 16 heads over 4: 8.7 us, 9.2 by the line with its second launch, whose call takes the host 14 us instead of 9).
 template <int DK, int DV, int QT, bool SHARED>
 __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
-  constexpr int NST = stages<DK, DV, QT>(), KS = DK + 16, VS = DV + 32, STEP = step_of(DV, QT), HV = STEP / 16, SB = stage_bytes<DK, DV>(STEP), QS = 2 * DK + 16, VCH = DV >= 128 ? 16 : 8,
+  constexpr int NST = stages<DK, DV, QT>(), KS = DK + 16, VS = DV + 32, STEP = step_of(DV), HV = STEP / 16, SB = stage_bytes<DK, DV>(STEP), QS = 2 * DK + 16, VCH = DV >= 128 ? 16 : 8,
                 HF = DV / (8 * VCH), NO = DV / 16;           // NO: tiles of 16 entries; a lane's entries are VCH neighbours, two to a tile
   constexpr bool QREG = QT * DK <= 256;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -719,7 +723,7 @@ __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
   __shared__ long long sums[2][QT * DV / 32];
   const int b = blockIdx.y, hr = blockIdx.x, per = gridDim.x;
   long long before = 0, all = 0;
-  for (int i = threadIdx.x; i < P.S.batch; i += QT * DV) { const int u = sequence<step_of(DV, QT)>(P, i).units; all += u; if (i < b) before += u; }
+  for (int i = threadIdx.x; i < P.S.batch; i += QT * DV) { const int u = sequence<step_of(DV)>(P, i).units; all += u; if (i < b) before += u; }
 #pragma unroll
   for (int o = 16; o; o >>= 1) { before += __shfl_xor_sync(0xffffffffu, before, o); all += __shfl_xor_sync(0xffffffffu, all, o); }
   if ((threadIdx.x & 31) == 0) { sums[0][threadIdx.x >> 5] = before; sums[1][threadIdx.x >> 5] = all; }
@@ -727,12 +731,12 @@ __global__ void __launch_bounds__(QT * DV) join(const Attn P, int ctas) {
   before = all = 0;
 #pragma unroll
   for (int i = 0; i < QT * DV / 32; i++) { before += sums[0][i]; all += sums[1][i]; }
-  const Seq q = sequence<step_of(DV, QT)>(P, b);
+  const Seq q = sequence<step_of(DV)>(P, b);
   const long long units = q.units, total = all * per, N = ctas_of(ctas, total, (long long)P.S.batch * per), u0 = before * per + hr * units;
   const int i0 = units ? (int)quotient((u0 + 1) * N + total - 1, total) - 1 : 0, i1 = units ? (int)quotient((u0 + units) * N + total - 1, total) - 1 : 0;   // the CTAs of its first and last unit
+  grid_wait();                                               // (every thread: what follows this kernel then follows the one ahead as well)
   if (i0 == i1) return;
   const int own = quotient(i0 * total, N) >= u0 ? 0 : 1;     // the first one's piece: its first or its last (the others' pieces are their first)
-  grid_wait();
   const int head = hr / P.row_tiles;
   join_pieces<DV, QT>(P, q, b, head, (hr - head * P.row_tiles) * QT * 8, threadIdx.x >> 5, threadIdx.x & 31, i1 - i0 + 1,
                       [&](int i) { return (const float*)P.part + (size_t)(2 * (i0 + i) + (i == 0 ? own : 0)) * (QT * (NO * 128 + 16)); });

@@ -1,13 +1,16 @@
-// dsk_kv8_tc5.cuh — softmax attention of portions (many query rows to a key head) over the 8-bit cache on the 5th-generation tensor cores, keys up to 192 entries, values up to 128.
+// dsk_kv8_tc5.cuh — softmax attention of portions (many query rows to a key head) over the 8-bit cache on the 5th-generation tensor cores.
 //
-// A CTA has 256 query rows of a key head (its query heads' rows one behind the other, so that all of them share the keys), two tiles of 128, and walks the keys that they see in tiles
-// of 128.  Roles: seven warps bring codes from the cache, four the keys' and three the values', turn them into fp16 (exact) and store them as swizzled operands, so that the cache
-// crosses HBM and L2 as bytes; one thread
-// issues the products, scores into TMEM, weights from TMEM; two groups of four warps have the softmax, a thread to a row, each group for its own tile, so that one tile's products run under the
-// other one's softmax.  Scales and weights as in dsk_kv8_attn.cuh: key scales on the scores, value scales inside the exponent, fp16 weights of at most 2^kLag.
-// The results stay in TMEM; they are scaled again only where a row's maximum is 2^kLag ahead of the reference of its weights, by the thread that has the row.  Weights lie where the scores were:
-// a tile's next scores wait for the product that reads its weights.
+// A CTA has query rows of a key head (its query heads' rows one behind the other, so that all of them share the keys), two tiles of 128 or one (up to 128 rows; heads of 256 entries, whose
+// queries, keys and values fill shared memory), and walks the keys that they see in tiles of 128.  Roles: seven or eight warps bring codes from the cache, four the keys' and three or four the
+// values', turn them into fp16 (exact) and store them as swizzled operands, so that the cache crosses HBM and L2 as bytes; one thread issues the products, scores into TMEM, weights from TMEM;
+// a group of four warps for each tile of rows has the softmax, a thread to a row.  Two tiles: one's products run under the other's softmax, weights lie where the scores were, and a
+// tile's next scores wait for the product that reads its weights.  One tile: scores lie in two places in turn, and the next tile's products run under this one's softmax.
+// Scales and weights as in dsk_kv8_attn.cuh: key scales on the scores, value scales inside the exponent, fp16 weights of at most 2^kLag.
+// The results stay in TMEM; they are scaled again only where a row's maximum is 2^kLag ahead of the reference of its weights, by the thread that has the row.
 // NaN among values: a tile that some row does not see whole goes to the products with zeros in their place, and rows that do see one get it back at the end.
+// Bound: the softmax.  Of some 4500 cycles for 256 rows and 128 keys of 192 + 128 entries the weights of one group take 1500 (1024 of the exponentials' pipe), its maxima 500, the products
+// 2560 of the tensor pipe, and a group's products and the way there and back stand 1700 behind its weights.  2048 queries behind 3952 tokens, 16 heads of 192 + 128: 133 us (104 GFLOP:
+// 785 TFLOP/s; a measured product of matrices 1638), heads of 256: 235 us (167 GFLOP: 710), 3 x 777 queries of 16 heads of 64 over 4 with a window of 512: 27 us.
 #pragma once
 
 #include "dsk_kv8_attn.cuh"
@@ -25,7 +28,7 @@ struct Portion {
 };
 
 // TILES: tiles of 128 query rows of a CTA (256 entries: its shared memory and TMEM are full with one)
-template <int DK, int DV, int TILES> __host__ __device__ constexpr int k_stages() { return DK == 64 ? 3 : DK == 256 ? 1 : 2; }
+template <int DK, int DV, int TILES> __host__ __device__ constexpr int k_stages() { return DK == 64 && TILES == 2 ? 3 : DK == 256 ? 1 : 2; }   // (one tile of rows: keys three tiles ahead would bring scales over those that a softmax may still read)
 template <int DK, int DV, int TILES> __host__ __device__ constexpr int v_stages() { return DK == 256 || (DK == 192 && TILES == 2) ? 1 : DK == 64 ? 3 : 2; }
 template <int DK, int DV, int TILES> __host__ __device__ constexpr int rows_smem() {
   return 1024 + 128 * TILES * DK * 2 + k_stages<DK, DV, TILES>() * kTile * DK * 2 + v_stages<DK, DV, TILES>() * kTile * DV * 2 + kSlots * 3 * 8 * 4 + 256;
@@ -584,9 +587,9 @@ __global__ void __launch_bounds__(128 * TILES) join_rows(const __grid_constant__
   const Attn& A = P.A;
   const int h = blockIdx.x / (DV / 16), d0 = blockIdx.x % (DV / 16) * 16, tile = blockIdx.y, b = blockIdx.z, row = tile * ROWS + threadIdx.x;
   const Walk w = walk_of(P, b, tile * ROWS, ROWS, 0);
+  grid_wait();                                               // (every thread: what follows this kernel then follows the one ahead as well)
   if (w.i0 >= w.count || row / A.group >= w.count) return;
   const float* part = A.part + (((size_t)b * A.C.heads + h) * gridDim.y + tile) * P.shares * ROWS * (DV + 2) + threadIdx.x;
-  grid_wait();
   float m = kLowest, l = 0.f, x[16];
 #pragma unroll
   for (int k = 0; k < 16; k++) x[k] = 0.f;

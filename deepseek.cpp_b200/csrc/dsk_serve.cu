@@ -157,7 +157,9 @@ template <typename T> int read_as(const dsk_kv8* c, const dsk_kv8_rows* s, const
 
 // How an attention call is laid out
 struct Layout { int shape, tiles, row_tiles, ctas, shares, cluster; size_t bytes; };   // shares > 0: attend_rows
-constexpr int kPortionRows = 32;                             // query rows of a key head from which on attend_rows has them
+// Query rows of a key head up to which attend_tokens has them, attend_rows behind that.  us for 16 sequences of 4000 tokens, 4 key heads, attend_tokens / attend_rows: 128 entries,
+// 24 rows 31 / 38, 32 rows 46 / 38; 192, 16 rows 44 / 41, 24 rows 54 / 41 (one sequence 17 / 20); 64, 24 rows 24 / 33, 32 rows 30 / 33; 256, 16 rows 44 / 80, 32 rows (two tiles twice) 72 / 80.
+constexpr int kPortionRows = 24, kWidePortionRows = 32;
 constexpr int kShapes[4][2] = {{64, 64}, {128, 128}, {192, 128}, {256, 256}};
 int window_of(int window) { return window >= 1 << 30 ? 0 : window; }   // (no table has more tokens)
 int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, int keep_first, Layout* L) {
@@ -172,8 +174,8 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
   if (!sms) return fail(-2, "device %d: no attributes", c->device);
   const long long keys = (long long)s->table_blocks * c->block;
   L->shares = L->cluster = 0;
-  if (rows > kPortionRows) {
-    L->tiles = rows > 128 && L->shape < 3 ? 2 : 1;
+  if (rows > (L->shape < 3 ? kPortionRows : kWidePortionRows)) {
+    L->tiles = rows > 128 && L->shape < 3 ? 2 : 1;           // (16 sequences of 4000, 40 rows of 128 entries: 54 us with tiles of rows that do not exist, 38 without)
     const int each = 128 * L->tiles;
     L->row_tiles = (int)((rows + each - 1) / each);
     const long long tiles = (long long)s->batch * c->kv_heads * L->row_tiles;
@@ -181,13 +183,14 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
     L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * each * (kShapes[L->shape][1] + 2) * sizeof(float) : 0;
     return 0;
   }
-  L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : rows <= 24 ? 3 : 4;      // (tiles of 8 queries; 256 entries: the results of two fill the registers)
+  L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : 3;       // (tiles of 8 queries; 256 entries: the results of two fill the registers)
   L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
   if ((long long)c->kv_heads * L->row_tiles > INT_MAX) return fail(-4, "%d key heads of %lld query rows", c->kv_heads, rows);
-  const int unit = kv8::kWarps * kv8::step_of(kShapes[L->shape][1], L->tiles);
+  const int unit = kv8::kWarps * kv8::step_of(kShapes[L->shape][1]);
   const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * ((keys + unit - 1) / unit + 1);
-  // A cluster to each (sequence, head, tile) where they are few and the tables short enough that eight CTAs have at most eight units each, or where clusters fill the SMs: one launch, no
-  // workspace.  Otherwise the line: any number of CTAs to a head, whatever the lengths.
+  // A cluster to each (sequence, head, tile) where its CTAs have at most four units each: one launch, no workspace.  Otherwise the line: any number of CTAs to a head, whatever the lengths.
+  // us by clusters / by the line, 128 entries, a token of 16 heads over 4: one sequence of 1000 tokens 8.7 / 9.2, of 4000 11.2 / 11.2, of 8000 (eight units) 16.6 / 15.5, 8 of 4000
+  // 13.9 / 15.1, 16 with a window of 1024 10.0 / 10.9, 18 of 4000 (288 CTAs: clusters do not find all places) 33 / 21.
   const long long each = (long long)s->batch * c->kv_heads * L->row_tiles, most = window ? std::min(keys, (long long)window + s->rows + keep_first) : keys, longest = (most + unit - 1) / unit + (window ? 2 : 0);
   for (int k = 8; k >= 2 && !L->cluster; k /= 2)
     if (each * k <= 7 * sms / 4 && longest <= 4 * k) L->cluster = k;
@@ -225,7 +228,6 @@ template <int DK, int DV> int attend_tiles(const kv8::Attn& P, const Layout& L, 
   if (L.tiles == 1) return attend_as<DK, DV, 1>(P, L, device, stream);
   if constexpr (DV < 256) {
     if (L.tiles == 3) return attend_as<DK, DV, 3>(P, L, device, stream);
-    if (L.tiles == 4) return attend_as<DK, DV, 4>(P, L, device, stream);
   }
   return attend_as<DK, DV, 2>(P, L, device, stream);
 }

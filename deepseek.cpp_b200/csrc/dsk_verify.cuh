@@ -7,7 +7,9 @@
 // neighbour.  pick takes that row's exponentials in two fp32 parts, good to 2^-33 of each, as whole numbers of 2^-45 (2^-42 where the vocabulary has more than 2^17 entries), whose sums
 // are exact in any order; p and q meet as such numbers too.  Where coin x q is
 // within 1e-4 of p, the row's sum is taken that way as well.
-// Bound: row_stats by the bytes of the logits; pick by the latency of its steps, two walks over a row that L2 holds and a cluster's barrier behind each among them.
+// Bound: row_stats by the bytes of the logits; pick by the instructions of its exponentials (some 77 each) where sequences are many, otherwise by the latency of its steps, two walks over a row
+// that L2 holds and a cluster's barrier behind each among them.  Seven drafts of 32 sequences over 129280 tokens: 48 us, 14.5 of them row_stats (exponentials in fp64: 71); four drafts of
+// one over 32000: 14 us (15.7 with the statistics in pick's clusters instead of a launch of their own).
 #pragma once
 
 #include <cooperative_groups.h>

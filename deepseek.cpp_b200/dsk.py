@@ -990,8 +990,12 @@ class Cache8:
             if t.get_device() < 0:
                 _no_device(t)
             raise DskError(f"{what}: float32, float16 or bfloat16 {tuple(shape)} on cuda:{self.device} with neighbouring entries is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if written and not t.is_contiguous() and any(s[i] < t.shape[3] and t.shape[i] > 1 for i in range(3)):
-            raise DskError(f"{what}: rows of the result must not overlap")
+        if written and not t.is_contiguous():
+            extent = t.shape[3]
+            for step, n in sorted((s[i], t.shape[i]) for i in range(3) if t.shape[i] > 1):
+                if step < extent:
+                    raise DskError(f"{what}: rows of the result must not overlap")
+                extent += step * (n - 1)
         return _VIEW.pack(t.data_ptr(), self._types[t.dtype], s[0], s[1], s[2])
 
     def write(self, k, v, table, first, count=None):
@@ -1029,6 +1033,7 @@ class Cache8:
             out = (torch.empty if count is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
         elif out.dtype is not q.dtype:
             raise DskError(f"results of {out.dtype} for queries of {q.dtype}")
+        window, keep_first = min(window, 0x7fffffff), min(keep_first, 0x7fffffff)
         s = self._rows(table, lens, count, rows)
         a, b = self._view("queries", q, (batch, rows, heads, self.dim_k)), self._view("output", out, shape, True)
         key = (batch, rows, heads, table.shape[1], window, keep_first)

@@ -204,6 +204,14 @@ SHAPES = [
     ([300, 129, 70], [130, 129, 1], 130, 8, 1, 128, 128, 32, "bf16", 0, 0),
     ([400], [300], 300, 2, 1, 80, 96, 64, "f16", 0, 0),
     ([333], [140], 140, 40, 2, 64, 48, 128, "f16", 77, 20),
+    ([700, 130], [40, 37], 40, 2, 1, 256, 256, 64, "bf16", 0, 0),
+    ([1300], [200], 200, 4, 2, 256, 128, 128, "f16", 0, 0),
+    ([600, 40, 257], [33, 0, 100], 100, 1, 1, 96, 256, 16, "bf16", 130, 7),
+    ([2100], [7], 7, 4, 1, 64, 64, 64, "bf16", 0, 0),
+    ([900, 5, 300], [12, 5, 7], 12, 16, 4, 128, 128, 32, "bf16", 0, 0),
+    ([1500, 128], [128, 128], 128, 2, 2, 192, 128, 64, "f16", 200, 4),
+    ([1500, 128], [31, 1], 31, 4, 1, 64, 64, 16, "f16", 0, 0),
+    ([650], [16], 16, 2, 1, 256, 256, 32, "f16", 0, 0),
 ]
 
 
@@ -273,17 +281,18 @@ def test_attend_strided_rows_and_an_unaligned_result():
     assert (room[..., 0] == 0).all() and (room[..., 65:] == 0).all()
 
 
-@pytest.mark.parametrize("rows", [4, 90])
-def test_attend_nan_and_large_values_where_a_row_does_not_look(rows):
+@pytest.mark.parametrize("size", [64, 256])
+@pytest.mark.parametrize("rows", [4, 40, 90])
+def test_attend_nan_and_large_values_where_a_row_does_not_look(rows, size):
     """A NaN key or value reaches the rows that see its token, entry by entry, and no other row; +-448 everywhere else is no harm."""
     n = 200
-    c = Case([n, n], 2, 64, 64, 64, dead=126)
+    c = Case([n, n], 2, size, size, 64, dead=126)
     for b, t, h, d in ((0, n - 1, 0, 5), (0, n - 2, 1, 60), (1, n - rows // 2, 0, 0), (1, n - rows // 2, 0, 63)):
         c.v[c.table[b][t // 64], h, t % 64, d] = 127 if d % 2 else 255
     c.k[c.table[1][(n - 2) // 64], 1, (n - 2) % 64, 3] = 255
     cache = c.device()
-    q = torch.randn(2, rows, 4, 64, device=DEV, dtype=torch.bfloat16)
-    out = cache.attend(q, c.t, ints([n, n]))
+    q = torch.randn(2, rows, 4, size, device=DEV, dtype=torch.bfloat16)
+    out = cache.attend(q, c.t, ints([n, n]), scale=0.125)
     want, tol = expect(c, q.double().cpu().numpy(), [rows] * 2, 4, 0.125)
     assert np.isnan(want).any() and not np.isnan(want[:, 0]).any()
     check(out, want, np.nan_to_num(tol, nan=0.0), [rows] * 2, "bf16")
@@ -367,7 +376,7 @@ def test_attend_lengths_and_windows_at_the_ends_of_their_type(rows):
         assert (out[:seen] == 0).all()
         want, tol = expect(c, q.double().cpu().numpy(), [rows] * 3, 2, 0.125, lens=[min(max(n, -1), 1000) for n in first])   # (behind the table's end a row sees all of it)
         check(out, want, tol, [rows] * 3, "bf16")
-        assert torch.equal(out, c.cache.attend(q, c.t, ints(first)))
+        assert torch.equal(out, c.cache.attend(q, c.t, ints(first))) and torch.equal(out, c.cache.attend(q, c.t, ints(first), window=2 ** 32 + 5))
         with pytest.raises(dsk.DskError, match="outside the table"):
             c.cache.check()
 
@@ -464,7 +473,7 @@ def test_refusals():
         (dict(q=q.float()), "F16 or BF16"), (dict(q=q[:, :, :3]), "multiple"), (dict(q=q[..., :32]), "queries"), (dict(q=q[..., ::2]), "queries"), (dict(q=q.cpu()), "CUDA"),
         (dict(table=c.t.long()), "table"), (dict(table=c.t.cpu()), "CUDA"), (dict(lens=ints([20, 20])), "lengths"), (dict(lens=ints([20]).long()), "lengths"), (dict(count=ints([1, 1])), "count"),
         (dict(window=-1), "negative"), (dict(keep_first=-1), "negative"), (dict(scale=float("nan")), "number"), (dict(out=q.half()), "results"), (dict(out=q[..., :32]), "output"),
-        (dict(out=q[:, :, :1].expand(1, 1, 4, 64)), "overlap"), (dict(q=q[:, :, :0]), "multiple"),
+        (dict(out=q[:, :, :1].expand(1, 1, 4, 64)), "overlap"), (dict(q=q.expand(1, 3, 4, 64), out=q.new_zeros(4096).as_strided((1, 3, 4, 64), (0, 64, 64, 1))), "overlap"), (dict(q=q[:, :, :0]), "multiple"),
     ]
     for kw, text in bad:
         a = dict(q=q, table=c.t, lens=ints([20]))
@@ -490,21 +499,22 @@ def test_refusals():
     assert dsk.lib().dsk_kv8_attn(cache._c, s, a, b, 4, 1.0, 0, 0, None, 0, None) != 0 and b"workspace" in dsk.lib().dsk_last_error()
 
 
-@pytest.mark.parametrize("rows", [3, 90])
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("rows", [3, 20, 90])
 @pytest.mark.parametrize("order", [1, -1])
-def test_attend_maxima_that_jump(rows, order):
+def test_attend_maxima_that_jump(rows, order, d):
     """Scores that grow (or fall) by some tens from one stretch of 16 keys to the next, up to some hundreds: references move inside tiles and between them, by much and by little."""
     n = 400
-    c = Case([n], 1, 64, 64, 16, seed=11, spread=0.1)
+    c = Case([n], 1, d, d, 16, seed=11, spread=0.1)
     grow = np.concatenate([np.linspace(0, 9, 20), np.array([0, 60, -40, 90, 91])])[::order]
-    q0 = c.rng.normal(size=64)
-    x = np.zeros((1, n, 1, 64))
+    q0 = c.rng.normal(size=d)
+    x = np.zeros((1, n, 1, d))
     for t in range(n):
-        x[0, t, 0] = q0 * grow[t // 16] / (q0 @ q0) * 8 + 0.01 * c.rng.normal(size=64)       # (score of q0 at 1/8: grow)
+        x[0, t, 0] = q0 * grow[t // 16] / (q0 @ q0) * 8 + 0.01 * c.rng.normal(size=d)       # (score of q0 at 1/8: grow)
     so.write(c.k, c.ks, c.table, [0], [n], x)
     cache = c.device()
     q = torch.from_numpy(q0[None, None, None, :] * np.array([1.0, 0.5, -1.0, 4.0])[None, None, :, None] * np.ones((1, rows, 1, 1))).to(torch.bfloat16)
-    out = cache.attend(q.to(DEV), c.t, ints([n]))
+    out = cache.attend(q.to(DEV), c.t, ints([n]), scale=0.125)
     want, tol = expect(c, q.double().numpy(), [rows], 4, 0.125)
     check(out, want, tol, [rows], "bf16")
 

@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       if (lane == 0) hy::tc_arrive(qfull);
     }
     auto factor = [&](float key_scale) { return fmaxf(row_scale * key_scale, 1.17549435e-38f); };   // (positive: -inf stays what it is)
-    float m = kLowest, l = 0.f;
+    float m = kLowest, l = 0.f, limit = -INFINITY;             // limit: where a maximum moves the reference; any does while that is beyond kFar
     bool ok = true;
     const bool idle = (row0 + warp * 32) / A.group >= w.count;              // none of the warp's rows exists
     for (int i = 0; i < n; i++) {
@@ -470,9 +470,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
           const float z = max3(__float_as_uint(max3(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]))), __float_as_uint(fmaxf(y[3], y[4])), x[16 * g + 15]);
           top = fmaxf(top, fmaf(z, fs[g], lift[g]));
         }
-        const bool far = fabsf(top) > kFar && top > -INFINITY;
-        if (__any_sync(0xffffffffu, far || top > m + kLag)) {
-          if (__any_sync(0xffffffffu, far)) {
+        if (__any_sync(0xffffffffu, top > limit)) {
+          const float to = fmaxf(m, ceilf(top)), by = exp2_fast(m - to);
+          m = to;
+          l *= by;
+          const bool far = fabsf(m) > kFar;
+          limit = far ? -INFINITY : m + kLag;
+          if (__any_sync(0xffffffffu, far)) {                // (maxima beyond it under a reference that is not have weights of zero as they are)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
 #pragma unroll
@@ -480,9 +484,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
               fs[g] = 1.f;
             }
           }
-          const float to = fmaxf(m, ceilf(top)), by = exp2_fast(m - to);
-          m = to;
-          l *= by;
           if (i > 0) {                                       // (two tiles of rows: the tile's last product was through ahead of these scores)
             if (TILES == 1) {
               ok = wait_warp(pvdone, (i - 1) & 1, A.C);

@@ -491,7 +491,7 @@ ARCHITECTURES = {"Desarax": hybrid_from_config, "Rutulix": rutulix_from_config, 
                  "Zetivik": zetivik_from_config, "Netusun": netusun_from_config}
 
 _lib = None
-ABI_VERSION = 10  # DSK_ABI_VERSION (include/dsk.h)
+ABI_VERSION = 9  # DSK_ABI_VERSION (include/dsk.h)
 
 
 def build(force: bool = False) -> str:

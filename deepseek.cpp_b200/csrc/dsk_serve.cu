@@ -8,7 +8,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <mutex>
@@ -185,7 +184,6 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
   }
   L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : 3;       // (tiles of 8 queries; 256 entries: the results of two fill the registers)
   L->row_tiles = (int)((rows + 8 * L->tiles - 1) / (8 * L->tiles));
-  if ((long long)c->kv_heads * L->row_tiles > INT_MAX) return fail(-4, "%d key heads of %lld query rows", c->kv_heads, rows);
   const int unit = kv8::kWarps * kv8::step_of(kShapes[L->shape][1]);
   const long long units = (long long)s->batch * c->kv_heads * L->row_tiles * ((keys + unit - 1) / unit + 1);
   // A cluster to each (sequence, head, tile) where its CTAs have at most four units each: one launch, no workspace.  Otherwise the line: any number of CTAs to a head, whatever the lengths.

@@ -4,7 +4,7 @@
 // behind accepted ones the next token is drawn from p.  Both draws take the lowest index whose running sum is over (last coin) x (whole sum).
 // Two kernels: row_stats reads every row of logits once (maximum and sum of a piece of 1024 per warp, in fp32); pick has a cluster of CTAs for each sequence, which decides
 // on the drafts and draws from one row.  A draw's result hangs on sums of up to the whole vocabulary next to a border: in fp32 one draw in some thousands of a flat row would take a
-// neighbour.  pick takes that row's exponentials in two fp32 parts, good to 2^-33 of each, as whole numbers of 2^-45 (2^-42 where the vocabulary has more than 2^17 entries), whose sums
+// neighbour.  pick takes that row's exponentials in two fp32 parts, good to 2^-36 of each, as whole numbers of 2^-45 (2^-42 where the vocabulary has more than 2^17 entries), whose sums
 // are exact in any order; p and q meet as such numbers too.  Where coin x q is
 // within 1e-4 of p, the row's sum is taken that way as well.
 // Bound: row_stats by the bytes of the logits; pick by the instructions of its exponentials (some 77 each) where sequences are many, otherwise by the latency of its steps, two walks over a row
@@ -90,11 +90,10 @@ __global__ void __launch_bounds__(kStatThreads) row_stats(const Params P) {
   if (lane == 0) *out = make_float2(top, s);
 }
 
-// 2^y for y <= 0 in fp64, for the few values that drafts are judged by: 2^(k / 64) from a table, the rest by the series of e^z (Tang, "Table-driven implementation of the
-// exponential function in IEEE floating-point arithmetic", 1989)
+// 2^y in fp64, for the few values that drafts are judged by
 __device__ __forceinline__ double power(double y) { return y > -1000.0 ? exp2(y) : y <= -1000.0 ? 0.0 : y; }
 
-// 2^y of many values as whole numbers of 2^-BITS.  y = 64 (l - m) / temperature log2(e) in two parts, its integer part k looks up 2^(k mod 64 / 64), the rest f gives e^(f ln2 / 64) - 1
+// 2^y of many values as whole numbers of 2^-BITS (table and series: Tang, "Table-driven implementation of the exponential function in IEEE floating-point arithmetic", 1989).  y = 64 (l - m) / temperature log2(e) in two parts, its integer part k looks up 2^(k mod 64 / 64), the rest f gives e^(f ln2 / 64) - 1
 // in two parts, of at most 0.0055; relative error 2^-36 (checked on 200000 values).  What the shift to the value's size cuts off counts as half a step: sums are not biased.
 struct Slope { float hi, lo; };                              // 64 log2(e) / temperature
 template <int BITS> __device__ __forceinline__ uint64_t whole_power(float l, float m, Slope s, const uint4* table) {

@@ -178,8 +178,17 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
     const int each = 128 * L->tiles;
     L->row_tiles = (int)((rows + each - 1) / each);
     const long long tiles = (long long)s->batch * c->kv_heads * L->row_tiles;
-    L->shares = (int)std::max<long long>(1, std::min<long long>(sms / tiles, (keys + kv8::kTile - 1) / kv8::kTile));   // where the row tiles leave SMs idle, their keys are shared out
-    L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * each * (kShapes[L->shape][1] + 2) * sizeof(float) : 0;
+    // Keys are shared out where that is expected to pay: waves of CTAs x (their tiles of keys, and what a CTA does once), and the pieces through memory (ns, from the cases below).  us with
+    // one share / with what the rule takes: 700 queries of 32 heads over 8 behind 7300 tokens 162 / 131 (three shares), 3 x 777 of 16 heads of 64 over 4, 4000 tokens, 126 / 114; with one,
+    // which the rule takes / with two: 2048 queries of 16 heads behind 3952 tokens 134 / 158, 1500 of 24 heads behind 1500 72 / 89, 500 queries of 64 heads over 8, two sequences, 139 / 163.
+    const int tile = L->shape == 3 ? 3500 : L->tiles == 2 ? 2400 : 1800, group = heads / c->kv_heads, cols = kShapes[L->shape][1] + 2;
+    const long long seen = window ? std::min(keys, (long long)window + each / group + keep_first + kv8::kTile) : keys, key_tiles = std::max(1ll, (seen + kv8::kTile - 1) / kv8::kTile);
+    long long best = -1;
+    for (long long n = 1; n <= std::min(key_tiles, std::max(4ll, sms / tiles)); n += std::max(1ll, n / 8)) {
+      const long long ns = (tiles * n + sms - 1) / sms * ((key_tiles + n - 1) / n * tile + 10000) + (n > 1 ? 3000 + tiles * n * each * cols * 8 / 5000 : 0);
+      if (best < 0 || ns < best) { best = ns; L->shares = (int)n; }
+    }
+    L->bytes = L->shares > 1 ? (size_t)tiles * L->shares * each * cols * sizeof(float) : 0;
     return 0;
   }
   L->tiles = rows <= 8 ? 1 : rows <= 16 || L->shape == 3 ? 2 : 3;       // (tiles of 8 queries; 256 entries: the results of two fill the registers)

@@ -484,6 +484,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
               fs[g] = 1.f;
             }
           }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");   // what the tile's newer half stored, weights and results, is read back: a load is not behind a store by itself
           if (i > 0) {                                       // (two tiles of rows: the tile's last product was through ahead of these scores)
             if (TILES == 1) {
               ok = wait_warp(pvdone, (i - 1) & 1, A.C);

@@ -519,6 +519,43 @@ def test_attend_maxima_that_jump(rows, order, d):
     check(out, want, tol, [rows], "bf16")
 
 
+def scored(levels, d, heads, seed, values=None):
+    """A sequence whose token t has the score levels[t] (in powers of two, at scale ln 2) with the one query of all rows: entry 0 of a key is its level, which E4M3 has exactly, entry 0 of the
+    query 1; the other entries are noise of keys that queries do not look at."""
+    n = len(levels)
+    c = Case([n], 1, d, d, 64, seed=seed)
+    for t, e in enumerate(levels):
+        page, row = c.table[0][t // 64], t % 64
+        c.k[page, 0, row, 0] = so.encode(np.array([float(e)]))[0]
+        assert so.TABLE[c.k[page, 0, row, 0]] == e
+        if values is not None:
+            c.v[page, 0, row] = so.encode(np.full(d, float(values[t])))
+    c.ks[:] = 1.0
+    c.vs[:] = 1.0
+    q = torch.zeros(1, heads, 1, d, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    return c, q.transpose(1, 2).contiguous()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [40, 200])
+def test_attend_references_that_move_in_both_halves_of_a_tile(rows, d):
+    """The newer 64 keys of a tile of 128 move a row's reference, then the older ones do: weights and results that were stored a moment ago are scaled again, in every tile but the first; and
+    rows that see none of the newer keys."""
+    levels = np.zeros(640)
+    for i in range(5):
+        levels[128 * i + 64:128 * (i + 1)] = 32 * i
+        levels[128 * i:128 * i + 64] = 32 * i + 16
+    levels[640 - 60:] = -20                                  # (the rows' own tokens)
+    c, q = scored(levels, d, 1, seed=21)
+    q = q.expand(1, rows, 1, d).contiguous()
+    for n in (640, 400, 300, rows + 7):
+        cache = c.device()
+        out = cache.attend(q.to(DEV), c.t, ints([n]), scale=float(np.log(2.0)))
+        want, tol = expect(c, q.double().numpy(), [rows], 1, float(np.float32(np.log(2.0))), lens=[n])
+        check(out, want, tol, [rows], "bf16")
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_offsets_beyond_32_bits(rows):
     """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""

@@ -556,6 +556,30 @@ def test_attend_references_that_move_in_both_halves_of_a_tile(rows, d):
         check(out, want, tol, [rows], "bf16")
 
 
+def many(c, q, rows, n, B=148):
+    """What every one of B sequences in the same blocks gets, as many as there are processors: no row's keys are shared out."""
+    cache = c.device()
+    out = cache.attend(q.to(DEV).expand(B, rows, 1, c.dk), c.t.expand(B, -1).contiguous(), ints([n] * B), scale=float(np.log(2.0)))
+    assert torch.equal(out, out[:1].expand_as(out))
+    want, tol = expect(c, q.expand(1, rows, 1, c.dk).double().numpy(), [rows], 1, float(np.float32(np.log(2.0))), lens=[n])
+    check(out[:1], want, tol, [rows], "bf16")
+    return want
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [40, 200])
+def test_attend_references_that_move_in_both_halves_of_every_tile(rows, d):
+    """The same where a CTA has tile after tile: results are scaled twice in a tile as well."""
+    levels = np.zeros(640)
+    for i in range(5):
+        levels[128 * i + 64:128 * (i + 1)] = 32 * i
+        levels[128 * i:128 * i + 64] = 32 * i + 16
+    levels[640 - 60:] = -20
+    c, q = scored(levels, d, 1, seed=21)
+    for n in (640, 400, 300, rows + 7):
+        many(c, q, rows, n)
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_offsets_beyond_32_bits(rows):
     """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""

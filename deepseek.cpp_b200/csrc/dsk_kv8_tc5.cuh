@@ -443,7 +443,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // Half a row of scores in registers at a time, each read once: the reference may lag behind the maximum by kLag, within fp16's range, so that the first half's weights do not wait for
-      // the second half's maximum; where that moves the reference after all, weights that are stored already are scaled again, exactly, since references are whole numbers.
+      // the second half's maximum; where that moves the reference after all, weights that are stored already are scaled again, by a power of two since references are whole numbers: exactly, but
+      // for what comes below 2^-14, where fp16 has multiples of 2^-24.
 #pragma unroll 1
       for (int half = 1; half >= 0; half--) {
         const int c = half * 64;
@@ -500,13 +501,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
             }
           }
           if (half == 0) {
-            const __half2 by2 = __float2half2_rn(by);
 #pragma unroll 1
             for (int d = 0; d < 32; d += 16) {
               uint32_t y[16];
               tmem_read16(s_at + 64 + d, y);
 #pragma unroll
-              for (int k = 0; k < 16; k++) { const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&y[k]), by2); y[k] = *reinterpret_cast<const uint32_t*>(&v); }
+              for (int k = 0; k < 16; k++) { const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&y[k])); y[k] = halves(v.x * by, v.y * by); }   // (fp16 has no factor below 2^-24)
               tmem_store16(s_at + 64 + d, y);
             }
           }

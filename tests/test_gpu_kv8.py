@@ -580,6 +580,20 @@ def test_attend_references_that_move_in_both_halves_of_every_tile(rows, d):
         many(c, q, rows, n)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [40, 200])
+def test_attend_weights_that_a_late_reference_makes_small(rows, d):
+    """A reference that lags by 14, then moves by 25 and more once the newer half's weights are stored: those are 2^-11 of the largest each, 2^-5 of the row together."""
+    levels = np.full(512, -20.0)
+    levels[:128] = 1
+    levels[192:256] = 15
+    levels[150] = 26
+    values = np.zeros(512)
+    values[192:256] = 16
+    c, q = scored(levels, d, 1, seed=22, values=values)
+    assert many(c, q, rows, 512).min() > 0.4
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_offsets_beyond_32_bits(rows):
     """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""

@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
     if (ahead > 0 && s < at.q.steps) {
       key = (s < at.q.kept ? s : at.q.low + s - at.q.kept) * STEP;
       page[0] = __ldg(at.table + (key >> P.C.shift));
-      if (HV == 2) page[HV - 1] = P.C.shift > 4 ? page[0] : key + 16 < at.q.len ? __ldg(at.table + (key >> 4) + 1) : 0;
+      if (HV == 2) page[HV - 1] = P.C.shift > 4 ? page[0] : key + 16 < at.q.len ? __ldg(at.table + (key >> 4) + 1) : -1;   // (-1: behind the last key)
     }
   };
   auto fetch = [&](int stage) {
@@ -329,8 +329,8 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
           copy_rows<DK / 32, 0, 16 * KS>(to, to_k, k, u);
           copy_rows<DV / 32, 0, 16 * VS>(to, to_v, v, u);
           if (lane < 2) copy4(to + STEP * (KS + VS) + u * 8 + lane * 4, scale, 4);
-        } else {                                             // what is behind the last key, or in a block outside the cache, comes as zeros
-          if (!ok && lane == 0) note(P.C, ST_PAGE);
+        } else {                                             // what is behind the last key, or in a block outside the cache, comes as zeros, its scales too where the block is nobody's
+          if (!ok && lane == 0 && key + 16 * u < at.q.len) note(P.C, ST_PAGE);
           const int there = ok ? at.q.len - key - 16 * u : 0;
           for (int i = lane; i < dk; i += 32) { const int row = i / dk16; copy16_or_zero(to + (u * 16 + row) * KS + (i - row * dk16) * 16, row < there ? k + (i - lane) * 16 : P.C.code[0], row < there); }
           for (int i = lane; i < dv; i += 32) { const int row = i / dv16; copy16_or_zero(to + STEP * KS + (u * 16 + row) * VS + (i - row * dv16) * 16, row < there ? v + (i - lane) * 16 : P.C.code[1], row < there); }

@@ -594,6 +594,43 @@ def test_attend_weights_that_a_late_reference_makes_small(rows, d):
     assert many(c, q, rows, 512).min() > 0.4
 
 
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (192, 128), (256, 256)])
+@pytest.mark.parametrize("rows", [1, 3, 20, 40])
+def test_attend_scales_of_blocks_that_no_sequence_owns(rows, dk, dv):
+    """Blocks of 16 tokens, lengths of every remainder by 32, where nobody ever wrote block 0 and scales that nobody wrote are NaN, by clusters and by the line."""
+    lens = list(range(rows, rows + 33))
+    c = Case(lens, 1, dk, dv, 16, seed=30)
+    c.table = (c.rng.permutation(c.blocks - 1)[:c.table.size] + 1).reshape(c.table.shape).astype(np.int32)   # block 0 is nobody's
+    for a, s, d in ((c.k, c.ks, dk), (c.v, c.vs, dv)):
+        a[:] = 127
+        s[:] = np.nan
+        so.write(a, s, c.table, [0] * c.B, lens, c.rng.normal(size=(c.B, max(lens), 1, d)))
+    cache = c.device()
+    q = torch.randn(c.B, rows, 1, dk, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    want, tol = expect(c, q.double().numpy(), [rows] * c.B, 1, dk ** -0.5)
+    wide = torch.full((c.B, 3000), -7, dtype=torch.int32, device=DEV)
+    wide[:, :c.t.shape[1]] = c.t
+    for t in (c.t, wide):
+        out = cache.attend(q.to(DEV), t, ints(lens))
+        check(out, want, tol, [rows] * c.B, "bf16")
+    cache.check()
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("rows", [1, 5, 20, 80])
+def test_attend_more_tokens_than_an_odd_table_has(rows, block):
+    """A row behind the table's end sees the table's tokens and nothing beside them."""
+    c = Case([5 * block, 5 * block], 1, 64, 64, block, seed=31)
+    cache = c.device()
+    q = torch.randn(2, rows, 2, 64, device=DEV, dtype=torch.bfloat16)
+    lens = [5 * block + rows + 40, 5 * block + rows + 16]
+    out = cache.attend(q, c.t, ints(lens))
+    want, tol = expect(c, q.double().cpu().numpy(), [rows] * 2, 2, 0.125, lens=lens)
+    check(out, want, tol, [rows] * 2, "bf16")
+    with pytest.raises(dsk.DskError, match="outside the table"):
+        cache.check()
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_offsets_beyond_32_bits(rows):
     """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""

@@ -169,6 +169,7 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
   const long long rows = (long long)(heads / c->kv_heads) * s->rows;
   if (rows > (1 << 22)) return fail(-4, "%lld query rows of a key head: at most 2^22", rows);
   for (L->shape = 0; c->dim_k > kShapes[L->shape][0] || c->dim_v > kShapes[L->shape][1];) L->shape++;
+  if (!rows || !s->batch) { *L = Layout{}; return 0; }      // (nothing to lay out)
   const int sms = multiprocessors(c->device);
   if (!sms) return fail(-2, "device %d: no attributes", c->device);
   const long long keys = (long long)s->table_blocks * c->block;

@@ -423,6 +423,25 @@ def test_attend_empty_calls():
     cache.check()
 
 
+@pytest.mark.parametrize("rows", [0, 1, 100])
+def test_attend_no_sequences(rows):
+    """A batch of none, of rows for either kernel: no workspace, nothing launched."""
+    cache = Case([20], 1, 64, 64, 16).device()
+    for heads in (1, 64):
+        q = torch.zeros(0, rows, heads, 64, device=DEV, dtype=torch.bfloat16)
+        for blocks in (0, 2, 3000):
+            table = torch.zeros(0, blocks, dtype=torch.int32, device=DEV)
+            for window in (0, 100):
+                assert cache.attend(q, table, ints([]), window=window).shape == (0, rows, heads, 64)
+                assert cache.attend(q, table, ints([]), count=ints([]), window=window).shape == (0, rows, heads, 64)
+    cache.write(q[:, :, :1], q[:, :, :1], table, ints([]))
+    assert cache.read(table, ints([]), rows)[0].shape == (0, rows, 1, 64)
+    logits = torch.zeros(0, 4, 50, device=DEV)
+    a, t = dsk.verify_drafts(logits, torch.zeros(0, 3, dtype=torch.int32, device=DEV), torch.zeros(0, 4, device=DEV))
+    assert a.shape == (0,) and t.shape == (0, 4)
+    cache.check()
+
+
 def test_attend_many_sequences():
     B = 700
     lens = [(37 * b) % 90 for b in range(B)]

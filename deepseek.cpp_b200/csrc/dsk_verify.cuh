@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
     for (int u = 0; u < 4; u++) {
       const uint64_t p = whole_power<BITS>(x[u], m, slope, table);
       if (!q) { d[u] = i + u >= end || i + u == certain ? 0 : p; continue; }
-      const uint32_t bits = __float_as_uint(y[u]);           // (nothing is left where q is negative or not a number; numbers below 2^-126 count as none)
+      const uint32_t bits = __float_as_uint(y[u] + 0.f);     // (-0 is 0; nothing is left where q is negative or not a number; numbers below 2^-126 count as none)
       const int ex = (int)(bits >> 23), by = past - ex;
       const uint64_t t = ((uint64_t)((bits & 0x7fffffu) | 0x800000u) * first) << 7;
       const uint64_t other = by < 0 ? p : ex == 0 || by > 63 ? 0 : t >> by;

@@ -384,6 +384,7 @@ int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view*
  * while coins[i] q_i(x_i) < p_i(x_i) (no draft_probs: q_i(x_i) = 1, the drafts are certain).  The first draft that is not is replaced by a draw from max(p_i - q_i, 0); behind
  * accepted ones the next token is drawn from p (temperature: 0, or at least 2^-120).  A draw is the lowest index whose running sum is over coins[drafts] x (whole sum), to 2^-32 of it.  temperature 0: a draft is accepted
  * if it is the lowest index of the largest logit, which replaces it otherwise.  Coins lie in [0, 1).  accepted[b]: drafts accepted; tokens[b]: those, the drawn token, -1 in the places behind.
+ * draft_probs lie in [0, 1] (-0 is 0); a token whose probability is negative or a NaN is not drawn in place of a draft.
  * A drafted token outside the vocabulary is refused; where a row's logits hold a NaN, or are no distribution (+inf at a temperature, nothing but -inf), its draft is refused and the drawn token is -1. */
 typedef struct dsk_verify_args {
   const void* logits;              /* [batch][drafts + 1][vocab], pitches in elements */

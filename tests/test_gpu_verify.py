@@ -106,6 +106,31 @@ def test_verify_masked_and_broken_rows():
         same(logits, drafts, coins, None, None, t)
 
 
+def draw(logits, coins, q=None):
+    """The token drawn from one row for every coin: behind no draft, or with q in place of a draft outside the vocabulary."""
+    B, n, V = len(coins), 0 if q is None else 1, logits.shape[-1]
+    c = torch.zeros(B, n + 1, device=DEV)
+    c[:, n] = torch.tensor(coins, device=DEV)
+    a, t = dsk.verify_drafts(logits.to(DEV).expand(B, n + 1, V), torch.full((B, n), -1, dtype=torch.int32, device=DEV), c, probs=None if q is None else q.to(DEV).expand(B, 1, V))
+    assert (a == 0).all() and (t[:, 1:] == -1).all()
+    return t[:, 0].tolist()
+
+
+def test_verify_probabilities_of_minus_zero():
+    """-0 is 0: such tokens are drawn by what the model gives them; those whose probability is negative or a NaN are not."""
+    q = torch.full((1, 1, 64), -0.0)
+    q[..., 5] = 1.0
+    coins = [0.0, 0.25, 0.5, 0.99]
+    assert draw(torch.zeros(1, 1, 64), coins, q) == [0, 16, 32, 63]           # (63 tokens of equal weight, 5 not among them)
+    logits, _, drafts, _ = make(4, 3, 500, seed=9)
+    drafts[:, 0] = -1
+    zeros = torch.zeros(4, 3, 500)
+    zeros[:, :, ::2] = -0.0
+    same(logits, drafts, torch.rand(4, 4, generator=torch.Generator().manual_seed(1)), zeros, None, 1.0)
+    q[..., :5], q[..., 6:9] = -0.5, float("nan")
+    assert draw(torch.zeros(1, 1, 64), [0.0], q) == [9]
+
+
 def test_verify_lowest_index_of_equal_logits():
     logits = torch.zeros(2, 2, 5000)
     logits[:, :, [4990, 1200, 77]] = 5.0

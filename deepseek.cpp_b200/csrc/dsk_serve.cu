@@ -324,8 +324,7 @@ extern "C" int dsk_verify_workspace(const dsk_verify_args* a, size_t* bytes) {
 template <typename T> static int verify_as(const verify::Params& P, cudaStream_t stream) {
   verify::row_stats<T><<<dim3((P.pieces + verify::kStatWarps - 1) / verify::kStatWarps, P.n + 1, P.batch), verify::kStatThreads, 0, stream>>>(P);
   CK(cudaGetLastError());
-  if (P.vocab <= 1 << 17) CK(launch_behind(verify::pick<T, 45>, dim3(P.batch * P.cluster), dim3(verify::kThreads), 0, stream, P.cluster, P));   // (sums of a row stay below 2^62)
-  else CK(launch_behind(verify::pick<T, 42>, dim3(P.batch * P.cluster), dim3(verify::kThreads), 0, stream, P.cluster, P));
+  CK(launch_behind(verify::pick<T>, dim3(P.batch * P.cluster), dim3(verify::kThreads), 0, stream, P.cluster, P));
   return 0;
 }
 

@@ -4,9 +4,9 @@
 // behind accepted ones the next token is drawn from p.  Both draws take the lowest index whose running sum is over (last coin) x (whole sum).
 // Two kernels: row_stats reads every row of logits once (maximum and sum of a piece of 1024 per warp, in fp32); pick has a cluster of CTAs for each sequence, which decides
 // on the drafts and draws from one row.  A draw's result hangs on sums of up to the whole vocabulary next to a border: in fp32 one draw in some thousands of a flat row would take a
-// neighbour.  pick takes that row's exponentials in two fp32 parts, good to 2^-36 of each, as whole numbers of 2^-45 (2^-42 where the vocabulary has more than 2^17 entries), whose sums
-// are exact in any order; p and q meet as such numbers too.  Where coin x q is
-// within 1e-4 of p, the row's sum is taken that way as well.
+// neighbour.  pick takes that row's exponentials in two fp32 parts, good to 2^-36 of each, as whole numbers of 2^-61 of the power of two above the row's sum, whose sums are the same in
+// any order and miss at most 2^-40 of the row by what each loses below one (2^20 entries; as multiples of a fixed 2^-45 at least one each, the tail of a row weighed up to 2^-28 of it, where
+// it should have had 2^-32); p and q meet as such numbers too.  Where coin x q is within 1e-4 of p, the row's sum is taken that way as well.
 // Bound: row_stats by the bytes of the logits; pick by the instructions of its exponentials (some 77 each) where sequences are many, otherwise by the latency of its steps, two walks over a row
 // that L2 holds and a cluster's barrier behind each among them.  Seven drafts of 32 sequences over 129280 tokens: 48 us, 14.5 of them row_stats (exponentials in fp64: 71); four drafts of
 // one over 32000: 14 us (15.7 with the statistics in pick's clusters instead of a launch of their own).
@@ -93,23 +93,24 @@ __global__ void __launch_bounds__(kStatThreads) row_stats(const Params P) {
 // 2^y in fp64, for the few values that drafts are judged by
 __device__ __forceinline__ double power(double y) { return y > -1000.0 ? exp2(y) : y <= -1000.0 ? 0.0 : y; }
 
-// 2^y of many values as whole numbers of 2^-BITS (table and series: Tang, "Table-driven implementation of the exponential function in IEEE floating-point arithmetic", 1989).  y = 64 (l - m) / temperature log2(e) in two parts, its integer part k looks up 2^(k mod 64 / 64), the rest f gives e^(f ln2 / 64) - 1
-// in two parts, of at most 0.0055; relative error 2^-36 (checked on 200000 values).  What the shift to the value's size cuts off counts as half a step: sums are not biased.
-struct Slope { float hi, lo; };                              // 64 log2(e) / temperature
-template <int BITS> __device__ __forceinline__ uint64_t whole_power(float l, float m, Slope s, const uint4* table) {
+// 2^y of many values as whole numbers of 2^(down - kBits) (table and series: Tang, "Table-driven implementation of the exponential function in IEEE floating-point arithmetic", 1989).  y = 64 (l - m) / temperature log2(e) in two parts, its integer part k looks up 2^(k mod 64 / 64), the rest f gives e^(f ln2 / 64) - 1
+// in two parts, of at most 0.0055; relative error 2^-36 (two roundings to 2^-39, 2^-37.5 for the first bits of the table's entry, less for the series).
+constexpr int kBits = 61;                                    // 2^0 is 2^(kBits - down); a row's sum stays below 2^62 where 2^down is above the row's sum
+struct Slope { float hi, lo; int down; };                    // 64 log2(e) / temperature; the row's shift
+__device__ __forceinline__ uint64_t whole_power(float l, float m, Slope s, const uint4* table) {
   constexpr float C = 0.010830424726009369f, C_LO = -2.976022e-11f;   // ln 2 / 64 in two parts
   const float d = l - m, b = d - l, d_lo = (l - (d - b)) - (m + b);   // l - m exactly
   float y = d * s.hi;
-  const bool none = !(y > -3200.f);                          // below 2^-50 (-inf among them)
+  const bool none = !(y > -4000.f);                          // below 2^-62 (-inf among them)
   const float e = fmaf(d_lo, s.hi, fmaf(d, s.lo, fmaf(d, s.hi, -y)));
   const float t = y + 12582912.f, f0 = y - (t - 12582912.f), f = f0 + e, f_lo = (f0 - f) + e;
   const float z = f * C, z_lo = fmaf(f_lo, C, fmaf(f, C_LO, fmaf(f, C, -z)));
   const float r = fmaf(z * z, fmaf(z, fmaf(z, 1.f / 24.f, 1.f / 6.f), 0.5f), z_lo);
   const int q = __float2int_rn(z * 274877906944.f) + __float2int_rn(r * 274877906944.f);   // 2^38
   const int n = __float_as_int(t) - 0x4b400000;
-  const uint4 p = table[n & 63];                             // 2^BITS to 2^(BITS + 1), and its first 31 bits
-  const uint64_t v = (((uint64_t)p.y << 32) | p.x) + (uint64_t)(((int64_t)(int)p.z * q) >> (68 - BITS));
-  return none ? 0 : (v >> (-(n >> 6) & 63)) | 1;
+  const uint4 p = table[n & 63];                             // 2^kBits to 2^(kBits + 1), and its first 31 bits
+  const uint64_t v = (((uint64_t)p.y << 32) | p.x) + (uint64_t)(((int64_t)(int)p.z * q) >> (68 - kBits));
+  return none ? 0 : v >> min(s.down - (n >> 6), 63);
 }
 __device__ __forceinline__ uint64_t sum64(uint64_t v) {
 #pragma unroll
@@ -122,7 +123,7 @@ __device__ __forceinline__ uint64_t running(uint64_t v, int lane) {
   return v;
 }
 
-template <typename T, int BITS>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
   namespace cg = cooperative_groups;
   __shared__ uint4 table[64];
@@ -138,10 +139,10 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
   const int* drafts = P.drafts + (size_t)b * P.n;
   const float* coins = P.coins + (size_t)b * (P.n + 1);
   const double slope64 = 64.0 * P.slope;
-  const Slope slope{(float)slope64, (float)(slope64 - (float)slope64)};
+  Slope slope{(float)slope64, (float)(slope64 - (float)slope64), 0};
   if (tid < 64) {
-    const uint64_t p = (uint64_t)__double2ll_rn(exp2(tid / 64.0 + BITS));
-    table[tid] = make_uint4((uint32_t)p, (uint32_t)(p >> 32), (uint32_t)(p >> (BITS - 30)), 0);
+    const uint64_t p = (uint64_t)__double2ll_rn(exp2(tid / 64.0 + kBits));
+    table[tid] = make_uint4((uint32_t)p, (uint32_t)(p >> 32), (uint32_t)(p >> (kBits - 30)), 0);
   }
   // what drafts are judged by does not wait for the kernel ahead, which only reads it
   struct Row { int x; float l, q, coin; };
@@ -194,11 +195,11 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
 #pragma unroll
       for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) s += whole_power<BITS>(x[u][k], m, slope, table);
+        for (int k = 0; k < 4; k++) s += whole_power(x[u][k], m, slope, table);
     }
     return sum64(s);
   };
-  const double unit = exp2(-(double)BITS);
+  auto down_of = [&](int r) { return (__float_as_int((float)row_sum[r]) >> 23) - 126; };   // (the sum is at least 1, and known to 1e-5 of it)
   const int all = P.cluster * kWarps, share = ((V + all - 1) / all + 127) / 128 * 128, mine = rank * kWarps + warp;   // a warp's indices of the row that is drawn from
   const int from = min(V, mine * share), to = min(V, from + share);
   int r = 0;                                                 // (the same in every CTA of the cluster)
@@ -206,6 +207,7 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
     int f = flag[r];
     if (f == 2) {
       const int each = ((V + kWarps - 1) / kWarps + 3) / 4 * 4;
+      slope.down = down_of(r);
       const uint64_t s = walk(r, min(V, warp * each), min(V, (warp + 1) * each), row_max[r]);
       if (lane == 0) sums[0][warp] = s;
       __syncthreads();
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
       for (int k = 0; k < kWarps; k++) whole += sums[0][k];
       __syncthreads();
       const Row y = look(r);
-      f = (double)y.coin * y.q < power(((double)y.l - row_max[r]) * P.slope) / ((double)whole * unit);
+      f = (double)y.coin * y.q < power(((double)y.l - row_max[r]) * P.slope) / ((double)whole * exp2((double)(slope.down - kBits)));
     }
     if (f != 1) break;
   }
@@ -227,6 +229,7 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
     return;                                                  // (the whole cluster)
   }
   const float m = row_max[r];
+  slope.down = down_of(r);
   const bool drafted = r < n;
   const float* q = drafted && P.probs ? P.probs + b * P.p_batch + r * P.p_row : nullptr;
   auto gather = [&](int which) {                             // sums of all warps of the cluster, in order
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
     if (q && i < end) four(q, i, V, P.wide_p, y);
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const uint64_t p = whole_power<BITS>(x[u], m, slope, table);
+      const uint64_t p = whole_power(x[u], m, slope, table);
       if (!q) { d[u] = i + u >= end || i + u == certain ? 0 : p; continue; }
       const uint32_t bits = __float_as_uint(y[u] + 0.f);     // (-0 is 0; nothing is left where q is negative or not a number; numbers below 2^-126 count as none)
       const int ex = (int)(bits >> 23), by = past - ex;

@@ -131,6 +131,46 @@ def test_verify_probabilities_of_minus_zero():
     assert draw(torch.zeros(1, 1, 64), [0.0], q) == [9]
 
 
+def allowed(left, coin, token, bound):
+    """Whether `token` is what a coin draws from `left` where running sums may be off by `bound` (p sums to 1)."""
+    s = np.cumsum(left)
+    border = np.longdouble(coin) * s[-1]
+    return 0 <= token < len(left) and s[token] > border - bound and (s[token - 1] if token else 0) <= border + bound
+
+
+@pytest.mark.parametrize("V", [1000, 129280, 1 << 17, (1 << 17) + 1, 1 << 20])
+@pytest.mark.parametrize("depth", [30.0, 31.5, 33.0, 34.0, 36.0])
+def test_verify_long_tails(V, depth):
+    """One large logit ahead of or behind all the others: these have what the definition gives them, however small each is.  Terms are good to 2^-36 of each, a border lies between two sums
+    of them (2^-35), what is cut off below a unit comes to 2^-40."""
+    coins = [0.0, 2.0 ** -34, 2.0 ** -32, 2.0 ** -31, 2.0 ** -30, 2.0 ** -28, 2.0 ** -26, 2.0 ** -23, 0.5, 1 - 2.0 ** -24]
+    for at in (0, V - 1):
+        row = np.full(V, -depth, dtype=np.longdouble)
+        row[at] = 0
+        p = np.exp(row)
+        p /= p.sum()
+        for coin, token in zip(coins, draw(torch.from_numpy(row.astype(np.float32))[None, None], coins)):
+            assert allowed(p, coin, token, 2.0 ** -34), (at, coin, token)
+
+
+@pytest.mark.parametrize("V", [(1 << 17) + 5, 1 << 20])
+@pytest.mark.parametrize("temperature", [1.0, 0.0])
+def test_verify_vocabularies_beyond_2_17(V, temperature):
+    logits, q, drafts, coins = make(2, 2, V, seed=42, temperature=temperature)
+    same(logits, drafts, coins, q, None, temperature)
+    same(logits, drafts, coins, None, [1, 2], temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_verify_as_many_drafts_as_there_may_be(dtype):
+    logits, q, drafts, coins = make(3, 127, 300, seed=41, noise=0.02, dtype=dtype)
+    coins[:2, :127] *= 0.9
+    a, _ = same(logits, drafts, coins, q, [127, 127, 90], 1.0)
+    assert a.max() > 100
+    same(logits, drafts, coins, None, None, 0.0)
+    same(logits, drafts, coins, None, [127, 64, 0], 1.0)
+
+
 def test_verify_lowest_index_of_equal_logits():
     logits = torch.zeros(2, 2, 5000)
     logits[:, :, [4990, 1200, 77]] = 5.0

@@ -245,9 +245,7 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
     for (int i = lane; i < all; i += 32) whole += ends[i];
     whole = sum64(whole);
   }
-  const int high = 63 - __clzll(whole | 1);                  // q x whole = (24 bits) x (the first 32 of whole), shifted
-  const uint32_t first = (uint32_t)(high >= 31 ? whole >> (high - 31) : whole << (31 - high));
-  const int past = 150 + 7 - (high - 31);                    // minus the exponent of q: how far to the right
+  const uint32_t whole_hi = (uint32_t)(whole >> 31), whole_lo = (uint32_t)(whole << 1);   // twice the sum (below 2^63)
   const T* row = logits + r * P.l_row;
   const int certain = drafted && !P.probs ? drafts[r] : -1;
   auto left = [&](int i, int end, uint64_t (&d)[4]) {        // what four indices have in the draw: (p - q) x (sum of the row), none below zero
@@ -259,8 +257,9 @@ __global__ void __launch_bounds__(kThreads, 2) pick(const Params P) {
       const uint64_t p = whole_power(x[u], m, slope, table);
       if (!q) { d[u] = i + u >= end || i + u == certain ? 0 : p; continue; }
       const uint32_t bits = __float_as_uint(y[u] + 0.f);     // (-0 is 0; nothing is left where q is negative or not a number; numbers below 2^-126 count as none)
-      const int ex = (int)(bits >> 23), by = past - ex;
-      const uint64_t t = ((uint64_t)((bits & 0x7fffffu) | 0x800000u) * first) << 7;
+      const int ex = (int)(bits >> 23), by = 127 - ex;
+      const uint32_t q32 = (bits & 0x7fffffu) << 8 | 0x80000000u;            // q = q32 2^(ex - 158)
+      const uint64_t t = (uint64_t)whole_hi * q32 + __umulhi(whole_lo, q32);   // q x sum x 2^by, cut to a whole number (of 32 bits of the sum alone: off by up to 2^-31 of q)
       const uint64_t other = by < 0 ? p : ex == 0 || by > 63 ? 0 : t >> by;
       d[u] = i + u >= end || other >= p ? 0 : p - other;
     }

@@ -382,7 +382,7 @@ int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view*
                  void* workspace, size_t workspace_bytes, void* stream);
 /* Speculative sampling, beside dsk_sample: sequence b has count[b] drafted tokens x_i and the model's logits of count[b] + 1 rows.  p_i = softmax(logits_i / temperature); draft i is accepted
  * while coins[i] q_i(x_i) < p_i(x_i) (no draft_probs: q_i(x_i) = 1, the drafts are certain).  The first draft that is not is replaced by a draw from max(p_i - q_i, 0); behind
- * accepted ones the next token is drawn from p (temperature: 0, or at least 2^-120).  A draw is the lowest index whose running sum is over coins[drafts] x (whole sum), to 2^-32 of it.  temperature 0: a draft is accepted
+ * accepted ones the next token is drawn from p (temperature: 0, or at least 2^-120).  A draw is the lowest index whose running sum is over coins[drafts] x (whole sum), sums good to 2^-35 (of p's, which is 1).  temperature 0: a draft is accepted
  * if it is the lowest index of the largest logit, which replaces it otherwise.  Coins lie in [0, 1).  accepted[b]: drafts accepted; tokens[b]: those, the drawn token, -1 in the places behind.
  * draft_probs lie in [0, 1] (-0 is 0); a token whose probability is negative or a NaN is not drawn in place of a draft.
  * A drafted token outside the vocabulary is refused; where a row's logits hold a NaN, or are no distribution (+inf at a temperature, nothing but -inf), its draft is refused and the drawn token is -1. */

@@ -171,6 +171,50 @@ def test_verify_as_many_drafts_as_there_may_be(dtype):
     same(logits, drafts, coins, None, [127, 64, 0], 1.0)
 
 
+def test_verify_draws_from_differences():
+    """p and q equal to the last bit of fp32 at one token, whose rest is then far below the bound, and 2^-20 apart at the others: a q x sum that is cut short leaves the first one too much.
+    p_0 is good to 2^-36 of itself, q_0 x sum as well: 2^-36 each of less than a half."""
+    rng = np.random.default_rng(40)
+    rows = []
+    while len(rows) < 24:
+        ab = rng.uniform(-2, 0, size=(200000, 2)).astype(np.float32).astype(np.longdouble)
+        whole = 1 + np.exp(ab).sum(1)
+        p0 = 1 / whole
+        rest = p0 - p0.astype(np.float32).astype(np.longdouble)
+        bits = whole * 2 ** 31 / 2.0 ** np.floor(np.log2(whole))                 # (32 bits ahead of the point)
+        rows += list(ab[(rest >= 0) & (rest < 2.0 ** -36) & (bits % 1 > 0.75) & (p0 > 0.35) & (p0 < 0.5)].astype(np.float32))
+    coins = [float(np.float32(2.0 ** e)) for e in (-16, -14, -13.5, -13, -12.5, -12, -11, -8, -4, -1)]
+    for a, b in rows[:24]:
+        p = np.exp(np.array([0.0, a, b], dtype=np.longdouble))
+        p /= p.sum()
+        q = p.astype(np.float32)
+        q[1:] *= np.float32(1 - 2.0 ** -20)
+        left = np.maximum(p - q.astype(np.longdouble), 0)
+        for coin, token in zip(coins, draw(torch.tensor([0.0, a, b])[None, None], coins, torch.from_numpy(q)[None, None])):
+            assert allowed(left, coin, token, 2.0 ** -35), (a, b, coin, token, left)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_verify_terms_one_by_one(temperature):
+    """Two tokens whose p - q is 2^-20 of p, beside one that leaves nothing: a draw between them tells their exponentials apart to 2^-36.  An error of 2^-36 in p and as much in q x sum is
+    2^-15 of p - q, which moves the border between two of about equal size by 2^-16 at most."""
+    rng = np.random.default_rng(43)
+    for _ in range(150):
+        x = np.array([0, 0, 0], dtype=np.float32)
+        x[0] = -rng.uniform(0, 14) * temperature
+        x[1] = x[0] - rng.uniform(0, 1) * temperature
+        e = np.exp(x.astype(np.longdouble) / np.longdouble(np.float32(temperature)))
+        p = e / e.sum()
+        q = (p * (1 - np.longdouble(2.0) ** -20)).astype(np.float32)
+        q[2] = 1
+        left = np.maximum(p - q.astype(np.longdouble), 0)
+        border = float(left[0] / left.sum())
+        coins = [float(np.float32(border - 2.0 ** -15)), float(np.float32(border + 2.0 ** -15))]
+        a, t = dsk.verify_drafts(torch.from_numpy(x).to(DEV).expand(2, 2, 3), torch.full((2, 1), -1, dtype=torch.int32, device=DEV), torch.tensor([[0, c] for c in coins], device=DEV),
+                                 probs=torch.from_numpy(q).to(DEV).expand(2, 1, 3), temperature=temperature)
+        assert t[:, 0].tolist() == [0, 1], (x, border)
+
+
 def test_verify_lowest_index_of_equal_logits():
     logits = torch.zeros(2, 2, 5000)
     logits[:, :, [4990, 1200, 77]] = 5.0

@@ -1049,10 +1049,12 @@ class Cache8:
         return out
 
     def check(self):
-        """Waits for the GPU and raises if a call met a block number outside the cache, tokens outside a table or a wait that gave up; the status is cleared."""
+        """Waits for the GPU, all of its streams, and raises if a call met a block number outside the cache, tokens outside a table or a wait that gave up; the status is cleared."""
+        self._torch.cuda.synchronize(self.device)
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
+            self._torch.cuda.synchronize(self.device)          # (a call behind this one may be on another stream)
             raise DskError("8-bit cache: " + ", ".join(t for b, t in ((1, "a block number outside the cache"), (2, "tokens outside the table"), (4, "a wait inside a kernel gave up")) if bits & b))
 
 

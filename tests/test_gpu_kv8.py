@@ -484,6 +484,24 @@ def test_attend_captured_replayed_and_on_two_streams(rows):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], third)
 
 
+def test_check_waits_for_every_stream():
+    """What a call on another stream is still to meet is not missed, and is cleared once it was told."""
+    c = Case([40], 1, 64, 64, 16)
+    cache = c.device()
+    bad = c.t.clone()
+    bad[0, 0] = -1
+    q = torch.randn(1, 1, 1, 64, device=DEV, dtype=torch.bfloat16)
+    lens, side = ints([40]), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)                       # (a fifth of a second)
+        cache.attend(q, bad, lens)
+    with pytest.raises(dsk.DskError, match="block number"):
+        cache.check()
+    torch.cuda.synchronize()
+    cache.check()
+
+
 def test_refusals():
     c = Case([20], 2, 64, 64, 16)
     cache = c.device()

@@ -242,11 +242,12 @@ template <int DK, int DV> int attend_tiles(const kv8::Attn& P, const Layout& L, 
 }  // namespace
 
 extern "C" int dsk_kv8_write(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, void* stream) {
-  if (check_cache(c, s)) return -1;
+  if (const int code = check_cache(c, s)) return code;
   const int dt = k ? k->dtype : -1;
   if (dt != DSK_DT_F32 && dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_write: keys and values are F32, F16 or BF16");
   if (!s->batch || !s->rows) return 0;
-  if (check_view("keys", k, dt) || check_view("values", v, dt)) return -1;
+  if (const int code = check_view("keys", k, dt)) return code;
+  if (const int code = check_view("values", v, dt)) return code;
   OnDevice on(c->device);
   CK(on.error);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -254,11 +255,12 @@ extern "C" int dsk_kv8_write(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_
 }
 
 extern "C" int dsk_kv8_read(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* k, const dsk_view* v, void* stream) {
-  if (check_cache(c, s)) return -1;
+  if (const int code = check_cache(c, s)) return code;
   const int dt = k ? k->dtype : -1;
   if (dt != DSK_DT_F32 && dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_read: keys and values are F32, F16 or BF16");
   if (!s->batch || !s->rows) return 0;
-  if (check_view("keys", k, dt) || check_view("values", v, dt)) return -1;
+  if (const int code = check_view("keys", k, dt)) return code;
+  if (const int code = check_view("values", v, dt)) return code;
   OnDevice on(c->device);
   CK(on.error);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -267,25 +269,26 @@ extern "C" int dsk_kv8_read(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_v
 
 extern "C" int dsk_kv8_attn_workspace(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, int keep_first, size_t* bytes) {
   if (!bytes) return fail(-1, "bad arguments");
-  if (check_cache(c, s)) return -1;
+  if (const int code = check_cache(c, s)) return code;
   Layout L{};
-  if (layout_of(c, s, heads, window, keep_first, &L)) return -1;
+  if (const int code = layout_of(c, s, heads, window, keep_first, &L)) return code;
   *bytes = L.bytes;
   return 0;
 }
 
 extern "C" int dsk_kv8_attn(const dsk_kv8* c, const dsk_kv8_rows* s, const dsk_view* q, const dsk_view* out, int heads, float scale, int window, int keep_first, void* workspace,
                             size_t workspace_bytes, void* stream) {
-  if (check_cache(c, s)) return -1;
+  if (const int code = check_cache(c, s)) return code;
   const int dt = q ? q->dtype : -1;
   if (dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_attn: queries are F16 or BF16");
   if (!(std::fabs(scale) < INFINITY)) return fail(-4, "dsk_kv8_attn: the scale is not a number");
   if (window < 0 || keep_first < 0) return fail(-4, "window %d and keep_first %d must not be negative", window, keep_first);
   if (heads <= 0 || heads % c->kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed", heads, c->kv_heads);
   if (!s->batch || !s->rows) return 0;
-  if (check_view("queries", q, dt) || check_view("output", out, dt)) return -1;
+  if (const int code = check_view("queries", q, dt)) return code;
+  if (const int code = check_view("output", out, dt)) return code;
   Layout L{};
-  if (layout_of(c, s, heads, window, keep_first, &L)) return -1;
+  if (const int code = layout_of(c, s, heads, window, keep_first, &L)) return code;
   if (L.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < L.bytes)) return fail(-1, "dsk_kv8_attn: a workspace of %zu bytes is needed, 16-byte aligned (%zu given)", L.bytes, workspace_bytes);
   OnDevice on(c->device);
   CK(on.error);
@@ -316,7 +319,7 @@ static int pieces_of(const dsk_verify_args* a) { return (a->vocab + verify::kPie
 
 extern "C" int dsk_verify_workspace(const dsk_verify_args* a, size_t* bytes) {
   if (!bytes) return fail(-1, "bad arguments");
-  if (check_verify(a)) return -1;
+  if (const int code = check_verify(a)) return code;
   *bytes = (size_t)a->batch * (a->drafts + 1) * pieces_of(a) * sizeof(float2);
   return 0;
 }
@@ -329,17 +332,17 @@ template <typename T> static int verify_as(const verify::Params& P, cudaStream_t
 }
 
 extern "C" int dsk_verify(const dsk_verify_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-  if (check_verify(a)) return -1;
+  if (const int code = check_verify(a)) return code;
   if (a->logits_dtype != DSK_DT_F32 && a->logits_dtype != DSK_DT_F16 && a->logits_dtype != DSK_DT_BF16) return fail(-4, "dsk_verify: logits are F32, F16 or BF16");
   if (!(a->temperature >= 0.f && a->temperature < INFINITY)) return fail(-4, "temperature must be >= 0");
   if (a->temperature > 0.f && a->temperature < 0x1p-120f) return fail(-4, "a temperature of %g: 0 or at least 2^-120 is needed", (double)a->temperature);   // (64 log2(e) / temperature is an fp32 number)
   if (!a->batch) return 0;
   if (!a->logits || !a->coins || !a->accepted || !a->tokens || (a->drafts && !a->draft_tokens)) return fail(-1, "dsk_verify: null memory");
   size_t need = 0;
-  if (dsk_verify_workspace(a, &need)) return -1;
+  if (const int code = dsk_verify_workspace(a, &need)) return code;
   if (!workspace || !aligned(workspace, 8) || workspace_bytes < need) return fail(-1, "dsk_verify: a workspace of %zu bytes is needed, 8-byte aligned (%zu given)", need, workspace_bytes);
   if (!aligned(a->logits, size_of(a->logits_dtype)) || !aligned(a->draft_probs, 4) || !aligned(a->draft_tokens, 4) || !aligned(a->count, 4) || !aligned(a->coins, 4) || !aligned(a->accepted, 4) || !aligned(a->tokens, 4)) return fail(-1, "dsk_verify: memory is not aligned to its element");
-  if (check_device(a->device)) return -1;
+  if (const int code = check_device(a->device)) return code;
   OnDevice on(a->device);
   CK(on.error);
   verify::Params P;

@@ -343,7 +343,7 @@ int dsk_comm_init(dsk_model* m, const void* nccl_unique_id128);
  * A key / value cache held in 8 bits, attention over it, and the verification of drafted tokens, for programs that serve several sequences or decode
  * speculatively.  (The reference has neither.)  They belong to no model and need no dsk_init: pointers are device memory of `device`, work goes to `stream` (a cudaStream_t, null: the
  * default stream), nothing is allocated, waited for or kept between calls, the caller's current device stays what it is, and calls can be captured into graphs.  Calls that may
- * run at the same time need workspaces of their own.  What the device alone can see (a block outside the cache, tokens outside the table) sets bits of `status`: such rows are not
+ * run at the same time need workspaces of their own.  A call that is refused returns -4 (a size or type that it does not have) or -1 (memory or a device that is not there), -2: an error of CUDA's.  What the device alone can see (a block outside the cache, tokens outside the table) sets bits of `status`: such rows are not
  * written, not read and not seen by attention.
  *
  * The cache is made of blocks of `block` tokens (16, 32, 64 or 128): codes [n_blocks][kv_heads][block][dim] in E4M3, one scale [n_blocks][kv_heads] for every block and head, value =

@@ -63,6 +63,30 @@ def test_row_refusals(kw, text):
     _says(L.dsk_kv8_attn(c, s, x, x, 4, 1.0, 0, 0, None, 0, None), text)
 
 
+@pytest.mark.parametrize("cache,rows,view,code", [(dict(), dict(), dict(dtype=3), -4), (dict(block=48), dict(), dict(), -4), (dict(dim_v=272), dict(), dict(), -4), (dict(kv_heads=40000), dict(), dict(), -4),
+                                                  (dict(), dict(batch=65536), dict(), -4), (dict(), dict(rows=-1), dict(), -4), (dict(k=None), dict(), dict(), -1), (dict(), dict(table=None), dict(), -1),
+                                                  (dict(device=-1), dict(), dict(), -1)])
+def test_refusals_return_their_code(cache, rows, view, code):
+    """-4: a form that the call does not have, -1: memory or a device that is not there."""
+    if view and not torch.cuda.is_available():
+        pytest.skip("types are looked at behind the device")
+    c, mem = _cache(**cache)
+    s, x = _rows(mem, **rows), _view(mem, **view)
+    L = dsk.lib()
+    assert L.dsk_kv8_write(c, s, x, x, None) == code and L.dsk_kv8_read(c, s, x, x, None) == code
+    assert L.dsk_kv8_attn(c, s, x, x, 4, 1.0, 0, 0, None, 0, None) == code
+    if not view:
+        assert L.dsk_kv8_attn_workspace(c, s, 4, 0, 0, C.byref(C.c_size_t())) == code
+
+
+@pytest.mark.parametrize("kw,code", [(dict(batch=-1), -4), (dict(vocab=0), -4), (dict(drafts=128), -4)])
+def test_verify_refusals_return_their_code(kw, code):
+    d = dict(batch=1, drafts=2, vocab=8)
+    d.update(kw)
+    a = dsk.VerifyArgs(**d)
+    assert dsk.lib().dsk_verify(a, None, 0, None) == code and dsk.lib().dsk_verify_workspace(a, C.byref(C.c_size_t())) == code
+
+
 def test_null_structures():
     c, mem = _cache()
     s, x = _rows(mem), _view(mem)

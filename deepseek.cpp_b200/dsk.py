@@ -500,7 +500,7 @@ def build(force: bool = False) -> str:
         if not os.path.exists(os.environ["DSK_LIB"]):
             raise DskError(f"DSK_LIB={os.environ['DSK_LIB']} does not exist")
         return os.environ["DSK_LIB"]
-    srcs = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc")) if f.endswith((".cu", ".cuh"))]
+    srcs = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc")) if f.endswith((".cu", ".cuh", ".h"))]
     srcs.append(os.path.join(REPO, "include", "dsk.h"))
     stale = not os.path.exists(LIB_PATH) or any(os.path.getmtime(s) > os.path.getmtime(LIB_PATH) for s in srcs)
     if (force or stale) and os.path.exists("/usr/local/cuda/bin/nvcc"):

@@ -118,6 +118,23 @@ def test_tensors_on_the_host_are_refused():
         dsk.Cache8.of(z, z, torch.ones(1, 1), torch.ones(1, 1))
 
 
+def test_every_source_of_the_library_makes_it_stale(monkeypatch):
+    """An edit of any file that its objects depend on compiles the library again."""
+    import os
+    if os.environ.get("DSK_LIB") or not os.path.exists("/usr/local/cuda/bin/nvcc"):
+        pytest.skip("an explicit library, or no compiler")
+    dsk.build()
+    folder = os.path.join(dsk.HERE, "csrc")
+    made, real = [], os.path.getmtime
+    monkeypatch.setattr(dsk.subprocess, "check_call", lambda *a, **k: made.append(a))
+    for f in sorted(f for f in os.listdir(folder) if os.path.isfile(os.path.join(folder, f))) + ["../../include/dsk.h"]:
+        new = os.path.abspath(os.path.join(folder, f))
+        monkeypatch.setattr(os.path, "getmtime", lambda p: real(p) if os.path.abspath(p) != new else real(dsk.LIB_PATH) + 10)
+        dsk.build()
+        assert len(made) == 1, f
+        made.clear()
+
+
 def test_structures_have_the_compilers_layout(tmp_path):
     import os
     import subprocess

@@ -5,7 +5,9 @@
 // empty with the few queries of decoding.  An E4M3 code is exact in fp16, so keys and values go from their codes to operands by a conversion alone; a query is divided by a power
 // of two that puts its largest entry near 2^10 (what that leaves below fp16's range is 2^-24 of it).  The scales are applied around the products: the key block's to the
 // scores, the value block's inside the softmax, w_j = 2^(t_j - m) with t_j = score_j + log2(value scale), so that a weight with its scale is one fp16 number of at most 2^kSlack
-// and the sum takes w_j / (value scale).  Rounding: the weights to fp16, 2^-11 of each; queries in fp16 or bf16 are exact.
+// and the sum takes w_j / (value scale).  Rounding: the weights to fp16, 2^-11 of each, and 2^-31 of the row's largest for those below 2^-20 of it: a reference m lies kLift below the largest
+// t_j that it was taken from (at that itself, fp16 ends at 2^-25 of the largest weight: of a long tail behind one large weight the sum kept what the results lost, 2^-9 of a row at 131072 keys
+// and all of an entry that the large one has as zero); queries in fp16 or bf16 are exact.
 // Work: the steps (32 keys, 16 where heads have 256 entries) of all sequences, key heads and query tiles lie in one line that the CTAs share out evenly, four steps to a unit, whatever the lengths; a CTA that has
 // a whole (sequence, head, tile) stores it, pieces are joined by `join`.  Every warp has every fourth step, with stages of its own that cp.async fills: no barrier but where
 // a piece ends, and the copies run on across pieces.
@@ -29,7 +31,7 @@ __host__ __device__ constexpr int step_of(int dv) { return dv < 256 ? 32 : 16; }
 __device__ __forceinline__ long long quotient(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }   // (of numbers >= 0)
 constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
 constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
-constexpr float kSlack = 8.f;                                // the reference of a row's weights follows its maximum once that is 2^8 ahead
+constexpr float kLift = 7.f, kSlack = 15.f;                  // the reference of a row's weights is taken kLift below its maximum, and follows once that is kSlack ahead (fp16 ends at 2^16)
 
 struct Attn {
   Cache C;
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(kThreads) attend_tokens(const Attn P) {
                 s[t][u][2 + e] = fmaf(s[t][u][2 + e], f[e][u], lift[u]) - lift[u];
                 f[e][u] = 1.f;
               }
-            const float to = fmaxf(m[t][e], mx[e]), by = exp2_fast(m[t][e] - to);
+            const float to = fmaxf(m[t][e], fabsf(mx[e]) > kFar ? mx[e] : mx[e] - kLift), by = exp2_fast(m[t][e] - to);
             m[t][e] = to;
             l[t][e] *= by;
 #pragma unroll

@@ -5,8 +5,8 @@
 // values', turn them into fp16 (exact) and store them as swizzled operands, so that the cache crosses HBM and L2 as bytes; one thread issues the products, scores into TMEM, weights from TMEM;
 // a group of four warps for each tile of rows has the softmax, a thread to a row.  Two tiles: one's products run under the other's softmax, weights lie where the scores were, and a
 // tile's next scores wait for the product that reads its weights.  One tile: scores lie in two places in turn, and the next tile's products run under this one's softmax.
-// Scales and weights as in dsk_kv8_attn.cuh: key scales on the scores, value scales inside the exponent, fp16 weights of at most 2^kLag.
-// The results stay in TMEM; they are scaled again only where a row's maximum is 2^kLag ahead of the reference of its weights, by the thread that has the row.
+// Scales and weights as in dsk_kv8_attn.cuh: key scales on the scores, value scales inside the exponent, fp16 weights of at most 2^kSlack, references kLift below a maximum, as whole numbers.
+// The results stay in TMEM; they are scaled again only where a row's maximum is kSlack ahead of the reference of its weights, by the thread that has the row.
 // NaN among values: a tile that some row does not see whole goes to the products with zeros in their place, and rows that do see one get it back at the end.
 // Bound: the softmax.  Of some 4500 cycles for 256 rows and 128 keys of 192 + 128 entries the weights of one group take 1500 (1024 of the exponentials' pipe), its maxima 500, the products
 // 2560 of the tensor pipe, and a group's products and the way there and back stand 1700 behind its weights.  2048 queries behind 3952 tokens, 16 heads of 192 + 128: 133 us (104 GFLOP:
@@ -20,7 +20,6 @@ namespace dsk {
 namespace kv8 {
 
 constexpr int kTile = 128, kRowThreads = 512, kSlots = 4;    // keys of a tile; threads of a CTA; tiles whose scales are held
-constexpr float kLag = 14.f;                                 // a row's weights are at most 2^kLag
 
 struct Portion {
   Attn A;                                                    // row_tiles: of a CTA's rows
@@ -438,7 +437,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
         continue;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      // Half a row of scores in registers at a time, each read once: the reference may lag behind the maximum by kLag, within fp16's range, so that the first half's weights do not wait for
+      // Half a row of scores in registers at a time, each read once: the reference may lag behind the maximum by kSlack, within fp16's range, so that the first half's weights do not wait for
       // the second half's maximum; where that moves the reference after all, weights that are stored already are scaled again, by a power of two since references are whole numbers: exactly, but
       // for what comes below 2^-14, where fp16 has multiples of 2^-24.
 #pragma unroll 1
@@ -468,11 +467,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
           top = fmaxf(top, fmaf(z, fs[g], lift[g]));
         }
         if (__any_sync(0xffffffffu, top > limit)) {
-          const float to = fmaxf(m, ceilf(top)), by = exp2_fast(m - to);
+          const float c_top = ceilf(top), to = fmaxf(m, fabsf(c_top) > kFar ? c_top : c_top - kLift), by = exp2_fast(m - to);
           m = to;
           l *= by;
           const bool far = fabsf(m) > kFar;
-          limit = far ? -INFINITY : m + kLag;
+          limit = far ? -INFINITY : m + kSlack;
           if (__any_sync(0xffffffffu, far)) {                // (maxima beyond it under a reference that is not have weights of zero as they are)
 #pragma unroll
             for (int g = 0; g < 4; g++) {

@@ -668,6 +668,27 @@ def test_attend_more_tokens_than_an_odd_table_has(rows, block):
         cache.check()
 
 
+@pytest.mark.parametrize("rows", [1, 6, 40, 1024])
+@pytest.mark.parametrize("sink", [0, 30000])
+def test_attend_long_tails_beside_one_large_weight(rows, sink):
+    """A key with nearly all of the weight and no value, and tens of thousands at 2^-25 of it, which are all of the result: each of their weights is off by 2^-11 of itself or 2^-31 of the
+    large one."""
+    n, kv, G, d = 32768, 8, 4, 64
+    one, top = (int(so.encode(np.array([x]))[0]) for x in (1.0, 26.0))
+    k = torch.zeros(n // 128, kv, 128, d, dtype=torch.uint8, device=DEV)
+    v = torch.full((n // 128, kv, 128, d), one, dtype=torch.uint8, device=DEV)
+    k[sink // 128, :, sink % 128, 0], v[sink // 128, :, sink % 128] = top, 0
+    scale = torch.ones(n // 128, kv, device=DEV)
+    cache = dsk.Cache8.of(k.view(F8), v.view(F8), scale, scale.clone())
+    table = torch.arange(n // 128, dtype=torch.int32, device=DEV)[None]
+    q = torch.zeros(1, rows, kv * G, d, dtype=torch.bfloat16, device=DEV)
+    q[..., 0] = 0.96875
+    out = cache.attend(q, table, ints([n]), scale=float(np.log(2.0)))[0].double().cpu().numpy()
+    tail = np.arange(n - rows, n) * 2.0 ** (-26 * 0.96875)   # (row i sees n - rows + i keys beside the large one)
+    want = (tail / (1 + tail))[:, None, None]
+    assert (np.abs(out - want) <= want * (2.0 ** -11 + 2.0 ** -8 + 2.0 ** -18) + n * 2.0 ** -31).all(), np.abs(out / want - 1).max()
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_offsets_beyond_32_bits(rows):
     """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""

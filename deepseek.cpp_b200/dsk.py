@@ -1033,7 +1033,7 @@ class Cache8:
             out = (torch.empty if count is None else torch.zeros)(shape, dtype=q.dtype, device=q.device)
         elif out.dtype is not q.dtype:
             raise DskError(f"results of {out.dtype} for queries of {q.dtype}")
-        window, keep_first = min(window, 0x7fffffff), min(keep_first, 0x7fffffff)
+        window, keep_first = max(-1, min(window, 0x7fffffff)), max(-1, min(keep_first, 0x7fffffff))   # (what an int has; negative ones are refused)
         s = self._rows(table, lens, count, rows)
         a, b = self._view("queries", q, (batch, rows, heads, self.dim_k)), self._view("output", out, shape, True)
         key = (batch, rows, heads, table.shape[1], window, keep_first)

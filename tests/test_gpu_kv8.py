@@ -484,6 +484,16 @@ def test_attend_captured_replayed_and_on_two_streams(rows):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], third)
 
 
+@pytest.mark.parametrize("far", [-1, -2 ** 31, -2 ** 32, -2 ** 40])
+def test_attend_negative_windows_of_any_size_are_refused(far):
+    c = Case([20], 1, 64, 64, 16)
+    cache = c.device()
+    q = torch.zeros(1, 1, 1, 64, device=DEV, dtype=torch.bfloat16)
+    for kw in (dict(window=far), dict(keep_first=far), dict(window=far, keep_first=far)):
+        with pytest.raises(dsk.DskError, match="negative"):
+            cache.attend(q, c.t, ints([20]), **kw)
+
+
 def test_check_waits_for_every_stream():
     """What a call on another stream is still to meet is not missed, and is cleared once it was told."""
     c = Case([40], 1, 64, 64, 16)

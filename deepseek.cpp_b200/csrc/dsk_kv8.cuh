@@ -4,10 +4,10 @@
 // Scales are powers of two, the smallest s with amax <= 448 s: multiplying by one is exact, so that a value is rounded once, by the conversion to E4M3
 // (at most half a step, 2^-4 of it, or 2^-10 s below 2^-6 s), whatever else the block holds.  A float code keeps its relative accuracy at any scale within its range, so
 // the up to one bit of range that a power of two leaves unused costs nothing but there.  A block is written in several calls: its scale never falls while it holds rows
-// of earlier ones, and where it grows, their codes are rounded again, which changes those alone that leave the normal range.  Exponents stay within +-kExp:
-// attention keeps weights times scales in fp32 (dsk_kv8_attn.cuh).
+// of earlier ones, and where it grows, their codes are rounded again, which changes those alone that leave the normal range.  Exponents stay within +-kExp,
+// so that attention's sums of weights over scales stay in fp32's range (dsk_kv8_attn.cuh).
 // Bound of both kernels: bytes; small calls by the chain of dependent loads (first token, block, rows).  Four prompts of up to 8191 tokens, 16 heads of 192 + 128 entries in bf16 are written in
-// 79 us (409 MB: 5.2 TB/s; a measured copy 6.5), 8 x 8000 tokens of 4 heads of 128 + 128 read in 32 us (160 MB: 5.0 TB/s), one token written in 2.0 us, 161 read in 2.3.
+// 79 us (409 MB: 5.2 TB/s; a measured copy 6.5), 8 x 8000 tokens of 4 heads of 128 + 128 read in 32 us (160 MB: 5.0 TB/s), one token written in 2.2 us, 161 read in 2.3.
 #pragma once
 
 #include <cuda_bf16.h>

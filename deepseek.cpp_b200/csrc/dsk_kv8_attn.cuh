@@ -14,7 +14,7 @@
 // A call of few pieces has clusters instead of the line (SHARED).
 // Bound: in large calls the dependent instructions of a step (some 560 for 32 keys and a tile of 8 queries: conversions, fragments, products, softmax; steps of 16 keys spend more of
 // them on what a step does once) at 8 warps an SM, which leave 64 % of the issue slots empty; in small calls the chain of a step and the joins.  64 sequences of up to 16000 tokens, 16 heads of 128 over 4: 107 us (533 MB: 5.0 TB/s; a measured copy 6.5);
-// a token and four drafts of 16 sequences, window 1024: 18 us; one token behind 1000: 8.4 us.  With queries as the left operand, half of whose rows were empty: 295 us for the first.
+// a token and four drafts of 16 sequences, window 1024: 18 us; one token behind 1000: 8.6 us.  With queries as the left operand, half of whose rows were empty: 295 us for the first.
 // Fragments come from shared memory as whole 16-byte pieces, entries and keys permuted alike on both sides of a product: a quarter warp's lanes (two
 // keys x four pieces) are keys j and j + 4, whose rows lie 16 banks apart.
 #pragma once

@@ -9,8 +9,8 @@
 // The results stay in TMEM; they are scaled again only where a row's maximum is kSlack ahead of the reference of its weights, by the thread that has the row.
 // NaN among values: a tile that some row does not see whole goes to the products with zeros in their place, and rows that do see one get it back at the end.
 // Bound: the softmax.  Of some 4500 cycles for 256 rows and 128 keys of 192 + 128 entries the weights of one group take 1500 (1024 of the exponentials' pipe), its maxima 500, the products
-// 2560 of the tensor pipe, and a group's products and the way there and back stand 1700 behind its weights.  2048 queries behind 3952 tokens, 16 heads of 192 + 128: 133 us (104 GFLOP:
-// 785 TFLOP/s; a measured product of matrices 1638), heads of 256: 235 us (167 GFLOP: 710), 3 x 777 queries of 16 heads of 64 over 4 with a window of 512: 27 us.
+// 2560 of the tensor pipe, and a group's products and the way there and back stand 1700 behind its weights.  2048 queries behind 3952 tokens, 16 heads of 192 + 128: 137 us (104 GFLOP:
+// 760 TFLOP/s; a measured product of matrices 1638), heads of 256: 240 us (167 GFLOP: 695), 3 x 777 queries of 16 heads of 64 over 4 with a window of 512: 27 us.
 #pragma once
 
 #include "dsk_kv8_attn.cuh"

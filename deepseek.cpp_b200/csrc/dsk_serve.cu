@@ -180,8 +180,9 @@ int layout_of(const dsk_kv8* c, const dsk_kv8_rows* s, int heads, int window, in
     L->row_tiles = (int)((rows + each - 1) / each);
     const long long tiles = (long long)s->batch * c->kv_heads * L->row_tiles;
     // Keys are shared out where that is expected to pay: waves of CTAs x (their tiles of keys, and what a CTA does once), and the pieces through memory (ns, from the cases below).  us with
-    // one share / with what the rule takes: 700 queries of 32 heads over 8 behind 7300 tokens 162 / 131 (three shares), 3 x 777 of 16 heads of 64 over 4, 4000 tokens, 126 / 114; with one,
-    // which the rule takes / with two: 2048 queries of 16 heads behind 3952 tokens 134 / 158, 1500 of 24 heads behind 1500 72 / 89, 500 queries of 64 heads over 8, two sequences, 139 / 163.
+    // one share / with what the rule takes: 700 queries of 32 heads over 8 behind 7300 tokens 161 / 131 (three shares), 3 x 777 of 16 heads of 64 over 4, 4000 tokens, 127 / 114; with one,
+    // which the rule takes / with two: 2048 queries of 16 heads behind 3952 tokens 137 / 160, 1500 of 24 heads behind 1500 74 / 90, 500 queries of 64 heads over 8, two sequences of 3000
+    // tokens, 134 / 181.  A table that has room for more than its sequence is priced as if that were there: 2048 tokens of 32 heads over 8 take 64 us, 159 behind a table for 32768.
     const int tile = L->shape == 3 ? 3500 : L->tiles == 2 ? 2400 : 1800, group = heads / c->kv_heads, cols = kShapes[L->shape][1] + 2;
     const long long seen = window ? std::min(keys, (long long)window + each / group + keep_first + kv8::kTile) : keys, key_tiles = std::max(1ll, (seen + kv8::kTile - 1) / kv8::kTile);
     long long best = -1;

@@ -7,7 +7,7 @@
 // neighbour.  pick takes that row's exponentials in two fp32 parts, good to 2^-36 of each, as whole numbers of 2^-61 of the power of two above the row's sum, whose sums are the same in
 // any order and miss at most 2^-40 of the row by what each loses below one (2^20 entries; as multiples of a fixed 2^-45 at least one each, the tail of a row weighed up to 2^-28 of it, where
 // it should have had 2^-32); p and q meet as such numbers too.  Where coin x q is within 1e-4 of p, the row's sum is taken that way as well.
-// Bound: row_stats by the bytes of the logits; pick by the instructions of its exponentials (some 77 each) where sequences are many, otherwise by the latency of its steps, two walks over a row
+// Bound: row_stats by the bytes of the logits; pick by the instructions of its exponentials (some 86 each, all that a value takes included) where sequences are many, otherwise by the latency of its steps, two walks over a row
 // that L2 holds and a cluster's barrier behind each among them.  Seven drafts of 32 sequences over 129280 tokens: 48 us, 14.5 of them row_stats (exponentials in fp64: 71); four drafts of
 // one over 32000: 14 us (15.7 with the statistics in pick's clusters instead of a launch of their own).
 #pragma once

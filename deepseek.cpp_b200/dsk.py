@@ -1023,7 +1023,8 @@ class Cache8:
 
     def attend(self, q, table, lens, count=None, scale: Optional[float] = None, window: int = 0, keep_first: int = 0, out=None):
         """Attention of queries q [batch, rows, heads, dim_k] (float16 or bfloat16), the last count[b] of a sequence's lens[b] tokens, over the cache (dsk_kv8_attn); scale: dim_k ** -0.5
-        unless given.  Returns [batch, rows, heads, dim_v] in the queries' type, `out` or a new tensor (zeros in rows from count[b] on)."""
+        unless given.  Returns [batch, rows, heads, dim_v] in the queries' type, `out` or a new tensor (zeros in rows from count[b] on).  Work is laid out for the width of `table`: pass
+        table[:, :blocks] where the longest sequence is known to be shorter."""
         torch = self._torch
         if q.dim() != 4 or q.shape[0] != table.shape[0]:
             raise DskError(f"queries are [batch, rows, heads, dim_k], got {tuple(q.shape)} for a table of {table.shape[0]} sequences")

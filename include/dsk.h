@@ -350,7 +350,9 @@ int dsk_comm_init(dsk_model* m, const void* nccl_unique_id128);
  * code x scale; dim_k and dim_v are multiples of 16 up to 256.  Token t of sequence b lies in block table[b][t / block] at row t % block.  Scales are powers of two from 2^-40 to 2^40:
  * dsk_kv8_write takes the smallest s with |x| <= 448 s over the finite values that it writes to a block and head, never less than the old one while the block holds
  * tokens ahead of the first written one, and where that grows it rounds their codes again; a block whose first token is written starts anew.  Values beyond the range (infinities
- * too) become +-448 s, NaN stays NaN.  A block that is written to belongs to one sequence; blocks that are only read may be shared. */
+ * too) become +-448 s, NaN stays NaN.  What a block holds behind the written tokens is given up: where the scale grows or the block starts anew, those codes no longer stand for their values.
+ * A block that is written to belongs to one sequence; blocks that are only read may be shared.  Codes behind a sequence's last token, and blocks that hold none of its tokens, may hold anything, scales too: no
+ * result depends on them. */
 enum { DSK_KV8_PAGE = 1,   /* status: a block number outside the cache */
        DSK_KV8_RANGE = 2,  /* status: tokens ahead of the first or behind the last block of a table */
        DSK_KV8_WAIT = 4 }; /* status: a wait inside a kernel gave up (results are not valid) */
@@ -370,13 +372,15 @@ typedef struct dsk_view {          /* [batch][row][head][entry], entries side by
   int dtype;                       /* DSK_DT_F32, DSK_DT_F16, DSK_DT_BF16 */
   int64_t batch, row, head;
 } dsk_view;
-/* Rows become tokens first[b] .. of their sequences (heads: kv_heads). */
+/* Rows become tokens first[b] .. of their sequences (heads: kv_heads).  A sequence whose first[b] lies ahead of or behind its table is passed over whole, by dsk_kv8_read too; otherwise the
+ * rows behind the table's end are. */
 int dsk_kv8_write(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* k, const dsk_view* v, void* stream);
 /* The values of tokens first[b] .. in rows, rounded to the view's type. */
 int dsk_kv8_read(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* k, const dsk_view* v, void* stream);
 /* Softmax attention.  first[b]: the sequence's tokens in the cache, the last count[b] of which are the queries' (written ahead of the call): query i is at t = first[b] - count[b] + i and
  * sees the tokens j <= t, with window > 0 those with t - j < window or j < keep_first.  Query head h reads key head h / (heads / kv_heads); out = softmax(scale q k) v in the queries' type
- * (F16 or BF16), zeros for a query that sees nothing.  At most 1024 sequences a call. */
+ * (F16 or BF16), zeros for a query that sees nothing or whose scores are all -inf.  At most 1024 sequences a call.  Work is laid out for the tokens that a table has room for, on the host,
+ * which does not know first[b]: a table much wider than the longest sequence costs time and workspace, so pass as many of its columns as may be in use (table_blocks, with table_pitch as it is). */
 int dsk_kv8_attn_workspace(const dsk_kv8* cache, const dsk_kv8_rows* rows, int heads, int window, int keep_first, size_t* bytes);   /* 0: none */
 int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* q, const dsk_view* out, int heads, float scale, int window, int keep_first,
                  void* workspace, size_t workspace_bytes, void* stream);
@@ -385,7 +389,7 @@ int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view*
  * accepted ones the next token is drawn from p (temperature: 0, or at least 2^-120).  A draw is the lowest index whose running sum is over coins[drafts] x (whole sum), sums good to 2^-35 (of p's, which is 1).  temperature 0: a draft is accepted
  * if it is the lowest index of the largest logit, which replaces it otherwise.  Coins lie in [0, 1).  accepted[b]: drafts accepted; tokens[b]: those, the drawn token, -1 in the places behind.
  * draft_probs lie in [0, 1] (-0 is 0); a token whose probability is negative or a NaN is not drawn in place of a draft.
- * A drafted token outside the vocabulary is refused; where a row's logits hold a NaN, or are no distribution (+inf at a temperature, nothing but -inf), its draft is refused and the drawn token is -1. */
+ * Where nothing is left of max(p_i - q_i, 0), the drawn token is -1.  A drafted token outside the vocabulary is refused; where a row's logits hold a NaN, or are no distribution (+inf at a temperature, nothing but -inf), its draft is refused and the drawn token is -1. */
 typedef struct dsk_verify_args {
   const void* logits;              /* [batch][drafts + 1][vocab], pitches in elements */
   const float* draft_probs;        /* [batch][drafts][vocab], nullable */

@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       __syncwarp();
       if (lane == 0) hy::tc_arrive(TILES == 2 ? pfull + 8 * t : pfull + 8 * (i & 1));
     }
-    ok = ok && wait_warp(cdone, 0, A.C) && (n == 0 || wait_warp(pvdone + 8 * t, (n - 1) & 1, A.C));
+    // One tile: the last scores wait for the product before the last but one alone, and a parity tells a phase from its neighbours only, so the last but one is waited for first.
+    ok = ok && wait_warp(cdone, 0, A.C) && (TILES == 2 || n < 2 || wait_warp(pvdone, (n - 2) & 1, A.C)) && (n == 0 || wait_warp(pvdone + 8 * t, (n - 1) & 1, A.C));
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       uint32_t lost[DV / 32] = {};                           // entries of this row that see a NaN

@@ -699,6 +699,36 @@ def test_attend_long_tails_beside_one_large_weight(rows, sink):
     assert (np.abs(out - want) <= want * (2.0 ** -11 + 2.0 ** -8 + 2.0 ** -18) + n * 2.0 ** -31).all(), np.abs(out / want - 1).max()
 
 
+@pytest.mark.parametrize("d,dtype", [(64, "bf16"), (128, "f16"), (192, "bf16"), (256, "f16")])
+def test_attend_values_that_come_late(d, dtype):
+    """One tile of rows to a CTA and more keys than L2 holds: a product that waits for its values is not through when the softmax of the next tile, the last one, is.  Every call gives the
+    same bits, and those are right (float64 on the GPU; the tolerances of the whole file)."""
+    B, H, rows, n, block, dv = 48, 4, 40, 5000, 32, min(d, 128)
+    g = torch.Generator(device=DEV).manual_seed(d)
+    per = -(-n // block)
+    lens = [n - (61 * b) % 2300 for b in range(B)]
+    table = torch.randperm(B * per, generator=torch.Generator().manual_seed(1)).to(torch.int32).reshape(B, per).to(DEV)
+    k, v = ((torch.randn(B * per, H, block, x, generator=g, device=DEV) * 100).clamp(-448, 448).to(F8) for x in (d, dv))
+    scale = torch.full((B * per, H), 2.0 ** -7, device=DEV)
+    cache = dsk.Cache8.of(k, v, scale, scale.clone())
+    q = (torch.randn(B, rows, H, d, generator=g, device=DEV) * 4).to(DT[dtype])
+    first = cache.attend(q, table, ints(lens))
+    for _ in range(60):
+        assert torch.equal(first, cache.attend(q, table, ints(lens)))
+    half = torch.finfo(DT[dtype]).eps / 2
+    for b in range(0, B, 5):
+        L = lens[b]
+        kk, vv = ((x[table[b].long()].double() * 2.0 ** -7).transpose(0, 1).flatten(1, 2)[:, :L] for x in (k, v))
+        qq = q[b].double().transpose(0, 1)
+        w = (qq @ kk.transpose(1, 2) * d ** -0.5).masked_fill(torch.arange(L, device=DEV) > torch.arange(L - rows, L, device=DEV)[:, None], -np.inf)
+        p = torch.softmax(w, -1)
+        size = (qq.abs() @ kk.abs().transpose(1, 2)).amax(-1, keepdim=True) * d ** -0.5
+        tol = p @ vv.abs() * (2.0 ** -11 + 2 * (d + 4) * 2.0 ** -23 * size + 2.0 ** -20 + L * 2.0 ** -24) + L * 2.0 ** -25 * 448 * 2.0 ** -7 * p.amax(-1, keepdim=True)
+        want = p @ vv
+        off = (first[b].double().transpose(0, 1) - want).abs()
+        assert (off <= tol + half * (want.abs() + tol) + 2.0 ** -25).all(), b
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_offsets_beyond_32_bits(rows):
     """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""

@@ -413,6 +413,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
     auto factor = [&](float key_scale) { return fmaxf(row_scale * key_scale, 1.17549435e-38f); };   // (positive: -inf stays what it is)
     float m = kLowest, l = 0.f, limit = -INFINITY;             // limit: where a maximum moves the reference; any does while that is beyond kFar
     bool ok = true;
+    // A wait by parity is right while the barrier is in the phase asked for or the one behind it.  With one tile, scores i are issued behind product i - 2 alone: product i - 1 is waited for by
+    // whoever reads results of tile i, and ahead of handing over the last weights, without which product n - 1 cannot be through; then the wait for that one is right as well.
+    auto product_ahead = [&](int i) {
+      if (TILES == 1 && i > 0 && i + 1 == n) ok = wait_warp(pvdone, (i - 1) & 1, A.C) && ok;
+    };
     const bool idle = (row0 + warp * 32) / A.group >= w.count;              // none of the warp's rows exists
     for (int i = 0; i < n; i++) {
       const int slot = i % kSlots, key0 = key_of(w, w.begin + i);
@@ -432,6 +437,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
       ok = ok && (TILES == 2 ? wait_warp(sfull + 8 * t, i & 1, A.C) : wait_warp(sfull + 8 * (i & 1), (i >> 1) & 1, A.C));
       if (!ok) break;
       if (idle) {                                            // (its rows' results are whatever comes of the scores as weights, and go nowhere)
+        product_ahead(i);
         __syncwarp();
         if (lane == 0) hy::tc_arrive(TILES == 2 ? pfull + 8 * t : pfull + 8 * (i & 1));
         continue;
@@ -527,13 +533,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) attend_rows(const __grid_const
         tmem_store32(s_at + c, p);
         if (half) scales_of(0);
       }
+      product_ahead(i);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) hy::tc_arrive(TILES == 2 ? pfull + 8 * t : pfull + 8 * (i & 1));
     }
-    // One tile: the last scores wait for the product before the last but one alone, and a parity tells a phase from its neighbours only, so the last but one is waited for first.
-    ok = ok && wait_warp(cdone, 0, A.C) && (TILES == 2 || n < 2 || wait_warp(pvdone, (n - 2) & 1, A.C)) && (n == 0 || wait_warp(pvdone + 8 * t, (n - 1) & 1, A.C));
+    ok = ok && wait_warp(cdone, 0, A.C) && (n == 0 || wait_warp(pvdone + 8 * t, (n - 1) & 1, A.C));
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       uint32_t lost[DV / 32] = {};                           // entries of this row that see a NaN

@@ -729,6 +729,34 @@ def test_attend_values_that_come_late(d, dtype):
         assert (off <= tol + half * (want.abs() + tol) + 2.0 ** -25).all(), b
 
 
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("tiles", [1, 2, 3, 7])
+def test_attend_no_wait_gives_up(tiles, d):
+    """Thousands of CTAs of one row tile and a few tiles of keys, call after call: no wait runs out, every call gives the same bits."""
+    B, H, n, dv = 64, 3, 128 * tiles - 5, min(d, 128) if d < 256 else d
+    g = torch.Generator(device=DEV).manual_seed(d + tiles)
+    per = -(-n // 64)
+    table = torch.arange(B * per, dtype=torch.int32, device=DEV).reshape(B, per)
+    k, v = ((torch.randn(B * per, H, 64, x, generator=g, device=DEV) * 100).clamp(-448, 448).to(F8) for x in (d, dv))
+    scale = torch.full((B * per, H), 2.0 ** -7, device=DEV)
+    cache = dsk.Cache8.of(k, v, scale, scale.clone())
+    for rows, window, keep in ((40, 0, 0), (100, 7, 17)):
+        q = torch.randn(B, rows, H, d, generator=g, device=DEV, dtype=torch.bfloat16)
+        first = cache.attend(q, table, ints([n] * B), window=window, keep_first=keep)
+        assert all(torch.equal(first, cache.attend(q, table, ints([n] * B), window=window, keep_first=keep)) for _ in range(100))
+        for b, i in ((0, 0), (B - 1, rows - 1), (B // 2, rows // 2)):                # (a row each against float64)
+            t, L = n - rows + i, n
+            kk, vv = ((x[table[b].long()].double() * 2.0 ** -7).transpose(0, 1).flatten(1, 2)[:, :L] for x in (k, v))
+            j = torch.arange(L, device=DEV)
+            seen = (j <= t) & ((t - j < window) | (j < keep) if window else j <= t)
+            p = torch.softmax((kk @ q[b, i].double()[:, :, None])[..., 0].mul(d ** -0.5).masked_fill(~seen, -np.inf), -1)
+            want, mass = (p[:, None] @ vv)[:, 0], (p[:, None] @ vv.abs())[:, 0]
+            size = (kk.abs() @ q[b, i].double().abs()[:, :, None]).amax(1) * d ** -0.5
+            tol = mass * (2.0 ** -11 + 2 * (d + 4) * 2.0 ** -23 * size + 2.0 ** -20 + L * 2.0 ** -24) + L * 2.0 ** -25 * 448 * 2.0 ** -7 * p.amax(-1, keepdim=True)
+            assert ((first[b, i].double() - want).abs() <= tol + (want.abs() + tol) * 2.0 ** -8 + 2.0 ** -25).all()
+    cache.check()
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_offsets_beyond_32_bits(rows):
     """A cache of more than 4 GB of keys: its last blocks are written, read and attended."""

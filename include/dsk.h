@@ -343,8 +343,8 @@ int dsk_comm_init(dsk_model* m, const void* nccl_unique_id128);
  * A key / value cache held in 8 bits, attention over it, and the verification of drafted tokens, for programs that serve several sequences or decode
  * speculatively.  (The reference has neither.)  They belong to no model and need no dsk_init: pointers are device memory of `device`, work goes to `stream` (a cudaStream_t, null: the
  * default stream), nothing is allocated, waited for or kept between calls, the caller's current device stays what it is, and calls can be captured into graphs.  Calls that may
- * run at the same time need workspaces of their own.  A call that is refused returns -4 (a size or type that it does not have) or -1 (memory or a device that is not there), -2: an error of CUDA's.  What the device alone can see (a block outside the cache, tokens outside the table) sets bits of `status`: such rows are not
- * written, not read and not seen by attention.
+ * run at the same time need workspaces of their own.  A call that is refused returns -4 (a size or type that it does not have) or -1 (memory or a device that is not there), -2 is an error of CUDA's.
+ * What the device alone can see (a block outside the cache, tokens outside the table) sets bits of `status`: such rows are not written, not read and not seen by attention.
  *
  * The cache is made of blocks of `block` tokens (16, 32, 64 or 128): codes [n_blocks][kv_heads][block][dim] in E4M3, one scale [n_blocks][kv_heads] for every block and head, value =
  * code x scale; dim_k and dim_v are multiples of 16 up to 256.  Token t of sequence b lies in block table[b][t / block] at row t % block.  Scales are powers of two from 2^-40 to 2^40:
@@ -389,7 +389,8 @@ int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view*
  * accepted ones the next token is drawn from p (temperature: 0, or at least 2^-120).  A draw is the lowest index whose running sum is over coins[drafts] x (whole sum), sums good to 2^-35 (of p's, which is 1).  temperature 0: a draft is accepted
  * if it is the lowest index of the largest logit, which replaces it otherwise.  Coins lie in [0, 1).  accepted[b]: drafts accepted; tokens[b]: those, the drawn token, -1 in the places behind.
  * draft_probs lie in [0, 1] (-0 is 0); a token whose probability is negative or a NaN is not drawn in place of a draft.
- * Where nothing is left of max(p_i - q_i, 0), the drawn token is -1.  A drafted token outside the vocabulary is refused; where a row's logits hold a NaN, or are no distribution (+inf at a temperature, nothing but -inf), its draft is refused and the drawn token is -1. */
+ * Where nothing is left of max(p_i - q_i, 0), the drawn token is -1.  A drafted token outside the vocabulary is refused; where a row's logits hold a NaN, or are no distribution (+inf at a
+ * temperature, nothing but -inf), its draft is refused and the drawn token is -1. */
 typedef struct dsk_verify_args {
   const void* logits;              /* [batch][drafts + 1][vocab], pitches in elements */
   const float* draft_probs;        /* [batch][drafts][vocab], nullable */

@@ -37,6 +37,10 @@ struct Rows {                                                // rows of a padded
   int table_blocks, batch, rows;
 };
 struct Pitch { long long batch, row, head; };                // in elements; entries of a head lie side by side
+struct Pieces {                                              // packed rows, cut where a sequence or a block ends: [n] (first row, rows, block, place in the block), no rows: nothing there
+  const int4* at;
+  int rows;                                                  // of the packed ones
+};
 
 __device__ __forceinline__ void note(const Cache& C, int bit) { if (C.status) atomicOr(C.status, bit); }
 
@@ -152,9 +156,19 @@ __device__ __forceinline__ bool piece(const Cache& C, const Rows& S, int b, Piec
   return true;
 }
 
+__device__ __forceinline__ bool piece(const Cache& C, const Pieces& S, int, Piece& p) {
+  const int4 x = __ldg(S.at + blockIdx.x);
+  if (x.y <= 0 || x.x < 0 || x.y > S.rows - x.x || x.w < 0 || x.y > C.block - x.w) return false;   // (nothing outside, whatever the plan says)
+  p.page = x.z;
+  p.kept = x.w;
+  p.rows = x.y;
+  p.from = x.x;
+  return true;
+}
+
 // A CTA of TH threads writes one block of one head, keys or values; its values stay in registers between the maximum and the codes (R eights a thread).
-template <typename T, int TH, int R, bool WIDE>
-__global__ void __launch_bounds__(TH) write_rows(const Cache C, const Rows S, const T* k, const T* v, const Pitch pk, const Pitch pv) {
+template <typename T, int TH, int R, bool WIDE, typename Where>
+__global__ void __launch_bounds__(TH) write_rows(const Cache C, const Where S, const T* k, const T* v, const Pitch pk, const Pitch pv) {
   __shared__ uint32_t most[TH / 32];
   const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
   Piece p;

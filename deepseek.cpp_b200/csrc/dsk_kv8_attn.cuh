@@ -22,6 +22,7 @@
 #include <cooperative_groups.h>
 
 #include "dsk_kv8.cuh"
+#include "dsk_tmem.cuh"
 
 namespace dsk {
 namespace kv8 {
@@ -100,16 +101,6 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {     // an 8 x 8 matrix 
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ float exp2_fast(float x) {        // 2 ulp, results below 2^-126 are zero
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t halves(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t lower_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {   // 0xff where a byte is NaN
   return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
 }

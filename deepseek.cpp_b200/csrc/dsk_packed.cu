@@ -1,0 +1,186 @@
+// dsk_packed.cu — C-ABI (include/dsk.h) of the operators on packed rows, several sequences one behind the other: places in a cache for tokens that join (and blocks that come
+// back), packed rows into the 8-bit cache, attention of whole prompts.  As in dsk_serve.cu nothing is allocated, waited for or kept.
+
+#include "dsk_serve_host.cuh"
+
+#include <algorithm>
+
+#include "dsk_blocks.cuh"
+#include "dsk_prompt.cuh"
+
+namespace {
+constexpr int kMaxRows = 1 << 20;
+
+int check_pool(const dsk_blocks* p, const int32_t* table, int64_t pitch, int table_blocks, int batch) {
+  if (!p) return fail(-1, "null blocks");
+  if (p->block != 16 && p->block != 32 && p->block != 64 && p->block != 128) return fail(-4, "blocks of %d tokens: 16, 32, 64 or 128 are supported", p->block);
+  if (p->n_blocks <= 0 || p->n_blocks > INT32_MAX / p->block) return fail(-4, "%d blocks of %d tokens: at least one, and less than 2^31 tokens", p->n_blocks, p->block);
+  if (batch < 0 || batch > blocks::kMaxBatch) return fail(-4, "%d sequences: at most %d a call", batch, blocks::kMaxBatch);
+  if (table_blocks < 0 || table_blocks > (1 << 30) / p->block) return fail(-4, "tables of %d blocks (2^30 tokens at most)", table_blocks);
+  if (batch > 1 && pitch < table_blocks) return fail(-4, "rows of %d blocks %lld apart: they must not overlap", table_blocks, (long long)pitch);
+  if (!p->free || !p->n_free) return fail(-1, "blocks: null memory");
+  if (!aligned(p->free, 4) || !aligned(p->n_free, 4) || !aligned(p->status, 4)) return fail(-1, "blocks: memory needs 4-byte alignment");
+  if (batch && (!table || !aligned(table, 4) || !table_blocks)) return fail(-1, "null, empty or unaligned table");
+  return 0;
+}
+blocks::Pool pool_of(const dsk_blocks* p) { return blocks::Pool{p->free, p->n_free, p->status, p->n_blocks, p->block == 16 ? 4 : p->block == 32 ? 5 : p->block == 64 ? 6 : 7}; }
+int check_packed(const dsk_packed* s) {
+  if (!s) return fail(-1, "null packed rows");
+  if (s->batch < 0 || s->batch > prompt::kMaxBatch || s->rows < 0 || s->rows > kMaxRows) return fail(-4, "%d sequences (at most %d a call) in %d packed rows (at most 2^20)", s->batch, prompt::kMaxBatch, s->rows);
+  if (!s->starts || !aligned(s->starts, 4) || !aligned(s->status, 4)) return fail(-1, "packed rows: starts are null or unaligned");
+  return 0;
+}
+int check_pieces(const dsk_packed* s, int block) {
+  const int most = std::min(s->rows, s->rows / block + 2 * s->batch);
+  if (s->n_pieces < most) return fail(-4, "room for %d pieces where %d rows of %d sequences may have %d", s->n_pieces, s->rows, s->batch, most);
+  if (s->n_pieces && (!s->pieces || !aligned(s->pieces, 16))) return fail(-1, "packed rows: pieces are null or not 16-byte aligned");
+  return 0;
+}
+}  // namespace
+
+extern "C" int dsk_blocks_extend(const dsk_blocks* p, int32_t* table, int64_t table_pitch, int table_blocks, const int32_t* lens, const int32_t* count, const dsk_packed* s, void* stream) {
+  if (const int code = check_packed(s)) return code;
+  if (const int code = check_pool(p, table, table_pitch, table_blocks, s->batch)) return code;
+  if (s->block != p->block) return fail(-4, "packed rows for blocks of %d tokens, blocks of %d", s->block, p->block);
+  if (const int code = check_pieces(s, p->block)) return code;
+  if (s->batch && (!lens || !count || !s->lens || !aligned(lens, 4) || !aligned(count, 4) || !aligned(s->lens, 4))) return fail(-1, "dsk_blocks_extend: lengths or counts are null or unaligned");
+  if (s->batch && s->lens < lens + s->batch && lens < s->lens + s->batch) return fail(-1, "dsk_blocks_extend: the new lengths must not lie over the old ones");
+  if (s->batch && s->lens < count + s->batch && count < s->lens + s->batch) return fail(-1, "dsk_blocks_extend: the new lengths must not lie over the counts");
+  if (s->rows && (!s->positions || !s->slots || !aligned(s->positions, 4) || !aligned(s->slots, 4))) return fail(-1, "dsk_blocks_extend: positions or slots are null or unaligned");
+  if (const int code = check_device(p->device)) return code;
+  if (s->device != p->device) return fail(-1, "packed rows on device %d, blocks on %d", s->device, p->device);
+  OnDevice on(p->device);
+  CK(on.error);
+  blocks::Extend A;
+  A.P = pool_of(p);
+  A.table = table; A.pitch = table_pitch; A.lens = lens; A.count = count;
+  A.starts = s->starts; A.lens_out = s->lens; A.positions = s->positions; A.slots = s->slots; A.pieces = reinterpret_cast<int4*>(s->pieces);
+  A.table_blocks = table_blocks; A.batch = s->batch; A.rows = s->rows; A.n_pieces = s->n_pieces;
+  const int ctas = std::max(1, std::min(148, (s->rows + 4 * blocks::kThreads - 1) / (4 * blocks::kThreads)));
+  blocks::extend<<<ctas, blocks::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(A);
+  CK(cudaGetLastError());
+  return 0;
+}
+
+extern "C" int dsk_blocks_cut(const dsk_blocks* p, int32_t* table, int64_t table_pitch, int table_blocks, const int32_t* lens, const int32_t* keep, int batch, void* stream) {
+  if (const int code = check_pool(p, table, table_pitch, table_blocks, batch)) return code;
+  if (!batch) return 0;
+  if (!lens || !keep || !aligned(lens, 4) || !aligned(keep, 4)) return fail(-1, "dsk_blocks_cut: lengths are null or unaligned");
+  if (const int code = check_device(p->device)) return code;
+  OnDevice on(p->device);
+  CK(on.error);
+  blocks::cut<<<1, blocks::kCutThreads, 0, static_cast<cudaStream_t>(stream)>>>(blocks::Cut{pool_of(p), table, table_pitch, lens, keep, table_blocks, batch});
+  CK(cudaGetLastError());
+  return 0;
+}
+
+extern "C" int dsk_kv8_append(const dsk_kv8* c, const dsk_packed* s, const dsk_view* k, const dsk_view* v, void* stream) {
+  if (const int code = check_cache(c)) return code;
+  if (const int code = check_packed(s)) return code;
+  if (s->block != c->block) return fail(-4, "packed rows for blocks of %d tokens, a cache of %d", s->block, c->block);
+  if (const int code = check_pieces(s, c->block)) return code;
+  const int dt = k ? k->dtype : -1;
+  if (dt != DSK_DT_F32 && dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_kv8_append: keys and values are F32, F16 or BF16");
+  if (!s->batch || !s->rows) return 0;
+  if (const int code = check_view("keys", k, dt)) return code;
+  if (const int code = check_view("values", v, dt)) return code;
+  if (const int code = check_device(c->device)) return code;
+  if (s->device != c->device) return fail(-1, "packed rows on device %d, a cache on %d", s->device, c->device);
+  OnDevice on(c->device);
+  CK(on.error);
+  return write_all(c, kv8::Pieces{reinterpret_cast<const int4*>(s->pieces), s->rows}, dim3(s->n_pieces, 2 * c->kv_heads), std::min(s->rows, c->block), k, v, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) { cudaGetLastError(); p = nullptr; }
+    return (EncodeTiledFn)p;
+  }();
+  return fn;
+}
+// [row][head][entry] of 16-bit entries, copied in boxes of 64 entries of box_heads heads of box_rows rows (what lies outside reads as zeros)
+int rows_map(CUtensorMap* m, const char* what, const dsk_view* v, int dim, int heads, int rows, int box_heads, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? v->head * 2 : 16), (cuuint64_t)(rows > 1 ? v->row * 2 : 16)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows}, one[3] = {1, 1, 1};
+  const CUresult r = encode_tiled()(m, v->dtype == DSK_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, v->data, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : fail(-4, "%s: no tensor map for %d rows of %d heads of %d entries, rows %lld and heads %lld entries apart (error %d)", what, rows, heads, dim, (long long)v->row, (long long)v->head, (int)r);
+}
+// rows that tensor-map copies can read: 16-byte pieces
+int check_rows(const char* what, const dsk_view* v, int heads, int rows) {
+  if (!aligned(v->data, 16)) return fail(-4, "%s: memory needs 16-byte alignment", what);
+  for (const auto& d : {std::pair<int, int64_t>{heads, v->head}, {rows, v->row}})
+    if (d.first > 1 && (d.second <= 0 || d.second % 8 || d.second >= (1ll << 39))) return fail(-4, "%s: rows and heads must lie a positive multiple of 8 entries apart, got %lld and %lld", what, (long long)v->row, (long long)v->head);
+  return 0;
+}
+template <int DK, int DV, bool BF16> int attend_as(const prompt::Params& P, int ctas, int device, cudaStream_t stream) {
+  CK((allow<prompt::attend_packed<DK, DV, BF16>>(device, prompt::smem_bytes<DK, DV>())));
+  prompt::attend_packed<DK, DV, BF16><<<ctas, prompt::kThreads, prompt::smem_bytes<DK, DV>(), stream>>>(P);
+  CK(cudaGetLastError());
+  return 0;
+}
+template <int DK, int DV> int attend_as(const prompt::Params& P, bool bf16, int ctas, int device, cudaStream_t stream) {
+  return bf16 ? attend_as<DK, DV, true>(P, ctas, device, stream) : attend_as<DK, DV, false>(P, ctas, device, stream);
+}
+}  // namespace
+
+extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk_view* k, const dsk_view* v, const dsk_view* out, int heads, int kv_heads, int dim_k, int dim_v, float scale,
+                               int window, int keep_first, void* stream) {
+  if (const int code = check_packed(s)) return code;
+  const int dt = q ? q->dtype : -1;
+  if (dt != DSK_DT_F16 && dt != DSK_DT_BF16) return fail(-4, "dsk_packed_attn: queries, keys and values are F16 or BF16");
+  for (int d : {dim_k, dim_v})
+    if (d <= 0 || d % 16 || d > 256) return fail(-4, "heads of %d entries: a multiple of 16 up to 256 is needed", d);
+  if (kv_heads <= 0 || heads <= 0 || heads > 32767 || heads % kv_heads) return fail(-4, "%d query heads over %d key heads: a multiple is needed, at most 32767", heads, kv_heads);
+  if (!(scale >= 0.f && scale < INFINITY)) return fail(-4, "dsk_packed_attn: the scale must be a number that is not negative");
+  if (window < 0 || keep_first < 0) return fail(-4, "window %d and keep_first %d must not be negative", window, keep_first);
+  if (!s->batch || !s->rows) return 0;
+  for (const auto& x : {std::pair<const char*, const dsk_view*>{"queries", q}, {"keys", k}, {"values", v}, {"output", out}})
+    if (const int code = check_view(x.first, x.second, dt)) return code;
+  if (const int code = check_rows("queries", q, heads, s->rows)) return code;
+  if (const int code = check_rows("keys", k, kv_heads, s->rows)) return code;
+  if (const int code = check_rows("values", v, kv_heads, s->rows)) return code;
+  if (const int code = check_device(s->device)) return code;
+  if (!encode_tiled()) return fail(-2, "the driver has no cuTensorMapEncodeTiled");
+  OnDevice on(s->device);
+  CK(on.error);
+  const int sms = multiprocessors(s->device);
+  if (!sms) return fail(-2, "device %d: no attributes", s->device);
+  prompt::Params P;
+  P.group = heads / kv_heads;
+  // heads of a row tile: a divisor of the group that fills most of its 128 rows, the largest of those (its tokens are then few, and their keys end close together)
+  P.pack = 1;
+  for (int n = 2; n <= std::min(P.group, 128); n++)
+    if (P.group % n == 0 && 128 / n * n >= 128 / P.pack * P.pack) P.pack = n;
+  P.tokens = 128 / P.pack; P.subs = P.group / P.pack; P.units = kv_heads * P.subs;
+  constexpr int kShapes[4][2] = {{64, 64}, {128, 128}, {192, 128}, {256, 256}};
+  int shape = 0;
+  while (dim_k > kShapes[shape][0] || dim_v > kShapes[shape][1]) shape++;
+  if (const int code = rows_map(&P.q, "queries", q, dim_k, heads, s->rows, P.pack, P.tokens)) return code;
+  if (const int code = rows_map(&P.k, "keys", k, dim_k, kv_heads, s->rows, 1, prompt::kTile)) return code;
+  if (const int code = rows_map(&P.v, "values", v, dim_v, kv_heads, s->rows, 1, prompt::kUnit / 2 / kShapes[shape][1])) return code;
+  P.starts = s->starts; P.status = s->status;
+  P.values = v->data; P.v_row = v->row; P.v_head = v->head;
+  P.out = out->data; P.o_row = out->row; P.o_head = out->head;
+  P.wide_o = aligned(out->data, 16) && out->row % 8 == 0 && out->head % 8 == 0;
+  P.rows = s->rows; P.batch = s->batch; P.dk = dim_k; P.dv = dim_v;
+  P.window = window >= s->rows ? 0 : window; P.keep = keep_first;
+  P.f = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);            // (positive: -inf stays what it is)
+  const int tokens = P.tokens * (shape == 3 ? 1 : 2);
+  const long long items = ((long long)s->rows / tokens + std::min(s->batch, s->rows)) * P.units;   // at most, whatever the lengths
+  const int ctas = (int)std::min<long long>(sms, items);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool bf16 = dt == DSK_DT_BF16;
+  switch (shape) {
+    case 0: return attend_as<64, 64>(P, bf16, ctas, s->device, st);
+    case 1: return attend_as<128, 128>(P, bf16, ctas, s->device, st);
+    case 2: return attend_as<192, 128>(P, bf16, ctas, s->device, st);
+    default: return attend_as<256, 256>(P, bf16, ctas, s->device, st);
+  }
+}

@@ -141,6 +141,16 @@ class View(C.Structure):
     _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("batch", C.c_int64), ("row", C.c_int64), ("head", C.c_int64)]
 
 
+class BlocksArgs(C.Structure):
+    """dsk_blocks (include/dsk.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("free", "n_free", "status")] + [(n, C.c_int) for n in ("device", "n_blocks", "block")]
+
+
+class PackedArgs(C.Structure):
+    """dsk_packed (include/dsk.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("starts", "lens", "positions", "slots", "pieces", "status")] + [(n, C.c_int) for n in ("rows", "batch", "n_pieces", "block", "device")]
+
+
 class VerifyArgs(C.Structure):
     """dsk_verify_args (include/dsk.h)."""
     _fields_ = [(n, C.c_void_p) for n in ("logits", "draft_probs", "draft_tokens", "count", "coins", "accepted", "tokens")] + \
@@ -570,6 +580,10 @@ def lib():
         L.dsk_kv8_attn.argtypes = [C.POINTER(Kv8), C.POINTER(Kv8Rows), C.POINTER(View), C.POINTER(View), C.c_int, C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
         L.dsk_verify_workspace.argtypes = [C.POINTER(VerifyArgs), C.POINTER(C.c_size_t)]
         L.dsk_verify.argtypes = [C.POINTER(VerifyArgs), C.c_void_p, C.c_size_t, C.c_void_p]
+        L.dsk_blocks_extend.argtypes = [C.POINTER(BlocksArgs), C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.POINTER(PackedArgs), C.c_void_p]
+        L.dsk_blocks_cut.argtypes = [C.POINTER(BlocksArgs), C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
+        L.dsk_kv8_append.argtypes = [C.POINTER(Kv8), C.POINTER(PackedArgs), C.POINTER(View), C.POINTER(View), C.c_void_p]
+        L.dsk_packed_attn.argtypes = [C.POINTER(PackedArgs)] + [C.POINTER(View)] * 4 + [C.c_int] * 4 + [C.c_float, C.c_int, C.c_int, C.c_void_p]
         L.dsk_attn.argtypes = [f32p, u16p, u16p, C.c_int, C.c_int, C.c_int, C.c_int, f32p]
         _lib = L
     return _lib
@@ -898,7 +912,7 @@ class Model:
 # ---- operators on device memory: torch tensors of one GPU, work on torch's current stream of that GPU ------------------------------
 
 # Arguments travel as packed structures (the classes above, laid out by struct): a call takes a few microseconds on the host, of which ctypes structures would be half.
-_ROWS, _VIEW, _VERIFY = struct.Struct("@PPPqiii4x"), struct.Struct("@Pi4xqqq"), struct.Struct("@PPPPPPPqqqqiiiiif")
+_ROWS, _VIEW, _VERIFY, _PACKED = struct.Struct("@PPPqiii4x"), struct.Struct("@Pi4xqqq"), struct.Struct("@PPPPPPPqqqqiiiiif"), struct.Struct("@PPPPPPiiiii4x")
 _raw = {}
 
 
@@ -911,6 +925,9 @@ def _fast(name):
         f.argtypes = {"dsk_kv8_write": [P, C.c_char_p, C.c_char_p, C.c_char_p, P], "dsk_kv8_read": [P, C.c_char_p, C.c_char_p, C.c_char_p, P],
                       "dsk_kv8_attn_workspace": [P, C.c_char_p, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)],
                       "dsk_kv8_attn": [P, C.c_char_p, C.c_char_p, C.c_char_p, C.c_int, C.c_float, C.c_int, C.c_int, P, C.c_size_t, P],
+                      "dsk_blocks_extend": [P, P, C.c_int64, C.c_int, P, P, C.c_char_p, P], "dsk_blocks_cut": [P, P, C.c_int64, C.c_int, P, P, C.c_int, P],
+                      "dsk_kv8_append": [P, C.c_char_p, C.c_char_p, C.c_char_p, P],
+                      "dsk_packed_attn": [C.c_char_p] * 5 + [C.c_int] * 4 + [C.c_float, C.c_int, C.c_int, P],
                       "dsk_verify_workspace": [C.c_char_p, C.POINTER(C.c_size_t)], "dsk_verify": [C.c_char_p, P, C.c_size_t, P]}[name]
         _raw[name] = f
     return f
@@ -931,6 +948,35 @@ def _dense(what, t, dtype, shape, device):
             _no_device(t)
         raise DskError(f"{what}: a contiguous {dtype} tensor {tuple(shape)} on cuda:{device} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
+
+
+def _table(torch, table, device):
+    """A table of block numbers: int32 [batch, blocks] on the device, entries of a row side by side."""
+    if table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != device or table.stride(1) != 1 and table.shape[1] > 1 and table.shape[0] > 0:
+        if table.get_device() < 0:
+            _no_device(table)
+        raise DskError(f"table: int32 [batch, blocks] on cuda:{device} with rows of neighbours is needed, got {table.dtype} {tuple(table.shape)} on {table.device}")
+    return table
+
+
+def _no_overlap(what, t):
+    if not t.is_contiguous():
+        extent = t.shape[-1]
+        for step, n in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+            if step < extent:
+                raise DskError(f"{what}: rows of the result must not overlap")
+            extent += step * (n - 1)
+
+
+def _status(torch, status, device, what):
+    """Waits for the GPU, all of its streams, and raises if a call has noted something; the status is cleared."""
+    torch.cuda.synchronize(device)
+    bits = int(status.item())
+    if bits:
+        status.zero_()
+        torch.cuda.synchronize(device)                         # (a call behind this one may be on another stream)
+        texts = (1, "a block number outside the cache"), (2, "tokens outside the table"), (4, "a wait inside a kernel gave up"), (8, "blocks or packed rows ran out"), (16, "more blocks came back than there are")
+        raise DskError(f"{what}: " + ", ".join(t for b, t in texts if bits & b))
 
 
 class Cache8:
@@ -976,10 +1022,7 @@ class Cache8:
         self._needs = {}            # bytes of attention's workspace by shape of the call
 
     def _rows(self, table, first, count, rows):
-        if table.dim() != 2 or table.dtype is not self._i32 or table.get_device() != self.device or table.stride(1) != 1 and table.shape[1] > 1:
-            if table.get_device() < 0:
-                _no_device(table)
-            raise DskError(f"table: int32 [batch, blocks] on cuda:{self.device} with rows of neighbours is needed, got {table.dtype} {tuple(table.shape)} on {table.device}")
+        _table(self._torch, table, self.device)
         batch, blocks = table.shape
         return _ROWS.pack(table.data_ptr(), _dense("first tokens / lengths", first, self._i32, (batch,), self.device),
                           0 if count is None else _dense("count", count, self._i32, (batch,), self.device), table.stride(0), blocks, batch, rows)
@@ -990,12 +1033,8 @@ class Cache8:
             if t.get_device() < 0:
                 _no_device(t)
             raise DskError(f"{what}: float32, float16 or bfloat16 {tuple(shape)} on cuda:{self.device} with neighbouring entries is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if written and not t.is_contiguous():
-            extent = t.shape[3]
-            for step, n in sorted((s[i], t.shape[i]) for i in range(3) if t.shape[i] > 1):
-                if step < extent:
-                    raise DskError(f"{what}: rows of the result must not overlap")
-                extent += step * (n - 1)
+        if written:
+            _no_overlap(what, t)
         return _VIEW.pack(t.data_ptr(), self._types[t.dtype], s[0], s[1], s[2])
 
     def write(self, k, v, table, first, count=None):
@@ -1007,6 +1046,14 @@ class Cache8:
             raise DskError(f"keys of {batch} sequences and {k.dtype}, values of {v.dtype}, a table of {table.shape[0]} sequences")
         _ck(_fast("dsk_kv8_write")(self._at, self._rows(table, first, count, rows), self._view("keys", k, (batch, rows, self.kv_heads, self.dim_k)),
                                    self._view("values", v, (batch, rows, self.kv_heads, self.dim_v)), _stream_of(self._torch, self.device)))
+
+    def append(self, k, v, packed):
+        """Packed rows k, v [rows, kv_heads, dim] to the places that `Blocks.extend` gave them (dsk_kv8_append)."""
+        if packed._pieces is None or packed.block != self.block:
+            raise DskError(f"packed rows with places in blocks of {self.block} tokens are needed (Blocks.extend)")
+        if k.dtype is not v.dtype:
+            raise DskError(f"keys of {k.dtype}, values of {v.dtype}")
+        _ck(_fast("dsk_kv8_append")(self._at, packed._c, packed._view("keys", k, self.kv_heads, self.dim_k), packed._view("values", v, self.kv_heads, self.dim_v), _stream_of(self._torch, self.device)))
 
     def read(self, table, first, rows: int, count=None, dtype=None, out=None):
         """The values of tokens first[b] .. first[b] + rows - 1 (dsk_kv8_read): (keys, values) [batch, rows, kv_heads, dim], `out` or new ones (zeros in rows from count[b] on)."""
@@ -1051,12 +1098,138 @@ class Cache8:
 
     def check(self):
         """Waits for the GPU, all of its streams, and raises if a call met a block number outside the cache, tokens outside a table or a wait that gave up; the status is cleared."""
-        self._torch.cuda.synchronize(self.device)
-        bits = int(self.status.item())
-        if bits:
-            self.status.zero_()
-            self._torch.cuda.synchronize(self.device)          # (a call behind this one may be on another stream)
-            raise DskError("8-bit cache: " + ", ".join(t for b, t in ((1, "a block number outside the cache"), (2, "tokens outside the table"), (4, "a wait inside a kernel gave up")) if bits & b))
+        _status(self._torch, self.status, self.device, "8-bit cache")
+
+
+class Packed:
+    """Packed rows (dsk_packed, include/dsk.h): the rows of several sequences one behind the other, `rows` of them, sequence b's from starts[b] on (int32 [batch + 1], on the GPU).  Rows from
+    starts[batch] on belong to no one.  `Blocks.extend` makes them, with lens [batch], positions [rows] and slots [rows] (-1 behind the last row); `of` takes starts alone, which is all that
+    `attend` needs."""
+
+    def __init__(self):
+        raise DskError("packed rows come from Blocks.extend or Packed.of")
+
+    @classmethod
+    def of(cls, starts, rows: int) -> "Packed":
+        """Packed rows of sequences that begin at starts[:-1]; they have no places in a cache."""
+        import torch
+        if starts.dim() != 1 or starts.shape[0] < 1:
+            raise DskError(f"starts: int32 [batch + 1] is needed, got {tuple(starts.shape)}")
+        p = cls.__new__(cls)
+        device = starts.get_device()
+        if device < 0:
+            _no_device(starts)
+        at = _dense("starts", starts, torch.int32, starts.shape, device)
+        p._torch, p.device, p.rows, p.batch, p.block = torch, device, rows, starts.shape[0] - 1, 0
+        p.starts, p.lens, p.positions, p.slots, p._pieces = starts, None, None, None, None
+        p.status = torch.zeros(1, dtype=torch.int32, device=starts.device)
+        p._c = _PACKED.pack(at, 0, 0, 0, 0, p.status.data_ptr(), rows, p.batch, 0, 0, device)
+        return p
+
+    @classmethod
+    def _room(cls, blocks, batch: int, rows: int) -> "Packed":
+        torch, p = blocks._torch, cls.__new__(cls)
+        n = min(rows, rows // blocks.block + 2 * batch)
+        up = lambda k: (k + 3) // 4 * 4                        # (16-byte aligned parts of one allocation)
+        sizes = up(4 * n), up(rows), up(rows), up(batch + 1), batch
+        p._pieces, positions, slots, starts, lens = torch.empty(sum(sizes), dtype=torch.int32, device=blocks.free.device).split(sizes)
+        p._torch, p.device, p.rows, p.batch, p.block, p.status = torch, blocks.device, rows, batch, blocks.block, blocks.status
+        p.positions, p.slots, p.starts, p.lens = positions[:rows], slots[:rows], starts[:batch + 1], lens
+        p._c = _PACKED.pack(starts.data_ptr(), lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), p._pieces.data_ptr(), p.status.data_ptr(), rows, batch, n, p.block, p.device)
+        return p
+
+    def _view(self, what, t, heads, dim, written=False):
+        kind = {self._torch.float32: 0, self._torch.float16: 1, self._torch.bfloat16: 2}.get(t.dtype)
+        s = t.stride()
+        if t.shape != (self.rows, heads, dim) or kind is None or t.get_device() != self.device or s[2] != 1:
+            if t.get_device() < 0:
+                _no_device(t)
+            raise DskError(f"{what}: float32, float16 or bfloat16 {(self.rows, heads, dim)} on cuda:{self.device} with neighbouring entries is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if written:
+            _no_overlap(what, t)
+        return _VIEW.pack(t.data_ptr(), kind, 0, s[0], s[1])
+
+    def attend(self, q, k, v, scale: Optional[float] = None, window: int = 0, keep_first: int = 0, out=None):
+        """Causal attention of every sequence's tokens over themselves (dsk_packed_attn): q [rows, heads, dim_k], k [rows, kv_heads, dim_k], v [rows, kv_heads, dim_v], all float16 or all bfloat16;
+        scale: dim_k ** -0.5 unless given.  Returns [rows, heads, dim_v], `out` or a new tensor (zeros in rows of no one)."""
+        torch = self._torch
+        if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+            raise DskError("queries, keys and values are [rows, heads, dim]")
+        if k.dtype is not q.dtype or v.dtype is not q.dtype:
+            raise DskError(f"keys of {k.dtype} and values of {v.dtype} for queries of {q.dtype}")
+        heads, dim_k, kv_heads, dim_v = q.shape[1], q.shape[2], k.shape[1], v.shape[2]
+        if out is None:
+            out = torch.zeros((self.rows, heads, dim_v), dtype=q.dtype, device=q.device)
+        elif out.dtype is not q.dtype:
+            raise DskError(f"results of {out.dtype} for queries of {q.dtype}")
+        window, keep_first = max(-1, min(window, 0x7fffffff)), max(-1, min(keep_first, 0x7fffffff))   # (what an int has; negative ones are refused)
+        _ck(_fast("dsk_packed_attn")(self._c, self._view("queries", q, heads, dim_k), self._view("keys", k, kv_heads, dim_k), self._view("values", v, kv_heads, dim_v),
+                                     self._view("output", out, heads, dim_v, True), heads, kv_heads, dim_k, dim_v, dim_k ** -0.5 if scale is None else scale, window, keep_first,
+                                     _stream_of(torch, self.device)))
+        return out
+
+    def check(self):
+        """Waits for the GPU, all of its streams, and raises if a call gave up a wait (or whatever `Blocks.check` would, where the rows are from there); the status is cleared."""
+        _status(self._torch, self.status, self.device, "packed rows")
+
+
+class Blocks:
+    """The free blocks of a cache (dsk_blocks, include/dsk.h), a stack on the GPU: `extend` gives places to tokens that join sequences, `cut` takes blocks back.  A sequence is a row of a table of
+    block numbers (int32 [batch, blocks]) as `Cache8` reads it; lens, count and keep are int32 [batch] tensors on the GPU, so that a captured graph serves other lengths.  No call waits for the
+    GPU: what only the GPU sees (blocks that ran out, tokens outside a table) shows in `check`.  Calls that share blocks or a table must not run at the same time."""
+
+    def __init__(self, n_blocks: int, block: int = 64, device=None):
+        import torch
+        dev = torch.device("cuda", torch.cuda.current_device() if device is None else device) if device is None or isinstance(device, int) else torch.device(device)
+        self._bind(torch.arange(n_blocks - 1, -1, -1, dtype=torch.int32, device=dev), n_blocks, block)    # (the lowest numbers are taken first)
+
+    @classmethod
+    def of(cls, free, n_blocks: int, block: int = 64) -> "Blocks":
+        """Blocks of a cache of which those in `free` (int32 [n], a copy is kept) are free; the last one is taken first."""
+        b = cls.__new__(cls)
+        b._bind(free, n_blocks, block)
+        return b
+
+    def _bind(self, free, n_blocks, block):
+        import torch
+        self._torch, self.device, self.n_blocks, self.block = torch, free.get_device(), n_blocks, block
+        if self.device < 0:
+            _no_device(free)
+        if free.dim() != 1 or free.dtype is not torch.int32 or free.shape[0] > n_blocks:
+            raise DskError(f"free blocks: int32 [at most {n_blocks}] is needed, got {free.dtype} {tuple(free.shape)}")
+        self.free = torch.zeros(n_blocks, dtype=torch.int32, device=free.device)
+        self.free[:free.shape[0]] = free
+        self._top = torch.tensor([free.shape[0], 0], dtype=torch.int32).to(free.device)
+        self.n_free = self._top[:1]
+        self.status = torch.zeros(1, dtype=torch.int32, device=free.device)
+        self._c = BlocksArgs(self.free.data_ptr(), self._top.data_ptr(), self.status.data_ptr(), self.device, n_blocks, block)
+        self._at = C.addressof(self._c)
+
+    def extend(self, table, lens, count, rows: int, out: Optional[Packed] = None) -> Packed:
+        """Places for count[b] more tokens of sequences that have lens[b] (dsk_blocks_extend): writes new blocks into `table`, returns `out` (of an earlier call with as many sequences and rows) or new
+        packed rows, with room for `rows` tokens of all sequences.  Sequences that no longer fit, and those behind them, get nothing."""
+        batch, blocks = _table(self._torch, table, self.device).shape
+        i32 = self._torch.int32
+        if rows < 0:
+            raise DskError(f"{rows} packed rows")
+        if out is None:
+            out = Packed._room(self, batch, rows)
+        elif out.batch != batch or out.rows != rows or out._pieces is None or out.block != self.block:
+            raise DskError(f"packed rows of {batch} sequences, {rows} rows and blocks of {self.block} tokens from an earlier call are needed")
+        _ck(_fast("dsk_blocks_extend")(self._at, table.data_ptr(), table.stride(0), blocks, _dense("lens", lens, i32, (batch,), self.device), _dense("count", count, i32, (batch,), self.device), out._c,
+                                       _stream_of(self._torch, self.device)))
+        return out
+
+    def cut(self, table, lens, keep):
+        """Sequences of lens[b] tokens give back the blocks behind their first keep[b] (dsk_blocks_cut); their entries in `table` become -1."""
+        batch, blocks = _table(self._torch, table, self.device).shape
+        i32 = self._torch.int32
+        _ck(_fast("dsk_blocks_cut")(self._at, table.data_ptr(), table.stride(0), blocks, _dense("lens", lens, i32, (batch,), self.device), _dense("keep", keep, i32, (batch,), self.device), batch,
+                                    _stream_of(self._torch, self.device)))
+
+    def check(self):
+        """Waits for the GPU, all of its streams, and raises if a call met a number that is no block, tokens outside a table, or too few or too many blocks; the status is cleared."""
+        _status(self._torch, self.status, self.device, "blocks")
 
 
 _verify_needs = {}                   # bytes of the workspace by shape of the call

@@ -384,6 +384,41 @@ int dsk_kv8_read(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view*
 int dsk_kv8_attn_workspace(const dsk_kv8* cache, const dsk_kv8_rows* rows, int heads, int window, int keep_first, size_t* bytes);   /* 0: none */
 int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* q, const dsk_view* out, int heads, float scale, int window, int keep_first,
                  void* workspace, size_t workspace_bytes, void* stream);
+/* Packed rows: the rows of several sequences one behind the other, sequence b's from starts[b] on (starts[batch]: behind the last one; rows from there on belong to no one and are neither read nor
+ * written).  At most 1024 sequences and 2^20 rows a call.  A starts that falls, or points outside the rows, is taken as the nearest one that does not.
+ * Blocks of a cache that are free are a stack, free[0 .. n_free[0] - 1]; n_free[1] is a word of the kernels, 0 between calls.  A sequence of len tokens holds the first ceil(len / block) entries of its row
+ * of the table.  Calls over the same blocks, or the same table, must not run at the same time. */
+enum { DSK_BLOCKS_SHORT = 8,  /* status: sequences got no places, for want of blocks or packed rows */
+       DSK_BLOCKS_TWICE = 16  /* status: more blocks came back than there are (those beyond are lost) */ };
+typedef struct dsk_blocks {
+  int32_t *free, *n_free;          /* [n_blocks]; [2] */
+  int32_t* status;                 /* nullable; bits are added, never cleared: DSK_KV8_PAGE, DSK_KV8_RANGE, DSK_BLOCKS_* */
+  int device, n_blocks, block;     /* n_blocks x block less than 2^31 */
+} dsk_blocks;
+typedef struct dsk_packed {
+  int32_t* starts;                 /* [batch + 1] */
+  int32_t* lens;                   /* [batch]: tokens of every sequence, its new ones among them */
+  int32_t *positions, *slots;      /* [rows]: a row's place in its sequence and in the cache, block number x block + place in the block; -1: none */
+  int32_t* pieces;                 /* [n_pieces][4], 16-byte aligned: what the rows have in each block (first row, rows, block number, place in it); rows 0: none */
+  int32_t* status;                 /* nullable: DSK_KV8_WAIT */
+  int rows, batch, n_pieces, block, device;   /* n_pieces: at least min(rows, rows / block + 2 batch) */
+} dsk_packed;
+/* Places for count[b] tokens that join sequences of lens[b]: new blocks come off the end of the stack, sequence by sequence, and into the table; starts, lens (not the caller's lens), positions, slots and pieces
+ * are written, those behind the last row as nothing.  A sequence whose blocks or rows no longer fit gets nothing, nor does any behind it (count 0, DSK_BLOCKS_SHORT); one with a negative length, or
+ * more tokens than its table has room for, gets nothing (DSK_KV8_RANGE); a negative count is 0.  Where an entry is no block number (DSK_KV8_PAGE), its tokens have the slot -1 and no piece. */
+int dsk_blocks_extend(const dsk_blocks* blocks, int32_t* table, int64_t table_pitch, int table_blocks, const int32_t* lens, const int32_t* count, const dsk_packed* rows, void* stream);
+/* Sequences of lens[b] tokens give back what lies behind their first keep[b] (drafts that were refused; 0: all): entries ceil(keep / block) .. ceil(lens / block) - 1 go back onto the stack in the reverse of the
+ * order in which extend takes them, and become -1.  0 <= keep <= lens, otherwise the sequence is left alone (DSK_KV8_RANGE).  Entries that are no block numbers do not go back (DSK_KV8_PAGE).  A
+ * block that several sequences share goes back once for each: keep those out of it. */
+int dsk_blocks_cut(const dsk_blocks* blocks, int32_t* table, int64_t table_pitch, int table_blocks, const int32_t* lens, const int32_t* keep, int batch, void* stream);
+/* dsk_kv8_write of packed rows, at the places that dsk_blocks_extend gave them (views: batch unused). */
+int dsk_kv8_append(const dsk_kv8* cache, const dsk_packed* rows, const dsk_view* k, const dsk_view* v, void* stream);
+/* Causal softmax attention of whole prompts, from their packed rows alone (no cache): token i of a sequence sees its tokens j <= i, with window > 0 those with i - j < window or j < keep_first.  Query
+ * head h reads key head h / (heads / kv_heads).  q, k, v, out: F16 or BF16, all of one type (views: batch unused); q, k and v 16-byte aligned, their rows and heads a positive multiple of 8 entries apart;
+ * dim_k and dim_v multiples of 16 up to 256; scale >= 0.  Zeros for a query whose scores are all -inf; one that sees an infinite or NaN value has no finite result in that entry, others do not
+ * notice.  Results below 2^-80 (BF16) lose accuracy. */
+int dsk_packed_attn(const dsk_packed* rows, const dsk_view* q, const dsk_view* k, const dsk_view* v, const dsk_view* out, int heads, int kv_heads, int dim_k, int dim_v, float scale, int window,
+                    int keep_first, void* stream);
 /* Speculative sampling, beside dsk_sample: sequence b has count[b] drafted tokens x_i and the model's logits of count[b] + 1 rows.  p_i = softmax(logits_i / temperature); draft i is accepted
  * while coins[i] q_i(x_i) < p_i(x_i) (no draft_probs: q_i(x_i) = 1, the drafts are certain).  The first draft that is not is replaced by a draw from max(p_i - q_i, 0); behind
  * accepted ones the next token is drawn from p (temperature: 0, or at least 2^-120).  A draw is the lowest index whose running sum is over coins[drafts] x (whole sum), sums good to 2^-35 (of p's, which is 1).  temperature 0: a draft is accepted

@@ -120,6 +120,13 @@ int check_rows(const char* what, const dsk_view* v, int heads, int rows) {
   return 0;
 }
 template <int DK, int DV, bool BF16> int attend_as(const prompt::Params& P, int ctas, int device, cudaStream_t stream) {
+  static std::atomic<int> registers{0};                      // of a thread at launch: what its warps give and take adds up to that, or they wait for good
+  if (registers.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes at{};
+    CK((cudaFuncGetAttributes(&at, prompt::attend_packed<DK, DV, BF16>)));
+    registers.store(at.numRegs, std::memory_order_relaxed);
+  }
+  if (registers.load(std::memory_order_relaxed) != 65536 / prompt::kThreads) return fail(-2, "dsk_packed_attn: built with %d registers a thread where %d are needed", registers.load(), 65536 / prompt::kThreads);
   CK((allow<prompt::attend_packed<DK, DV, BF16>>(device, prompt::smem_bytes<DK, DV>())));
   prompt::attend_packed<DK, DV, BF16><<<ctas, prompt::kThreads, prompt::smem_bytes<DK, DV>(), stream>>>(P);
   CK(cudaGetLastError());

@@ -21,7 +21,7 @@
 namespace dsk {
 namespace prompt {
 
-constexpr int kThreads = 512, kTile = 128, kUnit = 16384, kMaxBatch = 1024, kHeld = 8;   // keys of a tile; bytes of a copied unit; sequences whose tiles a lane of the dealing warp keeps in registers
+constexpr int kThreads = 512, kTile = 128, kUnit = 16384, kMaxBatch = 1024, kHeld = 8, kAhead = 4;   // keys of a tile; bytes of a copied unit; sequences whose tiles a lane of the dealing warp keeps in registers; tiles of keys under way
 constexpr int ST_WAIT = 4;                                   // a wait that gave up
 constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
 constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
@@ -43,16 +43,16 @@ template <int DK, int DV> __host__ __device__ constexpr int k_units() { return D
 template <int DK, int DV> __host__ __device__ constexpr int v_units() { return DK == 192 ? 3 : DK == 64 ? 5 : 4; }
 template <int DK, int DV> __host__ __device__ constexpr int smem_bytes() { return 1024 + 128 * tiles<DK, DV>() * DK * 2 + (k_units<DK, DV>() + v_units<DK, DV>()) * kUnit; }
 
-__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* status) {
-  const long long from = clock64();
-  do {
-    if (hy::tc_poll(bar, parity)) return true;
-  } while (clock64() - from < hy::kTcWaitCycles);
-  if (status) atomicOr(status, ST_WAIT);
-  return false;
+// Bounded, in line: a call would cost what the wait itself does
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status) {
+  bool ok = hy::tc_poll(bar, parity);
+  if (!ok) {
+    const uint32_t from = clock();
+    do ok = hy::tc_poll(bar, parity); while (!ok && (uint32_t)clock() - from < 1u << 31);
+    if (!ok && status) atomicOr(status, ST_WAIT);
+  }
+  return __all_sync(0xffffffffu, ok);
 }
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, int* status) { return hy::tc_poll(bar, parity) || wait_long(bar, parity, status); }
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status) { return __all_sync(0xffffffffu, wait_bar(bar, parity, status)); }
 __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int entry, int head, int row, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(entry), "r"(head), "r"(row) : "memory");
@@ -110,20 +110,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   constexpr int TILES = tiles<DK, DV>(), KU = k_units<DK, DV>(), VU = v_units<DK, DV>(), VK = kUnit / (2 * DV), STEPS = VK / 16, SOFT = 4 * TILES, USERS = SOFT + 7;   // VK: keys of a unit of values
   constexpr float LEAD = BF16 ? 40.f : -7.f, ROOM = BF16 ? -26.f : 14.f;       // a reference is taken LEAD above its maximum, and follows once that is above m + ROOM
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t bars[54];
+  __shared__ __align__(8) uint64_t bars[50];
   __shared__ int4 items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int odd_values;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, qs = base, ks = qs + 128 * TILES * DK * 2, vs = ks + KU * kUnit, b0 = smem_u32(bars);
-  const uint32_t kfull = b0, kempty = b0 + 48, vfull = b0 + 96, vempty = b0 + 136, vok = b0 + 176, qfull = b0 + 216, qempty = b0 + 232, sfull = b0 + 248, pfull = b0 + 264, phalf = b0 + 296,
-                 pvdone = b0 + 312, odone = b0 + 328, ifull = b0 + 344, iempty = b0 + 360, flushed = b0 + 376, vraw = b0 + 392;   // (vraw: where values land that are looked at ahead of their products)
+  const uint32_t kfull = b0, kempty = b0 + 32, vfull = b0 + 64, vempty = b0 + 104, vok = b0 + 144, vraw = b0 + 184, qfull = b0 + 224, qempty = b0 + 240, sfull = b0 + 256, pfull = b0 + 272,
+                 pvdone = b0 + 304, odone = b0 + 320, ifull = b0 + 336, iempty = b0 + 352, flushed = b0 + 368, turns = b0 + 384;   // keys: a barrier for each of kAhead tiles; vraw: where values land that are looked at ahead of their products
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tokens = TILES * P.tokens;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 6; i++) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); }
+    for (int i = 0; i < kAhead; i++) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); }
     for (int i = 0; i < 5; i++) { mbar_init(vfull + 8 * i, 1); mbar_init(vempty + 8 * i, TILES); mbar_init(vok + 8 * i, 3); mbar_init(vraw + 8 * i, 1); }
     for (int i = 0; i < 2; i++) {
-      mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 16 * i, 4); mbar_init(pfull + 16 * i + 8, 4); mbar_init(phalf + 8 * i, 1);
-      mbar_init(pvdone + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); mbar_init(flushed + 8 * i, 1);
+      mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 16 * i, 4); mbar_init(pfull + 16 * i + 8, 4);
+      mbar_init(pvdone + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); mbar_init(flushed + 8 * i, 1); mbar_init(turns + 8 * i, 4);
     }
     odd_values = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -137,6 +137,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [2][128], results [tile][DV]
 
+  // 512 threads have 128 registers each; a softmax thread holds a row of scores, the others little
+  constexpr int MANY = 192, FEW = 64;
+
   uint32_t turn = 0;                                         // items that this warp has taken
   auto take = [&](Item& w) {                                 // the next item, in every lane
     const uint32_t slot = turn & 1;
@@ -149,48 +152,58 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     return ok && w.len > 0;
   };
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
   if (warp == 8 || warp == 9) {                              // products: of row tile warp - 8 (one row tile: scores, results)
     const int t = warp - 8;
     const uint32_t lead = hy::tc_elect();
     const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);         // fp32 sums of bf16 or fp16, 128 rows
-    const uint32_t sdesc = idesc | ((uint32_t)(kTile / 8) << 17), pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17);
+    const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17);
     const int chunks = (P.dk + 63) / 64, ksteps = P.dk / 16;
-    uint32_t kn = 0, kpar = 0, vn = 0, vpar[2] = {0, 0}, passed = 0, took = 0;   // places in the rings and their parities (values: a bit for each place, as they came and looked at), tiles passed, items that had rows
-    auto scores = [&](uint32_t to, const bool mine) {       // all chunks of the next tile of keys
+    uint32_t kt = 0, kn = 0, vn = 0, vpar[2] = {0, 0}, passed = 0, took = 0;   // tiles of keys behind, places in the rings, parities of values (a bit for each place: as they came, looked at), tiles of this row tile, items that had rows
+    int pend = -1;                                           // a unit of values whose product is issued and that is to be given back
+    auto keys_there = [&] { return wait_warp(kfull + 8 * (kt % kAhead), (kt / kAhead) & 1, P.status); };
+    auto scores = [&](uint32_t to, int n, uint32_t full) {   // of the next tile of keys, of which the rows see the first 16 n
       const uint64_t a = hy::tc_desc(qs + (TILES == 2 ? t * (kTile * DK * 2) : 0));
+      const uint32_t sdesc = idesc | (uint32_t)(2 * n) << 17;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int c = 0; c < DK / 64; c++) {
         if (c >= chunks) break;
-        if (!wait_warp(kfull + 8 * kn, kpar, P.status)) return false;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (mine) {
-          const uint64_t k = hy::tc_desc(ks + kn * kUnit);
+        const uint64_t k = hy::tc_desc(ks + (kn + c < KU ? kn + c : kn + c - KU) * kUnit);
 #pragma unroll
-          for (int u = 0; u < 4; u++) if (4 * c + u < ksteps) mma_ss(to, a + c * (kTile * 128 >> 4) + 2 * u, k + 2 * u, sdesc, c > 0 || u > 0, lead);
-          commit(kempty + 8 * kn, lead);
-        } else if (lead) hy::tc_arrive(kempty + 8 * kn);
-        if (++kn == KU) { kn = 0; kpar ^= 1; }
+        for (int u = 0; u < 4; u++) if (4 * c + u < ksteps) mma_ss(to, a + c * (kTile * 128 >> 4) + 2 * u, k + 2 * u, sdesc, c > 0 || u > 0, lead);
+      }
+      commit(full, lead);
+      commit(kempty + 8 * (kt % kAhead), lead);
+    };
+    auto next_keys = [&] {
+      kt++;
+      kn += chunks;
+      if (kn >= KU) kn -= KU;
+    };
+    auto values_there = [&](const bool masked) {
+      uint32_t at = vn;
+#pragma unroll
+      for (int u = 0; u < kTile / VK; u++) {
+        if (!wait_warp((masked ? vok : vfull) + 8 * at, (masked ? vpar[1] : vpar[0]) >> at & 1, P.status)) return false;
+        if (masked) vpar[1] ^= 1u << at; else vpar[0] ^= 1u << at;
+        if (++at == VU) at = 0;
       }
       return true;
     };
-    auto results = [&](uint32_t weights, uint32_t to, uint32_t full, uint32_t half, uint32_t parity, const bool mine, const bool masked, const bool add) {
+    auto results = [&](uint32_t weights, uint32_t to, uint32_t full, uint32_t parity, int n, const bool add, uint32_t done) {
 #pragma unroll
       for (int u = 0; u < kTile / 16; u++) {
-        if (u % STEPS == 0) {
-          if (!wait_warp(masked ? vok + 8 * vn : vfull + 8 * vn, (masked ? vpar[1] : vpar[0]) >> vn & 1, P.status)) return false;
-          if (masked) vpar[1] ^= 1u << vn; else vpar[0] ^= 1u << vn;
+        if (u % 4 == 0) {
+          if (!wait_warp(full + (u / 4) * 8, parity, P.status)) return false;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
-        if (mine) {
-          if (u % 4 == 0) {
-            if (u == 4) commit(half, lead);
-            if (!wait_warp(full + (u / 4) * 8, parity, P.status)) return false;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          }
-          mma_ts(to, weights + (u >> 2) * 64 + (u & 3) * 8, value_desc(vs + vn * kUnit, VK) + (u % STEPS) * 128, pdesc, add || u > 0, lead);
-        }
+        if (u < n) mma_ts(to, weights + u * 8, value_desc(vs + vn * kUnit, VK) + (u % STEPS) * 128, pdesc, add || u > 0, lead);
+        if (u == kTile / 16 - 1) commit(done, lead);
         if (u % STEPS == STEPS - 1) {
-          if (mine) commit(vempty + 8 * vn, lead);
-          else if (lead) hy::tc_arrive(vempty + 8 * vn);
+          if (TILES == 2 && u == kTile / 16 - 1) pend = vn;  // (given back behind the next scores, which wait for this product and not for that)
+          else commit(vempty + 8 * vn, lead);
           if (++vn == VU) vn = 0;
         }
       }
@@ -204,33 +217,50 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const bool there = a < w.len;
       bool any = false;
       if (TILES == 2) {
-        alive = !there || wait_warp(qfull + 8 * t, took & 1, P.status);
+        alive = (!there || wait_warp(qfull + 8 * t, took & 1, P.status)) && keys_there();
         for (int i = 0; i < k.n && alive; i++) {
-          const int key0 = key_of(k, i);
-          const bool mine = there && sees_some(P, a, b, key0);
-          if (mine && passed) alive = wait_warp(pvdone + 8 * t, (passed - 1) & 1, P.status);       // the weights are read: their columns may have the next scores
-          if (!alive || !scores(tmem + t * 128, mine)) { alive = false; break; }
-          if (mine) commit(sfull + 8 * t, lead);
-          if (there && i == k.n - 1) commit(qempty + 8 * t, lead);
-          if (!results(tmem + t * 128, o_at + t * 128, pfull + 16 * t, phalf + 8 * t, passed & 1, mine, !sees_all(P, w.tok, k.t1 - 1, key0), any)) { alive = false; break; }
-          if (mine) { commit(pvdone + 8 * t, lead); passed++; any = true; }
+          const int key0 = key_of(k, i), n = min(8, (b - key0 + 16) / 16);
+          const bool mine = there && sees_some(P, a, b, key0), masked = !sees_all(P, w.tok, k.t1 - 1, key0);
+          if (mine) {
+            if (passed) alive = wait_warp(pvdone + 8 * t, (passed - 1) & 1, P.status);   // the weights are read: their columns may have the next scores
+            if (!alive) break;
+            scores(tmem + t * 128, n, sfull + 8 * t);
+          } else if (lead) hy::tc_arrive(kempty + 8 * (kt % kAhead));
+          if (pend >= 0) { commit(vempty + 8 * pend, lead); pend = -1; }
+          next_keys();
+          if (i + 1 < k.n) alive = keys_there();
+          else if (there) commit(qempty + 8 * t, lead);
+          alive = alive && values_there(masked);
+          if (!alive) break;
+          if (mine) {
+            alive = results(tmem + t * 128, o_at + t * 128, pfull + 16 * t, passed & 1, n, any, pvdone + 8 * t);
+            passed++;
+            any = true;
+          } else {
+#pragma unroll
+            for (int u = 0; u < kTile / VK; u++) {
+              if (lead) hy::tc_arrive(vempty + 8 * vn);
+              if (++vn == VU) vn = 0;
+            }
+          }
         }
         if (there && alive) { commit(odone + 8 * t, lead); took++; }
+        if (pend >= 0) { commit(vempty + 8 * pend, lead); pend = -1; }
       } else if (t == 0) {                                   // scores lie in two places in turn
         alive = wait_warp(qfull, took & 1, P.status);
-        for (int i = 0; i < k.n && alive; i++) {
-          if (passed > 1) alive = wait_warp(pvdone + 8 * (passed & 1), ((passed >> 1) - 1) & 1, P.status);
-          if (!alive || !scores(tmem + (passed & 1) * 128, true)) { alive = false; break; }
-          commit(sfull + 8 * (passed & 1), lead);
-          passed++;
+        for (int i = 0; i < k.n && alive; i++, passed++) {
+          const uint32_t s = passed & 1;
+          alive = keys_there() && (passed < 2 || wait_warp(pvdone + 8 * s, ((passed >> 1) - 1) & 1, P.status));
+          if (!alive) break;
+          scores(tmem + s * 128, min(8, (b - key_of(k, i) + 16) / 16), sfull + 8 * s);
+          next_keys();
         }
         if (alive) { commit(qempty, lead); took++; }
       } else {
-        for (int i = 0; i < k.n && alive; i++) {
+        for (int i = 0; i < k.n && alive; i++, passed++) {
           const uint32_t s = passed & 1;
-          if (!results(tmem + s * 128, o_at, pfull + 16 * s, phalf, (passed >> 1) & 1, true, !sees_all(P, w.tok, k.t1 - 1, key_of(k, i)), i > 0)) { alive = false; break; }
-          commit(pvdone + 8 * s, lead);
-          passed++;
+          const int key0 = key_of(k, i);
+          alive = values_there(!sees_all(P, w.tok, k.t1 - 1, key0)) && results(tmem + s * 128, o_at, pfull + 16 * s, (passed >> 1) & 1, min(8, (b - key0 + 16) / 16), i > 0, pvdone + 8 * s);
         }
         if (alive) commit(odone, lead);
       }
@@ -240,19 +270,24 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   } else if (warp == 10 || warp == 11) {                     // copies: keys and queries, values
     Item w;
     const int chunks = (P.dk + 63) / 64, boxes = (P.dv + 63) / 64;
-    uint32_t n = 0, par = 0, took[2] = {0, 0}, sent = 0, vpar[2] = {0, 0}, vsent[2] = {0, 0};
+    uint32_t n = 0, par = 0, took[2] = {0, 0}, vpar[2] = {0, 0}, vsent[2] = {0, 0};
+    int tile = 0, freed = 0, sent = 0;                       // tiles of keys begun and given back, units sent
     bool alive = true;
     auto keys = [&](const Item& w, int key0, int head) {
-      for (int c = 0; c < chunks && alive; c++) {
-        alive = wait_warp(kempty + 8 * n, par ^ 1, P.status);
-        if (!alive) break;
+      for (int c = 0; c < chunks; c++) {
+        while (freed + kAhead <= tile || freed * chunks + KU <= sent) {   // the barrier's last tile, and the unit that lies where this one goes
+          alive = wait_warp(kempty + 8 * (freed % kAhead), (freed / kAhead) & 1, P.status);
+          if (!alive) return;
+          freed++;
+        }
         if (lane == 0) {
-          mbar_expect_tx(kfull + 8 * n, kUnit);
-          copy_box(ks + n * kUnit, &P.k, 64 * c, head, w.row + key0, kfull + 8 * n);
+          if (c == 0) mbar_expect_tx(kfull + 8 * (tile % kAhead), chunks * kUnit);
+          copy_box(ks + n * kUnit, &P.k, 64 * c, head, w.row + key0, kfull + 8 * (tile % kAhead));
         }
         sent++;
-        if (++n == KU) { n = 0; par ^= 1; }
+        if (++n == KU) n = 0;
       }
+      tile++;
     };
     if (warp == 10) {
       while (alive && take(w)) {
@@ -272,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         for (int i = 1; i < k.n && alive; i++) keys(w, key_of(k, i), head);
       }
       for (int t = 0; t < TILES; t++) if (took[t]) wait_warp(qfull + 8 * t, (took[t] - 1) & 1, P.status);   // no copy is under way at the end, whatever happened
-      for (uint32_t s = 0; s < KU && s < sent; s++) { if (n == 0) { n = KU; par ^= 1; } n--; wait_warp(kfull + 8 * n, par, P.status); }
+      for (int s = max(0, tile - kAhead); s < tile; s++) wait_warp(kfull + 8 * (s % kAhead), (s / kAhead) & 1, P.status);
     } else {
       while (alive && take(w)) {
         const Walk k = walk_of(P, w, tokens);
@@ -347,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       if (slot) par ^= 1;
       if (item.y <= 0) break;
     }
-  } else if (warp >= 12) {                                   // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
+  } else {                                                   // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
     Item w;
     const int me = threadIdx.x - 12 * 32, boxes = (P.dv + 63) / 64;
     const uint32_t inf = BF16 ? 0x7f807f80u : 0x7c007c00u;
@@ -382,15 +417,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         }
       }
     }
+  }
   } else if (warp < SOFT) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MANY));
     const int t = warp >> 2, quad = warp & 3, r = threadIdx.x & 127, tok_of = r / P.pack;       // the thread's row: token tok_of of the tile, head r % pack
     const bool exists = r < P.tokens * P.pack;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, res = o_at + t * 128 + lanes;
-    uint32_t passed = 0, took = 0;
+    uint32_t passed = 0, took = 0, gated = 0;                // gated: tiles that both groups have
     Item w;
     bool ok = true;
     while (ok && take(w)) {
-      const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
+      const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1, other = w.tok + (t ^ 1) * P.tokens;
       if (a >= w.len) continue;
       const Walk k = walk_of(P, w, tokens);
       const int pos = exists ? a + tok_of : 0x3fffffff;
@@ -401,83 +438,95 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         const int key0 = key_of(k, i);
         if (!sees_some(P, a, b, key0)) continue;
         const uint32_t buf = TILES == 2 ? t : passed & 1, par = TILES == 2 ? passed & 1 : (passed >> 1) & 1, s_at = tmem + buf * 128 + lanes;
+        const bool masked = !sees_all(P, a, b, key0);
+        // The two groups' exponentials take turns: one's products then run under the other's, where both at a time would wait for the exponentials' pipe and leave the tensor pipe idle
+        const bool gate = TILES == 2 && other < w.len && sees_some(P, other, min(other + P.tokens, w.len) - 1, key0);
+        const uint32_t turn_of = turns + 8 * t, turn_par = (gated - 1 + t) & 1;
         ok = wait_warp(sfull + 8 * buf, par, P.status);
         if (!ok) break;
         if (idle) {                                          // (its rows' results are whatever comes of the scores as weights, and go nowhere)
           __syncwarp();
           if (lane < 2) hy::tc_arrive(pfull + 16 * buf + 8 * lane);
+          if (gate) { if (lane == 0) hy::tc_arrive(turns + 8 * (t ^ 1)); gated++; }
           passed++;
           any = true;
           continue;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const bool masked = !sees_all(P, a, b, key0);
+        const bool go = !gate || gated + t == 0 || hy::tc_poll(turn_of, turn_par);   // (asked ahead of the maxima, which the answer then comes under)
+        uint32_t x[128];                                     // the whole row: its weights then lie where the scores were
+        tmem_row(s_at, x);
+        if (masked) {                                        // keys that the row sees, a bit each: not behind its own, in the window or among the first
+#pragma unroll
+          for (int u = 0; u < 128; u += 32) {
+            const int j = key0 + u;
+            uint32_t see = lower_bits(pos + 1 - j);
+            if (P.window > 0) see &= ~lower_bits(pos - P.window + 1 - j) | lower_bits(P.keep - j);
+#pragma unroll
+            for (int e = 0; e < 32; e++) if (!(see >> e & 1)) x[u + e] = 0xff800000u;
+          }
+        }
+        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 128; e += 8)
+#pragma unroll
+          for (int g = 0; g < 4; g++) y[g] = max3(__float_as_uint(y[g]), x[e + 2 * g], x[e + 2 * g + 1]);
+        const float top = mine ? fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * P.f : -INFINITY;
+        float f = P.f;
+        if (__any_sync(0xffffffffu, top > limit)) {
+          const float c_top = ceilf(top), to = fmaxf(m, fabsf(c_top) > kFar ? c_top : c_top + LEAD), by = exp2_fast(m - to);
+          m = to;
+          l *= by;
+          const bool far = fabsf(m) > kFar;
+          limit = far ? -INFINITY : m + ROOM;
+          if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+            for (int e = 0; e < 128; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+            f = 1.f;
+          }
+          if (any) {                                         // (two row tiles: the last product was through ahead of these scores)
+            // A wait by parity is right while the barrier is in the phase asked for or the one behind it: these scores waited for the product before the one ahead
+            if (TILES == 1) ok = wait_warp(pvdone + 8 * (buf ^ 1), ((passed - 1) >> 1) & 1, P.status);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-        for (int half = 0; half < 2; half++) {
-          uint32_t x[64];
-          tmem_read64(s_at + half * 64, x);
-          if (masked) {                                      // keys that the row sees, a bit each: not behind its own, in the window or among the first
+            for (int d = 0; d < P.dv; d += 16) {
+              uint32_t z[16];
+              tmem_read16(res + d, z);
 #pragma unroll
-            for (int u = 0; u < 64; u += 32) {
-              const int j = key0 + half * 64 + u;
-              uint32_t see = lower_bits(pos + 1 - j);
-              if (P.window > 0) see &= ~lower_bits(pos - P.window + 1 - j) | lower_bits(P.keep - j);
-#pragma unroll
-              for (int e = 0; e < 32; e++) if (!(see >> e & 1)) x[u + e] = 0xff800000u;
+              for (int e = 0; e < 16; e++) z[e] = __float_as_uint(__uint_as_float(z[e]) * by);
+              tmem_store16(res + d, z);
             }
           }
-          float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        }
+        if (!__all_sync(0xffffffffu, go)) ok = wait_warp(turn_of, turn_par, P.status) && ok;
+        const uint64_t f2 = both(f, f), off = both(-m, -m);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-          for (int e = 0; e < 64; e += 8)
+        for (int u = 0; u < 4; u++) {
+          uint32_t p[16];
 #pragma unroll
-            for (int g = 0; g < 4; g++) y[g] = max3(__float_as_uint(y[g]), x[e + 2 * g], x[e + 2 * g + 1]);
-          const float top = mine ? fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * P.f : -INFINITY;
-          float f = P.f;
-          if (__any_sync(0xffffffffu, top > limit)) {
-            const float c_top = ceilf(top), to = fmaxf(m, fabsf(c_top) > kFar ? c_top : c_top + LEAD), by = exp2_fast(m - to);
-            m = to;
-            l *= by;
-            const bool far = fabsf(m) > kFar;
-            limit = far ? -INFINITY : m + ROOM;
-            if (__any_sync(0xffffffffu, far)) {
-#pragma unroll
-              for (int e = 0; e < 64; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-              f = 1.f;
-            }
-            if (any || half) {                               // products whose results are to be scaled must be through; what the tile's first half stored is read back as results, not by this thread
-              // (a wait by parity is right while the barrier is in the phase asked for or the one behind it: with one row tile, scores do not wait for the product ahead, so that this does)
-              if (TILES == 1 && passed > 0) ok = wait_warp(pvdone + 8 * (buf ^ 1), ((passed - 1) >> 1) & 1, P.status) && ok;
-              if (half) ok = wait_warp(phalf + 8 * (TILES == 2 ? t : 0), passed & 1, P.status) && ok;
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-              for (int d = 0; d < P.dv; d += 16) {
-                uint32_t z[16];
-                tmem_read16(res + d, z);
-#pragma unroll
-                for (int e = 0; e < 16; e++) z[e] = __float_as_uint(__uint_as_float(z[e]) * by);
-                tmem_store16(res + d, z);
-              }
-            }
-          }
-          const uint64_t f2 = both(f, f), off = both(-m, -m);
-          uint64_t sum[2] = {0, 0};
-          uint32_t p[32];                                    // weights of a half lie in the first 32 of its columns
-#pragma unroll
-          for (int e = 0; e < 32; e++) {
+          for (int e = 0; e < 16; e++) {
             float y0, y1;
-            fma2(x[2 * e], x[2 * e + 1], f2, off, y0, y1);
+            fma2(x[32 * u + 2 * e], x[32 * u + 2 * e + 1], f2, off, y0, y1);
             y0 = exp2_fast(y0);
             y1 = exp2_fast(y1);
             add2(sum[e & 1], y0, y1);
             p[e] = pair<BF16>(y0, y1);
           }
-          tmem_store32(s_at + half * 64, p);
-          l += (__uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32))) + (__uint_as_float((uint32_t)sum[1]) + __uint_as_float((uint32_t)(sum[1] >> 32)));
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) hy::tc_arrive(pfull + 16 * buf + 8 * half);
+          if (u == 3 && gate) {
+            __syncwarp();
+            if (lane == 0) hy::tc_arrive(turns + 8 * (t ^ 1));
+            gated++;
+          }
+          tmem_store16(s_at + 16 * u, p);
+          if (u & 1) {                                       // a half of the weights: its product starts
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) hy::tc_arrive(pfull + 16 * buf + 8 * (u >> 1));
+          }
         }
+        l += (__uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32))) + (__uint_as_float((uint32_t)sum[1]) + __uint_as_float((uint32_t)(sum[1] >> 32)));
         passed++;
         any = true;
       }

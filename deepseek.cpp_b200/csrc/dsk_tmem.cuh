@@ -38,6 +38,13 @@ __device__ __forceinline__ void tmem_read16(uint32_t addr, uint32_t (&r)[16]) { 
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
 }
+template <int N> __device__ __forceinline__ void tmem_row(uint32_t addr, uint32_t (&r)[N]) {   // N columns, 32 at a time; loaded when it returns
+#pragma unroll
+  for (int i = 0; i < N; i += 32) hy::tc_load32(addr + i, *reinterpret_cast<uint32_t(*)[32]>(&r[i]));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));   // (no use ahead of the wait)
+}
 // two fp32 operations at a time
 __device__ __forceinline__ uint64_t both(float a, float b) {
   uint64_t r;

@@ -20,6 +20,7 @@ class Bar:
         return lambda: (self.phase & 1) != parity & 1
 
 
+AHEAD = 4                                                    # tiles of keys under way
 SHAPES = {64: (2, 1, 1, 6, 5), 128: (2, 2, 2, 6, 4), 192: (2, 3, 2, 5, 3), 256: (1, 4, 4, 6, 4)}      # row tiles, units of keys and of values a tile, places for them
 
 
@@ -29,12 +30,12 @@ def run(rng, dk, work, idle, moves, early=True):
     tiles, per_k, per_v, KU, VU = SHAPES[dk]
     bars = lambda n, count: [Bar(count) for _ in range(n)]
     soft = 4 * tiles
-    kfull, kempty, vfull, vempty, vok, vraw = bars(KU, 1), bars(KU, tiles), bars(VU, 1), bars(VU, tiles), bars(VU, 3), bars(VU, 1)
-    qfull, qempty, sfull, phalf, pvdone, odone, ifull = (bars(2, 1) for _ in range(7))
+    kfull, kempty, vfull, vempty, vok, vraw = bars(AHEAD, 1), bars(AHEAD, tiles), bars(VU, 1), bars(VU, tiles), bars(VU, 3), bars(VU, 1)
+    qfull, qempty, sfull, pvdone, odone, ifull, turns = *(bars(2, 1) for _ in range(6)), bars(2, 4)
     pfull, iempty, flushed = [bars(2, 4) for _ in range(2)], bars(2, soft + 7), bars(2, 1)
     items = [None, None]
     keys, values, queries, looked = [None] * KU, [None] * VU, [None] * 2, [0] * VU
-    scores, weights, half_through, through = [None, None], [[{}, {}], [{}, {}]], [None, None], [None, None]
+    scores, weights, through = [None, None], [[{}, {}], [{}, {}]], [None, None]
     queue, flying = [], []                                   # products and commits in the order of their issue; copies in any order
 
     def take(state):
@@ -55,22 +56,28 @@ def run(rng, dk, work, idle, moves, early=True):
                 par ^= 1
 
     def copy_keys():
-        me, n, par, took = {"turn": 0}, 0, 0, [0, 0]
+        me, took = {"turn": 0}, [0, 0]
+        at = {"n": 0, "tile": 0, "freed": 0, "sent": 0}
         while True:
             yield from take(me)
             if me["item"] is None:
                 return
             walk, two = work[me["item"]]
 
-            def tile(i, n, par):
+            def tile(i):
+                bar = kfull[at["tile"] % AHEAD]
+                units = Bar(per_k)                           # (the barrier counts bytes: its phase ends with the last unit)
                 for c in range(per_k):
-                    yield kempty[n].wait(par ^ 1)
-                    flying.append((keys, n, (me["item"], i, c), kfull[n]))
-                    keys[n] = "under way"
-                    n, par = (0, par ^ 1) if n + 1 == KU else (n + 1, par)
-                return n, par
+                    while at["freed"] + AHEAD <= at["tile"] or at["freed"] * per_k + KU <= at["sent"]:
+                        yield kempty[at["freed"] % AHEAD].wait(at["freed"] // AHEAD)
+                        at["freed"] += 1
+                    flying.append((keys, at["n"], (me["item"], i, c), (units, bar)))
+                    keys[at["n"]] = "under way"
+                    at["sent"] += 1
+                    at["n"] = (at["n"] + 1) % KU
+                at["tile"] += 1
 
-            n, par = yield from tile(0, n, par)
+            yield from tile(0)
             for t in range(tiles):
                 if t and not two:
                     continue
@@ -79,7 +86,7 @@ def run(rng, dk, work, idle, moves, early=True):
                 queries[t] = "under way"
                 took[t] += 1
             for i in range(1, len(walk)):
-                n, par = yield from tile(i, n, par)
+                yield from tile(i)
 
     def copy_values():
         me, n, par = {"turn": 0}, 0, 0
@@ -132,45 +139,47 @@ def run(rng, dk, work, idle, moves, early=True):
                 through[buf if tiles == 1 else t] = (n, i)
         return product
 
-    def half_done(t, n, i):
-        def job():
-            half_through[t] = (n, i)
-        return job
+    def issue_scores(t, state, n, i, buf):
+        places = [(state["kn"] + c) % KU for c in range(per_k)]
+        queue.extend([product_of_scores(t, n, i, c, place, buf) for c, place in enumerate(places)] + [sfull[buf], kempty[state["kt"] % AHEAD]])
 
-    def issue_scores(t, state, n, i, buf, mine):
-        for c in range(per_k):
-            yield kfull[state["kn"]].wait(state["kpar"])
-            if mine:
-                queue.extend([product_of_scores(t, n, i, c, state["kn"], buf), kempty[state["kn"]]])
-            else:
-                kempty[state["kn"]].arrive()
-            state["kn"] += 1
-            if state["kn"] == KU:
-                state["kn"], state["kpar"] = 0, state["kpar"] ^ 1
+    def next_keys(state):
+        state["kt"] += 1
+        state["kn"] = (state["kn"] + per_k) % KU
 
-    def issue_results(t, state, n, i, buf, parity, mine, masked):
+    def keys_there(state):
+        return kfull[state["kt"] % AHEAD].wait(state["kt"] // AHEAD)
+
+    def values_there(state, masked):
+        for c in range(per_v):
+            place = (state["vn"] + c) % VU
+            yield (vok if masked else vfull)[place].wait(state["vpar"][masked][place])
+            state["vpar"][masked][place] ^= 1
+
+    def issue_results(t, state, n, i, buf, parity, masked):
         steps = 8 // per_v
         for u in range(8):
             place = state["vn"]
-            if u % steps == 0:
-                yield (vok if masked else vfull)[place].wait(state["vpar"][masked][place])
-                state["vpar"][masked][place] ^= 1
-            if mine and u % 4 == 0:
-                if u == 4:
-                    queue.extend([half_done(t, n, i), phalf[t]])
+            if u % 4 == 0:
                 yield pfull[buf][u // 4].wait(parity)
             if u % steps == steps - 1 or u == 3:
-                if mine:
-                    queue.append(product_of_results(t, n, i, u // steps, place, buf, masked, u // 4 if steps <= 4 else (0 if u == 3 else None), u == 7))
+                queue.append(product_of_results(t, n, i, u // steps, place, buf, masked, u // 4 if steps <= 4 else (0 if u == 3 else None), u == 7))
+                if u == 7:
+                    queue.append(pvdone[t if tiles == 2 else buf])
             if u % steps == steps - 1:
-                if mine:
-                    queue.append(vempty[place])
+                if tiles == 2 and u == 7:
+                    state["pend"] = place
                 else:
-                    vempty[place].arrive()
+                    queue.append(vempty[place])
                 state["vn"] = (place + 1) % VU
 
+    def give_back(state):
+        if state["pend"] is not None:
+            queue.append(vempty[state["pend"]])
+            state["pend"] = None
+
     def issuer(x):
-        me = {"turn": 0, "kn": 0, "kpar": 0, "vn": 0, "vpar": [[0] * VU, [0] * VU]}
+        me = {"turn": 0, "kt": 0, "kn": 0, "vn": 0, "vpar": [[0] * VU, [0] * VU], "pend": None}
         passed = took = 0
         while True:
             yield from take(me)
@@ -182,36 +191,48 @@ def run(rng, dk, work, idle, moves, early=True):
                 there = x == 0 or two
                 if there:
                     yield qfull[x].wait(took)
+                yield keys_there(me)
                 for i, (who, masked) in enumerate(walk):
                     mine = there and x in who
-                    if mine and passed:
-                        yield pvdone[x].wait(passed - 1)
-                    yield from issue_scores(x, me, n, i, x, mine)
                     if mine:
-                        queue.append(sfull[x])
-                    if there and i == len(walk) - 1:
+                        if passed:
+                            yield pvdone[x].wait(passed - 1)
+                        issue_scores(x, me, n, i, x)
+                    else:
+                        kempty[me["kt"] % AHEAD].arrive()
+                    give_back(me)
+                    next_keys(me)
+                    if i + 1 < len(walk):
+                        yield keys_there(me)
+                    elif there:
                         queue.append(qempty[x])
-                    yield from issue_results(x, me, n, i, x, passed, mine, masked)
+                    yield from values_there(me, masked)
                     if mine:
-                        queue.append(pvdone[x])
+                        yield from issue_results(x, me, n, i, x, passed, masked)
                         passed += 1
+                    else:
+                        for _ in range(per_v):
+                            vempty[me["vn"]].arrive()
+                            me["vn"] = (me["vn"] + 1) % VU
                 if there:
                     queue.append(odone[x])
                     took += 1
+                give_back(me)
             elif x == 0:
                 yield qfull[0].wait(took)
                 for i in range(len(walk)):
+                    yield keys_there(me)
                     if passed > 1:
                         yield pvdone[passed & 1].wait((passed >> 1) - 1)
-                    yield from issue_scores(0, me, n, i, passed & 1, True)
-                    queue.append(sfull[passed & 1])
+                    issue_scores(0, me, n, i, passed & 1)
+                    next_keys(me)
                     passed += 1
                 queue.append(qempty[0])
                 took += 1
             else:
                 for i, (_, masked) in enumerate(walk):
-                    yield from issue_results(0, me, n, i, passed & 1, passed >> 1, True, masked)
-                    queue.append(pvdone[passed & 1])
+                    yield from values_there(me, masked)
+                    yield from issue_results(0, me, n, i, passed & 1, passed >> 1, masked)
                     passed += 1
                 queue.append(odone[0])
         queue.append(flushed[x])
@@ -220,7 +241,7 @@ def run(rng, dk, work, idle, moves, early=True):
     def softmax(x):
         t, w = divmod(x, 4)
         me = {"turn": 0}
-        passed = took = 0
+        passed = took = gated = 0
         while True:
             yield from take(me)
             n = me["item"]
@@ -229,33 +250,35 @@ def run(rng, dk, work, idle, moves, early=True):
             walk, two = work[n]
             if t and not two:
                 continue
-            first = last = None
+            last = None
             for i, (who, _) in enumerate(walk):
                 if t not in who:
                     continue
                 buf, par = (t, passed) if tiles == 2 else (passed & 1, passed >> 1)
                 yield sfull[buf].wait(par)
-                for half in (0, 1):
-                    if idle[n][x]:
-                        pfull[buf][half].arrive()
-                        continue
+                if not idle[n][x]:
                     assert scores[buf] == (n, i)
                     yield None
-                    if (first is not None or half) and rng.random() < moves:          # results are scaled again
-                        if tiles == 1 and passed > 0 and early:
+                    if last is not None and rng.random() < moves:     # results are scaled again
+                        if tiles == 1 and early:
                             yield pvdone[buf ^ 1].wait((passed - 1) >> 1)
-                        if half:
-                            yield phalf[t].wait(passed)
-                            assert half_through[t] == (n, i)
-                        if last is not None:
-                            assert through[buf ^ 1 if tiles == 1 else t] == last
+                        assert through[buf ^ 1 if tiles == 1 else t] == last
                         yield None
-                    assert scores[buf] == (n, i)
-                    weights[buf][half][w] = (n, i)
-                    yield None
+                gate = len(who) == 2
+                if gate and not idle[n][x] and gated + t > 0:
+                    yield turns[t].wait(gated - 1 + t)
+                for half in (0, 1):
+                    if not idle[n][x]:
+                        assert scores[buf] == (n, i)
+                        weights[buf][half][w] = (n, i)
+                        yield None
+                    if half and gate:
+                        turns[t ^ 1].arrive()
+                        gated += 1
+                        yield None
                     pfull[buf][half].arrive()
                 passed += 1
-                first, last = first or (n, i), (n, i)
+                last = (n, i)
             yield odone[t if tiles == 2 else 0].wait(took)
             took += 1
             if not idle[n][x]:
@@ -275,7 +298,12 @@ def run(rng, dk, work, idle, moves, early=True):
         elif k > len(roles):
             where, place, what, bar = flying.pop(rng.randrange(len(flying)))
             where[place] = what
-            bar.arrive()
+            if isinstance(bar, tuple):
+                bar[0].arrive()
+                if bar[0].phase:
+                    bar[1].arrive()
+            else:
+                bar.arrive()
         else:
             at[k] = next(roles[k], False)
 
@@ -292,7 +320,9 @@ def draw(rng, dk):
         walk[0] = ({0, 1} if two else {0}, walk[0][1])       # (a row tile that has rows sees some tile)
         work.append((walk, two))
         row = [rng.random() < 0.2 for _ in range(4 * tiles)]
-        row[0] = False
+        row[0] = False                                       # (a row tile that has rows has its first)
+        if two:
+            row[4] = False
         idle.append(row)
     return dict(dk=dk, work=work, idle=idle, moves=rng.choice([0, 0.3, 1]))
 

@@ -157,8 +157,6 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   if (!encode_tiled()) return fail(-2, "the driver has no cuTensorMapEncodeTiled");
   OnDevice on(s->device);
   CK(on.error);
-  const int sms = multiprocessors(s->device);
-  if (!sms) return fail(-2, "device %d: no attributes", s->device);
   prompt::Params P;
   P.group = heads / kv_heads;
   // heads of a row tile: a divisor of the group that fills most of its 128 rows, the largest of those (its tokens are then few, and their keys end close together)
@@ -181,7 +179,8 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   P.f = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);            // (positive: -inf stays what it is)
   const int tokens = P.tokens * (shape == 3 ? 1 : 2);
   const long long items = ((long long)s->rows / tokens + std::min(s->batch, s->rows)) * P.units;   // at most, whatever the lengths
-  const int ctas = (int)std::min<long long>(sms, items);
+  if (items > INT32_MAX) return fail(-4, "%lld pieces of work: at most 2^31", items);
+  const int ctas = (int)items;                               // (those that are running take over the others)
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dt == DSK_DT_BF16;
   switch (shape) {

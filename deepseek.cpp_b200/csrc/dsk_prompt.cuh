@@ -21,7 +21,7 @@
 namespace dsk {
 namespace prompt {
 
-constexpr int kThreads = 512, kTile = 128, kUnit = 16384, kMaxBatch = 1024, kHeld = 8, kAhead = 4;   // keys of a tile; bytes of a copied unit; sequences whose tiles a lane of the dealing warp keeps in registers; tiles of keys under way
+constexpr int kThreads = 512, kTile = 128, kUnit = 16384, kMaxBatch = 1024, kHeld = 8, kAhead = 4, kEarly = 4;   // keys of a tile; bytes of a copied unit; sequences whose tiles a lane of the dealing warp keeps in registers; tiles of keys under way; tiles ahead of the end at which more work is asked for
 constexpr int ST_WAIT = 4;                                   // a wait that gave up
 constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
 constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
@@ -80,19 +80,19 @@ __device__ __forceinline__ Walk walk_of(const Params& P, const Item& w, int toke
   return k;
 }
 __device__ __forceinline__ int key_of(const Walk& k, int i) { return (i < k.kept ? i : k.low + i - k.kept) * kTile; }
-// whether tokens a .. b see all of a tile of keys; any of it
-__device__ __forceinline__ bool sees_all(const Params& P, int a, int b, int key0) {
-  return key0 + kTile - 1 <= a && (P.window <= 0 || b - key0 < P.window || key0 + kTile <= P.keep);
+// whether tokens a .. b see all of `keys` keys; any of them
+__device__ __forceinline__ bool sees_all(const Params& P, int a, int b, int key0, int keys) {
+  return key0 + keys - 1 <= a && (P.window <= 0 || b - key0 < P.window || key0 + keys <= P.keep);
 }
-__device__ __forceinline__ bool sees_some(const Params& P, int a, int b, int key0) {
-  return key0 <= b && (P.window <= 0 || a - key0 - kTile + 1 < P.window || key0 < P.keep);
+__device__ __forceinline__ bool sees_some(const Params& P, int a, int b, int key0, int keys) {
+  return key0 <= b && (P.window <= 0 || a - key0 - keys + 1 < P.window || key0 < P.keep);
 }
 
 // Infinities and NaN among the values that a row sees in tiles where they went to the products as zeros: its results c .. c + 15 become what they make of them
 template <bool BF16> __device__ __noinline__ void give_back(const Params& P, const Item& w, const Walk& k, int pos, int head, int c, uint32_t (&x)[16]) {
   for (int i = 0; i < k.n; i++) {
     const int key0 = key_of(k, i);
-    if (sees_all(P, w.tok, k.t1 - 1, key0)) continue;
+    if (sees_all(P, w.tok, k.t1 - 1, key0, kTile)) continue;
     for (int j = key0; j < min(key0 + kTile, pos + 1); j++) {
       if (P.window > 0 && pos - j >= P.window && j >= P.keep) continue;
       const uint16_t* v = static_cast<const uint16_t*>(P.values) + (long long)(w.row + j) * P.v_row + (long long)head * P.v_head + c;
@@ -107,24 +107,29 @@ template <bool BF16> __device__ __noinline__ void give_back(const Params& P, con
 
 template <int DK, int DV, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_constant__ Params P) {
-  constexpr int TILES = tiles<DK, DV>(), KU = k_units<DK, DV>(), VU = v_units<DK, DV>(), VK = kUnit / (2 * DV), STEPS = VK / 16, SOFT = 4 * TILES, USERS = SOFT + 7;   // VK: keys of a unit of values
+  constexpr int TILES = tiles<DK, DV>(), KU = k_units<DK, DV>(), VU = v_units<DK, DV>(), VK = kUnit / (2 * DV), STEPS = VK / 16, SOFT = 4 * TILES, USERS = SOFT + TILES + 5;   // VK: keys of a unit of values
+  constexpr int W = kTile / TILES, PER = kTile / W;          // keys of a step: a row tile has scores in two places of W columns, so that one's products run under the other's softmax; steps of a tile
   constexpr float LEAD = BF16 ? 40.f : -7.f, ROOM = BF16 ? -26.f : 14.f;       // a reference is taken LEAD above its maximum, and follows once that is above m + ROOM
+  constexpr int MANY = 192, FEW = 64;                        // registers of a softmax thread and of another one: 512 threads have 128 each
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t bars[50];
+  __shared__ __align__(8) uint64_t bars[56];
   __shared__ int4 items[2];
+  __shared__ __align__(16) uint4 claim;
   __shared__ uint32_t tmem_slot;
-  __shared__ int odd_values;
+  __shared__ int odd_values, pieces;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, qs = base, ks = qs + 128 * TILES * DK * 2, vs = ks + KU * kUnit, b0 = smem_u32(bars);
-  const uint32_t kfull = b0, kempty = b0 + 32, vfull = b0 + 64, vempty = b0 + 104, vok = b0 + 144, vraw = b0 + 184, qfull = b0 + 224, qempty = b0 + 240, sfull = b0 + 256, pfull = b0 + 272,
-                 pvdone = b0 + 304, odone = b0 + 320, ifull = b0 + 336, iempty = b0 + 352, flushed = b0 + 368, turns = b0 + 384;   // keys: a barrier for each of kAhead tiles; vraw: where values land that are looked at ahead of their products
+  const uint32_t kfull = b0, kempty = b0 + 32, vfull = b0 + 64, vempty = b0 + 104, vok = b0 + 144, vraw = b0 + 184, qfull = b0 + 224, qempty = b0 + 240, odone = b0 + 256, ifull = b0 + 272,
+                 iempty = b0 + 288, sfull = b0 + 304, pfull = b0 + 336, pvdone = b0 + 368, flushed = b0 + 400, want = b0 + 416, claimed = b0 + 424;
+  // keys: a barrier for each of kAhead tiles; values: one for each place (vraw: where they land that are looked at ahead of their products); scores, weights, products: [row tile][place]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tokens = TILES * P.tokens;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kAhead; i++) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); }
+    for (int i = 0; i < kAhead; i++) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); }
     for (int i = 0; i < 5; i++) { mbar_init(vfull + 8 * i, 1); mbar_init(vempty + 8 * i, TILES); mbar_init(vok + 8 * i, 3); mbar_init(vraw + 8 * i, 1); }
     for (int i = 0; i < 2; i++) {
-      mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 16 * i, 4); mbar_init(pfull + 16 * i + 8, 4);
-      mbar_init(pvdone + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); mbar_init(flushed + 8 * i, 1); mbar_init(turns + 8 * i, 4);
+      mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); mbar_init(flushed + 8 * i, 1);
     }
+    mbar_init(want, 1);
+    mbar_init(claimed, 1);
     odd_values = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -132,13 +137,33 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  // How many pieces of work there are: row tiles that are the j-th or a later one of their sequence, of all sequences
+  int held[kHeld], most = 0;                                 // (the dealing warp's: row tiles of sequences lane, lane + 32, ..)
+  auto tiles_of = [&](int b) {
+    if (b >= P.batch) return 0;
+    const int from = min(max(P.starts[b], 0), P.rows), to = min(max(P.starts[b + 1], from), P.rows);
+    return (to - from + tokens - 1) / tokens;
+  };
+  auto from_level = [&](int j) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) n += max(held[i] - j, 0);
+    for (int b = lane + 32 * kHeld; b < P.batch; b += 32) n += max(tiles_of(b) - j, 0);
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  if (warp == 15) {
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) { held[i] = tiles_of(lane + 32 * i); most = max(most, held[i]); }
+    for (int b = lane + 32 * kHeld; b < P.batch; b += 32) most = max(most, tiles_of(b));
+    most = __reduce_max_sync(0xffffffffu, most);
+    const int n = from_level(0);
+    if (lane == 0) pieces = n;
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [2][128], results [tile][DV]
-
-  // 512 threads have 128 registers each; a softmax thread holds a row of scores, the others little
-  constexpr int MANY = 192, FEW = 64;
+  const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [row tile][place][W], results [tile][DV]
+  const long long all = (long long)pieces * P.units;
 
   uint32_t turn = 0;                                         // items that this warp has taken
   auto take = [&](Item& w) {                                 // the next item, in every lane
@@ -152,313 +177,296 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     return ok && w.len > 0;
   };
 
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
-  if (warp == 8 || warp == 9) {                              // products: of row tile warp - 8 (one row tile: scores, results)
-    const int t = warp - 8;
-    const uint32_t lead = hy::tc_elect();
-    const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);         // fp32 sums of bf16 or fp16, 128 rows
-    const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17);
-    const int chunks = (P.dk + 63) / 64, ksteps = P.dk / 16;
-    uint32_t kt = 0, kn = 0, vn = 0, vpar[2] = {0, 0}, passed = 0, took = 0;   // tiles of keys behind, places in the rings, parities of values (a bit for each place: as they came, looked at), tiles of this row tile, items that had rows
-    int pend = -1;                                           // a unit of values whose product is issued and that is to be given back
-    auto keys_there = [&] { return wait_warp(kfull + 8 * (kt % kAhead), (kt / kAhead) & 1, P.status); };
-    auto scores = [&](uint32_t to, int n, uint32_t full) {   // of the next tile of keys, of which the rows see the first 16 n
-      const uint64_t a = hy::tc_desc(qs + (TILES == 2 ? t * (kTile * DK * 2) : 0));
-      const uint32_t sdesc = idesc | (uint32_t)(2 * n) << 17;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (blockIdx.x >= all) {                                   // (nothing for this CTA: the grid is launched for as many pieces as there may be)
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
+    if (warp < 8 + TILES) {                                  // products of row tile warp - 8
+      const int t = warp - 8;
+      const uint32_t lead = hy::tc_elect();
+      const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);         // fp32 sums of bf16 or fp16, 128 rows
+      const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17), s_at = tmem + t * 128, to = o_at + t * 128;
+      const uint64_t q_desc = hy::tc_desc(qs + t * (kTile * DK * 2));
+      const int chunks = (P.dk + 63) / 64, ksteps = P.dk / 16;
+      const bool whole = ksteps == DK / 16;
+      uint32_t kt = 0, kn = 0, vn = 0, vpar[2] = {0, 0}, sent = 0, done = 0, took = 0;   // tiles of keys behind, places in the rings, parities of values (a bit for each place: as they came, looked at),
+      Item w;                                                                            // steps whose scores, whose results are issued, items that had rows
+      bool alive = true;
+      while (alive && take(w)) {
+        const Walk k = walk_of(P, w, tokens);
+        const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1, last = k.n * PER;
+        const bool there = a < w.len;
+        int q_step = 0, v_step = 0;
+        bool any = false;
+        auto key_at = [&](int step) { return key_of(k, step / PER) + step % PER * W; };
+        auto is_mine = [&](int step) { return there && sees_some(P, a, b, key_at(step), W); };
+        auto ahead = [&] {                                   // scores of two steps ahead of their results (more, past steps that the rows do not see, and the two row tiles might wait for one another)
+          while (q_step < min(last, v_step + 2)) {
+            const int key0 = key_at(q_step);
+            const bool mine = is_mine(q_step);
+            if (q_step % PER == 0 && !wait_warp(kfull + 8 * (kt % kAhead), (kt / kAhead) & 1, P.status)) return false;
+            if (mine) {
+              const uint32_t place = sent & 1, sdesc = idesc | (uint32_t)(2 * min(W / 16, (b - key0 + 16) / 16)) << 17;   // (the rows see the first of them)
+              uint64_t k_desc[DK / 64];
 #pragma unroll
-      for (int c = 0; c < DK / 64; c++) {
-        if (c >= chunks) break;
-        const uint64_t k = hy::tc_desc(ks + (kn + c < KU ? kn + c : kn + c - KU) * kUnit);
+              for (int c = 0; c < DK / 64; c++) k_desc[c] = hy::tc_desc(ks + (kn + c < KU ? kn + c : kn + c - KU) * kUnit + q_step % PER * (W * 128));
+              if (sent > 1 && !wait_warp(pvdone + 16 * t + 8 * place, ((sent >> 1) - 1) & 1, P.status)) return false;   // the weights that lie there are read
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              if (whole) {
 #pragma unroll
-        for (int u = 0; u < 4; u++) if (4 * c + u < ksteps) mma_ss(to, a + c * (kTile * 128 >> 4) + 2 * u, k + 2 * u, sdesc, c > 0 || u > 0, lead);
-      }
-      commit(full, lead);
-      commit(kempty + 8 * (kt % kAhead), lead);
-    };
-    auto next_keys = [&] {
-      kt++;
-      kn += chunks;
-      if (kn >= KU) kn -= KU;
-    };
-    auto values_there = [&](const bool masked) {
-      uint32_t at = vn;
+                for (int c = 0; c < DK / 64; c++)
 #pragma unroll
-      for (int u = 0; u < kTile / VK; u++) {
-        if (!wait_warp((masked ? vok : vfull) + 8 * at, (masked ? vpar[1] : vpar[0]) >> at & 1, P.status)) return false;
-        if (masked) vpar[1] ^= 1u << at; else vpar[0] ^= 1u << at;
-        if (++at == VU) at = 0;
-      }
-      return true;
-    };
-    auto results = [&](uint32_t weights, uint32_t to, uint32_t full, uint32_t parity, int n, const bool add, uint32_t done) {
+                  for (int u = 0; u < 4; u++) mma_ss(s_at + place * W, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + 2 * u, sdesc, c > 0 || u > 0, lead);
+              } else {
 #pragma unroll
-      for (int u = 0; u < kTile / 16; u++) {
-        if (u % 4 == 0) {
-          if (!wait_warp(full + (u / 4) * 8, parity, P.status)) return false;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        }
-        if (u < n) mma_ts(to, weights + u * 8, value_desc(vs + vn * kUnit, VK) + (u % STEPS) * 128, pdesc, add || u > 0, lead);
-        if (u == kTile / 16 - 1) commit(done, lead);
-        if (u % STEPS == STEPS - 1) {
-          if (TILES == 2 && u == kTile / 16 - 1) pend = vn;  // (given back behind the next scores, which wait for this product and not for that)
-          else commit(vempty + 8 * vn, lead);
-          if (++vn == VU) vn = 0;
-        }
-      }
-      return true;
-    };
-    Item w;
-    bool alive = true;
-    while (alive && take(w)) {
-      const Walk k = walk_of(P, w, tokens);
-      const int a = w.tok + (TILES == 2 ? t * P.tokens : 0), b = min(a + (TILES == 2 ? P.tokens : tokens), w.len) - 1;
-      const bool there = a < w.len;
-      bool any = false;
-      if (TILES == 2) {
-        alive = (!there || wait_warp(qfull + 8 * t, took & 1, P.status)) && keys_there();
-        for (int i = 0; i < k.n && alive; i++) {
-          const int key0 = key_of(k, i), n = min(8, (b - key0 + 16) / 16);
-          const bool mine = there && sees_some(P, a, b, key0), masked = !sees_all(P, w.tok, k.t1 - 1, key0);
+                for (int c = 0; c < DK / 64; c++)
+#pragma unroll
+                  for (int u = 0; u < 4; u++) if (4 * c + u < ksteps) mma_ss(s_at + place * W, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + 2 * u, sdesc, c > 0 || u > 0, lead);
+              }
+              commit(sfull + 16 * t + 8 * place, lead);
+              sent++;
+            }
+            if (q_step % PER == PER - 1) {                   // (a commit stands for all products ahead of it)
+              if (there) commit(kempty + 8 * (kt % kAhead), lead);
+              else if (lead) hy::tc_arrive(kempty + 8 * (kt % kAhead));
+              kt++;
+              kn += chunks;
+              if (kn >= KU) kn -= KU;
+            }
+            q_step++;
+            if (q_step == last && there) commit(qempty + 8 * t, lead);
+          }
+          return true;
+        };
+        auto results = [&]() {                               // of the next step
+          const int key0 = key_at(v_step);
+          const bool mine = is_mine(v_step), masked = !sees_all(P, w.tok, k.t1 - 1, key0 - v_step % PER * W, kTile);
+          const uint32_t place = done & 1, weights = s_at + place * W;
+          const int n = min(W / 16, (b - key0 + 16) / 16);
+          constexpr int UNITS = W >= VK ? W / VK : 1, EACH = W >= VK ? 1 : VK / W;   // units of a step, or steps of a unit
+          uint64_t v_desc[UNITS];
+#pragma unroll
+          for (int u = 0; u < UNITS; u++) {
+            const uint32_t at = vn + u < VU ? vn + u : vn + u - VU;
+            if (EACH == 1 || v_step % EACH == 0) {
+              if (!wait_warp((masked ? vok : vfull) + 8 * at, (masked ? vpar[1] : vpar[0]) >> at & 1, P.status)) return false;
+              if (masked) vpar[1] ^= 1u << at; else vpar[0] ^= 1u << at;
+            }
+            v_desc[u] = value_desc(vs + at * kUnit + (EACH == 1 ? 0 : v_step % EACH * (W * 128)), VK);
+          }
           if (mine) {
-            if (passed) alive = wait_warp(pvdone + 8 * t, (passed - 1) & 1, P.status);   // the weights are read: their columns may have the next scores
-            if (!alive) break;
-            scores(tmem + t * 128, n, sfull + 8 * t);
-          } else if (lead) hy::tc_arrive(kempty + 8 * (kt % kAhead));
-          if (pend >= 0) { commit(vempty + 8 * pend, lead); pend = -1; }
-          next_keys();
-          if (i + 1 < k.n) alive = keys_there();
-          else if (there) commit(qempty + 8 * t, lead);
-          alive = alive && values_there(masked);
-          if (!alive) break;
-          if (mine) {
-            alive = results(tmem + t * 128, o_at + t * 128, pfull + 16 * t, passed & 1, n, any, pvdone + 8 * t);
-            passed++;
+            if (!wait_warp(pfull + 16 * t + 8 * place, (done >> 1) & 1, P.status)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (n == W / 16) {
+#pragma unroll
+              for (int u = 0; u < W / 16; u++) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
+            } else {
+#pragma unroll
+              for (int u = 0; u < W / 16; u++) if (u < n) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
+            }
+            commit(pvdone + 16 * t + 8 * place, lead);
+            done++;
             any = true;
-          } else {
+          }
+          if (EACH == 1 || v_step % EACH == EACH - 1) {
 #pragma unroll
-            for (int u = 0; u < kTile / VK; u++) {
-              if (lead) hy::tc_arrive(vempty + 8 * vn);
+            for (int u = 0; u < UNITS; u++) {
+              if (there) commit(vempty + 8 * vn, lead);
+              else if (lead) hy::tc_arrive(vempty + 8 * vn);
               if (++vn == VU) vn = 0;
             }
           }
-        }
+          v_step++;
+          return true;
+        };
+        alive = !there || wait_warp(qfull + 8 * t, took & 1, P.status);
+        while (alive && v_step < last) alive = ahead() && results();
         if (there && alive) { commit(odone + 8 * t, lead); took++; }
-        if (pend >= 0) { commit(vempty + 8 * pend, lead); pend = -1; }
-      } else if (t == 0) {                                   // scores lie in two places in turn
-        alive = wait_warp(qfull, took & 1, P.status);
-        for (int i = 0; i < k.n && alive; i++, passed++) {
-          const uint32_t s = passed & 1;
-          alive = keys_there() && (passed < 2 || wait_warp(pvdone + 8 * s, ((passed >> 1) - 1) & 1, P.status));
-          if (!alive) break;
-          scores(tmem + s * 128, min(8, (b - key_of(k, i) + 16) / 16), sfull + 8 * s);
-          next_keys();
-        }
-        if (alive) { commit(qempty, lead); took++; }
-      } else {
-        for (int i = 0; i < k.n && alive; i++, passed++) {
-          const uint32_t s = passed & 1;
-          const int key0 = key_of(k, i);
-          alive = values_there(!sees_all(P, w.tok, k.t1 - 1, key0)) && results(tmem + s * 128, o_at, pfull + 16 * s, (passed >> 1) & 1, min(8, (b - key0 + 16) / 16), i > 0, pvdone + 8 * s);
-        }
-        if (alive) commit(odone, lead);
       }
-    }
-    commit(flushed + 8 * t, lead);                           // no product is under way when TMEM is given back
-    wait_warp(flushed + 8 * t, 0, P.status);
-  } else if (warp == 10 || warp == 11) {                     // copies: keys and queries, values
-    Item w;
-    const int chunks = (P.dk + 63) / 64, boxes = (P.dv + 63) / 64;
-    uint32_t n = 0, par = 0, took[2] = {0, 0}, vpar[2] = {0, 0}, vsent[2] = {0, 0};
-    int tile = 0, freed = 0, sent = 0;                       // tiles of keys begun and given back, units sent
-    bool alive = true;
-    auto keys = [&](const Item& w, int key0, int head) {
-      for (int c = 0; c < chunks; c++) {
-        while (freed + kAhead <= tile || freed * chunks + KU <= sent) {   // the barrier's last tile, and the unit that lies where this one goes
-          alive = wait_warp(kempty + 8 * (freed % kAhead), (freed / kAhead) & 1, P.status);
-          if (!alive) return;
-          freed++;
-        }
-        if (lane == 0) {
-          if (c == 0) mbar_expect_tx(kfull + 8 * (tile % kAhead), chunks * kUnit);
-          copy_box(ks + n * kUnit, &P.k, 64 * c, head, w.row + key0, kfull + 8 * (tile % kAhead));
-        }
-        sent++;
-        if (++n == KU) n = 0;
-      }
-      tile++;
-    };
-    if (warp == 10) {
-      while (alive && take(w)) {
-        const Walk k = walk_of(P, w, tokens);
-        const int head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack;
-        keys(w, key_of(k, 0), head);
-        for (int t = 0; t < TILES && alive; t++) {
-          if (w.tok + t * P.tokens >= w.len) continue;
-          alive = wait_warp(qempty + 8 * t, (took[t] & 1) ^ 1, P.status);
-          if (!alive) break;
-          if (lane == 0) {
-            mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
-            for (int c = 0; c < chunks; c++) copy_box(qs + t * (kTile * DK * 2) + c * (kTile * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
+      commit(flushed + 8 * t, lead);                         // no product is under way when TMEM is given back
+      wait_warp(flushed + 8 * t, 0, P.status);
+    } else if (warp == 10 || warp == 11) {                   // copies: keys and queries, values
+      Item w;
+      const int chunks = (P.dk + 63) / 64, boxes = (P.dv + 63) / 64;
+      uint32_t n = 0, par = 0, took[2] = {0, 0}, vpar[2] = {0, 0}, vsent[2] = {0, 0};
+      int tile = 0, freed = 0, sent = 0;                     // tiles of keys begun and given back, units sent
+      bool alive = true;
+      auto keys = [&](const Item& w, int key0, int head) {
+        for (int c = 0; c < chunks; c++) {
+          while (freed + kAhead <= tile || freed * chunks + KU <= sent) {   // the barrier's last tile, and the unit that lies where this one goes
+            alive = wait_warp(kempty + 8 * (freed % kAhead), (freed / kAhead) & 1, P.status);
+            if (!alive) return;
+            freed++;
           }
-          took[t]++;
+          if (lane == 0) {
+            if (c == 0) mbar_expect_tx(kfull + 8 * (tile % kAhead), chunks * kUnit);
+            copy_box(ks + n * kUnit, &P.k, 64 * c, head, w.row + key0, kfull + 8 * (tile % kAhead));
+          }
+          sent++;
+          if (++n == KU) n = 0;
         }
-        for (int i = 1; i < k.n && alive; i++) keys(w, key_of(k, i), head);
-      }
-      for (int t = 0; t < TILES; t++) if (took[t]) wait_warp(qfull + 8 * t, (took[t] - 1) & 1, P.status);   // no copy is under way at the end, whatever happened
-      for (int s = max(0, tile - kAhead); s < tile; s++) wait_warp(kfull + 8 * (s % kAhead), (s / kAhead) & 1, P.status);
-    } else {
-      while (alive && take(w)) {
-        const Walk k = walk_of(P, w, tokens);
-        const int head = w.unit / P.subs;
-        for (int i = 0; i < k.n && alive; i++) {
-          const int key0 = key_of(k, i);
-          const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0);
-          const uint32_t full = masked ? vraw : vfull;
-          for (int u = 0; u < kTile / VK && alive; u++) {
-            alive = wait_warp(vempty + 8 * n, par ^ 1, P.status);
+        tile++;
+      };
+      if (warp == 10) {
+        while (alive && take(w)) {
+          const Walk k = walk_of(P, w, tokens);
+          const int head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack;
+          keys(w, key_of(k, 0), head);
+          if (k.n <= kEarly && lane == 0) hy::tc_arrive(want);
+          for (int t = 0; t < TILES && alive; t++) {
+            if (w.tok + t * P.tokens >= w.len) continue;
+            alive = wait_warp(qempty + 8 * t, (took[t] & 1) ^ 1, P.status);
             if (!alive) break;
             if (lane == 0) {
-              mbar_expect_tx(full + 8 * n, boxes * VK * 128);
-              for (int c = 0; c < boxes; c++) copy_box(vs + n * kUnit + c * (VK * 128), &P.v, 64 * c, head, w.row + key0 + u * VK, full + 8 * n);
+              mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
+              for (int c = 0; c < chunks; c++) copy_box(qs + t * (kTile * DK * 2) + c * (kTile * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
             }
-            vpar[masked] ^= 1u << n;
-            vsent[masked] |= 1u << n;
-            if (++n == VU) { n = 0; par ^= 1; }
+            took[t]++;
+          }
+          for (int i = 1; i < k.n && alive; i++) {
+            if (i == k.n - kEarly && lane == 0) hy::tc_arrive(want);
+            keys(w, key_of(k, i), head);
+          }
+        }
+        for (int t = 0; t < TILES; t++) if (took[t]) wait_warp(qfull + 8 * t, (took[t] - 1) & 1, P.status);   // no copy is under way at the end, whatever happened
+        for (int s = max(0, tile - kAhead); s < tile; s++) wait_warp(kfull + 8 * (s % kAhead), (s / kAhead) & 1, P.status);
+      } else {
+        while (alive && take(w)) {
+          const Walk k = walk_of(P, w, tokens);
+          const int head = w.unit / P.subs;
+          for (int i = 0; i < k.n && alive; i++) {
+            const int key0 = key_of(k, i);
+            const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0, kTile);
+            const uint32_t full = masked ? vraw : vfull;
+            for (int u = 0; u < kTile / VK && alive; u++) {
+              alive = wait_warp(vempty + 8 * n, par ^ 1, P.status);
+              if (!alive) break;
+              if (lane == 0) {
+                mbar_expect_tx(full + 8 * n, boxes * VK * 128);
+                for (int c = 0; c < boxes; c++) copy_box(vs + n * kUnit + c * (VK * 128), &P.v, 64 * c, head, w.row + key0 + u * VK, full + 8 * n);
+              }
+              vpar[masked] ^= 1u << n;
+              vsent[masked] |= 1u << n;
+              if (++n == VU) { n = 0; par ^= 1; }
+            }
+          }
+        }
+        for (uint32_t s = 0; s < 2 * VU; s++)                // no copy is under way at the end, whatever happened
+          if (vsent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
+      }
+    } else if (warp == 15) {                                 // deals out the work: rows with most keys first, so that the short ones fill the gaps
+      // CTAs take over work of CTAs that have not started yet, each when its copies near the end of what it has
+      long long at = blockIdx.x;
+      for (uint32_t round = 0;; round++) {
+        int4 item = make_int4(0, 0, 0, 0);
+        const int k = (int)(at / P.units);
+        if (at < all) {
+          int lo = 0, hi = most - 1;                         // the level j with from_level(j + 1) <= k < from_level(j)
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (from_level(mid) > k) lo = mid; else hi = mid - 1;
+          }
+          most = lo + 1;                                     // (later ones lie no higher)
+          int rank = k - from_level(lo + 1), b = -1;
+          for (int c = 0; b < 0 && c < P.batch; c += 32) {
+            const bool has = tiles_of(c + lane) > lo;
+            const uint32_t mask = __ballot_sync(0xffffffffu, has);
+            const uint32_t hit = __ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1)) == rank);
+            if (hit) b = c + __ffs(hit) - 1;
+            rank -= __popc(mask);
+          }
+          if (b >= 0) {
+            const int from = min(max(P.starts[b], 0), P.rows), to = min(max(P.starts[b + 1], from), P.rows);
+            item = make_int4(from, to - from, lo * tokens, (int)(at - (long long)k * P.units));
+          }
+        }
+        const uint32_t slot = round & 1;
+        if (!wait_warp(iempty + 8 * slot, (round >> 1 & 1) ^ 1, P.status)) break;
+        if (lane == 0) { items[slot] = item; hy::tc_arrive(ifull + 8 * slot); }
+        if (item.y <= 0 || !wait_warp(want, round & 1, P.status)) break;
+        if (lane == 0) {
+          mbar_expect_tx(claimed, 16);
+          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(&claim)), "r"(claimed) : "memory");
+        }
+        if (!wait_warp(claimed, round & 1, P.status)) break;
+        uint32_t got, next;
+        asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%2];\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                     "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}" : "=r"(got), "=r"(next) : "r"(smem_u32(&claim)) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (read ahead of the next claim's write)
+        __syncwarp();
+        at = got ? (long long)next : all;
+      }
+    } else if (warp >= 12) {                                 // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
+      Item w;
+      const int me = threadIdx.x - 12 * 32, boxes = (P.dv + 63) / 64;
+      const uint32_t inf = BF16 ? 0x7f807f80u : 0x7c007c00u;
+      uint32_t n = 0, par = 0;                               // par: a bit for each place
+      bool alive = true;
+      while (alive && take(w)) {
+        const Walk k = walk_of(P, w, tokens);
+        for (int i = 0; i < k.n && alive; i++) {
+          const int key0 = key_of(k, i);
+          const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0, kTile);
+          for (int u = 0; u < kTile / VK && alive; u++) {
+            if (masked) {
+              alive = wait_warp(vraw + 8 * n, par >> n & 1, P.status);
+              par ^= 1u << n;
+              const int first = key0 + u * VK;
+              bool odd = false;
+              for (int p = me; p < boxes * VK * 8; p += 96) {  // 16-byte pieces: eight to a row of 64 columns
+                const int row = first + ((p >> 3) & (VK - 1));
+                const uint32_t at = vs + n * kUnit + p * 16;
+                const uint4 x = lds128(at);
+                uint32_t y[4] = {x.x, x.y, x.z, x.w}, z[4], hit = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) { z[e] = row < w.len ? __vcmpeq2(y[e] & inf, inf) : 0xffffffffu; hit |= z[e]; y[e] &= ~z[e]; }
+                if (hit) { sts128(at, y[0], y[1], y[2], y[3]); odd |= row < w.len; }
+              }
+              if (odd) odd_values = 1;
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) hy::tc_arrive(vok + 8 * n);
+            }
+            if (++n == VU) n = 0;
           }
         }
       }
-      for (uint32_t s = 0; s < 2 * VU; s++)                  // no copy is under way at the end, whatever happened
-        if (vsent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
     }
-  } else if (warp == 15) {                                   // deals out the work: rows with most keys first, so that the short ones fill the gaps
-    int held[kHeld];                                         // row tiles of sequences lane, lane + 32, ..
-    auto tiles_of = [&](int b) {
-      if (b >= P.batch) return 0;
-      const int from = min(max(P.starts[b], 0), P.rows), to = min(max(P.starts[b + 1], from), P.rows);
-      return (to - from + tokens - 1) / tokens;
-    };
-    int most = 0;
-#pragma unroll
-    for (int i = 0; i < kHeld; i++) { held[i] = tiles_of(lane + 32 * i); most = max(most, held[i]); }
-    for (int b = lane + 32 * kHeld; b < P.batch; b += 32) most = max(most, tiles_of(b));
-    most = __reduce_max_sync(0xffffffffu, most);
-    auto from_level = [&](int j) {                           // row tiles that are the j-th or a later one of their sequence
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kHeld; i++) n += max(held[i] - j, 0);
-      for (int b = lane + 32 * kHeld; b < P.batch; b += 32) n += max(tiles_of(b) - j, 0);
-      return __reduce_add_sync(0xffffffffu, n);
-    };
-    const int all = from_level(0);
-    uint32_t par = 0, round = 0;
-    for (long long at = blockIdx.x;; at += gridDim.x, round++) {
-      int4 item = make_int4(0, 0, 0, 0);
-      const int k = (int)(at / P.units);
-      if (at < (long long)all * P.units) {
-        int lo = 0, hi = most - 1;                           // the level j with from_level(j + 1) <= k < from_level(j)
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (from_level(mid) > k) lo = mid; else hi = mid - 1;
-        }
-        most = lo + 1;                                       // (later ones lie no higher)
-        int rank = k - from_level(lo + 1), b = -1;
-        for (int c = 0; b < 0 && c < P.batch; c += 32) {
-          bool has = tiles_of(c + lane) > lo;
-          const uint32_t mask = __ballot_sync(0xffffffffu, has);
-          const uint32_t hit = __ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1)) == rank);
-          if (hit) b = c + __ffs(hit) - 1;
-          rank -= __popc(mask);
-        }
-        if (b >= 0) {
-          const int from = min(max(P.starts[b], 0), P.rows), to = min(max(P.starts[b + 1], from), P.rows);
-          item = make_int4(from, to - from, lo * tokens, (int)(at - (long long)k * P.units));
-        }
-      }
-      const uint32_t slot = round & 1;
-      if (!wait_warp(iempty + 8 * slot, par ^ 1, P.status)) break;
-      if (lane == 0) { items[slot] = item; hy::tc_arrive(ifull + 8 * slot); }
-      if (slot) par ^= 1;
-      if (item.y <= 0) break;
-    }
-  } else {                                                   // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
-    Item w;
-    const int me = threadIdx.x - 12 * 32, boxes = (P.dv + 63) / 64;
-    const uint32_t inf = BF16 ? 0x7f807f80u : 0x7c007c00u;
-    uint32_t n = 0, par = 0;                                 // par: a bit for each place
-    bool alive = true;
-    while (alive && take(w)) {
-      const Walk k = walk_of(P, w, tokens);
-      for (int i = 0; i < k.n && alive; i++) {
-        const int key0 = key_of(k, i);
-        const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0);
-        for (int u = 0; u < kTile / VK && alive; u++) {
-          if (masked) {
-            alive = wait_warp(vraw + 8 * n, par >> n & 1, P.status);
-            par ^= 1u << n;
-            const int first = key0 + u * VK;
-            bool odd = false;
-            for (int p = me; p < boxes * VK * 8; p += 96) {  // 16-byte pieces: eight to a row of 64 columns
-              const int row = first + ((p >> 3) & (VK - 1));
-              const uint32_t at = vs + n * kUnit + p * 16;
-              const uint4 x = lds128(at);
-              uint32_t y[4] = {x.x, x.y, x.z, x.w}, z[4], hit = 0;
-#pragma unroll
-              for (int e = 0; e < 4; e++) { z[e] = row < w.len ? __vcmpeq2(y[e] & inf, inf) : 0xffffffffu; hit |= z[e]; y[e] &= ~z[e]; }
-              if (hit) { sts128(at, y[0], y[1], y[2], y[3]); odd |= row < w.len; }
-            }
-            if (odd) odd_values = 1;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) hy::tc_arrive(vok + 8 * n);
-          }
-          if (++n == VU) n = 0;
-        }
-      }
-    }
-  }
   } else if (warp < SOFT) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MANY));
     const int t = warp >> 2, quad = warp & 3, r = threadIdx.x & 127, tok_of = r / P.pack;       // the thread's row: token tok_of of the tile, head r % pack
     const bool exists = r < P.tokens * P.pack;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, res = o_at + t * 128 + lanes;
-    uint32_t passed = 0, took = 0, gated = 0;                // gated: tiles that both groups have
+    uint32_t passed = 0, took = 0;
     Item w;
     bool ok = true;
     while (ok && take(w)) {
-      const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1, other = w.tok + (t ^ 1) * P.tokens;
+      const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
       if (a >= w.len) continue;
       const Walk k = walk_of(P, w, tokens);
       const int pos = exists ? a + tok_of : 0x3fffffff;
       const bool mine = pos < w.len, idle = !__any_sync(0xffffffffu, mine);
       float m = kLowest, l = 0.f, limit = -INFINITY;         // limit: where a maximum moves the reference; any does while that is beyond kFar
       bool any = false;
-      for (int i = 0; i < k.n; i++) {
-        const int key0 = key_of(k, i);
-        if (!sees_some(P, a, b, key0)) continue;
-        const uint32_t buf = TILES == 2 ? t : passed & 1, par = TILES == 2 ? passed & 1 : (passed >> 1) & 1, s_at = tmem + buf * 128 + lanes;
-        const bool masked = !sees_all(P, a, b, key0);
-        // The two groups' exponentials take turns: one's products then run under the other's, where both at a time would wait for the exponentials' pipe and leave the tensor pipe idle
-        const bool gate = TILES == 2 && other < w.len && sees_some(P, other, min(other + P.tokens, w.len) - 1, key0);
-        const uint32_t turn_of = turns + 8 * t, turn_par = (gated - 1 + t) & 1;
-        ok = wait_warp(sfull + 8 * buf, par, P.status);
+      for (int step = 0; step < k.n * PER; step++) {
+        const int key0 = key_of(k, step / PER) + step % PER * W;
+        if (!sees_some(P, a, b, key0, W)) continue;
+        const uint32_t place = passed & 1, s_at = tmem + t * 128 + place * W + lanes, p_bar = pfull + 16 * t + 8 * place;
+        const bool masked = !sees_all(P, a, b, key0, W);
+        ok = wait_warp(sfull + 16 * t + 8 * place, (passed >> 1) & 1, P.status);
         if (!ok) break;
         if (idle) {                                          // (its rows' results are whatever comes of the scores as weights, and go nowhere)
           __syncwarp();
-          if (lane < 2) hy::tc_arrive(pfull + 16 * buf + 8 * lane);
-          if (gate) { if (lane == 0) hy::tc_arrive(turns + 8 * (t ^ 1)); gated++; }
+          if (lane == 0) hy::tc_arrive(p_bar);
           passed++;
-          any = true;
           continue;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const bool go = !gate || gated + t == 0 || hy::tc_poll(turn_of, turn_par);   // (asked ahead of the maxima, which the answer then comes under)
-        uint32_t x[128];                                     // the whole row: its weights then lie where the scores were
-        tmem_row(s_at, x);
+        uint32_t x[W];
+        tmem_ask<0, W>(s_at, x);
+        tmem_got<0, W>(x);
         if (masked) {                                        // keys that the row sees, a bit each: not behind its own, in the window or among the first
 #pragma unroll
-          for (int u = 0; u < 128; u += 32) {
+          for (int u = 0; u < W; u += 32) {
             const int j = key0 + u;
             uint32_t see = lower_bits(pos + 1 - j);
             if (P.window > 0) see &= ~lower_bits(pos - P.window + 1 - j) | lower_bits(P.keep - j);
@@ -468,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         }
         float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 128; e += 8)
+        for (int e = 0; e < W; e += 8)
 #pragma unroll
           for (int g = 0; g < 4; g++) y[g] = max3(__float_as_uint(y[g]), x[e + 2 * g], x[e + 2 * g + 1]);
         const float top = mine ? fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * P.f : -INFINITY;
@@ -481,12 +489,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
           limit = far ? -INFINITY : m + ROOM;
           if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
-            for (int e = 0; e < 128; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+            for (int e = 0; e < W; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
             f = 1.f;
           }
-          if (any) {                                         // (two row tiles: the last product was through ahead of these scores)
-            // A wait by parity is right while the barrier is in the phase asked for or the one behind it: these scores waited for the product before the one ahead
-            if (TILES == 1) ok = wait_warp(pvdone + 8 * (buf ^ 1), ((passed - 1) >> 1) & 1, P.status);
+          if (any) {
+            // The product ahead must be through.  A wait by parity is right while the barrier is in the phase asked for or the one behind it: these scores waited for the product before that one
+            ok = wait_warp(pvdone + 16 * t + 8 * (place ^ 1), ((passed - 1) >> 1) & 1, P.status);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int d = 0; d < P.dv; d += 16) {
@@ -498,11 +506,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             }
           }
         }
-        if (!__all_sync(0xffffffffu, go)) ok = wait_warp(turn_of, turn_par, P.status) && ok;
         const uint64_t f2 = both(f, f), off = both(-m, -m);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < W / 32; u++) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) {
@@ -513,24 +520,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             add2(sum[e & 1], y0, y1);
             p[e] = pair<BF16>(y0, y1);
           }
-          if (u == 3 && gate) {
-            __syncwarp();
-            if (lane == 0) hy::tc_arrive(turns + 8 * (t ^ 1));
-            gated++;
-          }
           tmem_store16(s_at + 16 * u, p);
-          if (u & 1) {                                       // a half of the weights: its product starts
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) hy::tc_arrive(pfull + 16 * buf + 8 * (u >> 1));
-          }
         }
         l += (__uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32))) + (__uint_as_float((uint32_t)sum[1]) + __uint_as_float((uint32_t)(sum[1] >> 32)));
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) hy::tc_arrive(p_bar);
         passed++;
         any = true;
       }
-      ok = ok && wait_warp(odone + 8 * (TILES == 2 ? t : 0), took & 1, P.status);
+      ok = ok && wait_warp(odone + 8 * t, took & 1, P.status);
       took++;
       if (!ok || idle) continue;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

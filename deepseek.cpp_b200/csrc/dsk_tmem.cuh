@@ -38,12 +38,15 @@ __device__ __forceinline__ void tmem_read16(uint32_t addr, uint32_t (&r)[16]) { 
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
 }
-template <int N> __device__ __forceinline__ void tmem_row(uint32_t addr, uint32_t (&r)[N]) {   // N columns, 32 at a time; loaded when it returns
+// columns A .. B - 1 of a row, 32 at a time: asked for, and loaded
+template <int A, int B, int N> __device__ __forceinline__ void tmem_ask(uint32_t addr, uint32_t (&r)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 32) hy::tc_load32(addr + i, *reinterpret_cast<uint32_t(*)[32]>(&r[i]));
+  for (int i = A; i < B; i += 32) hy::tc_load32(addr + i, *reinterpret_cast<uint32_t(*)[32]>(&r[i]));
+}
+template <int A, int B, int N> __device__ __forceinline__ void tmem_got(uint32_t (&r)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));   // (no use ahead of the wait)
+  for (int i = A; i < B; i++) asm volatile("" : "+r"(r[i]));   // (no use ahead of the wait)
 }
 // two fp32 operations at a time
 __device__ __forceinline__ uint64_t both(float a, float b) {
@@ -54,12 +57,22 @@ __device__ __forceinline__ uint64_t both(float a, float b) {
 __device__ __forceinline__ void fma2(uint32_t x0, uint32_t x1, uint64_t f, uint64_t a, float& y0, float& y1) {
   asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%2, %3};\n\tfma.rn.f32x2 x, x, %4, %5;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(y0), "=f"(y1) : "r"(x0), "r"(x1), "l"(f), "l"(a));
 }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t f, uint64_t a) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(f), "l"(a));
+  return r;
+}
 __device__ __forceinline__ void add2(uint64_t& s, float y0, float y1) {
   asm("{\n\t.reg .b64 y;\n\tmov.b64 y, {%1, %2};\n\tadd.rn.f32x2 %0, %0, y;\n\t}" : "+l"(s) : "f"(y0), "f"(y1));
 }
 __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, uint32_t b, uint32_t c) {   // NaN where one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
   return r;
 }
 // Products and commits of one lane of a warp whose lanes all run the same code: descriptors then stay in uniform registers, where a branch to that lane would have them copied there

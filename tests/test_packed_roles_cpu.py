@@ -20,22 +20,23 @@ class Bar:
         return lambda: (self.phase & 1) != parity & 1
 
 
-AHEAD = 4                                                    # tiles of keys under way
+AHEAD, EARLY = 4, 4                                          # tiles of keys under way, tiles ahead of the end at which more work is asked for
 SHAPES = {64: (2, 1, 1, 6, 5), 128: (2, 2, 2, 6, 4), 192: (2, 3, 2, 5, 3), 256: (1, 4, 4, 6, 4)}      # row tiles, units of keys and of values a tile, places for them
 
 
 def run(rng, dk, work, idle, moves, early=True):
-    """work: items, each a list of (tiles of keys: (row tiles that see some of it, whether some row does not see all)) and whether the second row tile has rows.  idle: softmax warps without
-    rows; early: the wait for the product ahead, where a reference moves with one row tile."""
+    """work: items, each a list of (tiles of keys: (for each of its steps, the row tiles that see some of it; whether some row does not see all)) and whether the second row tile has rows.  idle:
+    softmax warps without rows; early: the wait for the product ahead, where a reference moves."""
     tiles, per_k, per_v, KU, VU = SHAPES[dk]
     bars = lambda n, count: [Bar(count) for _ in range(n)]
-    soft = 4 * tiles
+    soft, per = 4 * tiles, tiles                             # steps of a tile: two with two row tiles, of half as many keys
     kfull, kempty, vfull, vempty, vok, vraw = bars(AHEAD, 1), bars(AHEAD, tiles), bars(VU, 1), bars(VU, tiles), bars(VU, 3), bars(VU, 1)
-    qfull, qempty, sfull, pvdone, odone, ifull, turns = *(bars(2, 1) for _ in range(6)), bars(2, 4)
-    pfull, iempty, flushed = [bars(2, 4) for _ in range(2)], bars(2, soft + 7), bars(2, 1)
-    items = [None, None]
+    qfull, qempty, odone, ifull = (bars(2, 1) for _ in range(4))
+    sfull, pvdone, pfull = ([bars(2, n) for _ in range(2)] for n in (1, 1, 4))            # [row tile][place]
+    iempty, flushed = bars(2, soft + tiles + 5), bars(2, 1)
+    items, want = [None, None], Bar(1)
     keys, values, queries, looked = [None] * KU, [None] * VU, [None] * 2, [0] * VU
-    scores, weights, through = [None, None], [[{}, {}], [{}, {}]], [None, None]
+    scores, weights, through = [[None, None], [None, None]], [[{}, {}], [{}, {}]], [[], []]       # [row tile][place], steps whose product is through
     queue, flying = [], []                                   # products and commits in the order of their issue; copies in any order
 
     def take(state):
@@ -47,13 +48,13 @@ def run(rng, dk, work, idle, moves, early=True):
         state["turn"] += 1
 
     def deal():
-        par = 0
         for r, n in enumerate(list(range(len(work))) + [None]):
-            yield iempty[r & 1].wait(par ^ 1)
+            yield iempty[r & 1].wait((r >> 1) ^ 1)
             items[r & 1] = n
             ifull[r & 1].arrive()
-            if r & 1:
-                par ^= 1
+            if n is not None:
+                yield want.wait(r)
+                yield None                                   # (the claim)
 
     def copy_keys():
         me, took = {"turn": 0}, [0, 0]
@@ -78,6 +79,8 @@ def run(rng, dk, work, idle, moves, early=True):
                 at["tile"] += 1
 
             yield from tile(0)
+            if len(walk) <= EARLY:
+                want.arrive()
             for t in range(tiles):
                 if t and not two:
                     continue
@@ -86,6 +89,8 @@ def run(rng, dk, work, idle, moves, early=True):
                 queries[t] = "under way"
                 took[t] += 1
             for i in range(1, len(walk)):
+                if i == len(walk) - EARLY:
+                    want.arrive()
                 yield from tile(i)
 
     def copy_values():
@@ -119,129 +124,86 @@ def run(rng, dk, work, idle, moves, early=True):
                         vok[n].arrive()
                     n = (n + 1) % VU
 
-    def product_of_scores(t, n, i, c, place, buf):
+    def product_of_scores(t, n, step, c, place, at):
         def product():
-            assert keys[place] == (n, i, c) and queries[t] == n
+            assert keys[place] == (n, step // per, c) and queries[t] == n
             if c == 0:
-                if scores[buf] is not None:                  # what lay there was handed over and read
-                    assert through[buf if tiles == 1 else t] == scores[buf]
-                scores[buf], weights[buf] = None, [{}, {}]
+                assert scores[t][at] is None or scores[t][at] in through[t]      # what lay there was handed over and read
+                scores[t][at], weights[t][at] = None, {}
             if c == per_k - 1:
-                scores[buf] = (n, i)
+                scores[t][at] = (n, step)
         return product
 
-    def product_of_results(t, n, i, c, place, buf, masked, half, last):
+    def product_of_results(t, n, step, units, at, masked):
         def product():
-            assert values[place] == (n, i, c) and (not masked or looked[place] == 3) and scores[buf] == (n, i)
-            for h in ([half] if half is not None else [0, 1]):
-                assert all(idle[n][4 * t + w] or weights[buf][h].get(w) == (n, i) for w in range(4))
-            if last:
-                through[buf if tiles == 1 else t] = (n, i)
+            assert all(values[place] == (n, step // per, c) and (not masked or looked[place] == 3) for c, place in units)
+            assert scores[t][at] == (n, step) and all(idle[n][4 * t + w] or weights[t][at].get(w) == (n, step) for w in range(4))
+            through[t].append((n, step))
         return product
 
-    def issue_scores(t, state, n, i, buf):
-        places = [(state["kn"] + c) % KU for c in range(per_k)]
-        queue.extend([product_of_scores(t, n, i, c, place, buf) for c, place in enumerate(places)] + [sfull[buf], kempty[state["kt"] % AHEAD]])
-
-    def next_keys(state):
-        state["kt"] += 1
-        state["kn"] = (state["kn"] + per_k) % KU
-
-    def keys_there(state):
-        return kfull[state["kt"] % AHEAD].wait(state["kt"] // AHEAD)
-
-    def values_there(state, masked):
-        for c in range(per_v):
-            place = (state["vn"] + c) % VU
-            yield (vok if masked else vfull)[place].wait(state["vpar"][masked][place])
-            state["vpar"][masked][place] ^= 1
-
-    def issue_results(t, state, n, i, buf, parity, masked):
-        steps = 8 // per_v
-        for u in range(8):
-            place = state["vn"]
-            if u % 4 == 0:
-                yield pfull[buf][u // 4].wait(parity)
-            if u % steps == steps - 1 or u == 3:
-                queue.append(product_of_results(t, n, i, u // steps, place, buf, masked, u // 4 if steps <= 4 else (0 if u == 3 else None), u == 7))
-                if u == 7:
-                    queue.append(pvdone[t if tiles == 2 else buf])
-            if u % steps == steps - 1:
-                if tiles == 2 and u == 7:
-                    state["pend"] = place
-                else:
-                    queue.append(vempty[place])
-                state["vn"] = (place + 1) % VU
-
-    def give_back(state):
-        if state["pend"] is not None:
-            queue.append(vempty[state["pend"]])
-            state["pend"] = None
-
-    def issuer(x):
-        me = {"turn": 0, "kt": 0, "kn": 0, "vn": 0, "vpar": [[0] * VU, [0] * VU], "pend": None}
-        passed = took = 0
+    def issuer(t):
+        me = {"turn": 0}
+        kt = kn = vn = sent = done = took = 0
+        vpar = [[0] * VU, [0] * VU]
+        units, each = max(1, per_v // per), max(1, per // per_v)                  # units of a step, steps of a unit
         while True:
             yield from take(me)
             n = me["item"]
             if n is None:
                 break
             walk, two = work[n]
-            if tiles == 2:
-                there = x == 0 or two
-                if there:
-                    yield qfull[x].wait(took)
-                yield keys_there(me)
-                for i, (who, masked) in enumerate(walk):
-                    mine = there and x in who
+            there, last, q = t == 0 or two, len(walk) * per, 0
+            if there:
+                yield qfull[t].wait(took)
+            for v in range(last):
+                while q < min(last, v + 2):
+                    mine = there and t in walk[q // per][0][q % per]
+                    if q % per == 0:
+                        yield kfull[kt % AHEAD].wait(kt // AHEAD)
                     if mine:
-                        if passed:
-                            yield pvdone[x].wait(passed - 1)
-                        issue_scores(x, me, n, i, x)
-                    else:
-                        kempty[me["kt"] % AHEAD].arrive()
-                    give_back(me)
-                    next_keys(me)
-                    if i + 1 < len(walk):
-                        yield keys_there(me)
-                    elif there:
-                        queue.append(qempty[x])
-                    yield from values_there(me, masked)
-                    if mine:
-                        yield from issue_results(x, me, n, i, x, passed, masked)
-                        passed += 1
-                    else:
-                        for _ in range(per_v):
-                            vempty[me["vn"]].arrive()
-                            me["vn"] = (me["vn"] + 1) % VU
-                if there:
-                    queue.append(odone[x])
-                    took += 1
-                give_back(me)
-            elif x == 0:
-                yield qfull[0].wait(took)
-                for i in range(len(walk)):
-                    yield keys_there(me)
-                    if passed > 1:
-                        yield pvdone[passed & 1].wait((passed >> 1) - 1)
-                    issue_scores(0, me, n, i, passed & 1)
-                    next_keys(me)
-                    passed += 1
-                queue.append(qempty[0])
+                        at = sent & 1
+                        if sent > 1:
+                            yield pvdone[t][at].wait((sent >> 1) - 1)
+                        queue.extend([product_of_scores(t, n, q, c, (kn + c) % KU, at) for c in range(per_k)] + [sfull[t][at]])
+                        sent += 1
+                    if q % per == per - 1:
+                        if there:
+                            queue.append(kempty[kt % AHEAD])
+                        else:
+                            kempty[kt % AHEAD].arrive()
+                        kt, kn = kt + 1, (kn + per_k) % KU
+                    q += 1
+                    if q == last and there:
+                        queue.append(qempty[t])
+                who, masked = walk[v // per]
+                mine, at = there and t in who[v % per], done & 1
+                places = [(vn + u) % VU for u in range(units)]
+                if v % each == 0:
+                    for place in places:
+                        yield (vok if masked else vfull)[place].wait(vpar[masked][place])
+                        vpar[masked][place] ^= 1
+                if mine:
+                    yield pfull[t][at].wait(done >> 1)
+                    first = v % per * units if each == 1 else 0
+                    queue.extend([product_of_results(t, n, v, [(first + u, place) for u, place in enumerate(places)], at, masked), pvdone[t][at]])
+                    done += 1
+                if v % each == each - 1:
+                    for place in places:
+                        if there:
+                            queue.append(vempty[place])
+                        else:
+                            vempty[place].arrive()
+                    vn = (vn + units) % VU
+            if there:
+                queue.append(odone[t])
                 took += 1
-            else:
-                for i, (_, masked) in enumerate(walk):
-                    yield from values_there(me, masked)
-                    yield from issue_results(0, me, n, i, passed & 1, passed >> 1, masked)
-                    passed += 1
-                queue.append(odone[0])
-        queue.append(flushed[x])
-        yield flushed[x].wait(0)
+        queue.append(flushed[t])
+        yield flushed[t].wait(0)
 
     def softmax(x):
         t, w = divmod(x, 4)
         me = {"turn": 0}
-        passed = took = gated = 0
+        passed = took = 0
         while True:
             yield from take(me)
             n = me["item"]
@@ -251,41 +213,33 @@ def run(rng, dk, work, idle, moves, early=True):
             if t and not two:
                 continue
             last = None
-            for i, (who, _) in enumerate(walk):
-                if t not in who:
+            for step in range(len(walk) * per):
+                if t not in walk[step // per][0][step % per]:
                     continue
-                buf, par = (t, passed) if tiles == 2 else (passed & 1, passed >> 1)
-                yield sfull[buf].wait(par)
+                at = passed & 1
+                yield sfull[t][at].wait(passed >> 1)
                 if not idle[n][x]:
-                    assert scores[buf] == (n, i)
+                    assert scores[t][at] == (n, step)
                     yield None
                     if last is not None and rng.random() < moves:     # results are scaled again
-                        if tiles == 1 and early:
-                            yield pvdone[buf ^ 1].wait((passed - 1) >> 1)
-                        assert through[buf ^ 1 if tiles == 1 else t] == last
+                        if early:
+                            yield pvdone[t][at ^ 1].wait((passed - 1) >> 1)
+                        assert through[t][-1:] == [last]
                         yield None
-                gate = len(who) == 2
-                if gate and not idle[n][x] and gated + t > 0:
-                    yield turns[t].wait(gated - 1 + t)
-                for half in (0, 1):
-                    if not idle[n][x]:
-                        assert scores[buf] == (n, i)
-                        weights[buf][half][w] = (n, i)
-                        yield None
-                    if half and gate:
-                        turns[t ^ 1].arrive()
-                        gated += 1
-                        yield None
-                    pfull[buf][half].arrive()
+                        assert through[t][-1:] == [last]
+                    assert scores[t][at] == (n, step)
+                    weights[t][at][w] = (n, step)
+                    yield None
+                pfull[t][at].arrive()
                 passed += 1
-                last = (n, i)
-            yield odone[t if tiles == 2 else 0].wait(took)
+                last = (n, step)
+            yield odone[t].wait(took)
             took += 1
             if not idle[n][x]:
-                assert through[t if tiles == 2 else (passed - 1) & 1] == last
+                assert through[t][-1:] == [last]
                 yield None
 
-    roles = [deal(), copy_keys(), copy_values(), issuer(0), issuer(1)] + [look(k) for k in range(3)] + [softmax(x) for x in range(soft)]
+    roles = [deal(), copy_keys(), copy_values(), *(issuer(t) for t in range(tiles))] + [look(k) for k in range(3)] + [softmax(x) for x in range(soft)]
     speed = [rng.choice([1, 1, 1, 10, 0.05]) for _ in roles] + [rng.choice([1, 0.1, 10]) for _ in range(2)]
     at = [next(r, False) for r in roles]                      # what a role waits for: a test, None, or False at its end
     while queue or flying or any(a is not False for a in at):
@@ -313,11 +267,8 @@ def draw(rng, dk):
     work, idle = [], []
     for _ in range(rng.randint(1, 5)):
         two = tiles == 2 and rng.random() < 0.8
-        walk = []
-        for _ in range(rng.randint(1, 6)):
-            who = {0} if not two else rng.choice([{0, 1}, {0, 1}, {0}, {1}])
-            walk.append((who, rng.random() < 0.4))
-        walk[0] = ({0, 1} if two else {0}, walk[0][1])       # (a row tile that has rows sees some tile)
+        walk = [([{0} if not two else rng.choice([{0, 1}, {0, 1}, {0, 1}, {0}, {1}, set()]) for _ in range(tiles)], rng.random() < 0.4) for _ in range(rng.randint(1, 7))]
+        walk[0][0][0] = {0, 1} if two else {0}               # (a row tile that has rows sees something)
         work.append((walk, two))
         row = [rng.random() < 0.2 for _ in range(4 * tiles)]
         row[0] = False                                       # (a row tile that has rows has its first)
@@ -335,7 +286,7 @@ def test_roles_meet_in_every_order(dk):
 
 
 def test_the_wait_for_the_product_ahead_is_needed():
-    """The check itself sees what it is for: without that wait, results of one row tile are scaled while a product adds to them."""
+    """The check itself sees what it is for: without that wait, results are scaled while a product adds to them."""
     rng, found = random.Random(5), 0
     for _ in range(400):
         try:

@@ -107,7 +107,7 @@ template <bool BF16> __device__ __noinline__ void give_back(const Params& P, con
 
 template <int DK, int DV, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_constant__ Params P) {
-  constexpr int TILES = tiles<DK, DV>(), KU = k_units<DK, DV>(), VU = v_units<DK, DV>(), VK = kUnit / (2 * DV), STEPS = VK / 16, SOFT = 4 * TILES, USERS = SOFT + TILES + 5;   // VK: keys of a unit of values
+  constexpr int TILES = tiles<DK, DV>(), KU = k_units<DK, DV>(), VU = v_units<DK, DV>(), VK = kUnit / (2 * DV), STEPS = VK / 16, SOFT = 4 * TILES, USERS = SOFT + 2 * TILES + 3;   // VK: keys of a unit of values
   constexpr int W = kTile / TILES, PER = kTile / W;          // keys of a step: a row tile has scores in two places of W columns, so that one's products run under the other's softmax; steps of a tile
   constexpr float LEAD = BF16 ? 40.f : -7.f, ROOM = BF16 ? -26.f : 14.f;       // a reference is taken LEAD above its maximum, and follows once that is above m + ROOM
   constexpr int MANY = 192, FEW = 64;                        // registers of a softmax thread and of another one: 512 threads have 128 each
@@ -119,14 +119,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   __shared__ int odd_values, pieces;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, qs = base, ks = qs + 128 * TILES * DK * 2, vs = ks + KU * kUnit, b0 = smem_u32(bars);
   const uint32_t kfull = b0, kempty = b0 + 32, vfull = b0 + 64, vempty = b0 + 104, vok = b0 + 144, vraw = b0 + 184, qfull = b0 + 224, qempty = b0 + 240, odone = b0 + 256, ifull = b0 + 272,
-                 iempty = b0 + 288, sfull = b0 + 304, pfull = b0 + 336, pvdone = b0 + 368, flushed = b0 + 400, want = b0 + 416, claimed = b0 + 424;
+                 iempty = b0 + 288, sfull = b0 + 304, pfull = b0 + 336, pvdone = b0 + 368, flushed = b0 + 400, want = b0 + 432, claimed = b0 + 440;
   // keys: a barrier for each of kAhead tiles; values: one for each place (vraw: where they land that are looked at ahead of their products); scores, weights, products: [row tile][place]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tokens = TILES * P.tokens;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kAhead; i++) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); }
-    for (int i = 0; i < 5; i++) { mbar_init(vfull + 8 * i, 1); mbar_init(vempty + 8 * i, TILES); mbar_init(vok + 8 * i, 3); mbar_init(vraw + 8 * i, 1); }
+    for (int i = 0; i < 5; i++) { mbar_init(vfull + 8 * i, 1); mbar_init(vempty + 8 * i, TILES); mbar_init(vok + 8 * i, 2); mbar_init(vraw + 8 * i, 1); }
     for (int i = 0; i < 2; i++) {
-      mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); mbar_init(flushed + 8 * i, 1);
+      mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); mbar_init(flushed + 16 * i, 1); mbar_init(flushed + 16 * i + 8, 1);
     }
     mbar_init(want, 1);
     mbar_init(claimed, 1);
@@ -180,179 +180,182 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   if (blockIdx.x >= all) {                                   // (nothing for this CTA: the grid is launched for as many pieces as there may be)
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
-    if (warp < 8 + TILES) {                                  // products of row tile warp - 8
-      const int t = warp - 8;
+    const bool scoring = warp < 8 + TILES, adding = warp == 11 || warp == 10 + TILES;
+    if (scoring || adding) {                                 // products of a row tile: scores, or weights x values.  (A warp for each: in one, the way from weights to results and to the place of the next scores stood behind one another)
+      const int t = scoring ? warp - 8 : warp - 11;
       const uint32_t lead = hy::tc_elect();
       const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);         // fp32 sums of bf16 or fp16, 128 rows
-      const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17), s_at = tmem + t * 128, to = o_at + t * 128;
-      const uint64_t q_desc = hy::tc_desc(qs + t * (kTile * DK * 2));
-      const int chunks = (P.dk + 63) / 64, ksteps = P.dk / 16;
-      const bool whole = ksteps == DK / 16;
-      uint32_t kt = 0, kn = 0, vn = 0, vpar[2] = {0, 0}, sent = 0, done = 0, took = 0;   // tiles of keys behind, places in the rings, parities of values (a bit for each place: as they came, looked at),
-      Item w;                                                                            // steps whose scores, whose results are issued, items that had rows
+      const uint32_t s_at = tmem + t * 128, done_at = pvdone + 16 * t;
+      uint32_t n_steps = 0, took = 0;                        // steps of the row tile behind, items that had rows
+      Item w;
       bool alive = true;
-      while (alive && take(w)) {
-        const Walk k = walk_of(P, w, tokens);
-        const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1, last = k.n * PER;
-        const bool there = a < w.len;
-        int q_step = 0, v_step = 0;
-        bool any = false;
-        auto key_at = [&](int step) { return key_of(k, step / PER) + step % PER * W; };
-        auto is_mine = [&](int step) { return there && sees_some(P, a, b, key_at(step), W); };
-        auto ahead = [&] {                                   // scores of two steps ahead of their results (more, past steps that the rows do not see, and the two row tiles might wait for one another)
-          while (q_step < min(last, v_step + 2)) {
-            const int key0 = key_at(q_step);
-            const bool mine = is_mine(q_step);
-            if (q_step % PER == 0 && !wait_warp(kfull + 8 * (kt % kAhead), (kt / kAhead) & 1, P.status)) return false;
-            if (mine) {
-              const uint32_t place = sent & 1, sdesc = idesc | (uint32_t)(2 * min(W / 16, (b - key0 + 16) / 16)) << 17;   // (the rows see the first of them)
-              uint64_t k_desc[DK / 64];
+      if (scoring) {
+        const uint64_t q_desc = hy::tc_desc(qs + t * (kTile * DK * 2));
+        const int chunks = (P.dk + 63) / 64, ksteps = P.dk / 16;
+        const bool whole = ksteps == DK / 16;
+        uint32_t kt = 0, kn = 0;                             // tiles of keys behind, the next one's first place
+        while (alive && take(w)) {
+          const Walk k = walk_of(P, w, tokens);
+          const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
+          const bool there = a < w.len;
+          alive = !there || wait_warp(qfull + 8 * t, took & 1, P.status);
+          for (int i = 0; i < k.n && alive; i++) {
+            const int key0 = key_of(k, i);
+            uint64_t k_desc[DK / 64];
 #pragma unroll
-              for (int c = 0; c < DK / 64; c++) k_desc[c] = hy::tc_desc(ks + (kn + c < KU ? kn + c : kn + c - KU) * kUnit + q_step % PER * (W * 128));
-              if (sent > 1 && !wait_warp(pvdone + 16 * t + 8 * place, ((sent >> 1) - 1) & 1, P.status)) return false;   // the weights that lie there are read
+            for (int c = 0; c < DK / 64; c++) k_desc[c] = hy::tc_desc(ks + (kn + c < KU ? kn + c : kn + c - KU) * kUnit);
+            alive = wait_warp(kfull + 8 * (kt % kAhead), (kt / kAhead) & 1, P.status);
+#pragma unroll
+            for (int h = 0; h < PER; h++) {
+              if (!alive || !there || !sees_some(P, a, b, key0 + h * W, W)) continue;
+              const uint32_t place = n_steps & 1, at = s_at + place * W, sdesc = idesc | (uint32_t)(2 * min(W / 16, (b - key0 - h * W + 16) / 16)) << 17;   // (the rows see the first of them)
+              if (n_steps > 1) alive = wait_warp(done_at + 8 * place, ((n_steps >> 1) - 1) & 1, P.status);   // the weights that lie there are read
+              if (!alive) continue;
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
               if (whole) {
 #pragma unroll
                 for (int c = 0; c < DK / 64; c++)
 #pragma unroll
-                  for (int u = 0; u < 4; u++) mma_ss(s_at + place * W, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + 2 * u, sdesc, c > 0 || u > 0, lead);
+                  for (int u = 0; u < 4; u++) mma_ss(at, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + h * (W * 128 >> 4) + 2 * u, sdesc, c > 0 || u > 0, lead);
               } else {
 #pragma unroll
                 for (int c = 0; c < DK / 64; c++)
 #pragma unroll
-                  for (int u = 0; u < 4; u++) if (4 * c + u < ksteps) mma_ss(s_at + place * W, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + 2 * u, sdesc, c > 0 || u > 0, lead);
+                  for (int u = 0; u < 4; u++) if (4 * c + u < ksteps) mma_ss(at, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + h * (W * 128 >> 4) + 2 * u, sdesc, c > 0 || u > 0, lead);
               }
               commit(sfull + 16 * t + 8 * place, lead);
-              sent++;
+              n_steps++;
             }
-            if (q_step % PER == PER - 1) {                   // (a commit stands for all products ahead of it)
-              if (there) commit(kempty + 8 * (kt % kAhead), lead);
-              else if (lead) hy::tc_arrive(kempty + 8 * (kt % kAhead));
-              kt++;
-              kn += chunks;
-              if (kn >= KU) kn -= KU;
-            }
-            q_step++;
-            if (q_step == last && there) commit(qempty + 8 * t, lead);
+            if (there) commit(kempty + 8 * (kt % kAhead), lead);       // (stands for all products ahead of it)
+            else if (lead) hy::tc_arrive(kempty + 8 * (kt % kAhead));
+            kt++;
+            kn += chunks;
+            if (kn >= KU) kn -= KU;
           }
-          return true;
-        };
-        auto results = [&]() {                               // of the next step
-          const int key0 = key_at(v_step);
-          const bool mine = is_mine(v_step), masked = !sees_all(P, w.tok, k.t1 - 1, key0 - v_step % PER * W, kTile);
-          const uint32_t place = done & 1, weights = s_at + place * W;
-          const int n = min(W / 16, (b - key0 + 16) / 16);
-          constexpr int UNITS = W >= VK ? W / VK : 1, EACH = W >= VK ? 1 : VK / W;   // units of a step, or steps of a unit
-          uint64_t v_desc[UNITS];
-#pragma unroll
-          for (int u = 0; u < UNITS; u++) {
-            const uint32_t at = vn + u < VU ? vn + u : vn + u - VU;
-            if (EACH == 1 || v_step % EACH == 0) {
-              if (!wait_warp((masked ? vok : vfull) + 8 * at, (masked ? vpar[1] : vpar[0]) >> at & 1, P.status)) return false;
-              if (masked) vpar[1] ^= 1u << at; else vpar[0] ^= 1u << at;
-            }
-            v_desc[u] = value_desc(vs + at * kUnit + (EACH == 1 ? 0 : v_step % EACH * (W * 128)), VK);
-          }
-          if (mine) {
-            if (!wait_warp(pfull + 16 * t + 8 * place, (done >> 1) & 1, P.status)) return false;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (n == W / 16) {
-#pragma unroll
-              for (int u = 0; u < W / 16; u++) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
-            } else {
-#pragma unroll
-              for (int u = 0; u < W / 16; u++) if (u < n) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
-            }
-            commit(pvdone + 16 * t + 8 * place, lead);
-            done++;
-            any = true;
-          }
-          if (EACH == 1 || v_step % EACH == EACH - 1) {
-#pragma unroll
-            for (int u = 0; u < UNITS; u++) {
-              if (there) commit(vempty + 8 * vn, lead);
-              else if (lead) hy::tc_arrive(vempty + 8 * vn);
-              if (++vn == VU) vn = 0;
-            }
-          }
-          v_step++;
-          return true;
-        };
-        alive = !there || wait_warp(qfull + 8 * t, took & 1, P.status);
-        while (alive && v_step < last) alive = ahead() && results();
-        if (there && alive) { commit(odone + 8 * t, lead); took++; }
-      }
-      commit(flushed + 8 * t, lead);                         // no product is under way when TMEM is given back
-      wait_warp(flushed + 8 * t, 0, P.status);
-    } else if (warp == 10 || warp == 11) {                   // copies: keys and queries, values
-      Item w;
-      const int chunks = (P.dk + 63) / 64, boxes = (P.dv + 63) / 64;
-      uint32_t n = 0, par = 0, took[2] = {0, 0}, vpar[2] = {0, 0}, vsent[2] = {0, 0};
-      int tile = 0, freed = 0, sent = 0;                     // tiles of keys begun and given back, units sent
-      bool alive = true;
-      auto keys = [&](const Item& w, int key0, int head) {
-        for (int c = 0; c < chunks; c++) {
-          while (freed + kAhead <= tile || freed * chunks + KU <= sent) {   // the barrier's last tile, and the unit that lies where this one goes
-            alive = wait_warp(kempty + 8 * (freed % kAhead), (freed / kAhead) & 1, P.status);
-            if (!alive) return;
-            freed++;
-          }
-          if (lane == 0) {
-            if (c == 0) mbar_expect_tx(kfull + 8 * (tile % kAhead), chunks * kUnit);
-            copy_box(ks + n * kUnit, &P.k, 64 * c, head, w.row + key0, kfull + 8 * (tile % kAhead));
-          }
-          sent++;
-          if (++n == KU) n = 0;
+          if (there && alive) { commit(qempty + 8 * t, lead); took++; }
         }
-        tile++;
-      };
-      if (warp == 10) {
-        while (alive && take(w)) {
-          const Walk k = walk_of(P, w, tokens);
-          const int head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack;
-          keys(w, key_of(k, 0), head);
-          if (k.n <= kEarly && lane == 0) hy::tc_arrive(want);
-          for (int t = 0; t < TILES && alive; t++) {
-            if (w.tok + t * P.tokens >= w.len) continue;
-            alive = wait_warp(qempty + 8 * t, (took[t] & 1) ^ 1, P.status);
-            if (!alive) break;
-            if (lane == 0) {
-              mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
-              for (int c = 0; c < chunks; c++) copy_box(qs + t * (kTile * DK * 2) + c * (kTile * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
-            }
-            took[t]++;
-          }
-          for (int i = 1; i < k.n && alive; i++) {
-            if (i == k.n - kEarly && lane == 0) hy::tc_arrive(want);
-            keys(w, key_of(k, i), head);
-          }
-        }
-        for (int t = 0; t < TILES; t++) if (took[t]) wait_warp(qfull + 8 * t, (took[t] - 1) & 1, P.status);   // no copy is under way at the end, whatever happened
-        for (int s = max(0, tile - kAhead); s < tile; s++) wait_warp(kfull + 8 * (s % kAhead), (s / kAhead) & 1, P.status);
       } else {
+        const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17), to = o_at + t * 128;
+        constexpr int UNITS = W >= VK ? W / VK : 1, EACH = W >= VK ? 1 : VK / W;   // units of a step, or steps of a unit
+        uint32_t vn = 0, vpar[2] = {0, 0};                   // the next unit's place, parities (a bit for each place: as they came, looked at)
         while (alive && take(w)) {
           const Walk k = walk_of(P, w, tokens);
-          const int head = w.unit / P.subs;
+          const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
+          const bool there = a < w.len;
+          bool any = false;
           for (int i = 0; i < k.n && alive; i++) {
             const int key0 = key_of(k, i);
             const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0, kTile);
-            const uint32_t full = masked ? vraw : vfull;
-            for (int u = 0; u < kTile / VK && alive; u++) {
-              alive = wait_warp(vempty + 8 * n, par ^ 1, P.status);
-              if (!alive) break;
-              if (lane == 0) {
-                mbar_expect_tx(full + 8 * n, boxes * VK * 128);
-                for (int c = 0; c < boxes; c++) copy_box(vs + n * kUnit + c * (VK * 128), &P.v, 64 * c, head, w.row + key0 + u * VK, full + 8 * n);
+#pragma unroll
+            for (int h = 0; h < PER; h++) {
+              const int first = key0 + h * W, n = there && sees_some(P, a, b, first, W) ? min(W / 16, (b - first + 16) / 16) : 0;   // sixteenths that some row sees
+              uint64_t v_desc[UNITS];
+#pragma unroll
+              for (int u = 0; u < UNITS; u++) {
+                const uint32_t at = vn + u < VU ? vn + u : vn + u - VU;
+                if (h % EACH == 0) {
+                  alive = alive && wait_warp((masked ? vok : vfull) + 8 * at, (masked ? vpar[1] : vpar[0]) >> at & 1, P.status);
+                  if (masked) vpar[1] ^= 1u << at; else vpar[0] ^= 1u << at;
+                }
+                v_desc[u] = value_desc(vs + at * kUnit + h % EACH * (W * 128), VK);
               }
-              vpar[masked] ^= 1u << n;
-              vsent[masked] |= 1u << n;
-              if (++n == VU) { n = 0; par ^= 1; }
+              if (n) {
+                const uint32_t place = n_steps & 1, weights = s_at + place * W;
+                alive = alive && wait_warp(pfull + 16 * t + 8 * place, (n_steps >> 1) & 1, P.status);
+                if (!alive) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (n == W / 16) {
+#pragma unroll
+                  for (int u = 0; u < W / 16; u++) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
+                } else {
+#pragma unroll
+                  for (int u = 0; u < W / 16; u++) if (u < n) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
+                }
+                commit(done_at + 8 * place, lead);
+                n_steps++;
+                any = true;
+              }
+              if (!alive) break;
+              if (h % EACH == EACH - 1) {
+#pragma unroll
+                for (int u = 0; u < UNITS; u++) {
+                  if (there) commit(vempty + 8 * vn, lead);
+                  else if (lead) hy::tc_arrive(vempty + 8 * vn);
+                  if (++vn == VU) vn = 0;
+                }
+              }
             }
           }
+          if (there && alive) commit(odone + 8 * t, lead);
         }
-        for (uint32_t s = 0; s < 2 * VU; s++)                // no copy is under way at the end, whatever happened
-          if (vsent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
       }
+      const uint32_t last = flushed + 16 * t + (scoring ? 0 : 8);
+      commit(last, lead);                                    // no product is under way when TMEM is given back
+      wait_warp(last, 0, P.status);
+    } else if (warp == 10) {                                 // copies: a tile of values behind the next one of keys
+      Item w;
+      const int chunks = (P.dk + 63) / 64, boxes = (P.dv + 63) / 64;
+      uint32_t kn = 0, vn = 0, par = 0, took[2] = {0, 0}, vpar[2] = {0, 0}, vsent[2] = {0, 0};
+      int tile = 0, freed = 0, sent = 0;                     // tiles of keys begun and given back, units sent
+      bool alive = true;
+      while (alive && take(w)) {
+        const Walk k = walk_of(P, w, tokens);
+        const int head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack;
+        auto keys = [&](int i) {
+          for (int c = 0; c < chunks; c++) {
+            while (freed + kAhead <= tile || freed * chunks + KU <= sent) {   // the barrier's last tile, and the unit that lies where this one goes
+              alive = wait_warp(kempty + 8 * (freed % kAhead), (freed / kAhead) & 1, P.status);
+              if (!alive) return;
+              freed++;
+            }
+            if (lane == 0) {
+              if (c == 0) mbar_expect_tx(kfull + 8 * (tile % kAhead), chunks * kUnit);
+              copy_box(ks + kn * kUnit, &P.k, 64 * c, head, w.row + key_of(k, i), kfull + 8 * (tile % kAhead));
+            }
+            sent++;
+            if (++kn == KU) kn = 0;
+          }
+          tile++;
+        };
+        auto values = [&](int i) {
+          const int key0 = key_of(k, i);
+          const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0, kTile);
+          const uint32_t full = masked ? vraw : vfull;
+          for (int u = 0; u < kTile / VK && alive; u++) {
+            alive = wait_warp(vempty + 8 * vn, par ^ 1, P.status);
+            if (!alive) return;
+            if (lane == 0) {
+              mbar_expect_tx(full + 8 * vn, boxes * VK * 128);
+              for (int c = 0; c < boxes; c++) copy_box(vs + vn * kUnit + c * (VK * 128), &P.v, 64 * c, head, w.row + key0 + u * VK, full + 8 * vn);
+            }
+            vpar[masked] ^= 1u << vn;
+            vsent[masked] |= 1u << vn;
+            if (++vn == VU) { vn = 0; par ^= 1; }
+          }
+        };
+        keys(0);
+        if (k.n <= kEarly && lane == 0) hy::tc_arrive(want);
+        for (int t = 0; t < TILES && alive; t++) {
+          if (w.tok + t * P.tokens >= w.len) continue;
+          alive = wait_warp(qempty + 8 * t, (took[t] & 1) ^ 1, P.status);
+          if (!alive) break;
+          if (lane == 0) {
+            mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
+            for (int c = 0; c < chunks; c++) copy_box(qs + t * (kTile * DK * 2) + c * (kTile * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
+          }
+          took[t]++;
+        }
+        for (int i = 1; i < k.n && alive; i++) {
+          if (i == k.n - kEarly && lane == 0) hy::tc_arrive(want);
+          keys(i);
+          if (alive) values(i - 1);
+        }
+        if (alive) values(k.n - 1);
+      }
+      for (int t = 0; t < TILES; t++) if (took[t]) wait_warp(qfull + 8 * t, (took[t] - 1) & 1, P.status);   // no copy is under way at the end, whatever happened
+      for (int s = max(0, tile - kAhead); s < tile; s++) wait_warp(kfull + 8 * (s % kAhead), (s / kAhead) & 1, P.status);
+      for (uint32_t s = 0; s < 2 * VU; s++)
+        if (vsent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
     } else if (warp == 15) {                                 // deals out the work: rows with most keys first, so that the short ones fill the gaps
       // CTAs take over work of CTAs that have not started yet, each when its copies near the end of what it has
       long long at = blockIdx.x;
@@ -395,9 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         __syncwarp();
         at = got ? (long long)next : all;
       }
-    } else if (warp >= 12) {                                 // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
+    } else if (warp >= 13) {                                 // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
       Item w;
-      const int me = threadIdx.x - 12 * 32, boxes = (P.dv + 63) / 64;
+      const int me = threadIdx.x - 13 * 32, boxes = (P.dv + 63) / 64;
       const uint32_t inf = BF16 ? 0x7f807f80u : 0x7c007c00u;
       uint32_t n = 0, par = 0;                               // par: a bit for each place
       bool alive = true;
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
               par ^= 1u << n;
               const int first = key0 + u * VK;
               bool odd = false;
-              for (int p = me; p < boxes * VK * 8; p += 96) {  // 16-byte pieces: eight to a row of 64 columns
+              for (int p = me; p < boxes * VK * 8; p += 64) {  // 16-byte pieces: eight to a row of 64 columns
                 const int row = first + ((p >> 3) & (VK - 1));
                 const uint32_t at = vs + n * kUnit + p * 16;
                 const uint4 x = lds128(at);

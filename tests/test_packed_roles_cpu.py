@@ -30,10 +30,10 @@ def run(rng, dk, work, idle, moves, early=True):
     tiles, per_k, per_v, KU, VU = SHAPES[dk]
     bars = lambda n, count: [Bar(count) for _ in range(n)]
     soft, per = 4 * tiles, tiles                             # steps of a tile: two with two row tiles, of half as many keys
-    kfull, kempty, vfull, vempty, vok, vraw = bars(AHEAD, 1), bars(AHEAD, tiles), bars(VU, 1), bars(VU, tiles), bars(VU, 3), bars(VU, 1)
+    kfull, kempty, vfull, vempty, vok, vraw = bars(AHEAD, 1), bars(AHEAD, tiles), bars(VU, 1), bars(VU, tiles), bars(VU, 2), bars(VU, 1)
     qfull, qempty, odone, ifull = (bars(2, 1) for _ in range(4))
     sfull, pvdone, pfull = ([bars(2, n) for _ in range(2)] for n in (1, 1, 4))            # [row tile][place]
-    iempty, flushed = bars(2, soft + tiles + 5), bars(2, 1)
+    iempty, flushed = bars(2, soft + 2 * tiles + 3), [bars(2, 1) for _ in range(2)]
     items, want = [None, None], Bar(1)
     keys, values, queries, looked = [None] * KU, [None] * VU, [None] * 2, [0] * VU
     scores, weights, through = [[None, None], [None, None]], [[{}, {}], [{}, {}]], [[], []]       # [row tile][place], steps whose product is through
@@ -56,14 +56,15 @@ def run(rng, dk, work, idle, moves, early=True):
                 yield want.wait(r)
                 yield None                                   # (the claim)
 
-    def copy_keys():
-        me, took = {"turn": 0}, [0, 0]
+    def copies():
+        me, took, vn, par = {"turn": 0}, [0, 0], 0, 0
         at = {"n": 0, "tile": 0, "freed": 0, "sent": 0}
         while True:
             yield from take(me)
-            if me["item"] is None:
+            n = me["item"]
+            if n is None:
                 return
-            walk, two = work[me["item"]]
+            walk, two = work[n]
 
             def tile(i):
                 bar = kfull[at["tile"] % AHEAD]
@@ -72,11 +73,20 @@ def run(rng, dk, work, idle, moves, early=True):
                     while at["freed"] + AHEAD <= at["tile"] or at["freed"] * per_k + KU <= at["sent"]:
                         yield kempty[at["freed"] % AHEAD].wait(at["freed"] // AHEAD)
                         at["freed"] += 1
-                    flying.append((keys, at["n"], (me["item"], i, c), (units, bar)))
+                    flying.append((keys, at["n"], (n, i, c), (units, bar)))
                     keys[at["n"]] = "under way"
                     at["sent"] += 1
                     at["n"] = (at["n"] + 1) % KU
                 at["tile"] += 1
+
+            def some(i, vn, par):
+                for c in range(per_v):
+                    yield vempty[vn].wait(par ^ 1)
+                    looked[vn] = 0
+                    flying.append((values, vn, (n, i, c), (vraw if walk[i][1] else vfull)[vn]))
+                    values[vn] = "under way"
+                    vn, par = (0, par ^ 1) if vn + 1 == VU else (vn + 1, par)
+                return vn, par
 
             yield from tile(0)
             if len(walk) <= EARLY:
@@ -85,27 +95,15 @@ def run(rng, dk, work, idle, moves, early=True):
                 if t and not two:
                     continue
                 yield qempty[t].wait((took[t] & 1) ^ 1)
-                flying.append((queries, t, me["item"], qfull[t]))
+                flying.append((queries, t, n, qfull[t]))
                 queries[t] = "under way"
                 took[t] += 1
             for i in range(1, len(walk)):
                 if i == len(walk) - EARLY:
                     want.arrive()
                 yield from tile(i)
-
-    def copy_values():
-        me, n, par = {"turn": 0}, 0, 0
-        while True:
-            yield from take(me)
-            if me["item"] is None:
-                return
-            for i, (_, masked) in enumerate(work[me["item"]][0]):
-                for c in range(per_v):
-                    yield vempty[n].wait(par ^ 1)
-                    looked[n] = 0
-                    flying.append((values, n, (me["item"], i, c), (vraw if masked else vfull)[n]))
-                    values[n] = "under way"
-                    n, par = (0, par ^ 1) if n + 1 == VU else (n + 1, par)
+                vn, par = yield from some(i - 1, vn, par)
+            vn, par = yield from some(len(walk) - 1, vn, par)
 
     def look(_):
         me, n, par = {"turn": 0}, 0, [0] * VU
@@ -136,14 +134,47 @@ def run(rng, dk, work, idle, moves, early=True):
 
     def product_of_results(t, n, step, units, at, masked):
         def product():
-            assert all(values[place] == (n, step // per, c) and (not masked or looked[place] == 3) for c, place in units)
+            assert all(values[place] == (n, step // per, c) and (not masked or looked[place] == 2) for c, place in units)
             assert scores[t][at] == (n, step) and all(idle[n][4 * t + w] or weights[t][at].get(w) == (n, step) for w in range(4))
             through[t].append((n, step))
         return product
 
-    def issuer(t):
+    def scorer(t):
         me = {"turn": 0}
-        kt = kn = vn = sent = done = took = 0
+        kt = kn = steps = took = 0
+        while True:
+            yield from take(me)
+            n = me["item"]
+            if n is None:
+                break
+            walk, two = work[n]
+            there = t == 0 or two
+            if there:
+                yield qfull[t].wait(took)
+            for i, (who, _) in enumerate(walk):
+                yield kfull[kt % AHEAD].wait(kt // AHEAD)
+                for h in range(per):
+                    if not there or t not in who[h]:
+                        continue
+                    at = steps & 1
+                    if steps > 1:
+                        yield pvdone[t][at].wait((steps >> 1) - 1)
+                    queue.extend([product_of_scores(t, n, i * per + h, c, (kn + c) % KU, at) for c in range(per_k)] + [sfull[t][at]])
+                    steps += 1
+                if there:
+                    queue.append(kempty[kt % AHEAD])
+                else:
+                    kempty[kt % AHEAD].arrive()
+                kt, kn = kt + 1, (kn + per_k) % KU
+            if there:
+                queue.append(qempty[t])
+                took += 1
+        queue.append(flushed[0][t])
+        yield flushed[0][t].wait(0)
+
+    def adder(t):
+        me = {"turn": 0}
+        vn = steps = 0
         vpar = [[0] * VU, [0] * VU]
         units, each = max(1, per_v // per), max(1, per // per_v)                  # units of a step, steps of a unit
         while True:
@@ -152,53 +183,30 @@ def run(rng, dk, work, idle, moves, early=True):
             if n is None:
                 break
             walk, two = work[n]
-            there, last, q = t == 0 or two, len(walk) * per, 0
-            if there:
-                yield qfull[t].wait(took)
-            for v in range(last):
-                while q < min(last, v + 2):
-                    mine = there and t in walk[q // per][0][q % per]
-                    if q % per == 0:
-                        yield kfull[kt % AHEAD].wait(kt // AHEAD)
-                    if mine:
-                        at = sent & 1
-                        if sent > 1:
-                            yield pvdone[t][at].wait((sent >> 1) - 1)
-                        queue.extend([product_of_scores(t, n, q, c, (kn + c) % KU, at) for c in range(per_k)] + [sfull[t][at]])
-                        sent += 1
-                    if q % per == per - 1:
-                        if there:
-                            queue.append(kempty[kt % AHEAD])
-                        else:
-                            kempty[kt % AHEAD].arrive()
-                        kt, kn = kt + 1, (kn + per_k) % KU
-                    q += 1
-                    if q == last and there:
-                        queue.append(qempty[t])
-                who, masked = walk[v // per]
-                mine, at = there and t in who[v % per], done & 1
-                places = [(vn + u) % VU for u in range(units)]
-                if v % each == 0:
-                    for place in places:
-                        yield (vok if masked else vfull)[place].wait(vpar[masked][place])
-                        vpar[masked][place] ^= 1
-                if mine:
-                    yield pfull[t][at].wait(done >> 1)
-                    first = v % per * units if each == 1 else 0
-                    queue.extend([product_of_results(t, n, v, [(first + u, place) for u, place in enumerate(places)], at, masked), pvdone[t][at]])
-                    done += 1
-                if v % each == each - 1:
-                    for place in places:
-                        if there:
-                            queue.append(vempty[place])
-                        else:
-                            vempty[place].arrive()
-                    vn = (vn + units) % VU
+            there = t == 0 or two
+            for i, (who, masked) in enumerate(walk):
+                for h in range(per):
+                    places = [(vn + u) % VU for u in range(units)]
+                    if h % each == 0:
+                        for place in places:
+                            yield (vok if masked else vfull)[place].wait(vpar[masked][place])
+                            vpar[masked][place] ^= 1
+                    if there and t in who[h]:
+                        at, first = steps & 1, h * units if each == 1 else 0
+                        yield pfull[t][at].wait(steps >> 1)
+                        queue.extend([product_of_results(t, n, i * per + h, [(first + u, place) for u, place in enumerate(places)], at, masked), pvdone[t][at]])
+                        steps += 1
+                    if h % each == each - 1:
+                        for place in places:
+                            if there:
+                                queue.append(vempty[place])
+                            else:
+                                vempty[place].arrive()
+                        vn = (vn + units) % VU
             if there:
                 queue.append(odone[t])
-                took += 1
-        queue.append(flushed[t])
-        yield flushed[t].wait(0)
+        queue.append(flushed[1][t])
+        yield flushed[1][t].wait(0)
 
     def softmax(x):
         t, w = divmod(x, 4)
@@ -239,7 +247,7 @@ def run(rng, dk, work, idle, moves, early=True):
                 assert through[t][-1:] == [last]
                 yield None
 
-    roles = [deal(), copy_keys(), copy_values(), *(issuer(t) for t in range(tiles))] + [look(k) for k in range(3)] + [softmax(x) for x in range(soft)]
+    roles = [deal(), copies(), *(scorer(t) for t in range(tiles)), *(adder(t) for t in range(tiles))] + [look(k) for k in range(2)] + [softmax(x) for x in range(soft)]
     speed = [rng.choice([1, 1, 1, 10, 0.05]) for _ in roles] + [rng.choice([1, 0.1, 10]) for _ in range(2)]
     at = [next(r, False) for r in roles]                      # what a role waits for: a test, None, or False at its end
     while queue or flying or any(a is not False for a in at):

@@ -169,7 +169,7 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   while (dim_k > kShapes[shape][0] || dim_v > kShapes[shape][1]) shape++;
   if (const int code = rows_map(&P.q, "queries", q, dim_k, heads, s->rows, P.pack, P.tokens)) return code;
   if (const int code = rows_map(&P.k, "keys", k, dim_k, kv_heads, s->rows, 1, prompt::kTile)) return code;
-  if (const int code = rows_map(&P.v, "values", v, dim_v, kv_heads, s->rows, 1, prompt::kUnit / 2 / kShapes[shape][1])) return code;
+  if (const int code = rows_map(&P.v, "values", v, dim_v, kv_heads, s->rows, 1, prompt::kTile)) return code;
   P.starts = s->starts; P.status = s->status;
   P.values = v->data; P.v_row = v->row; P.v_head = v->head;
   P.out = out->data; P.o_row = out->row; P.o_head = out->head;

@@ -21,7 +21,7 @@
 namespace dsk {
 namespace prompt {
 
-constexpr int kThreads = 512, kTile = 128, kUnit = 16384, kMaxBatch = 1024, kHeld = 8, kAhead = 4, kEarly = 4;   // keys of a tile; bytes of a copied unit; sequences whose tiles a lane of the dealing warp keeps in registers; tiles of keys under way; tiles ahead of the end at which more work is asked for
+constexpr int kThreads = 512, kRows = 128, kTile = 64, kMaxBatch = 1024, kHeld = 8, kEarly = 8;   // rows of a row tile, keys of a tile; sequences whose tiles a lane of the dealing warp keeps in registers; tiles ahead of the end at which more work is asked for
 constexpr int ST_WAIT = 4;                                   // a wait that gave up
 constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
 constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
@@ -39,9 +39,12 @@ struct Params {
 };
 
 template <int DK, int DV> __host__ __device__ constexpr int tiles() { return DV == 256 ? 1 : 2; }
-template <int DK, int DV> __host__ __device__ constexpr int k_units() { return DK == 192 ? 5 : 6; }
-template <int DK, int DV> __host__ __device__ constexpr int v_units() { return DK == 192 ? 3 : DK == 64 ? 5 : 4; }
-template <int DK, int DV> __host__ __device__ constexpr int smem_bytes() { return 1024 + 128 * tiles<DK, DV>() * DK * 2 + (k_units<DK, DV>() + v_units<DK, DV>()) * kUnit; }
+// tiles of keys and of values that shared memory has room for beside the queries
+template <int DK, int DV> __host__ __device__ constexpr int k_places() { return DK == 64 ? 8 : DK == 128 ? 6 : 3; }
+template <int DK, int DV> __host__ __device__ constexpr int v_places() { return DK == 64 ? 8 : DK == 128 ? 4 : DK == 192 ? 3 : 2; }
+template <int DK, int DV> __host__ __device__ constexpr int smem_bytes() {
+  return 1024 + kRows * tiles<DK, DV>() * DK * 2 + k_places<DK, DV>() * kTile * DK * 2 + v_places<DK, DV>() * kTile * DV * 2;
+}
 
 // Bounded, in line: a call would cost what the wait itself does
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status) {
@@ -57,9 +60,9 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(entry), "r"(head), "r"(row) : "memory");
 }
-// operand whose rows are the depth, `keys` of them: 64 columns to a swizzled 128-byte row, groups of eight rows 1024 bytes apart, the next 64 columns `keys` rows behind
-__device__ __forceinline__ uint64_t value_desc(uint32_t addr, int keys) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(keys * 128 >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// operand whose rows are the depth, a tile of keys: 64 columns to a swizzled 128-byte row, groups of eight rows 1024 bytes apart, the next 64 columns kTile rows behind
+__device__ __forceinline__ uint64_t value_desc(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kTile * 128 >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 template <bool BF16> __device__ __forceinline__ uint32_t pair(float lo, float hi) {
   if (!BF16) return halves(lo, hi);
@@ -80,19 +83,19 @@ __device__ __forceinline__ Walk walk_of(const Params& P, const Item& w, int toke
   return k;
 }
 __device__ __forceinline__ int key_of(const Walk& k, int i) { return (i < k.kept ? i : k.low + i - k.kept) * kTile; }
-// whether tokens a .. b see all of `keys` keys; any of them
-__device__ __forceinline__ bool sees_all(const Params& P, int a, int b, int key0, int keys) {
-  return key0 + keys - 1 <= a && (P.window <= 0 || b - key0 < P.window || key0 + keys <= P.keep);
+// whether tokens a .. b see all of a tile of keys; any of it
+__device__ __forceinline__ bool sees_all(const Params& P, int a, int b, int key0) {
+  return key0 + kTile - 1 <= a && (P.window <= 0 || b - key0 < P.window || key0 + kTile <= P.keep);
 }
-__device__ __forceinline__ bool sees_some(const Params& P, int a, int b, int key0, int keys) {
-  return key0 <= b && (P.window <= 0 || a - key0 - keys + 1 < P.window || key0 < P.keep);
+__device__ __forceinline__ bool sees_some(const Params& P, int a, int b, int key0) {
+  return key0 <= b && (P.window <= 0 || a - key0 - kTile + 1 < P.window || key0 < P.keep);
 }
 
 // Infinities and NaN among the values that a row sees in tiles where they went to the products as zeros: its results c .. c + 15 become what they make of them
 template <bool BF16> __device__ __noinline__ void give_back(const Params& P, const Item& w, const Walk& k, int pos, int head, int c, uint32_t (&x)[16]) {
   for (int i = 0; i < k.n; i++) {
     const int key0 = key_of(k, i);
-    if (sees_all(P, w.tok, k.t1 - 1, key0, kTile)) continue;
+    if (sees_all(P, w.tok, k.t1 - 1, key0)) continue;
     for (int j = key0; j < min(key0 + kTile, pos + 1); j++) {
       if (P.window > 0 && pos - j >= P.window && j >= P.keep) continue;
       const uint16_t* v = static_cast<const uint16_t*>(P.values) + (long long)(w.row + j) * P.v_row + (long long)head * P.v_head + c;
@@ -107,27 +110,26 @@ template <bool BF16> __device__ __noinline__ void give_back(const Params& P, con
 
 template <int DK, int DV, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_constant__ Params P) {
-  constexpr int TILES = tiles<DK, DV>(), KU = k_units<DK, DV>(), VU = v_units<DK, DV>(), VK = kUnit / (2 * DV), STEPS = VK / 16, SOFT = 4 * TILES, USERS = SOFT + 2 * TILES + 3;   // VK: keys of a unit of values
-  constexpr int W = kTile / TILES, PER = kTile / W;          // keys of a step: a row tile has scores in two places of W columns, so that one's products run under the other's softmax; steps of a tile
+  constexpr int TILES = tiles<DK, DV>(), KP = k_places<DK, DV>(), VP = v_places<DK, DV>(), KB = kTile * DK * 2, VB = kTile * DV * 2, SOFT = 4 * TILES, USERS = SOFT + 2 * TILES + 3;
   constexpr float LEAD = BF16 ? 40.f : -7.f, ROOM = BF16 ? -26.f : 14.f;       // a reference is taken LEAD above its maximum, and follows once that is above m + ROOM
   constexpr int MANY = 192, FEW = 64;                        // registers of a softmax thread and of another one: 512 threads have 128 each
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t bars[56];
+  __shared__ __align__(8) uint64_t bars[76];
   __shared__ int4 items[2];
   __shared__ __align__(16) uint4 claim;
   __shared__ uint32_t tmem_slot;
   __shared__ int odd_values, pieces;
-  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, qs = base, ks = qs + 128 * TILES * DK * 2, vs = ks + KU * kUnit, b0 = smem_u32(bars);
-  const uint32_t kfull = b0, kempty = b0 + 32, vfull = b0 + 64, vempty = b0 + 104, vok = b0 + 144, vraw = b0 + 184, qfull = b0 + 224, qempty = b0 + 240, odone = b0 + 256, ifull = b0 + 272,
-                 iempty = b0 + 288, sfull = b0 + 304, pfull = b0 + 336, pvdone = b0 + 368, flushed = b0 + 400, want = b0 + 432, claimed = b0 + 440;
-  // keys: a barrier for each of kAhead tiles; values: one for each place (vraw: where they land that are looked at ahead of their products); scores, weights, products: [row tile][place]
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, qs = base, ks = qs + kRows * TILES * DK * 2, vs = ks + KP * KB, b0 = smem_u32(bars);
+  const uint32_t kfull = b0, kempty = b0 + 64, vfull = b0 + 128, vempty = b0 + 192, vok = b0 + 256, vraw = b0 + 320, sfull = b0 + 384, pfull = b0 + 416, pvdone = b0 + 448, flushed = b0 + 480,
+                 qfull = b0 + 512, qempty = b0 + 528, odone = b0 + 544, ifull = b0 + 560, iempty = b0 + 576, want = b0 + 592, claimed = b0 + 600;
+  // keys and values: for each place (vraw: where values land that are looked at ahead of their products); scores, weights, products: [row tile][place]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tokens = TILES * P.tokens;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kAhead; i++) { mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); }
-    for (int i = 0; i < 5; i++) { mbar_init(vfull + 8 * i, 1); mbar_init(vempty + 8 * i, TILES); mbar_init(vok + 8 * i, 2); mbar_init(vraw + 8 * i, 1); }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); mbar_init(flushed + 16 * i, 1); mbar_init(flushed + 16 * i + 8, 1);
+    for (int i = 0; i < 8; i++) {
+      mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); mbar_init(vfull + 8 * i, 1); mbar_init(vempty + 8 * i, TILES); mbar_init(vok + 8 * i, 1); mbar_init(vraw + 8 * i, 1);
     }
+    for (int i = 0; i < 4; i++) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); mbar_init(flushed + 8 * i, 1); }
+    for (int i = 0; i < 2; i++) { mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); }
     mbar_init(want, 1);
     mbar_init(claimed, 1);
     odd_values = 0;
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [row tile][place][W], results [tile][DV]
+  const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [row tile][place][64], results [tile][DV]
   const long long all = (long long)pieces * P.units;
 
   uint32_t turn = 0;                                         // items that this warp has taken
@@ -185,106 +187,71 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const int t = scoring ? warp - 8 : warp - 11;
       const uint32_t lead = hy::tc_elect();
       const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);         // fp32 sums of bf16 or fp16, 128 rows
-      const uint32_t s_at = tmem + t * 128, done_at = pvdone + 16 * t;
-      uint32_t n_steps = 0, took = 0;                        // steps of the row tile behind, items that had rows
+      const uint32_t s_at = tmem + t * 2 * kTile, done_at = pvdone + 16 * t;
+      uint32_t passed = 0, took = 0, n = 0, par[2] = {0, 0};  // tiles behind that the row tile sees, items that had rows; the next tile's place and its parities (values: a bit for each place, as they came and looked at)
       Item w;
       bool alive = true;
-      if (scoring) {
-        const uint64_t q_desc = hy::tc_desc(qs + t * (kTile * DK * 2));
-        const int chunks = (P.dk + 63) / 64, ksteps = P.dk / 16;
-        const bool whole = ksteps == DK / 16;
-        uint32_t kt = 0, kn = 0;                             // tiles of keys behind, the next one's first place
-        while (alive && take(w)) {
-          const Walk k = walk_of(P, w, tokens);
-          const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
-          const bool there = a < w.len;
+      while (alive && take(w)) {
+        const Walk k = walk_of(P, w, tokens);
+        const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
+        const bool there = a < w.len;
+        auto sixteenths = [&](int key0) { return there && sees_some(P, a, b, key0) ? min(kTile / 16, (b - key0 + 16) / 16) : 0; };   // those of a tile that some row sees
+        if (scoring) {
+          const uint64_t q_desc = hy::tc_desc(qs + t * (kRows * DK * 2));
+          const int ksteps = P.dk / 16;
           alive = !there || wait_warp(qfull + 8 * t, took & 1, P.status);
           for (int i = 0; i < k.n && alive; i++) {
-            const int key0 = key_of(k, i);
-            uint64_t k_desc[DK / 64];
-#pragma unroll
-            for (int c = 0; c < DK / 64; c++) k_desc[c] = hy::tc_desc(ks + (kn + c < KU ? kn + c : kn + c - KU) * kUnit);
-            alive = wait_warp(kfull + 8 * (kt % kAhead), (kt / kAhead) & 1, P.status);
-#pragma unroll
-            for (int h = 0; h < PER; h++) {
-              if (!alive || !there || !sees_some(P, a, b, key0 + h * W, W)) continue;
-              const uint32_t place = n_steps & 1, at = s_at + place * W, sdesc = idesc | (uint32_t)(2 * min(W / 16, (b - key0 - h * W + 16) / 16)) << 17;   // (the rows see the first of them)
-              if (n_steps > 1) alive = wait_warp(done_at + 8 * place, ((n_steps >> 1) - 1) & 1, P.status);   // the weights that lie there are read
-              if (!alive) continue;
+            const int see = sixteenths(key_of(k, i));
+            const uint64_t k_desc = hy::tc_desc(ks + n * KB);
+            alive = wait_warp(kfull + 8 * n, par[0], P.status);
+            if (see && alive) {
+              const uint32_t place = passed & 1, at = s_at + place * kTile, sdesc = idesc | (uint32_t)(2 * see) << 17;
+              if (passed > 1) alive = wait_warp(done_at + 8 * place, ((passed >> 1) - 1) & 1, P.status);   // the weights that lie there are read
+              if (!alive) break;
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              if (whole) {
+              if (ksteps == DK / 16) {
 #pragma unroll
-                for (int c = 0; c < DK / 64; c++)
-#pragma unroll
-                  for (int u = 0; u < 4; u++) mma_ss(at, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + h * (W * 128 >> 4) + 2 * u, sdesc, c > 0 || u > 0, lead);
+                for (int u = 0; u < DK / 16; u++) mma_ss(at, q_desc + (u >> 2) * (kRows * 128 >> 4) + 2 * (u & 3), k_desc + (u >> 2) * (kTile * 128 >> 4) + 2 * (u & 3), sdesc, u > 0, lead);
               } else {
 #pragma unroll
-                for (int c = 0; c < DK / 64; c++)
-#pragma unroll
-                  for (int u = 0; u < 4; u++) if (4 * c + u < ksteps) mma_ss(at, q_desc + c * (kTile * 128 >> 4) + 2 * u, k_desc[c] + h * (W * 128 >> 4) + 2 * u, sdesc, c > 0 || u > 0, lead);
+                for (int u = 0; u < DK / 16; u++) if (u < ksteps) mma_ss(at, q_desc + (u >> 2) * (kRows * 128 >> 4) + 2 * (u & 3), k_desc + (u >> 2) * (kTile * 128 >> 4) + 2 * (u & 3), sdesc, u > 0, lead);
               }
               commit(sfull + 16 * t + 8 * place, lead);
-              n_steps++;
+              passed++;
             }
-            if (there) commit(kempty + 8 * (kt % kAhead), lead);       // (stands for all products ahead of it)
-            else if (lead) hy::tc_arrive(kempty + 8 * (kt % kAhead));
-            kt++;
-            kn += chunks;
-            if (kn >= KU) kn -= KU;
+            if (there) commit(kempty + 8 * n, lead);         // (stands for all products ahead of it)
+            else if (lead) hy::tc_arrive(kempty + 8 * n);
+            if (++n == KP) { n = 0; par[0] ^= 1; }
           }
           if (there && alive) { commit(qempty + 8 * t, lead); took++; }
-        }
-      } else {
-        const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17), to = o_at + t * 128;
-        constexpr int UNITS = W >= VK ? W / VK : 1, EACH = W >= VK ? 1 : VK / W;   // units of a step, or steps of a unit
-        uint32_t vn = 0, vpar[2] = {0, 0};                   // the next unit's place, parities (a bit for each place: as they came, looked at)
-        while (alive && take(w)) {
-          const Walk k = walk_of(P, w, tokens);
-          const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
-          const bool there = a < w.len;
+        } else {
+          const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17), to = o_at + t * 128;
           bool any = false;
           for (int i = 0; i < k.n && alive; i++) {
-            const int key0 = key_of(k, i);
-            const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0, kTile);
-#pragma unroll
-            for (int h = 0; h < PER; h++) {
-              const int first = key0 + h * W, n = there && sees_some(P, a, b, first, W) ? min(W / 16, (b - first + 16) / 16) : 0;   // sixteenths that some row sees
-              uint64_t v_desc[UNITS];
-#pragma unroll
-              for (int u = 0; u < UNITS; u++) {
-                const uint32_t at = vn + u < VU ? vn + u : vn + u - VU;
-                if (h % EACH == 0) {
-                  alive = alive && wait_warp((masked ? vok : vfull) + 8 * at, (masked ? vpar[1] : vpar[0]) >> at & 1, P.status);
-                  if (masked) vpar[1] ^= 1u << at; else vpar[0] ^= 1u << at;
-                }
-                v_desc[u] = value_desc(vs + at * kUnit + h % EACH * (W * 128), VK);
-              }
-              if (n) {
-                const uint32_t place = n_steps & 1, weights = s_at + place * W;
-                alive = alive && wait_warp(pfull + 16 * t + 8 * place, (n_steps >> 1) & 1, P.status);
-                if (!alive) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (n == W / 16) {
-#pragma unroll
-                  for (int u = 0; u < W / 16; u++) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
-                } else {
-#pragma unroll
-                  for (int u = 0; u < W / 16; u++) if (u < n) mma_ts(to, weights + u * 8, v_desc[UNITS == 1 ? 0 : u / STEPS] + (UNITS == 1 ? u : u % STEPS) * 128, pdesc, any || u > 0, lead);
-                }
-                commit(done_at + 8 * place, lead);
-                n_steps++;
-                any = true;
-              }
+            const int key0 = key_of(k, i), see = sixteenths(key0);
+            const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0);
+            const uint64_t v_desc = value_desc(vs + n * VB);
+            alive = wait_warp((masked ? vok : vfull) + 8 * n, (masked ? par[1] : par[0]) >> n & 1, P.status);
+            if (masked) par[1] ^= 1u << n; else par[0] ^= 1u << n;
+            if (see && alive) {
+              const uint32_t place = passed & 1, weights = s_at + place * kTile;
+              alive = wait_warp(pfull + 16 * t + 8 * place, (passed >> 1) & 1, P.status);
               if (!alive) break;
-              if (h % EACH == EACH - 1) {
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              if (see == kTile / 16) {
 #pragma unroll
-                for (int u = 0; u < UNITS; u++) {
-                  if (there) commit(vempty + 8 * vn, lead);
-                  else if (lead) hy::tc_arrive(vempty + 8 * vn);
-                  if (++vn == VU) vn = 0;
-                }
+                for (int u = 0; u < kTile / 16; u++) mma_ts(to, weights + u * 8, v_desc + u * 128, pdesc, any || u > 0, lead);
+              } else {
+#pragma unroll
+                for (int u = 0; u < kTile / 16; u++) if (u < see) mma_ts(to, weights + u * 8, v_desc + u * 128, pdesc, any || u > 0, lead);
               }
+              commit(done_at + 8 * place, lead);
+              passed++;
+              any = true;
             }
+            if (there) commit(vempty + 8 * n, lead);
+            else if (lead) hy::tc_arrive(vempty + 8 * n);
+            if (++n == VP) n = 0;
           }
           if (there && alive) commit(odone + 8 * t, lead);
         }
@@ -292,70 +259,63 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const uint32_t last = flushed + 16 * t + (scoring ? 0 : 8);
       commit(last, lead);                                    // no product is under way when TMEM is given back
       wait_warp(last, 0, P.status);
-    } else if (warp == 10) {                                 // copies: a tile of values behind the next one of keys
+    } else if (warp == 10) {                                 // copies of keys and queries
       Item w;
-      const int chunks = (P.dk + 63) / 64, boxes = (P.dv + 63) / 64;
-      uint32_t kn = 0, vn = 0, par = 0, took[2] = {0, 0}, vpar[2] = {0, 0}, vsent[2] = {0, 0};
-      int tile = 0, freed = 0, sent = 0;                     // tiles of keys begun and given back, units sent
+      const int chunks = (P.dk + 63) / 64;
+      uint32_t n = 0, par = 0, took[2] = {0, 0}, sent = 0;
       bool alive = true;
       while (alive && take(w)) {
         const Walk k = walk_of(P, w, tokens);
         const int head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack;
-        auto keys = [&](int i) {
-          for (int c = 0; c < chunks; c++) {
-            while (freed + kAhead <= tile || freed * chunks + KU <= sent) {   // the barrier's last tile, and the unit that lies where this one goes
-              alive = wait_warp(kempty + 8 * (freed % kAhead), (freed / kAhead) & 1, P.status);
-              if (!alive) return;
-              freed++;
-            }
-            if (lane == 0) {
-              if (c == 0) mbar_expect_tx(kfull + 8 * (tile % kAhead), chunks * kUnit);
-              copy_box(ks + kn * kUnit, &P.k, 64 * c, head, w.row + key_of(k, i), kfull + 8 * (tile % kAhead));
-            }
-            sent++;
-            if (++kn == KU) kn = 0;
-          }
-          tile++;
-        };
-        auto values = [&](int i) {
-          const int key0 = key_of(k, i);
-          const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0, kTile);
-          const uint32_t full = masked ? vraw : vfull;
-          for (int u = 0; u < kTile / VK && alive; u++) {
-            alive = wait_warp(vempty + 8 * vn, par ^ 1, P.status);
-            if (!alive) return;
-            if (lane == 0) {
-              mbar_expect_tx(full + 8 * vn, boxes * VK * 128);
-              for (int c = 0; c < boxes; c++) copy_box(vs + vn * kUnit + c * (VK * 128), &P.v, 64 * c, head, w.row + key0 + u * VK, full + 8 * vn);
-            }
-            vpar[masked] ^= 1u << vn;
-            vsent[masked] |= 1u << vn;
-            if (++vn == VU) { vn = 0; par ^= 1; }
-          }
-        };
-        keys(0);
-        if (k.n <= kEarly && lane == 0) hy::tc_arrive(want);
-        for (int t = 0; t < TILES && alive; t++) {
-          if (w.tok + t * P.tokens >= w.len) continue;
-          alive = wait_warp(qempty + 8 * t, (took[t] & 1) ^ 1, P.status);
+        for (int i = 0; i < k.n && alive; i++) {
+          alive = wait_warp(kempty + 8 * n, par ^ 1, P.status);
           if (!alive) break;
           if (lane == 0) {
-            mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
-            for (int c = 0; c < chunks; c++) copy_box(qs + t * (kTile * DK * 2) + c * (kTile * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
+            mbar_expect_tx(kfull + 8 * n, chunks * kTile * 128);
+            for (int c = 0; c < chunks; c++) copy_box(ks + n * KB + c * (kTile * 128), &P.k, 64 * c, head, w.row + key_of(k, i), kfull + 8 * n);
           }
-          took[t]++;
+          sent |= 1u << n;
+          if (++n == KP) { n = 0; par ^= 1; }
+          if (i == max(0, k.n - kEarly) && lane == 0) hy::tc_arrive(want);
+          for (int t = 0; t < TILES && alive && i == 0; t++) {
+            if (w.tok + t * P.tokens >= w.len) continue;
+            alive = wait_warp(qempty + 8 * t, (took[t] & 1) ^ 1, P.status);
+            if (!alive) break;
+            if (lane == 0) {
+              mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
+              for (int c = 0; c < chunks; c++) copy_box(qs + t * (kRows * DK * 2) + c * (kRows * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
+            }
+            took[t]++;
+          }
         }
-        for (int i = 1; i < k.n && alive; i++) {
-          if (i == k.n - kEarly && lane == 0) hy::tc_arrive(want);
-          keys(i);
-          if (alive) values(i - 1);
-        }
-        if (alive) values(k.n - 1);
       }
       for (int t = 0; t < TILES; t++) if (took[t]) wait_warp(qfull + 8 * t, (took[t] - 1) & 1, P.status);   // no copy is under way at the end, whatever happened
-      for (int s = max(0, tile - kAhead); s < tile; s++) wait_warp(kfull + 8 * (s % kAhead), (s / kAhead) & 1, P.status);
-      for (uint32_t s = 0; s < 2 * VU; s++)
-        if (vsent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
+      for (uint32_t s = 0; s < KP; s++) if (sent >> s & 1) wait_warp(kfull + 8 * s, s < n ? par : par ^ 1, P.status);
+    } else if (warp == 13) {                                 // copies of values
+      Item w;
+      const int boxes = (P.dv + 63) / 64;
+      uint32_t n = 0, par = 0, vpar[2] = {0, 0}, sent[2] = {0, 0};
+      bool alive = true;
+      while (alive && take(w)) {
+        const Walk k = walk_of(P, w, tokens);
+        const int head = w.unit / P.subs;
+        for (int i = 0; i < k.n && alive; i++) {
+          const int key0 = key_of(k, i);
+          const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0);
+          const uint32_t full = masked ? vraw : vfull;
+          alive = wait_warp(vempty + 8 * n, par ^ 1, P.status);
+          if (!alive) break;
+          if (lane == 0) {
+            mbar_expect_tx(full + 8 * n, boxes * kTile * 128);
+            for (int c = 0; c < boxes; c++) copy_box(vs + n * VB + c * (kTile * 128), &P.v, 64 * c, head, w.row + key0, full + 8 * n);
+          }
+          vpar[masked] ^= 1u << n;
+          sent[masked] |= 1u << n;
+          if (++n == VP) { n = 0; par ^= 1; }
+        }
+      }
+      for (uint32_t s = 0; s < 2 * VP; s++)                  // no copy is under way at the end, whatever happened
+        if (sent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
     } else if (warp == 15) {                                 // deals out the work: rows with most keys first, so that the short ones fill the gaps
       // CTAs take over work of CTAs that have not started yet, each when its copies near the end of what it has
       long long at = blockIdx.x;
@@ -398,39 +358,34 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         __syncwarp();
         at = got ? (long long)next : all;
       }
-    } else if (warp >= 13) {                                 // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
+    } else if (warp == 14) {                                 // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
       Item w;
-      const int me = threadIdx.x - 13 * 32, boxes = (P.dv + 63) / 64;
+      const int boxes = (P.dv + 63) / 64;
       const uint32_t inf = BF16 ? 0x7f807f80u : 0x7c007c00u;
       uint32_t n = 0, par = 0;                               // par: a bit for each place
       bool alive = true;
       while (alive && take(w)) {
         const Walk k = walk_of(P, w, tokens);
-        for (int i = 0; i < k.n && alive; i++) {
+        for (int i = 0; i < k.n && alive; i++, n = n + 1 == VP ? 0 : n + 1) {
           const int key0 = key_of(k, i);
-          const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0, kTile);
-          for (int u = 0; u < kTile / VK && alive; u++) {
-            if (masked) {
-              alive = wait_warp(vraw + 8 * n, par >> n & 1, P.status);
-              par ^= 1u << n;
-              const int first = key0 + u * VK;
-              bool odd = false;
-              for (int p = me; p < boxes * VK * 8; p += 64) {  // 16-byte pieces: eight to a row of 64 columns
-                const int row = first + ((p >> 3) & (VK - 1));
-                const uint32_t at = vs + n * kUnit + p * 16;
-                const uint4 x = lds128(at);
-                uint32_t y[4] = {x.x, x.y, x.z, x.w}, z[4], hit = 0;
+          if (sees_all(P, w.tok, k.t1 - 1, key0)) continue;
+          alive = wait_warp(vraw + 8 * n, par >> n & 1, P.status);
+          par ^= 1u << n;
+          bool odd = false;
+#pragma unroll 4
+          for (int p = lane; p < boxes * kTile * 8; p += 32) {   // 16-byte pieces: eight to a row of 64 columns
+            const int row = key0 + ((p >> 3) & (kTile - 1));
+            const uint32_t at = vs + n * VB + p * 16;
+            const uint4 x = lds128(at);
+            uint32_t y[4] = {x.x, x.y, x.z, x.w}, z[4], hit = 0;
 #pragma unroll
-                for (int e = 0; e < 4; e++) { z[e] = row < w.len ? __vcmpeq2(y[e] & inf, inf) : 0xffffffffu; hit |= z[e]; y[e] &= ~z[e]; }
-                if (hit) { sts128(at, y[0], y[1], y[2], y[3]); odd |= row < w.len; }
-              }
-              if (odd) odd_values = 1;
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0) hy::tc_arrive(vok + 8 * n);
-            }
-            if (++n == VU) n = 0;
+            for (int e = 0; e < 4; e++) { z[e] = row < w.len ? __vcmpeq2(y[e] & inf, inf) : 0xffffffffu; hit |= z[e]; y[e] &= ~z[e]; }
+            if (hit) { sts128(at, y[0], y[1], y[2], y[3]); odd |= row < w.len; }
           }
+          if (odd) odd_values = 1;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) hy::tc_arrive(vok + 8 * n);
         }
       }
     }
@@ -450,11 +405,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const bool mine = pos < w.len, idle = !__any_sync(0xffffffffu, mine);
       float m = kLowest, l = 0.f, limit = -INFINITY;         // limit: where a maximum moves the reference; any does while that is beyond kFar
       bool any = false;
-      for (int step = 0; step < k.n * PER; step++) {
-        const int key0 = key_of(k, step / PER) + step % PER * W;
-        if (!sees_some(P, a, b, key0, W)) continue;
-        const uint32_t place = passed & 1, s_at = tmem + t * 128 + place * W + lanes, p_bar = pfull + 16 * t + 8 * place;
-        const bool masked = !sees_all(P, a, b, key0, W);
+      for (int i = 0; i < k.n; i++) {
+        const int key0 = key_of(k, i);
+        if (!sees_some(P, a, b, key0)) continue;
+        const uint32_t place = passed & 1, s_at = tmem + (2 * t + place) * kTile + lanes, p_bar = pfull + 16 * t + 8 * place;
+        const bool masked = !sees_all(P, a, b, key0);
         ok = wait_warp(sfull + 16 * t + 8 * place, (passed >> 1) & 1, P.status);
         if (!ok) break;
         if (idle) {                                          // (its rows' results are whatever comes of the scores as weights, and go nowhere)
@@ -464,12 +419,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
           continue;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t x[W];
-        tmem_ask<0, W>(s_at, x);
-        tmem_got<0, W>(x);
+        uint32_t x[kTile];
+        tmem_ask<0, kTile>(s_at, x);
+        tmem_got<0, kTile>(x);
         if (masked) {                                        // keys that the row sees, a bit each: not behind its own, in the window or among the first
 #pragma unroll
-          for (int u = 0; u < W; u += 32) {
+          for (int u = 0; u < kTile; u += 32) {
             const int j = key0 + u;
             uint32_t see = lower_bits(pos + 1 - j);
             if (P.window > 0) see &= ~lower_bits(pos - P.window + 1 - j) | lower_bits(P.keep - j);
@@ -479,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         }
         float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < W; e += 8)
+        for (int e = 0; e < kTile; e += 8)
 #pragma unroll
           for (int g = 0; g < 4; g++) y[g] = max3(__float_as_uint(y[g]), x[e + 2 * g], x[e + 2 * g + 1]);
         const float top = mine ? fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * P.f : -INFINITY;
@@ -492,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
           limit = far ? -INFINITY : m + ROOM;
           if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
-            for (int e = 0; e < W; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+            for (int e = 0; e < kTile; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
             f = 1.f;
           }
           if (any) {
@@ -512,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         const uint64_t f2 = both(f, f), off = both(-m, -m);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int u = 0; u < W / 32; u++) {
+        for (int u = 0; u < kTile / 32; u++) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) {

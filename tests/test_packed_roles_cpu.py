@@ -20,22 +20,22 @@ class Bar:
         return lambda: (self.phase & 1) != parity & 1
 
 
-AHEAD, EARLY = 4, 4                                          # tiles of keys under way, tiles ahead of the end at which more work is asked for
-SHAPES = {64: (2, 1, 1, 6, 5), 128: (2, 2, 2, 6, 4), 192: (2, 3, 2, 5, 3), 256: (1, 4, 4, 6, 4)}      # row tiles, units of keys and of values a tile, places for them
+EARLY = 8                                                    # tiles ahead of the end at which more work is asked for
+SHAPES = {64: (2, 8, 8), 128: (2, 6, 4), 192: (2, 3, 3), 256: (1, 3, 2)}      # row tiles, places of keys and of values
 
 
 def run(rng, dk, work, idle, moves, early=True):
-    """work: items, each a list of (tiles of keys: (for each of its steps, the row tiles that see some of it; whether some row does not see all)) and whether the second row tile has rows.  idle:
-    softmax warps without rows; early: the wait for the product ahead, where a reference moves."""
-    tiles, per_k, per_v, KU, VU = SHAPES[dk]
+    """work: items, each a list of (tiles of keys: (row tiles that see some of it, whether some row does not see all)) and whether the second row tile has rows.  idle: softmax warps without rows;
+    early: the wait for the product ahead, where a reference moves."""
+    tiles, KP, VP = SHAPES[dk]
     bars = lambda n, count: [Bar(count) for _ in range(n)]
-    soft, per = 4 * tiles, tiles                             # steps of a tile: two with two row tiles, of half as many keys
-    kfull, kempty, vfull, vempty, vok, vraw = bars(AHEAD, 1), bars(AHEAD, tiles), bars(VU, 1), bars(VU, tiles), bars(VU, 2), bars(VU, 1)
+    soft = 4 * tiles
+    kfull, kempty, vfull, vempty, vok, vraw = bars(KP, 1), bars(KP, tiles), bars(VP, 1), bars(VP, tiles), bars(VP, 1), bars(VP, 1)
     qfull, qempty, odone, ifull = (bars(2, 1) for _ in range(4))
     sfull, pvdone, pfull = ([bars(2, n) for _ in range(2)] for n in (1, 1, 4))            # [row tile][place]
     iempty, flushed = bars(2, soft + 2 * tiles + 3), [bars(2, 1) for _ in range(2)]
     items, want = [None, None], Bar(1)
-    keys, values, queries, looked = [None] * KU, [None] * VU, [None] * 2, [0] * VU
+    keys, values, queries, looked = [None] * KP, [None] * VP, [None] * 2, [0] * VP
     scores, weights, through = [[None, None], [None, None]], [[{}, {}], [{}, {}]], [[], []]       # [row tile][place], steps whose product is through
     queue, flying = [], []                                   # products and commits in the order of their issue; copies in any order
 
@@ -56,92 +56,77 @@ def run(rng, dk, work, idle, moves, early=True):
                 yield want.wait(r)
                 yield None                                   # (the claim)
 
-    def copies():
-        me, took, vn, par = {"turn": 0}, [0, 0], 0, 0
-        at = {"n": 0, "tile": 0, "freed": 0, "sent": 0}
+    def copy_keys():
+        me, took, at, par = {"turn": 0}, [0, 0], 0, 0
         while True:
             yield from take(me)
             n = me["item"]
             if n is None:
                 return
             walk, two = work[n]
-
-            def tile(i):
-                bar = kfull[at["tile"] % AHEAD]
-                units = Bar(per_k)                           # (the barrier counts bytes: its phase ends with the last unit)
-                for c in range(per_k):
-                    while at["freed"] + AHEAD <= at["tile"] or at["freed"] * per_k + KU <= at["sent"]:
-                        yield kempty[at["freed"] % AHEAD].wait(at["freed"] // AHEAD)
-                        at["freed"] += 1
-                    flying.append((keys, at["n"], (n, i, c), (units, bar)))
-                    keys[at["n"]] = "under way"
-                    at["sent"] += 1
-                    at["n"] = (at["n"] + 1) % KU
-                at["tile"] += 1
-
-            def some(i, vn, par):
-                for c in range(per_v):
-                    yield vempty[vn].wait(par ^ 1)
-                    looked[vn] = 0
-                    flying.append((values, vn, (n, i, c), (vraw if walk[i][1] else vfull)[vn]))
-                    values[vn] = "under way"
-                    vn, par = (0, par ^ 1) if vn + 1 == VU else (vn + 1, par)
-                return vn, par
-
-            yield from tile(0)
-            if len(walk) <= EARLY:
-                want.arrive()
-            for t in range(tiles):
-                if t and not two:
-                    continue
-                yield qempty[t].wait((took[t] & 1) ^ 1)
-                flying.append((queries, t, n, qfull[t]))
-                queries[t] = "under way"
-                took[t] += 1
-            for i in range(1, len(walk)):
-                if i == len(walk) - EARLY:
+            for i in range(len(walk)):
+                yield kempty[at].wait(par ^ 1)
+                flying.append((keys, at, (n, i), kfull[at]))
+                keys[at] = "under way"
+                at, par = (0, par ^ 1) if at + 1 == KP else (at + 1, par)
+                if i == max(0, len(walk) - EARLY):
                     want.arrive()
-                yield from tile(i)
-                vn, par = yield from some(i - 1, vn, par)
-            vn, par = yield from some(len(walk) - 1, vn, par)
+                for t in range(tiles if i == 0 else 0):
+                    if t and not two:
+                        continue
+                    yield qempty[t].wait((took[t] & 1) ^ 1)
+                    flying.append((queries, t, n, qfull[t]))
+                    queries[t] = "under way"
+                    took[t] += 1
 
-    def look(_):
-        me, n, par = {"turn": 0}, 0, [0] * VU
+    def copy_values():
+        me, at, par = {"turn": 0}, 0, 0
         while True:
             yield from take(me)
-            if me["item"] is None:
+            n = me["item"]
+            if n is None:
                 return
-            for i, (_, masked) in enumerate(work[me["item"]][0]):
-                for c in range(per_v):
-                    if masked:
-                        yield vraw[n].wait(par[n])
-                        par[n] ^= 1
-                        assert values[n] == (me["item"], i, c)
-                        yield None
-                        looked[n] += 1
-                        vok[n].arrive()
-                    n = (n + 1) % VU
+            for i, (_, masked) in enumerate(work[n][0]):
+                yield vempty[at].wait(par ^ 1)
+                looked[at] = 0
+                flying.append((values, at, (n, i), (vraw if masked else vfull)[at]))
+                values[at] = "under way"
+                at, par = (0, par ^ 1) if at + 1 == VP else (at + 1, par)
 
-    def product_of_scores(t, n, step, c, place, at):
+    def look():
+        me, at, par = {"turn": 0}, 0, [0] * VP
+        while True:
+            yield from take(me)
+            n = me["item"]
+            if n is None:
+                return
+            for i, (_, masked) in enumerate(work[n][0]):
+                if masked:
+                    yield vraw[at].wait(par[at])
+                    par[at] ^= 1
+                    assert values[at] == (n, i)
+                    yield None
+                    looked[at] += 1
+                    vok[at].arrive()
+                at = (at + 1) % VP
+
+    def product_of_scores(t, n, i, unit, at):
         def product():
-            assert keys[place] == (n, step // per, c) and queries[t] == n
-            if c == 0:
-                assert scores[t][at] is None or scores[t][at] in through[t]      # what lay there was handed over and read
-                scores[t][at], weights[t][at] = None, {}
-            if c == per_k - 1:
-                scores[t][at] = (n, step)
+            assert keys[unit] == (n, i) and queries[t] == n
+            assert scores[t][at] is None or scores[t][at] in through[t]          # what lay there was handed over and read
+            scores[t][at], weights[t][at] = (n, i), {}
         return product
 
-    def product_of_results(t, n, step, units, at, masked):
+    def product_of_results(t, n, i, unit, at, masked):
         def product():
-            assert all(values[place] == (n, step // per, c) and (not masked or looked[place] == 2) for c, place in units)
-            assert scores[t][at] == (n, step) and all(idle[n][4 * t + w] or weights[t][at].get(w) == (n, step) for w in range(4))
-            through[t].append((n, step))
+            assert values[unit] == (n, i) and (not masked or looked[unit] == 1)
+            assert scores[t][at] == (n, i) and all(idle[n][4 * t + w] or weights[t][at].get(w) == (n, i) for w in range(4))
+            through[t].append((n, i))
         return product
 
     def scorer(t):
         me = {"turn": 0}
-        kt = kn = steps = took = 0
+        kn = par = passed = took = 0
         while True:
             yield from take(me)
             n = me["item"]
@@ -152,20 +137,18 @@ def run(rng, dk, work, idle, moves, early=True):
             if there:
                 yield qfull[t].wait(took)
             for i, (who, _) in enumerate(walk):
-                yield kfull[kt % AHEAD].wait(kt // AHEAD)
-                for h in range(per):
-                    if not there or t not in who[h]:
-                        continue
-                    at = steps & 1
-                    if steps > 1:
-                        yield pvdone[t][at].wait((steps >> 1) - 1)
-                    queue.extend([product_of_scores(t, n, i * per + h, c, (kn + c) % KU, at) for c in range(per_k)] + [sfull[t][at]])
-                    steps += 1
+                yield kfull[kn].wait(par)
+                if there and t in who:
+                    at = passed & 1
+                    if passed > 1:
+                        yield pvdone[t][at].wait((passed >> 1) - 1)
+                    queue.extend([product_of_scores(t, n, i, kn, at), sfull[t][at]])
+                    passed += 1
                 if there:
-                    queue.append(kempty[kt % AHEAD])
+                    queue.append(kempty[kn])
                 else:
-                    kempty[kt % AHEAD].arrive()
-                kt, kn = kt + 1, (kn + per_k) % KU
+                    kempty[kn].arrive()
+                kn, par = (0, par ^ 1) if kn + 1 == KP else (kn + 1, par)
             if there:
                 queue.append(qempty[t])
                 took += 1
@@ -174,9 +157,8 @@ def run(rng, dk, work, idle, moves, early=True):
 
     def adder(t):
         me = {"turn": 0}
-        vn = steps = 0
-        vpar = [[0] * VU, [0] * VU]
-        units, each = max(1, per_v // per), max(1, per // per_v)                  # units of a step, steps of a unit
+        vn = passed = 0
+        par = [[0] * VP, [0] * VP]
         while True:
             yield from take(me)
             n = me["item"]
@@ -185,24 +167,18 @@ def run(rng, dk, work, idle, moves, early=True):
             walk, two = work[n]
             there = t == 0 or two
             for i, (who, masked) in enumerate(walk):
-                for h in range(per):
-                    places = [(vn + u) % VU for u in range(units)]
-                    if h % each == 0:
-                        for place in places:
-                            yield (vok if masked else vfull)[place].wait(vpar[masked][place])
-                            vpar[masked][place] ^= 1
-                    if there and t in who[h]:
-                        at, first = steps & 1, h * units if each == 1 else 0
-                        yield pfull[t][at].wait(steps >> 1)
-                        queue.extend([product_of_results(t, n, i * per + h, [(first + u, place) for u, place in enumerate(places)], at, masked), pvdone[t][at]])
-                        steps += 1
-                    if h % each == each - 1:
-                        for place in places:
-                            if there:
-                                queue.append(vempty[place])
-                            else:
-                                vempty[place].arrive()
-                        vn = (vn + units) % VU
+                yield (vok if masked else vfull)[vn].wait(par[masked][vn])
+                par[masked][vn] ^= 1
+                if there and t in who:
+                    at = passed & 1
+                    yield pfull[t][at].wait(passed >> 1)
+                    queue.extend([product_of_results(t, n, i, vn, at, masked), pvdone[t][at]])
+                    passed += 1
+                if there:
+                    queue.append(vempty[vn])
+                else:
+                    vempty[vn].arrive()
+                vn = (vn + 1) % VP
             if there:
                 queue.append(odone[t])
         queue.append(flushed[1][t])
@@ -221,8 +197,8 @@ def run(rng, dk, work, idle, moves, early=True):
             if t and not two:
                 continue
             last = None
-            for step in range(len(walk) * per):
-                if t not in walk[step // per][0][step % per]:
+            for step, (who, _) in enumerate(walk):
+                if t not in who:
                     continue
                 at = passed & 1
                 yield sfull[t][at].wait(passed >> 1)
@@ -247,7 +223,7 @@ def run(rng, dk, work, idle, moves, early=True):
                 assert through[t][-1:] == [last]
                 yield None
 
-    roles = [deal(), copies(), *(scorer(t) for t in range(tiles)), *(adder(t) for t in range(tiles))] + [look(k) for k in range(2)] + [softmax(x) for x in range(soft)]
+    roles = [deal(), copy_keys(), copy_values(), *(scorer(t) for t in range(tiles)), *(adder(t) for t in range(tiles)), look()] + [softmax(x) for x in range(soft)]
     speed = [rng.choice([1, 1, 1, 10, 0.05]) for _ in roles] + [rng.choice([1, 0.1, 10]) for _ in range(2)]
     at = [next(r, False) for r in roles]                      # what a role waits for: a test, None, or False at its end
     while queue or flying or any(a is not False for a in at):
@@ -260,12 +236,7 @@ def run(rng, dk, work, idle, moves, early=True):
         elif k > len(roles):
             where, place, what, bar = flying.pop(rng.randrange(len(flying)))
             where[place] = what
-            if isinstance(bar, tuple):
-                bar[0].arrive()
-                if bar[0].phase:
-                    bar[1].arrive()
-            else:
-                bar.arrive()
+            bar.arrive()
         else:
             at[k] = next(roles[k], False)
 
@@ -275,8 +246,8 @@ def draw(rng, dk):
     work, idle = [], []
     for _ in range(rng.randint(1, 5)):
         two = tiles == 2 and rng.random() < 0.8
-        walk = [([{0} if not two else rng.choice([{0, 1}, {0, 1}, {0, 1}, {0}, {1}, set()]) for _ in range(tiles)], rng.random() < 0.4) for _ in range(rng.randint(1, 7))]
-        walk[0][0][0] = {0, 1} if two else {0}               # (a row tile that has rows sees something)
+        walk = [({0} if not two else rng.choice([{0, 1}, {0, 1}, {0, 1}, {0}, {1}]), rng.random() < 0.4) for _ in range(rng.randint(1, 12))]
+        walk[0] = ({0, 1} if two else {0}, walk[0][1])       # (a row tile that has rows sees something)
         work.append((walk, two))
         row = [rng.random() < 0.2 for _ in range(4 * tiles)]
         row[0] = False                                       # (a row tile that has rows has its first)

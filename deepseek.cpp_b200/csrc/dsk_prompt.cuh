@@ -92,7 +92,7 @@ __device__ __forceinline__ bool sees_some(const Params& P, int a, int b, int key
 }
 
 // Infinities and NaN among the values that a row sees in tiles where they went to the products as zeros: its results c .. c + 15 become what they make of them
-template <bool BF16> __device__ __noinline__ void give_back(const Params& P, const Item& w, const Walk& k, int pos, int head, int c, uint32_t (&x)[16]) {
+template <bool BF16> __device__ __noinline__ void give_back(const Params& P, const Item& w, const Walk& k, int pos, int head, int c, float (&x)[16]) {
   for (int i = 0; i < k.n; i++) {
     const int key0 = key_of(k, i);
     if (sees_all(P, w.tok, k.t1 - 1, key0)) continue;
@@ -102,7 +102,7 @@ template <bool BF16> __device__ __noinline__ void give_back(const Params& P, con
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         const uint32_t u = v[e];
-        if (BF16 ? (u & 0x7f80u) == 0x7f80u : (u & 0x7c00u) == 0x7c00u) x[e] = __float_as_uint(__uint_as_float(x[e]) + (BF16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u))));
+        if (BF16 ? (u & 0x7f80u) == 0x7f80u : (u & 0x7c00u) == 0x7c00u) x[e] += BF16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
       }
     }
   }
@@ -502,14 +502,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         if (!mine) continue;
 #pragma unroll
         for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * inv);
-        if (odd) give_back<BF16>(P, w, k, pos, head, c, x);
+        if (odd) {                                           // (a copy: what a call is given by address lies in memory)
+          float z[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) z[e] = __uint_as_float(x[e]);
+          give_back<BF16>(P, w, k, pos, head, c, z);
+#pragma unroll
+          for (int e = 0; e < 16; e++) x[e] = __float_as_uint(z[e]);
+        }
         uint32_t y[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) y[e] = pair<BF16>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-        if (P.wide_o) {
-          uint4* at = reinterpret_cast<uint4*>(to + c);
-          at[0] = make_uint4(y[0], y[1], y[2], y[3]);
-          at[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        if (P.wide_o) {                                      // (whole sectors: in two pieces of 16 bytes the results of a short prompt took longer than all else)
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + c), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
         } else {
 #pragma unroll
           for (int e = 0; e < 8; e++) { to[c + 2 * e] = (uint16_t)y[e]; to[c + 2 * e + 1] = (uint16_t)(y[e] >> 16); }

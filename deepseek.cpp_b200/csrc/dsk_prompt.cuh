@@ -140,11 +140,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   // How many pieces of work there are: row tiles that are the j-th or a later one of their sequence, of all sequences
-  int held[kHeld], most = 0;                                 // (the dealing warp's: row tiles of sequences lane, lane + 32, ..)
+  int first[kHeld], size[kHeld], held[kHeld], most = 0;      // (the dealing warp's: first row, rows and row tiles of sequences lane, lane + 32, ..)
+  auto rows_of = [&](int b, int& from) {                     // whatever starts say, inside
+    from = b < P.batch ? min(max(P.starts[b], 0), P.rows) : 0;
+    return b < P.batch ? min(max(P.starts[b + 1], from), P.rows) - from : 0;
+  };
   auto tiles_of = [&](int b) {
-    if (b >= P.batch) return 0;
-    const int from = min(max(P.starts[b], 0), P.rows), to = min(max(P.starts[b + 1], from), P.rows);
-    return (to - from + tokens - 1) / tokens;
+    int from;
+    return (rows_of(b, from) + tokens - 1) / tokens;
   };
   auto from_level = [&](int j) {
     int n = 0;
@@ -155,7 +158,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   };
   if (warp == 15) {
 #pragma unroll
-    for (int i = 0; i < kHeld; i++) { held[i] = tiles_of(lane + 32 * i); most = max(most, held[i]); }
+    for (int i = 0; i < kHeld; i++) {
+      size[i] = rows_of(lane + 32 * i, first[i]);
+      held[i] = (size[i] + tokens - 1) / tokens;
+      most = max(most, held[i]);
+    }
     for (int b = lane + 32 * kHeld; b < P.batch; b += 32) most = max(most, tiles_of(b));
     most = __reduce_max_sync(0xffffffffu, most);
     const int n = from_level(0);
@@ -329,18 +336,25 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             if (from_level(mid) > k) lo = mid; else hi = mid - 1;
           }
           most = lo + 1;                                     // (later ones lie no higher)
-          int rank = k - from_level(lo + 1), b = -1;
-          for (int c = 0; b < 0 && c < P.batch; c += 32) {
-            const bool has = tiles_of(c + lane) > lo;
-            const uint32_t mask = __ballot_sync(0xffffffffu, has);
-            const uint32_t hit = __ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1)) == rank);
-            if (hit) b = c + __ffs(hit) - 1;
+          int rank = k - from_level(lo + 1), from = 0, len = 0;      // the rank-th sequence with more than lo row tiles
+          bool found = false;
+          auto among = [&](bool has, int row, int rows) {
+            const uint32_t mask = __ballot_sync(0xffffffffu, has), hit = __ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1)) == rank);
+            if (!found && hit) {
+              from = __shfl_sync(0xffffffffu, row, __ffs(hit) - 1);
+              len = __shfl_sync(0xffffffffu, rows, __ffs(hit) - 1);
+              found = true;
+            }
             rank -= __popc(mask);
+          };
+#pragma unroll
+          for (int i = 0; i < kHeld; i++) if (!found && 32 * i < P.batch) among(held[i] > lo, first[i], size[i]);
+          for (int c = 32 * kHeld; c < P.batch && !found; c += 32) {
+            int row;
+            const int rows = rows_of(c + lane, row);
+            among((rows + tokens - 1) / tokens > lo, row, rows);
           }
-          if (b >= 0) {
-            const int from = min(max(P.starts[b], 0), P.rows), to = min(max(P.starts[b + 1], from), P.rows);
-            item = make_int4(from, to - from, lo * tokens, (int)(at - (long long)k * P.units));
-          }
+          if (found) item = make_int4(from, len, lo * tokens, (int)(at - (long long)k * P.units));
         }
         const uint32_t slot = round & 1;
         if (!wait_warp(iempty + 8 * slot, (round >> 1 & 1) ^ 1, P.status)) break;
@@ -496,28 +510,35 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const int odd = odd_values, head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack + r - tok_of * P.pack;
       uint16_t* to = static_cast<uint16_t*>(P.out) + (long long)(w.row + pos) * P.o_row + (long long)q_head * P.o_head;
 #pragma unroll 1
-      for (int c = 0; c < P.dv; c += 16) {
-        uint32_t x[16];
-        tmem_read16(res + c, x);
+      for (int c0 = 0; c0 < P.dv; c0 += 64) {
+        uint32_t x[64];
+        tmem_ask<0, 64>(res + c0, x);
+        tmem_got<0, 64>(x);
         if (!mine) continue;
 #pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * inv);
-        if (odd) {                                           // (a copy: what a call is given by address lies in memory)
+        for (int g = 0; g < 64; g += 16) {
+          const int c = c0 + g;
+          if (c >= P.dv) break;
           float z[16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) z[e] = __uint_as_float(x[e]);
-          give_back<BF16>(P, w, k, pos, head, c, z);
+          for (int e = 0; e < 16; e++) z[e] = __uint_as_float(x[g + e]) * inv;
+          if (odd) {                                         // (a copy: what a call is given by address lies in memory)
+            float d[16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) x[e] = __float_as_uint(z[e]);
-        }
-        uint32_t y[8];
+            for (int e = 0; e < 16; e++) d[e] = z[e];
+            give_back<BF16>(P, w, k, pos, head, c, d);
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = pair<BF16>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-        if (P.wide_o) {                                      // (whole sectors: in two pieces of 16 bytes the results of a short prompt took longer than all else)
-          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + c), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
-        } else {
+            for (int e = 0; e < 16; e++) z[e] = d[e];
+          }
+          uint32_t y[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) { to[c + 2 * e] = (uint16_t)y[e]; to[c + 2 * e + 1] = (uint16_t)(y[e] >> 16); }
+          for (int e = 0; e < 8; e++) y[e] = pair<BF16>(z[2 * e], z[2 * e + 1]);
+          if (P.wide_o) {                                    // (whole sectors: in two pieces of 16 bytes they took twice as long)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + c), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) { to[c + 2 * e] = (uint16_t)y[e]; to[c + 2 * e + 1] = (uint16_t)(y[e] >> 16); }
+          }
         }
       }
     }

@@ -83,19 +83,24 @@ __device__ __forceinline__ Walk walk_of(const Params& P, const Item& w, int toke
   return k;
 }
 __device__ __forceinline__ int key_of(const Walk& k, int i) { return (i < k.kept ? i : k.low + i - k.kept) * kTile; }
-// whether tokens a .. b see all of a tile of keys; any of it
-__device__ __forceinline__ bool sees_all(const Params& P, int a, int b, int key0) {
-  return key0 + kTile - 1 <= a && (P.window <= 0 || b - key0 < P.window || key0 + kTile <= P.keep);
-}
-__device__ __forceinline__ bool sees_some(const Params& P, int a, int b, int key0) {
-  return key0 <= b && (P.window <= 0 || a - key0 - kTile + 1 < P.window || key0 < P.keep);
+// What tokens a .. b see of them, found once: any of the kept tiles and of those from some to upto - 1, all of those from all to end - 1
+struct Seen {
+  int kept, some, upto, all, end;
+  __device__ __forceinline__ bool any_of(int i) const { return (i < kept) | ((i >= some) & (i < upto)); }
+  __device__ __forceinline__ bool all_of(int i) const { return (i >= all) & (i < end); }
+};
+__device__ __forceinline__ Seen seen_by(const Params& P, const Walk& k, int a, int b) {
+  const int at = k.kept - k.low;                             // from a tile's number to its place in the walk
+  const bool windowed = P.window > 0;
+  return Seen{k.kept, windowed ? max(0, a + 1 - P.window) / kTile + at : 0, b / kTile + 1 + at, windowed ? max((max(0, b + 1 - P.window) + kTile - 1) / kTile + at, k.kept) : 0, (a + 1) / kTile + at};
 }
 
 // Infinities and NaN among the values that a row sees in tiles where they went to the products as zeros: its results c .. c + 15 become what they make of them
 template <bool BF16> __device__ __noinline__ void give_back(const Params& P, const Item& w, const Walk& k, int pos, int head, int c, float (&x)[16]) {
+  const Seen cta = seen_by(P, k, w.tok, k.t1 - 1);
   for (int i = 0; i < k.n; i++) {
     const int key0 = key_of(k, i);
-    if (sees_all(P, w.tok, k.t1 - 1, key0)) continue;
+    if (cta.all_of(i)) continue;
     for (int j = key0; j < min(key0 + kTile, pos + 1); j++) {
       if (P.window > 0 && pos - j >= P.window && j >= P.keep) continue;
       const uint16_t* v = static_cast<const uint16_t*>(P.values) + (long long)(w.row + j) * P.v_row + (long long)head * P.v_head + c;
@@ -202,13 +207,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         const Walk k = walk_of(P, w, tokens);
         const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
         const bool there = a < w.len;
-        auto sixteenths = [&](int key0) { return there && sees_some(P, a, b, key0) ? min(kTile / 16, (b - key0 + 16) / 16) : 0; };   // those of a tile that some row sees
+        const Seen mine = seen_by(P, k, a, b), cta = seen_by(P, k, w.tok, k.t1 - 1);
+        auto sixteenths = [&](int i) { return there && mine.any_of(i) ? mine.all_of(i) ? kTile / 16 : min(kTile / 16, (b - key_of(k, i) + 16) / 16) : 0; };   // those of a tile that some row sees
         if (scoring) {
           const uint64_t q_desc = hy::tc_desc(qs + t * (kRows * DK * 2));
           const int ksteps = P.dk / 16;
           alive = !there || wait_warp(qfull + 8 * t, took & 1, P.status);
           for (int i = 0; i < k.n && alive; i++) {
-            const int see = sixteenths(key_of(k, i));
+            const int see = sixteenths(i);
             const uint64_t k_desc = hy::tc_desc(ks + n * KB);
             alive = wait_warp(kfull + 8 * n, par[0], P.status);
             if (see && alive) {
@@ -235,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
           const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17), to = o_at + t * 128;
           bool any = false;
           for (int i = 0; i < k.n && alive; i++) {
-            const int key0 = key_of(k, i), see = sixteenths(key0);
-            const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0);
+            const int see = sixteenths(i);
+            const bool masked = !cta.all_of(i);
             const uint64_t v_desc = value_desc(vs + n * VB);
             alive = wait_warp((masked ? vok : vfull) + 8 * n, (masked ? par[1] : par[0]) >> n & 1, P.status);
             if (masked) par[1] ^= 1u << n; else par[0] ^= 1u << n;
@@ -305,10 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       bool alive = true;
       while (alive && take(w)) {
         const Walk k = walk_of(P, w, tokens);
+        const Seen cta = seen_by(P, k, w.tok, k.t1 - 1);
         const int head = w.unit / P.subs;
         for (int i = 0; i < k.n && alive; i++) {
           const int key0 = key_of(k, i);
-          const bool masked = !sees_all(P, w.tok, k.t1 - 1, key0);
+          const bool masked = !cta.all_of(i);
           const uint32_t full = masked ? vraw : vfull;
           alive = wait_warp(vempty + 8 * n, par ^ 1, P.status);
           if (!alive) break;
@@ -380,9 +387,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       bool alive = true;
       while (alive && take(w)) {
         const Walk k = walk_of(P, w, tokens);
+        const Seen cta = seen_by(P, k, w.tok, k.t1 - 1);
         for (int i = 0; i < k.n && alive; i++, n = n + 1 == VP ? 0 : n + 1) {
+          if (cta.all_of(i)) continue;
           const int key0 = key_of(k, i);
-          if (sees_all(P, w.tok, k.t1 - 1, key0)) continue;
           alive = wait_warp(vraw + 8 * n, par >> n & 1, P.status);
           par ^= 1u << n;
           bool odd = false;
@@ -419,11 +427,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const bool mine = pos < w.len, idle = !__any_sync(0xffffffffu, mine);
       float m = kLowest, l = 0.f, limit = -INFINITY;         // limit: where a maximum moves the reference; any does while that is beyond kFar
       bool any = false;
+      const Seen tile = seen_by(P, k, a, b);
       for (int i = 0; i < k.n; i++) {
+        if (!tile.any_of(i)) continue;
         const int key0 = key_of(k, i);
-        if (!sees_some(P, a, b, key0)) continue;
         const uint32_t place = passed & 1, s_at = tmem + (2 * t + place) * kTile + lanes, p_bar = pfull + 16 * t + 8 * place;
-        const bool masked = !sees_all(P, a, b, key0);
+        const bool masked = !tile.all_of(i);
         ok = wait_warp(sfull + 16 * t + 8 * place, (passed >> 1) & 1, P.status);
         if (!ok) break;
         if (idle) {                                          // (its rows' results are whatever comes of the scores as weights, and go nowhere)

@@ -83,16 +83,17 @@ __device__ __forceinline__ Walk walk_of(const Params& P, const Item& w, int toke
   return k;
 }
 __device__ __forceinline__ int key_of(const Walk& k, int i) { return (i < k.kept ? i : k.low + i - k.kept) * kTile; }
-// What tokens a .. b see of them, found once: any of the kept tiles and of those from some to upto - 1, all of those from all to end - 1
+// What tokens a .. b see of them, found once: something of those ahead of upto that have kept keys (the first `kept`, among them some that the walk has for its window) or come behind some, everything of
+// those from all to end - 1 (and perhaps of kept ones)
 struct Seen {
   int kept, some, upto, all, end;
-  __device__ __forceinline__ bool any_of(int i) const { return (i < kept) | ((i >= some) & (i < upto)); }
+  __device__ __forceinline__ bool any_of(int i) const { return (i < upto) & ((i < kept) | (i >= some)); }
   __device__ __forceinline__ bool all_of(int i) const { return (i >= all) & (i < end); }
 };
 __device__ __forceinline__ Seen seen_by(const Params& P, const Walk& k, int a, int b) {
   const int at = k.kept - k.low;                             // from a tile's number to its place in the walk
   const bool windowed = P.window > 0;
-  return Seen{k.kept, windowed ? max(0, a + 1 - P.window) / kTile + at : 0, b / kTile + 1 + at, windowed ? max((max(0, b + 1 - P.window) + kTile - 1) / kTile + at, k.kept) : 0, (a + 1) / kTile + at};
+  return Seen{windowed ? (min(P.keep, k.t1) + kTile - 1) / kTile : 0, windowed ? max(0, a + 1 - P.window) / kTile + at : 0, b / kTile + 1 + at, windowed ? max((max(0, b + 1 - P.window) + kTile - 1) / kTile + at, k.kept) : 0, (a + 1) / kTile + at};
 }
 
 // Infinities and NaN among the values that a row sees in tiles where they went to the products as zeros: its results c .. c + 15 become what they make of them

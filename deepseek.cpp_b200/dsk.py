@@ -1049,7 +1049,7 @@ class Cache8:
 
     def append(self, k, v, packed):
         """Packed rows k, v [rows, kv_heads, dim] to the places that `Blocks.extend` gave them (dsk_kv8_append)."""
-        if packed._pieces is None or packed.block != self.block:
+        if packed._all is None or packed.block != self.block:
             raise DskError(f"packed rows with places in blocks of {self.block} tokens are needed (Blocks.extend)")
         if k.dtype is not v.dtype:
             raise DskError(f"keys of {k.dtype}, values of {v.dtype}")
@@ -1121,7 +1121,7 @@ class Packed:
             _no_device(starts)
         at = _dense("starts", starts, torch.int32, starts.shape, device)
         p._torch, p.device, p.rows, p.batch, p.block = torch, device, rows, starts.shape[0] - 1, 0
-        p.starts, p.lens, p.positions, p.slots, p._pieces = starts, None, None, None, None
+        p._starts, p._all, p._at = starts, None, (0, 0)
         p.status = torch.zeros(1, dtype=torch.int32, device=starts.device)
         p._c = _PACKED.pack(at, 0, 0, 0, 0, p.status.data_ptr(), rows, p.batch, 0, 0, device)
         return p
@@ -1130,13 +1130,22 @@ class Packed:
     def _room(cls, blocks, batch: int, rows: int) -> "Packed":
         torch, p = blocks._torch, cls.__new__(cls)
         n = min(rows, rows // blocks.block + 2 * batch)
-        up = lambda k: (k + 3) // 4 * 4                        # (16-byte aligned parts of one allocation)
-        sizes = up(4 * n), up(rows), up(rows), up(batch + 1), batch
-        p._pieces, positions, slots, starts, lens = torch.empty(sum(sizes), dtype=torch.int32, device=blocks.free.device).split(sizes)
+        wide = (rows + 3) & ~3                                 # (16-byte aligned parts of one allocation: pieces, positions, slots, starts, lens; views are made when they are asked for)
+        at = p._at = (0, 4 * n, 4 * n + wide, 4 * n + 2 * wide, 4 * n + 2 * wide + ((batch + 4) & ~3))
+        p._all = torch.empty(at[4] + batch, dtype=torch.int32, device=blocks._place)
+        base = p._all.data_ptr()
         p._torch, p.device, p.rows, p.batch, p.block, p.status = torch, blocks.device, rows, batch, blocks.block, blocks.status
-        p.positions, p.slots, p.starts, p.lens = positions[:rows], slots[:rows], starts[:batch + 1], lens
-        p._c = _PACKED.pack(starts.data_ptr(), lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), p._pieces.data_ptr(), p.status.data_ptr(), rows, batch, n, p.block, p.device)
+        p._c = _PACKED.pack(base + 4 * at[3], base + 4 * at[4], base + 4 * at[1], base + 4 * at[2], base, blocks._status_at, rows, batch, n, p.block, p.device)
         return p
+
+    def _part(self, k, n):
+        return None if self._all is None else self._all.narrow(0, self._at[k], n)
+
+    starts = property(lambda self: self._starts if self._all is None else self._part(3, self.batch + 1))
+    lens = property(lambda self: self._part(4, self.batch))
+    positions = property(lambda self: self._part(1, self.rows))
+    slots = property(lambda self: self._part(2, self.rows))
+    _pieces = property(lambda self: self._part(0, self._at[1]))
 
     def _view(self, what, t, heads, dim, written=False):
         kind = {self._torch.float32: 0, self._torch.float16: 1, self._torch.bfloat16: 2}.get(t.dtype)
@@ -1202,7 +1211,8 @@ class Blocks:
         self._top = torch.tensor([free.shape[0], 0], dtype=torch.int32).to(free.device)
         self.n_free = self._top[:1]
         self.status = torch.zeros(1, dtype=torch.int32, device=free.device)
-        self._c = BlocksArgs(self.free.data_ptr(), self._top.data_ptr(), self.status.data_ptr(), self.device, n_blocks, block)
+        self._place, self._status_at = free.device, self.status.data_ptr()
+        self._c = BlocksArgs(self.free.data_ptr(), self._top.data_ptr(), self._status_at, self.device, n_blocks, block)
         self._at = C.addressof(self._c)
 
     def extend(self, table, lens, count, rows: int, out: Optional[Packed] = None) -> Packed:
@@ -1214,7 +1224,7 @@ class Blocks:
             raise DskError(f"{rows} packed rows")
         if out is None:
             out = Packed._room(self, batch, rows)
-        elif out.batch != batch or out.rows != rows or out._pieces is None or out.block != self.block:
+        elif out.batch != batch or out.rows != rows or out._all is None or out.block != self.block:
             raise DskError(f"packed rows of {batch} sequences, {rows} rows and blocks of {self.block} tokens from an earlier call are needed")
         _ck(_fast("dsk_blocks_extend")(self._at, table.data_ptr(), table.stride(0), blocks, _dense("lens", lens, i32, (batch,), self.device), _dense("count", count, i32, (batch,), self.device), out._c,
                                        _stream_of(self._torch, self.device)))

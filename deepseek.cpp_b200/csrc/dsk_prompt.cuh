@@ -33,7 +33,7 @@ struct Params {
   const void* values;
   void* out;
   long long v_row, v_head, o_row, o_head;
-  int rows, batch, group, pack, subs, tokens, units;         // pack: heads of a row tile; subs: group / pack; tokens: of a row tile; units: key heads x subs
+  int rows, batch, group, pack, subs, tokens, units, span;   // pack: heads of a row tile; subs: group / pack; tokens: of a row tile; units: key heads x subs; span: units that are worked on at a time
   int dk, dv, window, keep, wide_o;
   float f;                                                   // scale x log2(e), positive
 };
@@ -331,19 +331,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       }
       for (uint32_t s = 0; s < 2 * VP; s++)                  // no copy is under way at the end, whatever happened
         if (sent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
-    } else if (warp == 15) {                                 // deals out the work: rows with most keys first, so that the short ones fill the gaps
+    } else if (warp == 15) {                                 // deals out the work: rows with most keys first, so that the short ones fill the gaps, of as many heads at a time as the L2 holds
       // CTAs take over work of CTAs that have not started yet, each when its copies near the end of what it has
       long long at = blockIdx.x;
       for (uint32_t round = 0;; round++) {
         int4 item = make_int4(0, 0, 0, 0);
-        const int k = (int)(at / P.units);
         if (at < all) {
+          const int block = (int)(at / ((long long)pieces * P.span)), wide = min(P.span, P.units - block * P.span);
+          const long long in = at - (long long)block * pieces * P.span;
+          const int k = (int)(in / wide);
           int lo = 0, hi = most - 1;                         // the level j with from_level(j + 1) <= k < from_level(j)
           while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (from_level(mid) > k) lo = mid; else hi = mid - 1;
           }
-          most = lo + 1;                                     // (later ones lie no higher)
           int rank = k - from_level(lo + 1), from = 0, len = 0;      // the rank-th sequence with more than lo row tiles
           bool found = false;
           auto among = [&](bool has, int row, int rows) {
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             const int rows = rows_of(c + lane, row);
             among((rows + tokens - 1) / tokens > lo, row, rows);
           }
-          if (found) item = make_int4(from, len, lo * tokens, (int)(at - (long long)k * P.units));
+          if (found) item = make_int4(from, len, lo * tokens, block * P.span + (int)(in - (long long)k * wide));
         }
         const uint32_t slot = round & 1;
         if (!wait_warp(iempty + 8 * slot, (round >> 1 & 1) ^ 1, P.status)) break;

@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(kThreads) extend(const Extend A) {
   sums_ahead<kWarps>(sum, all, of_warp);
   const int have = free_now;
   bool refused = false;
+  int rows_end = 0, taken_end = 0;                           // behind the last served one of this thread
 #pragma unroll
   for (int k = 0; k < kEach; k++) {
     const int b = b0 + k;
@@ -100,12 +101,15 @@ __global__ void __launch_bounds__(kThreads) extend(const Extend A) {
       len[b] = l[k];
       taken[b] = sum[1];
       piece[b] = sum[2];
-      if (fits) { atomicMax(&served[0], sum[0] + c[k]); atomicMax(&served[1], sum[1] + need[k]); }
+      if (fits) { rows_end = sum[0] + c[k]; taken_end = sum[1] + need[k]; }
       else refused |= c[k] > 0;
       if (blockIdx.x == 0) A.lens_out[b] = l[k] + (fits ? c[k] : 0);
     }
     sum[0] += c[k]; sum[1] += need[k]; sum[2] += pieces[k];
   }
+  rows_end = __reduce_max_sync(0xffffffffu, rows_end);
+  taken_end = __reduce_max_sync(0xffffffffu, taken_end);
+  if ((threadIdx.x & 31) == 0 && rows_end + taken_end > 0) { atomicMax(&served[0], rows_end); atomicMax(&served[1], taken_end); }
   __syncthreads();
   const int total = served[0];
 #pragma unroll

@@ -1,15 +1,22 @@
 // dsk_prompt.cuh — causal softmax attention of packed prompts on the 5th-generation tensor cores: o_i = sum_j p_ij v_j, p_i = softmax over j of scale q_i k_j, j <= i, in a window or
 // among the first tokens.
 //
-// Query rows of a key head lie token by token, the heads that share it side by side, so that a tile of 128 rows has few tokens and its keys end close behind the rows' own.  A CTA has two
-// tiles (one where heads have more than 192 + 128 entries) and walks their keys in tiles of 128; tensor-map copies bring queries, keys and values as swizzled operands, in units of 16 KB that
-// are given back as soon as their product is through.  Roles: a warp for the copies of keys and queries, one for the values, one that issues each row tile's products (scores into TMEM, weights
-// from TMEM), four softmax warps for each row tile, a thread to a row, one that deals out the work, three that look at values of tiles which some row does not see whole.
+// Query rows of a key head lie token by token, the heads that share it side by side, so that a tile of 128 rows has few tokens and its keys end close behind the rows' own.  A CTA has two row
+// tiles (one where heads have more than 192 + 128 entries) and walks their keys in tiles of 64; tensor-map copies bring queries, keys and values as swizzled operands into rings whose places are
+// given back as soon as their products are through.  Roles: a warp for the copies of keys and queries, one for those of values; for each row tile one that issues products of scores, one that issues
+// products with the values (scores lie in TMEM, weights where the scores were) and four for the softmax, a thread to a row; one that deals out the work, one that looks at values of tiles which
+// some row does not see whole.  A row tile has scores in two places, so that the products and the way there and back (1400 cycles a tile) come under the softmax of the tile ahead.
 // Weights: y = f s - m in one fused operation, f = scale log2(e); the reference m is a whole number that may lag behind the maximum, so that the results in TMEM are scaled again, by
 // powers of two, where a maximum has moved far (the thread that has the row does it).  bf16 weights have fp32's range: references lead by 2^40, so that no sum of weights x values exceeds the
-// largest value; fp16 weights lie between 2^-24 and 2^14, references 2^7 below the maximum.
+// largest value; fp16 weights lie between 2^-24 and 2^14, references 2^7 below the maximum.  Sums are of the weights ahead of their rounding, which is off by half a step of the type at most.
 // Infinities and NaN among values that a row does not see must not reach it as 0 x inf: in tiles that some row does not see whole they go to the products as zeros, and rows that do see
 // one get it back at the end.
+// Work: pieces are dealt out with the longest walks first; CTAs take over pieces of CTAs that have not started (clusterlaunchcontrol), so that nothing but starts is needed to balance them.
+// Bound: between tensor pipe and softmax.  Of 1470 cycles for 256 rows and 64 keys of 128 + 128 entries the tensor pipe has 1280 (products of 64 keys read their operands from shared memory in 48 cycles
+// for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 820 us
+// (1.34 PFLOP/s; a measured product of matrices 1.68), at 1.6 GHz under the power limit; back to back 1000.  32 heads of 192 + 128, 8 prompts of up to 5001 tokens: 774 us (1.06); 256 + 256: 100 us
+// (0.80), 64 + 64, windowed: 159 us.  Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 for 820),
+// maxima only where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0023 in bf16, the plain form's 0.0016).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -21,13 +28,14 @@
 namespace dsk {
 namespace prompt {
 
-constexpr int kThreads = 512, kRows = 128, kTile = 64, kMaxBatch = 1024, kHeld = 8, kEarly = 8;   // rows of a row tile, keys of a tile; sequences whose tiles a lane of the dealing warp keeps in registers; tiles ahead of the end at which more work is asked for
+constexpr int kThreads = 512, kRows = 128, kTile = 64;       // rows of a row tile, keys of a tile
+constexpr int kMaxBatch = 1024, kHeld = 8, kEarly = 8;       // sequences; those whose rows a lane of the dealing warp keeps in registers; tiles ahead of the end at which more work is asked for
 constexpr int ST_WAIT = 4;                                   // a wait that gave up
 constexpr float kLowest = -3e38f;                            // a maximum ahead of the first score (finite: no difference of infinities)
 constexpr float kFar = 16777216.f;                           // scores beyond it are rounded ahead of the subtraction: what fma keeps of a product that its reference does not would be exponents
 
 struct Params {
-  CUtensorMap q, k, v;                                       // [row][head][entry]: boxes of 64 entries of (heads of a tile, its tokens), (one head, 128 keys), (one head, the keys of a unit)
+  CUtensorMap q, k, v;                                       // [row][head][entry]: boxes of 64 entries of (heads of a row tile, its tokens), (one head, a tile of keys) for both others
   const int* starts;                                         // [batch + 1]
   int* status;
   const void* values;
@@ -40,8 +48,8 @@ struct Params {
 
 template <int DK, int DV> __host__ __device__ constexpr int tiles() { return DV == 256 ? 1 : 2; }
 // tiles of keys and of values that shared memory has room for beside the queries
-template <int DK, int DV> __host__ __device__ constexpr int k_places() { return DK == 64 ? 8 : DK == 128 ? 6 : 3; }
-template <int DK, int DV> __host__ __device__ constexpr int v_places() { return DK == 64 ? 8 : DK == 128 ? 4 : DK == 192 ? 3 : 2; }
+template <int DK, int DV> __host__ __device__ constexpr int k_places() { return DK == 64 ? 8 : DK == 128 ? 6 : DK == 192 ? 3 : 2; }
+template <int DK, int DV> __host__ __device__ constexpr int v_places() { return DK == 64 ? 8 : DK == 128 ? 4 : 3; }
 template <int DK, int DV> __host__ __device__ constexpr int smem_bytes() {
   return 1024 + kRows * tiles<DK, DV>() * DK * 2 + k_places<DK, DV>() * kTile * DK * 2 + v_places<DK, DV>() * kTile * DV * 2;
 }
@@ -196,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
     const bool scoring = warp < 8 + TILES, adding = warp == 11 || warp == 10 + TILES;
-    if (scoring || adding) {                                 // products of a row tile: scores, or weights x values.  (A warp for each: in one, the way from weights to results and to the place of the next scores stood behind one another)
+    if (scoring || adding) {                                 // products of a row tile: scores, or weights x values.  (A warp for each: neither waits behind the other's)
       const int t = scoring ? warp - 8 : warp - 11;
       const uint32_t lead = hy::tc_elect();
       const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (8u << 24);         // fp32 sums of bf16 or fp16, 128 rows

@@ -57,22 +57,12 @@ __device__ __forceinline__ uint64_t both(float a, float b) {
 __device__ __forceinline__ void fma2(uint32_t x0, uint32_t x1, uint64_t f, uint64_t a, float& y0, float& y1) {
   asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%2, %3};\n\tfma.rn.f32x2 x, x, %4, %5;\n\tmov.b64 {%0, %1}, x;\n\t}" : "=f"(y0), "=f"(y1) : "r"(x0), "r"(x1), "l"(f), "l"(a));
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t f, uint64_t a) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(f), "l"(a));
-  return r;
-}
 __device__ __forceinline__ void add2(uint64_t& s, float y0, float y1) {
   asm("{\n\t.reg .b64 y;\n\tmov.b64 y, {%1, %2};\n\tadd.rn.f32x2 %0, %0, y;\n\t}" : "+l"(s) : "f"(y0), "f"(y1));
 }
 __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
-  return r;
-}
-__device__ __forceinline__ float max3_nan(float a, uint32_t b, uint32_t c) {   // NaN where one is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
   return r;
 }
 // Products and commits of one lane of a warp whose lanes all run the same code: descriptors then stay in uniform registers, where a branch to that lane would have them copied there

@@ -982,7 +982,7 @@ def _status(torch, status, device, what):
 class Cache8:
     """A key / value cache in 8 bits (dsk_kv8, include/dsk.h): blocks of `block` tokens, E4M3 codes [n_blocks, kv_heads, block, dim] and a scale, a power of
     two, for every block and head [n_blocks, kv_heads].  A sequence is a row of a table of block numbers (int32 [batch, blocks]); which blocks are free is the
-    caller's to know.  `first`, `lens`, `count` are int32 [batch] tensors on the GPU, so that a captured graph serves other lengths.  No call waits for
+    caller's to know (`Blocks` keeps them).  `first`, `lens`, `count` are int32 [batch] tensors on the GPU, so that a captured graph serves other lengths.  No call waits for
     the GPU: what only the GPU sees (a block number outside the cache, tokens outside the table) shows in `check`.  Memory of a call comes
     from torch's allocator on the current stream; calls may run on several streams at a time as long as none writes what another one uses."""
 

@@ -415,8 +415,8 @@ int dsk_blocks_cut(const dsk_blocks* blocks, int32_t* table, int64_t table_pitch
 int dsk_kv8_append(const dsk_kv8* cache, const dsk_packed* rows, const dsk_view* k, const dsk_view* v, void* stream);
 /* Causal softmax attention of whole prompts, from their packed rows alone (no cache): token i of a sequence sees its tokens j <= i, with window > 0 those with i - j < window or j < keep_first.  Query
  * head h reads key head h / (heads / kv_heads).  q, k, v, out: F16 or BF16, all of one type (views: batch unused); q, k and v 16-byte aligned, their rows and heads a positive multiple of 8 entries apart;
- * dim_k and dim_v multiples of 16 up to 256; scale >= 0.  Zeros for a query whose scores are all -inf; one that sees an infinite or NaN value has no finite result in that entry, others do not
- * notice.  Results below 2^-80 (BF16) lose accuracy. */
+ * dim_k and dim_v multiples of 16 up to 256; scale >= 0; out lies apart from the others.  Zeros for a query whose scores are all -inf; one that sees an infinite or NaN value has no finite result in that entry, others do not
+ * notice.  Scores (scaled) beyond 2^127 are infinite; results below 2^-80 (BF16) lose accuracy. */
 int dsk_packed_attn(const dsk_packed* rows, const dsk_view* q, const dsk_view* k, const dsk_view* v, const dsk_view* out, int heads, int kv_heads, int dim_k, int dim_v, float scale, int window,
                     int keep_first, void* stream);
 /* Speculative sampling, beside dsk_sample: sequence b has count[b] drafted tokens x_i and the model's logits of count[b] + 1 rows.  p_i = softmax(logits_i / temperature); draft i is accepted

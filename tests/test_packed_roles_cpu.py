@@ -21,7 +21,7 @@ class Bar:
 
 
 EARLY = 8                                                    # tiles ahead of the end at which more work is asked for
-SHAPES = {64: (2, 8, 8), 128: (2, 6, 4), 192: (2, 3, 3), 256: (1, 3, 2)}      # row tiles, places of keys and of values
+SHAPES = {64: (2, 8, 8), 128: (2, 6, 4), 192: (2, 3, 3), 256: (1, 2, 3)}      # row tiles, places of keys and of values
 
 
 def run(rng, dk, work, idle, moves, early=True):

@@ -176,7 +176,7 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   P.starts = s->starts; P.status = s->status;
   P.values = v->data; P.v_row = v->row; P.v_head = v->head;
   P.out = out->data; P.o_row = out->row; P.o_head = out->head;
-  P.wide_o = aligned(out->data, 32) && out->row % 16 == 0 && out->head % 16 == 0;
+  P.wide_o = aligned(out->data, 32) && out->row % 16 == 0 && out->head % 16 == 0 ? 2 : aligned(out->data, 16) && out->row % 8 == 0 && out->head % 8 == 0;
   P.rows = s->rows; P.batch = s->batch; P.dk = dim_k; P.dv = dim_v;
   P.window = window >= s->rows ? 0 : window; P.keep = keep_first;
   P.f = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);            // (positive: -inf stays what it is)

@@ -42,7 +42,7 @@ struct Params {
   void* out;
   long long v_row, v_head, o_row, o_head;
   int rows, batch, group, pack, subs, tokens, units, span;   // pack: heads of a row tile; subs: group / pack; tokens: of a row tile; units: key heads x subs; span: units that are worked on at a time
-  int dk, dv, window, keep, wide_o;
+  int dk, dv, window, keep, wide_o;                          // wide_o: rows of results lie on 32 bytes (2), on 16
   float f;                                                   // scale x log2(e), positive
 };
 
@@ -529,35 +529,33 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const int odd = odd_values, head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack + r - tok_of * P.pack;
       uint16_t* to = static_cast<uint16_t*>(P.out) + (long long)(w.row + pos) * P.o_row + (long long)q_head * P.o_head;
 #pragma unroll 1
-      for (int c0 = 0; c0 < P.dv; c0 += 64) {
-        uint32_t x[64];
-        tmem_ask<0, 64>(res + c0, x);
-        tmem_got<0, 64>(x);
+      for (int c = 0; c < P.dv; c += 16) {                   // (64 columns at a time: as long, and more code, which a short prompt waits for)
+        uint32_t x[16];
+        tmem_read16(res + c, x);
         if (!mine) continue;
+        float z[16];
 #pragma unroll
-        for (int g = 0; g < 64; g += 16) {
-          const int c = c0 + g;
-          if (c >= P.dv) break;
-          float z[16];
+        for (int e = 0; e < 16; e++) z[e] = __uint_as_float(x[e]) * inv;
+        if (odd) {                                           // (a copy: what a call is given by address lies in memory)
+          float d[16];
 #pragma unroll
-          for (int e = 0; e < 16; e++) z[e] = __uint_as_float(x[g + e]) * inv;
-          if (odd) {                                         // (a copy: what a call is given by address lies in memory)
-            float d[16];
+          for (int e = 0; e < 16; e++) d[e] = z[e];
+          give_back<BF16>(P, w, k, pos, head, c, d);
 #pragma unroll
-            for (int e = 0; e < 16; e++) d[e] = z[e];
-            give_back<BF16>(P, w, k, pos, head, c, d);
+          for (int e = 0; e < 16; e++) z[e] = d[e];
+        }
+        uint32_t y[8];
 #pragma unroll
-            for (int e = 0; e < 16; e++) z[e] = d[e];
-          }
-          uint32_t y[8];
+        for (int e = 0; e < 8; e++) y[e] = pair<BF16>(z[2 * e], z[2 * e + 1]);
+        if (P.wide_o == 2) {                                 // (whole sectors: in two pieces of 16 bytes they took twice as long)
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + c), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
+        } else if (P.wide_o) {
+          uint4* at = reinterpret_cast<uint4*>(to + c);
+          at[0] = make_uint4(y[0], y[1], y[2], y[3]);
+          at[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        } else {
 #pragma unroll
-          for (int e = 0; e < 8; e++) y[e] = pair<BF16>(z[2 * e], z[2 * e + 1]);
-          if (P.wide_o) {                                    // (whole sectors: in two pieces of 16 bytes they took twice as long)
-            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to + c), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) { to[c + 2 * e] = (uint16_t)y[e]; to[c + 2 * e + 1] = (uint16_t)(y[e] >> 16); }
-          }
+          for (int e = 0; e < 8; e++) { to[c + 2 * e] = (uint16_t)y[e]; to[c + 2 * e + 1] = (uint16_t)(y[e] >> 16); }
         }
       }
     }

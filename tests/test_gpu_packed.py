@@ -195,6 +195,46 @@ def test_orders_of_rows_and_heads():
     odd = torch.full((p.rows, 4 * 64 + 3), 7.0, dtype=torch.bfloat16, device=DEV)
     p.run(out=odd[:, 1:257].unflatten(1, (4, 64)))
     assert (odd[:, 0] == 7).all() and (odd[:, 257:] == 7).all()
+    half = torch.full((p.rows, 4 * 64 + 8), 7.0, dtype=torch.bfloat16, device=DEV)
+    p.run(out=half[:, 8:].unflatten(1, (4, 64)))             # on 16 bytes, not on 32
+    assert (half[:, :8] == 7).all()
+
+
+def test_rows_beyond_four_gigabytes():
+    """Queries, keys, values and results as parts of rows that lie 16 KB apart: offsets beyond 2^32 bytes and 2^31 entries."""
+    p = Prompt([90, 60], 2, 1, 64, 64, seed=16)
+    rows = 290_000
+    wide = torch.zeros(rows, 8192, dtype=torch.bfloat16, device=DEV)
+    at = rows - 150
+    for x, c in ((p.q, 0), (p.k, 4096), (p.v, 8128)):
+        wide[at:, c:c + x.shape[1] * 64] = x.flatten(1).to(DEV)
+    out = wide[:, 1024:1152].unflatten(1, (2, 64))
+    dsk.Packed.of(ints([at, at + 90, rows]), rows).attend(wide[:, :128].unflatten(1, (2, 64)), wide[:, 4096:4160, None].transpose(1, 2), wide[:, 8128:, None].transpose(1, 2), out=out)
+    p.check(out[at:].contiguous())
+    assert (out[:at] == 0).all()
+
+
+@pytest.mark.parametrize("H,G", [(1, 1), (16, 16), (16, 2)])
+def test_more_heads_than_the_cache_holds(H, G):
+    """Heads are worked on a few at a time where their keys and values are many: every piece of work is done once."""
+    n = 300_000 if G == 1 else 150_000
+    lens = [64] * 2 + [n - 300] + [1] * 40 + [70]
+    g = torch.Generator(device=DEV).manual_seed(17)
+    q, k, v = (torch.randn(n, h, 64, generator=g, device=DEV).to(torch.bfloat16) for h in (H, G, G))
+    out = torch.full((n, H, 64), float("nan"), dtype=torch.bfloat16, device=DEV)
+    packed = dsk.Packed.of(torch.from_numpy(starts_of(lens)).to(DEV), n)
+    packed.attend(q, k, v, window=100, out=out)
+    packed.check()
+    end = sum(lens)
+    assert torch.isfinite(out[:end]).all() and torch.isnan(out[end:]).all()
+    for row, first in ((3, 0), (100, 64), (n // 2, 128), (128 + n - 301, 128), (128 + n - 300 + 39, 128 + n - 300 + 39), (end - 1, end - 70)):
+        lo = max(first, row - 99)
+        for h in (0, H - 1):
+            kk, vv = k[lo:row + 1, h * G // H].double(), v[lo:row + 1, h * G // H].double()
+            w = torch.softmax(kk @ q[row, h].double() * 64 ** -0.5, 0)
+            # (as Prompt.check: weights, scores and the result are rounded)
+            tol = (w @ vv.abs()) * 2.0 ** -7.5 + 2.0 ** -8 * (w @ vv).abs() + 2.0 ** -20
+            assert ((out[row, h].double() - w @ vv).abs() <= tol).all()
 
 
 def test_starts_that_fall_or_point_outside_stay_inside():

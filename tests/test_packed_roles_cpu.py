@@ -273,3 +273,36 @@ def test_the_wait_for_the_product_ahead_is_needed():
         except AssertionError:
             found += 1
     assert found > 20
+
+
+def test_what_rows_see_of_the_tiles():
+    """walk_of and seen_by (csrc/dsk_prompt.cuh), restated, against the mask itself: every key that a token sees lies in a tile of the walk, once, and ranges say rightly which tiles some token sees and
+    which ones all of them see whole."""
+    T, rng = 64, random.Random(0)
+    for _ in range(4000):
+        window, keep = rng.choice([0, 0, 1, 2, rng.randint(1, 300), rng.randint(1, 900)]), rng.choice([0, 1, 64, 65, rng.randint(0, 400)])
+        tok, n = rng.randint(0, 700), rng.choice([1, 2, 7, 32, 64, 128])
+        length = tok + rng.randint(1, 2 * n)
+        t1 = min(tok + 2 * n, length)
+        low = max(0, tok + 1 - window) // T if window else 0
+        first = -(-min(keep, t1) // T) if window else 0
+        kept = min(first, low)
+        tiles = [i if i < kept else low + i - kept for i in range(kept + -(-t1 // T) - low)]
+        assert len(set(tiles)) == len(tiles)
+        sees = lambda i, j: j <= i and (not window or i - j < window or j < keep)
+        for a in (tok, tok + n):
+            if a >= length:
+                continue
+            b, at = min(a + n, length) - 1, kept - low
+            some, upto = max(0, a + 1 - window) // T + at if window else 0, b // T + 1 + at
+            whole, end = max(-(-max(0, b + 1 - window) // T) + at, kept) if window else 0, (a + 1) // T + at
+            seen = {j // T for i in (a, b, (a + b) // 2) for j in (0, keep - 1, i - window + 1, i) if 0 <= j and sees(i, j)}
+            assert seen <= set(tiles)
+            for i, tile in enumerate(tiles):
+                keys = [tile * T, tile * T + T - 1]
+                any_of = keys[0] <= b and (not window or a - keys[1] < window or keys[0] < keep)
+                assert (i < upto and (i < first or i >= some)) == any_of
+                if whole <= i < end:
+                    assert all(sees(x, y) for x in (a, b) for y in keys)
+                elif not window:
+                    assert not all(sees(a, y) for y in keys)

@@ -12,6 +12,9 @@
 // Infinities and NaN among values that a row does not see must not reach it as 0 x inf: in tiles that some row does not see whole they go to the products as zeros, and rows that do see
 // one get it back at the end.
 // Work: pieces are dealt out with the longest walks first; CTAs take over pieces of CTAs that have not started (clusterlaunchcontrol), so that nothing but starts is needed to balance them.
+// Short prompts: a piece of one tile runs through the code of every role once, and what does not fit the instruction cache is fetched each time (39 % of its lines, a softmax of one tile 4500 cycles
+// where it has 1350 by itself).  So the code that pieces run through is kept small: walks are worked out by the warp that deals, one form of each product, one place that counts levels, waits that
+// note in a register that they gave up (222 prompts of 60 tokens, 8 heads over 8: 43 us where it was 60; 64 prompts of 1 to 200: 26, was 31).
 // Bound: between tensor pipe and softmax.  Of 1470 cycles for 256 rows and 64 keys of 128 + 128 entries the tensor pipe has 1280 (products of 64 keys read their operands from shared memory in 48 cycles
 // for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 820 us
 // (1.34 PFLOP/s; a measured product of matrices 1.68), at 1.6 GHz under the power limit; back to back 1000.  32 heads of 192 + 128, 8 prompts of up to 5001 tokens: 774 us (1.06); 256 + 256: 100 us
@@ -54,15 +57,14 @@ template <int DK, int DV> __host__ __device__ constexpr int smem_bytes() {
   return 1024 + kRows * tiles<DK, DV>() * DK * 2 + k_places<DK, DV>() * kTile * DK * 2 + v_places<DK, DV>() * kTile * DV * 2;
 }
 
-// Bounded, in line: a call would cost what the wait itself does
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status) {
+// Bounded (a poll that fails has waited some microseconds), in line: a call would cost what the wait itself does
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, bool& lost) {
   bool ok = hy::tc_poll(bar, parity);
-  if (!ok) {
-    const uint32_t from = clock();
-    do ok = hy::tc_poll(bar, parity); while (!ok && (uint32_t)clock() - from < 1u << 31);
-    if (!ok && status) atomicOr(status, ST_WAIT);
-  }
-  return __all_sync(0xffffffffu, ok);
+#pragma unroll 1
+  for (int i = 0; i < 1 << 20 && !ok; i++) ok = hy::tc_poll(bar, parity);
+  ok = __all_sync(0xffffffffu, ok);
+  lost |= !ok;
+  return ok;
 }
 __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int entry, int head, int row, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   constexpr int MANY = 192, FEW = 64;                        // registers of a softmax thread and of another one: 512 threads have 128 each
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[76];
-  __shared__ int4 items[2];
+  __shared__ int4 items[2][4];                               // [slot][item, walk, what its rows see (and the end of that)]
   __shared__ __align__(16) uint4 claim;
   __shared__ uint32_t tmem_slot;
   __shared__ int odd_values, pieces;
@@ -186,17 +188,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot, o_at = tmem + 256;        // columns: scores (then weights) [row tile][place][64], results [tile][DV]
-  const long long all = (long long)pieces * P.units;
+  const int all = pieces * P.units;
 
+  bool lost = false;                                         // a wait of this warp gave up
   uint32_t turn = 0;                                         // items that this warp has taken
-  auto take = [&](Item& w) {                                 // the next item, in every lane
+  auto take = [&](Item& w, Walk& k, Seen& cta) {             // the next item, the walk of its keys and what all its rows see of them, in every lane
     const uint32_t slot = turn & 1;
-    const bool ok = wait_warp(ifull + 8 * slot, (turn >> 1) & 1, P.status);
-    const int4 x = items[slot];
+    const bool ok = wait_warp(ifull + 8 * slot, (turn >> 1) & 1, lost);
+    const int4 x = items[slot][0], y = items[slot][1], z = items[slot][2];
+    const int last = items[slot][3].x;
     __syncwarp();
     if (lane == 0) hy::tc_arrive(iempty + 8 * slot);
     turn++;
     w = Item{x.x, x.y, x.z, x.w};
+    k = Walk{y.x, y.y, y.z, y.w};
+    cta = Seen{z.x, z.y, z.z, z.w, last};
     return ok && w.len > 0;
   };
 
@@ -211,33 +217,29 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       const uint32_t s_at = tmem + t * 2 * kTile, done_at = pvdone + 16 * t;
       uint32_t passed = 0, took = 0, n = 0, par[2] = {0, 0};  // tiles behind that the row tile sees, items that had rows; the next tile's place and its parities (values: a bit for each place, as they came and looked at)
       Item w;
+      Walk k;
+      Seen cta;
       bool alive = true;
-      while (alive && take(w)) {
-        const Walk k = walk_of(P, w, tokens);
+      while (alive && take(w, k, cta)) {
         const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
         const bool there = a < w.len;
-        const Seen mine = seen_by(P, k, a, b), cta = seen_by(P, k, w.tok, k.t1 - 1);
+        const Seen mine = seen_by(P, k, a, b);
         auto sixteenths = [&](int i) { return there && mine.any_of(i) ? mine.all_of(i) ? kTile / 16 : min(kTile / 16, (b - key_of(k, i) + 16) / 16) : 0; };   // those of a tile that some row sees
         if (scoring) {
           const uint64_t q_desc = hy::tc_desc(qs + t * (kRows * DK * 2));
           const int ksteps = P.dk / 16;
-          alive = !there || wait_warp(qfull + 8 * t, took & 1, P.status);
+          alive = !there || wait_warp(qfull + 8 * t, took & 1, lost);
           for (int i = 0; i < k.n && alive; i++) {
             const int see = sixteenths(i);
             const uint64_t k_desc = hy::tc_desc(ks + n * KB);
-            alive = wait_warp(kfull + 8 * n, par[0], P.status);
+            alive = wait_warp(kfull + 8 * n, par[0], lost);
             if (see && alive) {
               const uint32_t place = passed & 1, at = s_at + place * kTile, sdesc = idesc | (uint32_t)(2 * see) << 17;
-              if (passed > 1) alive = wait_warp(done_at + 8 * place, ((passed >> 1) - 1) & 1, P.status);   // the weights that lie there are read
+              if (passed > 1) alive = wait_warp(done_at + 8 * place, ((passed >> 1) - 1) & 1, lost);   // the weights that lie there are read
               if (!alive) break;
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              if (ksteps == DK / 16) {
 #pragma unroll
-                for (int u = 0; u < DK / 16; u++) mma_ss(at, q_desc + (u >> 2) * (kRows * 128 >> 4) + 2 * (u & 3), k_desc + (u >> 2) * (kTile * 128 >> 4) + 2 * (u & 3), sdesc, u > 0, lead);
-              } else {
-#pragma unroll
-                for (int u = 0; u < DK / 16; u++) if (u < ksteps) mma_ss(at, q_desc + (u >> 2) * (kRows * 128 >> 4) + 2 * (u & 3), k_desc + (u >> 2) * (kTile * 128 >> 4) + 2 * (u & 3), sdesc, u > 0, lead);
-              }
+              for (int u = 0; u < DK / 16; u++) if (u < ksteps) mma_ss(at, q_desc + (u >> 2) * (kRows * 128 >> 4) + 2 * (u & 3), k_desc + (u >> 2) * (kTile * 128 >> 4) + 2 * (u & 3), sdesc, u > 0, lead);
               commit(sfull + 16 * t + 8 * place, lead);
               passed++;
             }
@@ -253,20 +255,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             const int see = sixteenths(i);
             const bool masked = !cta.all_of(i);
             const uint64_t v_desc = value_desc(vs + n * VB);
-            alive = wait_warp((masked ? vok : vfull) + 8 * n, (masked ? par[1] : par[0]) >> n & 1, P.status);
+            alive = wait_warp((masked ? vok : vfull) + 8 * n, (masked ? par[1] : par[0]) >> n & 1, lost);
             if (masked) par[1] ^= 1u << n; else par[0] ^= 1u << n;
             if (see && alive) {
               const uint32_t place = passed & 1, weights = s_at + place * kTile;
-              alive = wait_warp(pfull + 16 * t + 8 * place, (passed >> 1) & 1, P.status);
+              alive = wait_warp(pfull + 16 * t + 8 * place, (passed >> 1) & 1, lost);
               if (!alive) break;
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              if (see == kTile / 16) {
 #pragma unroll
-                for (int u = 0; u < kTile / 16; u++) mma_ts(to, weights + u * 8, v_desc + u * 128, pdesc, any || u > 0, lead);
-              } else {
-#pragma unroll
-                for (int u = 0; u < kTile / 16; u++) if (u < see) mma_ts(to, weights + u * 8, v_desc + u * 128, pdesc, any || u > 0, lead);
-              }
+              for (int u = 0; u < kTile / 16; u++) if (u < see) mma_ts(to, weights + u * 8, v_desc + u * 128, pdesc, any || u > 0, lead);
               commit(done_at + 8 * place, lead);
               passed++;
               any = true;
@@ -280,56 +277,62 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       }
       const uint32_t last = flushed + 16 * t + (scoring ? 0 : 8);
       commit(last, lead);                                    // no product is under way when TMEM is given back
-      wait_warp(last, 0, P.status);
+      wait_warp(last, 0, lost);
     } else if (warp == 10) {                                 // copies of keys and queries
       Item w;
+      Walk k;
+      Seen cta;
       const int chunks = (P.dk + 63) / 64;
-      uint32_t n = 0, par = 0, took[2] = {0, 0}, sent = 0;
+      uint32_t n = 0, par = 0, took = 0, asked = 0, sent = 0;  // took, asked: a bit for each row tile (its next copy's parity; there was one)
       bool alive = true;
-      while (alive && take(w)) {
-        const Walk k = walk_of(P, w, tokens);
+      while (alive && take(w, k, cta)) {
         const int head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack;
         for (int i = 0; i < k.n && alive; i++) {
-          alive = wait_warp(kempty + 8 * n, par ^ 1, P.status);
+          alive = wait_warp(kempty + 8 * n, par ^ 1, lost);
           if (!alive) break;
           if (lane == 0) {
             mbar_expect_tx(kfull + 8 * n, chunks * kTile * 128);
+#pragma unroll 1
             for (int c = 0; c < chunks; c++) copy_box(ks + n * KB + c * (kTile * 128), &P.k, 64 * c, head, w.row + key_of(k, i), kfull + 8 * n);
           }
           sent |= 1u << n;
           if (++n == KP) { n = 0; par ^= 1; }
           if (i == max(0, k.n - kEarly) && lane == 0) hy::tc_arrive(want);
+#pragma unroll 1
           for (int t = 0; t < TILES && alive && i == 0; t++) {
             if (w.tok + t * P.tokens >= w.len) continue;
-            alive = wait_warp(qempty + 8 * t, (took[t] & 1) ^ 1, P.status);
+            alive = wait_warp(qempty + 8 * t, (took >> t & 1) ^ 1, lost);
             if (!alive) break;
             if (lane == 0) {
               mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
+#pragma unroll 1
               for (int c = 0; c < chunks; c++) copy_box(qs + t * (kRows * DK * 2) + c * (kRows * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
             }
-            took[t]++;
+            took ^= 1u << t;
+            asked |= 1u << t;
           }
         }
       }
-      for (int t = 0; t < TILES; t++) if (took[t]) wait_warp(qfull + 8 * t, (took[t] - 1) & 1, P.status);   // no copy is under way at the end, whatever happened
-      for (uint32_t s = 0; s < KP; s++) if (sent >> s & 1) wait_warp(kfull + 8 * s, s < n ? par : par ^ 1, P.status);
+      for (int t = 0; t < TILES; t++) if (asked >> t & 1) wait_warp(qfull + 8 * t, (took >> t & 1) ^ 1, lost);   // no copy is under way at the end, whatever happened
+      for (uint32_t s = 0; s < KP; s++) if (sent >> s & 1) wait_warp(kfull + 8 * s, s < n ? par : par ^ 1, lost);
     } else if (warp == 13) {                                 // copies of values
       Item w;
+      Walk k;
+      Seen cta;
       const int boxes = (P.dv + 63) / 64;
       uint32_t n = 0, par = 0, vpar[2] = {0, 0}, sent[2] = {0, 0};
       bool alive = true;
-      while (alive && take(w)) {
-        const Walk k = walk_of(P, w, tokens);
-        const Seen cta = seen_by(P, k, w.tok, k.t1 - 1);
+      while (alive && take(w, k, cta)) {
         const int head = w.unit / P.subs;
         for (int i = 0; i < k.n && alive; i++) {
           const int key0 = key_of(k, i);
           const bool masked = !cta.all_of(i);
           const uint32_t full = masked ? vraw : vfull;
-          alive = wait_warp(vempty + 8 * n, par ^ 1, P.status);
+          alive = wait_warp(vempty + 8 * n, par ^ 1, lost);
           if (!alive) break;
           if (lane == 0) {
             mbar_expect_tx(full + 8 * n, boxes * kTile * 128);
+#pragma unroll 1
             for (int c = 0; c < boxes; c++) copy_box(vs + n * VB + c * (kTile * 128), &P.v, 64 * c, head, w.row + key0, full + 8 * n);
           }
           vpar[masked] ^= 1u << n;
@@ -338,22 +341,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         }
       }
       for (uint32_t s = 0; s < 2 * VP; s++)                  // no copy is under way at the end, whatever happened
-        if (sent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, P.status);
+        if (sent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, lost);
     } else if (warp == 15) {                                 // deals out the work: rows with most keys first, so that the short ones fill the gaps, of as many heads at a time as the L2 holds
       // CTAs take over work of CTAs that have not started yet, each when its copies near the end of what it has
-      long long at = blockIdx.x;
+      int at = blockIdx.x;
       for (uint32_t round = 0;; round++) {
         int4 item = make_int4(0, 0, 0, 0);
         if (at < all) {
-          const int block = (int)(at / ((long long)pieces * P.span)), wide = min(P.span, P.units - block * P.span);
-          const long long in = at - (long long)block * pieces * P.span;
-          const int k = (int)(in / wide);
-          int lo = 0, hi = most - 1;                         // the level j with from_level(j + 1) <= k < from_level(j)
-          while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (from_level(mid) > k) lo = mid; else hi = mid - 1;
+          const int block = (uint32_t)at / (uint32_t)(pieces * P.span), wide = min(P.span, P.units - block * P.span), in = at - block * pieces * P.span, k = (uint32_t)in / (uint32_t)wide;
+          int lo = 0, hi = most - 1, rank, from = 0, len = 0;          // the level lo with from_level(lo + 1) <= k < from_level(lo); the rank-th sequence with more than lo row tiles
+          for (;;) {
+            const int mid = lo < hi ? (lo + hi + 1) >> 1 : lo + 1, n = from_level(mid);
+            if (lo >= hi) { rank = k - n; break; }
+            if (n > k) lo = mid; else hi = mid - 1;
           }
-          int rank = k - from_level(lo + 1), from = 0, len = 0;      // the rank-th sequence with more than lo row tiles
           bool found = false;
           auto among = [&](bool has, int row, int rows) {
             const uint32_t mask = __ballot_sync(0xffffffffu, has), hit = __ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1)) == rank);
@@ -371,37 +372,46 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             const int rows = rows_of(c + lane, row);
             among((rows + tokens - 1) / tokens > lo, row, rows);
           }
-          if (found) item = make_int4(from, len, lo * tokens, block * P.span + (int)(in - (long long)k * wide));
+          if (found) item = make_int4(from, len, lo * tokens, block * P.span + in - k * wide);
         }
         const uint32_t slot = round & 1;
-        if (!wait_warp(iempty + 8 * slot, (round >> 1 & 1) ^ 1, P.status)) break;
-        if (lane == 0) { items[slot] = item; hy::tc_arrive(ifull + 8 * slot); }
-        if (item.y <= 0 || !wait_warp(want, round & 1, P.status)) break;
+        if (!wait_warp(iempty + 8 * slot, (round >> 1 & 1) ^ 1, lost)) break;
+        if (lane == 0) {
+          const Item w{item.x, item.y, item.z, item.w};
+          const Walk k = walk_of(P, w, tokens);
+          const Seen cta = seen_by(P, k, w.tok, k.t1 - 1);
+          items[slot][0] = item;
+          items[slot][1] = make_int4(k.t1, k.low, k.kept, k.n);
+          items[slot][2] = make_int4(cta.kept, cta.some, cta.upto, cta.all);
+          items[slot][3].x = cta.end;
+          hy::tc_arrive(ifull + 8 * slot);
+        }
+        if (item.y <= 0 || !wait_warp(want, round & 1, lost)) break;
         if (lane == 0) {
           mbar_expect_tx(claimed, 16);
           asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(&claim)), "r"(claimed) : "memory");
         }
-        if (!wait_warp(claimed, round & 1, P.status)) break;
+        if (!wait_warp(claimed, round & 1, lost)) break;
         uint32_t got, next;
         asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%2];\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
                      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}" : "=r"(got), "=r"(next) : "r"(smem_u32(&claim)) : "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (read ahead of the next claim's write)
         __syncwarp();
-        at = got ? (long long)next : all;
+        at = got ? (int)next : all;
       }
     } else if (warp == 14) {                                 // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
       Item w;
+      Walk k;
+      Seen cta;
       const int boxes = (P.dv + 63) / 64;
       const uint32_t inf = BF16 ? 0x7f807f80u : 0x7c007c00u;
       uint32_t n = 0, par = 0;                               // par: a bit for each place
       bool alive = true;
-      while (alive && take(w)) {
-        const Walk k = walk_of(P, w, tokens);
-        const Seen cta = seen_by(P, k, w.tok, k.t1 - 1);
+      while (alive && take(w, k, cta)) {
         for (int i = 0; i < k.n && alive; i++, n = n + 1 == VP ? 0 : n + 1) {
           if (cta.all_of(i)) continue;
           const int key0 = key_of(k, i);
-          alive = wait_warp(vraw + 8 * n, par >> n & 1, P.status);
+          alive = wait_warp(vraw + 8 * n, par >> n & 1, lost);
           par ^= 1u << n;
           bool odd = false;
 #pragma unroll 4
@@ -428,11 +438,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, res = o_at + t * 128 + lanes;
     uint32_t passed = 0, took = 0;
     Item w;
+    Walk k;
+    Seen cta;
     bool ok = true;
-    while (ok && take(w)) {
+    while (ok && take(w, k, cta)) {
       const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
       if (a >= w.len) continue;
-      const Walk k = walk_of(P, w, tokens);
       const int pos = exists ? a + tok_of : 0x3fffffff;
       const bool mine = pos < w.len, idle = !__any_sync(0xffffffffu, mine);
       float m = kLowest, l = 0.f, limit = -INFINITY;         // limit: where a maximum moves the reference; any does while that is beyond kFar
@@ -443,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         const int key0 = key_of(k, i);
         const uint32_t place = passed & 1, s_at = tmem + (2 * t + place) * kTile + lanes, p_bar = pfull + 16 * t + 8 * place;
         const bool masked = !tile.all_of(i);
-        ok = wait_warp(sfull + 16 * t + 8 * place, (passed >> 1) & 1, P.status);
+        ok = wait_warp(sfull + 16 * t + 8 * place, (passed >> 1) & 1, lost);
         if (!ok) break;
         if (idle) {                                          // (its rows' results are whatever comes of the scores as weights, and go nowhere)
           __syncwarp();
@@ -485,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
           }
           if (any) {
             // The product ahead must be through.  A wait by parity is right while the barrier is in the phase asked for or the one behind it: these scores waited for the product before that one
-            ok = wait_warp(pvdone + 16 * t + 8 * (place ^ 1), ((passed - 1) >> 1) & 1, P.status);
+            ok = wait_warp(pvdone + 16 * t + 8 * (place ^ 1), ((passed - 1) >> 1) & 1, lost);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int d = 0; d < P.dv; d += 16) {
@@ -521,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         passed++;
         any = true;
       }
-      ok = ok && wait_warp(odone + 8 * t, took & 1, P.status);
+      ok = ok && wait_warp(odone + 8 * t, took & 1, lost);
       took++;
       if (!ok || idle) continue;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -560,6 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       }
     }
   }
+  if (lost && lane == 0 && P.status) atomicOr(P.status, ST_WAIT);
   __syncthreads();
   if (warp == 8) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

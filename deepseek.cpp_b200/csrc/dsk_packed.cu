@@ -159,10 +159,15 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   CK(on.error);
   prompt::Params P;
   P.group = heads / kv_heads;
-  // heads of a row tile: a divisor of the group that fills most of its 128 rows, the largest of those (its tokens are then few, and their keys end close together)
+  // Heads of a row tile, a divisor of the group: with more of them a tile has fewer tokens, whose keys end close together, and short prompts make fewer pieces.  The most that fill all 128 rows,
+  // if those are four or more; else the most that leave at most 8 of them empty (us, packed / a head by itself or in pairs: 7 heads, 222 prompts of 60 tokens 35 / 86, 8192 tokens 211 / 210; 3: 18 / 34,
+  // 119 / 122; 6: 28 / 40, 178 / 174; 12 in fours 30, 170, all together 27, 180)
   P.pack = 1;
   for (int n = 2; n <= std::min(P.group, 128); n++)
-    if (P.group % n == 0 && 128 / n * n >= 128 / P.pack * P.pack) P.pack = n;
+    if (P.group % n == 0 && 128 % n == 0) P.pack = n;
+  if (P.pack < 4)
+    for (int n = P.pack + 1; n <= std::min(P.group, 128); n++)
+      if (P.group % n == 0 && 128 % n <= 8) P.pack = n;
   P.tokens = 128 / P.pack; P.subs = P.group / P.pack; P.units = kv_heads * P.subs;
   // Key heads that are worked on at a time: those whose keys and values take half of the L2, so that later rows find there what earlier ones read (32 heads of 192 + 128 entries, 22508 rows:
   // 870 us with all at a time, at 1420 MHz under the power limit; 774 with 4, 789 with 8); with fewer than that the last ones leave gaps (16 heads of 128, 8192 rows: 147 with all, 150 with 4)

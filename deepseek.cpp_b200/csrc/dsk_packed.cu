@@ -119,21 +119,23 @@ int check_rows(const char* what, const dsk_view* v, int heads, int rows) {
     if (d.first > 1 && (d.second <= 0 || d.second % 8 || d.second >= (1ll << 39))) return fail(-4, "%s: rows and heads must lie a positive multiple of 8 entries apart, got %lld and %lld", what, (long long)v->row, (long long)v->head);
   return 0;
 }
-template <int DK, int DV, bool BF16> int attend_as(const prompt::Params& P, int ctas, int device, cudaStream_t stream) {
+template <int DK, int DV, bool BF16, int JOINT> int attend_as(const prompt::Params& P, int ctas, int device, cudaStream_t stream) {
   static std::atomic<int> registers{0};                      // of a thread at launch: what its warps give and take adds up to that, or they wait for good
   if (registers.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes at{};
-    CK((cudaFuncGetAttributes(&at, prompt::attend_packed<DK, DV, BF16>)));
+    CK((cudaFuncGetAttributes(&at, prompt::attend_packed<DK, DV, BF16, JOINT>)));
     registers.store(at.numRegs, std::memory_order_relaxed);
   }
   if (registers.load(std::memory_order_relaxed) != 65536 / prompt::kThreads) return fail(-2, "dsk_packed_attn: built with %d registers a thread where %d are needed", registers.load(), 65536 / prompt::kThreads);
-  CK((allow<prompt::attend_packed<DK, DV, BF16>>(device, prompt::smem_bytes<DK, DV>())));
-  prompt::attend_packed<DK, DV, BF16><<<ctas, prompt::kThreads, prompt::smem_bytes<DK, DV>(), stream>>>(P);
+  CK((allow<prompt::attend_packed<DK, DV, BF16, JOINT>>(device, prompt::smem_bytes<DK, DV>())));
+  prompt::attend_packed<DK, DV, BF16, JOINT><<<ctas, prompt::kThreads, prompt::smem_bytes<DK, DV>(), stream>>>(P);
   CK(cudaGetLastError());
   return 0;
 }
-template <int DK, int DV> int attend_as(const prompt::Params& P, bool bf16, int ctas, int device, cudaStream_t stream) {
-  return bf16 ? attend_as<DK, DV, true>(P, ctas, device, stream) : attend_as<DK, DV, false>(P, ctas, device, stream);
+template <int DK, int DV> int attend_as(const prompt::Params& P, bool bf16, bool joint, int ctas, int device, cudaStream_t stream) {
+  if constexpr (prompt::tiles<DK, DV>() == 2)
+    if (joint) return bf16 ? attend_as<DK, DV, true, 1>(P, ctas, device, stream) : attend_as<DK, DV, false, 1>(P, ctas, device, stream);
+  return bf16 ? attend_as<DK, DV, true, 0>(P, ctas, device, stream) : attend_as<DK, DV, false, 0>(P, ctas, device, stream);
 }
 }  // namespace
 
@@ -185,16 +187,20 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   P.rows = s->rows; P.batch = s->batch; P.dk = dim_k; P.dv = dim_v;
   P.window = window >= s->rows ? 0 : window; P.keep = keep_first;
   P.f = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);            // (positive: -inf stays what it is)
-  const int tokens = P.tokens * (shape == 3 ? 1 : 2);
+  // Few pieces: both row tiles of a CTA have the same rows, each every second tile of its keys, so that the longest walk takes half the time and there are twice the pieces.  Where pieces of two row
+  // tiles would not fill the GPU (one prompt of 8192 tokens, 4 heads over 1: 69 us for 115; 20 prompts of 60, 16 over 4: 11.2 for 10.4); beyond, keys and values are read twice as often (four
+  // prompts of 4096 tokens: 73 us for 65)
+  const bool joint = shape != 3 && s->rows / (2ll * P.tokens) * P.units <= multiprocessors(s->device);
+  const int tokens = P.tokens * (shape == 3 || joint ? 1 : 2);
   const long long items = ((long long)s->rows / tokens + std::min(s->batch, s->rows)) * P.units;   // at most, whatever the lengths
   if (items > INT32_MAX) return fail(-4, "%lld pieces of work: at most 2^31", items);
   const int ctas = (int)items;                               // (those that are running take over the others)
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dt == DSK_DT_BF16;
   switch (shape) {
-    case 0: return attend_as<64, 64>(P, bf16, ctas, s->device, st);
-    case 1: return attend_as<128, 128>(P, bf16, ctas, s->device, st);
-    case 2: return attend_as<192, 128>(P, bf16, ctas, s->device, st);
-    default: return attend_as<256, 256>(P, bf16, ctas, s->device, st);
+    case 0: return attend_as<64, 64>(P, bf16, joint, ctas, s->device, st);
+    case 1: return attend_as<128, 128>(P, bf16, joint, ctas, s->device, st);
+    case 2: return attend_as<192, 128>(P, bf16, joint, ctas, s->device, st);
+    default: return attend_as<256, 256>(P, bf16, joint, ctas, s->device, st);
   }
 }

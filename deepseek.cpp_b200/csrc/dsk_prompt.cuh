@@ -11,6 +11,7 @@
 // largest value; fp16 weights lie between 2^-24 and 2^14, references 2^7 below the maximum.  Sums are of the weights ahead of their rounding, which is off by half a step of the type at most.
 // Infinities and NaN among values that a row does not see must not reach it as 0 x inf: in tiles that some row does not see whole they go to the products as zeros, and rows that do see
 // one get it back at the end.
+// Few rows: both row tiles of a CTA have the same rows, each every second tile of their keys (joint; the second one's results are added in the reference of both, from its half of TMEM, at the end).
 // Work: pieces are dealt out with the longest walks first; CTAs take over pieces of CTAs that have not started (clusterlaunchcontrol), so that nothing but starts is needed to balance them.
 // Short prompts: a piece of one tile runs through the code of every role once, and what does not fit the instruction cache is fetched each time (39 % of its lines, a softmax of one tile 4500 cycles
 // where it has 1350 by itself).  So the code that pieces run through is kept small: walks are worked out by the warp that deals, one form of each product, one place that counts levels, waits that
@@ -124,29 +125,31 @@ template <bool BF16> __device__ __noinline__ void give_back(const Params& P, con
   }
 }
 
-template <int DK, int DV, bool BF16>
+template <int DK, int DV, bool BF16, int joint>              // joint: 1: both row tiles have the same rows
 __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_constant__ Params P) {
   constexpr int TILES = tiles<DK, DV>(), KP = k_places<DK, DV>(), VP = v_places<DK, DV>(), KB = kTile * DK * 2, VB = kTile * DV * 2, SOFT = 4 * TILES, USERS = SOFT + 2 * TILES + 3;
   constexpr float LEAD = BF16 ? 40.f : -7.f, ROOM = BF16 ? -26.f : 14.f;       // a reference is taken LEAD above its maximum, and follows once that is above m + ROOM
   constexpr int MANY = 192, FEW = 64;                        // registers of a softmax thread and of another one: 512 threads have 128 each
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t bars[76];
+  __shared__ __align__(8) uint64_t bars[78];
   __shared__ int4 items[2][4];                               // [slot][item, walk, what its rows see (and the end of that)]
   __shared__ __align__(16) uint4 claim;
   __shared__ uint32_t tmem_slot;
   __shared__ int odd_values, pieces;
+  __shared__ float2 halves[TILES == 2 ? kRows : 1];          // reference and sum of the second row tile's rows, where both have the same (0 and no weight: it had no tile)
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, qs = base, ks = qs + kRows * TILES * DK * 2, vs = ks + KP * KB, b0 = smem_u32(bars);
   const uint32_t kfull = b0, kempty = b0 + 64, vfull = b0 + 128, vempty = b0 + 192, vok = b0 + 256, vraw = b0 + 320, sfull = b0 + 384, pfull = b0 + 416, pvdone = b0 + 448, flushed = b0 + 480,
-                 qfull = b0 + 512, qempty = b0 + 528, odone = b0 + 544, ifull = b0 + 560, iempty = b0 + 576, want = b0 + 592, claimed = b0 + 600;
+                 qfull = b0 + 512, qempty = b0 + 528, odone = b0 + 544, ifull = b0 + 560, iempty = b0 + 576, want = b0 + 592, claimed = b0 + 600, joined = b0 + 608, joint_read = b0 + 616;
   // keys and values: for each place (vraw: where values land that are looked at ahead of their products); scores, weights, products: [row tile][place]
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tokens = TILES * P.tokens;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tokens = TILES == 2 && !joint ? 2 * P.tokens : P.tokens, apart = joint ? 0 : P.tokens;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; i++) {
       mbar_init(kfull + 8 * i, 1); mbar_init(kempty + 8 * i, TILES); mbar_init(vfull + 8 * i, 1); mbar_init(vempty + 8 * i, TILES); mbar_init(vok + 8 * i, 1); mbar_init(vraw + 8 * i, 1);
     }
     for (int i = 0; i < 4; i++) { mbar_init(sfull + 8 * i, 1); mbar_init(pfull + 8 * i, 4); mbar_init(pvdone + 8 * i, 1); mbar_init(flushed + 8 * i, 1); }
-    for (int i = 0; i < 2; i++) { mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); }
+    for (int i = 0; i < 2; i++) { mbar_init(qfull + 8 * i, 1); mbar_init(qempty + 8 * i, 1 + joint); mbar_init(odone + 8 * i, 1); mbar_init(ifull + 8 * i, 1); mbar_init(iempty + 8 * i, USERS); }
     mbar_init(want, 1);
+    mbar_init(joined, 4); mbar_init(joint_read, 4);
     mbar_init(claimed, 1);
     odd_values = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -221,14 +224,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       Seen cta;
       bool alive = true;
       while (alive && take(w, k, cta)) {
-        const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
+        const int a = w.tok + t * apart, b = min(a + P.tokens, w.len) - 1;
         const bool there = a < w.len;
         const Seen mine = seen_by(P, k, a, b);
-        auto sixteenths = [&](int i) { return there && mine.any_of(i) ? mine.all_of(i) ? kTile / 16 : min(kTile / 16, (b - key_of(k, i) + 16) / 16) : 0; };   // those of a tile that some row sees
+        auto sixteenths = [&](int i) { return there && mine.any_of(i) && !(joint & (i ^ t)) ? mine.all_of(i) ? kTile / 16 : min(kTile / 16, (b - key_of(k, i) + 16) / 16) : 0; };   // those of a tile that some row sees
         if (scoring) {
-          const uint64_t q_desc = hy::tc_desc(qs + t * (kRows * DK * 2));
+          const int from = joint ? 0 : t;                    // the row tile whose queries these are
+          const uint64_t q_desc = hy::tc_desc(qs + from * (kRows * DK * 2));
           const int ksteps = P.dk / 16;
-          alive = !there || wait_warp(qfull + 8 * t, took & 1, lost);
+          alive = !there || wait_warp(qfull + 8 * from, took & 1, lost);
           for (int i = 0; i < k.n && alive; i++) {
             const int see = sixteenths(i);
             const uint64_t k_desc = hy::tc_desc(ks + n * KB);
@@ -247,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             else if (lead) hy::tc_arrive(kempty + 8 * n);
             if (++n == KP) { n = 0; par[0] ^= 1; }
           }
-          if (there && alive) { commit(qempty + 8 * t, lead); took++; }
+          if (there && alive) { commit(qempty + 8 * from, lead); took++; }
         } else {
           const uint32_t pdesc = idesc | (1u << 16) | ((uint32_t)(P.dv / 8) << 17), to = o_at + t * 128;
           bool any = false;
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
             else if (lead) hy::tc_arrive(vempty + 8 * n);
             if (++n == VP) n = 0;
           }
-          if (there && alive) commit(odone + 8 * t, lead);
+          if (any && alive) commit(odone + 8 * t, lead);
         }
       }
       const uint32_t last = flushed + 16 * t + (scoring ? 0 : 8);
@@ -300,13 +304,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
           if (i == max(0, k.n - kEarly) && lane == 0) hy::tc_arrive(want);
 #pragma unroll 1
           for (int t = 0; t < TILES && alive && i == 0; t++) {
-            if (w.tok + t * P.tokens >= w.len) continue;
+            if (w.tok + t * apart >= w.len || (joint & t)) continue;
             alive = wait_warp(qempty + 8 * t, (took >> t & 1) ^ 1, lost);
             if (!alive) break;
             if (lane == 0) {
               mbar_expect_tx(qfull + 8 * t, chunks * P.tokens * P.pack * 128);
 #pragma unroll 1
-              for (int c = 0; c < chunks; c++) copy_box(qs + t * (kRows * DK * 2) + c * (kRows * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * P.tokens, qfull + 8 * t);
+              for (int c = 0; c < chunks; c++) copy_box(qs + t * (kRows * DK * 2) + c * (kRows * 128), &P.q, 64 * c, q_head, w.row + w.tok + t * apart, qfull + 8 * t);
             }
             took ^= 1u << t;
             asked |= 1u << t;
@@ -436,21 +440,22 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     const int t = warp >> 2, quad = warp & 3, r = threadIdx.x & 127, tok_of = r / P.pack;       // the thread's row: token tok_of of the tile, head r % pack
     const bool exists = r < P.tokens * P.pack;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, res = o_at + t * 128 + lanes;
-    uint32_t passed = 0, took = 0;
+    uint32_t passed = 0, took = 0, pairs = 0;                // pairs: items whose rows both row tiles had
     Item w;
     Walk k;
     Seen cta;
     bool ok = true;
     while (ok && take(w, k, cta)) {
-      const int a = w.tok + t * P.tokens, b = min(a + P.tokens, w.len) - 1;
+      const int a = w.tok + t * apart, b = min(a + P.tokens, w.len) - 1;
       if (a >= w.len) continue;
       const int pos = exists ? a + tok_of : 0x3fffffff;
       const bool mine = pos < w.len, idle = !__any_sync(0xffffffffu, mine);
       float m = kLowest, l = 0.f, limit = -INFINITY;         // limit: where a maximum moves the reference; any does while that is beyond kFar
-      bool any = false;
+      bool any = false, there = false;
       const Seen tile = seen_by(P, k, a, b);
       for (int i = 0; i < k.n; i++) {
-        if (!tile.any_of(i)) continue;
+        if (!tile.any_of(i) || (joint & (i ^ t))) continue;
+        there = true;
         const int key0 = key_of(k, i);
         const uint32_t place = passed & 1, s_at = tmem + (2 * t + place) * kTile + lanes, p_bar = pfull + 16 * t + 8 * place;
         const bool masked = !tile.all_of(i);
@@ -532,21 +537,51 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         passed++;
         any = true;
       }
-      ok = ok && wait_warp(odone + 8 * t, took & 1, lost);
-      took++;
-      if (!ok || idle) continue;
+      if (there) {
+        ok = ok && wait_warp(odone + 8 * t, took & 1, lost);
+        took++;
+      }
+      float mine_by = 1.f, other_by = 0.f;                   // what becomes of the results of the two row tiles, in one reference
+      if (joint && ok) {
+        if (t) {
+          halves[r] = make_float2(m, l);
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) hy::tc_arrive(joined);
+          ok = wait_warp(joint_read, pairs++ & 1, lost);     // (its results and halves are free again)
+          continue;
+        }
+        ok = wait_warp(joined, pairs++ & 1, lost);
+        const float2 other = halves[r];
+        const float to = fmaxf(m, other.x);
+        mine_by = exp2_fast(m - to);
+        other_by = k.n > 1 ? exp2_fast(other.x - to) : 0.f;  // (a walk of one tile leaves the second row tile none)
+        l = l * mine_by + other.y * other_by;
+      }
+      if (!ok || idle) {
+        __syncwarp();
+        if (joint && lane == 0) hy::tc_arrive(joint_read);
+        continue;
+      }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int odd = odd_values, head = w.unit / P.subs, q_head = head * P.group + (w.unit - head * P.subs) * P.pack + r - tok_of * P.pack;
       uint16_t* to = static_cast<uint16_t*>(P.out) + (long long)(w.row + pos) * P.o_row + (long long)q_head * P.o_head;
+      mine_by *= inv;
+      other_by *= inv;
 #pragma unroll 1
       for (int c = 0; c < P.dv; c += 16) {                   // (64 columns at a time: as long, and more code, which a short prompt waits for)
         uint32_t x[16];
         tmem_read16(res + c, x);
-        if (!mine) continue;
         float z[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) z[e] = __uint_as_float(x[e]) * inv;
+        for (int e = 0; e < 16; e++) z[e] = __uint_as_float(x[e]) * mine_by;
+        if (joint && k.n > 1) {
+          tmem_read16(res + 128 + c, x);
+#pragma unroll
+          for (int e = 0; e < 16; e++) z[e] = fmaf(__uint_as_float(x[e]), other_by, z[e]);
+        }
+        if (!mine) continue;
         if (odd) {                                           // (a copy: what a call is given by address lies in memory)
           float d[16];
 #pragma unroll
@@ -568,6 +603,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
 #pragma unroll
           for (int e = 0; e < 8; e++) { to[c + 2 * e] = (uint16_t)y[e]; to[c + 2 * e + 1] = (uint16_t)(y[e] >> 16); }
         }
+      }
+      if (joint) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) hy::tc_arrive(joint_read);
       }
     }
   }

@@ -200,6 +200,52 @@ def test_orders_of_rows_and_heads():
     assert (half[:, :8] == 7).all()
 
 
+def many(H):
+    """Rows of no one behind the sequences, so many that CTAs have two row tiles each (with few rows both have the same rows, each every second tile of keys)."""
+    return 42_000 // H
+
+
+@pytest.mark.parametrize("dk,dv", [(16, 16), (64, 64), (112, 128), (128, 128), (192, 128)])
+@pytest.mark.parametrize("lens", [[1], [64, 65], [300, 1, 0, 129], [700]])
+def test_two_row_tiles(lens, dk, dv):
+    Prompt(lens, 8, 4, dk, dv, dtype="f16" if dk == 64 else "bf16", spare=many(8), seed=dk + len(lens)).run()
+
+
+@pytest.mark.parametrize("H,G", [(8, 8), (14, 2), (6, 2), (24, 2), (10, 1)])
+@pytest.mark.parametrize("window,keep", [(0, 0), (100, 3), (1, 1), (64, 200)])
+def test_two_row_tiles_heads_and_windows(H, G, window, keep):
+    Prompt([400, 33], H, G, 64, 64, spare=many(H), seed=H).run(window=window, keep=keep)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_two_row_tiles_maxima_that_jump(dtype, d):
+    p = Prompt([900, 130], 8, 4, d, d, dtype=dtype, seed=8, spread=0.3, spare=many(8))
+    for at, size in ((0, 1.0), (70, 4.0), (130, 9.0), (200, 14.0), (300, 25.0), (440, 40.0), (441, 41.0), (700, 60.0)):
+        p.k[at] = torch.sign(p.q[at + 1:at + 2, 0]) * size
+    p.run()
+
+
+@pytest.mark.parametrize("window,keep", [(0, 0), (50, 3)])
+@pytest.mark.parametrize("spare", [0, many(8)])
+def test_two_row_tiles_and_what_is_not_finite(spare, window, keep):
+    p = Prompt([300, 140, 60], 8, 4, 64, 64, seed=5, spare=4 + spare)
+    p.v[40, 0, 3], p.v[70, 2, 1], p.v[131, 3, 0], p.v[299, 0, 5], p.v[300, 0, 1], p.v[439, 0, 9] = (float(x) for x in ("nan", "-inf", "inf", "-inf", "nan", "inf"))
+    p.k[450, 1, 0] = float("nan")
+    p.run(window=window, keep=keep)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_few_rows_whose_maximum_lies_in_either_half(seed):
+    """Where both row tiles of a CTA have the same rows, either one's reference may be beyond the other's by more than a weight can say, or one may have no key of a row at all."""
+    p = Prompt([130, 65, 64, 193], 2, 1, 64, 64, dtype="bf16" if seed % 2 else "f16", seed=seed, spread=0.5)
+    g = torch.Generator().manual_seed(seed)
+    for at in torch.randperm(450, generator=g)[:6].tolist():
+        p.k[at] *= 2.0 ** (seed + 2)
+    p.run()
+    p.run(window=70, keep=2)
+
+
 def test_rows_beyond_four_gigabytes():
     """Queries, keys, values and results as parts of rows that lie 16 KB apart: offsets beyond 2^32 bytes and 2^31 entries."""
     p = Prompt([90, 60], 2, 1, 64, 64, seed=16)

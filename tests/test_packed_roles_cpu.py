@@ -24,14 +24,15 @@ EARLY = 8                                                    # tiles ahead of th
 SHAPES = {64: (2, 8, 8), 128: (2, 6, 4), 192: (2, 3, 3), 256: (1, 2, 3)}      # row tiles, places of keys and of values
 
 
-def run(rng, dk, work, idle, moves, early=True):
+def run(rng, dk, work, idle, moves, early=True, joint=False):
     """work: items, each a list of (tiles of keys: (row tiles that see some of it, whether some row does not see all)) and whether the second row tile has rows.  idle: softmax warps without rows;
-    early: the wait for the product ahead, where a reference moves."""
+    early: the wait for the product ahead, where a reference moves; joint: both row tiles have the same rows, each every second tile of keys."""
     tiles, KP, VP = SHAPES[dk]
     bars = lambda n, count: [Bar(count) for _ in range(n)]
     soft = 4 * tiles
     kfull, kempty, vfull, vempty, vok, vraw = bars(KP, 1), bars(KP, tiles), bars(VP, 1), bars(VP, tiles), bars(VP, 1), bars(VP, 1)
-    qfull, qempty, odone, ifull = (bars(2, 1) for _ in range(4))
+    qfull, qempty, odone, ifull = bars(2, 1), bars(2, 2 if joint else 1), bars(2, 1), bars(2, 1)
+    joined, read, halves = Bar(4), Bar(4), [None] * 4        # what the second row tile has is ready, was read; by which item and step its warps' results are
     sfull, pvdone, pfull = ([bars(2, n) for _ in range(2)] for n in (1, 1, 4))            # [row tile][place]
     iempty, flushed = bars(2, soft + 2 * tiles + 3), [bars(2, 1) for _ in range(2)]
     items, want = [None, None], Bar(1)
@@ -72,7 +73,7 @@ def run(rng, dk, work, idle, moves, early=True):
                 if i == max(0, len(walk) - EARLY):
                     want.arrive()
                 for t in range(tiles if i == 0 else 0):
-                    if t and not two:
+                    if t and (joint or not two):
                         continue
                     yield qempty[t].wait((took[t] & 1) ^ 1)
                     flying.append((queries, t, n, qfull[t]))
@@ -112,7 +113,7 @@ def run(rng, dk, work, idle, moves, early=True):
 
     def product_of_scores(t, n, i, unit, at):
         def product():
-            assert keys[unit] == (n, i) and queries[t] == n
+            assert keys[unit] == (n, i) and queries[0 if joint else t] == n
             assert scores[t][at] is None or scores[t][at] in through[t]          # what lay there was handed over and read
             scores[t][at], weights[t][at] = (n, i), {}
         return product
@@ -135,7 +136,7 @@ def run(rng, dk, work, idle, moves, early=True):
             walk, two = work[n]
             there = t == 0 or two
             if there:
-                yield qfull[t].wait(took)
+                yield qfull[0 if joint else t].wait(took)
             for i, (who, _) in enumerate(walk):
                 yield kfull[kn].wait(par)
                 if there and t in who:
@@ -150,7 +151,7 @@ def run(rng, dk, work, idle, moves, early=True):
                     kempty[kn].arrive()
                 kn, par = (0, par ^ 1) if kn + 1 == KP else (kn + 1, par)
             if there:
-                queue.append(qempty[t])
+                queue.append(qempty[0 if joint else t])
                 took += 1
         queue.append(flushed[0][t])
         yield flushed[0][t].wait(0)
@@ -179,7 +180,7 @@ def run(rng, dk, work, idle, moves, early=True):
                 else:
                     vempty[vn].arrive()
                 vn = (vn + 1) % VP
-            if there:
+            if there and any(t in who for who, _ in walk):
                 queue.append(odone[t])
         queue.append(flushed[1][t])
         yield flushed[1][t].wait(0)
@@ -187,7 +188,7 @@ def run(rng, dk, work, idle, moves, early=True):
     def softmax(x):
         t, w = divmod(x, 4)
         me = {"turn": 0}
-        passed = took = 0
+        passed = took = pairs = 0
         while True:
             yield from take(me)
             n = me["item"]
@@ -217,11 +218,27 @@ def run(rng, dk, work, idle, moves, early=True):
                 pfull[t][at].arrive()
                 passed += 1
                 last = (n, step)
-            yield odone[t].wait(took)
-            took += 1
-            if not idle[n][x]:
+            if any(t in who for who, _ in walk):
+                yield odone[t].wait(took)
+                took += 1
+            if not idle[n][x] and last is not None:
                 assert through[t][-1:] == [last]
                 yield None
+            if joint and t:
+                halves[w] = (n, last)
+                yield None
+                joined.arrive()
+                yield read.wait(pairs)
+                pairs += 1
+            elif joint:
+                yield joined.wait(pairs)
+                if not idle[n][x]:
+                    assert halves[w] == (n, last and max(((n, i) for i, (who, _) in enumerate(walk) if 1 in who), default=None))
+                    assert halves[w][1] is None or through[1][-1:] == [halves[w][1]]
+                    yield None
+                    assert (halves[w][1] is None or through[1][-1:] == [halves[w][1]]) and through[0][-1:] == [last]
+                read.arrive()
+                pairs += 1
 
     roles = [deal(), copy_keys(), copy_values(), *(scorer(t) for t in range(tiles)), *(adder(t) for t in range(tiles)), look()] + [softmax(x) for x in range(soft)]
     speed = [rng.choice([1, 1, 1, 10, 0.05]) for _ in roles] + [rng.choice([1, 0.1, 10]) for _ in range(2)]
@@ -262,6 +279,16 @@ def test_roles_meet_in_every_order(dk):
     rng = random.Random(dk)
     for _ in range(400):
         run(rng, **draw(rng, dk))
+
+
+@pytest.mark.parametrize("dk", [64, 128, 192])
+def test_roles_meet_where_row_tiles_share_their_rows(dk):
+    rng = random.Random(dk + 1)
+    for _ in range(400):
+        x = draw(rng, dk)
+        x["work"] = [([({i & 1}, masked) for i, (_, masked) in enumerate(walk)], True) for walk, _ in x["work"]]
+        x["idle"] = [row[:4] * 2 for row in x["idle"]]
+        run(rng, **x, joint=True)
 
 
 def test_the_wait_for_the_product_ahead_is_needed():
@@ -306,3 +333,17 @@ def test_what_rows_see_of_the_tiles():
                     assert all(sees(x, y) for x in (a, b) for y in keys)
                 elif not window:
                     assert not all(sees(a, y) for y in keys)
+
+
+def test_a_row_tile_by_itself_sees_something_of_every_tile():
+    """Where both row tiles have the same rows, each every second tile of the walk (seen_by, csrc/dsk_prompt.cuh): a walk of two tiles or more has work for both."""
+    T, rng = 64, random.Random(1)
+    for _ in range(4000):
+        window, keep = rng.choice([0, 0, 1, 2, rng.randint(1, 300), rng.randint(1, 900)]), rng.choice([0, 1, 64, 65, rng.randint(0, 400)])
+        a, n = rng.randint(0, 700), rng.choice([1, 2, 7, 32, 64, 128])
+        t1 = a + rng.randint(1, n)
+        low = max(0, a + 1 - window) // T if window else 0
+        first = -(-min(keep, t1) // T) if window else 0
+        kept = min(first, low)
+        some, upto = max(0, a + 1 - window) // T + kept - low if window else 0, (t1 - 1) // T + 1 + kept - low
+        assert all(i < upto and (i < first or i >= some) for i in range(kept + -(-t1 // T) - low))

@@ -166,6 +166,16 @@ __device__ __forceinline__ bool piece(const Cache& C, const Pieces& S, int, Piec
   return true;
 }
 
+__device__ __forceinline__ uint4 in_new_scale(uint4 c, float ratio) {                  // 16 codes, times a power of two
+  uint32_t* w = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const float2 lo = two_values(w[u]), hi = two_values(w[u] >> 16);
+    w[u] = four_codes(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+  }
+  return c;
+}
+
 // A CTA of TH threads writes one block of one head, keys or values; its values stay in registers between the maximum and the codes (R eights a thread).
 template <typename T, int TH, int R, bool WIDE, typename Where>
 __global__ void __launch_bounds__(TH) write_rows(const Cache C, const Where S, const T* k, const T* v, const Pitch pk, const Pitch pv) {
@@ -213,16 +223,7 @@ __global__ void __launch_bounds__(TH) write_rows(const Cache C, const Where S, c
   if (threadIdx.x == 0) *scale = now;                        // (every thread has read the old one ahead of the maximum)
   if (p.kept && old != now) {                                // rows of earlier calls, in the new scale
     const float ratio = old * inv;
-    for (int i = threadIdx.x; i < p.kept * dim / 16; i += TH) {
-      uint4 c = reinterpret_cast<uint4*>(dst)[i];
-      uint32_t* w = reinterpret_cast<uint32_t*>(&c);
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const float2 lo = two_values(w[u]), hi = two_values(w[u] >> 16);
-        w[u] = four_codes(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
-      }
-      reinterpret_cast<uint4*>(dst)[i] = c;
-    }
+    for (int i = threadIdx.x; i < p.kept * dim / 16; i += TH) reinterpret_cast<uint4*>(dst)[i] = in_new_scale(reinterpret_cast<uint4*>(dst)[i], ratio);
   }
   uint2* to = reinterpret_cast<uint2*>(dst + p.kept * dim) + threadIdx.x;
 #pragma unroll
@@ -235,6 +236,56 @@ __global__ void __launch_bounds__(TH) write_rows(const Cache C, const Where S, c
       c.y = four_codes(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
       to[i * TH] = c;
     }
+}
+
+// The same where most pieces have few rows: 64 threads that read their values twice (the second time from the L1, mostly), so that many CTAs fit and one for a row or for nothing costs little.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(64) write_few(const Cache C, const Pieces S, const T* k, const T* v, const Pitch pk, const Pitch pv) {
+  constexpr int TH = 64, AHEAD = 4;
+  __shared__ uint32_t most[TH / 32];
+  const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
+  Piece p;
+  if (!piece(C, S, 0, p) || !known(C, p)) return;
+  const int dim = C.dim[which], per = dim / 8, total = p.rows * per;
+  const Pitch at = which ? pv : pk;
+  const T* src = (which ? v : k) + p.from * at.row + h * at.head;
+  auto eight = [&](int i) { const int row = i / per; return load_eight<T, WIDE>(src + row * at.row + (i - row * per) * 8); };
+  float* scale = C.scale[which] + (size_t)p.page * C.heads + h;
+  unsigned char* dst = C.code[which] + ((size_t)p.page * C.heads + h) * C.block * dim;
+  const float old = p.kept ? *scale : 0.f;
+  Highest<T> top;
+#pragma unroll AHEAD
+  for (int i = threadIdx.x; i < total; i += TH) higher(top, eight(i));
+  float m = magnitude(top);
+  if (!(m < INFINITY)) {                                     // an infinity, which makes no scale: once more without
+    top.v = 0;
+    for (int i = threadIdx.x; i < total; i += TH) highest_number(top, eight(i));
+    m = magnitude(top);
+  }
+  const uint32_t own = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+  if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = own;
+  __syncthreads();
+  const float need = pow2(scale_exponent(__uint_as_float(max(most[0], most[1])))), now = p.kept ? fmaxf(old, need) : need, inv = __uint_as_float((254u << 23) - __float_as_uint(now));
+  if (threadIdx.x == 0) *scale = now;                        // (every thread has read the old one ahead of the barrier)
+  if (p.kept && old != now) {                                // rows of earlier calls, in the new scale
+    const float ratio = old * inv;
+    uint4* codes = reinterpret_cast<uint4*>(dst);
+    const int n = p.kept * dim / 16;
+    for (int i = threadIdx.x; i < n; i += AHEAD * TH) {
+      uint4 c[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; u++) if (i + u * TH < n) c[u] = codes[i + u * TH];
+#pragma unroll
+      for (int u = 0; u < AHEAD; u++) if (i + u * TH < n) codes[i + u * TH] = in_new_scale(c[u], ratio);
+    }
+  }
+  uint2* to = reinterpret_cast<uint2*>(dst + p.kept * dim);
+#pragma unroll AHEAD
+  for (int i = threadIdx.x; i < total; i += TH) {
+    float f[8];
+    floats(eight(i), f);
+    to[i] = make_uint2(four_codes(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), four_codes(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+  }
 }
 
 template <typename T> __device__ __forceinline__ T rounded(float x);

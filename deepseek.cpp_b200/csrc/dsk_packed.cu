@@ -74,6 +74,16 @@ extern "C" int dsk_blocks_cut(const dsk_blocks* p, int32_t* table, int64_t table
   return 0;
 }
 
+namespace {
+template <typename T> int write_few(const dsk_kv8* c, const kv8::Pieces& at, dim3 grid, const dsk_view* k, const dsk_view* v, cudaStream_t stream) {
+  const T *pk = static_cast<const T*>(k->data), *pv = static_cast<const T*>(v->data);
+  if (wide(k) && wide(v)) kv8::write_few<T, true><<<grid, 64, 0, stream>>>(cache_of(c), at, pk, pv, pitch_of(k), pitch_of(v));
+  else kv8::write_few<T, false><<<grid, 64, 0, stream>>>(cache_of(c), at, pk, pv, pitch_of(k), pitch_of(v));
+  CK(cudaGetLastError());
+  return 0;
+}
+}  // namespace
+
 extern "C" int dsk_kv8_append(const dsk_kv8* c, const dsk_packed* s, const dsk_view* k, const dsk_view* v, void* stream) {
   if (const int code = check_cache(c)) return code;
   if (const int code = check_packed(s)) return code;
@@ -88,7 +98,14 @@ extern "C" int dsk_kv8_append(const dsk_kv8* c, const dsk_packed* s, const dsk_v
   if (s->device != c->device) return fail(-1, "packed rows on device %d, a cache on %d", s->device, c->device);
   OnDevice on(c->device);
   CK(on.error);
-  return write_all(c, kv8::Pieces{reinterpret_cast<const int4*>(s->pieces), s->rows}, dim3(s->n_pieces, 2 * c->kv_heads), std::min(s->rows, c->block), k, v, static_cast<cudaStream_t>(stream));
+  const kv8::Pieces at{reinterpret_cast<const int4*>(s->pieces), s->rows};
+  const dim3 grid(s->n_pieces, 2 * c->kv_heads);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Fewer than 32 rows to a sequence, and blocks that take more than a warp or two: 64 threads read their values twice (211 sequences of one token, 8 heads of 192 + 128, blocks of 128: 4.9 us where a
+  // CTA with registers for the whole block takes 26; 200 of one and one of 2000: 16 for 33; 100 of 32: 9.1 for 20.5; but 31 of one and one of 1000, 32 on average: 9.8 for 8.6)
+  if (s->rows / s->batch < 32 && std::min(s->rows, c->block) * std::max(c->dim_k, c->dim_v) / 8 > 512)
+    return dt == DSK_DT_F32 ? write_few<float>(c, at, grid, k, v, st) : dt == DSK_DT_F16 ? write_few<__half>(c, at, grid, k, v, st) : write_few<__nv_bfloat16>(c, at, grid, k, v, st);
+  return write_all(c, at, grid, std::min(s->rows, c->block), k, v, st);
 }
 
 namespace {

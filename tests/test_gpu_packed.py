@@ -556,6 +556,43 @@ def test_append(dtype, H, dk, dv, block):
     cache.check()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("H,dk,dv,block,odd", [(2, 128, 128, 64, 0), (1, 80, 256, 128, 0), (2, 192, 128, 128, 0), (1, 96, 80, 64, 3)])
+def test_append_few_rows_to_many_sequences(dtype, H, dk, dv, block, odd):
+    """Decoded tokens of many sequences with a prompt or two among them (odd: rows at odd pitches), infinities and NaN among the values: codes and scales are those of the definition, bit for bit."""
+    B = 24
+    p = Pool(200, block, B, 6, seed=dk + block)
+    cache, k, ks, v, vs = cache_of(p.rng, 200, H, block, dk, dv)
+    lens = [0] * B
+    mixed = [1] * 18 + [0, 130, 3, block, 1, block + 1]
+    for step, (count, spare) in enumerate(((mixed, 0), ([1] * B, 60), (mixed[::-1], 7), ([4] * B, 0), ([0] * 23 + [block - 1], 40))):
+        plan, new, _ = p.extend(lens, count, sum(count) + spare)
+        rows = sum(count) + spare
+        size = torch.exp(2.5 * torch.randn(rows, H, 1))
+        x, y = ((torch.randn(rows, H, d + odd) * size).to(DT[dtype]) for d in (dk, dv))
+        x, y = x[..., odd:], y[..., :dv]
+        x[sum(count):], y[sum(count):] = float("nan"), float("inf")
+        if step in (0, 2):
+            y[3, 0, 5], y[sum(count) - 1, H - 1, dv - 1], x[20, 0, 0] = float("inf"), float("-inf"), float("nan")
+        cache.append(x.to(DEV) if not odd else torch.cat([x, x[..., :odd]], -1).to(DEV)[..., :dk], y.to(DEV) if not odd else torch.cat([y, y[..., :odd]], -1).to(DEV)[..., :dv], plan)
+        for b in range(B):
+            at = slice(sum(count[:b]), sum(count[:b + 1]))
+            so.write(k, ks, p.table[b:b + 1], [lens[b]], [count[b]], x[None, at].double().numpy())
+            so.write(v, vs, p.table[b:b + 1], [lens[b]], [count[b]], y[None, at].double().numpy())
+        lens = new
+        assert np.array_equal(cache.k_scale.cpu().numpy(), ks) and np.array_equal(cache.v_scale.cpu().numpy(), vs)
+        for got, want in ((cache.k, k), (cache.v, v)):       # (a NaN's sign is nobody's)
+            g = got.view(torch.uint8).cpu().numpy()
+            assert ((g == want) | ((g & 0x7f == 0x7f) & (want & 0x7f == 0x7f))).all()
+    cache.check()
+    small = dsk.Cache8(3, H, dk, dv, block=block, device=0)  # fewer blocks than the plan has numbers: nothing outside is touched
+    plan, _, _ = p.extend(lens, mixed, sum(mixed))
+    x, y = (torch.ones(sum(mixed), H, d, dtype=DT[dtype], device=DEV) for d in (dk, dv))
+    small.append(x, y, plan)
+    with pytest.raises(dsk.DskError, match="outside the cache"):
+        small.check()
+
+
 def test_append_strided_and_refused():
     p = Pool(20, 16, 2, 4, seed=8)
     cache, k, ks, v, vs = cache_of(p.rng, 20, 2, 16, 64, 64)

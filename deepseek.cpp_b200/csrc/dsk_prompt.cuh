@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     for (int b = lane + 32 * kHeld; b < P.batch; b += 32) most = max(most, tiles_of(b));
     most = __reduce_max_sync(0xffffffffu, most);
     const int n = from_level(0);
-    if (lane == 0) pieces = n;
+    if (lane == 0) pieces = min(n, 0x7fffffff / P.units);    // (starts that fall may make more of them than the host allows for)
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();

@@ -17,9 +17,9 @@
 // where it has 1350 by itself).  So the code that pieces run through is kept small: walks are worked out by the warp that deals, one form of each product, one place that counts levels, waits that
 // note in a register that they gave up (222 prompts of 60 tokens, 8 heads over 8: 43 us where it was 60; 64 prompts of 1 to 200: 26, was 31).
 // Bound: between tensor pipe and softmax.  Of 1470 cycles for 256 rows and 64 keys of 128 + 128 entries the tensor pipe has 1280 (products of 64 keys read their operands from shared memory in 48 cycles
-// for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 832 us
-// (1.32 PFLOP/s; a measured product of matrices 1.68), at 1.6 GHz under the power limit; back to back 940.  32 heads of 192 + 128, 8 prompts of up to 5001 tokens: 775 us (1.06); 256 + 256: 99 us
-// (0.80), 64 + 64, windowed: 155 us.  Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820),
+// for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 823 us
+// (1.34 PFLOP/s; a measured product of matrices 1.68), at 1.6 GHz under the power limit; back to back 940.  32 heads of 192 + 128, 8 prompts of up to 5001 tokens: 751 us (1.09); 256 + 256: 99 us
+// (0.80), 64 + 64, windowed: 151 us.  Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820),
 // maxima only where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0023 in bf16, the plain form's 0.0016).
 #pragma once
 
@@ -209,8 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
     return ok && w.len > 0;
   };
 
-  if (blockIdx.x >= all) {                                   // (nothing for this CTA: the grid is launched for as many pieces as there may be)
-  } else if (warp >= 8) {
+  if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW));
     const bool scoring = warp < 8 + TILES, adding = warp == 11 || warp == 10 + TILES;
     if (scoring || adding) {                                 // products of a row tile: scores, or weights x values.  (A warp for each: neither waits behind the other's)
@@ -347,11 +346,29 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
       for (uint32_t s = 0; s < 2 * VP; s++)                  // no copy is under way at the end, whatever happened
         if (sent[s & 1] >> (s >> 1) & 1) wait_warp((s & 1 ? vraw : vfull) + 8 * (s >> 1), ~(vpar[s & 1] >> (s >> 1)) & 1, lost);
     } else if (warp == 15) {                                 // deals out the work: rows with most keys first, so that the short ones fill the gaps, of as many heads at a time as the L2 holds
-      // CTAs take over work of CTAs that have not started yet, each when its copies near the end of what it has
+      // CTAs take over work of CTAs that have not started yet, each when its copies near the end of what it has.  The grid is launched for as many pieces as there may be: CTAs that have none are
+      // taken over one behind the other, without a start (37 tokens in 65536 rows, 901 sequences, 16 heads over 4: 20 us where each started and ended 157)
+      uint32_t claims = 0;
+      auto take_over = [&] {                                 // the CTA whose work is taken over, -1: none is left (and no other may be asked for)
+        if (lane == 0) {
+          mbar_expect_tx(claimed, 16);
+          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(&claim)), "r"(claimed) : "memory");
+        }
+        if (!wait_warp(claimed, claims++ & 1, lost)) return -1;
+        uint32_t got, next;
+        asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%2];\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                     "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}" : "=r"(got), "=r"(next) : "r"(smem_u32(&claim)) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (read ahead of the next claim's write)
+        __syncwarp();
+        return got ? (int)next : -1;
+      };
       int at = blockIdx.x;
+      bool asks = false;
       for (uint32_t round = 0;; round++) {
         int4 item = make_int4(0, 0, 0, 0);
-        if (at < all) {
+#pragma unroll 1
+        while (asks || at >= all) { at = take_over(); asks = false; }
+        if (at >= 0) {
           const int block = (uint32_t)at / (uint32_t)(pieces * P.span), wide = min(P.span, P.units - block * P.span), in = at - block * pieces * P.span, k = (uint32_t)in / (uint32_t)wide;
           int lo = 0, hi = most - 1, rank, from = 0, len = 0;          // the level lo with from_level(lo + 1) <= k < from_level(lo); the rank-th sequence with more than lo row tiles
           for (;;) {
@@ -391,17 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
           hy::tc_arrive(ifull + 8 * slot);
         }
         if (item.y <= 0 || !wait_warp(want, round & 1, lost)) break;
-        if (lane == 0) {
-          mbar_expect_tx(claimed, 16);
-          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(&claim)), "r"(claimed) : "memory");
-        }
-        if (!wait_warp(claimed, round & 1, lost)) break;
-        uint32_t got, next;
-        asm volatile("{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%2];\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
-                     "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}" : "=r"(got), "=r"(next) : "r"(smem_u32(&claim)) : "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (read ahead of the next claim's write)
-        __syncwarp();
-        at = got ? (int)next : all;
+        asks = true;
       }
     } else if (warp == 14) {                                 // values of tiles that some row does not see whole: rows behind the sequence, infinities and NaN become zeros
       Item w;

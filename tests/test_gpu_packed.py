@@ -661,3 +661,33 @@ def test_serving_with_packed_rows():
     cache.check()
     pool.cut(table, t_lens, ints([0] * B))
     assert sorted(pool.free[:30].tolist()) == list(range(30)) and int(pool.n_free.item()) == 30
+
+
+def falling(batch, rows, seed):
+    """Starts of which every eighth falls or lies outside, and the last one is not the highest."""
+    rng = np.random.default_rng(seed)
+    s = np.sort(rng.integers(0, rows + 1, size=batch + 1))
+    odd = rng.permutation(batch + 1)[:batch // 8 + 1]
+    s[odd] = rng.integers(-rows, 2 * rows, size=len(odd))
+    s[-1] = rows // 3
+    return s
+
+
+@pytest.mark.parametrize("H,G,d,rows,starts", [
+    (2, 1, 64, 210, [0, 100, 150, 120, 1 << 30, -5, 90]), (2, 1, 64, 210, [0, 100, 150, 120, 200, -5, 90]), (1, 1, 64, 300, [120, 40]), (16, 16, 64, 4096, [0, 4096, 0, 4096]),
+    (4, 2, 128, 9000, [0, 9000] * 40), (16, 16, 192, 3000, [0, 2000, 100, 3000, -1, 3000]), (8, 4, 256, 2500, [7, 2500, 7, 2400, 2500, 0])]
+    + [(4, 1, 64, 2000, falling(b, 2000, b)) for b in (7, 33, 256, 257, 300, 1024)] + [(16, 16, 128, 20000, falling(b, 20000, b)) for b in (5, 1000)])
+def test_starts_that_fall_are_the_highest_ahead_of_them(H, G, d, rows, starts):
+    """Results are those of the starts that include/dsk.h says they are taken as, and rows of no one stay what they were, in every call."""
+    g = torch.Generator(device=DEV).manual_seed(rows + len(starts))
+    q, k, v = (torch.randn(rows, n, d, device=DEV, dtype=torch.bfloat16, generator=g) for n in (H, G, G))
+    taken = np.maximum.accumulate(np.clip(np.asarray(starts, dtype=np.int64), 0, rows))
+    results = []
+    for s in (taken, starts, starts):
+        results.append(torch.full((rows, H, d), 7.0, dtype=torch.bfloat16, device=DEV))
+        packed = dsk.Packed.of(ints(s), rows)
+        packed.attend(q, k, v, out=results[-1])
+        packed.check()
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+    first, last = int(taken[0]), int(taken[-1])
+    assert (results[1][:first] == 7.0).all() and (results[1][last:] == 7.0).all() and not (results[1][first:last] == 7.0).all(dim=(1, 2)).any()

@@ -200,13 +200,16 @@ __global__ void __launch_bounds__(kCutThreads) cut(const Cut A) {
     if (lane == 0) good[s] = n;
   }
   __syncthreads();
-  const int from = A.batch - 1 - b;                          // sums over the sequences behind a thread's own: the last one's blocks go first
-  int sum[3] = {b < A.batch ? good[from] : 0, 0, 0}, all[3];
-  const bool lost = b < A.batch && good[from] < high[from] - low[from];
+  // Sums over the sequences behind a thread's own: the last one's blocks go first.  Entries that repeat may make them up to 2^36, which two sums of 16 and 11 bits of each count hold; what comes back beyond
+  // the stack's end goes nowhere, so that a sum that is larger may be taken as that many
+  const int from = A.batch - 1 - b, count = b < A.batch ? good[from] : 0;
+  int sum[3] = {count & 0xffff, count >> 16, 0}, all[3];
+  const bool lost = b < A.batch && count < high[from] - low[from];
   sums_ahead<WARPS>(sum, all, of_warp);
-  if (b < A.batch) good[from] = sum[0];
+  auto whole = [&](const int (&x)[3]) { return (int)min((long long)x[1] * 65536 + x[0], (long long)A.P.n_blocks + 1); };
+  if (b < A.batch) good[from] = whole(sum);
   if (lost) note(A.P, ST_PAGE);
-  const int have = height;
+  const int have = height, back = whole(all);
   __syncthreads();
   for (int s = warp; s < A.batch; s += WARPS) {
     int* row = A.table + s * A.pitch;
@@ -222,8 +225,8 @@ __global__ void __launch_bounds__(kCutThreads) cut(const Cut A) {
     }
   }
   if (threadIdx.x == 0) {
-    if (have + all[0] > A.P.n_blocks) note(A.P, ST_TWICE);
-    *A.P.top = min(have + all[0], A.P.n_blocks);
+    if (have + back > A.P.n_blocks) note(A.P, ST_TWICE);
+    *A.P.top = min(have + back, A.P.n_blocks);
   }
 }
 

@@ -691,3 +691,19 @@ def test_starts_that_fall_are_the_highest_ahead_of_them(H, G, d, rows, starts):
     assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
     first, last = int(taken[0]), int(taken[-1])
     assert (results[1][:first] == 7.0).all() and (results[1][last:] == 7.0).all() and not (results[1][first:last] == 7.0).all(dim=(1, 2)).any()
+
+
+def test_more_entries_come_back_than_31_bits_count():
+    """Entries that repeat one block number, 2^31 and more of them in a call: the stack fills up and is reported, and nothing is written ahead of it or behind it."""
+    batch, width, block, n = 1024, (1 << 21) + 2048, 16, 5
+    around = torch.full((n + 200,), 77, dtype=torch.int32, device=DEV)
+    free, status = around[100:100 + n], torch.zeros(1, dtype=torch.int32, device=DEV)
+    free.copy_(ints([4, 2, -3, -3, -3]))
+    top = ints([2, 0])
+    table = torch.full((batch, width), 3, dtype=torch.int32, device=DEV)
+    lens, keep = torch.full((batch,), width * block, dtype=torch.int32, device=DEV), torch.zeros(batch, dtype=torch.int32, device=DEV)
+    args = dsk.BlocksArgs(free.data_ptr(), top.data_ptr(), status.data_ptr(), 0, n, block)
+    assert dsk.lib().dsk_blocks_cut(args, table.data_ptr(), width, width, lens.data_ptr(), keep.data_ptr(), batch, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert free.tolist() == [4, 2, 3, 3, 3] and top.tolist() == [n, 0] and int(status) == po.TWICE
+    assert (around[:100] == 77).all() and (around[100 + n:] == 77).all() and bool((table.view(-1)[:1 << 31] == -1).all()) and bool((table.view(-1)[1 << 31:] == -1).all())

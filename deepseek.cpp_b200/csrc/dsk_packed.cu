@@ -4,6 +4,7 @@
 #include "dsk_serve_host.cuh"
 
 #include <algorithm>
+#include <cstring>
 
 #include "dsk_blocks.cuh"
 #include "dsk_prompt.cuh"
@@ -203,7 +204,13 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   P.wide_o = aligned(out->data, 32) && out->row % 16 == 0 && out->head % 16 == 0 ? 2 : aligned(out->data, 16) && out->row % 8 == 0 && out->head % 8 == 0;
   P.rows = s->rows; P.batch = s->batch; P.dk = dim_k; P.dv = dim_v;
   P.window = window >= s->rows ? 0 : window; P.keep = keep_first;
-  P.f = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);            // (positive: -inf stays what it is)
+  // Positive, so that -inf stays what it is: scale 0 becomes the smallest number there is, 2^-149, with which no finite score reaches 2^-21.  By its bits: a host that takes such numbers for zero gives no
+  // other way
+  P.f = scale * 1.44269504088896340736f;
+  uint32_t bits;
+  std::memcpy(&bits, &P.f, 4);
+  if (!(bits & 0x7fffffffu)) bits = 1;
+  std::memcpy(&P.f, &bits, 4);
   // Few pieces: both row tiles of a CTA have the same rows, each every second tile of its keys, so that the longest walk takes half the time and there are twice the pieces.  Where pieces of two row
   // tiles would not fill the GPU (one prompt of 8192 tokens, 4 heads over 1: 69 us for 115; 20 prompts of 60, 16 over 4: 11.2 for 10.4); beyond, keys and values are read twice as often (four
   // prompts of 4096 tokens: 73 us for 65)

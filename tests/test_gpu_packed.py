@@ -707,3 +707,16 @@ def test_more_entries_come_back_than_31_bits_count():
     torch.cuda.synchronize()
     assert free.tolist() == [4, 2, 3, 3, 3] and top.tolist() == [n, 0] and int(status) == po.TWICE
     assert (around[:100] == 77).all() and (around[100 + n:] == 77).all() and bool((table.view(-1)[:1 << 31] == -1).all()) and bool((table.view(-1)[1 << 31:] == -1).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 2.0 ** -149, 1e-40, 3e-39, 2e-38])
+@pytest.mark.parametrize("H,d", [(2, 64), (16, 128)])
+def test_scales_next_to_zero(scale, H, d):
+    """Scores of up to 2^126 ahead of a scale that takes them to next to nothing: weights are all alike at 0.  (A scale off by 2^-150, as numbers that small are rounded, is off by 2^-24 in such a score.)"""
+    p = Prompt([300, 45, 1], H, 1, d, d, seed=31)
+    p.q *= 2.0 ** 59
+    p.k *= 2.0 ** 59
+    got = p.run(scale=scale)
+    if scale == 0.0:
+        mean = p.v[:300, 0].double().cumsum(0) / torch.arange(1, 301)[:, None]
+        assert ((got[:300, 0].double().cpu() - mean).abs() <= 2.0 ** -8 * mean.abs() + 2.0 ** -8 * p.v[:300, 0].double().abs().cumsum(0) / torch.arange(1, 301)[:, None] * 1.01).all()

@@ -6,8 +6,9 @@
 // given back as soon as their products are through.  Roles: a warp for the copies of keys and queries, one for those of values; for each row tile one that issues products of scores, one that issues
 // products with the values (scores lie in TMEM, weights where the scores were) and four for the softmax, a thread to a row; one that deals out the work, one that looks at values of tiles which
 // some row does not see whole.  A row tile has scores in two places, so that the products and the way there and back (1400 cycles a tile) come under the softmax of the tile ahead.
-// Weights: y = f s - m in one fused operation, f = scale log2(e); the reference m is a whole number that may lag behind the maximum, so that the results in TMEM are scaled again, by
-// powers of two, where a maximum has moved far (the thread that has the row does it).  bf16 weights have fp32's range: references lead by 2^40, so that no sum of weights x values exceeds the
+// Weights: y = f s - m in one fused operation, f = scale log2(e); the reference m is a maximum, moved by a power of two, that may lag behind, so that the results in TMEM are scaled
+// again where a maximum has moved far (the thread that has the row does it).  A weight that is the row's largest when its reference is taken is that power of two, which its rounding leaves as it is: a row
+// that sees one key has its value, bit for bit (with references that are whole numbers it was off by half a step).  bf16 weights have fp32's range: references lead by 2^40, so that no sum of weights x values exceeds the
 // largest value; fp16 weights lie between 2^-24 and 2^14, references 2^7 below the maximum.  Sums are of the weights ahead of their rounding, which is off by half a step of the type at most.
 // Infinities and NaN among values that a row does not see must not reach it as 0 x inf: in tiles that some row does not see whole they go to the products as zeros, and rows that do see
 // one get it back at the end.
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_packed(const __grid_consta
         const float top = mine ? fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * P.f : -INFINITY;
         float f = P.f;
         if (__any_sync(0xffffffffu, top > limit)) {
-          const float c_top = ceilf(top), to = fmaxf(m, fabsf(c_top) > kFar ? c_top : c_top + LEAD), by = exp2_fast(m - to);
+          const float to = fmaxf(m, fabsf(top) > kFar ? top : top + LEAD), by = exp2_fast(m - to);
           m = to;
           l *= by;
           const bool far = fabsf(m) > kFar;

@@ -720,3 +720,19 @@ def test_scales_next_to_zero(scale, H, d):
     if scale == 0.0:
         mean = p.v[:300, 0].double().cumsum(0) / torch.arange(1, 301)[:, None]
         assert ((got[:300, 0].double().cpu() - mean).abs() <= 2.0 ** -8 * mean.abs() + 2.0 ** -8 * p.v[:300, 0].double().abs().cumsum(0) / torch.arange(1, 301)[:, None] * 1.01).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("H,G,dk,dv,lens", [(4, 2, 64, 64, [300, 1, 70]), (16, 16, 128, 128, [500, 64, 65]), (3, 1, 192, 128, [200]), (2, 2, 256, 256, [150, 3]), (16, 16, 64, 64, [1] * 300)])
+def test_a_row_that_sees_one_key_has_its_value(dtype, H, G, dk, dv, lens):
+    """First rows of sequences, and every row of a window of 1, bit for bit: the one weight is the power of two that the reference lies ahead, up to what scores and the reference are rounded by.  Scores
+    here are below 2^6, which makes that 2^-18 of the weight (two roundings of half a step, 2^-19 each), and 2^-17 of the result with the exponential and the sum: less than the quarter of a step, 2^-9 or
+    2^-12, that takes a result to the next number."""
+    p = Prompt(lens, H, G, dk, dv, dtype=dtype, seed=41)
+    q, k, v = (x.to(DEV) for x in (p.q, p.k, p.v))
+    want = v.repeat_interleave(H // G, 1)
+    packed = dsk.Packed.of(torch.from_numpy(p.starts).to(DEV), p.rows)
+    first = torch.from_numpy(p.starts[:-1]).long()
+    assert torch.equal(packed.attend(q, k, v)[first], want[first])
+    assert torch.equal(packed.attend(q, k, v, window=1), want)
+    packed.check()

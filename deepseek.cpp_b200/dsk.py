@@ -968,6 +968,11 @@ def _no_overlap(what, t):
             extent += step * (n - 1)
 
 
+def _rows_fit(rows):
+    if not 0 <= rows <= 1 << 20:                               # (ahead of memory for them, and of a structure that could not hold the number)
+        raise DskError(f"{rows} packed rows: at most 2^20 a call")
+
+
 def _status(torch, status, device, what):
     """Waits for the GPU, all of its streams, and raises if a call has noted something; the status is cleared."""
     torch.cuda.synchronize(device)
@@ -1115,6 +1120,7 @@ class Packed:
         import torch
         if starts.dim() != 1 or starts.shape[0] < 1:
             raise DskError(f"starts: int32 [batch + 1] is needed, got {tuple(starts.shape)}")
+        _rows_fit(rows)
         p = cls.__new__(cls)
         device = starts.get_device()
         if device < 0:
@@ -1173,7 +1179,7 @@ class Packed:
             raise DskError(f"results of {out.dtype} for queries of {q.dtype}")
         window, keep_first = max(-1, min(window, 0x7fffffff)), max(-1, min(keep_first, 0x7fffffff))   # (what an int has; negative ones are refused)
         _ck(_fast("dsk_packed_attn")(self._c, self._view("queries", q, heads, dim_k), self._view("keys", k, kv_heads, dim_k), self._view("values", v, kv_heads, dim_v),
-                                     self._view("output", out, heads, dim_v, True), heads, kv_heads, dim_k, dim_v, dim_k ** -0.5 if scale is None else scale, window, keep_first,
+                                     self._view("output", out, heads, dim_v, True), heads, kv_heads, dim_k, dim_v, max(dim_k, 1) ** -0.5 if scale is None else scale, window, keep_first,
                                      _stream_of(torch, self.device)))
         return out
 
@@ -1206,6 +1212,8 @@ class Blocks:
             _no_device(free)
         if free.dim() != 1 or free.dtype is not torch.int32 or free.shape[0] > n_blocks:
             raise DskError(f"free blocks: int32 [at most {n_blocks}] is needed, got {free.dtype} {tuple(free.shape)}")
+        if n_blocks >= 1 << 31:
+            raise DskError(f"{n_blocks} blocks: less than 2^31 tokens are supported")
         self.free = torch.zeros(n_blocks, dtype=torch.int32, device=free.device)
         self.free[:free.shape[0]] = free
         self._top = torch.tensor([free.shape[0], 0], dtype=torch.int32).to(free.device)
@@ -1220,8 +1228,7 @@ class Blocks:
         packed rows, with room for `rows` tokens of all sequences.  Sequences that no longer fit, and those behind them, get nothing."""
         batch, blocks = _table(self._torch, table, self.device).shape
         i32 = self._torch.int32
-        if rows < 0:
-            raise DskError(f"{rows} packed rows")
+        _rows_fit(rows)
         if out is None:
             out = Packed._room(self, batch, rows)
         elif out.batch != batch or out.rows != rows or out._all is None or out.block != self.block:

@@ -736,3 +736,15 @@ def test_a_row_that_sees_one_key_has_its_value(dtype, H, G, dk, dv, lens):
     assert torch.equal(packed.attend(q, k, v)[first], want[first])
     assert torch.equal(packed.attend(q, k, v, window=1), want)
     packed.check()
+
+
+def test_sizes_that_no_structure_holds_are_refused():
+    z, t = ints([0, 0]), torch.zeros(2, 4, dtype=torch.int32, device=DEV)
+    pool = dsk.Blocks(8, block=16, device=0)
+    none = torch.zeros(4, 2, 0, dtype=torch.bfloat16, device=DEV)
+    some = torch.zeros(4, 2, 16, dtype=torch.bfloat16, device=DEV)
+    for call, text in ((lambda: dsk.Packed.of(z, 1 << 40), "2\\^20"), (lambda: dsk.Packed.of(z, -1), "2\\^20"), (lambda: pool.extend(t, z, z, 1 << 31), "2\\^20"), (lambda: pool.extend(t, z, z, 1 << 60), "2\\^20"),
+                       (lambda: dsk.Blocks.of(z, (1 << 32) + 8), "2\\^31"), (lambda: dsk.Packed.of(z, 4).attend(none, none, some), "multiple of 16"), (lambda: dsk.Packed.of(z, 4).attend(some, some, none), "multiple of 16"),
+                       (lambda: dsk.Packed.of(z, 4).attend(some[:, :0], some, some), "multiple"), (lambda: dsk.Packed.of(z, 4).attend(some, some[:, :0], some[:, :0]), "multiple")):
+        with pytest.raises(dsk.DskError, match=text):
+            call()

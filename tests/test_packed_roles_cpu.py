@@ -347,3 +347,84 @@ def test_a_row_tile_by_itself_sees_something_of_every_tile():
         kept = min(first, low)
         some, upto = max(0, a + 1 - window) // T + kept - low if window else 0, (t1 - 1) // T + 1 + kept - low
         assert all(i < upto and (i < first or i >= some) for i in range(kept + -(-t1 // T) - low))
+
+
+def deal(rng, given, users, waits=True):
+    """The warp that deals out work, by itself: given are the CTAs whose work it gets, its own first and then one for each claim (True: there is a piece for it; False: none, so that it claims the
+    next one), users the roles that take items, of which the first asks for more.  Several claims may come ahead of the first item, and between two.  waits: for an answer, ahead of reading it.
+    Returns what each role took."""
+    claimed, want, ifull, iempty = Bar(1), Bar(1), [Bar(1) for _ in range(2)], [Bar(users) for _ in range(2)]
+    items, answer, flying, took = [None, None], [None], [], [[] for _ in range(users)]
+
+    def dealer():
+        at, asks, claims, got = 0, False, 0, 0
+        r = 0
+        while True:
+            while at is not None and (asks or not given[at]):
+                asks, got = False, got + 1
+                flying.append(got if got < len(given) else None)          # (the answer lands some time later; None: no CTA is left, and no other may be asked for)
+                if waits:
+                    yield claimed.wait(claims)
+                else:
+                    yield None
+                claims += 1
+                at = answer[0]
+                assert at == (got if got < len(given) else None)
+                yield None
+            yield iempty[r & 1].wait((r >> 1) ^ 1)
+            items[r & 1] = at
+            yield None
+            ifull[r & 1].arrive()
+            if at is None:
+                return
+            yield want.wait(r)
+            asks = True
+            r += 1
+
+    def user(x):
+        turn = 0
+        while True:
+            yield ifull[turn & 1].wait(turn >> 1)
+            n = items[turn & 1]
+            yield None
+            assert items[turn & 1] == n
+            iempty[turn & 1].arrive()
+            turn += 1
+            if n is None:
+                return
+            took[x].append(n)
+            if x == 0:
+                want.arrive()
+            yield None
+
+    roles = [dealer()] + [user(x) for x in range(users)]
+    speed = [rng.choice([1, 10, 0.05]) for _ in range(users + 2)]
+    at = [next(r, False) for r in roles]
+    while flying or any(a is not False for a in at):
+        able = [k for k, a in enumerate(at) if a is None or (a is not False and a())] + ([users + 1] if flying else [])
+        assert able, "nobody can go on"
+        k = rng.choices(able, [speed[j] for j in able])[0]
+        if k == users + 1:
+            answer[0] = flying.pop(0)
+            claimed.arrive()
+        else:
+            at[k] = next(roles[k], False)
+    return took
+
+
+def test_claims_of_ctas_without_a_piece():
+    rng = random.Random(7)
+    for _ in range(1500):
+        given = [rng.random() < rng.choice([0.2, 0.5, 1.0]) for _ in range(rng.randint(1, 12))]
+        took = deal(rng, given, rng.choice([1, 2, 11]))
+        assert all(x == [n for n, piece in enumerate(given) if piece] for x in took), (given, took)
+
+
+def test_the_wait_for_an_answer_is_needed():
+    rng, found = random.Random(8), 0
+    for _ in range(200):
+        try:
+            deal(rng, [True, False, True], 3, waits=False)
+        except AssertionError:
+            found += 1
+    assert found > 20

@@ -17,11 +17,11 @@
 // Short prompts: a piece of one tile runs through the code of every role once, and what does not fit the instruction cache is fetched each time (39 % of its lines, a softmax of one tile 4500 cycles
 // where it has 1350 by itself).  So the code that pieces run through is kept small: walks are worked out by the warp that deals, one form of each product, one place that counts levels, waits that
 // note in a register that they gave up (222 prompts of 60 tokens, 8 heads over 8: 43 us where it was 60; 64 prompts of 1 to 200: 26, was 31).
-// Bound: between tensor pipe and softmax.  Of 1470 cycles for 256 rows and 64 keys of 128 + 128 entries the tensor pipe has 1280 (products of 64 keys read their operands from shared memory in 48 cycles
-// for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 823 us
-// (1.34 PFLOP/s; a measured product of matrices 1.68), at 1.6 GHz under the power limit; back to back 940.  32 heads of 192 + 128, 8 prompts of up to 5001 tokens: 751 us (1.09); 256 + 256: 99 us
-// (0.80), 64 + 64, windowed: 151 us.  Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820),
-// maxima only where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0023 in bf16, the plain form's 0.0016).
+// Bound: between tensor pipe and softmax.  Of 1505 cycles for 256 rows and 64 keys of 128 + 128 entries the tensor pipe has 1280 (products of 64 keys read their operands from shared memory in 48 cycles
+// for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 957 us
+// one call behind another (1.15 PFLOP/s; a measured product of matrices 1.41 so), 828 us in a few of them (1.33, of 1.68), at 1.65 GHz: the power limit has both.  32 heads of 192 + 128, 8 prompts of up to
+// 5001 tokens: 872 and 752 us (0.94, 1.09), 2000 cycles; 256 + 256: 107 and 94 us (0.75, 0.85), 2155 cycles for 128 rows; 64 + 64, windowed: 141 and 151 us, 1835 cycles.  Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820),
+// maxima only where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0021 in bf16, the plain form's 0.0016).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -385,7 +385,7 @@ int dsk_kv8_attn_workspace(const dsk_kv8* cache, const dsk_kv8_rows* rows, int h
 int dsk_kv8_attn(const dsk_kv8* cache, const dsk_kv8_rows* rows, const dsk_view* q, const dsk_view* out, int heads, float scale, int window, int keep_first,
                  void* workspace, size_t workspace_bytes, void* stream);
 /* Packed rows: the rows of several sequences one behind the other, sequence b's from starts[b] on (starts[batch]: behind the last one; rows from there on belong to no one and are neither read nor
- * written).  At most 1024 sequences and 2^20 rows a call.  A starts that falls, or points outside the rows, is taken as the nearest one that does not.
+ * written).  At most 1024 sequences and 2^20 rows a call.  A start outside the rows is taken as the nearest inside, one that falls as the highest ahead of it.
  * Blocks of a cache that are free are a stack, free[0 .. n_free[0] - 1]; n_free[1] is a word of the kernels, 0 between calls.  A sequence of len tokens holds the first ceil(len / block) entries of its row
  * of the table.  Calls over the same blocks, or the same table, must not run at the same time. */
 enum { DSK_BLOCKS_SHORT = 8,  /* status: sequences got no places, for want of blocks or packed rows */
@@ -416,7 +416,7 @@ int dsk_kv8_append(const dsk_kv8* cache, const dsk_packed* rows, const dsk_view*
 /* Causal softmax attention of whole prompts, from their packed rows alone (no cache): token i of a sequence sees its tokens j <= i, with window > 0 those with i - j < window or j < keep_first.  Query
  * head h reads key head h / (heads / kv_heads).  q, k, v, out: F16 or BF16, all of one type (views: batch unused); q, k and v 16-byte aligned, their rows and heads a positive multiple of 8 entries apart;
  * dim_k and dim_v multiples of 16 up to 256; scale >= 0; out lies apart from the others.  Zeros for a query whose scores are all -inf; one that sees an infinite or NaN value has no finite result in that entry, others do not
- * notice.  Scores (scaled) beyond 2^127 are infinite; results below 2^-80 (BF16) lose accuracy. */
+ * notice.  Scores (scaled) beyond 2^127 are infinite; results below 2^-80 (BF16) lose accuracy.  Weights are rounded to the type of the operands for the product with the values, their sum is not. */
 int dsk_packed_attn(const dsk_packed* rows, const dsk_view* q, const dsk_view* k, const dsk_view* v, const dsk_view* out, int heads, int kv_heads, int dim_k, int dim_v, float scale, int window,
                     int keep_first, void* stream);
 /* Speculative sampling, beside dsk_sample: sequence b has count[b] drafted tokens x_i and the model's logits of count[b] + 1 rows.  p_i = softmax(logits_i / temperature); draft i is accepted

@@ -213,7 +213,7 @@ extern "C" int dsk_packed_attn(const dsk_packed* s, const dsk_view* q, const dsk
   std::memcpy(&P.f, &bits, 4);
   // Few pieces: both row tiles of a CTA have the same rows, each every second tile of its keys, so that the longest walk takes half the time and there are twice the pieces.  Where pieces of two row
   // tiles would not fill the GPU (one prompt of 8192 tokens, 4 heads over 1: 69 us for 115; 20 prompts of 60, 16 over 4: 11.2 for 10.4); beyond, keys and values are read twice as often (four
-  // prompts of 4096 tokens: 73 us for 65)
+  // prompts of 4096 tokens: 73 us for 65).  By rows alone, what a captured call has to spare among them: one prompt of 9600 tokens, 4 heads over 1, takes 147 us where 9472 take 84
   const bool joint = shape != 3 && s->rows / (2ll * P.tokens) * P.units <= multiprocessors(s->device);
   const int tokens = P.tokens * (shape == 3 || joint ? 1 : 2);
   const long long items = ((long long)s->rows / tokens + std::min(s->batch, s->rows)) * P.units;   // at most, whatever the lengths

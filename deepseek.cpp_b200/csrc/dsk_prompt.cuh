@@ -8,8 +8,8 @@
 // some row does not see whole.  A row tile has scores in two places, so that the products and the way there and back (1400 cycles a tile) come under the softmax of the tile ahead.
 // Weights: y = f s - m in one fused operation, f = scale log2(e); the reference m is a maximum, moved by a power of two, that may lag behind, so that the results in TMEM are scaled
 // again where a maximum has moved far (the thread that has the row does it).  A weight that is the row's largest when its reference is taken is that power of two, which its rounding leaves as it is: a row
-// that sees one key has its value, bit for bit (with references that are whole numbers it was off by half a step).  bf16 weights have fp32's range: references lead by 2^40, so that no sum of weights x values exceeds the
-// largest value; fp16 weights lie between 2^-24 and 2^14, references 2^7 below the maximum.  Sums are of the weights ahead of their rounding, which is off by half a step of the type at most.
+// that sees one key has its value, bit for bit (with references that are whole numbers it was off by half a step).  bf16 weights have fp32's range: references lead by 2^40, so that no sum of weights x values
+// exceeds the largest value; fp16 weights lie between 2^-24 and 2^14, references 2^7 below the maximum.  Sums are of the weights ahead of their rounding, which is off by half a step of the type at most.
 // Infinities and NaN among values that a row does not see must not reach it as 0 x inf: in tiles that some row does not see whole they go to the products as zeros, and rows that do see
 // one get it back at the end.
 // Few rows: both row tiles of a CTA have the same rows, each every second tile of their keys (joint; the second one's results are added in the reference of both, from its half of TMEM, at the end).
@@ -20,8 +20,8 @@
 // Bound: between tensor pipe and softmax.  Of 1505 cycles for 256 rows and 64 keys of 128 + 128 entries the tensor pipe has 1280 (products of 64 keys read their operands from shared memory in 48 cycles
 // for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 957 us
 // one call behind another (1.15 PFLOP/s; a measured product of matrices 1.41 so), 828 us in a few of them (1.33, of 1.68), at 1.65 GHz: the power limit has both.  32 heads of 192 + 128, 8 prompts of up to
-// 5001 tokens: 872 and 752 us (0.94, 1.09), 2000 cycles; 256 + 256: 107 and 94 us (0.75, 0.85), 2155 cycles for 128 rows; 64 + 64, windowed: 141 and 151 us, 1835 cycles.  Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820),
-// maxima only where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0021 in bf16, the plain form's 0.0016).
+// 5001 tokens: 872 and 752 us (0.94, 1.09), 2000 cycles; 256 + 256: 107 and 94 us (0.75, 0.85), 2155 cycles for 128 rows; 64 + 64, windowed: 141 and 151 us, 1835 cycles.
+// Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820), maxima only where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0021 in bf16, the plain form's 0.0016).
 #pragma once
 
 #include <cuda_bf16.h>

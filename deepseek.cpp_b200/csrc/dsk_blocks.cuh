@@ -179,7 +179,9 @@ __global__ void __launch_bounds__(kThreads) extend(const Extend A) {
 }
 
 // One CTA.  A thread has one sequence's count of entries, a warp walks a sequence's entries: numbers that are no blocks do not go back, so they are counted first.
-__global__ void __launch_bounds__(kCutThreads) cut(const Cut A) {
+// MANY: the table has 2^31 entries or more, and if they repeat as many may come back: two sums, of 16 and 11 bits of each count (4.1 us for a call that has nothing to do, 3.1 with one sum).  What comes back
+// beyond the stack's end, which has at most 2^27 places, goes nowhere: a sum beyond is taken as one more than those.
+template <bool MANY> __global__ void __launch_bounds__(kCutThreads) cut(const Cut A) {
   constexpr int WARPS = kCutThreads / 32;
   __shared__ int low[kMaxBatch], high[kMaxBatch], good[kMaxBatch], of_warp[3][WARPS], height;
   const int shift = A.P.shift, block = 1 << shift, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = threadIdx.x;
@@ -200,13 +202,11 @@ __global__ void __launch_bounds__(kCutThreads) cut(const Cut A) {
     if (lane == 0) good[s] = n;
   }
   __syncthreads();
-  // Sums over the sequences behind a thread's own: the last one's blocks go first.  Entries that repeat may make them up to 2^36, which two sums of 16 and 11 bits of each count hold; what comes back beyond
-  // the stack's end goes nowhere, so that a sum that is larger may be taken as that many
-  const int from = A.batch - 1 - b, count = b < A.batch ? good[from] : 0;
-  int sum[3] = {count & 0xffff, count >> 16, 0}, all[3];
+  const int from = A.batch - 1 - b, count = b < A.batch ? good[from] : 0;   // sums over the sequences behind a thread's own: the last one's blocks go first
+  int sum[3] = {MANY ? count & 0xffff : count, MANY ? count >> 16 : 0, 0}, all[3];
   const bool lost = b < A.batch && count < high[from] - low[from];
   sums_ahead<WARPS>(sum, all, of_warp);
-  auto whole = [&](const int (&x)[3]) { return (int)min((long long)x[1] * 65536 + x[0], (long long)A.P.n_blocks + 1); };
+  auto whole = [&](const int (&x)[3]) { return min(MANY ? (min(x[1], 1 << 12) << 16) + x[0] : x[0], A.P.n_blocks + 1); };
   if (b < A.batch) good[from] = whole(sum);
   if (lost) note(A.P, ST_PAGE);
   const int have = height, back = whole(all);

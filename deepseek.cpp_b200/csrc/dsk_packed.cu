@@ -70,7 +70,9 @@ extern "C" int dsk_blocks_cut(const dsk_blocks* p, int32_t* table, int64_t table
   if (const int code = check_device(p->device)) return code;
   OnDevice on(p->device);
   CK(on.error);
-  blocks::cut<<<1, blocks::kCutThreads, 0, static_cast<cudaStream_t>(stream)>>>(blocks::Cut{pool_of(p), table, table_pitch, lens, keep, table_blocks, batch});
+  const blocks::Cut A{pool_of(p), table, table_pitch, lens, keep, table_blocks, batch};
+  if ((long long)batch * table_blocks > INT32_MAX) blocks::cut<true><<<1, blocks::kCutThreads, 0, static_cast<cudaStream_t>(stream)>>>(A);
+  else blocks::cut<false><<<1, blocks::kCutThreads, 0, static_cast<cudaStream_t>(stream)>>>(A);
   CK(cudaGetLastError());
   return 0;
 }

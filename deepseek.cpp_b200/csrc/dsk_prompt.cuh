@@ -21,7 +21,8 @@
 // for 32 of work; tiles of 128 keys, whose products are whole, leave one place for scores: 1860 for as many keys), the exponentials' pipe 1024.  16384 tokens of 16 heads over 4, 128 + 128: 957 us
 // one call behind another (1.15 PFLOP/s; a measured product of matrices 1.41 so), 828 us in a few of them (1.33, of 1.68), at 1.65 GHz: the power limit has both.  32 heads of 192 + 128, 8 prompts of up to
 // 5001 tokens: 872 and 752 us (0.94, 1.09), 2000 cycles; 256 + 256: 107 and 94 us (0.75, 0.85), 2155 cycles for 128 rows; 64 + 64, windowed: 141 and 151 us, 1835 cycles.
-// Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820), maxima only where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0021 in bf16, the plain form's 0.0016).
+// Taken back: four softmax warps more that share the columns of a row (1300 us where it was 1080), shares of the exponentials as polynomials (850 to 870 where it was 820), maxima only
+// where the sum of a tile's weights asks for them (910), sums of rounded weights (937; the error against 64 bits is 0.0021 in bf16, the plain form's 0.0016).
 #pragma once
 
 #include <cuda_bf16.h>
